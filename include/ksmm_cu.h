@@ -364,6 +364,67 @@ KSMM_API int ksmm_cu_chain_forward_static(const void* input, const void* const* 
                                           int bs_last, void* stream);
 
 /*
+ * The passage from one block of a network to the next, in one pass:
+ *
+ *   p = post(y) * post_weight + post_bias                    (post_norm; p = y without one)
+ *   z = alpha * x + gate * p                                 (z = x without y)
+ *   h = (pre(z) * weight + bias) * (1 + scale) + shift       (norm; no h without one)
+ *
+ * over the `channels` of each of `rows` tokens; (rows, channels) batch-first, (channels, rows) batch-last,
+ * contiguous.  Statistics, sums and the z that h is made from are fp32.  weight, bias, post_weight and
+ * post_bias hold `channels` elements of param_dtype (dtype or fp32) or are NULL (1, 0).  scale, shift and gate
+ * hold one row of `channels` elements (stride 0) or one per sample, `stride` elements apart; sample s is the
+ * rows / samples tokens from s * rows / samples on.  NULL: 0, 0, 1.
+ *
+ * ksmm_cu_norm_forward reads x, y and the parameters; writes z (with y), h (with a norm) and, where stats is
+ * not NULL, 4 floats per token for the backward pass.  The reference composes these steps from separate
+ * PyTorch calls (src/ksmm_py/model/vit.py:416-431, 770-800).
+ * ksmm_cu_norm_backward reads grad_z and / or grad_h, the forward's x or z, y and stats, and the
+ * parameters; writes those of grad_* that are not NULL: grad_x and grad_y laid out as x and y, the others
+ * contiguous rows of param_dtype (grad_scale, grad_shift, grad_gate: `samples` rows where their stride is not 0).
+ * Its sums over tokens have a fixed order.  Up to 16384 channels; outputs overlap no input.
+ */
+typedef enum { KSMM_NORM_NONE = 0, KSMM_NORM_LAYER = 1, KSMM_NORM_RMS = 2 } ksmm_norm_t;
+
+typedef struct {
+  const void* x;
+  const void* y;
+  void* z;
+  void* h;
+  float* stats;
+  const void* weight;
+  const void* bias;
+  const void* post_weight;
+  const void* post_bias;
+  const void* scale;
+  const void* shift;
+  const void* gate;
+  int64_t scale_stride, shift_stride, gate_stride;
+  int64_t rows, samples;
+  int32_t channels;
+  int32_t norm, post_norm; /* ksmm_norm_t */
+  int32_t bs_last;
+  int32_t dtype, param_dtype;
+  float alpha, eps;
+  /* backward only */
+  const void* grad_z;
+  const void* grad_h;
+  void* grad_x;
+  void* grad_y;
+  void* grad_weight;
+  void* grad_bias;
+  void* grad_post_weight;
+  void* grad_post_bias;
+  void* grad_scale;
+  void* grad_shift;
+  void* grad_gate;
+} ksmm_norm_desc_t;
+
+KSMM_API int ksmm_cu_norm_forward(const ksmm_norm_desc_t* desc, void* stream);
+KSMM_API size_t ksmm_cu_norm_backward_workspace_bytes(const ksmm_norm_desc_t* desc);
+KSMM_API int ksmm_cu_norm_backward(const ksmm_norm_desc_t* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Host-memory variant of ksmm_cu_chain_forward: input, values and output are
  * HOST buffers; the call stages them through device memory that the library
  * owns (grown on demand, reused across calls), runs the chain and returns

@@ -24,6 +24,8 @@ KSMM_ERR_NO_DEVICE = 6
 KSMM_F32, KSMM_F16, KSMM_BF16, KSMM_F8E4M3 = 0, 1, 2, 3
 KSMM_ALGO_AUTO, KSMM_ALGO_SIMT, KSMM_ALGO_TC, KSMM_ALGO_CONVERT = 0, 1, 2, 3
 KSMM_ACT_NONE, KSMM_ACT_GELU, KSMM_ACT_RELU = 0, 1, 2
+KSMM_NORM_NONE, KSMM_NORM_LAYER, KSMM_NORM_RMS = 0, 1, 2
+NORMS = {None: KSMM_NORM_NONE, "layer": KSMM_NORM_LAYER, "rms": KSMM_NORM_RMS}
 ACTIVATIONS = {None: KSMM_ACT_NONE, "none": KSMM_ACT_NONE, "gelu": KSMM_ACT_GELU, "relu": KSMM_ACT_RELU}
 STATIC_SCRATCH_BYTES = 40 * 1024 * 1024  # KSMM_CU_STATIC_SCRATCH_BYTES
 
@@ -43,6 +45,7 @@ EXPORTS = (
     "ksmm_cu_backward_weights_workspace_bytes", "ksmm_cu_backward_weights",
     "ksmm_cu_chain_train_bytes", "ksmm_cu_chain_train_forward", "ksmm_cu_chain_backward",
     "ksmm_cu_chain_fp8_workspace_bytes", "ksmm_cu_chain_forward_fp8",
+    "ksmm_cu_norm_forward", "ksmm_cu_norm_backward_workspace_bytes", "ksmm_cu_norm_backward",
 )
 
 
@@ -86,6 +89,19 @@ class ChainDesc(ctypes.Structure):
         ("patterns", ctypes.POINTER(ctypes.c_int32)), ("dtype", ctypes.c_int32), ("bs_last", ctypes.c_int32),
         ("out_layout", ctypes.c_int32), ("activation", ctypes.c_int32),
     ]
+
+
+class NormDesc(ctypes.Structure):
+    """Mirror of ksmm_norm_desc_t."""
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("x", "y", "z", "h", "stats", "weight", "bias", "post_weight", "post_bias", "scale",
+                                        "shift", "gate")]
+        + [(n, ctypes.c_int64) for n in ("scale_stride", "shift_stride", "gate_stride", "rows", "samples")]
+        + [(n, ctypes.c_int32) for n in ("channels", "norm", "post_norm", "bs_last", "dtype", "param_dtype")]
+        + [("alpha", ctypes.c_float), ("eps", ctypes.c_float)]
+        + [(n, ctypes.c_void_p) for n in ("grad_z", "grad_h", "grad_x", "grad_y", "grad_weight", "grad_bias",
+                                          "grad_post_weight", "grad_post_bias", "grad_scale", "grad_shift", "grad_gate")]
+    )
 
 
 class KsmmError(RuntimeError):
@@ -168,6 +184,12 @@ def load():
     lib.ksmm_cu_chain_forward_fp8.restype = i32
     lib.ksmm_cu_chain_forward_fp8.argtypes = [vp, i32, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_float), vp, vp, vp,
                                               ctypes.c_size_t, i64, i32, ctypes.POINTER(ctypes.c_int32), i32, vp]
+    lib.ksmm_cu_norm_forward.restype = i32
+    lib.ksmm_cu_norm_forward.argtypes = [ctypes.POINTER(NormDesc), vp]
+    lib.ksmm_cu_norm_backward_workspace_bytes.restype = ctypes.c_size_t
+    lib.ksmm_cu_norm_backward_workspace_bytes.argtypes = [ctypes.POINTER(NormDesc)]
+    lib.ksmm_cu_norm_backward.restype = i32
+    lib.ksmm_cu_norm_backward.argtypes = [ctypes.POINTER(NormDesc), vp, ctypes.c_size_t, vp]
     lib.ksmm_cu_host_wait.restype = i32
     lib.ksmm_cu_host_wait.argtypes = [ctypes.c_uint64]
     lib.ksmm_cu_num_configs.restype = i32
