@@ -76,7 +76,9 @@ typedef enum {
 typedef enum {
   KSMM_ACT_NONE = 0,
   KSMM_ACT_GELU = 1,   /* 0.5 x (1 + erf(x / sqrt 2)), torch.nn.functional.gelu's default */
-  KSMM_ACT_RELU = 2
+  KSMM_ACT_RELU = 2,
+  KSMM_ACT_SILU = 3,   /* x / (1 + exp(-x)); this and the next one: gated calls only */
+  KSMM_ACT_SIGMOID = 4
 } ksmm_activation_t;
 
 typedef struct {
@@ -364,6 +366,48 @@ KSMM_API int ksmm_cu_chain_forward_static(const void* input, const void* const* 
                                           int bs_last, void* stream);
 
 /*
+ * A gated layer: two chains of the same patterns on one input, h = act(gate(x)) * up(x), the first half of a
+ * gated feed-forward block.  values[f] holds the gate's kernel-format factor f and the up projection's after
+ * it, (2*a*d*c, b); bias, if not NULL, 2 * out elements in the same order.  The chains' factors run in pairs, and
+ * where the last factor's kernel can (16-bit types on the tensor cores) it forms the product in its epilogue, so
+ * that neither half is written.  out_layout: 0 the input's layout, 1 batch-first, 2 batch-last.  activation: any
+ * ksmm_activation_t; it applies to the gate.
+ *
+ * saved == NULL: inference; `workspace` holds ksmm_cu_gated_workspace_bytes().
+ * saved != NULL: the forward pass of a training step, which keeps in `saved` what ksmm_cu_gated_backward
+ * reads, both halves before the product among it, and its layouts in `layouts` (nfactors values).
+ * ksmm_cu_gated_train_bytes gives the sizes of saved, of the forward's and of the backward's workspace.
+ * Workspaces and saved are aligned to 256 bytes, input, output and gradients of the backward to 16.  Up to 16
+ * factors, fp32, fp16 and bf16.  The reference has no gated layer; it replaces the calls that one would
+ * build it from (KSLinear.forward twice, interface.py:439-467, and two element-wise kernels).
+ */
+typedef struct {
+  const void* input;
+  const void* const* values;
+  void* output;
+  const void* bias;
+  void* workspace;
+  size_t workspace_bytes;
+  void* saved;
+  size_t saved_bytes;
+  int32_t* layouts;
+  int64_t batch;
+  int32_t nfactors;
+  const int32_t* patterns;
+  int32_t dtype, bs_last, out_layout, activation;
+} ksmm_gated_desc_t;
+
+KSMM_API size_t ksmm_cu_gated_workspace_bytes(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last,
+                                              int out_bs_last);
+KSMM_API int ksmm_cu_gated_train_bytes(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last,
+                                       int out_bs_last, size_t* saved_bytes, size_t* forward_bytes, size_t* backward_bytes);
+KSMM_API int ksmm_cu_gated_forward(const ksmm_gated_desc_t* desc, void* stream);
+/* desc: as the forward pass had it (output and bias are not read); workspace: the backward's.  grad_input,
+ * grad_values[f] and grad_bias are laid out as input, values[f] and bias; NULL where not wanted. */
+KSMM_API int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* grad_output, void* grad_input,
+                                    void* const* grad_values, void* grad_bias, void* stream);
+
+/*
  * The passage from one block of a network to the next, in one pass:
  *
  *   p = post(y) * post_weight + post_bias                    (post_norm; p = y without one)
@@ -382,7 +426,7 @@ KSMM_API int ksmm_cu_chain_forward_static(const void* input, const void* const* 
  * ksmm_cu_norm_backward reads grad_z and / or grad_h, the forward's x or z, y and stats, and the
  * parameters; writes those of grad_* that are not NULL: grad_x and grad_y laid out as x and y, the others
  * contiguous rows of param_dtype (grad_scale, grad_shift, grad_gate: `samples` rows where their stride is not 0).
- * Its sums over tokens have a fixed order.  Up to 16384 channels; outputs overlap no input.
+ * Its sums over tokens have a fixed order.  Up to 8192 channels; outputs overlap no input.
  */
 typedef enum { KSMM_NORM_NONE = 0, KSMM_NORM_LAYER = 1, KSMM_NORM_RMS = 2 } ksmm_norm_t;
 

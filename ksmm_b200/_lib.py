@@ -26,6 +26,8 @@ KSMM_ALGO_AUTO, KSMM_ALGO_SIMT, KSMM_ALGO_TC, KSMM_ALGO_CONVERT = 0, 1, 2, 3
 KSMM_ACT_NONE, KSMM_ACT_GELU, KSMM_ACT_RELU = 0, 1, 2
 KSMM_NORM_NONE, KSMM_NORM_LAYER, KSMM_NORM_RMS = 0, 1, 2
 NORMS = {None: KSMM_NORM_NONE, "layer": KSMM_NORM_LAYER, "rms": KSMM_NORM_RMS}
+KSMM_ACT_SILU, KSMM_ACT_SIGMOID = 3, 4  # gated layers only
+GATES = {None: KSMM_ACT_NONE, "gelu": KSMM_ACT_GELU, "relu": KSMM_ACT_RELU, "silu": KSMM_ACT_SILU, "sigmoid": KSMM_ACT_SIGMOID}
 ACTIVATIONS = {None: KSMM_ACT_NONE, "none": KSMM_ACT_NONE, "gelu": KSMM_ACT_GELU, "relu": KSMM_ACT_RELU}
 STATIC_SCRATCH_BYTES = 40 * 1024 * 1024  # KSMM_CU_STATIC_SCRATCH_BYTES
 
@@ -45,6 +47,7 @@ EXPORTS = (
     "ksmm_cu_backward_weights_workspace_bytes", "ksmm_cu_backward_weights",
     "ksmm_cu_chain_train_bytes", "ksmm_cu_chain_train_forward", "ksmm_cu_chain_backward",
     "ksmm_cu_chain_fp8_workspace_bytes", "ksmm_cu_chain_forward_fp8",
+    "ksmm_cu_gated_workspace_bytes", "ksmm_cu_gated_train_bytes", "ksmm_cu_gated_forward", "ksmm_cu_gated_backward",
     "ksmm_cu_norm_forward", "ksmm_cu_norm_backward_workspace_bytes", "ksmm_cu_norm_backward",
 )
 
@@ -60,7 +63,7 @@ def _load_native():
         from . import ksmm_torch_ext
     except ImportError:
         return None
-    return ksmm_torch_ext if hasattr(ksmm_torch_ext, "layer_train") else None
+    return ksmm_torch_ext if hasattr(ksmm_torch_ext, "gated_train") else None
 
 
 native = _load_native()
@@ -88,6 +91,17 @@ class ChainDesc(ctypes.Structure):
         ("workspace_bytes", ctypes.c_size_t), ("batch", ctypes.c_int64), ("nfactors", ctypes.c_int32),
         ("patterns", ctypes.POINTER(ctypes.c_int32)), ("dtype", ctypes.c_int32), ("bs_last", ctypes.c_int32),
         ("out_layout", ctypes.c_int32), ("activation", ctypes.c_int32),
+    ]
+
+
+class GatedDesc(ctypes.Structure):
+    """Mirror of ksmm_gated_desc_t."""
+    _fields_ = [
+        ("input", ctypes.c_void_p), ("values", ctypes.POINTER(ctypes.c_void_p)), ("output", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("saved", ctypes.c_void_p), ("saved_bytes", ctypes.c_size_t), ("layouts", ctypes.POINTER(ctypes.c_int32)),
+        ("batch", ctypes.c_int64), ("nfactors", ctypes.c_int32), ("patterns", ctypes.POINTER(ctypes.c_int32)),
+        ("dtype", ctypes.c_int32), ("bs_last", ctypes.c_int32), ("out_layout", ctypes.c_int32), ("activation", ctypes.c_int32),
     ]
 
 
@@ -184,6 +198,14 @@ def load():
     lib.ksmm_cu_chain_forward_fp8.restype = i32
     lib.ksmm_cu_chain_forward_fp8.argtypes = [vp, i32, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_float), vp, vp, vp,
                                               ctypes.c_size_t, i64, i32, ctypes.POINTER(ctypes.c_int32), i32, vp]
+    lib.ksmm_cu_gated_workspace_bytes.restype = ctypes.c_size_t
+    lib.ksmm_cu_gated_workspace_bytes.argtypes = [i32, pi32, i64, i32, i32, i32]
+    lib.ksmm_cu_gated_train_bytes.restype = i32
+    lib.ksmm_cu_gated_train_bytes.argtypes = [i32, pi32, i64, i32, i32, i32, psz, psz, psz]
+    lib.ksmm_cu_gated_forward.restype = i32
+    lib.ksmm_cu_gated_forward.argtypes = [ctypes.POINTER(GatedDesc), vp]
+    lib.ksmm_cu_gated_backward.restype = i32
+    lib.ksmm_cu_gated_backward.argtypes = [ctypes.POINTER(GatedDesc), vp, vp, pvp, vp, vp]
     lib.ksmm_cu_norm_forward.restype = i32
     lib.ksmm_cu_norm_forward.argtypes = [ctypes.POINTER(NormDesc), vp]
     lib.ksmm_cu_norm_backward_workspace_bytes.restype = ctypes.c_size_t

@@ -1,0 +1,111 @@
+// The product of a gated layer, h = act(g) * u, and its backward, dg = dh u act'(g) and du = dh act(g), as passes
+// over whole tensors: for types and shapes whose last factor does not form the product in its epilogue, and
+// for every backward pass.  Memory is what bounds them: three tensors move forward, five backward.
+#include <algorithm>
+
+#include "gated.cuh"
+#include "gated.h"
+
+namespace ksmm {
+namespace {
+
+template <typename T, int V>
+__device__ __forceinline__ void get(const T* p, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = ElemTraits<T>::to_float(*p);
+  } else {
+    __align__(16) T t[V];
+    *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = ElemTraits<T>::to_float(t[e]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void put(T* p, const float (&f)[V]) {
+  __align__(16) T t[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) t[e] = ElemTraits<T>::from_float(f[e]);
+  if constexpr (V == 1) *p = t[0];
+  else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+}
+
+// `pieces` pieces of V elements per line; `half`: elements between g and u, `out_half`: between dg and du
+template <typename T, int V, bool BACKWARD>
+__global__ void __launch_bounds__(256)
+    gate_kernel(const T* __restrict__ gu, int64_t ld, const T* __restrict__ dh, int64_t h_ld, T* __restrict__ out,
+                int64_t half, int64_t out_half, int64_t lines, uint32_t pieces, int act) {
+  const int64_t total = lines * pieces;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < total; t += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t line = total <= 0xffffffffLL ? static_cast<uint32_t>(t) / pieces : t / pieces;
+    const int64_t x = (t - line * pieces) * V;
+    const T* at = gu + line * ld + x;
+    float g[V], u[V];
+    get<T, V>(at, g);
+    get<T, V>(at + half, u);
+    if constexpr (BACKWARD) {
+      float d[V], a[V], b[V];
+      get<T, V>(dh + line * h_ld + x, d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float value, slope;
+        gate_slope<sizeof(T) == 2>(g[e], act, value, slope);
+        a[e] = d[e] * u[e] * slope;
+        b[e] = d[e] * value;
+      }
+      put<T, V>(out + line * ld + x, a);
+      put<T, V>(out + out_half + line * ld + x, b);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = gate_value<sizeof(T) == 2>(g[e], act) * u[e];
+      put<T, V>(out + line * h_ld + x, g);
+    }
+  }
+}
+
+template <typename T, bool BACKWARD>
+int gate_typed(const void* gu, int64_t ld, const void* dh, int64_t h_ld, void* out, int64_t out_half, int64_t lines, int64_t len,
+               int act, cudaStream_t stream) {
+  if (lines <= 0 || len <= 0) return KSMM_OK;
+  constexpr int V = 16 / sizeof(T);
+  const int64_t half = lines * ld;
+  const void* narrow = BACKWARD ? dh : out;
+  const bool aligned = reinterpret_cast<uintptr_t>(gu) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(narrow) % 16 == 0 && half % V == 0 && out_half % V == 0;
+  if (ld == len && h_ld == len) {  // lines that follow one another are one line
+    len *= lines;
+    ld = h_ld = len;
+    lines = 1;
+  }
+  const bool vec = aligned && len % V == 0 && (lines == 1 || (ld % V == 0 && h_ld % V == 0));
+  const int64_t pieces = vec ? len / V : len;
+  if (pieces > 0xffffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "gated layer: too many elements");
+  const int64_t blocks = std::min<int64_t>((lines * pieces + 255) / 256, 148 * 64);
+  auto go = [&](auto kern) {
+    kern<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(gu), ld, static_cast<const T*>(dh), h_ld,
+                                                             static_cast<T*>(out), half, out_half, lines, static_cast<uint32_t>(pieces), act);
+  };
+  if (vec) go(gate_kernel<T, V, BACKWARD>);
+  else go(gate_kernel<T, 1, BACKWARD>);
+  count_launch();
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "gate kernel launch failed: %s", cudaGetErrorString(err));
+  return KSMM_OK;
+}
+
+}  // namespace
+
+int launch_gate(const void* gu, int64_t ld, void* h, int64_t h_ld, int64_t lines, int64_t len, int dtype, int act,
+                cudaStream_t stream) {
+  if (dtype == KSMM_F32) return gate_typed<float, false>(gu, ld, nullptr, h_ld, h, 0, lines, len, act, stream);
+  if (dtype == KSMM_F16) return gate_typed<__half, false>(gu, ld, nullptr, h_ld, h, 0, lines, len, act, stream);
+  return gate_typed<__nv_bfloat16, false>(gu, ld, nullptr, h_ld, h, 0, lines, len, act, stream);
+}
+
+int launch_gate_backward(const void* gu, int64_t ld, const void* dh, int64_t dh_ld, void* out, int64_t out_half, int64_t lines,
+                         int64_t len, int dtype, int act, cudaStream_t stream) {
+  if (dtype == KSMM_F32) return gate_typed<float, true>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, stream);
+  if (dtype == KSMM_F16) return gate_typed<__half, true>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, stream);
+  return gate_typed<__nv_bfloat16, true>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, stream);
+}
+
+}  // namespace ksmm

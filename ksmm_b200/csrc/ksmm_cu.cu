@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "backward.h"
+#include "gated.h"
 #include "common.cuh"
 #include "tc_host.h"
 #include "tc_kernel.h"
@@ -1428,10 +1429,11 @@ static double wgrad_copy_cost(const int32_t* q, int64_t batch, int dtype, int la
   return 1.5 * dtype_size(dtype) * q[0] * q[1] * q[3] * static_cast<double>(batch);
 }
 
-static void plan_backward(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last, bool need_input,
-                          bool allow_switch, BackwardPlan* plan) {
+// (`grad_last`: layout of the output's gradient; without switches it is the input's)
+static void plan_backward(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last, int grad_last,
+                          bool need_input, bool allow_switch, BackwardPlan* plan) {
   for (int f = 0; f < nfactors; ++f) plan->in_last[f] = plan->out_last[f] = bs_last;
-  plan->pre = false;
+  plan->pre = grad_last != bs_last;
   if (!allow_switch) return;
   const int32_t* pl = patterns + 4 * (nfactors - 1);
   const double kTranspose = 0.75 * 2.0, es = dtype_size(dtype);
@@ -1440,12 +1442,12 @@ static void plan_backward(int nfactors, const int32_t* patterns, int64_t batch, 
   double best = -1.0;
   for (int pre = 0; pre < 2; ++pre) {
     for (unsigned mask = 0; mask < (1u << nfactors); ++mask) {
-      int state = pre ? !bs_last : bs_last;
+      int state = pre ? !grad_last : grad_last;
       double cost = pre ? kTranspose * out_bytes : 0.0;
       bool ok = true;
       for (int f = nfactors - 1; f >= 0 && ok; --f) {
         const int32_t* q = patterns + 4 * f;
-        cost += wgrad_copy_cost(q, batch, dtype, state || (f == nfactors - 1 && (pre || bs_last)));
+        cost += wgrad_copy_cost(q, batch, dtype, state || (f == nfactors - 1 && (pre || grad_last)));
         const int o = (mask >> f) & 1;
         if (f == 0 && !need_input) {
           if (o != state) ok = false;  // nothing is multiplied
@@ -1462,7 +1464,7 @@ static void plan_backward(int nfactors, const int32_t* patterns, int64_t batch, 
       if (best < 0 || cost < best * 0.999) {
         best = cost;
         plan->pre = pre != 0;
-        int s2 = pre ? !bs_last : bs_last;
+        int s2 = pre ? !grad_last : grad_last;
         for (int f = nfactors - 1; f >= 0; --f) {
           plan->in_last[f] = s2;
           plan->out_last[f] = s2 = (mask >> f) & 1;
@@ -1475,21 +1477,25 @@ static void plan_backward(int nfactors, const int32_t* patterns, int64_t batch, 
 // Plans (run == false: the workspace's bytes through *need) or runs the backward of a chain.  The plan knows
 // neither the alignment of grad_input nor what is tuned by the time of the run, so the run takes no more
 // than `ws_bytes`: a factor whose scratch is not there runs on the register-staged kernel, which needs none.
-static int chain_backward_walk(bool run, const void* input, const void* const* values, const void* saved,
+// `grad_last`, `grad_ld`: layout of grad_output and, batch-last, its row stride; `add`: laid out as grad_input,
+// added to it.
+// `inters[f]`: the kept output of factor f.
+static int chain_backward_walk(bool run, const void* input, const void* const* values, const void* const* inters,
                                const int32_t* layouts, const void* grad_output, void* grad_input,
                                void* const* grad_values, void* grad_bias, char* ws, size_t ws_bytes, int64_t batch,
                                int nfactors, const int32_t* patterns, int dtype, int bs_last, bool need_input,
-                               bool allow_switch, bool one_layout, cudaStream_t stream, size_t* need) {
+                               bool allow_switch, bool one_layout, cudaStream_t stream, size_t* need, int grad_last,
+                               int64_t grad_ld, const void* add = nullptr) {
   const int es = dtype_size(dtype);
   const int64_t ld = one_layout ? batch : padded_ld(batch, es);
   BackwardPlan plan;
-  plan_backward(nfactors, patterns, batch, dtype, bs_last, need_input, allow_switch && !one_layout, &plan);
+  plan_backward(nfactors, patterns, batch, dtype, bs_last, grad_last, need_input, allow_switch && !one_layout, &plan);
   const int32_t* pl = patterns + 4 * (nfactors - 1);
   const int64_t n_out = static_cast<int64_t>(pl[0]) * pl[1] * pl[3];
   const int64_t n_in = static_cast<int64_t>(patterns[0]) * patterns[2] * patterns[3];
   const size_t one = train_buffer_bytes(nfactors, patterns, batch, dtype);
   // a second version of the output's gradient: the other layout, or padded rows
-  const bool pad_copy = !plan.pre && bs_last && ld != batch;
+  const bool pad_copy = !plan.pre && grad_last && ld != grad_ld;
   const size_t second_bytes = plan.pre || pad_copy ? align_up(static_cast<size_t>(n_out) * ld * es, 256) : 0;
   const bool post = need_input && plan.out_last[0] != bs_last;
   const size_t post_bytes = post ? align_up(static_cast<size_t>(n_in) * ld * es, 256) : 0;
@@ -1503,18 +1509,18 @@ static int chain_backward_walk(bool run, const void* input, const void* const* v
   size_t tail_bytes = 0;
 
   // versions of the output's gradient
-  WgradOperand dy{run ? grad_output : dummy, bs_last, batch}, dy2 = dy;
-  if (plan.pre) dy2 = WgradOperand{second, !bs_last, !bs_last ? ld : 0};
+  WgradOperand dy{run ? grad_output : dummy, grad_last, grad_last ? grad_ld : batch}, dy2 = dy;
+  if (plan.pre) dy2 = WgradOperand{second, !grad_last, !grad_last ? ld : 0};
   if (pad_copy) dy2 = WgradOperand{second, 1, ld};
   int st = KSMM_OK;
   // the transpose of a batch-first gradient sums its columns on the way (12 us for 12544 x 3072 fp16 as a
   // pass of its own)
-  const bool sum_on_way = plan.pre && !bs_last && (grad_bias || !run);
+  const bool sum_on_way = plan.pre && !grad_last && (grad_bias || !run);
   if (run && plan.pre)
-    st = bs_last ? launch_transpose(grad_output, second, n_out, batch, es, stream)
-                 : launch_transpose(grad_output, second, batch, n_out, es, stream, ld, 0,
-                                    sum_on_way ? reinterpret_cast<float*>(tail) : nullptr, dtype);
-  if (run && pad_copy) st = launch_copy_rows(grad_output, batch, second, ld, n_out, batch, es, stream);
+    st = grad_last ? launch_transpose(grad_output, second, n_out, batch, es, stream, 0, grad_ld)
+                   : launch_transpose(grad_output, second, batch, n_out, es, stream, ld, 0,
+                                      sum_on_way ? reinterpret_cast<float*>(tail) : nullptr, dtype);
+  if (run && pad_copy) st = launch_copy_rows(grad_output, grad_ld, second, ld, n_out, batch, es, stream);
   if (st != KSMM_OK) return st;
   if (sum_on_way) {
     const int slices = transpose_row_tiles(batch, es);
@@ -1534,7 +1540,7 @@ static int chain_backward_walk(bool run, const void* input, const void* const* v
       Problem p = backward_problem(nullptr, nullptr, run ? grad_values[f] : dummy, batch, q[0], q[1], q[2], q[3], dtype, bs_last);
       WgradOperand x{run ? input : dummy, bs_last, batch};
       if (f > 0) {
-        x.ptr = run ? static_cast<const char*>(saved) + static_cast<size_t>(f - 1) * one : dummy;
+        x.ptr = run ? inters[f - 1] : dummy;
         x.last = layouts[f - 1] == 1;
         x.ld = x.last ? ld : 0;
         x.regrouped = layouts[f - 1] == 2;
@@ -1555,6 +1561,7 @@ static int chain_backward_walk(bool run, const void* input, const void* const* v
     if (plan.out_last[f] && own_ld != batch) p.out_ld = own_ld;
     if (p.in_ld && !p.out_ld && plan.out_last[f]) p.out_ld = batch;
     p.no_alloc = 1;
+    if (to_input) p.residual = add;
     const bool turns = plan.in_last[f] != plan.out_last[f];
     if (turns) p.out_bs_last = plan.out_last[f];
     Choice ch = turns ? Choice{KSMM_ALGO_TC, -1} : auto_choice(p);
@@ -1579,6 +1586,12 @@ static int chain_backward_walk(bool run, const void* input, const void* const* v
   if (run && post)
     st = bs_last ? launch_transpose(g0, grad_input, batch, n_in, es, stream)
                  : launch_transpose(g0, grad_input, n_in, batch, es, stream, 0, ld);
+  if (run && post && add && st == KSMM_OK) {
+    Problem rp;
+    rp.out = grad_input; rp.residual = add; rp.out_dtype = dtype;
+    rp.a = patterns[0]; rp.b = patterns[2]; rp.d = patterns[3]; rp.batch = batch;
+    st = residual_pass(rp, stream);
+  }
   if (need) *need = second_bytes + 2 * one + post_bytes + align_up(tail_bytes, 256);
   return st;
 }
@@ -1617,7 +1630,8 @@ int ksmm_cu_chain_train_bytes(int nfactors, const int32_t* patterns, int64_t bat
       for (int f = 0; f + 1 < nfactors && kind == 1; ++f) layouts[f] = one_layout ? bs_last : 0;
       for (int need_input = 0; need_input < 2; ++need_input) {
         st = chain_backward_walk(false, nullptr, nullptr, nullptr, layouts, nullptr, nullptr, nullptr, nullptr, nullptr, SIZE_MAX,
-                                 batch, nfactors, patterns, dtype, bs_last, need_input != 0, allow != 0, one_layout, nullptr, &need);
+                                 batch, nfactors, patterns, dtype, bs_last, need_input != 0, allow != 0, one_layout, nullptr, &need,
+                                 bs_last, batch);
         if (st != KSMM_OK) return st;
         *backward_bytes = std::max(*backward_bytes, need);
       }
@@ -1675,14 +1689,405 @@ int ksmm_cu_chain_backward(const void* input, const void* const* values, const v
   const bool one_layout = train_one_layout(nfactors, patterns, batch, dtype, bs_last);
   bool allow = aligned16(grad_input) && train_may_switch(nfactors, patterns, batch, dtype, bs_last, true, grad_input != nullptr);
   for (int f = 0; f < nfactors; ++f) allow = allow && aligned16(values[f]);
+  const void* inters[ChainPlan::kMax] = {};
+  for (int f = 0; f + 1 < nfactors; ++f)
+    inters[f] = static_cast<const char*>(saved) + f * train_buffer_bytes(nfactors, patterns, batch, dtype);
   size_t need = 0;
   for (int run = 0; run < 2; ++run) {
-    st = chain_backward_walk(run != 0, input, values, saved, layouts, grad_output, grad_input, grad_values, grad_bias,
+    st = chain_backward_walk(run != 0, input, values, inters, layouts, grad_output, grad_input, grad_values, grad_bias,
                              static_cast<char*>(workspace), run ? workspace_bytes : SIZE_MAX, batch, nfactors, patterns, dtype,
-                             bs_last, grad_input != nullptr, allow, one_layout, s, run ? nullptr : &need);
+                             bs_last, grad_input != nullptr, allow, one_layout, s, run ? nullptr : &need, bs_last, batch);
     if (st != KSMM_OK) return st;
     if (!run && need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < need))
       return set_error(KSMM_ERR_WORKSPACE, "chain backward: need %zu bytes aligned to 256, got %zu", need, workspace_bytes);
+  }
+  return KSMM_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Gated layers: two chains of the same patterns on one input and the product of their results.
+// The factors run in pairs, in one launch where a grouped kernel takes them; an intermediate is one tensor
+// with the gate's half first.  The layouts are planned as a chain's, with the costs of pairs.  In training
+// both halves before the product are kept, in the layout L in which the last factor leaves them; the
+// gradient of the output is brought into L, the product's backward runs there, and the two chains follow.
+// ---------------------------------------------------------------------------
+struct GatedPlan {
+  bool pre = false, post = false;  // transposes at the ends
+  int in_last[ChainPlan::kMax], out_last[ChainPlan::kMax];
+};
+
+static double gated_last_cost(const int32_t* q, int64_t batch, int dtype, int in_last, int out_last, bool pad) {
+  const double out = static_cast<double>(dtype_size(dtype)) * q[0] * q[1] * q[3] * batch;
+  const double c = step_cost(q, batch, dtype, in_last, out_last, pad);
+  return c < 0 ? c : 2.0 * c + 3.0 * out;  // a pass that reads both halves and writes the product
+}
+
+static void plan_gated(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int in_last, int out_last,
+                       bool allow_switch, bool pad, GatedPlan* plan) {
+  for (int f = 0; f < nfactors; ++f) plan->in_last[f] = plan->out_last[f] = in_last;
+  plan->pre = false;
+  plan->post = in_last != out_last;
+  if (!allow_switch || nfactors > 8 || batch <= 0) return;
+  const double es = dtype_size(dtype);
+  const int32_t* pl = patterns + 4 * (nfactors - 1);
+  const double in_bytes = es * patterns[0] * patterns[2] * patterns[3] * batch, out_bytes = es * pl[0] * pl[1] * pl[3] * batch;
+  const double kTranspose = 0.75 * 2.0;
+  double best = -1.0;
+  for (int pre = 0; pre < 2; ++pre) {
+    for (unsigned mask = 0; mask < (1u << nfactors); ++mask) {
+      int state = pre ? !in_last : in_last;
+      double cost = pre ? kTranspose * in_bytes : 0.0;
+      bool ok = true;
+      for (int f = 0; f < nfactors && ok; ++f) {
+        const int o = (mask >> f) & 1;
+        const int32_t* q = patterns + 4 * f;
+        const double c = f + 1 == nfactors ? gated_last_cost(q, batch, dtype, state, o, pad)
+                                           : 2.0 * step_cost(q, batch, dtype, state, o, pad);
+        if (c < 0) ok = false;
+        cost += c;
+        state = o;
+      }
+      if (!ok) continue;
+      if (state != out_last) cost += kTranspose * out_bytes;
+      if (best < 0 || cost < best * 0.999) {
+        best = cost;
+        int s2 = pre ? !in_last : in_last;
+        for (int f = 0; f < nfactors; ++f) {
+          plan->in_last[f] = s2;
+          s2 = plan->out_last[f] = (mask >> f) & 1;
+        }
+        plan->pre = pre != 0;
+        plan->post = s2 != out_last;
+      }
+    }
+  }
+}
+
+// bytes of one intermediate (both halves), and of both halves before the product
+static size_t gated_buffer_bytes(int nfactors, const int32_t* patterns, int64_t ld, int es) {
+  size_t mx = 0;
+  for (int f = 0; f + 1 < nfactors; ++f) {
+    const int32_t* q = patterns + 4 * f;
+    mx = std::max(mx, static_cast<size_t>(q[0]) * q[1] * q[3]);
+  }
+  return align_up(2 * mx * ld * es, 256);
+}
+
+// Runs one factor of both chains: the input is shared or two halves, weights, output and bias are two halves.
+static int run_pair(const Problem& p, int shared_input, size_t scratch_room, cudaStream_t stream) {
+  Problem g = p;
+  g.groups = 2;
+  g.group_shared_input = shared_input;
+  g.scratch = nullptr;
+  g.scratch_bytes = 0;
+  Choice pin;
+  const int cfg = p.in_dtype != KSMM_F32 && !lookup_choice(p, &pin) && 2 * ((p.b + 63) / 64) <= tc::num_sms() ? tc_default_config(g) : -1;
+  if (cfg >= 0) return tc_launch(g, cfg, stream);
+  const size_t es = dtype_size(p.in_dtype);
+  const size_t in_half = static_cast<size_t>(p.a) * p.c * p.d * (p.bs_last ? in_stride(p) : p.batch) * es;
+  const size_t out_half = static_cast<size_t>(p.a) * p.b * p.d * (out_is_last(p) ? out_stride(p) : p.batch) * es;
+  for (int q = 0; q < 2; ++q) {
+    Problem h = p;
+    h.in = static_cast<const char*>(p.in) + (shared_input ? 0 : q * in_half);
+    h.w = static_cast<const char*>(p.w) + q * (static_cast<size_t>(p.a) * p.b * p.c * p.d * es);
+    h.out = static_cast<char*>(p.out) + q * out_half;
+    if (p.bias) h.bias = static_cast<const char*>(p.bias) + q * (static_cast<size_t>(p.a) * p.b * p.d * es);
+    Choice ch = h.out_bs_last >= 0 ? Choice{KSMM_ALGO_TC, -1} : auto_choice(h);
+    const size_t need = h.out_bs_last >= 0 ? 0 : scratch_need(h, ch);
+    if (need > scratch_room) ch = Choice{KSMM_ALGO_SIMT, -1};
+    else h.scratch_bytes = need;
+    const int st = run_family(h, ch.algo, ch.config, stream);
+    if (st != KSMM_OK) return st;
+  }
+  return KSMM_OK;
+}
+
+// Plans (run == false) or runs the forward pass.  keep: intermediates and both halves go to `saved`, else they are
+// part of the workspace.  *need: bytes of the workspace.  *layout: where the last factor leaves its halves.
+static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool keep, bool allow, bool one_layout,
+                      cudaStream_t stream, size_t* need) {
+  const int n = D.nfactors, es = dtype_size(D.dtype);
+  const int64_t batch = D.batch;
+  // Rows of batch-last tensors between the ends: padded where tensor maps could not address them; a layer that
+  // keeps one layout has rows of the batch, and factors pad their own copies.
+  const int64_t ld = one_layout ? batch : padded_ld(batch, es);
+  GatedPlan plan;
+  plan_gated(n, D.patterns, batch, D.dtype, D.bs_last, out_last, allow && !one_layout, !one_layout, &plan);
+  const int32_t* p0 = D.patterns;
+  const int32_t* pl = D.patterns + 4 * (n - 1);
+  const int64_t n_in = static_cast<int64_t>(p0[0]) * p0[2] * p0[3], n_out = static_cast<int64_t>(pl[0]) * pl[1] * pl[3];
+  const int L = plan.out_last[n - 1];
+  const bool pad_in = ld != batch && D.bs_last && !plan.pre && p0[1] >= 32 && p0[2] >= 16;
+  const size_t pre_bytes = plan.pre || pad_in ? align_up(static_cast<size_t>(n_in) * ld * es, 256) : 0;
+  const size_t one = gated_buffer_bytes(n, D.patterns, ld, es);
+  const size_t halves_bytes = align_up(2 * static_cast<size_t>(n_out) * ld * es, 256);
+  const size_t post_bytes = plan.post ? align_up(static_cast<size_t>(n_out) * ld * es, 256) : 0;
+  const int buffers = std::min(n - 1, 2);
+  char* ws = run ? static_cast<char*>(D.workspace) : reinterpret_cast<char*>(static_cast<uintptr_t>(1) << 20);
+  char* kept = run ? static_cast<char*>(D.saved) : ws;
+  char* x2 = ws;
+  char* h2 = x2 + pre_bytes;
+  char* at = h2 + post_bytes;
+  char* inter = keep ? kept : at;
+  if (!keep) at += one * buffers;
+  char* halves = keep ? kept + one * (n - 1) : at;
+  if (!keep) at += halves_bytes;
+  const size_t used = static_cast<size_t>(at - ws);
+  const size_t room = run ? D.workspace_bytes - used : SIZE_MAX;
+  size_t scratch = 0;
+  int st = KSMM_OK;
+  const void* cur = run ? D.input : ws;
+  if (run && plan.pre)
+    st = D.bs_last ? launch_transpose(D.input, x2, n_in, batch, es, stream)
+                   : launch_transpose(D.input, x2, batch, n_in, es, stream, ld);
+  if (run && pad_in) st = launch_copy_rows(D.input, batch, x2, ld, n_in, batch, es, stream);
+  if (st != KSMM_OK) return st;
+  if (plan.pre || pad_in) cur = x2;
+  for (int f = 0; f < n; ++f) {
+    const int32_t* q = D.patterns + 4 * f;
+    const bool last = f + 1 == n;
+    Problem p;
+    p.in = cur; p.w = run ? D.values[f] : ws; p.bias = last ? D.bias : nullptr;
+    p.out = last ? halves : inter + (keep ? f : f & 1) * one;
+    p.batch = batch; p.a = q[0]; p.b = q[1]; p.c = q[2]; p.d = q[3];
+    p.in_dtype = p.out_dtype = D.dtype; p.alpha = 1.f;
+    p.bs_last = plan.in_last[f];
+    p.out_bs_last = plan.out_last[f] == plan.in_last[f] ? -1 : plan.out_last[f];
+    if (ld != batch) {
+      if (plan.in_last[f]) p.in_ld = f > 0 || plan.pre || pad_in ? ld : batch;
+      if (plan.out_last[f]) p.out_ld = ld;
+    }
+    p.no_alloc = 1;
+    if (run) {
+      p.scratch = at;
+      st = run_pair(p, f == 0, room, stream);
+      if (st != KSMM_OK) return st;
+    } else {
+      st = check_problem(p);
+      if (st != KSMM_OK) return st;
+      if (p.out_bs_last < 0) scratch = std::max(scratch, scratch_need(p, auto_choice(p)));
+    }
+    cur = p.out;
+    if (D.layouts) D.layouts[f] = plan.out_last[f];
+  }
+  if (run) {
+    void* h = plan.post ? h2 : D.output;
+    if (L) st = launch_gate(halves, ld, h, plan.post ? ld : batch, n_out, batch, D.dtype, D.activation, stream);
+    else st = launch_gate(halves, n_out, h, n_out, batch, n_out, D.dtype, D.activation, stream);
+    if (st == KSMM_OK && plan.post)
+      st = L ? launch_transpose(h2, D.output, n_out, batch, es, stream, 0, ld)
+             : launch_transpose(h2, D.output, batch, n_out, es, stream);
+  }
+  if (need) *need = used + align_up(scratch, 256);
+  return st;
+}
+
+static int gated_backward_walk(bool run, const ksmm_gated_desc_t& D, int out_last, const void* grad_output, void* grad_input,
+                               void* const* grad_values, void* grad_bias, bool need_input, bool allow, bool one_layout,
+                               cudaStream_t stream, size_t* need) {
+  const int n = D.nfactors, es = dtype_size(D.dtype);
+  const int64_t batch = D.batch;
+  const int64_t ld = one_layout ? batch : padded_ld(batch, es);
+  const int32_t* pl = D.patterns + 4 * (n - 1);
+  const int64_t n_out = static_cast<int64_t>(pl[0]) * pl[1] * pl[3];
+  const int64_t n_in = static_cast<int64_t>(D.patterns[0]) * D.patterns[2] * D.patterns[3];
+  const int L = D.layouts[n - 1];
+  const size_t one = gated_buffer_bytes(n, D.patterns, ld, es);
+  const size_t turn_bytes = L != out_last ? align_up(static_cast<size_t>(n_out) * ld * es, 256) : 0;
+  const size_t half_bytes = static_cast<size_t>(n_out) * (L ? ld : batch) * es;
+  const size_t half_at = align_up(half_bytes, 256);  // the up projection's gradient starts aligned
+  const size_t gx_bytes = need_input ? align_up(static_cast<size_t>(n_in) * batch * es, 256) : 0;
+  char* ws = run ? static_cast<char*>(D.workspace) : reinterpret_cast<char*>(static_cast<uintptr_t>(1) << 20);
+  char* turned = ws;
+  char* grads = turned + turn_bytes;
+  char* gx = grads + 2 * half_at;
+  char* tail = gx + gx_bytes;
+  const size_t used = static_cast<size_t>(tail - ws);
+  int st = KSMM_OK;
+  if (run) {
+    const char* halves = static_cast<const char*>(D.saved) + one * (n - 1);
+    const void* dh = grad_output;
+    int64_t dh_ld = L ? batch : n_out;
+    if (turn_bytes) {
+      st = L ? launch_transpose(grad_output, turned, batch, n_out, es, stream, ld)
+             : launch_transpose(grad_output, turned, n_out, batch, es, stream);
+      if (st != KSMM_OK) return st;
+      dh = turned;
+      if (L) dh_ld = ld;
+    }
+    st = launch_gate_backward(halves, L ? ld : n_out, dh, dh_ld, grads, static_cast<int64_t>(half_at) / es, L ? n_out : batch, L ? batch : n_out, D.dtype,
+                              D.activation, stream);
+    if (st != KSMM_OK) return st;
+  }
+  const void *vals[ChainPlan::kMax] = {}, *inters[ChainPlan::kMax] = {};
+  void* gv[ChainPlan::kMax] = {};
+  size_t tail_need = 0;
+  for (int q = 0; q < 2; ++q) {
+    for (int f = 0; f < n && run; ++f) {
+      const int32_t* t = D.patterns + 4 * f;
+      const size_t half = static_cast<size_t>(t[0]) * t[1] * t[2] * t[3] * es;
+      vals[f] = static_cast<const char*>(D.values[f]) + q * half;
+      gv[f] = grad_values[f] ? static_cast<char*>(grad_values[f]) + q * half : nullptr;
+    }
+    for (int f = 0; f + 1 < n; ++f) {
+      const int32_t* t = D.patterns + 4 * f;
+      inters[f] = static_cast<const char*>(D.saved) + f * one +
+                  q * (static_cast<size_t>(t[0]) * t[1] * t[3] * (D.layouts[f] ? ld : batch) * es);
+    }
+    size_t w = 0;
+    st = chain_backward_walk(run, D.input, vals, inters, D.layouts, grads + q * half_at,
+                             q == 0 ? gx : grad_input, gv,
+                             grad_bias ? static_cast<char*>(grad_bias) + q * (n_out * es) : nullptr, tail,
+                             run ? D.workspace_bytes - used : SIZE_MAX, batch, n, D.patterns, D.dtype, D.bs_last, need_input, allow,
+                             one_layout, stream, run ? nullptr : &w, L, ld,
+                             need_input && q == 1 ? gx : nullptr);
+    if (st != KSMM_OK) return st;
+    tail_need = std::max(tail_need, w);
+  }
+  if (need) *need = used + tail_need;
+  return st;
+}
+
+static int check_gated(int nfactors, const int32_t* patterns, const void* const* values, int64_t batch, int dtype, int bs_last,
+                       int out_last, int activation) {
+  if (activation < 0 || activation > KSMM_ACT_SIGMOID)
+    return set_error(KSMM_ERR_BAD_ARGUMENT, "unknown activation %d", activation);
+  int st = check_train(nfactors, patterns, values, batch, dtype, bs_last);
+  if (st != KSMM_OK) return st;
+  if (out_last != 0 && out_last != 1) return set_error(KSMM_ERR_BAD_ARGUMENT, "the output's layout must be 0 or 1");
+  return KSMM_OK;
+}
+
+static ksmm_gated_desc_t gated_desc(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last, int32_t* layouts) {
+  ksmm_gated_desc_t D = {};
+  D.nfactors = nfactors; D.patterns = patterns; D.batch = batch; D.dtype = dtype; D.bs_last = bs_last;
+  D.layouts = layouts;
+  return D;
+}
+
+static int gated_forward_need(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last, int out_last, bool keep,
+                              bool one_layout, size_t* most) {
+  *most = 0;
+  for (int allow = 0; allow < (one_layout ? 1 : 2); ++allow) {
+    size_t need = 0;
+    int st = gated_walk(false, gated_desc(nfactors, patterns, batch, dtype, bs_last, nullptr), out_last, keep, allow != 0, one_layout,
+                        nullptr, &need);
+    if (st != KSMM_OK) return st;
+    *most = std::max(*most, need);
+  }
+  return KSMM_OK;
+}
+
+size_t ksmm_cu_gated_workspace_bytes(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last, int out_bs_last) {
+  const void* dummy = nullptr;
+  if (check_gated(nfactors, patterns, &dummy, batch, dtype, bs_last, out_bs_last, 0) != KSMM_OK || batch == 0) return 0;
+  size_t need = 0;
+  const int st = gated_forward_need(nfactors, patterns, batch, dtype, bs_last, out_bs_last, false, false, &need);
+  return st == KSMM_OK ? need : 0;
+}
+
+int ksmm_cu_gated_train_bytes(int nfactors, const int32_t* patterns, int64_t batch, int dtype, int bs_last, int out_bs_last,
+                              size_t* saved_bytes, size_t* forward_bytes, size_t* backward_bytes) {
+  const void* dummy = nullptr;
+  int st = check_gated(nfactors, patterns, &dummy, batch, dtype, bs_last, out_bs_last, 0);
+  if (st != KSMM_OK) return st;
+  if (!saved_bytes || !forward_bytes || !backward_bytes) return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
+  *saved_bytes = *forward_bytes = *backward_bytes = 0;
+  if (batch == 0) return KSMM_OK;
+  const bool one_layout = train_one_layout(nfactors, patterns, batch, dtype, bs_last);
+  const int es = dtype_size(dtype);
+  const int64_t ld = one_layout ? batch : padded_ld(batch, es);
+  const int32_t* pl = patterns + 4 * (nfactors - 1);
+  *saved_bytes = gated_buffer_bytes(nfactors, patterns, ld, es) * (nfactors - 1) +
+                 align_up(2 * static_cast<size_t>(pl[0]) * pl[1] * pl[3] * ld * es, 256);
+  if ((st = gated_forward_need(nfactors, patterns, batch, dtype, bs_last, out_bs_last, true, one_layout, forward_bytes)) != KSMM_OK)
+    return st;
+  for (int fwd = 0; fwd < (one_layout ? 1 : 2); ++fwd) {  // layouts of a forward pass with and without switches
+    int32_t layouts[ChainPlan::kMax] = {};
+    const ksmm_gated_desc_t D = gated_desc(nfactors, patterns, batch, dtype, bs_last, layouts);
+    size_t need = 0;
+    st = gated_walk(false, D, out_bs_last, true, fwd != 0, one_layout, nullptr, &need);
+    for (int mode = 0; mode < 4 && st == KSMM_OK; ++mode) {
+      st = gated_backward_walk(false, D, out_bs_last, nullptr, nullptr, nullptr, nullptr, (mode & 1) != 0, (mode >> 1) != 0, one_layout,
+                               nullptr, &need);
+      *backward_bytes = std::max(*backward_bytes, need);
+    }
+    if (st != KSMM_OK) return st;
+  }
+  return KSMM_OK;
+}
+
+static bool aligned_values(const ksmm_gated_desc_t& D) {
+  bool ok = true;
+  for (int f = 0; f < D.nfactors; ++f) {
+    const int32_t* q = D.patterns + 4 * f;
+    ok = ok && aligned16(D.values[f]) && (static_cast<int64_t>(q[0]) * q[1] * q[2] * q[3] * dtype_size(D.dtype)) % 16 == 0;
+  }
+  return ok;
+}
+
+int ksmm_cu_gated_forward(const ksmm_gated_desc_t* desc, void* stream) {
+  if (!desc) return set_error(KSMM_ERR_BAD_ARGUMENT, "null descriptor");
+  const ksmm_gated_desc_t& D = *desc;
+  if (D.out_layout < 0 || D.out_layout > 2) return set_error(KSMM_ERR_BAD_ARGUMENT, "unknown output layout %d", D.out_layout);
+  const int out_last = D.out_layout == 0 ? D.bs_last : D.out_layout - 1;
+  int st = check_gated(D.nfactors, D.patterns, D.values, D.batch, D.dtype, D.bs_last, out_last, D.activation);
+  if (st != KSMM_OK || D.batch == 0) return st;
+  if (!D.input || !D.output) return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
+  if ((st = check_values(D.nfactors, D.values)) != KSMM_OK) return st;
+  const bool keep = D.saved != nullptr;
+  const bool one_layout = keep && train_one_layout(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last);
+  size_t want[3] = {0, 0, 0};
+  st = keep ? ksmm_cu_gated_train_bytes(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, out_last, &want[0], &want[1], &want[2])
+            : gated_forward_need(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, out_last, false, false, &want[1]);
+  if (st != KSMM_OK) return st;
+  if (keep && !D.layouts) return set_error(KSMM_ERR_BAD_ARGUMENT, "null layouts");
+  if ((keep && (reinterpret_cast<uintptr_t>(D.saved) % 256 || D.saved_bytes < want[0])) ||
+      (want[1] && (!D.workspace || reinterpret_cast<uintptr_t>(D.workspace) % 256 || D.workspace_bytes < want[1])))
+    return set_error(KSMM_ERR_WORKSPACE, "gated layer: need %zu bytes kept and %zu of workspace, aligned to 256", want[0], want[1]);
+  // (a trainable fp32 layer keeps the kernels that its factors have one by one, as a chain does)
+  const bool allow = !one_layout && aligned16(D.input) && aligned16(D.output) && aligned_values(D) &&
+                     (!keep || train_may_switch(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, false, true));
+  return gated_walk(true, D, out_last, keep, allow, one_layout, static_cast<cudaStream_t>(stream), nullptr);
+}
+
+int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* grad_output, void* grad_input, void* const* grad_values,
+                           void* grad_bias, void* stream) {
+  if (!desc) return set_error(KSMM_ERR_BAD_ARGUMENT, "null descriptor");
+  const ksmm_gated_desc_t& D = *desc;
+  if (D.out_layout < 0 || D.out_layout > 2) return set_error(KSMM_ERR_BAD_ARGUMENT, "unknown output layout %d", D.out_layout);
+  const int out_last = D.out_layout == 0 ? D.bs_last : D.out_layout - 1;
+  int st = check_gated(D.nfactors, D.patterns, D.values, D.batch, D.dtype, D.bs_last, out_last, D.activation);
+  if (st != KSMM_OK) return st;
+  if (!grad_values) return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int es = dtype_size(D.dtype);
+  const int32_t* pl = D.patterns + 4 * (D.nfactors - 1);
+  if (D.batch == 0) {
+    // sums over nothing
+    for (int f = 0; f < D.nfactors; ++f) {
+      const int32_t* q = D.patterns + 4 * f;
+      if (grad_values[f]) KSMM_CUDA_OK(cudaMemsetAsync(grad_values[f], 0, 2 * static_cast<size_t>(q[0]) * q[1] * q[2] * q[3] * es, s));
+    }
+    if (grad_bias) KSMM_CUDA_OK(cudaMemsetAsync(grad_bias, 0, 2 * static_cast<size_t>(pl[0]) * pl[1] * pl[3] * es, s));
+    return KSMM_OK;
+  }
+  if (!D.input || !grad_output || !D.saved || !D.layouts) return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
+  if ((st = check_values(D.nfactors, D.values)) != KSMM_OK) return st;
+  if (!aligned16(D.input) || !aligned16(grad_output))
+    return set_error(KSMM_ERR_BAD_ARGUMENT, "the backward of a gated layer takes an input and a gradient aligned to 16 bytes");
+  for (int f = 0; f < D.nfactors; ++f)
+    if (D.layouts[f] != 0 && D.layouts[f] != 1) return set_error(KSMM_ERR_BAD_ARGUMENT, "layouts are those of the forward pass");
+  const bool one_layout = train_one_layout(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last);
+  const bool allow = aligned16(grad_input) && aligned_values(D) &&
+                     train_may_switch(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, true, grad_input != nullptr);
+  size_t need = 0;
+  for (int run = 0; run < 2; ++run) {
+    st = gated_backward_walk(run != 0, D, out_last, grad_output, grad_input, grad_values, grad_bias, grad_input != nullptr, allow,
+                             one_layout, s, run ? nullptr : &need);
+    if (st != KSMM_OK) return st;
+    if (!run && (!D.workspace || reinterpret_cast<uintptr_t>(D.workspace) % 256 || D.workspace_bytes < need))
+      return set_error(KSMM_ERR_WORKSPACE, "gated backward: need %zu bytes aligned to 256, got %zu", need, D.workspace_bytes);
   }
   return KSMM_OK;
 }

@@ -32,7 +32,7 @@ namespace ksmm {
 namespace {
 
 enum { kNone = KSMM_NORM_NONE, kLayer = KSMM_NORM_LAYER, kRms = KSMM_NORM_RMS };
-constexpr int kMaxChannels = 16384;
+constexpr int kMaxChannels = 8192;
 
 // a parameter: one row of the channels (ld = 0) or one per sample
 struct Row {
@@ -792,13 +792,14 @@ int launch_rows(const Args& A, cudaStream_t stream) {
     if (pieces <= 128) return go(norm_rows_kernel<T, V, 4, 32>, 32);
     if (pieces <= 256) return go(norm_rows_kernel<T, V, 2, 128>, 128);
     if (pieces <= 512) return go(norm_rows_kernel<T, V, 4, 128>, 128);
-    if (pieces <= 1024) return go(norm_rows_kernel<T, V, 4, 256>, 256);
-    return go(norm_rows_kernel<T, V, 4, 1024>, 1024);
+    if constexpr (V == 4) {
+      if (pieces > 1024) return go(norm_rows_kernel<T, V, 4, 512>, 512);
+    }
+    return go(norm_rows_kernel<T, V, 4, 256>, 256);
   } else {
     if (pieces <= 256) return go(norm_rows_kernel<T, 1, 8, 32>, 32);
-    if (pieces <= 1024) return go(norm_rows_kernel<T, 1, 32, 32>, 32);
-    if (pieces <= 4096) return go(norm_rows_kernel<T, 1, 32, 128>, 128);
-    return go(norm_rows_kernel<T, 1, 32, 512>, 512);
+    if (pieces <= 1024) return go(norm_rows_kernel<T, 1, 8, 128>, 128);
+    return go(norm_rows_kernel<T, 1, 16, 512>, 512);
   }
 }
 
@@ -815,15 +816,14 @@ int launch_rows_backward(const Args& A, cudaStream_t stream) {
   };
   if constexpr (V > 1) {
     if (k <= 1) return go(norm_rows_backward_kernel<T, V, 1, 2>, 1);
-    if (k <= 2) return go(norm_rows_backward_kernel<T, V, 2, 1>, 2);
-    if (k <= 4) return go(norm_rows_backward_kernel<T, V, 4, 1>, 4);
-    return go(norm_rows_backward_kernel<T, V, 8, 1>, 8);
+    if constexpr (V == 4) {
+      if (k > 2) return go(norm_rows_backward_kernel<T, V, 4, 1>, 4);
+    }
+    return go(norm_rows_backward_kernel<T, V, 2, 1>, 2);
   } else {
     if (k <= 1) return go(norm_rows_backward_kernel<T, 1, 1, 4>, 1);
-    if (k <= 2) return go(norm_rows_backward_kernel<T, 1, 2, 4>, 2);
     if (k <= 4) return go(norm_rows_backward_kernel<T, 1, 4, 2>, 4);
-    if (k <= 8) return go(norm_rows_backward_kernel<T, 1, 8, 1>, 8);
-    return go(norm_rows_backward_kernel<T, 1, 32, 1>, 32);
+    return go(norm_rows_backward_kernel<T, 1, 16, 1>, 16);
   }
 }
 

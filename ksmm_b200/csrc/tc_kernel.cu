@@ -854,8 +854,8 @@ bool tc_config_supported(const Problem& p, int config, bool check_pointers) {
   }
   const bool out_last = p.out_bs_last < 0 ? p.bs_last != 0 : p.out_bs_last != 0;
   if (out_last != (p.bs_last != 0)) {
-    // a factor that changes the layout: 16-bit, d = 1, no groups, no regrouping
-    if (p.d != 1 || p.groups > 1 || p.out_regroup_d || p.in_regrouped) return false;
+    // a factor that changes the layout: 16-bit, d = 1, no regrouping
+    if (p.d != 1 || p.out_regroup_d || p.in_regrouped) return false;
     if (p.in_dtype == KSMM_F32) return config >= 0 && config <= 3 && tc_f32x3_supported(p, check_pointers);
     if ((p.in_dtype != KSMM_F16 && p.in_dtype != KSMM_BF16) || p.out_dtype != p.in_dtype) return false;
     if (p.batch <= 0 || p.batch > 0x7fffffffLL) return false;

@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -447,6 +448,146 @@ py::object layer_train(const at::Tensor& x, const std::vector<at::Tensor>& facto
   return py::cast(out);
 }
 
+// a gated layer without gradients
+bool gated_fits(const at::Tensor& x, const std::vector<at::Tensor>& factors, const Patterns& p, bool last,
+                const c10::optional<at::Tensor>& bias) {
+  return p.n <= 16 && usable(x) && plain_dtype(x) && chain_fits(x, factors, p, last, x.scalar_type(), 2) &&
+         bias_fits(bias, x, 2 * p.out(p.n - 1), x.scalar_type());
+}
+
+ksmm_gated_desc_t gated_desc(const at::Tensor& x, const void* const* values, const int32_t* patterns, int n, bool last, bool out_last,
+                             int activation) {
+  ksmm_gated_desc_t d = {};
+  d.input = x.data_ptr();
+  d.values = values;
+  d.batch = x.size(last ? 1 : 0);
+  d.nfactors = n;
+  d.patterns = patterns;
+  d.dtype = dtype_code(x);
+  d.bs_last = last;
+  d.out_layout = out_last ? 2 : 1;
+  d.activation = activation;
+  return d;
+}
+
+py::object gated_forward(const at::Tensor& x, const std::vector<at::Tensor>& factors, const py::handle& patterns, bool last,
+                         bool out_last, const c10::optional<at::Tensor>& bias, int activation) {
+  Patterns p;
+  if (!read_patterns(patterns, &p) || !gated_fits(x, factors, p, last, bias)) return py::none();
+  int st;
+  at::Tensor out;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto vals = pointers(factors);
+    ksmm_gated_desc_t d = gated_desc(x, vals.data(), p.flat.data(), p.n, last, out_last, activation);
+    out = new_tensor(p.out(p.n - 1), d.batch, out_last, x.options().requires_grad(false));
+    d.workspace_bytes = ksmm_cu_gated_workspace_bytes(p.n, p.flat.data(), d.batch, d.dtype, last, out_last);
+    const at::Tensor ws = new_bytes(d.workspace_bytes, x);
+    d.workspace = ws.data_ptr();
+    d.output = out.data_ptr();
+    d.bias = ptr_or_null(bias);
+    st = ksmm_cu_gated_forward(&d, stream_of(x));
+  }
+  return result(st, out);
+}
+
+// A trainable gated layer as one autograd node: ksmm_b200.kernel.GatedFunction without Python in its backward.
+struct GatedNode : torch::autograd::Function<GatedNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x_in, const c10::optional<at::Tensor>& bias,
+                            at::TensorList factors, std::vector<int64_t> patterns, bool last, bool out_last, int64_t activation) {
+    const at::Tensor x = aligned(x_in);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int n = static_cast<int>(factors.size());
+    const std::vector<int32_t> flat(patterns.begin(), patterns.end());
+    std::vector<const void*> vals(n);
+    for (int f = 0; f < n; ++f) vals[f] = factors[f].data_ptr();
+    ksmm_gated_desc_t d = gated_desc(x, vals.data(), flat.data(), n, last, out_last, static_cast<int>(activation));
+    const int32_t* pl = flat.data() + 4 * (n - 1);
+    size_t bytes[3];
+    raise_status(ksmm_cu_gated_train_bytes(n, flat.data(), d.batch, d.dtype, last, out_last, &bytes[0], &bytes[1], &bytes[2]));
+    at::Tensor out = new_tensor(static_cast<int64_t>(pl[0]) * pl[1] * pl[3], d.batch, out_last, x.options());
+    // (an empty batch keeps nothing, but a saved pointer says that this is training)
+    const at::Tensor saved = new_bytes(std::max<size_t>(bytes[0], 1), x), ws = new_bytes(bytes[1], x);
+    int32_t layouts[16] = {};
+    d.output = out.data_ptr();
+    d.bias = ptr_or_null(bias);
+    d.saved = saved.data_ptr();
+    d.saved_bytes = bytes[0];
+    d.workspace = ws.data_ptr();
+    d.workspace_bytes = bytes[1];
+    d.layouts = layouts;
+    raise_status(ksmm_cu_gated_forward(&d, stream_of(x)));
+    torch::autograd::variable_list keep{x, saved};
+    keep.insert(keep.end(), factors.begin(), factors.end());
+    ctx->save_for_backward(std::move(keep));
+    // number of factors, layouts, activation, bytes of the backward, patterns, kept layouts, the bias's shape
+    std::vector<int64_t> meta{n, last, out_last, activation, static_cast<int64_t>(bytes[2])};
+    meta.insert(meta.end(), patterns.begin(), patterns.end());
+    for (int f = 0; f < n; ++f) meta.push_back(layouts[f]);
+    meta.push_back(bias.has_value());
+    if (bias.has_value()) meta.insert(meta.end(), bias->sizes().begin(), bias->sizes().end());
+    ctx->saved_data["gated"] = std::move(meta);
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto kept = ctx->get_saved_variables();
+    const std::vector<int64_t> meta = ctx->saved_data["gated"].toIntVector();
+    const int n = static_cast<int>(meta[0]);
+    const bool last = meta[1] != 0, out_last = meta[2] != 0;
+    const std::vector<int32_t> flat(meta.begin() + 5, meta.begin() + 5 + 4 * n);
+    std::vector<int32_t> layouts(meta.begin() + 5 + 4 * n, meta.begin() + 5 + 5 * n);
+    const size_t at_bias = 5 + 5 * static_cast<size_t>(n);
+    const bool has_bias = meta[at_bias] != 0;
+    const at::Tensor& x = kept[0];
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor g = aligned(grads[0].contiguous());
+    // edges of the graph: the input, the bias if there is one, the factors
+    at::Tensor gx, gb;
+    if (ctx->needs_input_grad(0)) gx = at::empty(x.sizes(), x.options());
+    if (has_bias && ctx->needs_input_grad(1))
+      gb = at::empty(at::IntArrayRef(meta.data() + at_bias + 1, meta.size() - at_bias - 1), x.options());
+    std::vector<at::Tensor> gw(n);
+    std::vector<const void*> vals(n);
+    std::vector<void*> outs(n, nullptr);
+    for (int f = 0; f < n; ++f) {
+      const at::Tensor& w = kept[2 + f];
+      vals[f] = w.data_ptr();
+      if (ctx->needs_input_grad(1 + has_bias + f)) {
+        gw[f] = at::empty(w.sizes(), w.options());
+        outs[f] = gw[f].data_ptr();
+      }
+    }
+    ksmm_gated_desc_t d = gated_desc(x, vals.data(), flat.data(), n, last, out_last, static_cast<int>(meta[3]));
+    const at::Tensor ws = new_bytes(static_cast<size_t>(meta[4]), x);
+    d.workspace = ws.data_ptr();
+    d.workspace_bytes = static_cast<size_t>(meta[4]);
+    d.saved = kept[1].data_ptr();
+    d.saved_bytes = static_cast<size_t>(kept[1].numel());
+    d.layouts = layouts.data();
+    raise_status(ksmm_cu_gated_backward(&d, g.data_ptr(), gx.defined() ? gx.data_ptr() : nullptr, outs.data(),
+                                        gb.defined() ? gb.data_ptr() : nullptr, stream_of(x)));
+    torch::autograd::variable_list r{gx, gb};
+    r.insert(r.end(), gw.begin(), gw.end());
+    for (int q = 0; q < 4; ++q) r.emplace_back();  // patterns, layouts, activation
+    return r;
+  }
+};
+
+py::object gated_train(const at::Tensor& x, const std::vector<at::Tensor>& factors, const py::handle& patterns, bool last,
+                       bool out_last, const c10::optional<at::Tensor>& bias, int activation) {
+  Patterns p;
+  if (!read_patterns(patterns, &p) || !gated_fits(x, factors, p, last, bias)) return py::none();
+  at::Tensor out;
+  {
+    py::gil_scoped_release nogil;
+    out = GatedNode::apply(x, bias, at::TensorList(factors), std::vector<int64_t>(p.flat.begin(), p.flat.end()), last, out_last,
+                           static_cast<int64_t>(activation));
+  }
+  return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -459,4 +600,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("factor_forward", &factor_forward, "One factor in its input's type");
   m.def("fp8_forward", &fp8_forward, "The factors of an fp8 KSLinear");
   m.def("grouped_forward", &grouped_forward, "Several chains on one input");
+  m.def("gated_forward", &gated_forward, "A gated layer without gradients");
+  m.def("gated_train", &gated_train, "A trainable gated layer as one autograd node");
 }

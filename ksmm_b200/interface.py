@@ -313,3 +313,97 @@ class KSLinearGroup(nn.Module):
         factors, bias = self._stack()
         out = _k.grouped_chain_forward(x, factors, first.patterns, first.bs_last, len(self.layers), bias=bias)
         return tuple(first.post_process(tensor, out[g]) for g in range(len(self.layers)))
+
+
+class KSGatedLinear(nn.Module):
+    r"""``activation(gate(x)) * up(x)`` with two Kronecker-sparse layers of the same patterns: the first half of a
+    gated feed-forward block (``KSLinear`` is the second).  The reference builds feed-forward blocks from
+    single layers only (src/ksmm_py/model/vit.py:416-431); this layer is an addition to it, with
+    ``KSLinear``'s constructor where they share arguments.
+
+    ``factors[f]`` is (2 * a*d*c, b): the gate's kernel-format factor, then the up projection's; ``bias``
+    holds 2 * out_size elements in the same order.  ``gate_weights`` and ``up_weights`` are lists of optional
+    4-D ``(a,b,c,d)`` tensors.  ``activation``: "silu", "gelu", "relu", "sigmoid" or None; ``out_bs_last`` as
+    in ``KSLinear`` (also with gradients).  Types: fp32, fp16 and bf16; up to 16 factors."""
+
+    def __init__(self, patterns, gate_weights=None, up_weights=None, bias=True, algo="kernel",
+                 dtype: torch.dtype = torch.float16, bs_last: bool = False, vsize: int = 4, device: str = "cuda",
+                 activation="silu", requires_grad: bool = False, out_bs_last=None):
+        super().__init__()
+        if algo != "kernel":
+            raise NotImplementedError(f"algo={algo!r}: this library implements the reference's algo='kernel' only")
+        if activation not in _lib.GATES:
+            raise ValueError(f"activation={activation!r}: expected None, 'silu', 'gelu', 'relu' or 'sigmoid'")
+        if not 0 < len(patterns) <= _k.MAX_GATED_FACTORS:
+            raise ValueError(f"a gated layer has 1 to {_k.MAX_GATED_FACTORS} factors")
+        for pattern in patterns:
+            assert len(pattern) == 4
+        for p, q in zip(patterns[:-1], patterns[1:]):
+            if p[0] * p[1] * p[3] != q[0] * q[2] * q[3]:
+                raise ValueError(f"pattern {tuple(p)} feeds {p[0] * p[1] * p[3]} features into {tuple(q)}")
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise TypeError(f"gated layers run in float32, float16 or bfloat16, not {dtype}")
+        if str(device) == "cpu":
+            raise Exception("kernel expects device='cuda'.")
+        self.patterns = [tuple(int(v) for v in p) for p in patterns]
+        self.in_size = patterns[0][0] * patterns[0][2] * patterns[0][3]
+        self.out_size = patterns[-1][0] * patterns[-1][1] * patterns[-1][3]
+        self.num_mat = len(patterns)
+        self.algo, self.dtype, self.bs_last, self.vsize, self.device = algo, dtype, bs_last, vsize, device
+        self.activation = activation
+        self.out_bs_last = bool(bs_last) if out_bs_last is None else bool(out_bs_last)
+        gate_weights = [None] * self.num_mat if gate_weights is None else gate_weights
+        up_weights = [None] * self.num_mat if up_weights is None else up_weights
+        if len(gate_weights) != self.num_mat or len(up_weights) != self.num_mat:
+            raise ValueError("need one weight per pattern")
+        self.factors = nn.ParameterList([
+            nn.Parameter(torch.cat([self._factor(p, w, dtype, device) for w in pair]), requires_grad=bool(requires_grad))
+            for p, *pair in zip(self.patterns, gate_weights, up_weights)])
+        if bias:
+            bound = 1 / math.sqrt(self.in_size)
+            shape = (2 * self.out_size, 1) if bs_last else (2 * self.out_size,)
+            self.bias = nn.Parameter(torch.empty(*shape, device=device).uniform_(-bound, bound).to(dtype),
+                                     requires_grad=bool(requires_grad))
+        else:
+            self.register_parameter("bias", None)
+
+    @staticmethod
+    def _factor(pattern, weights, dtype, device):
+        if weights is not None:
+            return generate_factor(*pattern, "kernel", weights, dtype, device)
+        # (drawn where it is used: half a million values on the host and their copy take milliseconds)
+        a, b, c, d = pattern
+        scaling = 1.0 / math.sqrt(c)
+        return torch.empty(a * d * c, b, device=device).uniform_(-scaling, scaling).to(dtype)
+
+    def forward(self, tensor):
+        """tensor: (..., in_size) for batch-first, (in_size, ...) for batch-last.  A layer that changes the layout
+        returns a 2-D tensor."""
+        if tensor.dtype != self.dtype:
+            raise TypeError(f"input dtype {tensor.dtype} differs from the layer's {self.dtype}")
+        x = (tensor.reshape(tensor.size(0), -1) if self.bs_last else tensor.reshape(-1, tensor.size(-1))).contiguous()
+        factors = list(self.factors)
+        learns = torch.is_grad_enabled() and (x.requires_grad or any(f.requires_grad for f in factors)
+                                              or (self.bias is not None and self.bias.requires_grad))
+        call = _k.gated_chain_train if learns else _k.gated_chain_forward
+        y = call(x, factors, self.patterns, self.bs_last, self.bias, self.activation, self.out_bs_last)
+        if self.out_bs_last != bool(self.bs_last):
+            return y
+        if self.bs_last:
+            return y.view(self.out_size, *tensor.shape[1:])
+        return y.view(*tensor.shape[:-1], self.out_size)
+
+    def get_dense_products(self):
+        """Dense (out_size, in_size) matrices of the gate's and the up projection's chain."""
+        both = []
+        for q in range(2):
+            dense = None
+            for factor, pattern in zip(self.factors, self.patterns):
+                m = from_kernel_format_to_dense(factor.data.chunk(2)[q].float(), pattern)
+                dense = m if dense is None else torch.matmul(m, dense)
+            both.append(dense)
+        return tuple(both)
+
+    def extra_repr(self):
+        return "in_size={}, out_size={}, num_mat={}, patterns={}, algo={}, bias={}, activation={!r}".format(
+            self.in_size, self.out_size, self.num_mat, self.patterns, self.algo, self.bias is not None, self.activation)

@@ -322,6 +322,119 @@ def grouped_chain_forward(input, stacked_factors, patterns, bs_last, groups, bia
     return out
 
 
+def _gated_desc(input, stacked_factors, patterns, bs_last, out_last, bias, activation):
+    """Checks the arguments of a gated call; returns its descriptor and (batch, out features, dtype code)."""
+    bs_last = int(bool(bs_last))
+    nf = len(patterns)
+    if activation not in _lib.GATES:
+        raise ValueError(f"activation={activation!r}: expected None, 'silu', 'gelu', 'relu' or 'sigmoid'")
+    if nf == 0 or len(stacked_factors) != nf:
+        raise ValueError("need one stacked factor per pattern")
+    if nf > MAX_GATED_FACTORS:
+        raise ValueError(f"gated layers have up to {MAX_GATED_FACTORS} factors")
+    if input.dim() != 2 or not input.is_cuda or not input.is_contiguous():
+        raise ValueError("input must be a contiguous 2-D CUDA tensor")
+    code = dtype_code(input.dtype)
+    if input.dtype == torch.float8_e4m3fn:
+        raise TypeError("gated layers run in float32, float16 or bfloat16")
+    feats = input.shape[0] if bs_last else input.shape[1]
+    for f, ((a, b, c, d), w) in enumerate(zip(patterns, stacked_factors)):
+        if a * c * d != feats:
+            raise ValueError(f"factor {f} expects {a * c * d} features but receives {feats}")
+        if tuple(w.shape) != (2 * a * d * c, b) or w.dtype != input.dtype or not w.is_contiguous() or w.device != input.device:
+            raise ValueError(f"stacked factor {f} must be a contiguous ({2 * a * d * c}, {b}) tensor of {input.dtype}")
+        feats = a * b * d
+    if bias is not None and (bias.numel() != 2 * feats or bias.dtype != input.dtype or not bias.is_contiguous()
+                             or bias.device != input.device):
+        raise ValueError("bias must hold 2 * out_size contiguous elements of the input dtype on the input's device")
+    batch = input.shape[1] if bs_last else input.shape[0]
+    desc = _lib.GatedDesc(
+        input=input.data_ptr(), values=(ctypes.c_void_p * nf)(*[w.data_ptr() for w in stacked_factors]),
+        bias=bias.data_ptr() if bias is not None else None, batch=batch, nfactors=nf,
+        patterns=_lib.int32_array([int(v) for p in patterns for v in p]), dtype=code, bs_last=bs_last,
+        out_layout=2 if out_last else 1, activation=_lib.GATES[activation])
+    return desc, (batch, feats, code)
+
+
+MAX_GATED_FACTORS = 16
+
+
+def gated_chain_forward(input, stacked_factors, patterns, bs_last, bias=None, activation="silu", out_bs_last=None):
+    """``activation(gate(x)) * up(x)`` for two chains of the same ``patterns`` on one input
+    (``ksmm_cu_gated_forward``): ``stacked_factors[f]`` is the (2 * a*d*c, b) concatenation of the gate's and the up
+    projection's kernel-format factors f, ``bias`` (2 * out features) their biases.  ``activation``: "silu",
+    "gelu", "relu", "sigmoid" or None.  ``out_bs_last`` as in ``chain_forward``.  Without gradients;
+    ``KSGatedLinear`` is the layer."""
+    out_last = bool(bs_last) if out_bs_last is None else bool(out_bs_last)
+    if _native is not None and activation in _lib.GATES:
+        out = _native.gated_forward(input, list(stacked_factors), patterns, bool(bs_last), out_last, bias, _lib.GATES[activation])
+        if out is not None:
+            return _result(out)
+    lib = _lib.load()
+    desc, (batch, feats, code) = _gated_desc(input, stacked_factors, patterns, bs_last, out_last, bias, activation)
+    out = torch.empty((feats, batch) if out_last else (batch, feats), dtype=input.dtype, device=input.device)
+    need = lib.ksmm_cu_gated_workspace_bytes(desc.nfactors, desc.patterns, batch, code, desc.bs_last, int(out_last))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=input.device)
+    desc.output, desc.workspace, desc.workspace_bytes = out.data_ptr(), ws.data_ptr(), need
+    with torch.cuda.device(input.device):
+        _lib.check(lib.ksmm_cu_gated_forward(ctypes.byref(desc), _stream_ptr(input.device)))
+    return out
+
+
+class GatedFunction(torch.autograd.Function):
+    """A gated layer as one differentiable operation (``ksmm_cu_gated_forward``, ``ksmm_cu_gated_backward``)."""
+
+    @staticmethod
+    def forward(ctx, input, bias, bs_last, out_last, patterns, activation, *factors):
+        lib = _lib.load()
+        input = _aligned(input)
+        desc, (batch, feats, code) = _gated_desc(input, factors, patterns, bs_last, out_last, bias, activation)
+        sizes = (ctypes.c_size_t * 3)()
+        at = [ctypes.cast(ctypes.byref(sizes, 8 * q), ctypes.POINTER(ctypes.c_size_t)) for q in range(3)]
+        _lib.check(lib.ksmm_cu_gated_train_bytes(desc.nfactors, desc.patterns, batch, code, desc.bs_last, int(bool(out_last)), *at))
+        out = torch.empty((feats, batch) if out_last else (batch, feats), dtype=input.dtype, device=input.device)
+        saved = torch.empty(max(sizes[0], 1), dtype=torch.uint8, device=input.device)
+        ws = torch.empty(max(sizes[1], 1), dtype=torch.uint8, device=input.device)
+        layouts = (ctypes.c_int32 * desc.nfactors)()
+        desc.output, desc.workspace, desc.workspace_bytes = out.data_ptr(), ws.data_ptr(), sizes[1]
+        desc.saved, desc.saved_bytes, desc.layouts = saved.data_ptr(), sizes[0], layouts
+        with torch.cuda.device(input.device):
+            _lib.check(lib.ksmm_cu_gated_forward(ctypes.byref(desc), _stream_ptr(input.device)))
+        ctx.save_for_backward(input, saved, *factors)
+        ctx.gated = (bs_last, out_last, patterns, activation, layouts, int(sizes[2]), bias.shape if bias is not None else None)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        input, saved, *factors = ctx.saved_tensors
+        bs_last, out_last, patterns, activation, layouts, need, bias_shape = ctx.gated
+        desc, _ = _gated_desc(input, factors, patterns, bs_last, out_last, None, activation)
+        grad_output = _aligned(grad_output.contiguous())
+        grad_input = torch.empty_like(input) if ctx.needs_input_grad[0] else None
+        grad_bias = torch.empty(bias_shape, dtype=input.dtype, device=input.device) if ctx.needs_input_grad[1] else None
+        grads = [torch.empty_like(w) if n else None for w, n in zip(factors, ctx.needs_input_grad[6:])]
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=input.device)
+        desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
+        desc.saved, desc.saved_bytes, desc.layouts = saved.data_ptr(), saved.numel(), layouts
+        ptr = [None if t is None else t.data_ptr() for t in (grad_input, grad_bias, *grads)]
+        with torch.cuda.device(input.device):
+            _lib.check(_lib.load().ksmm_cu_gated_backward(
+                ctypes.byref(desc), grad_output.data_ptr(), ptr[0], (ctypes.c_void_p * len(grads))(*ptr[2:]), ptr[1],
+                _stream_ptr(input.device)))
+        return grad_input, grad_bias, None, None, None, None, *grads
+
+
+def gated_chain_train(input, stacked_factors, patterns, bs_last, bias=None, activation="silu", out_bs_last=None):
+    """``gated_chain_forward`` as one autograd node."""
+    out_last = bool(bs_last) if out_bs_last is None else bool(out_bs_last)
+    if _native is not None and activation in _lib.GATES:
+        out = _native.gated_train(input, list(stacked_factors), patterns, bool(bs_last), out_last, bias, _lib.GATES[activation])
+        if out is not None:
+            return out
+    return GatedFunction.apply(input, bias, bool(bs_last), out_last, patterns, activation, *stacked_factors)
+
+
 def _check_grad_output(grad_output, input_like_shape, bs_last, a, b, d):
     if not grad_output.is_cuda or grad_output.dim() != 2:
         raise ValueError("grad_output must be a 2-D CUDA tensor")
