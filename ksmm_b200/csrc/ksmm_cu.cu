@@ -1718,6 +1718,10 @@ struct GatedPlan {
 
 static double gated_last_cost(const int32_t* q, int64_t batch, int dtype, int in_last, int out_last, bool pad) {
   const double out = static_cast<double>(dtype_size(dtype)) * q[0] * q[1] * q[3] * batch;
+  if (tc_gated_fits(q, batch, dtype, in_last, out_last)) {  // the product in the kernel's epilogue
+    const double in = static_cast<double>(dtype_size(dtype)) * q[0] * q[2] * q[3] * batch;
+    return (in_last != out_last ? 1.05 : 1.0) * (2.0 * in + out);
+  }
   const double c = step_cost(q, batch, dtype, in_last, out_last, pad);
   return c < 0 ? c : 2.0 * c + 3.0 * out;  // a pass that reads both halves and writes the product
 }
@@ -1817,6 +1821,8 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   const int32_t* pl = D.patterns + 4 * (n - 1);
   const int64_t n_in = static_cast<int64_t>(p0[0]) * p0[2] * p0[3], n_out = static_cast<int64_t>(pl[0]) * pl[1] * pl[3];
   const int L = plan.out_last[n - 1];
+  // (without `allow` pointers may start anywhere)
+  const bool fuse = allow && !one_layout && tc_gated_fits(pl, batch, D.dtype, plan.in_last[n - 1], L);
   const bool pad_in = ld != batch && D.bs_last && !plan.pre && p0[1] >= 32 && p0[2] >= 16;
   const size_t pre_bytes = plan.pre || pad_in ? align_up(static_cast<size_t>(n_in) * ld * es, 256) : 0;
   const size_t one = gated_buffer_bytes(n, D.patterns, ld, es);
@@ -1831,7 +1837,7 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   char* inter = keep ? kept : at;
   if (!keep) at += one * buffers;
   char* halves = keep ? kept + one * (n - 1) : at;
-  if (!keep) at += halves_bytes;
+  if (!keep && !fuse) at += halves_bytes;
   const size_t used = static_cast<size_t>(at - ws);
   const size_t room = run ? D.workspace_bytes - used : SIZE_MAX;
   size_t scratch = 0;
@@ -1858,7 +1864,14 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
       if (plan.out_last[f]) p.out_ld = ld;
     }
     p.no_alloc = 1;
-    if (run) {
+    if (last && fuse) {
+      p.out = plan.post ? h2 : static_cast<char*>(D.output);
+      if (L && ld != batch) p.out_ld = plan.post ? ld : batch;
+      p.activation = D.activation;
+      p.group_shared_input = f == 0;
+      if (run) st = tc_gated_launch(p, keep ? halves : nullptr, ld, stream);
+      if (st != KSMM_OK) return st;
+    } else if (run) {
       p.scratch = at;
       st = run_pair(p, f == 0, room, stream);
       if (st != KSMM_OK) return st;
@@ -1872,7 +1885,8 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   }
   if (run) {
     void* h = plan.post ? h2 : D.output;
-    if (L) st = launch_gate(halves, ld, h, plan.post ? ld : batch, n_out, batch, D.dtype, D.activation, stream);
+    if (fuse) st = KSMM_OK;
+    else if (L) st = launch_gate(halves, ld, h, plan.post ? ld : batch, n_out, batch, D.dtype, D.activation, stream);
     else st = launch_gate(halves, n_out, h, n_out, batch, n_out, D.dtype, D.activation, stream);
     if (st == KSMM_OK && plan.post)
       st = L ? launch_transpose(h2, D.output, n_out, batch, es, stream, 0, ld)

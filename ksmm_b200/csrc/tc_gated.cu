@@ -1,0 +1,468 @@
+// The last factor of a gated layer (16-bit types): both halves and their product in one tcgen05 kernel.
+//
+//   h[j, n] = act(sum_k Wg[j, k] Xg[k, n] + bg[j]) * (sum_k Wu[j, k] Xu[k, n] + bu[j])
+//
+// per block of the pattern, Wg, Wu the two halves of the stacked factor, Xg, Xu the two halves of the
+// intermediate (or one shared input).  A tile is 128 x 128 of the output with two fp32 accumulators in tensor
+// memory, 128 columns each, double-buffered (all 512 columns): the gate's MMAs, then the up projection's, then
+// one commit.  The epilogue reads both accumulators, adds the biases, forms the product in fp32 and rounds
+// once, so that neither half goes to memory (training stores both as well, rounded, for the backward pass).
+//
+// Work split, ring, descriptors and epilogue staging are those of tc_kernel.cu: a persistent CTA keeps one tile of
+// output features, its weights of both halves resident in shared memory where three k chunks of 64 hold them
+// (c <= 192; 96 KB), and walks (block, batch tile) pairs; longer blocks stream weights through the ring.
+// Against the halves written by a grouped launch and multiplied by a pass over them, the last factor's traffic
+// falls from 2 c + 2 b + 3 b to 2 c + b elements per block and batch entry.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "gated.cuh"
+#include "gated.h"
+#include "tc_epilogue.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
+
+namespace ksmm {
+namespace tc {
+namespace {
+
+constexpr int kNT = 128, kKC = 64, kBox = 64;    // columns of an accumulator, k per chunk, elements per 128-byte row
+constexpr int kChunk = 128 * kKC * 2;            // bytes of one k chunk of either operand
+constexpr int kBarBytes = 256;
+
+struct Params {
+  int a, b, c, d;
+  int64_t batch;
+  int tiles_n, tiles_j;
+  uint32_t rows, row_groups;
+  int nk;
+  uint32_t idesc;
+  const void* bias;
+  int dtype, act;
+  int stacked_input;  // the halves have an input each
+  int* status;
+  void* y;            // batch-last output rows that no tensor map can address (y_direct)
+  int64_t y_ld;
+  int y_direct;
+};
+
+template <bool WRES, int NWC, int SX, int STGN>
+struct Cfg {
+  static constexpr int kStage = kChunk * (WRES ? 1 : 2);
+  static constexpr int kStgWarp = STGN * 32 * 128;
+  static constexpr int kSmem = 2 * NWC * kChunk + SX * kStage + kEpilogueWarps * kStgWarp + kBarBytes + 1024;
+  static_assert(kSmem <= 232448, "shared memory budget");
+  static_assert(8 * (2 * SX + 6) + 8 <= kBarBytes, "barrier area");
+};
+
+// act(g) * u for two values each
+template <int ACT>
+__device__ __forceinline__ void gate_2(float g0, float g1, float u0, float u1, float& h0, float& h1) {
+  if constexpr (ACT == KSMM_ACT_GELU) {
+    uint32_t r0 = __float_as_uint(g0), r1 = __float_as_uint(g1);
+    gelu_16bit_2(r0, r1);
+    h0 = __uint_as_float(r0) * u0;
+    h1 = __uint_as_float(r1) * u1;
+  } else {
+    h0 = gate_value<true>(g0, ACT) * u0;
+    h1 = gate_value<true>(g1, ACT) * u1;
+  }
+}
+
+template <int ACT>
+__device__ __forceinline__ void gate_32(const uint32_t (&g)[32], const uint32_t (&u)[32], int dtype, uint32_t* w) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    float h0, h1;
+    gate_2<ACT>(__uint_as_float(g[e]), __uint_as_float(g[e + 1]), __uint_as_float(u[e]), __uint_as_float(u[e + 1]), h0, h1);
+    w[e / 2] = pack2(h0, h1, dtype);
+  }
+}
+
+// IN_LAST / OUT_LAST: layouts of input and output as in tc_kernel.cu.  KEEP: both halves are stored as well.
+template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, bool KEEP>
+__global__ void __launch_bounds__(kThreads, 1)
+    gated_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                 const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmH, const Params P) {
+  using C = Cfg<WRES, NWC, SX, STGN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t wres0 = (raw + 1023u) & ~1023u;  // 1024-byte alignment for the 128-byte swizzle
+  const uint32_t ring0 = wres0 + 2 * NWC * kChunk;
+  const uint32_t stg0 = ring0 + SX * C::kStage;
+  const uint32_t bar0 = stg0 + kEpilogueWarps * C::kStgWarp;
+  uint8_t* bar_gen = smem_raw + (bar0 - raw);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (SX + s); };
+  const uint32_t wfull_bar = bar0 + 8u * (2 * SX), wempty_bar = wfull_bar + 8u;
+  auto tfull_bar = [&](int q) { return bar0 + 8u * (2 * SX + 2 + q); };
+  auto tempty_bar = [&](int q) { return bar0 + 8u * (2 * SX + 4 + q); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * (2 * SX + 6));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * (2 * SX + 6) + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SX; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(wfull_bar, 1);
+    mbar_init(wempty_bar, 1);
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(tfull_bar(q), 1);
+      mbar_init(tempty_bar(q), kEpilogueWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tmX);
+    prefetch_tensormap(&tmW);
+    prefetch_tensormap(&tmY);
+    if (KEEP) prefetch_tensormap(&tmH);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  const uint32_t d = P.d;
+  const int nk = P.nk;
+  const int tj = static_cast<int>(blockIdx.x % P.tiles_j);
+  const uint32_t rc = blockIdx.x / P.tiles_j;
+  const uint32_t row_begin = static_cast<uint32_t>(static_cast<uint64_t>(rc) * P.rows / P.row_groups);
+  const uint32_t row_end = static_cast<uint32_t>(static_cast<uint64_t>(rc + 1) * P.rows / P.row_groups);
+  const int j0 = tj * 128;
+  const int blocks = P.a * P.d;
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    if (lane == 0) {
+      uint32_t si = 0, sph = 0, wph = 0;
+      int cur_blk = -1;
+      bool ok = true;
+      auto load_w = [&](uint32_t dst, uint32_t bar, int kc, int blk) {
+#pragma unroll
+        for (int wb = 0; wb < 2; ++wb)
+          tma_load_3d(dst + wb * kKC * 128, &tmW, bar, j0 + wb * kBox, kc * kKC, blk);
+      };
+      for (uint32_t row = row_begin; row < row_end && ok; ++row) {
+        const int blk = static_cast<int>(row / P.tiles_n);
+        const int n0 = static_cast<int>(row % P.tiles_n) * 128;
+        const int i = blk / d, l = blk % d;
+        if (WRES && blk != cur_blk) {
+          if (!mbar_wait<64>(wempty_bar, wph ^ 1u, abort_flag, P.status, kGatedWaits + 0)) { ok = false; break; }
+          wph ^= 1u;
+          mbar_expect_tx(wfull_bar, 2 * nk * kChunk);
+          for (int g = 0; g < 2; ++g)
+            for (int kc = 0; kc < nk; ++kc) load_w(wres0 + (g * NWC + kc) * kChunk, wfull_bar, kc, blk + g * blocks);
+          cur_blk = blk;
+        }
+        for (int t = 0; t < 2 * nk; ++t) {
+          const int g = t >= nk ? 1 : 0, kc = t - g * nk;
+          if (!mbar_wait<64>(empty_bar(si), sph ^ 1u, abort_flag, P.status, kGatedWaits + 1)) { ok = false; break; }
+          const uint32_t dst = ring0 + si * C::kStage, bar = full_bar(si);
+          mbar_expect_tx(bar, C::kStage);
+          const int gx = P.stacked_input ? g : 0;
+          if constexpr (IN_LAST) {
+#pragma unroll
+            for (int xb = 0; xb < 2; ++xb)
+              tma_load_4d(dst + xb * kKC * 128, &tmX, bar, n0 + xb * kBox, l, kc * kKC, i + gx * P.a);
+          } else {
+            tma_load_3d(dst, &tmX, bar, kc * kKC, i, n0 + gx * static_cast<int>(P.batch));
+          }
+          if (!WRES) load_w(dst + kChunk, bar, kc, blk + g * blocks);
+          if (++si == SX) { si = 0; sph ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ===================== MMA issuer =====================
+    if (lane == 0) {
+      constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t kLboMN = static_cast<uint32_t>((kKC * 128) >> 4) << 16, kLboK = 1u << 16;
+      constexpr uint32_t kStepMN = (16 * 128) >> 4, kStepK = (16 * 2) >> 4;
+      uint32_t si = 0, sph = 0, wph = 0, ut = 0;
+      int cur_blk = -1;
+      bool ok = true;
+      for (uint32_t row = row_begin; row < row_end && ok; ++row, ++ut) {
+        const int blk = static_cast<int>(row / P.tiles_n);
+        if (WRES && blk != cur_blk) {
+          if (!mbar_wait<0>(wfull_bar, wph, abort_flag, P.status, kGatedWaits + 2)) { ok = false; break; }
+          wph ^= 1u;
+          cur_blk = blk;
+        }
+        const uint32_t buf = ut & 1u, bph = (ut >> 1) & 1u;
+        if (!mbar_wait<0>(tempty_bar(buf), bph ^ 1u, abort_flag, P.status, kGatedWaits + 3)) { ok = false; break; }
+        tc_fence_after();
+        for (int t = 0; t < 2 * nk; ++t) {
+          const int g = t >= nk ? 1 : 0, kc = t - g * nk;
+          if (!mbar_wait<0>(full_bar(si), sph, abort_flag, P.status, kGatedWaits + 4)) { ok = false; break; }
+          const uint32_t dcol = tmem_base + buf * 2 * kNT + g * kNT;
+          const uint32_t xsrc = ring0 + si * C::kStage;
+          const uint32_t wsrc = WRES ? wres0 + (g * NWC + kc) * kChunk : xsrc + kChunk;
+          const uint32_t xlo = (xsrc >> 4) | (IN_LAST ? kLboMN : kLboK), wlo = (wsrc >> 4) | kLboMN;
+#pragma unroll
+          for (int k = 0; k < kKC / 16; ++k) {
+            const uint64_t xdesc = (static_cast<uint64_t>(kDescHi) << 32) | (xlo + k * (IN_LAST ? kStepMN : kStepK));
+            const uint64_t wdesc = (static_cast<uint64_t>(kDescHi) << 32) | (wlo + k * kStepMN);
+            umma<2>(dcol, OUT_LAST ? wdesc : xdesc, OUT_LAST ? xdesc : wdesc, P.idesc, (kc | k) != 0 ? 1u : 0u);
+          }
+          umma_commit(empty_bar(si));
+          if (++si == SX) { si = 0; sph ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit(tfull_bar(buf));
+        if (WRES && (row + 1 == row_end || static_cast<int>((row + 1) / P.tiles_n) != blk)) umma_commit(wempty_bar);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ===================== epilogue =====================
+    // Warp w: TMEM lane quarter w mod 4, columns 64 * ((w - 2) / 4) on; 32 columns of both halves at a time.
+    const int ew = warp - 2, q = warp & 3, box = ew >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t stg_base = stg0 + ew * C::kStgWarp;
+    const int64_t bias_half = static_cast<int64_t>(blocks) * P.b;
+    uint32_t ut = 0, sti = 0;
+    for (uint32_t row = row_begin; row < row_end; ++row, ++ut) {
+      const int blk = static_cast<int>(row / P.tiles_n);
+      const int n0 = static_cast<int>(row % P.tiles_n) * 128;
+      const int i = blk / d, l = blk % d;
+      const uint32_t buf = ut & 1u, bph = (ut >> 1) & 1u;
+      int got = 1;
+      if (lane == 0) got = mbar_wait<128>(tfull_bar(buf), bph, abort_flag, P.status, kGatedWaits + 5) ? 1 : 0;
+      got = __shfl_sync(0xffffffffu, got, 0);
+      if (!got) break;
+      tc_fence_after();
+      const int row_limit = OUT_LAST ? P.b - j0 : static_cast<int>(min(P.batch - n0, static_cast<int64_t>(128)));
+      const int col_limit = OUT_LAST ? static_cast<int>(min(P.batch - n0, static_cast<int64_t>(kNT))) : P.b - j0;
+      const int cols = col_limit - box * 64;
+      if (q * 32 < row_limit && cols > 0) {
+        float bg = 0.f, bu = 0.f;
+        if (OUT_LAST && P.bias != nullptr && q * 32 + lane < row_limit) {
+          const int64_t at = (static_cast<int64_t>(i) * P.b + j0 + q * 32 + lane) * d + l;
+          bg = bias_at(P.bias, at, P.dtype);
+          bu = bias_at(P.bias, at + bias_half, P.dtype);
+        }
+        // the next staging tile, once the store that used it last has read it
+        auto next_tile = [&]() {
+          if (lane == 0) bulk_wait_read<STGN - 1>();
+          __syncwarp();
+          const uint32_t s = stg_base + (STGN > 1 ? sti * 4096u : 0u);
+          if (STGN > 1) sti = (sti + 1 == STGN) ? 0u : sti + 1;
+          return s;
+        };
+        uint32_t stg = next_tile();
+        const bool col_bias = !OUT_LAST && P.bias != nullptr;
+        if (col_bias) {  // the columns' biases pass through the staging tile, which is free here
+          const int64_t e0 = static_cast<int64_t>(i) * P.b + j0 + box * 64;
+          stage_bias_16<1>(P.bias, e0, 2 * lane < cols, P.dtype, stg, lane);
+          stage_bias_16<1>(P.bias, bias_half + e0, 2 * lane < cols, P.dtype, stg + 256, lane);
+          __syncwarp();
+        }
+        uint32_t hw[32], gw[KEEP ? 32 : 1], uw[KEEP ? 32 : 1];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          uint32_t g[32], u[32];
+          const uint32_t t0 = tmem_base + lane_addr + buf * 2 * kNT + box * 64 + s * 32;
+          tmem_ld32(t0, g);
+          tmem_ld32(t0 + kNT, u);
+          tmem_ld_wait();
+          auto gv = [&](int e) -> uint32_t& { return g[e]; };
+          auto uv = [&](int e) -> uint32_t& { return u[e]; };
+          if (col_bias) {
+            scale_and_bias<32>(gv, 1.f, stg + s * 128);
+            scale_and_bias<32>(uv, 1.f, stg + 256 + s * 128);
+          } else if (OUT_LAST) {
+            scale_and_add<32>(gv, 1.f, bg);
+            scale_and_add<32>(uv, 1.f, bu);
+          }
+          if constexpr (KEEP) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              gw[s * 16 + e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
+              uw[s * 16 + e] = pack2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]), P.dtype);
+            }
+          }
+          uint32_t* w = hw + s * 16;
+          switch (P.act) {
+            case KSMM_ACT_SILU: gate_32<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
+            case KSMM_ACT_GELU: gate_32<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
+            case KSMM_ACT_SIGMOID: gate_32<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
+            case KSMM_ACT_RELU: gate_32<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
+            default: gate_32<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+          }
+        }
+        __syncwarp();  // (the biases have been read)
+        auto fill = [&](const uint32_t* w) {
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128 + ((ch ^ (lane & 7)) << 4)), "r"(w[4 * ch]),
+                         "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
+                         : "memory");
+        };
+        auto send = [&](const CUtensorMap* tm, int half) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (OUT_LAST) tma_store_4d(tm, stg, n0 + box * 64, l, j0 + q * 32, i + half * P.a);
+            else tma_store_4d(tm, stg, j0 + box * 64, i, n0 + q * 32, half);
+            bulk_commit();
+          }
+        };
+        if constexpr (KEEP) {
+          fill(gw);
+          send(&tmH, 0);
+          stg = next_tile();
+          fill(uw);
+          send(&tmH, 1);
+          stg = next_tile();
+        }
+        fill(hw);
+        if (OUT_LAST && P.y_direct) {
+          __syncwarp();
+          uint8_t* yrow = static_cast<uint8_t*>(P.y) +
+                          (((static_cast<int64_t>(i) * P.b + j0 + q * 32) * d + l) * P.y_ld + n0 + box * 64) * 2;
+          store_rows<2>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * 2, min(32, row_limit - q * 32), cols, lane);
+        } else {
+          send(&tmY, 0);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty_bar(buf));
+    }
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
+  }
+
+  // ===================== teardown =====================
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // copies that may still be in flight land before the shared memory is handed on
+    __nanosleep(20000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, bool KEEP>
+int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+  using C = Cfg<WRES, NWC, SX, STGN>;
+  auto kern = gated_kernel<IN_LAST, OUT_LAST, WRES, NWC, SX, STGN, KEEP>;
+  static std::atomic<bool> attr_set[64];  // once per device (a repeated set is harmless)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess)
+      return set_error(KSMM_ERR_CUDA, "cannot reserve %d bytes of shared memory: %s", C::kSmem, cudaGetErrorString(e));
+    attr_set[dev] = true;
+  }
+  const uint64_t a = p.a, b = p.b, c = p.c, d = p.d, B = p.batch, GX = p.group_shared_input ? 1 : 2;
+  CUtensorMap tmX, tmW, tmY, tmH;
+  int st;
+  {
+    const uint64_t dims[3] = {b, c, 2 * a * d}, str[3] = {1, b, c * b};
+    const uint32_t box[3] = {kBox, kKC, 1};
+    if ((st = encode_map(&tmW, p.in_dtype, 3, p.w, dims, str, box)) != KSMM_OK) return st;
+  }
+  if (IN_LAST) {
+    const uint64_t L = in_stride(p), dims[4] = {B, d, c, GX * a}, str[4] = {1, L, d * L, c * d * L};
+    const uint32_t box[4] = {kBox, 1, kKC, 1};
+    if ((st = encode_map(&tmX, p.in_dtype, 4, p.in, dims, str, box)) != KSMM_OK) return st;
+  } else {
+    const uint64_t dims[3] = {c, a, GX * B}, str[3] = {1, c, a * c};
+    const uint32_t box[3] = {kKC, 1, 128};
+    if ((st = encode_map(&tmX, p.in_dtype, 3, p.in, dims, str, box)) != KSMM_OK) return st;
+  }
+  Params P = {};
+  P.y = p.out;
+  P.y_ld = out_stride(p);
+  P.y_direct = OUT_LAST && !rows_addressable(p.out, P.y_ld, 2);
+  auto output_map = [&](CUtensorMap* tm, const void* ptr, int64_t ld, uint64_t groups) {
+    if (OUT_LAST) {
+      const uint64_t L = ld, dims[4] = {B, d, b, groups * a}, str[4] = {1, L, d * L, b * d * L};
+      const uint32_t box[4] = {kBox, 1, 32, 1};
+      return encode_map(tm, p.out_dtype, 4, ptr, dims, str, box);
+    }
+    const uint64_t dims[4] = {b, a, B, groups}, str[4] = {1, b, a * b, a * b * B};
+    const uint32_t box[4] = {kBox, 1, 32, 1};
+    return encode_map(tm, p.out_dtype, 4, ptr, dims, str, box);
+  };
+  tmY = tmH = tmX;  // (unused ones)
+  if (!P.y_direct && (st = output_map(&tmY, p.out, P.y_ld, 1)) != KSMM_OK) return st;
+  if (KEEP && (st = output_map(&tmH, halves, halves_ld, 2)) != KSMM_OK) return st;
+  P.a = p.a; P.b = p.b; P.c = p.c; P.d = p.d;
+  P.batch = p.batch;
+  P.nk = (p.c + kKC - 1) / kKC;
+  P.bias = p.bias;
+  P.dtype = p.out_dtype;
+  P.act = p.activation;
+  P.stacked_input = GX == 2;
+  P.status = status_word();
+  if (!P.status) return set_error(KSMM_ERR_CUDA, "cannot resolve the device status word");
+  const uint32_t fmt = p.in_dtype == KSMM_BF16 ? 1u : 0u;
+  const uint32_t a_mn = (OUT_LAST || IN_LAST) ? 1u : 0u, b_mn = (!OUT_LAST || IN_LAST) ? 1u : 0u;
+  P.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) | (static_cast<uint32_t>(kNT >> 3) << 17) |
+            (static_cast<uint32_t>(128 >> 4) << 24);
+  P.tiles_n = static_cast<int>((B + 127) / 128);
+  P.tiles_j = static_cast<int>((b + 127) / 128);
+  const int sms = num_sms();
+  if (sms <= 0) return set_error(KSMM_ERR_NO_DEVICE, "no CUDA device");
+  const int64_t rows = static_cast<int64_t>(P.tiles_n) * p.a * p.d;
+  if (rows <= 0 || rows > 0x7fffffffLL || P.tiles_j > sms)
+    return set_error(KSMM_ERR_UNSUPPORTED, "gated kernel: %lld rows x %d j tiles exceed the work-split limits",
+                     static_cast<long long>(rows), P.tiles_j);
+  P.rows = static_cast<uint32_t>(rows);
+  const int64_t groups = std::min<int64_t>(sms / P.tiles_j, rows);
+  P.row_groups = static_cast<uint32_t>(groups);
+  cudaError_t err = launch_pdl(kern, static_cast<unsigned>(groups * P.tiles_j), kThreads, C::kSmem, stream, tmX, tmW, tmY, tmH, P);
+  count_launch();
+  if (err == cudaSuccess) err = cudaGetLastError();
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "gated kernel launch failed: %s", cudaGetErrorString(err));
+  return KSMM_OK;
+}
+
+template <bool IN_LAST, bool OUT_LAST>
+int launch_layout(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+  if (p.c <= 3 * kKC)
+    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 4, 2, true>(p, halves, halves_ld, stream)
+                  : launch<IN_LAST, OUT_LAST, true, 3, 6, 1, false>(p, halves, halves_ld, stream);
+  return halves ? launch<IN_LAST, OUT_LAST, false, 0, 4, 2, true>(p, halves, halves_ld, stream)
+                : launch<IN_LAST, OUT_LAST, false, 0, 5, 1, false>(p, halves, halves_ld, stream);
+}
+
+}  // namespace
+}  // namespace tc
+
+bool tc_gated_fits(const int32_t* q, int64_t batch, int dtype, int in_last, int out_last) {
+  if (dtype != KSMM_F16 && dtype != KSMM_BF16) return false;
+  // (smaller blocks are bandwidth problems that the register-tiled kernels serve more tightly)
+  if (q[1] < 32 || q[2] < 16 || q[1] % 8 != 0 || q[1] > 16384) return false;
+  if ((!in_last || !out_last) && (q[3] != 1 || q[2] % 8 != 0)) return false;
+  return batch > 0 && batch <= 0x3fffffffLL && static_cast<int64_t>(q[0]) * q[3] <= 0x3fffffffLL;
+}
+
+int tc_gated_launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+  const bool in_last = in_is_last(p), out_last = out_is_last(p);
+  if (in_last) return out_last ? tc::launch_layout<true, true>(p, halves, halves_ld, stream)
+                               : tc::launch_layout<true, false>(p, halves, halves_ld, stream);
+  return out_last ? tc::launch_layout<false, true>(p, halves, halves_ld, stream)
+                  : tc::launch_layout<false, false>(p, halves, halves_ld, stream);
+}
+
+}  // namespace ksmm

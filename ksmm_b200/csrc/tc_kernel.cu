@@ -51,6 +51,7 @@
 
 #include <mutex>
 
+#include "gated.h"
 #include "tc_epilogue.cuh"
 #include "tc_kernel.h"
 #include "tc_host.h"
@@ -470,55 +471,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<IN_LAST, OUT_LAST, ES, OS, NT, K
             }
           }
           if (BS_LAST && P.y_direct) {
-            // Rows that start anywhere: the warp writes the staging tile one output row at a time, 32
-            // words per store instruction.  A 16-bit row that starts on an odd element takes its
-            // words from two neighbouring lanes and its two ends as single elements.  Sixteen rows are
-            // read ahead of their stores; the stores are what it costs: a call of (1,768,192,2) fp16 takes
-            // 12.5 us at 6504 columns, 28 at 6502 and 41 at 6501 (the copy of the input included).
             __syncwarp();
-            const int cols = col_limit - cbi * C::CB;                      // columns of this tile that exist
-            const int rows_here = min(32, row_limit - q * 32);
             uint8_t* yrow = static_cast<uint8_t*>(P.y) +
                             (((static_cast<int64_t>(i + yi0) * P.b + j0 + q * 32) * d + l) * P.y_ld + n0 + cbi * C::CB) * OS;
-            const int64_t ystep = static_cast<int64_t>(d) * P.y_ld * OS;
-#pragma unroll
-            for (int r0 = 0; r0 < 32; r0 += 16) {
-              uint32_t w[16], prev[16];
-#pragma unroll
-              for (int rr = 0; rr < 16; ++rr)
-                asm volatile("ld.shared.b32 %0, [%1];"
-                             : "=r"(w[rr])
-                             : "r"(stg + (r0 + rr) * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + ((lane & 3) << 2)));
-              if constexpr (OS == 2) {
-#pragma unroll
-                for (int rr = 0; rr < 16; ++rr) prev[rr] = __shfl_up_sync(0xffffffffu, w[rr], 1);
-              }
-#pragma unroll
-              for (int rr = 0; rr < 16; ++rr, yrow += ystep) {
-                if (r0 + rr >= rows_here) break;
-                if constexpr (OS == 4) {
-                  if (lane < cols) reinterpret_cast<uint32_t*>(yrow)[lane] = w[rr];
-                } else {
-                  uint16_t* y16 = reinterpret_cast<uint16_t*>(yrow);
-                  if ((reinterpret_cast<uintptr_t>(yrow) & 2) == 0) {
-                    if (2 * lane + 1 < cols) reinterpret_cast<uint32_t*>(yrow)[lane] = w[rr];
-                    else if (2 * lane < cols) y16[2 * lane] = static_cast<uint16_t>(w[rr]);
-                  } else {
-                    // word of elements 2 lane - 1 and 2 lane
-                    if (cols >= 64) {
-                      // a whole box: the words in one store, both ends in another
-                      const uint16_t end = static_cast<uint16_t>(lane == 0 ? w[rr] : w[rr] >> 16);
-                      if (lane != 0) *reinterpret_cast<uint32_t*>(y16 + 2 * lane - 1) = (prev[rr] >> 16) | (w[rr] << 16);
-                      if (lane == 0 || lane == 31) y16[lane == 0 ? 0 : 63] = end;
-                      continue;
-                    }
-                    if (lane == 0) y16[0] = static_cast<uint16_t>(w[rr]);
-                    else if (2 * lane < cols) *reinterpret_cast<uint32_t*>(y16 + 2 * lane - 1) = (prev[rr] >> 16) | (w[rr] << 16);
-                    else if (2 * lane - 1 < cols) y16[2 * lane - 1] = static_cast<uint16_t>(prev[rr] >> 16);
-                  }
-                }
-              }
-            }
+            store_rows<OS>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * OS, min(32, row_limit - q * 32), col_limit - cbi * C::CB,
+                           lane);
             continue;  // (the next tile's writes come after the __syncwarp at the top of the loop)
           }
           fence_proxy_async();
@@ -1029,6 +986,7 @@ static const char* wait_place(int code) {
   if (code < 70) return "the batch-first kernel for groups of eight blocks (tc_bsfirst_g.cu)";
   if (code < 80) return "the kernel for block-ordered inputs (tc_bsfirst_dp.cu)";
   if (code < 90) return "the fp32 weight-gradient kernel (tc_wgrad_f32.cu)";
+  if (code >= kGatedWaits && code < kGatedWaits + 6) return "the gated kernel (tc_gated.cu)";
   return "the wait probe";
 }
 
