@@ -63,7 +63,7 @@ def _load_native():
         from . import ksmm_torch_ext
     except ImportError:
         return None
-    return ksmm_torch_ext if hasattr(ksmm_torch_ext, "gated_train") else None
+    return ksmm_torch_ext if hasattr(ksmm_torch_ext, "residual_norm") else None
 
 
 native = _load_native()

@@ -27,6 +27,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "tc_epilogue.cuh"
 
 namespace ksmm {
 namespace {
@@ -49,92 +50,151 @@ struct Args {
   int64_t rows, per_sample;  // tokens, tokens of a sample
   int64_t samples;
   int chunks;     // chunks of tokens of one sample
-  int C, pre, post, p32, pvec;  // p32: parameters are fp32; pvec: they can be read in pieces of V
+  int C, pre, post, p32;  // p32: parameters are fp32
   float alpha, eps;
 };
 
-template <typename T>
-__device__ __forceinline__ float bits_to_float(uint16_t b) {
-  if constexpr (sizeof(T) == 2 && ElemTraits<T>::kDtype == KSMM_BF16) return __uint_as_float(static_cast<uint32_t>(b) << 16);
-  else return __half2float(__ushort_as_half(b));
+// Arithmetic runs on pairs (the two-wide fp32 instructions: same roundings, half the issue slots), or on single
+// values where rows start anywhere (V = 1).
+__device__ __forceinline__ uint64_t e_fma(uint64_t a, uint64_t b, uint64_t c) { return tc::fma_f2(a, b, c); }
+__device__ __forceinline__ uint64_t e_mul(uint64_t a, uint64_t b) { return tc::mul_f2(a, b); }
+__device__ __forceinline__ uint64_t e_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
+__device__ __forceinline__ float e_fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float e_mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float e_add(float a, float b) { return a + b; }
+__device__ __forceinline__ float e_sum(uint64_t a) {
+  float x, y;
+  tc::unpack_f2(a, x, y);
+  return x + y;
+}
+__device__ __forceinline__ float e_sum(float a) { return a; }
+
+template <int V>
+struct Elem {
+  using E = uint64_t;
+  static constexpr int N = V / 2;
+  static __device__ __forceinline__ E all(float x) { return tc::pack_f2(x, x); }
+};
+template <>
+struct Elem<1> {
+  using E = float;
+  static constexpr int N = 1;
+  static __device__ __forceinline__ E all(float x) { return x; }
+};
 
 // V consecutive elements (16 bytes, or one element)
 template <typename T, int V>
 struct Raw {
-  static_assert(V == 1 || V * sizeof(T) == 16, "a 16-byte piece or an element");
+  static_assert(V * sizeof(T) == 16, "a 16-byte piece");
   uint4 v;
-  T one;
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (V == 1) one = *p;
-    else v = __ldg(reinterpret_cast<const uint4*>(p));
-  }
-  __device__ __forceinline__ void zero() {
-    if constexpr (V == 1) one = ElemTraits<T>::from_float(0.f);
-    else v = make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ float at(int e) const {
-    if constexpr (V == 1) {
-      return ElemTraits<T>::to_float(one);
+  __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint64_t get(int i) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (sizeof(T) == 4) {
+      return tc::pack_f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    } else if constexpr (ElemTraits<T>::kDtype == KSMM_BF16) {
+      return tc::pack_f2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
-      else return bits_to_float<T>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      return tc::pack_f2(f.x, f.y);
     }
   }
 };
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void zero() { v = ElemTraits<T>::from_float(0.f); }
+  __device__ __forceinline__ float get(int) const { return ElemTraits<T>::to_float(v); }
+};
 
 template <typename T, int V>
-__device__ __forceinline__ void store_piece(T* p, const float (&f)[V]) {
+__device__ __forceinline__ void store_piece(T* p, const typename Elem<V>::E (&f)[Elem<V>::N]) {
   if constexpr (V == 1) {
     *p = ElemTraits<T>::from_float(f[0]);
   } else {
-    __align__(16) T t[V];
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[e] = ElemTraits<T>::from_float(f[e]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+    for (int i = 0; i < V / 2; ++i) {
+      float x, y;
+      tc::unpack_f2(f[i], x, y);
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(x);
+        w[2 * i + 1] = __float_as_uint(y);
+      } else if constexpr (ElemTraits<T>::kDtype == KSMM_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-// V parameters from channel c of a sample's row; `other` where there is no such parameter
+// V parameters from channel c of a sample's row; `other` where there is no such parameter.  (Pieces need aligned
+// parameters; the host takes V = 1 otherwise.)
 template <typename T, int V>
-__device__ __forceinline__ void load_param(const Args& A, const Row& r, int64_t sample, int c, float other, float (&f)[V]) {
+__device__ __forceinline__ void load_param(const Args& A, const Row& r, int64_t sample, int c, float other,
+                                           typename Elem<V>::E (&f)[Elem<V>::N]) {
   if (r.p == nullptr) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = other;
+    for (int i = 0; i < Elem<V>::N; ++i) f[i] = Elem<V>::all(other);
     return;
   }
   const int64_t at = sample * r.ld + c;
   if (A.p32) {
     const float* p = static_cast<const float*>(r.p) + at;
-    if (V >= 4 && A.pvec) {
-#pragma unroll
-      for (int e = 0; e + 3 < V; e += 4) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(p + e));
-        f[e] = q.x; f[e + 1] = q.y; f[e + 2] = q.z; f[e + 3] = q.w;
-      }
+    if constexpr (V == 1) {
+      f[0] = __ldg(p);
     } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = __ldg(p + e);
+      for (int i = 0; i < V / 2; i += 2) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(p + 2 * i));
+        f[i] = tc::pack_f2(q.x, q.y);
+        f[i + 1] = tc::pack_f2(q.z, q.w);
+      }
     }
   } else {
-    const T* p = static_cast<const T*>(r.p) + at;
-    if (V > 1 && A.pvec) {
-      Raw<T, V> q;
-      q.load(p);
+    Raw<T, V> q;
+    q.load(static_cast<const T*>(r.p) + at);
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = q.at(e);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = ElemTraits<T>::to_float(p[e]);
-    }
+    for (int i = 0; i < Elem<V>::N; ++i) f[i] = q.get(i);
   }
 }
+
+// one parameter as it lies in memory, and its value: loads first, conversions later, so that a thread's loads overlap
+__device__ __forceinline__ uint32_t raw_param(const Args& A, const Row& r, int64_t sample, int c) {
+  if (r.p == nullptr) return 0;
+  const int64_t at = sample * r.ld + c;
+  return A.p32 ? __ldg(static_cast<const uint32_t*>(r.p) + at) : __ldg(static_cast<const uint16_t*>(r.p) + at);
+}
 template <typename T>
-__device__ __forceinline__ float param_at(const Args& A, const Row& r, int64_t sample, int c, float other) {
-  float f[1];
-  load_param<T, 1>(A, r, sample, c, other, f);
-  return f[0];
+__device__ __forceinline__ float param_value(const Args& A, const Row& r, uint32_t raw, float other) {
+  if (r.p == nullptr) return other;
+  if (A.p32) return __uint_as_float(raw);
+  if constexpr (sizeof(T) == 4) return __uint_as_float(raw);
+  else if constexpr (ElemTraits<T>::kDtype == KSMM_BF16) return __uint_as_float(raw << 16);
+  else return __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
+}
+
+// the parameters of channel c as z and h use them: gate * post_weight, gate * post_bias, weight (1 + scale),
+// bias (1 + scale) + shift
+template <typename T>
+__device__ __forceinline__ float4 combined(const Args& A, int64_t sample, int c) {
+  const uint32_t g = raw_param(A, A.gate, sample, c), pw = raw_param(A, A.post_weight, 0, c), pb = raw_param(A, A.post_bias, 0, c);
+  const uint32_t w = raw_param(A, A.weight, 0, c), b = raw_param(A, A.bias, 0, c);
+  const uint32_t sc = raw_param(A, A.scale, sample, c), sh = raw_param(A, A.shift, sample, c);
+  const float gate = param_value<T>(A, A.gate, g, 1.f), by = 1.f + param_value<T>(A, A.scale, sc, 0.f);
+  return make_float4(gate * param_value<T>(A, A.post_weight, pw, 1.f), gate * param_value<T>(A, A.post_bias, pb, 0.f),
+                     by * param_value<T>(A, A.weight, w, 1.f),
+                     fmaf(by, param_value<T>(A, A.bias, b, 0.f), param_value<T>(A, A.shift, sh, 0.f)));
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -142,21 +202,36 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// the sums of N values over all threads of the block; `red` holds 32 * N floats and is free again after it
+// The sums of N = 1, 2 or 4 values over the block, in a fixed order.  Within a warp the lanes share the values out
+// (6 exchanges for four sums instead of 20), then every thread adds the warps' sums up.  `red` holds
+// 2 * 32 * N floats; calls alternate between its halves (`turn`), so that one barrier per call is enough.
 template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float* red) {
+__device__ __forceinline__ void block_sum(float (&v)[N], float* red, int& turn) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int o = 16;
 #pragma unroll
-  for (int q = 0; q < N; ++q) v[q] = warp_sum(v[q]);
-  if (warps == 1) return;
-  if (lane == 0) {
+  for (int n = N; n > 1; n >>= 1, o >>= 1) {
+    const bool up = (lane & o) != 0;
 #pragma unroll
-    for (int q = 0; q < N; ++q) red[warp * N + q] = v[q];
+    for (int i = 0; i < n / 2; ++i) {
+      const float keep = up ? v[i + n / 2] : v[i], send = up ? v[i] : v[i + n / 2];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
   }
+#pragma unroll
+  for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  // lane bits 4, 3, ... pick the upper half of the values left: value i sits in lanes with those bits
+  float* buf = red + (turn & 1) * 32 * N;
+  ++turn;
+  const int idx = N == 1 ? 0 : (N == 2 ? lane >> 4 : ((lane >> 4) & 1) * 2 + ((lane >> 3) & 1));
+  if ((lane & (32 / N - 1)) == 0) buf[warp * N + idx] = v[0];
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < N; ++q) v[q] = warp_sum(lane < warps ? red[lane * N + q] : 0.f);
-  __syncthreads();
+  for (int q = 0; q < N; ++q) v[q] = 0.f;
+  for (int w = 0; w < warps; ++w) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] += buf[w * N + q];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -164,136 +239,185 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float* red) {
 // ---------------------------------------------------------------------------
 // TPR threads hold a row in registers, K pieces each: a warp per row up to 1024 channels (no barrier),
 // a block per row beyond.
-template <typename T, int V, int K, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_rows_kernel(const Args A) {
-  constexpr int kBlock = TPR < 128 ? 128 : TPR;
-  __shared__ float red[32];
-  const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / TPR) + threadIdx.x / TPR;
-  if (row >= A.rows) return;  // (whole warps, or the whole block)
+// WALK: a block walks a run of one sample's rows (eight at a time, or one) with the combined parameters in shared
+// memory, and loads its next row while it works on this one; else every row reads its parameters.
+constexpr int kWalkBlock = 256;
+
+template <typename T, int V, int K, int TPR, bool WALK>
+__global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), WALK ? 2 : (TPR > 256 ? 1 : (TPR == 256 ? (K <= 2 ? 3 : 2) : 4)))
+    norm_rows_kernel(const Args A) {
+  using L = Elem<V>;
+  using E = typename L::E;
+  constexpr int kBlock = WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR);
+  constexpr int kGroups = kBlock / TPR;
+  __shared__ float red[TPR == 32 ? 1 : 64];
+  extern __shared__ float4 coef[];  // WALK: [4 kinds][V / 4 quarters of a piece][pieces]
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  int turn = 0;
   auto sum = [&](float v) {
     if constexpr (TPR == 32) {
       return warp_sum(v);
     } else {
       float q[1] = {v};
-      block_sum<1>(q, red);
+      block_sum<1>(q, red, turn);
       return q[0];
     }
   };
-  const int64_t sample = A.samples == 1 ? 0 : row / A.per_sample;
-  const T* x = static_cast<const T*>(A.x) + row * A.C;
-  const float inv = 1.f / static_cast<float>(A.C);
-  float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group, end = row + 1;
+  if (row >= A.rows) end = row;  // (whole warps, or the whole block)
+  int64_t sample = 0;
+  const int pieces = A.C / V;
   Raw<T, V> xr[K], yr[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (t + k * TPR) * V;
-    if (c < A.C) xr[k].load(x + c);
-    else xr[k].zero();
-  }
-  if (A.y) {
-    const T* y = static_cast<const T*>(A.y) + row * A.C;
+  auto load = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (t + k * TPR) * V;
-      if (c < A.C) yr[k].load(y + c);
+      const bool ok = r < end && c < A.C;
+      if (ok) xr[k].load(static_cast<const T*>(A.x) + r * A.C + c);
+      else xr[k].zero();
+      if (ok && A.y) yr[k].load(static_cast<const T*>(A.y) + r * A.C + c);
       else yr[k].zero();
     }
-    if (A.post != kNone) {
-      float s = 0.f;
-      if (A.post == kLayer) {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int e = 0; e < V; ++e) s += yr[k].at(e);
-        st.z = sum(s) * inv;
-      }
-      s = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if ((t + k * TPR) * V >= A.C) break;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = yr[k].at(e) - st.z;
-          s = fmaf(d, d, s);
-        }
-      }
-      st.w = rsqrtf(sum(s) * inv + A.eps);
+  };
+  if constexpr (WALK) {
+    sample = blockIdx.x / A.chunks;
+    const int chunk = static_cast<int>(blockIdx.x % A.chunks);
+    row = sample * A.per_sample + A.per_sample * chunk / A.chunks + group;
+    end = sample * A.per_sample + A.per_sample * (chunk + 1) / A.chunks;
+    load(row);
+    float* flat = reinterpret_cast<float*>(coef);
+    for (int c = threadIdx.x; c < A.C; c += kBlock) {
+      const float4 q = combined<T>(A, sample, c);
+      const int at = ((c % V / 4) * pieces + c / V) * 4 + c % 4;
+      flat[at] = q.x;
+      flat[A.C + at] = q.y;
+      flat[2 * A.C + at] = q.z;
+      flat[3 * A.C + at] = q.w;
     }
+    __syncthreads();
+  } else {
+    if (A.samples > 1 && row < end) sample = row / A.per_sample;
+    load(row);
   }
-  float z[K][V];
+  auto coefs = [&](int kind, int c, E (&f)[L::N]) {
+    if constexpr (WALK) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (t + k * TPR) * V;
-    if (A.y == nullptr) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[k][e] = xr[k].at(e);
-    } else if (c < A.C) {
-      float g[V], p[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) p[e] = yr[k].at(e);
-      if (A.post != kNone) {
-        float w[V], b[V];
-        load_param<T, V>(A, A.post_weight, 0, c, 1.f, w);
-        load_param<T, V>(A, A.post_bias, 0, c, 0.f, b);
-#pragma unroll
-        for (int e = 0; e < V; ++e) p[e] = fmaf((p[e] - st.z) * st.w, w[e], b[e]);
+      for (int i = 0; i < L::N; i += 2) {
+        const float4 q = coef[(kind * (V / 4) + i / 2) * pieces + c / V];
+        f[i] = tc::pack_f2(q.x, q.y);
+        f[i + 1] = tc::pack_f2(q.z, q.w);
       }
-      load_param<T, V>(A, A.gate, sample, c, 1.f, g);
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[k][e] = fmaf(A.alpha, xr[k].at(e), g[e] * p[e]);
-      store_piece<T, V>(static_cast<T*>(A.z) + row * A.C + c, z[k]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[k][e] = 0.f;
     }
-  }
-  if (A.pre != kNone) {
-    float s = 0.f;
-    if (A.pre == kLayer) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) s += z[k][e];
-      st.x = sum(s) * inv;
-    }
-    s = 0.f;
+  };
+  // sum of squares of (v - mean), of the channels that exist
+  auto squares = [&](auto&& v, float mean) {
+    E s = L::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if ((t + k * TPR) * V >= A.C) break;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = z[k][e] - st.x;
-        s = fmaf(d, d, s);
+      for (int i = 0; i < L::N; ++i) {
+        const E d = e_add(v(k, i), L::all(-mean));
+        s = e_fma(d, d, s);
       }
     }
-    st.y = rsqrtf(sum(s) * inv + A.eps);
+    return e_sum(s);
+  };
+  auto total = [&](auto&& v) {
+    E s = L::all(0.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) s = e_add(s, v(k, i));
+    return e_sum(s);
+  };
+  const float inv = 1.f / static_cast<float>(A.C);
+  for (; row < end; row += WALK ? kGroups : 1) {
+    float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+    if (A.y && A.post != kNone) {
+      auto y = [&](int k, int i) { return yr[k].get(i); };
+      if (A.post == kLayer) st.z = sum(total(y)) * inv;
+      st.w = rsqrtf(sum(squares(y, st.z)) * inv + A.eps);
+    }
+    E z[K][L::N];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (t + k * TPR) * V;
-      if (c >= A.C) break;
-      float w[V], b[V], o[V];
-      load_param<T, V>(A, A.weight, 0, c, 1.f, w);
-      load_param<T, V>(A, A.bias, 0, c, 0.f, b);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = fmaf((z[k][e] - st.x) * st.y, w[e], b[e]);
-      if (A.scale.p || A.shift.p) {
-        load_param<T, V>(A, A.scale, sample, c, 0.f, w);
-        load_param<T, V>(A, A.shift, sample, c, 0.f, b);
+      for (int i = 0; i < L::N; ++i) z[k][i] = xr[k].get(i);
+      if (A.y == nullptr || c >= A.C) continue;
+      E g[L::N], p[L::N];
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(o[e], 1.f + w[e], b[e]);
+      for (int i = 0; i < L::N; ++i) p[i] = yr[k].get(i);
+      if constexpr (WALK) coefs(0, c, g);
+      else load_param<T, V>(A, A.gate, sample, c, 1.f, g);
+      if (A.post != kNone) {
+        E b[L::N];
+        const E r = L::all(st.w), m = L::all(-st.z);
+        if constexpr (WALK) {
+          coefs(1, c, b);
+#pragma unroll
+          for (int i = 0; i < L::N; ++i) p[i] = e_fma(e_mul(e_add(p[i], m), r), g[i], b[i]);
+        } else {
+          E w[L::N];
+          load_param<T, V>(A, A.post_weight, 0, c, 1.f, w);
+          load_param<T, V>(A, A.post_bias, 0, c, 0.f, b);
+#pragma unroll
+          for (int i = 0; i < L::N; ++i) p[i] = e_mul(g[i], e_fma(e_mul(e_add(p[i], m), r), w[i], b[i]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < L::N; ++i) p[i] = e_mul(g[i], p[i]);
       }
-      store_piece<T, V>(static_cast<T*>(A.h) + row * A.C + c, o);
+      const E al = L::all(A.alpha);
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) z[k][i] = e_fma(al, z[k][i], p[i]);
+      store_piece<T, V>(static_cast<T*>(A.z) + row * A.C + c, z[k]);
     }
+    if constexpr (WALK) load(row + kGroups);
+    if (A.pre != kNone) {
+      auto zv = [&](int k, int i) { return z[k][i]; };
+      if (A.pre == kLayer) st.x = sum(total(zv)) * inv;
+      st.y = rsqrtf(sum(squares(zv, st.x)) * inv + A.eps);
+      const E r = L::all(st.y), m = L::all(-st.x);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (t + k * TPR) * V;
+        if (c >= A.C) break;
+        E w[L::N], b[L::N], o[L::N];
+        if constexpr (WALK) {
+          coefs(2, c, w);
+          coefs(3, c, b);
+        } else {
+          load_param<T, V>(A, A.weight, 0, c, 1.f, w);
+          load_param<T, V>(A, A.bias, 0, c, 0.f, b);
+        }
+#pragma unroll
+        for (int i = 0; i < L::N; ++i) o[i] = e_fma(e_mul(e_add(z[k][i], m), r), w[i], b[i]);
+        if constexpr (!WALK) {
+          if (A.scale.p || A.shift.p) {
+            load_param<T, V>(A, A.scale, sample, c, 0.f, w);
+            load_param<T, V>(A, A.shift, sample, c, 0.f, b);
+#pragma unroll
+            for (int i = 0; i < L::N; ++i) o[i] = e_fma(o[i], e_add(w[i], L::all(1.f)), b[i]);
+          }
+        }
+        store_piece<T, V>(static_cast<T*>(A.h) + row * A.C + c, o);
+      }
+    }
+    if (A.stats && t == 0) A.stats[row] = st;
   }
-  if (A.stats && t == 0) A.stats[row] = st;
 }
 
 // A block walks a run of one sample's rows, R at a time; a thread keeps its channels, so that the sums over
-// rows stay in its registers.
-template <typename T, int V, int K, int R>
-__global__ void __launch_bounds__(512) norm_rows_backward_kernel(const Args A) {
-  __shared__ float red[32 * 2 * R];
+// rows stay in its registers.  The next R rows are loaded while these are worked on.
+template <typename T, int V, int K, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_kernel(const Args A) {
+  using L = Elem<V>;
+  using E = typename L::E;
+  constexpr int N = L::N;
+  __shared__ float red[2 * 32 * 2 * R];
+  int turn = 0;
   const int t = threadIdx.x, nt = blockDim.x;
   const int64_t sample = blockIdx.x / A.chunks;
   const int chunk = static_cast<int>(blockIdx.x % A.chunks);
@@ -304,73 +428,84 @@ __global__ void __launch_bounds__(512) norm_rows_backward_kernel(const Args A) {
   const T* yp = static_cast<const T*>(A.y);
   const T* gzp = static_cast<const T*>(A.gz);
   const T* ghp = static_cast<const T*>(A.gh);
-  float wp[K][V], wq[K][V];  // weight (1 + scale), gate * post_weight
-  float sa[K][V], sb[K][V], sc[K][V], sd[K][V];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (t + k * nt) * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) wp[k][e] = wq[k][e] = sa[k][e] = sb[k][e] = sc[k][e] = sd[k][e] = 0.f;
-    if (c < A.C) {
-      float q[V];
-      load_param<T, V>(A, A.weight, 0, c, 1.f, wp[k]);
-      load_param<T, V>(A, A.scale, sample, c, 0.f, q);
-#pragma unroll
-      for (int e = 0; e < V; ++e) wp[k][e] *= 1.f + q[e];
-      load_param<T, V>(A, A.gate, sample, c, 1.f, wq[k]);
-      if (A.post != kNone) {
-        load_param<T, V>(A, A.post_weight, 0, c, 1.f, q);
-#pragma unroll
-        for (int e = 0; e < V; ++e) wq[k][e] *= q[e];
-      }
-    }
-  }
-  for (int64_t row0 = begin; row0 < end; row0 += R) {
-    Raw<T, V> zr[R][K], yr[R][K], gz[R][K], gh[R][K];
+  struct Rows {
+    Raw<T, V> z[R][K], y[R][K], gz[R][K], gh[R][K];
     float4 st[R];
+  };
+  auto load = [&](Rows& b, int64_t row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = row0 + r;
-      st[r] = row < end ? __ldg(A.stats + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+      b.st[r] = row < end ? __ldg(A.stats + row) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = (t + k * nt) * V;
         const bool live = row < end && c < A.C;
         const int64_t at = row * A.C + c;
-        if (live && ghp) { gh[r][k].load(ghp + at); zr[r][k].load(zp + at); }
-        else { gh[r][k].zero(); zr[r][k].zero(); }
-        if (live && gzp) gz[r][k].load(gzp + at); else gz[r][k].zero();
-        if (live && yp) yr[r][k].load(yp + at); else yr[r][k].zero();
+        if (live && ghp) { b.gh[r][k].load(ghp + at); b.z[r][k].load(zp + at); }
+        else { b.gh[r][k].zero(); b.z[r][k].zero(); }
+        if (live && gzp) b.gz[r][k].load(gzp + at); else b.gz[r][k].zero();
+        if (live && yp) b.y[r][k].load(yp + at); else b.y[r][k].zero();
       }
     }
-    float G[R][K][V];
+  };
+  Rows cur, next;
+  load(cur, begin);
+  E wp[K][N], wq[K][N];  // weight (1 + scale), gate * post_weight
+  E sa[K][N], sb[K][N], sc[K][N], sd[K][N];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (t + k * nt) * V;
+#pragma unroll
+    for (int i = 0; i < N; ++i) wp[k][i] = wq[k][i] = sa[k][i] = sb[k][i] = sc[k][i] = sd[k][i] = L::all(0.f);
+    if (c < A.C) {
+      E q[N];
+      load_param<T, V>(A, A.weight, 0, c, 1.f, wp[k]);
+      load_param<T, V>(A, A.scale, sample, c, 0.f, q);
+#pragma unroll
+      for (int i = 0; i < N; ++i) wp[k][i] = e_fma(wp[k][i], q[i], wp[k][i]);
+      load_param<T, V>(A, A.gate, sample, c, 1.f, wq[k]);
+      if (A.post != kNone) {
+        load_param<T, V>(A, A.post_weight, 0, c, 1.f, q);
+#pragma unroll
+        for (int i = 0; i < N; ++i) wq[k][i] = e_mul(wq[k][i], q[i]);
+      }
+    }
+  }
+  for (int64_t row0 = begin; row0 < end; row0 += R) {
+    load(next, row0 + R);
+    E G[R][K][N];
     if (ghp) {
       float s[2 * R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        s[2 * r] = s[2 * r + 1] = 0.f;
+        const E by = L::all(cur.st[r].y), shift = L::all(-cur.st[r].x * cur.st[r].y);
+        E s1 = L::all(0.f), s2 = L::all(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float g = gh[r][k].at(e), n = (zr[r][k].at(e) - st[r].x) * st[r].y;
-            const float w = g * wp[k][e];
-            s[2 * r] += w;
-            s[2 * r + 1] = fmaf(w, n, s[2 * r + 1]);
-            sa[k][e] += g;
-            sb[k][e] = fmaf(g, n, sb[k][e]);
+          for (int i = 0; i < N; ++i) {
+            const E g = cur.gh[r][k].get(i), n = e_fma(cur.z[r][k].get(i), by, shift);
+            const E w = e_mul(g, wp[k][i]);
+            s1 = e_add(s1, w);
+            s2 = e_fma(w, n, s2);
+            sa[k][i] = e_add(sa[k][i], g);
+            sb[k][i] = e_fma(g, n, sb[k][i]);
           }
+        s[2 * r] = e_sum(s1);
+        s[2 * r + 1] = e_sum(s2);
       }
-      block_sum<2 * R>(s, red);
+      block_sum<2 * R>(s, red, turn);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float m1 = A.pre == kLayer ? s[2 * r] * inv : 0.f, m2 = s[2 * r + 1] * inv;
+        const E m1 = L::all(A.pre == kLayer ? -s[2 * r] * inv : 0.f), m2 = L::all(-s[2 * r + 1] * inv);
+        const E by = L::all(cur.st[r].y), shift = L::all(-cur.st[r].x * cur.st[r].y);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float n = (zr[r][k].at(e) - st[r].x) * st[r].y;
-            G[r][k][e] = fmaf(st[r].y, gh[r][k].at(e) * wp[k][e] - m1 - n * m2, gz[r][k].at(e));
+          for (int i = 0; i < N; ++i) {
+            const E n = e_fma(cur.z[r][k].get(i), by, shift);
+            G[r][k][i] = e_fma(by, e_fma(n, m2, e_fma(cur.gh[r][k].get(i), wp[k][i], m1)), cur.gz[r][k].get(i));
           }
       }
     } else {
@@ -379,7 +514,7 @@ __global__ void __launch_bounds__(512) norm_rows_backward_kernel(const Args A) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int e = 0; e < V; ++e) G[r][k][e] = gz[r][k].at(e);
+          for (int i = 0; i < N; ++i) G[r][k][i] = cur.gz[r][k].get(i);
     }
     if (A.gx) {
 #pragma unroll
@@ -388,9 +523,9 @@ __global__ void __launch_bounds__(512) norm_rows_backward_kernel(const Args A) {
         for (int k = 0; k < K; ++k) {
           const int c = (t + k * nt) * V;
           if (row0 + r >= end || c >= A.C) continue;
-          float o[V];
+          E o[N];
 #pragma unroll
-          for (int e = 0; e < V; ++e) o[e] = A.alpha * G[r][k][e];
+          for (int i = 0; i < N; ++i) o[i] = e_mul(L::all(A.alpha), G[r][k][i]);
           store_piece<T, V>(static_cast<T*>(A.gx) + (row0 + r) * A.C + c, o);
         }
     }
@@ -400,40 +535,45 @@ __global__ void __launch_bounds__(512) norm_rows_backward_kernel(const Args A) {
       for (int r = 0; r < R; ++r) {
         s[2 * r] = s[2 * r + 1] = 0.f;
         if (row0 + r >= end) continue;  // (rows of the next run must not join the sums)
+        const E by = L::all(cur.st[r].w), shift = L::all(-cur.st[r].z * cur.st[r].w);
+        E s1 = L::all(0.f), s2 = L::all(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if ((t + k * nt) * V >= A.C) continue;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float m = (yr[r][k].at(e) - st[r].z) * st[r].w;
-            const float f = G[r][k][e] * wq[k][e];
-            s[2 * r] += f;
-            s[2 * r + 1] = fmaf(f, m, s[2 * r + 1]);
-            sc[k][e] += G[r][k][e];
-            sd[k][e] = fmaf(G[r][k][e], m, sd[k][e]);
+          for (int i = 0; i < N; ++i) {
+            const E m = e_fma(cur.y[r][k].get(i), by, shift), f = e_mul(G[r][k][i], wq[k][i]);
+            s1 = e_add(s1, f);
+            s2 = e_fma(f, m, s2);
+            sc[k][i] = e_add(sc[k][i], G[r][k][i]);
+            sd[k][i] = e_fma(G[r][k][i], m, sd[k][i]);
           }
         }
+        s[2 * r] = e_sum(s1);
+        s[2 * r + 1] = e_sum(s2);
       }
-      if (A.post != kNone) block_sum<2 * R>(s, red);
+      if (A.post != kNone) block_sum<2 * R>(s, red, turn);
       if (A.gy) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float m1 = A.post == kLayer ? s[2 * r] * inv : 0.f, m2 = A.post != kNone ? s[2 * r + 1] * inv : 0.f;
+          const E m1 = L::all(A.post == kLayer ? -s[2 * r] * inv : 0.f), m2 = L::all(A.post != kNone ? -s[2 * r + 1] * inv : 0.f);
+          const E by = L::all(cur.st[r].w), shift = L::all(-cur.st[r].z * cur.st[r].w);
 #pragma unroll
           for (int k = 0; k < K; ++k) {
             const int c = (t + k * nt) * V;
             if (row0 + r >= end || c >= A.C) continue;
-            float o[V];
+            E o[N];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float m = (yr[r][k].at(e) - st[r].z) * st[r].w;
-              o[e] = st[r].w * (G[r][k][e] * wq[k][e] - m1 - m * m2);
+            for (int i = 0; i < N; ++i) {
+              const E m = e_fma(cur.y[r][k].get(i), by, shift);
+              o[i] = e_mul(by, e_fma(m, m2, e_fma(G[r][k][i], wq[k][i], m1)));
             }
             store_piece<T, V>(static_cast<T*>(A.gy) + (row0 + r) * A.C + c, o);
           }
         }
       }
     }
+    cur = next;
   }
   if (A.part) {
     float* part = A.part + static_cast<int64_t>(blockIdx.x) * 4 * A.C;
@@ -442,11 +582,18 @@ __global__ void __launch_bounds__(512) norm_rows_backward_kernel(const Args A) {
       const int c = (t + k * nt) * V;
       if (c >= A.C) break;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        part[c + e] = sa[k][e];
-        part[A.C + c + e] = sb[k][e];
-        part[2 * A.C + c + e] = sc[k][e];
-        part[3 * A.C + c + e] = sd[k][e];
+      for (int i = 0; i < N; ++i) {
+        if constexpr (V == 1) {
+          part[c] = sa[k][0];
+          part[A.C + c] = sb[k][0];
+          part[2 * A.C + c] = sc[k][0];
+          part[3 * A.C + c] = sd[k][0];
+        } else {
+          *reinterpret_cast<uint64_t*>(part + c + 2 * i) = sa[k][i];
+          *reinterpret_cast<uint64_t*>(part + A.C + c + 2 * i) = sb[k][i];
+          *reinterpret_cast<uint64_t*>(part + 2 * A.C + c + 2 * i) = sc[k][i];
+          *reinterpret_cast<uint64_t*>(part + 3 * A.C + c + 2 * i) = sd[k][i];
+        }
       }
     }
   }
@@ -470,9 +617,17 @@ __device__ __forceinline__ float column_sum(float v, float* red) {
   return s;
 }
 
-template <typename T>
+// With CACHE z stays in shared memory (128 bytes per channel, up to 1536 of them); without, it is formed again
+// for each statistic, from x and y in the L2 cache.  Every thread has 16 to 32 loads in flight: the block's latencies
+// are what bounds it (768 x 6501 fp16: 93 us when the loads waited for one another).
+constexpr int kColStep = 16;  // channels that a warp loads at once
+constexpr int kCacheChannels = 1536;
+
+template <typename T, bool CACHE>
 __global__ void __launch_bounds__(kColWarps * 32) norm_columns_kernel(const Args A) {
   __shared__ float red[kColWarps * 32];
+  extern __shared__ float4 coef[];  // combined parameters of the channels, then z
+  float* const zc = reinterpret_cast<float*>(coef + A.C);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t sample = blockIdx.x / A.chunks;
   const int64_t in_sample = static_cast<int64_t>(blockIdx.x % A.chunks) * 32 + lane;
@@ -481,59 +636,68 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_kernel(const Args
   const T* x = static_cast<const T*>(A.x) + tok;
   const T* y = A.y ? static_cast<const T*>(A.y) + tok : nullptr;
   const float inv = 1.f / static_cast<float>(A.C);
-  auto at = [&](const T* p, int c) { return ElemTraits<T>::to_float(p[c * A.rows]); };
+  const int last = A.C - 1;
+  for (int c = threadIdx.x; c < A.C; c += kColWarps * 32) coef[c] = combined<T>(A, sample, c);
+  __syncthreads();
+  // calls f(c, p[c], q[c]) for the warp's channels, loads of a step ahead of their uses
+  auto walk = [&](const T* p, const T* q, auto&& f) {
+    for (int c0 = warp; c0 < A.C; c0 += kColWarps * kColStep) {
+      T a[kColStep], b[kColStep];
+#pragma unroll
+      for (int u = 0; u < kColStep; ++u) {
+        const int64_t at = static_cast<int64_t>(min(c0 + u * kColWarps, last)) * A.rows;
+        a[u] = p[at];
+        if (q) b[u] = q[at];
+      }
+#pragma unroll
+      for (int u = 0; u < kColStep; ++u)
+        if (c0 + u * kColWarps < A.C) f(c0 + u * kColWarps, ElemTraits<T>::to_float(a[u]), q ? ElemTraits<T>::to_float(b[u]) : 0.f);
+    }
+  };
   float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
   if (y && A.post != kNone) {
     float s = 0.f;
     if (A.post == kLayer) {
-#pragma unroll 8
-      for (int c = warp; c < A.C; c += kColWarps) s += at(y, c);
+      walk(y, nullptr, [&](int, float v, float) { s += v; });
       st.z = column_sum(s, red) * inv;
       s = 0.f;
     }
-#pragma unroll 8
-    for (int c = warp; c < A.C; c += kColWarps) {
-      const float d = at(y, c) - st.z;
-      s = fmaf(d, d, s);
-    }
+    walk(y, nullptr, [&](int, float v, float) { s = fmaf(v - st.z, v - st.z, s); });
     st.w = rsqrtf(column_sum(s, red) * inv + A.eps);
   }
-  auto z_at = [&](int c) {
-    const float xv = at(x, c);
+  auto join = [&](int c, float xv, float yv) {
     if (!y) return xv;
-    float p = at(y, c);
-    if (A.post != kNone)
-      p = fmaf((p - st.z) * st.w, param_at<T>(A, A.post_weight, 0, c, 1.f), param_at<T>(A, A.post_bias, 0, c, 0.f));
-    return fmaf(A.alpha, xv, param_at<T>(A, A.gate, sample, c, 1.f) * p);
+    const float4 q = coef[c];
+    return fmaf(A.alpha, xv, A.post != kNone ? fmaf((yv - st.z) * st.w, q.x, q.y) : q.x * yv);
   };
+  // z of every channel, to shared memory and (where there is a y) to memory, and its sum
+  float s = 0.f;
+  walk(x, y, [&](int c, float xv, float yv) {
+    const float z = join(c, xv, yv);
+    s += z;
+    if (CACHE) zc[c * 32 + lane] = z;
+    if (y && live) static_cast<T*>(A.z)[c * A.rows + tok] = ElemTraits<T>::from_float(z);
+  });
   if (A.pre != kNone) {
-    float s = 0.f;
-    if (A.pre == kLayer) {
-#pragma unroll 8
-      for (int c = warp; c < A.C; c += kColWarps) s += z_at(c);
-      st.x = column_sum(s, red) * inv;
-      s = 0.f;
-    }
-#pragma unroll 8
-    for (int c = warp; c < A.C; c += kColWarps) {
-      const float d = z_at(c) - st.x;
-      s = fmaf(d, d, s);
-    }
-    st.y = rsqrtf(column_sum(s, red) * inv + A.eps);
-  }
-  if (live) {
+    auto again = [&](auto&& f) {
+      if constexpr (CACHE) {  // (a thread reads what it has written)
 #pragma unroll 4
-    for (int c = warp; c < A.C; c += kColWarps) {
-      const float z = z_at(c);
-      if (y) static_cast<T*>(A.z)[c * A.rows + tok] = ElemTraits<T>::from_float(z);
-      if (A.pre != kNone) {
-        float o = fmaf((z - st.x) * st.y, param_at<T>(A, A.weight, 0, c, 1.f), param_at<T>(A, A.bias, 0, c, 0.f));
-        o = fmaf(o, 1.f + param_at<T>(A, A.scale, sample, c, 0.f), param_at<T>(A, A.shift, sample, c, 0.f));
-        static_cast<T*>(A.h)[c * A.rows + tok] = ElemTraits<T>::from_float(o);
+        for (int c = warp; c < A.C; c += kColWarps) f(c, zc[c * 32 + lane]);
+      } else {
+        walk(x, y, [&](int c, float xv, float yv) { f(c, join(c, xv, yv)); });
       }
-    }
-    if (A.stats && warp == 0) A.stats[tok] = st;
+    };
+    if (A.pre == kLayer) st.x = column_sum(s, red) * inv;
+    float v = 0.f;
+    again([&](int, float z) { v = fmaf(z - st.x, z - st.x, v); });
+    st.y = rsqrtf(column_sum(v, red) * inv + A.eps);
+    if (live)
+      again([&](int c, float z) {
+        const float4 q = coef[c];
+        static_cast<T*>(A.h)[c * A.rows + tok] = ElemTraits<T>::from_float(fmaf((z - st.x) * st.y, q.z, q.w));
+      });
   }
+  if (live && A.stats && warp == 0) A.stats[tok] = st;
 }
 
 // v[i] of all lanes summed into lane i (31 exchanges for 32 sums)
@@ -554,11 +718,18 @@ __device__ __forceinline__ float reduce_scatter(float (&v)[32]) {
 template <typename T>
 __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(const Args A) {
   __shared__ float red[kColWarps * 32];
+  extern __shared__ float2 pair[];  // per channel: weight (1 + scale), gate * post_weight
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t sample = blockIdx.x / A.chunks;
   const int64_t in_sample = static_cast<int64_t>(blockIdx.x % A.chunks) * 32 + lane;
   const bool live = in_sample < A.per_sample;
   const int64_t tok = sample * A.per_sample + (live ? in_sample : 0);
+  for (int c = threadIdx.x; c < A.C; c += kColWarps * 32)
+  {
+    const float4 q = combined<T>(A, sample, c);
+    pair[c] = make_float2(q.z, q.x);
+  }
+  __syncthreads();
   const T* zp = static_cast<const T*>(A.z_in) + tok;
   const T* yp = A.y ? static_cast<const T*>(A.y) + tok : nullptr;
   const T* gzp = A.gz ? static_cast<const T*>(A.gz) + tok : nullptr;
@@ -572,7 +743,7 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll 8
     for (int c = warp; c < A.C; c += kColWarps) {
-      const float w = (live ? at(ghp, c) : 0.f) * param_at<T>(A, A.weight, 0, c, 1.f) * (1.f + param_at<T>(A, A.scale, sample, c, 0.f));
+      const float w = (live ? at(ghp, c) : 0.f) * pair[c].x;
       s1 += w;
       s2 = fmaf(w, (at(zp, c) - st.x) * st.y, s2);
     }
@@ -582,7 +753,7 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
   auto G_at = [&](int c, float gh, float n) {
     float g = live && gzp ? at(gzp, c) : 0.f;
     if (ghp) {
-      const float w = gh * param_at<T>(A, A.weight, 0, c, 1.f) * (1.f + param_at<T>(A, A.scale, sample, c, 0.f));
+      const float w = gh * pair[c].x;
       g = fmaf(st.y, w - m1 - n * m2, g);
     }
     return live ? g : 0.f;
@@ -592,7 +763,7 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
 #pragma unroll 8
     for (int c = warp; c < A.C; c += kColWarps) {
       const float gh = live && ghp ? at(ghp, c) : 0.f, n = ghp ? (at(zp, c) - st.x) * st.y : 0.f;
-      const float f = G_at(c, gh, n) * param_at<T>(A, A.gate, sample, c, 1.f) * param_at<T>(A, A.post_weight, 0, c, 1.f);
+      const float f = G_at(c, gh, n) * pair[c].y;
       s1 += f;
       s2 = fmaf(f, (at(yp, c) - st.z) * st.w, s2);
     }
@@ -618,8 +789,7 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
         if (yp) {
           m = (at(yp, c) - st.z) * st.w;
           if (live && A.gy) {
-            float f = G * param_at<T>(A, A.gate, sample, c, 1.f);
-            if (A.post != kNone) f = f * param_at<T>(A, A.post_weight, 0, c, 1.f) - q1 - m * q2;
+            const float f = G * pair[c].y - q1 - m * q2;
             static_cast<T*>(A.gy)[c * A.rows + tok] = ElemTraits<T>::from_float(st.w * f);
           }
         }
@@ -652,68 +822,76 @@ __device__ __forceinline__ void put(const Args& A, void* p, int64_t at, float v)
   else static_cast<T*>(p)[at] = ElemTraits<T>::from_float(v);
 }
 
-// 32 channels x 32 slices: first == 1 adds the chunks of sample blockIdx.y and writes the gradients of
+constexpr int kSlices = 8;
+
+// the parameters of one channel and sample
+struct Params {
+  float w, b, pw, pb, sc, ga;
+};
+template <typename T>
+__device__ __forceinline__ Params params_at(const Args& A, int64_t sample, int c) {
+  const uint32_t w = raw_param(A, A.weight, 0, c), b = raw_param(A, A.bias, 0, c), pw = raw_param(A, A.post_weight, 0, c);
+  const uint32_t pb = raw_param(A, A.post_bias, 0, c), sc = raw_param(A, A.scale, sample, c), ga = raw_param(A, A.gate, sample, c);
+  return {param_value<T>(A, A.weight, w, 1.f), param_value<T>(A, A.bias, b, 0.f), param_value<T>(A, A.post_weight, pw, 1.f),
+          param_value<T>(A, A.post_bias, pb, 0.f), 1.f + param_value<T>(A, A.scale, sc, 0.f), param_value<T>(A, A.gate, ga, 1.f)};
+}
+
+// 32 channels x 8 slices: first == 1 adds the chunks of sample blockIdx.y and writes the gradients of
 // per-sample parameters and the sample's sums; first == 0 adds the samples.  With one sample the first does all.
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_param_grads_kernel(const Args A, const Grads g, const float* part, float* sums,
-                                                                int first) {
-  __shared__ float red[32][33];
+__global__ void __launch_bounds__(32 * kSlices) norm_param_grads_kernel(const Args A, const Grads g, const float* part, float* sums,
+                                                                        int first) {
+  __shared__ float red[kSlices][7][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const bool ok = c < A.C;
+  const int at_c = ok ? c : 0;
   const int64_t sample = blockIdx.y;
-  // the totals that the last stage needs: A, B, C, D weighted for weight, bias, post_weight, post_bias, plus plain ones
+  const Params own = params_at<T>(A, sample, at_c);  // (its loads are in flight with those of the sums)
   float t[7] = {};
   if (first) {
-    const float* p = part + sample * A.chunks * 4 * A.C + c;
-    if (ok)
-      for (int q = slice; q < A.chunks; q += 32)
+    const float* p = part + sample * A.chunks * 4 * A.C + at_c;
+#pragma unroll 2
+    for (int q = slice; q < A.chunks; q += kSlices)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) t[s] += p[(static_cast<int64_t>(q) * 4 + s) * A.C];
-  } else if (ok) {
-    const float pw = param_at<T>(A, A.post_weight, 0, c, 1.f), pb = param_at<T>(A, A.post_bias, 0, c, 0.f);
-    const float w = param_at<T>(A, A.weight, 0, c, 1.f), b = param_at<T>(A, A.bias, 0, c, 0.f);
-    for (int64_t s = slice; s < A.samples; s += 32) {
-      const float* p = part + s * 4 * A.C + c;
+      for (int s = 0; s < 4; ++s) t[s] += p[(static_cast<int64_t>(q) * 4 + s) * A.C];
+  } else {
+#pragma unroll 2
+    for (int64_t s = slice; s < A.samples; s += kSlices) {
+      const float* p = part + s * 4 * A.C + at_c;
       const float a = p[0], bb = p[A.C], cc = p[2 * A.C], d = p[3 * A.C];
-      const float sc = 1.f + param_at<T>(A, A.scale, s, c, 0.f), ga = param_at<T>(A, A.gate, s, c, 1.f);
+      const uint32_t sr = raw_param(A, A.scale, s, at_c), gr = raw_param(A, A.gate, s, at_c);
+      const float sc = 1.f + param_value<T>(A, A.scale, sr, 0.f), ga = param_value<T>(A, A.gate, gr, 1.f);
       t[0] = fmaf(sc, bb, t[0]);
       t[1] = fmaf(sc, a, t[1]);
       t[2] = fmaf(ga, d, t[2]);
       t[3] = fmaf(ga, cc, t[3]);
-      t[4] += fmaf(w, bb, b * a);
+      t[4] += fmaf(own.w, bb, own.b * a);
       t[5] += a;
-      t[6] += fmaf(pw, d, pb * cc);
+      t[6] += fmaf(own.pw, d, own.pb * cc);
     }
   }
+#pragma unroll
+  for (int s = 0; s < 7; ++s) red[slice][s][lane] = t[s];
+  __syncthreads();
+  if (slice != 0 || !ok) return;
 #pragma unroll
   for (int s = 0; s < 7; ++s) {
-    if (first && s >= 4) break;
-    red[slice][lane] = t[s];
-    __syncthreads();
-    if (slice == 0) {
-      float v = 0.f;
+    t[s] = 0.f;
 #pragma unroll
-      for (int q = 0; q < 32; ++q) v += red[q][lane];
-      t[s] = v;
-    }
-    __syncthreads();
+    for (int q = 0; q < kSlices; ++q) t[s] += red[q][s][lane];
   }
-  if (slice != 0 || !ok) return;
   if (first) {
-    const float pw = param_at<T>(A, A.post_weight, 0, c, 1.f), pb = param_at<T>(A, A.post_bias, 0, c, 0.f);
-    const float w = param_at<T>(A, A.weight, 0, c, 1.f), b = param_at<T>(A, A.bias, 0, c, 0.f);
-    const float sc = 1.f + param_at<T>(A, A.scale, sample, c, 0.f), ga = param_at<T>(A, A.gate, sample, c, 1.f);
     const bool one = A.samples == 1;
     const int64_t at = sample * A.C + c;
-    if (one || g.scale_rows) put<T>(A, g.scale, at, fmaf(w, t[1], b * t[0]));
+    if (one || g.scale_rows) put<T>(A, g.scale, at, fmaf(own.w, t[1], own.b * t[0]));
     if (one || g.shift_rows) put<T>(A, g.shift, at, t[0]);
-    if (one || g.gate_rows) put<T>(A, g.gate, at, fmaf(pw, t[3], pb * t[2]));
+    if (one || g.gate_rows) put<T>(A, g.gate, at, fmaf(own.pw, t[3], own.pb * t[2]));
     if (one) {
-      put<T>(A, g.weight, c, sc * t[1]);
-      put<T>(A, g.bias, c, sc * t[0]);
-      put<T>(A, g.post_weight, c, ga * t[3]);
-      put<T>(A, g.post_bias, c, ga * t[2]);
+      put<T>(A, g.weight, c, own.sc * t[1]);
+      put<T>(A, g.bias, c, own.sc * t[0]);
+      put<T>(A, g.post_weight, c, own.ga * t[3]);
+      put<T>(A, g.post_bias, c, own.ga * t[2]);
     } else if (sums) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) sums[(sample * 4 + s) * A.C + c] = t[s];
@@ -743,9 +921,13 @@ bool whole_pieces(const void* p, int64_t ld, int es) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * es) % 16 == 0;
 }
 
-// can tokens be read in 16-byte pieces?
+// can tokens and parameters be read in 16-byte pieces?
 bool vector_rows(const ksmm_norm_desc_t& d) {
-  const int es = dtype_size(d.dtype);
+  const int es = dtype_size(d.dtype), ps = dtype_size(d.param_dtype);
+  const struct { const void* p; int64_t ld; } params[7] = {{d.weight, 0}, {d.bias, 0}, {d.post_weight, 0}, {d.post_bias, 0},
+                                                          {d.scale, d.scale_stride}, {d.shift, d.shift_stride}, {d.gate, d.gate_stride}};
+  for (const auto& q : params)
+    if (!whole_pieces(q.p, q.ld, ps)) return false;
   for (const void* p : {d.x, d.y, static_cast<const void*>(d.z), static_cast<const void*>(d.h), d.grad_z, d.grad_h,
                         static_cast<const void*>(d.grad_x), static_cast<const void*>(d.grad_y)})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
@@ -766,40 +948,60 @@ Args args_of(const ksmm_norm_desc_t& d) {
   A.per_sample = d.samples > 0 ? d.rows / d.samples : 0;
   A.C = d.channels; A.pre = d.norm; A.post = d.post_norm;
   A.p32 = d.param_dtype == KSMM_F32;
-  const int ps = dtype_size(d.param_dtype);
-  A.pvec = 1;
-  for (const Row& r : {A.weight, A.bias, A.post_weight, A.post_bias, A.scale, A.shift, A.gate})
-    A.pvec &= whole_pieces(r.p, r.ld, ps) ? 1 : 0;
   A.alpha = d.y ? d.alpha : 1.f;
   A.eps = d.eps;
   return A;
 }
 
+// dynamic shared memory beyond 48 KB needs a word with the driver, once per kernel and device
+int allow_smem(const void* kern, size_t bytes) {
+  if (bytes <= 48 * 1024) return KSMM_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  return e == cudaSuccess ? KSMM_OK
+                          : set_error(KSMM_ERR_CUDA, "cannot reserve %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+}
+
+template <typename T, int V, int K, int TPR, bool WALK = false>
+int go_rows(Args A, cudaStream_t stream) {
+  constexpr int kBlock = WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR);
+  int64_t grid = (A.rows + kBlock / TPR - 1) / (kBlock / TPR);
+  size_t smem = 0;
+  if (WALK) {
+    // two blocks per SM, four rounds at most, six rows per group of threads
+    A.chunks = static_cast<int>(
+        std::max<int64_t>(1, std::min((148 * 8 + A.samples - 1) / A.samples, A.per_sample / (6 * (kBlock / TPR)))));
+    grid = A.samples * A.chunks;
+    smem = static_cast<size_t>(A.C) * 4 * sizeof(float);
+  }
+  if (grid > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many rows");
+  const int st = allow_smem(reinterpret_cast<const void*>(norm_rows_kernel<T, V, K, TPR, WALK>), smem);
+  if (st != KSMM_OK) return st;
+  norm_rows_kernel<T, V, K, TPR, WALK><<<static_cast<unsigned>(grid), kBlock, smem, stream>>>(A);
+  return launched("norm");
+}
+
 template <typename T, int V>
 int launch_rows(const Args& A, cudaStream_t stream) {
   const int pieces = (A.C + V - 1) / V;
-  auto go = [&](auto kern, int tpr) {
-    const int block = tpr < 128 ? 128 : tpr;
-    const int64_t grid = (A.rows + block / tpr - 1) / (block / tpr);
-    if (grid > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many rows");
-    kern<<<static_cast<unsigned>(grid), block, 0, stream>>>(A);
-    return launched("norm");
-  };
   if constexpr (V > 1) {
-    if (pieces <= 32) return go(norm_rows_kernel<T, V, 1, 32>, 32);
-    if (pieces <= 64) return go(norm_rows_kernel<T, V, 2, 32>, 32);
-    if (pieces <= 96) return go(norm_rows_kernel<T, V, 3, 32>, 32);
-    if (pieces <= 128) return go(norm_rows_kernel<T, V, 4, 32>, 32);
-    if (pieces <= 256) return go(norm_rows_kernel<T, V, 2, 128>, 128);
-    if (pieces <= 512) return go(norm_rows_kernel<T, V, 4, 128>, 128);
-    if constexpr (V == 4) {
-      if (pieces > 1024) return go(norm_rows_kernel<T, V, 4, 512>, 512);
+    if (pieces <= 128 && A.per_sample >= 32 && A.rows >= 148 * 16) {
+      if (pieces <= 32) return go_rows<T, V, 1, 32, true>(A, stream);
+      if (pieces <= 64) return go_rows<T, V, 2, 32, true>(A, stream);
+      if (pieces <= 96) return go_rows<T, V, 3, 32, true>(A, stream);
+      return go_rows<T, V, 4, 32, true>(A, stream);
     }
-    return go(norm_rows_kernel<T, V, 4, 256>, 256);
+    if (pieces <= 64) return go_rows<T, V, 2, 32>(A, stream);
+    if (pieces <= 128) return go_rows<T, V, 4, 32>(A, stream);
+    if (pieces <= 256) return go_rows<T, V, 1, 256>(A, stream);
+    if (pieces <= 512) return go_rows<T, V, 4, 128>(A, stream);
+    if constexpr (V == 4) {
+      if (pieces > 1024) return go_rows<T, V, 4, 512>(A, stream);
+    }
+    return go_rows<T, V, 4, 256>(A, stream);
   } else {
-    if (pieces <= 256) return go(norm_rows_kernel<T, 1, 8, 32>, 32);
-    if (pieces <= 1024) return go(norm_rows_kernel<T, 1, 8, 128>, 128);
-    return go(norm_rows_kernel<T, 1, 16, 512>, 512);
+    if (pieces <= 256) return go_rows<T, 1, 8, 32>(A, stream);
+    if (pieces <= 1024) return go_rows<T, 1, 8, 128>(A, stream);
+    return go_rows<T, 1, 8, 1024>(A, stream);
   }
 }
 
@@ -808,22 +1010,23 @@ int launch_rows_backward(const Args& A, cudaStream_t stream) {
   const int pieces = (A.C + V - 1) / V;
   const int64_t grid = A.samples * A.chunks;
   if (grid > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many rows");
-  const int k = (pieces + 511) / 512, per = (pieces + k - 1) / k, block = (per + 31) / 32 * 32;
+  const int k = (pieces + 511) / 512;
   auto go = [&](auto kern, int kk) {
-    const int n = kk == k ? block : ((pieces + kk - 1) / kk + 31) / 32 * 32;
+    const int n = ((pieces + kk - 1) / kk + 31) / 32 * 32;
     kern<<<static_cast<unsigned>(grid), n, 0, stream>>>(A);
     return launched("norm backward");
   };
   if constexpr (V > 1) {
-    if (k <= 1) return go(norm_rows_backward_kernel<T, V, 1, 2>, 1);
+    if (pieces <= 128) return go(norm_rows_backward_kernel<T, V, 1, 2, 128>, 1);
+    if (k <= 1) return go(norm_rows_backward_kernel<T, V, 1, 1, 512>, 1);
     if constexpr (V == 4) {
-      if (k > 2) return go(norm_rows_backward_kernel<T, V, 4, 1>, 4);
+      if (k > 2) return go(norm_rows_backward_kernel<T, V, 4, 1, 512>, 4);
     }
-    return go(norm_rows_backward_kernel<T, V, 2, 1>, 2);
+    return go(norm_rows_backward_kernel<T, V, 2, 1, 512>, 2);
   } else {
-    if (k <= 1) return go(norm_rows_backward_kernel<T, 1, 1, 4>, 1);
-    if (k <= 4) return go(norm_rows_backward_kernel<T, 1, 4, 2>, 4);
-    return go(norm_rows_backward_kernel<T, 1, 16, 1>, 16);
+    if (k <= 1) return go(norm_rows_backward_kernel<T, 1, 1, 2, 512>, 1);
+    if (k <= 4) return go(norm_rows_backward_kernel<T, 1, 4, 1, 512>, 4);
+    return go(norm_rows_backward_kernel<T, 1, 8, 1, 1024>, 8);
   }
 }
 
@@ -835,17 +1038,26 @@ int forward_typed(const ksmm_norm_desc_t& d, cudaStream_t stream) {
   const int64_t chunks = (A.per_sample + 31) / 32;
   if (chunks * A.samples > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many tokens");
   A.chunks = static_cast<int>(chunks);
-  norm_columns_kernel<T><<<static_cast<unsigned>(chunks * A.samples), kColWarps * 32, 0, stream>>>(A);
-  return launched("norm");
+  const bool cache = A.C <= kCacheChannels;
+  const size_t smem = static_cast<size_t>(A.C) * (sizeof(float4) + (cache ? 32 * sizeof(float) : 0));
+  auto go = [&](auto kern) {
+    const int st = allow_smem(reinterpret_cast<const void*>(kern), smem);
+    if (st != KSMM_OK) return st;
+    kern<<<static_cast<unsigned>(chunks * A.samples), kColWarps * 32, smem, stream>>>(A);
+    return launched("norm");
+  };
+  return cache ? go(norm_columns_kernel<T, true>) : go(norm_columns_kernel<T, false>);
 }
 
-// Tokens of a sample are cut into runs, one block each: 32 columns, or enough runs of rows to give every SM
-// several blocks.
+// Tokens of a sample are cut into runs, one block each: 32 columns, or as many runs of rows as blocks fit the SMs
+// at once (168 registers a thread up to 128 threads, 128 beyond).
 int64_t chunks_of(const ksmm_norm_desc_t& d) {
   const int64_t per = d.samples > 0 ? d.rows / d.samples : 0;
   if (per <= 0) return 1;
   if (d.bs_last) return (per + 31) / 32;
-  const int64_t want = std::max<int64_t>(1, 148 * 8 / d.samples);
+  const int64_t pieces = (d.channels * dtype_size(d.dtype) + 15) / 16, threads = std::min<int64_t>(512, (pieces + 31) / 32 * 32);
+  const int64_t blocks = std::min<int64_t>(8, 65536 / ((threads <= 128 ? 168 : 128) * threads));
+  const int64_t want = std::max<int64_t>(1, 148 * blocks / d.samples);
   return std::max<int64_t>(1, std::min(want, (per + 7) / 8));
 }
 
@@ -863,7 +1075,9 @@ int backward_typed(const ksmm_norm_desc_t& d, void* workspace, cudaStream_t stre
   A.part = sums ? static_cast<float*>(workspace) : nullptr;
   int st;
   if (d.bs_last) {
-    norm_columns_backward_kernel<T><<<static_cast<unsigned>(chunks * d.samples), kColWarps * 32, 0, stream>>>(A);
+    const size_t smem = static_cast<size_t>(A.C) * sizeof(float2);
+    if ((st = allow_smem(reinterpret_cast<const void*>(norm_columns_backward_kernel<T>), smem)) != KSMM_OK) return st;
+    norm_columns_backward_kernel<T><<<static_cast<unsigned>(chunks * d.samples), kColWarps * 32, smem, stream>>>(A);
     st = launched("norm backward");
   } else {
     st = vector_rows(d) ? launch_rows_backward<T, 16 / sizeof(T)>(A, stream) : launch_rows_backward<T, 1>(A, stream);
@@ -884,12 +1098,12 @@ int backward_typed(const ksmm_norm_desc_t& d, void* workspace, cudaStream_t stre
     gs.scale = skip(g.scale, g.scale_rows); gs.shift = skip(g.shift, g.shift_rows); gs.gate = skip(g.gate, g.gate_rows);
     auto row = [&](Row r) { return Row{r.p ? static_cast<const char*>(r.p) + s0 * r.ld * ps : nullptr, r.ld}; };
     B.scale = row(A.scale); B.shift = row(A.shift); B.gate = row(A.gate);
-    norm_param_grads_kernel<T><<<dim3(cx, ns), 1024, 0, stream>>>(B, gs, A.part + s0 * chunks * 4 * A.C,
+    norm_param_grads_kernel<T><<<dim3(cx, ns), 32 * kSlices, 0, stream>>>(B, gs, A.part + s0 * chunks * 4 * A.C,
                                                                   totals ? per_sample + s0 * 4 * A.C : nullptr, 1);
     if ((st = launched("norm gradients")) != KSMM_OK) return st;
   }
   if (d.samples > 1 && totals) {
-    norm_param_grads_kernel<T><<<cx, 1024, 0, stream>>>(A, g, per_sample, nullptr, 0);
+    norm_param_grads_kernel<T><<<cx, 32 * kSlices, 0, stream>>>(A, g, per_sample, nullptr, 0);
     st = launched("norm gradients");
   }
   return st;

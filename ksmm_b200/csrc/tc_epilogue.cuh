@@ -138,11 +138,13 @@ __device__ __forceinline__ void activate(Ref&& r, int act) {
 // that starts on an odd element takes its words from two neighbouring lanes and its two ends as single
 // elements.  Sixteen rows are read ahead of their stores; the stores are what it costs: a call of
 // (1,768,192,2) fp16 takes 12.5 us at 6504 columns, 28 at 6502 and 41 at 6501 (the copy of the input included).
-// `rows_here` rows and `cols` columns of the tile exist.
+// `rows_here` rows and `cols` columns of the tile exist; rows from `first` up to `last` (multiples of 16) are stored.
 template <int OS>
-__device__ __forceinline__ void store_rows(uint32_t stg, uint8_t* yrow, int64_t step, int rows_here, int cols, int lane) {
+__device__ __forceinline__ void store_rows(uint32_t stg, uint8_t* yrow, int64_t step, int rows_here, int cols, int lane,
+                                           int first = 0, int last = 32) {
+  yrow += first * step;
 #pragma unroll
-  for (int r0 = 0; r0 < 32; r0 += 16) {
+  for (int r0 = first; r0 < last; r0 += 16) {
     uint32_t w[16], prev[16];
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr)

@@ -30,6 +30,7 @@ namespace {
 constexpr int kNT = 128, kKC = 64, kBox = 64;    // columns of an accumulator, k per chunk, elements per 128-byte row
 constexpr int kChunk = 128 * kKC * 2;            // bytes of one k chunk of either operand
 constexpr int kBarBytes = 256;
+constexpr int kEpi = 16, kBlock = 64 + kEpi * 32; // epilogue warps, threads
 
 struct Params {
   int a, b, c, d;
@@ -50,16 +51,44 @@ struct Params {
 template <bool WRES, int NWC, int SX, int STGN>
 struct Cfg {
   static constexpr int kStage = kChunk * (WRES ? 1 : 2);
-  static constexpr int kStgWarp = STGN * 32 * 128;
-  static constexpr int kSmem = 2 * NWC * kChunk + SX * kStage + kEpilogueWarps * kStgWarp + kBarBytes + 1024;
+  static constexpr int kStgPair = STGN * 32 * 128;  // staging of a pair of warps: 32 rows of 128 bytes
+  static constexpr int kSmem = 2 * NWC * kChunk + SX * kStage + kEpi / 2 * kStgPair + kBarBytes + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
   static_assert(8 * (2 * SX + 6) + 8 <= kBarBytes, "barrier area");
 };
 
-// act(g) * u for two values each
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// act(g) * u for two values each, for results that are rounded to 16 bits.  The special-function unit (16 values
+// a cycle) is what the epilogue has least of, so the two sigmoids of SiLU share one reciprocal:
+// 1 / p = q / (p q) with p = 1 + 2^s.  s stops at 62 so that p q stays finite: below g = -43 the factor stays at
+// 2^-62, and what is off is smaller than 1e-17.  (A NaN in one value of a pair must not reach the other: its s
+// becomes 62, and g itself carries it into its product.)
 template <int ACT>
 __device__ __forceinline__ void gate_2(float g0, float g1, float u0, float u1, float& h0, float& h1) {
-  if constexpr (ACT == KSMM_ACT_GELU) {
+  if constexpr (ACT == KSMM_ACT_SILU) {
+    const uint64_t g = pack_f2(g0, g1);
+    float s0, s1, p0, p1;
+    unpack_f2(mul_f2(g, pack_f2(-1.4426950409f, -1.4426950409f)), s0, s1);
+    const uint64_t p = add_f2(pack_f2(exp2_ftz(fminf(s0, 62.f)), exp2_ftz(fminf(s1, 62.f))), pack_f2(1.f, 1.f));
+    unpack_f2(p, p0, p1);
+    const float r = rcp_ftz(p0 * p1);
+    unpack_f2(mul_f2(mul_f2(mul_f2(pack_f2(p1, p0), pack_f2(r, r)), g), pack_f2(u0, u1)), h0, h1);
+  } else if constexpr (ACT == KSMM_ACT_GELU) {
     uint32_t r0 = __float_as_uint(g0), r1 = __float_as_uint(g1);
     gelu_16bit_2(r0, r1);
     h0 = __uint_as_float(r0) * u0;
@@ -71,7 +100,7 @@ __device__ __forceinline__ void gate_2(float g0, float g1, float u0, float u1, f
 }
 
 template <int ACT>
-__device__ __forceinline__ void gate_32(const uint32_t (&g)[32], const uint32_t (&u)[32], int dtype, uint32_t* w) {
+__device__ __forceinline__ void gate_32(const uint32_t (&g)[32], const uint32_t (&u)[32], int dtype, uint32_t (&w)[16]) {
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
     float h0, h1;
@@ -80,9 +109,44 @@ __device__ __forceinline__ void gate_32(const uint32_t (&g)[32], const uint32_t 
   }
 }
 
+// r[e] += bias[at + e] for the 32 columns of a batch-first tile, of which `exist` exist (a multiple of 8): every lane
+// reads the same 16 bytes, one transaction per eight columns
+__device__ __forceinline__ void add_column_bias(uint32_t (&r)[32], const void* bias, int64_t at, int exist, int dtype) {
+  const uint16_t* bp = static_cast<const uint16_t*>(bias) + at;
+  const bool whole = (reinterpret_cast<uintptr_t>(bp) & 15) == 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (c * 8 >= exist) break;
+    uint32_t w[4];
+    if (whole) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(bp + c * 8));
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = static_cast<uint32_t>(__ldg(bp + c * 8 + 2 * e)) | (static_cast<uint32_t>(__ldg(bp + c * 8 + 2 * e + 1)) << 16);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float b0, b1;
+      if (dtype == KSMM_BF16) {
+        b0 = __uint_as_float(w[e] << 16);
+        b1 = __uint_as_float(w[e] & 0xffff0000u);
+      } else {
+        b0 = __half2float(__ushort_as_half(static_cast<uint16_t>(w[e] & 0xffffu)));
+        b1 = __half2float(__ushort_as_half(static_cast<uint16_t>(w[e] >> 16)));
+      }
+      uint32_t& r0 = r[c * 8 + 2 * e];
+      uint32_t& r1 = r[c * 8 + 2 * e + 1];
+      r0 = __float_as_uint(__uint_as_float(r0) + b0);
+      r1 = __float_as_uint(__uint_as_float(r1) + b1);
+    }
+  }
+}
+
 // IN_LAST / OUT_LAST: layouts of input and output as in tc_kernel.cu.  KEEP: both halves are stored as well.
 template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, bool KEEP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kBlock, 1)
     gated_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmH, const Params P) {
   using C = Cfg<WRES, NWC, SX, STGN>;
@@ -91,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t wres0 = (raw + 1023u) & ~1023u;  // 1024-byte alignment for the 128-byte swizzle
   const uint32_t ring0 = wres0 + 2 * NWC * kChunk;
   const uint32_t stg0 = ring0 + SX * C::kStage;
-  const uint32_t bar0 = stg0 + kEpilogueWarps * C::kStgWarp;
+  const uint32_t bar0 = stg0 + kEpi / 2 * C::kStgPair;
   uint8_t* bar_gen = smem_raw + (bar0 - raw);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (SX + s); };
@@ -111,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(wempty_bar, 1);
     for (int q = 0; q < 2; ++q) {
       mbar_init(tfull_bar(q), 1);
-      mbar_init(tempty_bar(q), kEpilogueWarps);
+      mbar_init(tempty_bar(q), kEpi);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -227,10 +291,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ===================== epilogue =====================
-    // Warp w: TMEM lane quarter w mod 4, columns 64 * ((w - 2) / 4) on; 32 columns of both halves at a time.
+    // Sixteen warps (with eight, two per scheduler, the latencies of this chain of operations were the time of a
+    // tile: 70 us against 46 for 25088 rows of (1,512,192,4)).  Warp w: TMEM lane quarter w mod 4, 32 columns
+    // of both halves; two warps fill one staging tile of 64 columns, and the first of them stores it.
     const int ew = warp - 2, q = warp & 3, box = ew >> 2;
+    const int pair = q + 4 * (box >> 1), side = box & 1;
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t stg_base = stg0 + ew * C::kStgWarp;
+    const uint32_t stg_base = stg0 + pair * C::kStgPair;
     const int64_t bias_half = static_cast<int64_t>(blocks) * P.b;
     uint32_t ut = 0, sti = 0;
     for (uint32_t row = row_begin; row < row_end; ++row, ++ut) {
@@ -239,107 +306,100 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int i = blk / d, l = blk % d;
       const uint32_t buf = ut & 1u, bph = (ut >> 1) & 1u;
       int got = 1;
-      if (lane == 0) got = mbar_wait<128>(tfull_bar(buf), bph, abort_flag, P.status, kGatedWaits + 5) ? 1 : 0;
+      if (lane == 0) got = mbar_wait<64>(tfull_bar(buf), bph, abort_flag, P.status, kGatedWaits + 5) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
       if (!got) break;
       tc_fence_after();
       const int row_limit = OUT_LAST ? P.b - j0 : static_cast<int>(min(P.batch - n0, static_cast<int64_t>(128)));
       const int col_limit = OUT_LAST ? static_cast<int>(min(P.batch - n0, static_cast<int64_t>(kNT))) : P.b - j0;
-      const int cols = col_limit - box * 64;
-      if (q * 32 < row_limit && cols > 0) {
-        float bg = 0.f, bu = 0.f;
-        if (OUT_LAST && P.bias != nullptr && q * 32 + lane < row_limit) {
-          const int64_t at = (static_cast<int64_t>(i) * P.b + j0 + q * 32 + lane) * d + l;
-          bg = bias_at(P.bias, at, P.dtype);
-          bu = bias_at(P.bias, at + bias_half, P.dtype);
-        }
-        // the next staging tile, once the store that used it last has read it
-        auto next_tile = [&]() {
-          if (lane == 0) bulk_wait_read<STGN - 1>();
-          __syncwarp();
-          const uint32_t s = stg_base + (STGN > 1 ? sti * 4096u : 0u);
-          if (STGN > 1) sti = (sti + 1 == STGN) ? 0u : sti + 1;
-          return s;
-        };
-        uint32_t stg = next_tile();
-        const bool col_bias = !OUT_LAST && P.bias != nullptr;
-        if (col_bias) {  // the columns' biases pass through the staging tile, which is free here
-          const int64_t e0 = static_cast<int64_t>(i) * P.b + j0 + box * 64;
-          stage_bias_16<1>(P.bias, e0, 2 * lane < cols, P.dtype, stg, lane);
-          stage_bias_16<1>(P.bias, bias_half + e0, 2 * lane < cols, P.dtype, stg + 256, lane);
-          __syncwarp();
-        }
-        uint32_t hw[32], gw[KEEP ? 32 : 1], uw[KEEP ? 32 : 1];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          uint32_t g[32], u[32];
-          const uint32_t t0 = tmem_base + lane_addr + buf * 2 * kNT + box * 64 + s * 32;
-          tmem_ld32(t0, g);
-          tmem_ld32(t0 + kNT, u);
-          tmem_ld_wait();
-          auto gv = [&](int e) -> uint32_t& { return g[e]; };
-          auto uv = [&](int e) -> uint32_t& { return u[e]; };
-          if (col_bias) {
-            scale_and_bias<32>(gv, 1.f, stg + s * 128);
-            scale_and_bias<32>(uv, 1.f, stg + 256 + s * 128);
-          } else if (OUT_LAST) {
-            scale_and_add<32>(gv, 1.f, bg);
-            scale_and_add<32>(uv, 1.f, bu);
-          }
-          if constexpr (KEEP) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              gw[s * 16 + e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
-              uw[s * 16 + e] = pack2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]), P.dtype);
-            }
-          }
-          uint32_t* w = hw + s * 16;
-          switch (P.act) {
-            case KSMM_ACT_SILU: gate_32<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
-            case KSMM_ACT_GELU: gate_32<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
-            case KSMM_ACT_SIGMOID: gate_32<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
-            case KSMM_ACT_RELU: gate_32<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
-            default: gate_32<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
-          }
-        }
-        __syncwarp();  // (the biases have been read)
-        auto fill = [&](const uint32_t* w) {
-#pragma unroll
-          for (int ch = 0; ch < 8; ++ch)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128 + ((ch ^ (lane & 7)) << 4)), "r"(w[4 * ch]),
-                         "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
-                         : "memory");
-        };
-        auto send = [&](const CUtensorMap* tm, int half) {
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (OUT_LAST) tma_store_4d(tm, stg, n0 + box * 64, l, j0 + q * 32, i + half * P.a);
-            else tma_store_4d(tm, stg, j0 + box * 64, i, n0 + q * 32, half);
-            bulk_commit();
-          }
-        };
-        if constexpr (KEEP) {
-          fill(gw);
-          send(&tmH, 0);
-          stg = next_tile();
-          fill(uw);
-          send(&tmH, 1);
-          stg = next_tile();
-        }
-        fill(hw);
-        if (OUT_LAST && P.y_direct) {
-          __syncwarp();
-          uint8_t* yrow = static_cast<uint8_t*>(P.y) +
-                          (((static_cast<int64_t>(i) * P.b + j0 + q * 32) * d + l) * P.y_ld + n0 + box * 64) * 2;
-          store_rows<2>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * 2, min(32, row_limit - q * 32), cols, lane);
-        } else {
-          send(&tmY, 0);
-        }
+      const int col0 = (box >> 1) * 64;     // of the pair's staging tile
+      const bool active = q * 32 < row_limit && col0 < col_limit;  // (the same for both warps of a pair)
+      uint32_t g[32], u[32];
+      if (active) {
+        const uint32_t t0 = tmem_base + lane_addr + buf * 2 * kNT + box * 32;
+        tmem_ld32(t0, g);
+        tmem_ld32(t0 + kNT, u);
+        tmem_ld_wait();
       }
+      // the accumulators are in registers: hand them back
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(tempty_bar(buf));
+      if (!active) continue;
+      if (P.bias != nullptr) {
+        if constexpr (OUT_LAST) {
+          float bg = 0.f, bu = 0.f;
+          if (q * 32 + lane < row_limit) {
+            const int64_t at = (static_cast<int64_t>(i) * P.b + j0 + q * 32 + lane) * d + l;
+            bg = bias_at(P.bias, at, P.dtype);
+            bu = bias_at(P.bias, at + bias_half, P.dtype);
+          }
+          const uint64_t b2 = pack_f2(bg, bg), c2 = pack_f2(bu, bu);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float y0, y1;
+            unpack_f2(add_f2(pack_f2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), b2), y0, y1);
+            g[e] = __float_as_uint(y0); g[e + 1] = __float_as_uint(y1);
+            unpack_f2(add_f2(pack_f2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), c2), y0, y1);
+            u[e] = __float_as_uint(y0); u[e + 1] = __float_as_uint(y1);
+          }
+        } else {
+          const int64_t at = static_cast<int64_t>(i) * P.b + j0 + box * 32;
+          add_column_bias(g, P.bias, at, col_limit - box * 32, P.dtype);
+          add_column_bias(u, P.bias, bias_half + at, col_limit - box * 32, P.dtype);
+        }
+      }
+      uint32_t stg = 0;
+      // 32 values of each row into the pair's next staging tile, once the store that used it last has read it
+      auto fill = [&](const uint32_t (&w)[16]) {
+        stg = stg_base + (STGN > 1 ? sti * 4096u : 0u);
+        if (STGN > 1) sti = (sti + 1 == STGN) ? 0u : sti + 1;
+        if (side == 0 && lane == 0) bulk_wait_read<STGN - 1>();
+        bar_sync_named(1 + pair, 64);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128 + (((side * 4 + ch) ^ (lane & 7)) << 4)),
+                       "r"(w[4 * ch]), "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
+                       : "memory");
+      };
+      auto send = [&](const CUtensorMap* tm, int half) {
+        fence_proxy_async();
+        bar_sync_named(1 + pair, 64);
+        if (side == 0 && lane == 0) {
+          if constexpr (OUT_LAST) tma_store_4d(tm, stg, n0 + col0, l, j0 + q * 32, i + half * P.a);
+          else tma_store_4d(tm, stg, j0 + col0, i, n0 + q * 32, half);
+          bulk_commit();
+        }
+      };
+      uint32_t w[16];
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
+        fill(w);
+        send(&tmH, 0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]), P.dtype);
+        fill(w);
+        send(&tmH, 1);
+      }
+      switch (P.act) {
+        case KSMM_ACT_SILU: gate_32<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
+        case KSMM_ACT_GELU: gate_32<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
+        case KSMM_ACT_SIGMOID: gate_32<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
+        case KSMM_ACT_RELU: gate_32<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
+        default: gate_32<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+      }
+      fill(w);
+      if (OUT_LAST && P.y_direct) {
+        // each warp of the pair stores half of the tile's rows
+        bar_sync_named(1 + pair, 64);
+        uint8_t* yrow = static_cast<uint8_t*>(P.y) +
+                        (((static_cast<int64_t>(i) * P.b + j0 + q * 32) * d + l) * P.y_ld + n0 + col0) * 2;
+        store_rows<2>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * 2, min(32, row_limit - q * 32), col_limit - col0, lane,
+                      16 * side, 16 * side + 16);
+      } else {
+        send(&tmY, 0);
+      }
     }
     if (lane == 0) bulk_wait<0>();
     __syncwarp();
@@ -430,7 +490,7 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
   P.rows = static_cast<uint32_t>(rows);
   const int64_t groups = std::min<int64_t>(sms / P.tiles_j, rows);
   P.row_groups = static_cast<uint32_t>(groups);
-  cudaError_t err = launch_pdl(kern, static_cast<unsigned>(groups * P.tiles_j), kThreads, C::kSmem, stream, tmX, tmW, tmY, tmH, P);
+  cudaError_t err = launch_pdl(kern, static_cast<unsigned>(groups * P.tiles_j), kBlock, C::kSmem, stream, tmX, tmW, tmY, tmH, P);
   count_launch();
   if (err == cudaSuccess) err = cudaGetLastError();
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "gated kernel launch failed: %s", cudaGetErrorString(err));

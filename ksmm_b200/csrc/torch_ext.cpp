@@ -19,6 +19,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <array>
 #include <string>
 #include <vector>
 
@@ -588,6 +589,205 @@ py::object gated_train(const at::Tensor& x, const std::vector<at::Tensor>& facto
   return py::cast(out);
 }
 
+// ---------------------------------------------------------------------------
+// residual_norm
+// ---------------------------------------------------------------------------
+constexpr int kNormParams = 7;  // weight, bias, post_weight, post_bias, scale, shift, gate
+using NormParams = std::array<c10::optional<at::Tensor>, kNormParams>;
+
+struct NormCall {
+  int64_t norm, post_norm, bs_last;
+  double alpha, eps;
+  int64_t rows = 0, channels = 0, samples = 1;
+  int param_dtype = 0;
+};
+
+// Tensors that the kernel takes as they are; everything else goes through Python, which converts or raises.
+bool norm_fits(const at::Tensor& x, const c10::optional<at::Tensor>& y, const NormParams& p, NormCall* c) {
+  if (!usable(x) || !plain_dtype(x) || x.dim() < 1 || x.dim() > 64 || c->norm < 0 || c->norm > 2 || c->post_norm < 0 || c->post_norm > 2)
+    return false;
+  c->channels = x.size(c->bs_last ? 0 : x.dim() - 1);
+  if (c->channels <= 0 || c->channels > 0x7fffffff || (c->norm == 0 && !y.has_value())) return false;
+  c->rows = x.numel() / c->channels;
+  if (y.has_value()) {
+    if (!usable(*y) || y->sizes() != x.sizes() || y->scalar_type() != x.scalar_type() || y->device() != x.device()) return false;
+  } else if (c->post_norm || p[2].has_value() || p[3].has_value() || p[6].has_value()) {
+    return false;
+  }
+  if ((!c->post_norm && (p[2].has_value() || p[3].has_value())) ||
+      (!c->norm && (p[0].has_value() || p[1].has_value() || p[4].has_value() || p[5].has_value())))
+    return false;
+  at::ScalarType type = x.scalar_type();
+  bool any = false;
+  for (int q = 0; q < kNormParams; ++q) {
+    if (!p[q].has_value()) continue;
+    const at::Tensor& t = *p[q];
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || t.is_conj() || t.device() != x.device()) return false;
+    if (any && t.scalar_type() != type) return false;
+    type = t.scalar_type();
+    any = true;
+    if (t.dim() == 1) {
+      if (t.size(0) != c->channels || (t.stride(0) != 1 && c->channels != 1)) return false;
+      continue;
+    }
+    if (q < 4 || t.dim() != 2 || t.size(1) != c->channels || t.size(0) < 1 || (t.stride(1) != 1 && c->channels != 1)) return false;
+    if (t.size(0) > 1) {
+      if (t.stride(0) <= 0 || (c->samples != 1 && c->samples != t.size(0))) return false;
+      c->samples = t.size(0);
+    }
+  }
+  if (type != x.scalar_type() && type != at::kFloat) return false;
+  if (c->rows % c->samples) return false;
+  c->param_dtype = type == at::kFloat ? KSMM_F32 : dtype_code(x);
+  return true;
+}
+
+int64_t sample_stride(const at::Tensor& t) { return t.dim() == 2 && t.size(0) > 1 ? t.stride(0) : 0; }
+
+ksmm_norm_desc_t norm_desc(const at::Tensor& x, const c10::optional<at::Tensor>& y, const NormParams& p, const NormCall& c) {
+  ksmm_norm_desc_t d = {};
+  d.x = x.data_ptr();
+  d.y = ptr_or_null(y);
+  d.weight = ptr_or_null(p[0]); d.bias = ptr_or_null(p[1]);
+  d.post_weight = ptr_or_null(p[2]); d.post_bias = ptr_or_null(p[3]);
+  d.scale = ptr_or_null(p[4]); d.shift = ptr_or_null(p[5]); d.gate = ptr_or_null(p[6]);
+  if (p[4].has_value()) d.scale_stride = sample_stride(*p[4]);
+  if (p[5].has_value()) d.shift_stride = sample_stride(*p[5]);
+  if (p[6].has_value()) d.gate_stride = sample_stride(*p[6]);
+  d.rows = c.rows; d.samples = c.samples; d.channels = static_cast<int32_t>(c.channels);
+  d.norm = static_cast<int32_t>(c.norm); d.post_norm = static_cast<int32_t>(c.post_norm);
+  d.bs_last = static_cast<int32_t>(c.bs_last);
+  d.dtype = dtype_code(x); d.param_dtype = c.param_dtype;
+  d.alpha = static_cast<float>(c.alpha); d.eps = static_cast<float>(c.eps);
+  return d;
+}
+
+int norm_run(const at::Tensor& x, const c10::optional<at::Tensor>& y, const NormParams& p, const NormCall& c, at::Tensor* z,
+             at::Tensor* h, at::Tensor* stats) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  ksmm_norm_desc_t d = norm_desc(x, y, p, c);
+  const auto o = x.options().requires_grad(false);
+  if (y.has_value()) {
+    *z = at::empty(x.sizes(), o);
+    d.z = z->data_ptr();
+  }
+  if (c.norm) {
+    *h = at::empty(x.sizes(), o);
+    d.h = h->data_ptr();
+  }
+  if (stats) {
+    *stats = at::empty({c.rows * 4}, o.dtype(at::kFloat));
+    d.stats = stats->data_ptr<float>();
+  }
+  return ksmm_cu_norm_forward(&d, stream_of(x));
+}
+
+// residual_norm as one autograd node: ksmm_b200.norm.NormFunction without Python in its backward.
+struct NormNode : torch::autograd::Function<NormNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                const c10::optional<at::Tensor>& y, const c10::optional<at::Tensor>& p0,
+                                                const c10::optional<at::Tensor>& p1, const c10::optional<at::Tensor>& p2,
+                                                const c10::optional<at::Tensor>& p3, const c10::optional<at::Tensor>& p4,
+                                                const c10::optional<at::Tensor>& p5, const c10::optional<at::Tensor>& p6,
+                                                std::vector<int64_t> ints, double alpha, double eps) {
+    const NormParams p{p0, p1, p2, p3, p4, p5, p6};
+    const NormCall c{ints[0], ints[1], ints[2], alpha, eps, ints[3], ints[4], ints[5], static_cast<int>(ints[6])};
+    at::Tensor z, h, stats;
+    raise_status(norm_run(x, y, p, c, &z, &h, &stats));
+    torch::autograd::variable_list keep{y.has_value() ? z : x, y.has_value() ? *y : at::Tensor(), stats};
+    for (const auto& t : p) keep.push_back(t.has_value() ? *t : at::Tensor());
+    ctx->save_for_backward(std::move(keep));
+    ctx->saved_data["ints"] = std::move(ints);
+    ctx->saved_data["alpha"] = alpha;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    torch::autograd::variable_list out;
+    if (z.defined()) out.push_back(z);
+    if (h.defined()) out.push_back(h);
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto kept = ctx->get_saved_variables();
+    const std::vector<int64_t> ints = ctx->saved_data["ints"].toIntVector();
+    const at::Tensor& z = kept[0];
+    const bool has_y = kept[1].defined();
+    c10::optional<at::Tensor> y;
+    if (has_y) y = kept[1];
+    NormParams p;
+    for (int q = 0; q < kNormParams; ++q)
+      if (kept[3 + q].defined()) p[q] = kept[3 + q];
+    const NormCall c{ints[0], ints[1], ints[2], ctx->saved_data["alpha"].toDouble(), ctx->saved_data["eps"].toDouble(),
+                     ints[3], ints[4], ints[5], static_cast<int>(ints[6])};
+    torch::autograd::variable_list r(2 + kNormParams + 3);
+    at::Tensor gz, gh;
+    if (has_y) gz = grads[0];
+    if (c.norm) gh = grads.back();
+    if (!gz.defined() && !gh.defined()) return r;
+    const c10::cuda::CUDAGuard guard(z.device());
+    ksmm_norm_desc_t d = norm_desc(z, y, p, c);
+    d.z = z.data_ptr();
+    d.stats = kept[2].data_ptr<float>();
+    if (gz.defined()) {
+      gz = gz.to(z.scalar_type()).contiguous();
+      d.grad_z = gz.data_ptr();
+    }
+    if (gh.defined()) {
+      gh = gh.to(z.scalar_type()).contiguous();
+      d.grad_h = gh.data_ptr();
+    }
+    // edges of the graph: x, y if there is one, the parameters that there are
+    int edge = 0;
+    auto wanted = [&](bool there, const at::Tensor& like, int at) -> void* {
+      if (!there || !ctx->needs_input_grad(edge++)) return nullptr;
+      r[at] = at::empty(like.sizes(), like.options().requires_grad(false));
+      return r[at].data_ptr();
+    };
+    d.grad_x = wanted(true, z, 0);
+    d.grad_y = wanted(has_y, z, 1);
+    void** const outs[kNormParams] = {&d.grad_weight, &d.grad_bias, &d.grad_post_weight, &d.grad_post_bias,
+                                      &d.grad_scale, &d.grad_shift, &d.grad_gate};
+    for (int q = 0; q < kNormParams; ++q)
+      *outs[q] = wanted(p[q].has_value(), p[q].has_value() ? *p[q] : z, 2 + q);
+    // (sizes of a cut row are dense in a new tensor: the kernel writes rows one after the other)
+    const size_t need = ksmm_cu_norm_backward_workspace_bytes(&d);
+    at::Tensor ws;
+    if (need) ws = new_bytes(need, z);
+    raise_status(ksmm_cu_norm_backward(&d, need ? ws.data_ptr() : nullptr, need, stream_of(z)));
+    return r;
+  }
+};
+
+py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& y, const c10::optional<at::Tensor>& weight,
+                         const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& post_weight,
+                         const c10::optional<at::Tensor>& post_bias, const c10::optional<at::Tensor>& scale,
+                         const c10::optional<at::Tensor>& shift, const c10::optional<at::Tensor>& gate, int64_t norm, int64_t post_norm,
+                         double alpha, double eps, bool bs_last) {
+  const NormParams p{weight, bias, post_weight, post_bias, scale, shift, gate};
+  NormCall c{norm, post_norm, bs_last, alpha, eps};
+  if (!norm_fits(x, y, p, &c)) return py::none();
+  bool learns = x.requires_grad() || (y.has_value() && y->requires_grad());
+  for (const auto& t : p) learns = learns || (t.has_value() && t->requires_grad());
+  if (learns && at::GradMode::is_enabled()) {
+    torch::autograd::variable_list out;
+    {
+      py::gil_scoped_release nogil;
+      out = NormNode::apply(x, y, p[0], p[1], p[2], p[3], p[4], p[5], p[6],
+                            std::vector<int64_t>{norm, post_norm, bs_last, c.rows, c.channels, c.samples, c.param_dtype}, alpha, eps);
+    }
+    return out.size() > 1 ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+  }
+  at::Tensor z, h;
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = norm_run(x, y, p, c, &z, &h, nullptr);
+  }
+  if (st != KSMM_OK) return py::cast(st);
+  if (z.defined() && h.defined()) return py::make_tuple(z, h);
+  return py::cast(z.defined() ? z : h);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -600,6 +800,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("factor_forward", &factor_forward, "One factor in its input's type");
   m.def("fp8_forward", &fp8_forward, "The factors of an fp8 KSLinear");
   m.def("grouped_forward", &grouped_forward, "Several chains on one input");
+  m.def("residual_norm", &residual_norm, "Norms around a block, gate, residual scale and modulation");
   m.def("gated_forward", &gated_forward, "A gated layer without gradients");
   m.def("gated_train", &gated_train, "A trainable gated layer as one autograd node");
 }

@@ -13,7 +13,8 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernel import _stream_ptr, dtype_code
+from ._lib import native as _native
+from .kernel import _result, _stream_ptr, dtype_code
 
 _ROWS = ("weight", "bias", "post_weight", "post_bias")
 _PER_SAMPLE = ("scale", "shift", "gate")
@@ -170,6 +171,12 @@ def residual_norm(x, y=None, *, norm="layer", post_norm=None, weight=None, bias=
 
     Returns ``(z, h)``; ``h`` alone without ``y``; ``z`` alone with ``norm=None``.  Differentiable in every
     tensor.  ``h`` is made from the unrounded ``z``."""
+    if _native is not None and isinstance(x, torch.Tensor) and norm in _lib.NORMS and post_norm in _lib.NORMS:
+        # one call of the extension module; None where it is not for it (a wrong argument, parameters of two types, ...)
+        out = _native.residual_norm(x, y, weight, bias, post_weight, post_bias, scale, shift, gate, _lib.NORMS[norm],
+                                    _lib.NORMS[post_norm], alpha, eps, bool(bs_last))
+        if out is not None:
+            return _result(out)
     params = dict(weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, scale=scale, shift=shift, gate=gate)
     x, y, params, sizes = _plan(x, y, params, norm, post_norm, bs_last)
     kinds = (norm, post_norm, float(alpha), float(eps), bool(bs_last))
