@@ -27,7 +27,10 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "norm.h"
 #include "tc_epilogue.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
 
 namespace ksmm {
 namespace {
@@ -52,6 +55,8 @@ struct Args {
   int chunks;     // chunks of tokens of one sample
   int C, pre, post, p32;  // p32: parameters are fp32
   float alpha, eps;
+  int stages;     // rows in flight per group of threads
+  int* status;    // where a wait that ran out leaves its code
 };
 
 // Arithmetic runs on pairs (the two-wide fp32 instructions: same roundings, half the issue slots), or on single
@@ -184,6 +189,25 @@ __device__ __forceinline__ float param_value(const Args& A, const Row& r, uint32
   else return __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
 }
 
+// V parameters from channel c as they lie in memory, and their values
+template <typename T, int V>
+__device__ __forceinline__ void raw_piece(const Args& A, const Row& r, int64_t sample, int c, uint4 (&q)[2]) {
+  q[0] = q[1] = make_uint4(0, 0, 0, 0);
+  if (r.p == nullptr) return;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.p) + (sample * r.ld + c) * (A.p32 ? 4 : static_cast<int>(sizeof(T))));
+  q[0] = __ldg(p);
+  if (V == 8 && A.p32) q[1] = __ldg(p + 1);
+}
+template <typename T, int V>
+__device__ __forceinline__ float piece_value(const Args& A, const Row& r, const uint4 (&q)[2], int e, float other) {
+  if (r.p == nullptr) return other;
+  const uint32_t w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+  if (sizeof(T) == 4 || A.p32) return __uint_as_float(w[e]);
+  const uint16_t h = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+  if constexpr (ElemTraits<T>::kDtype == KSMM_BF16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
+  else return __half2float(__ushort_as_half(h));
+}
+
 // the parameters of channel c as z and h use them: gate * post_weight, gate * post_bias, weight (1 + scale),
 // bias (1 + scale) + shift
 template <typename T>
@@ -237,70 +261,100 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float* red, int& turn) 
 // ---------------------------------------------------------------------------
 // batch-first: a token is a row
 // ---------------------------------------------------------------------------
-// TPR threads hold a row in registers, K pieces each: a warp per row up to 1024 channels (no barrier),
-// a block per row beyond.
-// WALK: a block walks a run of one sample's rows (eight at a time, or one) with the combined parameters in shared
-// memory, and loads its next row while it works on this one; else every row reads its parameters.
-constexpr int kWalkBlock = 256;
+// A row of `bytes` from memory to shared memory; the barrier expects them
+__device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
+}
 
-template <typename T, int V, int K, int TPR, bool WALK>
-__global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), WALK ? 2 : (TPR > 256 ? 1 : (TPR == 256 ? (K <= 2 ? 3 : 2) : 4)))
+// TPR threads hold a row in registers, K pieces each: a warp per row up to 1024 channels (no barrier), a group of
+// threads beyond.
+// RING: blocks that stay on their SM take equal runs of rows.  Rows come to shared memory by bulk copies, `stages` of
+// them in flight per group of threads, and the parameters of the run's sample are combined there once, for every
+// row of it; a run may pass on to the next sample.  Else every row reads its parameters.
+constexpr int kRingBlock = 256, kRingWide = 512;
+
+// the sum over a group of TPR threads
+template <int TPR>
+__device__ __forceinline__ float group_sum(float v, float* red, int& turn, int group) {
+  v = warp_sum(v);
+  if constexpr (TPR == 32) {
+    return v;
+  } else {
+    constexpr int W = TPR / 32;
+    float* buf = red + (group * 2 + (turn & 1)) * W;
+    ++turn;
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x % TPR / 32] = v;
+    tc::bar_sync_named(1 + group, TPR);
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) v += buf[w];
+    return v;
+  }
+}
+
+template <typename T, int V, int K, int TPR, bool RING>
+__global__ void __launch_bounds__(RING ? (TPR == 32 ? kRingBlock : kRingWide) : (TPR < 128 ? 128 : TPR),
+                                  RING ? (TPR == 32 ? 2 : 1) : (TPR > 256 ? 1 : (TPR == 256 ? (K <= 2 ? 3 : 2) : 4)))
     norm_rows_kernel(const Args A) {
   using L = Elem<V>;
   using E = typename L::E;
-  constexpr int kBlock = WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR);
+  constexpr int kBlock = RING ? (TPR == 32 ? kRingBlock : kRingWide) : (TPR < 128 ? 128 : TPR);
   constexpr int kGroups = kBlock / TPR;
-  __shared__ float red[TPR == 32 ? 1 : 64];
-  extern __shared__ float4 coef[];  // WALK: [4 kinds][V / 4 quarters of a piece][pieces]
+  constexpr int kMaxStages = 12;
+  __shared__ float red[2 * kBlock / 32];
+  __shared__ __align__(8) uint64_t bars[RING ? kGroups * kMaxStages : 1];
+  __shared__ int abort_flag;
+  extern __shared__ __align__(16) float4 coef[];  // RING: [4 kinds][V / 4 quarters of a piece][pieces], then the rows
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   int turn = 0;
-  auto sum = [&](float v) {
-    if constexpr (TPR == 32) {
-      return warp_sum(v);
-    } else {
-      float q[1] = {v};
-      block_sum<1>(q, red, turn);
-      return q[0];
-    }
-  };
+  auto sum = [&](float v) { return group_sum<TPR>(v, red, turn, group); };
   int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group, end = row + 1;
   if (row >= A.rows) end = row;  // (whole warps, or the whole block)
   int64_t sample = 0;
   const int pieces = A.C / V;
   Raw<T, V> xr[K], yr[K];
-  auto load = [&](int64_t r) {
+  // RING: slot s of a group holds a row of x and one of y
+  const uint32_t row_bytes = static_cast<uint32_t>(A.C * sizeof(T));
+  uint8_t* const slots = reinterpret_cast<uint8_t*>(coef + A.C) + static_cast<size_t>(group) * A.stages * 2 * row_bytes;
+  auto bar = [&](int slot) { return tc::smem_u32(&bars[group * kMaxStages + slot]); };
+  auto fetch = [&](int slot, int64_t r) {
+    tc::mbar_expect_tx(bar(slot), A.y ? 2 * row_bytes : row_bytes);
+    const uint32_t dst = tc::smem_u32(slots + static_cast<size_t>(slot) * 2 * row_bytes);
+    bulk_row(dst, static_cast<const T*>(A.x) + r * A.C, row_bytes, bar(slot));
+    if (A.y) bulk_row(dst + row_bytes, static_cast<const T*>(A.y) + r * A.C, row_bytes, bar(slot));
+  };
+  int slot = 0;
+  uint32_t phase = 0;
+  int64_t run_end = end;
+  if constexpr (RING) {
+    if (threadIdx.x == 0) {
+      for (int q = 0; q < kGroups * kMaxStages; ++q) tc::mbar_init(tc::smem_u32(&bars[q]), 1);
+      abort_flag = 0;
+      tc::fence_mbar_init();
+    }
+    __syncthreads();
+    row = A.rows * blockIdx.x / gridDim.x;
+    run_end = A.rows * (blockIdx.x + 1) / gridDim.x;
+    sample = A.samples == 1 ? 0 : row / A.per_sample;
+    row += group;
+    if (t == 0)
+      for (int q = 0; q < A.stages && row + q * kGroups < run_end; ++q) fetch(q, row + q * kGroups);
+  } else {
+    if (A.samples > 1 && row < end) sample = row / A.per_sample;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (t + k * TPR) * V;
-      const bool ok = r < end && c < A.C;
-      if (ok) xr[k].load(static_cast<const T*>(A.x) + r * A.C + c);
+      const bool ok = row < end && c < A.C;
+      if (ok) xr[k].load(static_cast<const T*>(A.x) + row * A.C + c);
       else xr[k].zero();
-      if (ok && A.y) yr[k].load(static_cast<const T*>(A.y) + r * A.C + c);
+      if (ok && A.y) yr[k].load(static_cast<const T*>(A.y) + row * A.C + c);
       else yr[k].zero();
     }
-  };
-  if constexpr (WALK) {
-    sample = blockIdx.x / A.chunks;
-    const int chunk = static_cast<int>(blockIdx.x % A.chunks);
-    row = sample * A.per_sample + A.per_sample * chunk / A.chunks + group;
-    end = sample * A.per_sample + A.per_sample * (chunk + 1) / A.chunks;
-    load(row);
-    float* flat = reinterpret_cast<float*>(coef);
-    for (int c = threadIdx.x; c < A.C; c += kBlock) {
-      const float4 q = combined<T>(A, sample, c);
-      const int at = ((c % V / 4) * pieces + c / V) * 4 + c % 4;
-      flat[at] = q.x;
-      flat[A.C + at] = q.y;
-      flat[2 * A.C + at] = q.z;
-      flat[3 * A.C + at] = q.w;
-    }
-    __syncthreads();
-  } else {
-    if (A.samples > 1 && row < end) sample = row / A.per_sample;
-    load(row);
   }
   auto coefs = [&](int kind, int c, E (&f)[L::N]) {
-    if constexpr (WALK) {
+    if constexpr (RING) {
 #pragma unroll
       for (int i = 0; i < L::N; i += 2) {
         const float4 q = coef[(kind * (V / 4) + i / 2) * pieces + c / V];
@@ -332,7 +386,62 @@ __global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), W
     return e_sum(s);
   };
   const float inv = 1.f / static_cast<float>(A.C);
-  for (; row < end; row += WALK ? kGroups : 1) {
+  // one round per sample of the block's run (RING), else one row
+  for (bool more = true; more;) {
+  more = false;
+  if constexpr (RING) {
+    end = min((sample + 1) * A.per_sample, run_end);
+    more = end < run_end;
+    float* flat = reinterpret_cast<float*>(coef);
+    for (int pc = threadIdx.x; pc < pieces; pc += kBlock) {
+      // every load before the first use
+      uint4 g[2], pw[2], pb[2], w[2], b[2], sc[2], sh[2];
+      const int c = pc * V;
+      raw_piece<T, V>(A, A.gate, sample, c, g);
+      raw_piece<T, V>(A, A.post_weight, 0, c, pw);
+      raw_piece<T, V>(A, A.post_bias, 0, c, pb);
+      raw_piece<T, V>(A, A.weight, 0, c, w);
+      raw_piece<T, V>(A, A.bias, 0, c, b);
+      raw_piece<T, V>(A, A.scale, sample, c, sc);
+      raw_piece<T, V>(A, A.shift, sample, c, sh);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float gate = piece_value<T, V>(A, A.gate, g, e, 1.f), by = 1.f + piece_value<T, V>(A, A.scale, sc, e, 0.f);
+        float* at = flat + ((e / 4) * pieces + pc) * 4 + e % 4;
+        at[0] = gate * piece_value<T, V>(A, A.post_weight, pw, e, 1.f);
+        at[A.C] = gate * piece_value<T, V>(A, A.post_bias, pb, e, 0.f);
+        at[2 * A.C] = by * piece_value<T, V>(A, A.weight, w, e, 1.f);
+        at[3 * A.C] = fmaf(by, piece_value<T, V>(A, A.bias, b, e, 0.f), piece_value<T, V>(A, A.shift, sh, e, 0.f));
+      }
+    }
+    __syncthreads();
+  }
+  for (; row < end; row += kGroups) {
+    if constexpr (RING) {
+      // (a wait that ran out leaves its code; the rows of this block are then not to be used)
+      tc::mbar_wait<0>(bar(slot), phase, &abort_flag, A.status, kNormWaits);
+      const T* src = reinterpret_cast<const T*>(slots + static_cast<size_t>(slot) * 2 * row_bytes);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (t + k * TPR) * V;
+        if (c < A.C) {
+          xr[k].v = *reinterpret_cast<const uint4*>(src + c);
+          if (A.y) yr[k].v = *reinterpret_cast<const uint4*>(src + A.C + c);
+          else yr[k].zero();
+        } else {
+          xr[k].zero();
+          yr[k].zero();
+        }
+      }
+      // the row is in registers: its place takes the next one
+      if constexpr (TPR == 32) __syncwarp();
+      else tc::bar_sync_named(1 + group, TPR);
+      if (t == 0 && row + static_cast<int64_t>(A.stages) * kGroups < run_end) fetch(slot, row + static_cast<int64_t>(A.stages) * kGroups);
+      if (++slot == A.stages) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    }
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (A.y && A.post != kNone) {
       auto y = [&](int k, int i) { return yr[k].get(i); };
@@ -349,12 +458,12 @@ __global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), W
       E g[L::N], p[L::N];
 #pragma unroll
       for (int i = 0; i < L::N; ++i) p[i] = yr[k].get(i);
-      if constexpr (WALK) coefs(0, c, g);
+      if constexpr (RING) coefs(0, c, g);
       else load_param<T, V>(A, A.gate, sample, c, 1.f, g);
       if (A.post != kNone) {
         E b[L::N];
         const E r = L::all(st.w), m = L::all(-st.z);
-        if constexpr (WALK) {
+        if constexpr (RING) {
           coefs(1, c, b);
 #pragma unroll
           for (int i = 0; i < L::N; ++i) p[i] = e_fma(e_mul(e_add(p[i], m), r), g[i], b[i]);
@@ -374,7 +483,6 @@ __global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), W
       for (int i = 0; i < L::N; ++i) z[k][i] = e_fma(al, z[k][i], p[i]);
       store_piece<T, V>(static_cast<T*>(A.z) + row * A.C + c, z[k]);
     }
-    if constexpr (WALK) load(row + kGroups);
     if (A.pre != kNone) {
       auto zv = [&](int k, int i) { return z[k][i]; };
       if (A.pre == kLayer) st.x = sum(total(zv)) * inv;
@@ -385,7 +493,7 @@ __global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), W
         const int c = (t + k * TPR) * V;
         if (c >= A.C) break;
         E w[L::N], b[L::N], o[L::N];
-        if constexpr (WALK) {
+        if constexpr (RING) {
           coefs(2, c, w);
           coefs(3, c, b);
         } else {
@@ -394,7 +502,7 @@ __global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), W
         }
 #pragma unroll
         for (int i = 0; i < L::N; ++i) o[i] = e_fma(e_mul(e_add(z[k][i], m), r), w[i], b[i]);
-        if constexpr (!WALK) {
+        if constexpr (!RING) {
           if (A.scale.p || A.shift.p) {
             load_param<T, V>(A, A.scale, sample, c, 0.f, w);
             load_param<T, V>(A, A.shift, sample, c, 0.f, b);
@@ -407,6 +515,12 @@ __global__ void __launch_bounds__(WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR), W
     }
     if (A.stats && t == 0) A.stats[row] = st;
   }
+  if (RING && more) {
+    __syncthreads();  // (the parameters have been read)
+    ++sample;
+  }
+  }
+  if (RING && abort_flag) __nanosleep(20000);  // rows in flight land before the shared memory is handed on
 }
 
 // A block walks a run of one sample's rows, R at a time; a thread keeps its channels, so that the sums over
@@ -953,7 +1067,7 @@ Args args_of(const ksmm_norm_desc_t& d) {
   return A;
 }
 
-// dynamic shared memory beyond 48 KB needs a word with the driver, once per kernel and device
+// dynamic shared memory beyond 48 KB needs a word with the driver
 int allow_smem(const void* kern, size_t bytes) {
   if (bytes <= 48 * 1024) return KSMM_OK;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
@@ -961,22 +1075,24 @@ int allow_smem(const void* kern, size_t bytes) {
                           : set_error(KSMM_ERR_CUDA, "cannot reserve %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
 }
 
-template <typename T, int V, int K, int TPR, bool WALK = false>
+template <typename T, int V, int K, int TPR, bool RING = false>
 int go_rows(Args A, cudaStream_t stream) {
-  constexpr int kBlock = WALK ? kWalkBlock : (TPR < 128 ? 128 : TPR);
+  constexpr int kBlock = RING ? (TPR == 32 ? kRingBlock : kRingWide) : (TPR < 128 ? 128 : TPR);
   int64_t grid = (A.rows + kBlock / TPR - 1) / (kBlock / TPR);
   size_t smem = 0;
-  if (WALK) {
-    // two blocks per SM, four rounds at most, six rows per group of threads
-    A.chunks = static_cast<int>(
-        std::max<int64_t>(1, std::min((148 * 8 + A.samples - 1) / A.samples, A.per_sample / (6 * (kBlock / TPR)))));
-    grid = A.samples * A.chunks;
-    smem = static_cast<size_t>(A.C) * 4 * sizeof(float);
+  if (RING) {
+    A.status = tc::status_word();
+    if (!A.status) return set_error(KSMM_ERR_CUDA, "cannot resolve the device status word");
+    grid = tc::num_sms() * (TPR == 32 ? 2 : 1);
+    const size_t coefs = static_cast<size_t>(A.C) * sizeof(float4), slot = static_cast<size_t>(A.C) * 2 * sizeof(T) * (kBlock / TPR);
+    const size_t room = TPR == 32 ? 110 * 1024 : 224 * 1024;
+    A.stages = static_cast<int>(std::min<size_t>(TPR == 32 ? 6 : 12, (room - coefs) / slot));
+    smem = coefs + A.stages * slot;
   }
   if (grid > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many rows");
-  const int st = allow_smem(reinterpret_cast<const void*>(norm_rows_kernel<T, V, K, TPR, WALK>), smem);
+  const int st = allow_smem(reinterpret_cast<const void*>(norm_rows_kernel<T, V, K, TPR, RING>), smem);
   if (st != KSMM_OK) return st;
-  norm_rows_kernel<T, V, K, TPR, WALK><<<static_cast<unsigned>(grid), kBlock, smem, stream>>>(A);
+  norm_rows_kernel<T, V, K, TPR, RING><<<static_cast<unsigned>(grid), kBlock, smem, stream>>>(A);
   return launched("norm");
 }
 
@@ -990,6 +1106,9 @@ int launch_rows(const Args& A, cudaStream_t stream) {
       if (pieces <= 96) return go_rows<T, V, 3, 32, true>(A, stream);
       return go_rows<T, V, 4, 32, true>(A, stream);
     }
+    // (beyond 5461 channels of 16 bits the parameters and two rows for each group do not fit)
+    if (pieces > 128 && pieces <= 512 && A.per_sample >= 24 && A.rows >= 148 * 8)
+      return pieces <= 256 ? go_rows<T, V, 2, 128, true>(A, stream) : go_rows<T, V, 4, 128, true>(A, stream);
     if (pieces <= 64) return go_rows<T, V, 2, 32>(A, stream);
     if (pieces <= 128) return go_rows<T, V, 4, 32>(A, stream);
     if (pieces <= 256) return go_rows<T, V, 1, 256>(A, stream);

@@ -52,6 +52,7 @@
 #include <mutex>
 
 #include "gated.h"
+#include "norm.h"
 #include "tc_epilogue.cuh"
 #include "tc_kernel.h"
 #include "tc_host.h"
@@ -987,6 +988,7 @@ static const char* wait_place(int code) {
   if (code < 80) return "the kernel for block-ordered inputs (tc_bsfirst_dp.cu)";
   if (code < 90) return "the fp32 weight-gradient kernel (tc_wgrad_f32.cu)";
   if (code >= kGatedWaits && code < kGatedWaits + 6) return "the gated kernel (tc_gated.cu)";
+  if (code >= kNormWaits && code < kNormWaits + 3) return "the norm kernel (norm.cu)";
   return "the wait probe";
 }
 

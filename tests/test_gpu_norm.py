@@ -178,3 +178,21 @@ def test_fp32_parameters_of_16_bit_tensors(bs_last):
 def test_more_dimensions():
     check(torch.float16, (4, 3, 5, 64), keys=EVERY, samples=4, post_norm="rms")
     check(torch.float16, (64, 4, 3, 5), keys=EVERY, samples=4, post_norm="rms", bs_last=True)
+
+
+@pytest.mark.parametrize("dtype,channels", [(torch.bfloat16, 64), (torch.bfloat16, 768), (torch.bfloat16, 1024), (torch.float16, 384),
+                                            (torch.float32, 512), (torch.float32, 96)])
+@pytest.mark.parametrize("rows,samples", [(2400, 1), (2380, 7), (12544, 64), (2368, 74)])
+def test_many_rows(dtype, channels, rows, samples):
+    """Runs of rows through shared memory, a warp per row; also runs shorter than the rows in flight."""
+    check(dtype, (rows, channels), norm="layer", post_norm="rms", samples=samples, keys=EVERY)
+    check(dtype, (rows, channels), norm="rms", residual=False, keys=("weight",), train=False)
+
+
+@pytest.mark.parametrize("dtype,channels", [(torch.bfloat16, 1152), (torch.bfloat16, 4096), (torch.bfloat16, 8192), (torch.float32, 2048),
+                                            (torch.float32, 8192), (torch.float16, 5000)])
+@pytest.mark.parametrize("rows,samples", [(601, 1), (750, 25), (608, 2)])
+def test_many_wide_rows(dtype, channels, rows, samples):
+    """Runs of rows through shared memory, a block per row."""
+    check(dtype, (rows, channels), norm="layer", post_norm="layer", samples=samples, keys=EVERY)
+    check(dtype, (rows, channels), norm="rms", residual=False, keys=("weight",), train=False)
