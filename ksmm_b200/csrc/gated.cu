@@ -2,6 +2,7 @@
 // over whole tensors: for types and shapes whose last factor does not form the product in its epilogue, and
 // for every backward pass.  Memory is what bounds them: three tensors move forward, five backward.
 #include <algorithm>
+#include <type_traits>
 
 #include "gated.cuh"
 #include "gated.h"
@@ -62,6 +63,77 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// The backward with the sums of its lines (features of a batch-last tensor), which are the gradients of the biases:
+// a block per line.  Against a pass of its own over dg and du, 2 x 2048 x 12544 bf16: 21 us saved.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    gate_lines_kernel(const T* __restrict__ gu, int64_t ld, const T* __restrict__ dh, int64_t h_ld, T* __restrict__ out,
+                      int64_t half, int64_t out_half, int64_t len, int act, T* __restrict__ bias_grad) {
+  using Sum = typename std::conditional<sizeof(T) == 4, double, float>::type;  // (a thread's share of a long line)
+  const int64_t line = blockIdx.x;
+  const T* at = gu + line * ld;
+  const T* dp = dh + line * h_ld;
+  T* op = out + line * ld;
+  Sum sg = 0, su = 0;
+  for (int64_t x = threadIdx.x * V; x < len; x += 256 * V) {
+    float g[V], u[V], d[V], a[V], b[V];
+    get<T, V>(at + x, g);
+    get<T, V>(at + half + x, u);
+    get<T, V>(dp + x, d);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float value, slope;
+      gate_slope<sizeof(T) == 2>(g[e], act, value, slope);
+      a[e] = d[e] * u[e] * slope;
+      b[e] = d[e] * value;
+      s1 += a[e];
+      s2 += b[e];
+    }
+    put<T, V>(op + x, a);
+    put<T, V>(op + out_half + x, b);
+    sg += s1;
+    su += s2;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sg += __shfl_xor_sync(0xffffffffu, sg, o);
+    su += __shfl_xor_sync(0xffffffffu, su, o);
+  }
+  __shared__ Sum part[2][8];
+  if ((threadIdx.x & 31) == 0) {
+    part[0][threadIdx.x >> 5] = sg;
+    part[1][threadIdx.x >> 5] = su;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    Sum t = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += part[threadIdx.x][w];
+    bias_grad[threadIdx.x * gridDim.x + line] = ElemTraits<T>::from_float(static_cast<float>(t));
+  }
+}
+
+template <typename T>
+int gate_lines_typed(const void* gu, int64_t ld, const void* dh, int64_t dh_ld, void* out, int64_t out_half, int64_t lines,
+                     int64_t len, int act, void* bias_grad, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  if (lines > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "gated layer: too many features");
+  const int64_t half = lines * ld;
+  const bool vec = reinterpret_cast<uintptr_t>(gu) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(dh) % 16 == 0 && ld % V == 0 && dh_ld % V == 0 && len % V == 0 && out_half % V == 0;
+  auto go = [&](auto kern) {
+    kern<<<static_cast<unsigned>(lines), 256, 0, stream>>>(static_cast<const T*>(gu), ld, static_cast<const T*>(dh), dh_ld,
+                                                           static_cast<T*>(out), half, out_half, len, act, static_cast<T*>(bias_grad));
+  };
+  if (vec) go(gate_lines_kernel<T, V>);
+  else go(gate_lines_kernel<T, 1>);
+  count_launch();
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "gate kernel launch failed: %s", cudaGetErrorString(err));
+  return KSMM_OK;
+}
+
 template <typename T, bool BACKWARD>
 int gate_typed(const void* gu, int64_t ld, const void* dh, int64_t h_ld, void* out, int64_t out_half, int64_t lines, int64_t len,
                int act, cudaStream_t stream) {
@@ -102,7 +174,12 @@ int launch_gate(const void* gu, int64_t ld, void* h, int64_t h_ld, int64_t lines
 }
 
 int launch_gate_backward(const void* gu, int64_t ld, const void* dh, int64_t dh_ld, void* out, int64_t out_half, int64_t lines,
-                         int64_t len, int dtype, int act, cudaStream_t stream) {
+                         int64_t len, int dtype, int act, void* bias_grad, cudaStream_t stream) {
+  if (bias_grad) {
+    if (dtype == KSMM_F32) return gate_lines_typed<float>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, bias_grad, stream);
+    if (dtype == KSMM_F16) return gate_lines_typed<__half>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, bias_grad, stream);
+    return gate_lines_typed<__nv_bfloat16>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, bias_grad, stream);
+  }
   if (dtype == KSMM_F32) return gate_typed<float, true>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, stream);
   if (dtype == KSMM_F16) return gate_typed<__half, true>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, stream);
   return gate_typed<__nv_bfloat16, true>(gu, ld, dh, dh_ld, out, out_half, lines, len, act, stream);

@@ -1777,6 +1777,13 @@ static size_t gated_buffer_bytes(int nfactors, const int32_t* patterns, int64_t 
   return align_up(2 * mx * ld * es, 256);
 }
 
+// what a training step keeps: every intermediate, and both halves before the product
+static size_t gated_saved_bytes(int nfactors, const int32_t* patterns, int64_t ld, int es) {
+  const int32_t* pl = patterns + 4 * (nfactors - 1);
+  return gated_buffer_bytes(nfactors, patterns, ld, es) * (nfactors - 1) +
+         align_up(2 * static_cast<size_t>(pl[0]) * pl[1] * pl[3] * ld * es, 256);
+}
+
 // Runs one factor of both chains: the input is shared or two halves, weights, output and bias are two halves.
 static int run_pair(const Problem& p, int shared_input, size_t scratch_room, cudaStream_t stream) {
   Problem g = p;
@@ -1788,6 +1795,18 @@ static int run_pair(const Problem& p, int shared_input, size_t scratch_room, cud
   const int cfg = p.in_dtype != KSMM_F32 && !lookup_choice(p, &pin) && 2 * ((p.b + 63) / 64) <= tc::num_sms() ? tc_default_config(g) : -1;
   if (cfg >= 0) return tc_launch(g, cfg, stream);
   const size_t es = dtype_size(p.in_dtype);
+  if (!shared_input && in_is_last(p) && out_is_last(p)) {
+    // halves that follow one another are blocks of one problem
+    Problem h = p;
+    h.a = 2 * p.a;
+    Choice ch = auto_choice(h);
+    h.scratch_bytes = scratch_need(h, ch);
+    if (h.scratch_bytes > scratch_room) {
+      ch = Choice{KSMM_ALGO_SIMT, -1};
+      h.scratch_bytes = 0;
+    }
+    return run_family(h, ch.algo, ch.config, stream);
+  }
   const size_t in_half = static_cast<size_t>(p.a) * p.c * p.d * (p.bs_last ? in_stride(p) : p.batch) * es;
   const size_t out_half = static_cast<size_t>(p.a) * p.b * p.d * (out_is_last(p) ? out_stride(p) : p.batch) * es;
   for (int q = 0; q < 2; ++q) {
@@ -1839,6 +1858,8 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   char* halves = keep ? kept + one * (n - 1) : at;
   if (!keep && !fuse) at += halves_bytes;
   const size_t used = static_cast<size_t>(at - ws);
+  if (run && used > D.workspace_bytes)
+    return set_error(KSMM_ERR_WORKSPACE, "gated layer: need at least %zu bytes of workspace, got %zu", used, D.workspace_bytes);
   const size_t room = run ? D.workspace_bytes - used : SIZE_MAX;
   size_t scratch = 0;
   int st = KSMM_OK;
@@ -1879,6 +1900,9 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
       st = check_problem(p);
       if (st != KSMM_OK) return st;
       if (p.out_bs_last < 0) scratch = std::max(scratch, scratch_need(p, auto_choice(p)));
+      Problem h = p;
+      h.a = 2 * p.a;
+      if (f > 0 && in_is_last(p) && out_is_last(p)) scratch = std::max(scratch, scratch_need(h, auto_choice(h)));
     }
     cur = p.out;
     if (D.layouts) D.layouts[f] = plan.out_last[f];
@@ -1896,8 +1920,106 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   return st;
 }
 
+// The two chains' backward in one: where every tensor between the ends is batch-last, the halves that follow one
+// another are one problem of a pattern with twice as many blocks, (2a, b, c, d), and only the first factor, whose
+// input they share, has two weight gradients and a sum.  `grads`: dg and du, rows ld apart.
+// 12544 rows of 768 -> 2048 bf16: STACKED_A us chain by chain, STACKED_B so.
+static int gated_stacked_backward(bool run, const ksmm_gated_desc_t& D, const void* grads, void* grad_input, void* const* grad_values,
+                                  char* ws, size_t ws_bytes, bool need_input, cudaStream_t stream, size_t* need) {
+  const int n = D.nfactors, es = dtype_size(D.dtype);
+  const int64_t batch = D.batch, ld = padded_ld(batch, es);
+  const size_t one = gated_buffer_bytes(n, D.patterns, ld, es);
+  const int32_t* q0 = D.patterns;
+  const int64_t n_in = static_cast<int64_t>(q0[0]) * q0[2] * q0[3];
+  // the input's gradient: in its own layout where the first factor can turn, else transposed afterwards
+  const int32_t t0[4] = {q0[0], q0[2], q0[1], q0[3]};
+  const bool sums = tc_gated_fits(t0, batch, D.dtype, 1, D.bs_last);
+  const bool to_input = sums || D.bs_last || can_switch_layout(t0, batch, D.dtype, true);
+  const size_t input_bytes = align_up(static_cast<size_t>(n_in) * ld * es, 256);
+  char* const dummy = reinterpret_cast<char*>(static_cast<uintptr_t>(1) << 20);
+  if (!run) ws = dummy;
+  char* gbuf = ws;                                   // gradients of the intermediates, two alternating buffers
+  char* gx = gbuf + 2 * one;                         // the gate's share of the input's gradient
+  char* turned = gx + (need_input && !sums ? input_bytes : 0);
+  char* tail = turned + (need_input && !to_input ? input_bytes : 0);
+  const size_t room = ws_bytes - static_cast<size_t>(tail - ws);
+  size_t tail_bytes = 0;
+  const char* g = run ? static_cast<const char*>(grads) : dummy;
+  int st = KSMM_OK;
+  for (int f = n - 1; f >= 0; --f) {
+    const int32_t* q = D.patterns + 4 * f;
+    const size_t welems = static_cast<size_t>(q[0]) * q[1] * q[2] * q[3];
+    const size_t out_half = static_cast<size_t>(q[0]) * q[1] * q[3] * ld * es;
+    if (!run || grad_values[f]) {
+      for (int h = 0; h < (f == 0 ? 2 : 1); ++h) {
+        Problem p = backward_problem(nullptr, nullptr, run ? static_cast<char*>(grad_values[f]) + h * welems * es : dummy, batch,
+                                     f == 0 ? q[0] : 2 * q[0], q[1], q[2], q[3], D.dtype, f == 0 ? D.bs_last : 1);
+        WgradOperand x{run ? D.input : dummy, D.bs_last, batch}, gw{g + h * out_half, 1, ld};
+        if (f > 0) x = WgradOperand{run ? static_cast<const char*>(D.saved) + static_cast<size_t>(f - 1) * one : dummy, 1, ld};
+        tail_bytes = std::max(tail_bytes, wgrad_workspace_bytes(p, x, gw));
+        if (run) st = wgrad_launch(p, x, gw, tail, room, stream);
+        if (st != KSMM_OK) return st;
+      }
+    }
+    if (f == 0 && !need_input) break;
+    const size_t wt = align_up(2 * welems * es, 256);
+    tail_bytes = std::max(tail_bytes, wt);
+    if (run) st = launch_transpose_blocks(D.values[f], tail, 2 * static_cast<int64_t>(q[0]) * q[3], q[2], q[1], es, stream);
+    if (st != KSMM_OK) return st;
+    char* dst = f == 0 ? (to_input ? (run ? static_cast<char*>(grad_input) : dummy) : turned) : gbuf + (f & 1) * one;
+    const int64_t dst_ld = f == 0 && to_input ? batch : ld;
+    for (int h = 0; h < (f == 0 && !sums ? 2 : 1); ++h) {
+      const bool half = f == 0 && !sums;
+      Problem p = backward_problem(g + (half ? h * out_half : 0), tail + (half ? h * welems * es : 0), half && h == 0 ? gx : dst, batch,
+                                   f == 0 ? q[0] : 2 * q[0], q[2], q[1], q[3], D.dtype, 1);
+      if (ld != batch) {
+        p.in_ld = ld;
+        p.out_ld = dst_ld;
+      }
+      p.no_alloc = 1;
+      const bool turns = f == 0 && to_input && !D.bs_last;
+      if (turns) p.out_bs_last = 0;
+      if (f == 0 && sums) {
+        p.group_shared_input = 0;
+        if (run) st = tc_gated_sum(p, stream);
+      } else {
+        if (half && h == 1 && to_input) p.residual = gx;
+        Choice ch = turns ? Choice{KSMM_ALGO_TC, -1} : auto_choice(p);
+        size_t sneed = turns ? 0 : scratch_need(p, ch);
+        tail_bytes = std::max(tail_bytes, wt + sneed);
+        if (run) {
+          if (sneed > room - wt) {
+            ch = Choice{KSMM_ALGO_SIMT, -1};
+            sneed = 0;
+          }
+          if (sneed) {
+            p.scratch = tail + wt;
+            p.scratch_bytes = sneed;
+          }
+          st = run_family(p, ch.algo, ch.config, stream);
+        }
+      }
+      if (st != KSMM_OK) return st;
+    }
+    g = dst;
+  }
+  if (run && need_input && !to_input) {
+    // (the halves' sums in the input's layout: the second one is turned and the first, turned into its place, added)
+    st = launch_transpose(turned, grad_input, n_in, batch, es, stream, 0, ld);
+    if (st == KSMM_OK && !sums) {
+      st = launch_transpose(gx, turned, n_in, batch, es, stream, 0, ld);
+      Problem rp;
+      rp.out = grad_input; rp.residual = turned; rp.out_dtype = D.dtype;
+      rp.a = q0[0]; rp.b = q0[2]; rp.d = q0[3]; rp.batch = batch;
+      if (st == KSMM_OK) st = residual_pass(rp, stream);
+    }
+  }
+  if (need) *need = static_cast<size_t>(tail - ws) + align_up(tail_bytes, 256);
+  return st;
+}
+
 static int gated_backward_walk(bool run, const ksmm_gated_desc_t& D, int out_last, const void* grad_output, void* grad_input,
-                               void* const* grad_values, void* grad_bias, bool need_input, bool allow, bool one_layout,
+                               void* const* grad_values, void* grad_bias, bool need_input, bool aligned, bool allow, bool one_layout,
                                cudaStream_t stream, size_t* need) {
   const int n = D.nfactors, es = dtype_size(D.dtype);
   const int64_t batch = D.batch;
@@ -1906,18 +2028,22 @@ static int gated_backward_walk(bool run, const ksmm_gated_desc_t& D, int out_las
   const int64_t n_out = static_cast<int64_t>(pl[0]) * pl[1] * pl[3];
   const int64_t n_in = static_cast<int64_t>(D.patterns[0]) * D.patterns[2] * D.patterns[3];
   const int L = D.layouts[n - 1];
+  bool stacked = aligned && !one_layout && (D.bs_last || allow);
+  for (int f = 0; f < n; ++f) stacked = stacked && D.layouts[f] == 1;
   const size_t one = gated_buffer_bytes(n, D.patterns, ld, es);
   const size_t turn_bytes = L != out_last ? align_up(static_cast<size_t>(n_out) * ld * es, 256) : 0;
   const size_t half_bytes = static_cast<size_t>(n_out) * (L ? ld : batch) * es;
-  const size_t half_at = align_up(half_bytes, 256);  // the up projection's gradient starts aligned
-  const size_t gx_bytes = need_input ? align_up(static_cast<size_t>(n_in) * batch * es, 256) : 0;
+  const size_t half_at = stacked ? half_bytes : align_up(half_bytes, 256);  // else the second gradient starts aligned
+  const size_t gx_bytes = need_input && !stacked ? align_up(static_cast<size_t>(n_in) * batch * es, 256) : 0;
   char* ws = run ? static_cast<char*>(D.workspace) : reinterpret_cast<char*>(static_cast<uintptr_t>(1) << 20);
   char* turned = ws;
   char* grads = turned + turn_bytes;
-  char* gx = grads + 2 * half_at;
+  char* gx = grads + align_up(2 * half_at, 256);
   char* tail = gx + gx_bytes;
   const size_t used = static_cast<size_t>(tail - ws);
   int st = KSMM_OK;
+  // the sums of a batch-last gradient's lines come from the kernel that forms it, where the lines fill the GPU
+  const bool own_sums = grad_bias && L == 1 && (n_out >= 296 || stacked);
   if (run) {
     const char* halves = static_cast<const char*>(D.saved) + one * (n - 1);
     const void* dh = grad_output;
@@ -1929,13 +2055,19 @@ static int gated_backward_walk(bool run, const ksmm_gated_desc_t& D, int out_las
       dh = turned;
       if (L) dh_ld = ld;
     }
-    st = launch_gate_backward(halves, L ? ld : n_out, dh, dh_ld, grads, static_cast<int64_t>(half_at) / es, L ? n_out : batch, L ? batch : n_out, D.dtype,
-                              D.activation, stream);
+    st = launch_gate_backward(halves, L ? ld : n_out, dh, dh_ld, grads, static_cast<int64_t>(half_at) / es, L ? n_out : batch,
+                              L ? batch : n_out, D.dtype, D.activation, own_sums ? grad_bias : nullptr, stream);
     if (st != KSMM_OK) return st;
+  }
+  size_t tail_need = 0;
+  if (stacked) {
+    st = gated_stacked_backward(run, D, grads, grad_input, grad_values, tail, run ? D.workspace_bytes - used : SIZE_MAX, need_input,
+                                stream, run ? nullptr : &tail_need);
+    if (need) *need = used + tail_need;
+    return st;
   }
   const void *vals[ChainPlan::kMax] = {}, *inters[ChainPlan::kMax] = {};
   void* gv[ChainPlan::kMax] = {};
-  size_t tail_need = 0;
   for (int q = 0; q < 2; ++q) {
     for (int f = 0; f < n && run; ++f) {
       const int32_t* t = D.patterns + 4 * f;
@@ -1951,7 +2083,7 @@ static int gated_backward_walk(bool run, const ksmm_gated_desc_t& D, int out_las
     size_t w = 0;
     st = chain_backward_walk(run, D.input, vals, inters, D.layouts, grads + q * half_at,
                              q == 0 ? gx : grad_input, gv,
-                             grad_bias ? static_cast<char*>(grad_bias) + q * (n_out * es) : nullptr, tail,
+                             grad_bias && !own_sums ? static_cast<char*>(grad_bias) + q * (n_out * es) : nullptr, tail,
                              run ? D.workspace_bytes - used : SIZE_MAX, batch, n, D.patterns, D.dtype, D.bs_last, need_input, allow,
                              one_layout, stream, run ? nullptr : &w, L, ld,
                              need_input && q == 1 ? gx : nullptr);
@@ -2010,10 +2142,7 @@ int ksmm_cu_gated_train_bytes(int nfactors, const int32_t* patterns, int64_t bat
   if (batch == 0) return KSMM_OK;
   const bool one_layout = train_one_layout(nfactors, patterns, batch, dtype, bs_last);
   const int es = dtype_size(dtype);
-  const int64_t ld = one_layout ? batch : padded_ld(batch, es);
-  const int32_t* pl = patterns + 4 * (nfactors - 1);
-  *saved_bytes = gated_buffer_bytes(nfactors, patterns, ld, es) * (nfactors - 1) +
-                 align_up(2 * static_cast<size_t>(pl[0]) * pl[1] * pl[3] * ld * es, 256);
+  *saved_bytes = gated_saved_bytes(nfactors, patterns, one_layout ? batch : padded_ld(batch, es), es);
   if ((st = gated_forward_need(nfactors, patterns, batch, dtype, bs_last, out_bs_last, true, one_layout, forward_bytes)) != KSMM_OK)
     return st;
   for (int fwd = 0; fwd < (one_layout ? 1 : 2); ++fwd) {  // layouts of a forward pass with and without switches
@@ -2021,9 +2150,9 @@ int ksmm_cu_gated_train_bytes(int nfactors, const int32_t* patterns, int64_t bat
     const ksmm_gated_desc_t D = gated_desc(nfactors, patterns, batch, dtype, bs_last, layouts);
     size_t need = 0;
     st = gated_walk(false, D, out_bs_last, true, fwd != 0, one_layout, nullptr, &need);
-    for (int mode = 0; mode < 4 && st == KSMM_OK; ++mode) {
-      st = gated_backward_walk(false, D, out_bs_last, nullptr, nullptr, nullptr, nullptr, (mode & 1) != 0, (mode >> 1) != 0, one_layout,
-                               nullptr, &need);
+    for (int mode = 0; mode < 8 && st == KSMM_OK; ++mode) {
+      st = gated_backward_walk(false, D, out_bs_last, nullptr, nullptr, nullptr, nullptr, (mode & 1) != 0, (mode & 2) != 0, (mode & 4) != 0,
+                               one_layout, nullptr, &need);
       *backward_bytes = std::max(*backward_bytes, need);
     }
     if (st != KSMM_OK) return st;
@@ -2051,14 +2180,16 @@ int ksmm_cu_gated_forward(const ksmm_gated_desc_t* desc, void* stream) {
   if ((st = check_values(D.nfactors, D.values)) != KSMM_OK) return st;
   const bool keep = D.saved != nullptr;
   const bool one_layout = keep && train_one_layout(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last);
-  size_t want[3] = {0, 0, 0};
-  st = keep ? ksmm_cu_gated_train_bytes(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, out_last, &want[0], &want[1], &want[2])
-            : gated_forward_need(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, out_last, false, false, &want[1]);
-  if (st != KSMM_OK) return st;
-  if (keep && !D.layouts) return set_error(KSMM_ERR_BAD_ARGUMENT, "null layouts");
-  if ((keep && (reinterpret_cast<uintptr_t>(D.saved) % 256 || D.saved_bytes < want[0])) ||
-      (want[1] && (!D.workspace || reinterpret_cast<uintptr_t>(D.workspace) % 256 || D.workspace_bytes < want[1])))
-    return set_error(KSMM_ERR_WORKSPACE, "gated layer: need %zu bytes kept and %zu of workspace, aligned to 256", want[0], want[1]);
+  if (keep) {
+    const int es = dtype_size(D.dtype);
+    const int64_t ld = one_layout ? D.batch : padded_ld(D.batch, es);
+    const size_t want = gated_saved_bytes(D.nfactors, D.patterns, ld, es);
+    if (!D.layouts) return set_error(KSMM_ERR_BAD_ARGUMENT, "null layouts");
+    if (reinterpret_cast<uintptr_t>(D.saved) % 256 || D.saved_bytes < want)
+      return set_error(KSMM_ERR_WORKSPACE, "gated layer: need %zu bytes kept, aligned to 256, got %zu", want, D.saved_bytes);
+  }
+  if (D.workspace_bytes && (!D.workspace || reinterpret_cast<uintptr_t>(D.workspace) % 256))
+    return set_error(KSMM_ERR_WORKSPACE, "gated layer: the workspace is aligned to 256 bytes");
   // (a trainable fp32 layer keeps the kernels that its factors have one by one, as a chain does)
   const bool allow = !one_layout && aligned16(D.input) && aligned16(D.output) && aligned_values(D) &&
                      (!keep || train_may_switch(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, false, true));
@@ -2093,12 +2224,13 @@ int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* grad_outpu
   for (int f = 0; f < D.nfactors; ++f)
     if (D.layouts[f] != 0 && D.layouts[f] != 1) return set_error(KSMM_ERR_BAD_ARGUMENT, "layouts are those of the forward pass");
   const bool one_layout = train_one_layout(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last);
-  const bool allow = aligned16(grad_input) && aligned_values(D) &&
-                     train_may_switch(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, true, grad_input != nullptr);
+  bool aligned = aligned16(grad_input) && aligned_values(D);
+  for (int f = 0; f < D.nfactors; ++f) aligned = aligned && aligned16(grad_values[f]);
+  const bool allow = aligned && train_may_switch(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, true, grad_input != nullptr);
   size_t need = 0;
   for (int run = 0; run < 2; ++run) {
-    st = gated_backward_walk(run != 0, D, out_last, grad_output, grad_input, grad_values, grad_bias, grad_input != nullptr, allow,
-                             one_layout, s, run ? nullptr : &need);
+    st = gated_backward_walk(run != 0, D, out_last, grad_output, grad_input, grad_values, grad_bias, grad_input != nullptr, aligned,
+                             allow, one_layout, s, run ? nullptr : &need);
     if (st != KSMM_OK) return st;
     if (!run && (!D.workspace || reinterpret_cast<uintptr_t>(D.workspace) % 256 || D.workspace_bytes < need))
       return set_error(KSMM_ERR_WORKSPACE, "gated backward: need %zu bytes aligned to 256, got %zu", need, D.workspace_bytes);

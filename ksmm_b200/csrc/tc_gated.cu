@@ -11,6 +11,8 @@
 // Work split, ring, descriptors and epilogue staging are those of tc_kernel.cu: a persistent CTA keeps one tile of
 // output features, its weights of both halves resident in shared memory where three k chunks of 64 hold them
 // (c <= 192; 96 KB), and walks (block, batch tile) pairs; longer blocks stream weights through the ring.
+// The same kernel with one accumulator adds the halves' products instead (kSum): the gradient of a gated layer's
+// input, Wg^T dg + Wu^T du, rounded once, in place of two multiplications and an addition.
 // Against the halves written by a grouped launch and multiplied by a pass over them, the last factor's traffic
 // falls from 2 c + 2 b + 3 b to 2 c + b elements per block and batch entry.
 #include <cuda.h>
@@ -47,6 +49,8 @@ struct Params {
   int64_t y_ld;
   int y_direct;
 };
+
+enum { kProduct, kKeep, kSum };  // h; h and both halves; the sum of the halves
 
 template <bool WRES, int NWC, int SX, int STGN>
 struct Cfg {
@@ -144,12 +148,13 @@ __device__ __forceinline__ void add_column_bias(uint32_t (&r)[32], const void* b
   }
 }
 
-// IN_LAST / OUT_LAST: layouts of input and output as in tc_kernel.cu.  KEEP: both halves are stored as well.
-template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, bool KEEP>
+// IN_LAST / OUT_LAST: layouts of input and output as in tc_kernel.cu.
+template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE>
 __global__ void __launch_bounds__(kBlock, 1)
     gated_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmH, const Params P) {
   using C = Cfg<WRES, NWC, SX, STGN>;
+  constexpr bool KEEP = MODE == kKeep, SUM = MODE == kSum;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t wres0 = (raw + 1023u) & ~1023u;  // 1024-byte alignment for the 128-byte swizzle
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         for (int t = 0; t < 2 * nk; ++t) {
           const int g = t >= nk ? 1 : 0, kc = t - g * nk;
           if (!mbar_wait<0>(full_bar(si), sph, abort_flag, P.status, kGatedWaits + 4)) { ok = false; break; }
-          const uint32_t dcol = tmem_base + buf * 2 * kNT + g * kNT;
+          const uint32_t dcol = tmem_base + buf * 2 * kNT + (SUM ? 0 : g * kNT);
           const uint32_t xsrc = ring0 + si * C::kStage;
           const uint32_t wsrc = WRES ? wres0 + (g * NWC + kc) * kChunk : xsrc + kChunk;
           const uint32_t xlo = (xsrc >> 4) | (IN_LAST ? kLboMN : kLboK), wlo = (wsrc >> 4) | kLboMN;
@@ -278,7 +283,7 @@ __global__ void __launch_bounds__(kBlock, 1)
           for (int k = 0; k < kKC / 16; ++k) {
             const uint64_t xdesc = (static_cast<uint64_t>(kDescHi) << 32) | (xlo + k * (IN_LAST ? kStepMN : kStepK));
             const uint64_t wdesc = (static_cast<uint64_t>(kDescHi) << 32) | (wlo + k * kStepMN);
-            umma<2>(dcol, OUT_LAST ? wdesc : xdesc, OUT_LAST ? xdesc : wdesc, P.idesc, (kc | k) != 0 ? 1u : 0u);
+            umma<2>(dcol, OUT_LAST ? wdesc : xdesc, OUT_LAST ? xdesc : wdesc, P.idesc, ((SUM ? t : kc) | k) != 0 ? 1u : 0u);
           }
           umma_commit(empty_bar(si));
           if (++si == SX) { si = 0; sph ^= 1u; }
@@ -318,7 +323,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       if (active) {
         const uint32_t t0 = tmem_base + lane_addr + buf * 2 * kNT + box * 32;
         tmem_ld32(t0, g);
-        tmem_ld32(t0 + kNT, u);
+        if constexpr (!SUM) tmem_ld32(t0 + kNT, u);
         tmem_ld_wait();
       }
       // the accumulators are in registers: hand them back
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(tempty_bar(buf));
       if (!active) continue;
-      if (P.bias != nullptr) {
+      if (!SUM && P.bias != nullptr) {
         if constexpr (OUT_LAST) {
           float bg = 0.f, bu = 0.f;
           if (q * 32 + lane < row_limit) {
@@ -382,12 +387,17 @@ __global__ void __launch_bounds__(kBlock, 1)
         fill(w);
         send(&tmH, 1);
       }
-      switch (P.act) {
-        case KSMM_ACT_SILU: gate_32<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
-        case KSMM_ACT_GELU: gate_32<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
-        case KSMM_ACT_SIGMOID: gate_32<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
-        case KSMM_ACT_RELU: gate_32<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
-        default: gate_32<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+      if constexpr (SUM) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
+      } else {
+        switch (P.act) {
+          case KSMM_ACT_SILU: gate_32<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
+          case KSMM_ACT_GELU: gate_32<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
+          case KSMM_ACT_SIGMOID: gate_32<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
+          case KSMM_ACT_RELU: gate_32<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
+          default: gate_32<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+        }
       }
       fill(w);
       if (OUT_LAST && P.y_direct) {
@@ -419,10 +429,11 @@ __global__ void __launch_bounds__(kBlock, 1)
   }
 }
 
-template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, bool KEEP>
+template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE>
 int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
   using C = Cfg<WRES, NWC, SX, STGN>;
-  auto kern = gated_kernel<IN_LAST, OUT_LAST, WRES, NWC, SX, STGN, KEEP>;
+  constexpr bool KEEP = MODE == kKeep;
+  auto kern = gated_kernel<IN_LAST, OUT_LAST, WRES, NWC, SX, STGN, MODE>;
   static std::atomic<bool> attr_set[64];  // once per device (a repeated set is harmless)
   int dev = 0;
   cudaGetDevice(&dev);
@@ -500,10 +511,16 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
 template <bool IN_LAST, bool OUT_LAST>
 int launch_layout(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
   if (p.c <= 3 * kKC)
-    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 4, 2, true>(p, halves, halves_ld, stream)
-                  : launch<IN_LAST, OUT_LAST, true, 3, 6, 1, false>(p, halves, halves_ld, stream);
-  return halves ? launch<IN_LAST, OUT_LAST, false, 0, 4, 2, true>(p, halves, halves_ld, stream)
-                : launch<IN_LAST, OUT_LAST, false, 0, 5, 1, false>(p, halves, halves_ld, stream);
+    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 4, 2, kKeep>(p, halves, halves_ld, stream)
+                  : launch<IN_LAST, OUT_LAST, true, 3, 6, 1, kProduct>(p, halves, halves_ld, stream);
+  return halves ? launch<IN_LAST, OUT_LAST, false, 0, 4, 2, kKeep>(p, halves, halves_ld, stream)
+                : launch<IN_LAST, OUT_LAST, false, 0, 5, 1, kProduct>(p, halves, halves_ld, stream);
+}
+
+template <bool OUT_LAST>
+int launch_sum(const Problem& p, cudaStream_t stream) {
+  return p.c <= 3 * kKC ? launch<true, OUT_LAST, true, 3, 6, 1, kSum>(p, nullptr, 0, stream)
+                        : launch<true, OUT_LAST, false, 0, 5, 1, kSum>(p, nullptr, 0, stream);
 }
 
 }  // namespace
@@ -523,6 +540,10 @@ int tc_gated_launch(const Problem& p, void* halves, int64_t halves_ld, cudaStrea
                                : tc::launch_layout<true, false>(p, halves, halves_ld, stream);
   return out_last ? tc::launch_layout<false, true>(p, halves, halves_ld, stream)
                   : tc::launch_layout<false, false>(p, halves, halves_ld, stream);
+}
+
+int tc_gated_sum(const Problem& p, cudaStream_t stream) {
+  return out_is_last(p) ? tc::launch_sum<true>(p, stream) : tc::launch_sum<false>(p, stream);
 }
 
 }  // namespace ksmm

@@ -576,8 +576,10 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 };
 
-py::object gated_train(const at::Tensor& x, const std::vector<at::Tensor>& factors, const py::handle& patterns, bool last,
+// KSGatedLinear: with gradients where something learns
+py::object gated_layer(const at::Tensor& x, const std::vector<at::Tensor>& factors, const py::handle& patterns, bool last,
                        bool out_last, const c10::optional<at::Tensor>& bias, int activation) {
+  if (!wants_grad(x, factors, bias)) return gated_forward(x, factors, patterns, last, out_last, bias, activation);
   Patterns p;
   if (!read_patterns(patterns, &p) || !gated_fits(x, factors, p, last, bias)) return py::none();
   at::Tensor out;
@@ -802,5 +804,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_forward", &grouped_forward, "Several chains on one input");
   m.def("residual_norm", &residual_norm, "Norms around a block, gate, residual scale and modulation");
   m.def("gated_forward", &gated_forward, "A gated layer without gradients");
-  m.def("gated_train", &gated_train, "A trainable gated layer as one autograd node");
+  m.def("gated_layer", &gated_layer, "A gated layer, as one autograd node where something learns");
 }

@@ -382,11 +382,7 @@ class KSGatedLinear(nn.Module):
         if tensor.dtype != self.dtype:
             raise TypeError(f"input dtype {tensor.dtype} differs from the layer's {self.dtype}")
         x = (tensor.reshape(tensor.size(0), -1) if self.bs_last else tensor.reshape(-1, tensor.size(-1))).contiguous()
-        factors = list(self.factors)
-        learns = torch.is_grad_enabled() and (x.requires_grad or any(f.requires_grad for f in factors)
-                                              or (self.bias is not None and self.bias.requires_grad))
-        call = _k.gated_chain_train if learns else _k.gated_chain_forward
-        y = call(x, factors, self.patterns, self.bs_last, self.bias, self.activation, self.out_bs_last)
+        y = _k.gated_layer(x, list(self.factors), self.patterns, self.bs_last, self.bias, self.activation, self.out_bs_last)
         if self.out_bs_last != bool(self.bs_last):
             return y
         if self.bs_last:

@@ -425,14 +425,17 @@ class GatedFunction(torch.autograd.Function):
         return grad_input, grad_bias, None, None, None, None, *grads
 
 
-def gated_chain_train(input, stacked_factors, patterns, bs_last, bias=None, activation="silu", out_bs_last=None):
-    """``gated_chain_forward`` as one autograd node."""
+def gated_layer(input, stacked_factors, patterns, bs_last, bias=None, activation="silu", out_bs_last=None):
+    """``gated_chain_forward``, as one autograd node where something learns."""
     out_last = bool(bs_last) if out_bs_last is None else bool(out_bs_last)
     if _native is not None and activation in _lib.GATES:
-        out = _native.gated_train(input, list(stacked_factors), patterns, bool(bs_last), out_last, bias, _lib.GATES[activation])
+        out = _native.gated_layer(input, stacked_factors, patterns, bool(bs_last), out_last, bias, _lib.GATES[activation])
         if out is not None:
-            return out
-    return GatedFunction.apply(input, bias, bool(bs_last), out_last, patterns, activation, *stacked_factors)
+            return _result(out)
+    if torch.is_grad_enabled() and (input.requires_grad or any(f.requires_grad for f in stacked_factors)
+                                    or (bias is not None and bias.requires_grad)):
+        return GatedFunction.apply(input, bias, bool(bs_last), out_last, patterns, activation, *stacked_factors)
+    return gated_chain_forward(input, stacked_factors, patterns, bs_last, bias, activation, out_last)
 
 
 def _check_grad_output(grad_output, input_like_shape, bs_last, a, b, d):
