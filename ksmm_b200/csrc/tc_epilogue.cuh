@@ -139,24 +139,24 @@ __device__ __forceinline__ void activate(Ref&& r, int act) {
 // elements.  Sixteen rows are read ahead of their stores; the stores are what it costs: a call of
 // (1,768,192,2) fp16 takes 12.5 us at 6504 columns, 28 at 6502 and 41 at 6501 (the copy of the input included).
 // `rows_here` rows and `cols` columns of the tile exist; rows from `first` up to `last` (multiples of 16) are stored.
-template <int OS>
+template <int OS, int AHEAD = 16>
 __device__ __forceinline__ void store_rows(uint32_t stg, uint8_t* yrow, int64_t step, int rows_here, int cols, int lane,
                                            int first = 0, int last = 32) {
   yrow += first * step;
 #pragma unroll
-  for (int r0 = first; r0 < last; r0 += 16) {
-    uint32_t w[16], prev[16];
+  for (int r0 = first; r0 < last; r0 += AHEAD) {
+    uint32_t w[AHEAD], prev[AHEAD];
 #pragma unroll
-    for (int rr = 0; rr < 16; ++rr)
+    for (int rr = 0; rr < AHEAD; ++rr)
       asm volatile("ld.shared.b32 %0, [%1];"
                    : "=r"(w[rr])
                    : "r"(stg + (r0 + rr) * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + ((lane & 3) << 2)));
     if constexpr (OS == 2) {
 #pragma unroll
-      for (int rr = 0; rr < 16; ++rr) prev[rr] = __shfl_up_sync(0xffffffffu, w[rr], 1);
+      for (int rr = 0; rr < AHEAD; ++rr) prev[rr] = __shfl_up_sync(0xffffffffu, w[rr], 1);
     }
 #pragma unroll
-    for (int rr = 0; rr < 16; ++rr, yrow += step) {
+    for (int rr = 0; rr < AHEAD; ++rr, yrow += step) {
       if (r0 + rr >= rows_here) break;
       if constexpr (OS == 4) {
         if (lane < cols) reinterpret_cast<uint32_t*>(yrow)[lane] = w[rr];

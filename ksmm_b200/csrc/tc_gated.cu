@@ -8,6 +8,13 @@
 // one commit.  The epilogue reads both accumulators, adds the biases, forms the product in fp32 and rounds
 // once, so that neither half goes to memory (training stores both as well, rounded, for the backward pass).
 //
+// PAIR: two CTAs of a cluster work on one tile of 256 features x 128 batch entries with the two-SM form of the MMA.
+// Each holds its own 128 features' weights and accumulators and loads half of the input chunk, so that an SM moves
+// half the input from L2 and reads a quarter less shared memory per product (25088 rows of (1,512,192,4): 54 us on
+// single SMs, 44 by pairs; floor 24 from 54 GFLOP, 22 from the bytes).  The leading CTA issues the MMAs for both; its
+// barriers count both CTAs' copies and epilogue warps.  (Arrivals at the other CTA's barrier carry no cluster-scope
+// release: what they order are tensor-memory reads, which have completed; with one, each cost a microsecond.)
+//
 // Work split, ring, descriptors and epilogue staging are those of tc_kernel.cu: a persistent CTA keeps one tile of
 // output features, its weights of both halves resident in shared memory where three k chunks of 64 hold them
 // (c <= 192; 96 KB), and walks (block, batch tile) pairs; longer blocks stream weights through the ring.
@@ -52,14 +59,77 @@ struct Params {
 
 enum { kProduct, kKeep, kSum };  // h; h and both halves; the sum of the halves
 
-template <bool WRES, int NWC, int SX, int STGN>
+template <bool WRES, int NWC, int SX, int STGN, bool PAIR>
 struct Cfg {
-  static constexpr int kStage = kChunk * (WRES ? 1 : 2);
+  static_assert(!PAIR || WRES, "pairs keep their weights");
+  static constexpr int kX = kChunk / (PAIR ? 2 : 1);  // a CTA's part of an input chunk
+  static constexpr int kStage = 2 * (kX + (WRES ? 0 : kChunk));  // a k chunk of both halves
   static constexpr int kStgPair = STGN * 32 * 128;  // staging of a pair of warps: 32 rows of 128 bytes
   static constexpr int kSmem = 2 * NWC * kChunk + SX * kStage + kEpi / 2 * kStgPair + kBarBytes + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
   static_assert(8 * (2 * SX + 6) + 8 <= kBarBytes, "barrier area");
 };
+
+// one lane of a warp that has converged
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// ---- two CTAs of a cluster ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// the address of this CTA's shared variable in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// loads into this CTA's shared memory whose bytes count at a barrier of either CTA
+__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void pair_load_4d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void pair_umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrives at the barrier at this offset in both CTAs once the MMAs issued so far are done
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t slot_smem, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_smem), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
 
 __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   uint64_t r;
@@ -104,22 +174,34 @@ __device__ __forceinline__ void gate_2(float g0, float g1, float u0, float u1, f
 }
 
 template <int ACT>
-__device__ __forceinline__ void gate_32(const uint32_t (&g)[32], const uint32_t (&u)[32], int dtype, uint32_t (&w)[16]) {
+__device__ __forceinline__ void gate_16(const uint32_t (&g)[16], const uint32_t (&u)[16], int dtype, uint32_t (&w)[8]) {
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) {
+  for (int e = 0; e < 16; e += 2) {
     float h0, h1;
     gate_2<ACT>(__uint_as_float(g[e]), __uint_as_float(g[e + 1]), __uint_as_float(u[e]), __uint_as_float(u[e + 1]), h0, h1);
     w[e / 2] = pack2(h0, h1, dtype);
   }
 }
 
-// r[e] += bias[at + e] for the 32 columns of a batch-first tile, of which `exist` exist (a multiple of 8): every lane
+// r[e] += b for 16 values of a row
+__device__ __forceinline__ void add_row_bias(uint32_t (&r)[16], float b) {
+  const uint64_t b2 = pack_f2(b, b);
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {
+    float y0, y1;
+    unpack_f2(add_f2(pack_f2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), b2), y0, y1);
+    r[e] = __float_as_uint(y0);
+    r[e + 1] = __float_as_uint(y1);
+  }
+}
+
+// r[e] += bias[at + e] for 16 columns of a batch-first tile, of which `exist` exist (a multiple of 8): every lane
 // reads the same 16 bytes, one transaction per eight columns
-__device__ __forceinline__ void add_column_bias(uint32_t (&r)[32], const void* bias, int64_t at, int exist, int dtype) {
+__device__ __forceinline__ void add_column_bias(uint32_t (&r)[16], const void* bias, int64_t at, int exist, int dtype) {
   const uint16_t* bp = static_cast<const uint16_t*>(bias) + at;
   const bool whole = (reinterpret_cast<uintptr_t>(bp) & 15) == 0;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     if (c * 8 >= exist) break;
     uint32_t w[4];
     if (whole) {
@@ -149,11 +231,12 @@ __device__ __forceinline__ void add_column_bias(uint32_t (&r)[32], const void* b
 }
 
 // IN_LAST / OUT_LAST: layouts of input and output as in tc_kernel.cu.
-template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE>
+template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE, bool PAIR>
 __global__ void __launch_bounds__(kBlock, 1)
     gated_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmH, const Params P) {
-  using C = Cfg<WRES, NWC, SX, STGN>;
+  static_assert(!PAIR || OUT_LAST, "pairs split the features, rows of the accumulator");
+  using C = Cfg<WRES, NWC, SX, STGN, PAIR>;
   constexpr bool KEEP = MODE == kKeep, SUM = MODE == kSum;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -180,7 +263,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     mbar_init(wempty_bar, 1);
     for (int q = 0; q < 2; ++q) {
       mbar_init(tfull_bar(q), 1);
-      mbar_init(tempty_bar(q), kEpi);
+      mbar_init(tempty_bar(q), PAIR ? 2 * kEpi : kEpi);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -192,20 +275,31 @@ __global__ void __launch_bounds__(kBlock, 1)
     if (KEEP) prefetch_tensormap(&tmH);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      pair_tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    } else {
+      tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // (the other CTA's barriers are set up)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  // barriers that count for both CTAs are the leader's
+  auto lead = [&](uint32_t bar) { return PAIR ? map_rank(bar, 0) : bar; };
+  (void)lead;
   grid_dep_wait();
   grid_dep_launch();
 
   const uint32_t d = P.d;
   const int nk = P.nk;
-  const int tj = static_cast<int>(blockIdx.x % P.tiles_j);
-  const uint32_t rc = blockIdx.x / P.tiles_j;
+  // (PAIR: tiles_j counts pairs of feature tiles)
+  const uint32_t unit = PAIR ? blockIdx.x / 2 : blockIdx.x;
+  const int tj = PAIR ? static_cast<int>(unit % P.tiles_j * 2 + rank) : static_cast<int>(unit % P.tiles_j);
+  const uint32_t rc = unit / P.tiles_j;
   const uint32_t row_begin = static_cast<uint32_t>(static_cast<uint64_t>(rc) * P.rows / P.row_groups);
   const uint32_t row_end = static_cast<uint32_t>(static_cast<uint64_t>(rc + 1) * P.rows / P.row_groups);
   const int j0 = tj * 128;
@@ -213,91 +307,132 @@ __global__ void __launch_bounds__(kBlock, 1)
 
   if (warp == 0) {
     // ===================== TMA producer =====================
-    if (lane == 0) {
-      uint32_t si = 0, sph = 0, wph = 0;
-      int cur_blk = -1;
-      bool ok = true;
-      auto load_w = [&](uint32_t dst, uint32_t bar, int kc, int blk) {
+    // (the whole warp walks the loop and one elected lane issues, as below)
+    const bool one = elect_one();
+    uint32_t si = 0, sph = 0, wph = 0;
+    int cur_blk = -1;
+    bool ok = true;
+    auto load_w = [&](uint32_t dst, uint32_t bar, int kc, int blk) {
 #pragma unroll
-        for (int wb = 0; wb < 2; ++wb)
-          tma_load_3d(dst + wb * kKC * 128, &tmW, bar, j0 + wb * kBox, kc * kKC, blk);
-      };
-      for (uint32_t row = row_begin; row < row_end && ok; ++row) {
-        const int blk = static_cast<int>(row / P.tiles_n);
-        const int n0 = static_cast<int>(row % P.tiles_n) * 128;
-        const int i = blk / d, l = blk % d;
-        if (WRES && blk != cur_blk) {
-          if (!mbar_wait<64>(wempty_bar, wph ^ 1u, abort_flag, P.status, kGatedWaits + 0)) { ok = false; break; }
-          wph ^= 1u;
-          mbar_expect_tx(wfull_bar, 2 * nk * kChunk);
+      for (int wb = 0; wb < 2; ++wb) {
+        if constexpr (PAIR) pair_load_3d(dst + wb * kKC * 128, &tmW, bar, j0 + wb * kBox, kc * kKC, blk);
+        else tma_load_3d(dst + wb * kKC * 128, &tmW, bar, j0 + wb * kBox, kc * kKC, blk);
+      }
+    };
+    // one input of a shared pair is loaded once and read by both halves' MMAs
+    const int inputs = P.stacked_input ? 2 : 1;
+    const uint32_t stage_bytes = (PAIR ? 2 : 1) * (inputs * C::kX + (WRES ? 0 : 2 * kChunk));
+    const uint32_t wfull_lead = lead(wfull_bar);
+    for (uint32_t row = row_begin; row < row_end && ok; ++row) {
+      const int blk = static_cast<int>(row / P.tiles_n);
+      const int n0 = static_cast<int>(row % P.tiles_n) * 128 + (PAIR ? static_cast<int>(rank) * 64 : 0);
+      const int i = blk / d, l = blk % d;
+      if (WRES && blk != cur_blk) {
+        ok = __all_sync(0xffffffffu, mbar_wait<64>(wempty_bar, wph ^ 1u, abort_flag, P.status, kGatedWaits + 0));
+        if (!ok) break;
+        wph ^= 1u;
+        if (one) {
+          if (rank == 0) mbar_expect_tx(wfull_bar, (PAIR ? 4 : 2) * nk * kChunk);
           for (int g = 0; g < 2; ++g)
-            for (int kc = 0; kc < nk; ++kc) load_w(wres0 + (g * NWC + kc) * kChunk, wfull_bar, kc, blk + g * blocks);
-          cur_blk = blk;
+            for (int kc = 0; kc < nk; ++kc) load_w(wres0 + (g * NWC + kc) * kChunk, wfull_lead, kc, blk + g * blocks);
         }
-        for (int t = 0; t < 2 * nk; ++t) {
-          const int g = t >= nk ? 1 : 0, kc = t - g * nk;
-          if (!mbar_wait<64>(empty_bar(si), sph ^ 1u, abort_flag, P.status, kGatedWaits + 1)) { ok = false; break; }
-          const uint32_t dst = ring0 + si * C::kStage, bar = full_bar(si);
-          mbar_expect_tx(bar, C::kStage);
-          const int gx = P.stacked_input ? g : 0;
-          if constexpr (IN_LAST) {
+        cur_blk = blk;
+      }
+      for (int kc = 0; kc < nk; ++kc) {
+        ok = __all_sync(0xffffffffu, mbar_wait<64>(empty_bar(si), sph ^ 1u, abort_flag, P.status, kGatedWaits + 1));
+        if (!ok) break;
+        const uint32_t dst = ring0 + si * C::kStage, bar = lead(full_bar(si));
+        if (one) {
+          if (rank == 0) mbar_expect_tx(full_bar(si), stage_bytes);
+          for (int g = 0; g < inputs; ++g) {
+            const uint32_t at = dst + g * C::kX;
+            if constexpr (PAIR) {
+              // this CTA's 64 of the tile's 128 batch entries
+              if constexpr (IN_LAST) pair_load_4d(at, &tmX, bar, n0, l, kc * kKC, i + g * P.a);
+              else pair_load_3d(at, &tmX, bar, kc * kKC, i, n0 + g * static_cast<int>(P.batch));
+            } else if constexpr (IN_LAST) {
 #pragma unroll
-            for (int xb = 0; xb < 2; ++xb)
-              tma_load_4d(dst + xb * kKC * 128, &tmX, bar, n0 + xb * kBox, l, kc * kKC, i + gx * P.a);
-          } else {
-            tma_load_3d(dst, &tmX, bar, kc * kKC, i, n0 + gx * static_cast<int>(P.batch));
+              for (int xb = 0; xb < 2; ++xb)
+                tma_load_4d(at + xb * kKC * 128, &tmX, bar, n0 + xb * kBox, l, kc * kKC, i + g * P.a);
+            } else {
+              tma_load_3d(at, &tmX, bar, kc * kKC, i, n0 + g * static_cast<int>(P.batch));
+            }
           }
-          if (!WRES) load_w(dst + kChunk, bar, kc, blk + g * blocks);
-          if (++si == SX) { si = 0; sph ^= 1u; }
+          if (!WRES) {
+            for (int g = 0; g < 2; ++g) load_w(dst + 2 * C::kX + g * kChunk, bar, kc, blk + g * blocks);
+          }
         }
+        if (++si == SX) { si = 0; sph ^= 1u; }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ===================== MMA issuer =====================
-    if (lane == 0) {
+    // The whole warp walks the loop, so that descriptors stay in uniform registers, and one elected lane issues.  With
+    // the loop inside `if (lane == 0)` an MMA's operands moved there one by one, and the issuing thread took 640
+    // cycles per 64 of k where the MMAs take 256: 25088 rows of (1,512,192,4),
+    // batch-last: 70 -> 59 us, with both halves' chunks in one ring stage 54, by pairs 44.
+    if (rank == 0) {
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
       constexpr uint32_t kLboMN = static_cast<uint32_t>((kKC * 128) >> 4) << 16, kLboK = 1u << 16;
       constexpr uint32_t kStepMN = (16 * 128) >> 4, kStepK = (16 * 2) >> 4;
+      constexpr unsigned kAll = 0xffffffffu;
+      const bool one = elect_one();
       uint32_t si = 0, sph = 0, wph = 0, ut = 0;
       int cur_blk = -1;
       bool ok = true;
+      auto commit = [&](uint32_t bar) {
+        if (one) {
+          if constexpr (PAIR) pair_commit(bar);
+          else umma_commit(bar);
+        }
+      };
       for (uint32_t row = row_begin; row < row_end && ok; ++row, ++ut) {
         const int blk = static_cast<int>(row / P.tiles_n);
         if (WRES && blk != cur_blk) {
-          if (!mbar_wait<0>(wfull_bar, wph, abort_flag, P.status, kGatedWaits + 2)) { ok = false; break; }
+          ok = __all_sync(kAll, mbar_wait<0>(wfull_bar, wph, abort_flag, P.status, kGatedWaits + 2));
+          if (!ok) break;
           wph ^= 1u;
           cur_blk = blk;
         }
         const uint32_t buf = ut & 1u, bph = (ut >> 1) & 1u;
-        if (!mbar_wait<0>(tempty_bar(buf), bph ^ 1u, abort_flag, P.status, kGatedWaits + 3)) { ok = false; break; }
+        ok = __all_sync(kAll, mbar_wait<0>(tempty_bar(buf), bph ^ 1u, abort_flag, P.status, kGatedWaits + 3));
+        if (!ok) break;
         tc_fence_after();
-        for (int t = 0; t < 2 * nk; ++t) {
-          const int g = t >= nk ? 1 : 0, kc = t - g * nk;
-          if (!mbar_wait<0>(full_bar(si), sph, abort_flag, P.status, kGatedWaits + 4)) { ok = false; break; }
-          const uint32_t dcol = tmem_base + buf * 2 * kNT + (SUM ? 0 : g * kNT);
-          const uint32_t xsrc = ring0 + si * C::kStage;
-          const uint32_t wsrc = WRES ? wres0 + (g * NWC + kc) * kChunk : xsrc + kChunk;
-          const uint32_t xlo = (xsrc >> 4) | (IN_LAST ? kLboMN : kLboK), wlo = (wsrc >> 4) | kLboMN;
+        const uint32_t half_x = P.stacked_input ? C::kX : 0;
+        for (int kc = 0; kc < nk; ++kc) {
+          ok = __all_sync(kAll, mbar_wait<0>(full_bar(si), sph, abort_flag, P.status, kGatedWaits + 4));
+          if (!ok) break;
+          const uint32_t stage = ring0 + si * C::kStage;
+          if (one) {
 #pragma unroll
-          for (int k = 0; k < kKC / 16; ++k) {
-            const uint64_t xdesc = (static_cast<uint64_t>(kDescHi) << 32) | (xlo + k * (IN_LAST ? kStepMN : kStepK));
-            const uint64_t wdesc = (static_cast<uint64_t>(kDescHi) << 32) | (wlo + k * kStepMN);
-            umma<2>(dcol, OUT_LAST ? wdesc : xdesc, OUT_LAST ? xdesc : wdesc, P.idesc, ((SUM ? t : kc) | k) != 0 ? 1u : 0u);
+            for (int g = 0; g < 2; ++g) {
+              const uint32_t dcol = tmem_base + buf * 2 * kNT + (SUM ? 0 : g * kNT);
+              const uint32_t xsrc = stage + g * half_x;
+              const uint32_t wsrc = WRES ? wres0 + (g * NWC + kc) * kChunk : stage + 2 * C::kX + g * kChunk;
+              const uint32_t xlo = (xsrc >> 4) | (IN_LAST ? kLboMN : kLboK), wlo = (wsrc >> 4) | kLboMN;
+#pragma unroll
+              for (int k = 0; k < kKC / 16; ++k) {
+                const uint64_t xdesc = (static_cast<uint64_t>(kDescHi) << 32) | (xlo + k * (IN_LAST ? kStepMN : kStepK));
+                const uint64_t wdesc = (static_cast<uint64_t>(kDescHi) << 32) | (wlo + k * kStepMN);
+                const uint32_t more = k != 0 || kc != 0 || (SUM && g != 0) ? 1u : 0u;
+                if constexpr (PAIR) pair_umma(dcol, wdesc, xdesc, P.idesc, more);
+                else umma<2>(dcol, OUT_LAST ? wdesc : xdesc, OUT_LAST ? xdesc : wdesc, P.idesc, more);
+              }
+            }
           }
-          umma_commit(empty_bar(si));
+          commit(empty_bar(si));
           if (++si == SX) { si = 0; sph ^= 1u; }
         }
         if (!ok) break;
-        umma_commit(tfull_bar(buf));
-        if (WRES && (row + 1 == row_end || static_cast<int>((row + 1) / P.tiles_n) != blk)) umma_commit(wempty_bar);
+        commit(tfull_bar(buf));
+        if (WRES && (row + 1 == row_end || static_cast<int>((row + 1) / P.tiles_n) != blk)) commit(wempty_bar);
       }
     }
     __syncwarp();
   } else {
     // ===================== epilogue =====================
-    // Sixteen warps (with eight, two per scheduler, the latencies of this chain of operations were the time of a
-    // tile: 70 us against 46 for 25088 rows of (1,512,192,4)).  Warp w: TMEM lane quarter w mod 4, 32 columns
+    // Sixteen warps, four per scheduler, with 16 columns of both halves in registers at a time.  Warp w: TMEM lane quarter w mod 4, 32 columns
     // of both halves; two warps fill one staging tile of 64 columns, and the first of them stores it.
     const int ew = warp - 2, q = warp & 3, box = ew >> 2;
     const int pair = q + 4 * (box >> 1), side = box & 1;
@@ -305,65 +440,68 @@ __global__ void __launch_bounds__(kBlock, 1)
     const uint32_t stg_base = stg0 + pair * C::kStgPair;
     const int64_t bias_half = static_cast<int64_t>(blocks) * P.b;
     uint32_t ut = 0, sti = 0;
+    int bias_blk = -1;
+    float bg = 0.f, bu = 0.f;  // batch-last: the biases of this lane's row, loaded when the block changes
     for (uint32_t row = row_begin; row < row_end; ++row, ++ut) {
       const int blk = static_cast<int>(row / P.tiles_n);
       const int n0 = static_cast<int>(row % P.tiles_n) * 128;
       const int i = blk / d, l = blk % d;
       const uint32_t buf = ut & 1u, bph = (ut >> 1) & 1u;
+      const int row_limit = OUT_LAST ? P.b - j0 : static_cast<int>(min(P.batch - n0, static_cast<int64_t>(128)));
+      const int col_limit = OUT_LAST ? static_cast<int>(min(P.batch - n0, static_cast<int64_t>(kNT))) : P.b - j0;
+      if (OUT_LAST && !SUM && P.bias != nullptr && blk != bias_blk) {
+        if (q * 32 + lane < row_limit) {
+          const int64_t at = (static_cast<int64_t>(i) * P.b + j0 + q * 32 + lane) * d + l;
+          bg = bias_at(P.bias, at, P.dtype);
+          bu = bias_at(P.bias, at + bias_half, P.dtype);
+        }
+        bias_blk = blk;
+      }
       int got = 1;
       if (lane == 0) got = mbar_wait<64>(tfull_bar(buf), bph, abort_flag, P.status, kGatedWaits + 5) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
       if (!got) break;
       tc_fence_after();
-      const int row_limit = OUT_LAST ? P.b - j0 : static_cast<int>(min(P.batch - n0, static_cast<int64_t>(128)));
-      const int col_limit = OUT_LAST ? static_cast<int>(min(P.batch - n0, static_cast<int64_t>(kNT))) : P.b - j0;
       const int col0 = (box >> 1) * 64;     // of the pair's staging tile
       const bool active = q * 32 < row_limit && col0 < col_limit;  // (the same for both warps of a pair)
-      uint32_t g[32], u[32];
-      if (active) {
-        const uint32_t t0 = tmem_base + lane_addr + buf * 2 * kNT + box * 32;
-        tmem_ld32(t0, g);
-        if constexpr (!SUM) tmem_ld32(t0 + kNT, u);
-        tmem_ld_wait();
-      }
-      // the accumulators are in registers: hand them back
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tempty_bar(buf));
-      if (!active) continue;
-      if (!SUM && P.bias != nullptr) {
-        if constexpr (OUT_LAST) {
-          float bg = 0.f, bu = 0.f;
-          if (q * 32 + lane < row_limit) {
-            const int64_t at = (static_cast<int64_t>(i) * P.b + j0 + q * 32 + lane) * d + l;
-            bg = bias_at(P.bias, at, P.dtype);
-            bu = bias_at(P.bias, at + bias_half, P.dtype);
-          }
-          const uint64_t b2 = pack_f2(bg, bg), c2 = pack_f2(bu, bu);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float y0, y1;
-            unpack_f2(add_f2(pack_f2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), b2), y0, y1);
-            g[e] = __float_as_uint(y0); g[e + 1] = __float_as_uint(y1);
-            unpack_f2(add_f2(pack_f2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), c2), y0, y1);
-            u[e] = __float_as_uint(y0); u[e + 1] = __float_as_uint(y1);
-          }
-        } else {
-          const int64_t at = static_cast<int64_t>(i) * P.b + j0 + box * 32;
-          add_column_bias(g, P.bias, at, col_limit - box * 32, P.dtype);
-          add_column_bias(u, P.bias, bias_half + at, col_limit - box * 32, P.dtype);
+      const uint32_t t0 = tmem_base + lane_addr + buf * 2 * kNT + box * 32;
+      // the accumulators have been read: hand them back
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) arrive_at(lead(tempty_bar(buf)));
+          else mbar_arrive(tempty_bar(buf));
         }
+      };
+      if (!active) {
+        release();
+        continue;
       }
+      // 16 columns from s * 16 on of either half, with its bias
+      auto take_g = [&](uint32_t (&r)[16], int s) {
+        if (SUM || P.bias == nullptr) return;
+        if constexpr (OUT_LAST) add_row_bias(r, bg);
+        else add_column_bias(r, P.bias, static_cast<int64_t>(i) * P.b + j0 + box * 32 + s * 16, col_limit - box * 32 - s * 16, P.dtype);
+      };
+      auto take_u = [&](uint32_t (&r)[16], int s) {
+        if (P.bias == nullptr) return;
+        if constexpr (OUT_LAST) add_row_bias(r, bu);
+        else add_column_bias(r, P.bias, bias_half + static_cast<int64_t>(i) * P.b + j0 + box * 32 + s * 16,
+                             col_limit - box * 32 - s * 16, P.dtype);
+      };
       uint32_t stg = 0;
-      // 32 values of each row into the pair's next staging tile, once the store that used it last has read it
-      auto fill = [&](const uint32_t (&w)[16]) {
+      // the pair's next staging tile, once the store that used it last has read it
+      auto next_tile = [&]() {
         stg = stg_base + (STGN > 1 ? sti * 4096u : 0u);
         if (STGN > 1) sti = (sti + 1 == STGN) ? 0u : sti + 1;
         if (side == 0 && lane == 0) bulk_wait_read<STGN - 1>();
         bar_sync_named(1 + pair, 64);
+      };
+      auto fill = [&](const uint32_t (&w)[8], int s) {
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128 + (((side * 4 + ch) ^ (lane & 7)) << 4)),
+        for (int ch = 0; ch < 2; ++ch)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * 128 + (((side * 4 + s * 2 + ch) ^ (lane & 7)) << 4)),
                        "r"(w[4 * ch]), "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
                        : "memory");
       };
@@ -376,37 +514,58 @@ __global__ void __launch_bounds__(kBlock, 1)
           bulk_commit();
         }
       };
-      uint32_t w[16];
       if constexpr (KEEP) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          next_tile();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
-        fill(w);
-        send(&tmH, 0);
+          for (int s = 0; s < 2; ++s) {
+            uint32_t r[16], w[8];
+            tmem_ld16(t0 + half * kNT + s * 16, r);
+            tmem_ld_wait();
+            if (half) take_u(r, s);
+            else take_g(r, s);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]), P.dtype);
-        fill(w);
-        send(&tmH, 1);
-      }
-      if constexpr (SUM) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
-      } else {
-        switch (P.act) {
-          case KSMM_ACT_SILU: gate_32<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
-          case KSMM_ACT_GELU: gate_32<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
-          case KSMM_ACT_SIGMOID: gate_32<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
-          case KSMM_ACT_RELU: gate_32<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
-          default: gate_32<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+            for (int e = 0; e < 8; ++e) w[e] = pack2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]), P.dtype);
+            fill(w, s);
+          }
+          send(&tmH, half);
         }
       }
-      fill(w);
+      next_tile();
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint32_t g[16], w[8];
+        tmem_ld16(t0 + s * 16, g);
+        if constexpr (SUM) {
+          tmem_ld_wait();
+          if (s == 1) release();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), P.dtype);
+        } else {
+          uint32_t u[16];
+          tmem_ld16(t0 + kNT + s * 16, u);
+          tmem_ld_wait();
+          if (s == 1) release();
+          take_g(g, s);
+          take_u(u, s);
+          switch (P.act) {
+            case KSMM_ACT_SILU: gate_16<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
+            case KSMM_ACT_GELU: gate_16<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
+            case KSMM_ACT_SIGMOID: gate_16<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
+            case KSMM_ACT_RELU: gate_16<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
+            default: gate_16<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+          }
+        }
+        fill(w, s);
+      }
       if (OUT_LAST && P.y_direct) {
         // each warp of the pair stores half of the tile's rows
         bar_sync_named(1 + pair, 64);
         uint8_t* yrow = static_cast<uint8_t*>(P.y) +
                         (((static_cast<int64_t>(i) * P.b + j0 + q * 32) * d + l) * P.y_ld + n0 + col0) * 2;
-        store_rows<2>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * 2, min(32, row_limit - q * 32), col_limit - col0, lane,
-                      16 * side, 16 * side + 16);
+        store_rows<2, 8>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * 2, min(32, row_limit - q * 32), col_limit - col0, lane,
+                         16 * side, 16 * side + 16);
       } else {
         send(&tmY, 0);
       }
@@ -418,6 +577,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   // ===================== teardown =====================
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other's MMAs or arrivals reach its shared memory
   if (*abort_flag) {
     // copies that may still be in flight land before the shared memory is handed on
     __nanosleep(20000);
@@ -425,15 +585,16 @@ __global__ void __launch_bounds__(kBlock, 1)
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (PAIR) pair_tmem_dealloc(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
-template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE>
+template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE, bool PAIR = false>
 int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
-  using C = Cfg<WRES, NWC, SX, STGN>;
+  using C = Cfg<WRES, NWC, SX, STGN, PAIR>;
   constexpr bool KEEP = MODE == kKeep;
-  auto kern = gated_kernel<IN_LAST, OUT_LAST, WRES, NWC, SX, STGN, MODE>;
+  auto kern = gated_kernel<IN_LAST, OUT_LAST, WRES, NWC, SX, STGN, MODE, PAIR>;
   static std::atomic<bool> attr_set[64];  // once per device (a repeated set is harmless)
   int dev = 0;
   cudaGetDevice(&dev);
@@ -457,7 +618,7 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
     if ((st = encode_map(&tmX, p.in_dtype, 4, p.in, dims, str, box)) != KSMM_OK) return st;
   } else {
     const uint64_t dims[3] = {c, a, GX * B}, str[3] = {1, c, a * c};
-    const uint32_t box[3] = {kKC, 1, 128};
+    const uint32_t box[3] = {kKC, 1, PAIR ? 64 : 128};
     if ((st = encode_map(&tmX, p.in_dtype, 3, p.in, dims, str, box)) != KSMM_OK) return st;
   }
   Params P = {};
@@ -489,10 +650,32 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
   const uint32_t fmt = p.in_dtype == KSMM_BF16 ? 1u : 0u;
   const uint32_t a_mn = (OUT_LAST || IN_LAST) ? 1u : 0u, b_mn = (!OUT_LAST || IN_LAST) ? 1u : 0u;
   P.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) | (static_cast<uint32_t>(kNT >> 3) << 17) |
-            (static_cast<uint32_t>(128 >> 4) << 24);
+            (static_cast<uint32_t>((PAIR ? 256 : 128) >> 4) << 24);
   P.tiles_n = static_cast<int>((B + 127) / 128);
-  P.tiles_j = static_cast<int>((b + 127) / 128);
-  const int sms = num_sms();
+  P.tiles_j = static_cast<int>((b + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
+  int sms = num_sms();  // CTAs, or pairs, at the same time
+  if constexpr (PAIR) {
+    // A pair needs the two SMs of one TPC; ask how many there are rather than run a last pair on its own
+    static std::atomic<int> pairs[64];
+    int n = dev >= 0 && dev < 64 ? pairs[dev].load(std::memory_order_relaxed) : 0;
+    if (!n) {
+      cudaLaunchConfig_t q = {};
+      q.gridDim = dim3(2);
+      q.blockDim = dim3(kBlock);
+      q.dynamicSmemBytes = C::kSmem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = 2;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      q.attrs = at;
+      q.numAttrs = 1;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &q);
+      if (e != cudaSuccess || n <= 0)
+        return set_error(KSMM_ERR_CUDA, "cannot place pairs of CTAs: %s", cudaGetErrorString(e));
+      if (dev >= 0 && dev < 64) pairs[dev].store(n, std::memory_order_relaxed);
+    }
+    sms = n;
+  }
   if (sms <= 0) return set_error(KSMM_ERR_NO_DEVICE, "no CUDA device");
   const int64_t rows = static_cast<int64_t>(P.tiles_n) * p.a * p.d;
   if (rows <= 0 || rows > 0x7fffffffLL || P.tiles_j > sms)
@@ -501,26 +684,56 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
   P.rows = static_cast<uint32_t>(rows);
   const int64_t groups = std::min<int64_t>(sms / P.tiles_j, rows);
   P.row_groups = static_cast<uint32_t>(groups);
-  cudaError_t err = launch_pdl(kern, static_cast<unsigned>(groups * P.tiles_j), kBlock, C::kSmem, stream, tmX, tmW, tmY, tmH, P);
+  cudaError_t err;
+  if constexpr (PAIR) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(groups * P.tiles_j * 2));
+    cfg.blockDim = dim3(kBlock);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    err = cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmY, tmH, P);
+  } else {
+    err = launch_pdl(kern, static_cast<unsigned>(groups * P.tiles_j), kBlock, C::kSmem, stream, tmX, tmW, tmY, tmH, P);
+  }
   count_launch();
   if (err == cudaSuccess) err = cudaGetLastError();
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "gated kernel launch failed: %s", cudaGetErrorString(err));
   return KSMM_OK;
 }
 
+// Two CTAs per tile where there are two feature tiles for them and rows enough to keep the MMAs busy
+bool use_pair(const Problem& p) { return p.c <= 3 * kKC && p.b > 128 && p.batch >= 2048; }
+
 template <bool IN_LAST, bool OUT_LAST>
 int launch_layout(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+  if constexpr (OUT_LAST) {
+    if (use_pair(p))
+      return halves ? launch<IN_LAST, true, true, 3, 4, 2, kKeep, true>(p, halves, halves_ld, stream)
+                    : launch<IN_LAST, true, true, 3, 6, 1, kProduct, true>(p, halves, halves_ld, stream);
+  }
   if (p.c <= 3 * kKC)
-    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 4, 2, kKeep>(p, halves, halves_ld, stream)
-                  : launch<IN_LAST, OUT_LAST, true, 3, 6, 1, kProduct>(p, halves, halves_ld, stream);
-  return halves ? launch<IN_LAST, OUT_LAST, false, 0, 4, 2, kKeep>(p, halves, halves_ld, stream)
-                : launch<IN_LAST, OUT_LAST, false, 0, 5, 1, kProduct>(p, halves, halves_ld, stream);
+    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 2, 2, kKeep>(p, halves, halves_ld, stream)
+                  : launch<IN_LAST, OUT_LAST, true, 3, 3, 1, kProduct>(p, halves, halves_ld, stream);
+  if constexpr (IN_LAST && OUT_LAST) {
+    return halves ? launch<true, true, false, 0, 2, 2, kKeep>(p, halves, halves_ld, stream)
+                  : launch<true, true, false, 0, 2, 1, kProduct>(p, halves, halves_ld, stream);
+  }
+  return set_error(KSMM_ERR_UNSUPPORTED, "gated kernel: blocks longer than %d keep the batch-last layout", 3 * kKC);
 }
 
 template <bool OUT_LAST>
 int launch_sum(const Problem& p, cudaStream_t stream) {
-  return p.c <= 3 * kKC ? launch<true, OUT_LAST, true, 3, 6, 1, kSum>(p, nullptr, 0, stream)
-                        : launch<true, OUT_LAST, false, 0, 5, 1, kSum>(p, nullptr, 0, stream);
+  if (p.c <= 3 * kKC) return launch<true, OUT_LAST, true, 3, 3, 1, kSum>(p, nullptr, 0, stream);
+  if constexpr (OUT_LAST) return launch<true, true, false, 0, 2, 1, kSum>(p, nullptr, 0, stream);
+  return set_error(KSMM_ERR_UNSUPPORTED, "gated kernel: blocks longer than %d keep the batch-last layout", 3 * kKC);
 }
 
 }  // namespace
@@ -530,7 +743,8 @@ bool tc_gated_fits(const int32_t* q, int64_t batch, int dtype, int in_last, int 
   if (dtype != KSMM_F16 && dtype != KSMM_BF16) return false;
   // (smaller blocks are bandwidth problems that the register-tiled kernels serve more tightly)
   if (q[1] < 32 || q[2] < 16 || q[1] % 8 != 0 || q[1] > 16384) return false;
-  if ((!in_last || !out_last) && (q[3] != 1 || q[2] % 8 != 0)) return false;
+  // (longer blocks stream their weights, in one layout only)
+  if ((!in_last || !out_last) && (q[3] != 1 || q[2] % 8 != 0 || q[2] > 3 * tc::kKC)) return false;
   return batch > 0 && batch <= 0x3fffffffLL && static_cast<int64_t>(q[0]) * q[3] <= 0x3fffffffLL;
 }
 
