@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(256)
 // The backward with the sums of its lines (features of a batch-last tensor), which are the gradients of the biases:
 // a block per line.  Against a pass of its own over dg and du, 2 x 2048 x 12544 bf16: 21 us saved.
 template <typename T, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
     gate_lines_kernel(const T* __restrict__ gu, int64_t ld, const T* __restrict__ dh, int64_t h_ld, T* __restrict__ out,
                       int64_t half, int64_t out_half, int64_t len, int act, T* __restrict__ bias_grad) {
   using Sum = typename std::conditional<sizeof(T) == 4, double, float>::type;  // (a thread's share of a long line)

@@ -750,33 +750,36 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_kernel(const Args
   const T* x = static_cast<const T*>(A.x) + tok;
   const T* y = A.y ? static_cast<const T*>(A.y) + tok : nullptr;
   const float inv = 1.f / static_cast<float>(A.C);
-  const int last = A.C - 1;
   for (int c = threadIdx.x; c < A.C; c += kColWarps * 32) coef[c] = combined<T>(A, sample, c);
   __syncthreads();
-  // calls f(c, p[c], q[c]) for the warp's channels, loads of a step ahead of their uses
+  const int64_t step = kColWarps * A.rows;  // elements between a warp's channels
+  // calls f(c, o, p[o], q[o]) for the warp's channels, o = c * rows, loads of a step ahead of their uses
   auto walk = [&](const T* p, const T* q, auto&& f) {
-    for (int c0 = warp; c0 < A.C; c0 += kColWarps * kColStep) {
+    int c = warp;
+    int64_t o = c * A.rows;
+    for (; c + (kColStep - 1) * kColWarps < A.C; c += kColStep * kColWarps, o += kColStep * step) {
       T a[kColStep], b[kColStep];
 #pragma unroll
       for (int u = 0; u < kColStep; ++u) {
-        const int64_t at = static_cast<int64_t>(min(c0 + u * kColWarps, last)) * A.rows;
-        a[u] = p[at];
-        if (q) b[u] = q[at];
+        a[u] = p[o + u * step];
+        if (q) b[u] = q[o + u * step];
       }
 #pragma unroll
       for (int u = 0; u < kColStep; ++u)
-        if (c0 + u * kColWarps < A.C) f(c0 + u * kColWarps, ElemTraits<T>::to_float(a[u]), q ? ElemTraits<T>::to_float(b[u]) : 0.f);
+        f(c + u * kColWarps, o + u * step, ElemTraits<T>::to_float(a[u]), q ? ElemTraits<T>::to_float(b[u]) : 0.f);
     }
+#pragma unroll 4
+    for (; c < A.C; c += kColWarps, o += step) f(c, o, ElemTraits<T>::to_float(p[o]), q ? ElemTraits<T>::to_float(q[o]) : 0.f);
   };
   float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
   if (y && A.post != kNone) {
     float s = 0.f;
     if (A.post == kLayer) {
-      walk(y, nullptr, [&](int, float v, float) { s += v; });
+      walk(y, nullptr, [&](int, int64_t, float v, float) { s += v; });
       st.z = column_sum(s, red) * inv;
       s = 0.f;
     }
-    walk(y, nullptr, [&](int, float v, float) { s = fmaf(v - st.z, v - st.z, s); });
+    walk(y, nullptr, [&](int, int64_t, float v, float) { s = fmaf(v - st.z, v - st.z, s); });
     st.w = rsqrtf(column_sum(s, red) * inv + A.eps);
   }
   auto join = [&](int c, float xv, float yv) {
@@ -786,29 +789,32 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_kernel(const Args
   };
   // z of every channel, to shared memory and (where there is a y) to memory, and its sum
   float s = 0.f;
-  walk(x, y, [&](int c, float xv, float yv) {
+  T* const zo = static_cast<T*>(A.z) + tok;
+  T* const ho = static_cast<T*>(A.h) + tok;
+  walk(x, y, [&](int c, int64_t o, float xv, float yv) {
     const float z = join(c, xv, yv);
     s += z;
     if (CACHE) zc[c * 32 + lane] = z;
-    if (y && live) static_cast<T*>(A.z)[c * A.rows + tok] = ElemTraits<T>::from_float(z);
+    if (y && live) zo[o] = ElemTraits<T>::from_float(z);
   });
   if (A.pre != kNone) {
     auto again = [&](auto&& f) {
       if constexpr (CACHE) {  // (a thread reads what it has written)
-#pragma unroll 4
-        for (int c = warp; c < A.C; c += kColWarps) f(c, zc[c * 32 + lane]);
+        int64_t o = warp * A.rows;
+#pragma unroll 8
+        for (int c = warp; c < A.C; c += kColWarps, o += step) f(c, o, zc[c * 32 + lane]);
       } else {
-        walk(x, y, [&](int c, float xv, float yv) { f(c, join(c, xv, yv)); });
+        walk(x, y, [&](int c, int64_t o, float xv, float yv) { f(c, o, join(c, xv, yv)); });
       }
     };
     if (A.pre == kLayer) st.x = column_sum(s, red) * inv;
     float v = 0.f;
-    again([&](int, float z) { v = fmaf(z - st.x, z - st.x, v); });
+    again([&](int, int64_t, float z) { v = fmaf(z - st.x, z - st.x, v); });
     st.y = rsqrtf(column_sum(v, red) * inv + A.eps);
     if (live)
-      again([&](int c, float z) {
+      again([&](int c, int64_t o, float z) {
         const float4 q = coef[c];
-        static_cast<T*>(A.h)[c * A.rows + tok] = ElemTraits<T>::from_float(fmaf((z - st.x) * st.y, q.z, q.w));
+        ho[o] = ElemTraits<T>::from_float(fmaf((z - st.x) * st.y, q.z, q.w));
       });
   }
   if (live && A.stats && warp == 0) A.stats[tok] = st;

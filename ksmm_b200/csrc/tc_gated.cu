@@ -70,13 +70,6 @@ struct Cfg {
   static_assert(8 * (2 * SX + 6) + 8 <= kBarBytes, "barrier area");
 };
 
-// one lane of a warp that has converged
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-
 // ---- two CTAs of a cluster ----
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -368,9 +361,8 @@ __global__ void __launch_bounds__(kBlock, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ===================== MMA issuer =====================
-    // The whole warp walks the loop, so that descriptors stay in uniform registers, and one elected lane issues.  With
-    // the loop inside `if (lane == 0)` an MMA's operands moved there one by one, and the issuing thread took 640
-    // cycles per 64 of k where the MMAs take 256: 25088 rows of (1,512,192,4),
+    // (elect_one: with the loop in one lane the issuing thread took 640 cycles per 64 of k where the MMAs take 256.)
+    // 25088 rows of (1,512,192,4),
     // batch-last: 70 -> 59 us, with both halves' chunks in one ring stage 54, by pairs 44.
     if (rank == 0) {
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);

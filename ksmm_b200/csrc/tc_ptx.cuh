@@ -198,6 +198,15 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
+// One lane of a warp that has converged.  A warp that issues MMAs walks its loop as a whole and lets this lane
+// issue: inside `if (lane == 0)` the compiler cannot keep descriptors in uniform registers, and moving an MMA's
+// operands there one by one costs the issuing thread more time than an MMA with N = 128 takes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 template <int ES>
 __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
                                      uint32_t idesc, uint32_t accumulate) {
