@@ -449,6 +449,11 @@ py::object layer_train(const at::Tensor& x, const std::vector<at::Tensor>& facto
   return py::cast(out);
 }
 
+// A backward pass that is to be differentiated again would come back as a constant.
+void differentiable_once() {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "this operator is differentiable once (create_graph=True)");
+}
+
 // a gated layer without gradients
 bool gated_fits(const at::Tensor& x, const std::vector<at::Tensor>& factors, const Patterns& p, bool last,
                 const c10::optional<at::Tensor>& bias) {
@@ -533,6 +538,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    differentiable_once();
     const auto kept = ctx->get_saved_variables();
     const std::vector<int64_t> meta = ctx->saved_data["gated"].toIntVector();
     const int n = static_cast<int>(meta[0]);
@@ -710,6 +716,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    differentiable_once();
     const auto kept = ctx->get_saved_variables();
     const std::vector<int64_t> ints = ctx->saved_data["ints"].toIntVector();
     const at::Tensor& z = kept[0];

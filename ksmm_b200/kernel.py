@@ -322,6 +322,12 @@ def grouped_chain_forward(input, stacked_factors, patterns, bs_last, groups, bia
     return out
 
 
+def differentiable_once():
+    """For backward passes: one that is to be differentiated again would come back as a constant."""
+    if torch.is_grad_enabled():
+        raise NotImplementedError("this operator is differentiable once (create_graph=True)")
+
+
 def _gated_desc(input, stacked_factors, patterns, bs_last, out_last, bias, activation):
     """Checks the arguments of a gated call; returns its descriptor and (batch, out features, dtype code)."""
     bs_last = int(bool(bs_last))
@@ -405,8 +411,8 @@ class GatedFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
+        differentiable_once()
         input, saved, *factors = ctx.saved_tensors
         bs_last, out_last, patterns, activation, layouts, need, bias_shape = ctx.gated
         desc, _ = _gated_desc(input, factors, patterns, bs_last, out_last, None, activation)

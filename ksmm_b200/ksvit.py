@@ -12,6 +12,10 @@ benchmark/ksvit_time.py:167-229).  Architecture: 224x224 images, 16x16 patches
 
     fc1 = KSLinear([(4,192,192,1), (1,768,192,4)])   768 -> 3072
     fc2 = KSLinear([(1,192,768,4), (4,192,192,1)])   3072 -> 768
+
+``KSViTB(gated_mlp=True)`` is the same network with gated feed-forward blocks (SwiGLU), 768 -> 2048 -> 768:
+the attention's output joins the stream and is normalised in one kernel (``ResidualNorm``), gate and up
+projection are one layer (``KSGatedLinear``).
 """
 from __future__ import annotations
 
@@ -19,10 +23,13 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .interface import KSLinear
+from .interface import KSGatedLinear, KSLinear
+from .norm import ResidualNorm
 
 FC1_PATTERNS = [(4, 192, 192, 1), (1, 768, 192, 4)]
 FC2_PATTERNS = [(1, 192, 768, 4), (4, 192, 192, 1)]
+GATE_PATTERNS = [(4, 192, 192, 1), (1, 512, 192, 4)]
+DOWN_PATTERNS = [(1, 192, 512, 4), (4, 192, 192, 1)]
 
 
 def posemb_sincos_2d(h, w, dim, temperature=10000.0):
@@ -73,6 +80,27 @@ class KSFeedForward(nn.Module):
         return y.view(x.shape) if self.layout_plan else y
 
 
+class KSGatedFeedForward(nn.Module):
+    """``z = x + a``, ``z + down(silu(gate(n)) * up(n))`` with ``n = norm(z)``: a block's second half from the residual
+    stream ``x`` and the attention's output ``a``.  The 2048 wide activations between the layers are batch-last
+    (see KSFeedForward); without gradients the last sum is formed inside the down projection's last kernel."""
+
+    def __init__(self, dtype, device, norm="layer", requires_grad=False):
+        super().__init__()
+        kw = dict(algo="kernel", dtype=dtype, device=device, requires_grad=requires_grad)
+        self.gate_up = KSGatedLinear(GATE_PATTERNS, bias=True, bs_last=False, out_bs_last=True, activation="silu", **kw)
+        # (a trainable layer that changes the layout transposes in a pass of its own, as it keeps one inside)
+        self.down = KSLinear(DOWN_PATTERNS, bias=True, bs_last=True, out_bs_last=False, **kw)
+        self.norm = ResidualNorm(self.gate_up.in_size, norm=norm, dtype=dtype, device=device, requires_grad=requires_grad)
+
+    def forward(self, x, a):
+        z, n = self.norm(x, a)
+        h = self.gate_up(n)
+        if torch.is_grad_enabled() and (h.requires_grad or self.down.factors[0].requires_grad):
+            return self.down(h).view(z.shape) + z
+        return self.down(h, residual=z).view(z.shape)
+
+
 class Attention(nn.Module):
     def __init__(self, dim, heads=12, dim_head=64):
         super().__init__()
@@ -90,14 +118,18 @@ class Attention(nn.Module):
 
 class KSViTB(nn.Module):
     def __init__(self, dtype=torch.float16, device="cuda", depth=12, dim=768, num_classes=1000,
-                 dense_mlp=False, fuse_gelu=True, layout_plan=True, fuse_residual=False):
+                 dense_mlp=False, fuse_gelu=True, layout_plan=True, fuse_residual=False, gated_mlp=False):
         super().__init__()
+        if gated_mlp and (dense_mlp or dim != 768):
+            raise ValueError("gated feed-forward blocks are Kronecker-sparse and 768 wide")
+        self.gated_mlp = gated_mlp
         self.patch = 16
         patch_dim = 3 * 16 * 16
         self.embed = nn.Sequential(nn.LayerNorm(patch_dim), nn.Linear(patch_dim, dim), nn.LayerNorm(dim))
         self.register_buffer("pos", posemb_sincos_2d(14, 14, dim), persistent=False)
         self.layers = nn.ModuleList(
-            [nn.ModuleList([Attention(dim), KSFeedForward(dim, dtype, device, dense_mlp, fuse_gelu, layout_plan)])
+            [nn.ModuleList([Attention(dim), KSGatedFeedForward(dtype, device) if gated_mlp
+                            else KSFeedForward(dim, dtype, device, dense_mlp, fuse_gelu, layout_plan)])
              for _ in range(depth)])
         self.norm = nn.LayerNorm(dim)
         self.head = nn.Linear(dim, num_classes)
@@ -114,6 +146,9 @@ class KSViTB(nn.Module):
         x = img.view(b, c, h // p, p, w // p, p).permute(0, 2, 4, 3, 5, 1).reshape(b, -1, p * p * c)
         x = self.embed(x) + self.pos
         for attn, ff in self.layers:
+            if self.gated_mlp:
+                x = ff(x, attn(x))
+                continue
             x = attn(x) + x
             x = ff(x, add_residual=True) if self.fuse_residual else ff(x) + x
         return self.head(self.norm(x).mean(dim=1))

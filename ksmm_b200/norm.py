@@ -10,11 +10,10 @@ import ctypes
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import native as _native
-from .kernel import _result, _stream_ptr, dtype_code
+from .kernel import _result, _stream_ptr, differentiable_once, dtype_code
 
 _ROWS = ("weight", "bias", "post_weight", "post_bias")
 _PER_SAMPLE = ("scale", "shift", "gate")
@@ -122,8 +121,8 @@ class NormFunction(torch.autograd.Function):
         return (h,) if z is None else (z,) if h is None else (z, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
+        differentiable_once()
         z, y, stats, *params = ctx.saved_tensors
         sizes, kinds = ctx.plan
         grad_z = grads[0] if y is not None else None
