@@ -426,7 +426,8 @@ KSMM_API int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* g
  * ksmm_cu_norm_backward reads grad_z and / or grad_h, the forward's x or z, y and stats, and the
  * parameters; writes those of grad_* that are not NULL: grad_x and grad_y laid out as x and y, the others
  * contiguous rows of param_dtype (grad_scale, grad_shift, grad_gate: `samples` rows where their stride is not 0).
- * Its sums over tokens have a fixed order.  Up to 8192 channels; outputs overlap no input.
+ * Its sums over tokens have a fixed order.  Workspaces of the sizes that the two ..._workspace_bytes calls give
+ * (often 0), aligned to 16 bytes as stats is.  Up to 8192 channels; outputs overlap no input.
  */
 typedef enum { KSMM_NORM_NONE = 0, KSMM_NORM_LAYER = 1, KSMM_NORM_RMS = 2 } ksmm_norm_t;
 
@@ -464,7 +465,8 @@ typedef struct {
   void* grad_gate;
 } ksmm_norm_desc_t;
 
-KSMM_API int ksmm_cu_norm_forward(const ksmm_norm_desc_t* desc, void* stream);
+KSMM_API size_t ksmm_cu_norm_forward_workspace_bytes(const ksmm_norm_desc_t* desc);
+KSMM_API int ksmm_cu_norm_forward(const ksmm_norm_desc_t* desc, void* workspace, size_t workspace_bytes, void* stream);
 KSMM_API size_t ksmm_cu_norm_backward_workspace_bytes(const ksmm_norm_desc_t* desc);
 KSMM_API int ksmm_cu_norm_backward(const ksmm_norm_desc_t* desc, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -48,7 +48,7 @@ EXPORTS = (
     "ksmm_cu_chain_train_bytes", "ksmm_cu_chain_train_forward", "ksmm_cu_chain_backward",
     "ksmm_cu_chain_fp8_workspace_bytes", "ksmm_cu_chain_forward_fp8",
     "ksmm_cu_gated_workspace_bytes", "ksmm_cu_gated_train_bytes", "ksmm_cu_gated_forward", "ksmm_cu_gated_backward",
-    "ksmm_cu_norm_forward", "ksmm_cu_norm_backward_workspace_bytes", "ksmm_cu_norm_backward",
+    "ksmm_cu_norm_forward_workspace_bytes", "ksmm_cu_norm_forward", "ksmm_cu_norm_backward_workspace_bytes", "ksmm_cu_norm_backward",
 )
 
 
@@ -207,7 +207,9 @@ def load():
     lib.ksmm_cu_gated_backward.restype = i32
     lib.ksmm_cu_gated_backward.argtypes = [ctypes.POINTER(GatedDesc), vp, vp, pvp, vp, vp]
     lib.ksmm_cu_norm_forward.restype = i32
-    lib.ksmm_cu_norm_forward.argtypes = [ctypes.POINTER(NormDesc), vp]
+    lib.ksmm_cu_norm_forward.argtypes = [ctypes.POINTER(NormDesc), vp, ctypes.c_size_t, vp]
+    lib.ksmm_cu_norm_forward_workspace_bytes.restype = ctypes.c_size_t
+    lib.ksmm_cu_norm_forward_workspace_bytes.argtypes = [ctypes.POINTER(NormDesc)]
     lib.ksmm_cu_norm_backward_workspace_bytes.restype = ctypes.c_size_t
     lib.ksmm_cu_norm_backward_workspace_bytes.argtypes = [ctypes.POINTER(NormDesc)]
     lib.ksmm_cu_norm_backward.restype = i32

@@ -1885,6 +1885,13 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
       if (plan.out_last[f]) p.out_ld = ld;
     }
     p.no_alloc = 1;
+    // The fp32 tensor-core kernel takes batches of whole pieces.  Between padded buffers the padding goes through it
+    // as well (a column's sums never meet another's): 3902 rows 768 -> 2048 146 us against 263 by the FFMA kernel.
+    if (D.dtype == KSMM_F32 && !keep && p.in_ld == ld && p.out_ld == ld && ld != batch && plan.in_last[f] && plan.out_last[f] &&
+        !(last && fuse)) {
+      p.batch = ld;
+      p.in_ld = p.out_ld = 0;
+    }
     if (last && fuse) {
       p.out = plan.post ? h2 : static_cast<char*>(D.output);
       if (L && ld != batch) p.out_ld = plan.post ? ld : batch;

@@ -27,6 +27,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "backward.h"
 #include "common.cuh"
 #include "norm.h"
 #include "tc_epilogue.cuh"
@@ -735,13 +736,13 @@ __device__ __forceinline__ float column_sum(float v, float* red) {
   return s;
 }
 
-// With CACHE z stays in shared memory (128 bytes per channel, up to 1536 of them); without, it is formed again
-// for each statistic, from x and y in the L2 cache.  Every thread has 16 to 32 loads in flight: the block's latencies
-// are what bounds it (768 x 6501 fp16: 93 us when the loads waited for one another).
+// z stays in shared memory (128 bytes per channel, up to 1536 of them).  Every thread has 16 to 32 loads in flight:
+// the block's latencies are what bounds it (768 x 6501 fp16, 40 MB: 93 us when every statistic read the tensors
+// again and the loads waited for one another, 25 now; floor 6).
 constexpr int kColStep = 16;  // channels that a warp loads at once
-constexpr int kCacheChannels = 1536;
+constexpr int kColumnChannels = 1536;
 
-template <typename T, bool CACHE>
+template <typename T>
 __global__ void __launch_bounds__(kColWarps * 32) norm_columns_kernel(const Args A) {
   __shared__ float red[kColWarps * 32];
   extern __shared__ float4 coef[];  // combined parameters of the channels, then z
@@ -798,18 +799,14 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_kernel(const Args
   walk(x, y, [&](int c, int64_t o, float xv, float yv) {
     const float z = join(c, xv, yv);
     s += z;
-    if (CACHE) zc[c * 32 + lane] = z;
+    zc[c * 32 + lane] = z;
     if (y && live) zo[o] = ElemTraits<T>::from_float(z);
   });
   if (A.pre != kNone) {
-    auto again = [&](auto&& f) {
-      if constexpr (CACHE) {  // (a thread reads what it has written)
-        int64_t o = warp * A.rows;
+    auto again = [&](auto&& f) {  // (a thread reads what it has written)
+      int64_t o = warp * A.rows;
 #pragma unroll 8
-        for (int c = warp; c < A.C; c += kColWarps, o += step) f(c, o, zc[c * 32 + lane]);
-      } else {
-        walk(x, y, [&](int c, int64_t o, float xv, float yv) { f(c, o, join(c, xv, yv)); });
-      }
+      for (int c = warp; c < A.C; c += kColWarps, o += step) f(c, o, zc[c * 32 + lane]);
     };
     if (A.pre == kLayer) st.x = column_sum(s, red) * inv;
     float v = 0.f;
@@ -1123,9 +1120,10 @@ int launch_rows(const Args& A, cudaStream_t stream) {
       if (pieces <= 96) return go_rows<T, V, 3, 32, true>(A, stream);
       return go_rows<T, V, 4, 32, true>(A, stream);
     }
-    // (beyond 5461 channels of 16 bits the parameters and two rows for each group do not fit)
-    if (pieces > 128 && pieces <= 512 && A.per_sample >= 24 && A.rows >= 148 * 8)
-      return pieces <= 256 ? go_rows<T, V, 2, 128, true>(A, stream) : go_rows<T, V, 4, 128, true>(A, stream);
+    if (pieces > 128 && pieces <= 1024 && A.per_sample >= 24 && A.rows >= 148 * 8) {
+      if (pieces <= 256) return go_rows<T, V, 2, 128, true>(A, stream);
+      return pieces <= 512 ? go_rows<T, V, 4, 128, true>(A, stream) : go_rows<T, V, 4, 256, true>(A, stream);
+    }
     if (pieces <= 64) return go_rows<T, V, 2, 32>(A, stream);
     if (pieces <= 128) return go_rows<T, V, 4, 32>(A, stream);
     if (pieces <= 256) return go_rows<T, V, 1, 256>(A, stream);
@@ -1174,16 +1172,91 @@ int forward_typed(const ksmm_norm_desc_t& d, cudaStream_t stream) {
   const int64_t chunks = (A.per_sample + 31) / 32;
   if (chunks * A.samples > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many tokens");
   A.chunks = static_cast<int>(chunks);
-  const bool cache = A.C <= kCacheChannels;
-  const size_t smem = static_cast<size_t>(A.C) * (sizeof(float4) + (cache ? 32 * sizeof(float) : 0));
-  static Granted granted[2];
-  auto go = [&](auto kern) {
-    const int st = allow_smem(reinterpret_cast<const void*>(kern), smem, granted[cache]);
-    if (st != KSMM_OK) return st;
-    kern<<<static_cast<unsigned>(chunks * A.samples), kColWarps * 32, smem, stream>>>(A);
-    return launched("norm");
+  const size_t smem = static_cast<size_t>(A.C) * (sizeof(float4) + 32 * sizeof(float));
+  static Granted granted;
+  const int st = allow_smem(reinterpret_cast<const void*>(norm_columns_kernel<T>), smem, granted);
+  if (st != KSMM_OK) return st;
+  norm_columns_kernel<T><<<static_cast<unsigned>(chunks * A.samples), kColWarps * 32, smem, stream>>>(A);
+  return launched("norm");
+}
+
+// Batch-last tensors of more channels than a block keeps: transposed copies, the kernels for rows, transposes back.
+// (4 x 305 tokens of 6950 channels fp32: 229 us by columns that were read again for every statistic, 179 so.)
+bool turned(const ksmm_norm_desc_t& d) { return d.bs_last && d.channels > kColumnChannels; }
+
+size_t tensor_bytes(const ksmm_norm_desc_t& d) {
+  return (static_cast<size_t>(d.rows) * d.channels * dtype_size(d.dtype) + 255) / 256 * 256;
+}
+
+// copies of up to four inputs and two outputs
+size_t turned_bytes(const ksmm_norm_desc_t& d, bool backward) {
+  if (!turned(d)) return 0;
+  int n = backward ? (d.grad_h ? 2 : 0) + (d.grad_z ? 1 : 0) + (d.y ? 1 : 0) + (d.grad_x ? 1 : 0) + (d.grad_y ? 1 : 0)
+                   : 1 + (d.y ? 2 : 0) + (d.norm != kNone ? 1 : 0);
+  return n * tensor_bytes(d);
+}
+
+// `t` with its tensors replaced by transposed copies in `ws`; outputs to turn back in out[]
+struct Turn {
+  ksmm_norm_desc_t t;
+  struct { const void* from; void* to; } out[2];
+  int outs = 0;
+};
+
+int turn_in(const ksmm_norm_desc_t& d, bool backward, char* ws, cudaStream_t stream, Turn* r) {
+  r->t = d;
+  r->t.bs_last = 0;
+  const int es = dtype_size(d.dtype);
+  auto take = [&]() {
+    char* p = ws;
+    ws += tensor_bytes(d);
+    return p;
   };
-  return cache ? go(norm_columns_kernel<T, true>) : go(norm_columns_kernel<T, false>);
+  auto in = [&](const void* src, int* st) -> void* {
+    if (!src || *st != KSMM_OK) return nullptr;
+    void* p = take();
+    *st = launch_transpose(src, p, d.channels, d.rows, es, stream);
+    return p;
+  };
+  auto out = [&](void* dst) -> void* {
+    if (!dst) return nullptr;
+    void* p = take();
+    r->out[r->outs++] = {p, dst};
+    return p;
+  };
+  int st = KSMM_OK;
+  if (!backward) {
+    r->t.x = in(d.x, &st);
+    r->t.y = in(d.y, &st);
+    r->t.z = out(d.y ? d.z : nullptr);
+    r->t.h = out(d.norm != kNone ? d.h : nullptr);
+    return st;
+  }
+  if (d.grad_h) {  // the value that pre normalised
+    void* z = in(d.y ? d.z : d.x, &st);
+    if (d.y) r->t.z = z;
+    else r->t.x = z;
+    r->t.grad_h = in(d.grad_h, &st);
+  }
+  r->t.grad_z = in(d.grad_z, &st);
+  r->t.y = in(d.y, &st);
+  r->t.grad_x = out(d.grad_x);
+  r->t.grad_y = out(d.grad_y);
+  return st;
+}
+
+int turn_out(const ksmm_norm_desc_t& d, const Turn& r, cudaStream_t stream) {
+  for (int q = 0; q < r.outs; ++q) {
+    const int st = launch_transpose(r.out[q].from, r.out[q].to, d.rows, d.channels, dtype_size(d.dtype), stream);
+    if (st != KSMM_OK) return st;
+  }
+  return KSMM_OK;
+}
+
+int forward_any(const ksmm_norm_desc_t& d, cudaStream_t s) {
+  if (d.dtype == KSMM_F32) return forward_typed<float>(d, s);
+  if (d.dtype == KSMM_F16) return forward_typed<__half>(d, s);
+  return forward_typed<__nv_bfloat16>(d, s);
 }
 
 // Tokens of a sample are cut into runs, one block each: 32 columns, or as many runs of rows as blocks fit the SMs
@@ -1191,7 +1264,7 @@ int forward_typed(const ksmm_norm_desc_t& d, cudaStream_t stream) {
 int64_t chunks_of(const ksmm_norm_desc_t& d) {
   const int64_t per = d.samples > 0 ? d.rows / d.samples : 0;
   if (per <= 0) return 1;
-  if (d.bs_last) return (per + 31) / 32;
+  if (d.bs_last && !turned(d)) return (per + 31) / 32;
   const int64_t pieces = (d.channels * dtype_size(d.dtype) + 15) / 16, threads = std::min<int64_t>(512, (pieces + 31) / 32 * 32);
   const int64_t blocks = std::min<int64_t>(8, 65536 / ((threads <= 128 ? 168 : 128) * threads));
   const int64_t want = std::max<int64_t>(1, 148 * blocks / d.samples);
@@ -1270,8 +1343,21 @@ int check_norm(const ksmm_norm_desc_t* d) {
   return KSMM_OK;
 }
 
-size_t norm_workspace(const ksmm_norm_desc_t& d) {
-  return static_cast<size_t>(chunks_of(d) + 1) * d.samples * 4 * d.channels * sizeof(float);
+size_t sums_bytes(const ksmm_norm_desc_t& d) {
+  if (!wants_sums(d)) return 0;
+  return (static_cast<size_t>(chunks_of(d) + 1) * d.samples * 4 * d.channels * sizeof(float) + 255) / 256 * 256;
+}
+
+int backward_any(const ksmm_norm_desc_t& d, void* workspace, cudaStream_t s) {
+  if (d.dtype == KSMM_F32) return backward_typed<float>(d, workspace, s);
+  if (d.dtype == KSMM_F16) return backward_typed<__half>(d, workspace, s);
+  return backward_typed<__nv_bfloat16>(d, workspace, s);
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
+    return set_error(KSMM_ERR_WORKSPACE, "norm: need %zu bytes of workspace aligned to 16, got %zu", need, bytes);
+  return KSMM_OK;
 }
 
 }  // namespace
@@ -1281,19 +1367,28 @@ using namespace ksmm;
 
 extern "C" {
 
-int ksmm_cu_norm_forward(const ksmm_norm_desc_t* d, void* stream) {
+size_t ksmm_cu_norm_forward_workspace_bytes(const ksmm_norm_desc_t* d) {
+  return check_norm(d) != KSMM_OK || d->rows == 0 ? 0 : turned_bytes(*d, false);
+}
+
+int ksmm_cu_norm_forward(const ksmm_norm_desc_t* d, void* workspace, size_t workspace_bytes, void* stream) {
   int st = check_norm(d);
   if (st != KSMM_OK || d->rows == 0) return st;
   if (!d->x || (d->y && !d->z) || (d->norm != kNone && !d->h)) return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
+  if (d->stats && reinterpret_cast<uintptr_t>(d->stats) % 16 != 0)
+    return set_error(KSMM_ERR_BAD_ARGUMENT, "the statistics are aligned to 16 bytes");
+  if ((st = check_workspace(workspace, workspace_bytes, turned_bytes(*d, false))) != KSMM_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d->dtype == KSMM_F32) return forward_typed<float>(*d, s);
-  if (d->dtype == KSMM_F16) return forward_typed<__half>(*d, s);
-  return forward_typed<__nv_bfloat16>(*d, s);
+  if (!turned(*d)) return forward_any(*d, s);
+  Turn r;
+  st = turn_in(*d, false, static_cast<char*>(workspace), s, &r);
+  if (st == KSMM_OK) st = forward_any(r.t, s);
+  return st == KSMM_OK ? turn_out(*d, r, s) : st;
 }
 
 size_t ksmm_cu_norm_backward_workspace_bytes(const ksmm_norm_desc_t* d) {
-  if (check_norm(d) != KSMM_OK || d->rows == 0 || !wants_sums(*d)) return 0;
-  return norm_workspace(*d);
+  if (check_norm(d) != KSMM_OK || d->rows == 0) return 0;
+  return sums_bytes(*d) + turned_bytes(*d, true);
 }
 
 int ksmm_cu_norm_backward(const ksmm_norm_desc_t* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1320,12 +1415,12 @@ int ksmm_cu_norm_backward(const ksmm_norm_desc_t* d, void* workspace, size_t wor
   if (d->grad_z && !d->y) return set_error(KSMM_ERR_BAD_ARGUMENT, "a gradient of z without y");
   if (reinterpret_cast<uintptr_t>(d->stats) % 16 != 0)
     return set_error(KSMM_ERR_BAD_ARGUMENT, "the statistics are aligned to 16 bytes");
-  const size_t need = wants_sums(*d) ? norm_workspace(*d) : 0;
-  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
-    return set_error(KSMM_ERR_WORKSPACE, "norm backward: need %zu bytes aligned to 16, got %zu", need, workspace_bytes);
-  if (d->dtype == KSMM_F32) return backward_typed<float>(*d, workspace, s);
-  if (d->dtype == KSMM_F16) return backward_typed<__half>(*d, workspace, s);
-  return backward_typed<__nv_bfloat16>(*d, workspace, s);
+  if ((st = check_workspace(workspace, workspace_bytes, sums_bytes(*d) + turned_bytes(*d, true))) != KSMM_OK) return st;
+  if (!turned(*d)) return backward_any(*d, workspace, s);
+  Turn r;
+  st = turn_in(*d, true, static_cast<char*>(workspace) + sums_bytes(*d), s, &r);
+  if (st == KSMM_OK) st = backward_any(r.t, workspace, s);
+  return st == KSMM_OK ? turn_out(*d, r, s) : st;
 }
 
 }  // extern "C"

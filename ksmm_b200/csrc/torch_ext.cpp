@@ -687,7 +687,10 @@ int norm_run(const at::Tensor& x, const c10::optional<at::Tensor>& y, const Norm
     *stats = at::empty({c.rows * 4}, o.dtype(at::kFloat));
     d.stats = stats->data_ptr<float>();
   }
-  return ksmm_cu_norm_forward(&d, stream_of(x));
+  at::Tensor ws;
+  const size_t need = c.bs_last ? ksmm_cu_norm_forward_workspace_bytes(&d) : 0;
+  if (need) ws = new_bytes(need, x);
+  return ksmm_cu_norm_forward(&d, need ? ws.data_ptr() : nullptr, need, stream_of(x));
 }
 
 // residual_norm as one autograd node: ksmm_b200.norm.NormFunction without Python in its backward.

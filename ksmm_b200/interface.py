@@ -381,9 +381,13 @@ class KSGatedLinear(nn.Module):
         returns a 2-D tensor."""
         if tensor.dtype != self.dtype:
             raise TypeError(f"input dtype {tensor.dtype} differs from the layer's {self.dtype}")
-        x = (tensor.reshape(tensor.size(0), -1) if self.bs_last else tensor.reshape(-1, tensor.size(-1))).contiguous()
-        y = _k.gated_layer(x, list(self.factors), self.patterns, self.bs_last, self.bias, self.activation, self.out_bs_last)
-        if self.out_bs_last != bool(self.bs_last):
+        x = tensor
+        if x.dim() != 2:
+            x = x.reshape(x.size(0), -1) if self.bs_last else x.reshape(-1, x.size(-1))
+        # (a ParameterList takes longer to walk than the call to launch)
+        y = _k.gated_layer(x.contiguous(), list(self.factors._parameters.values()), self.patterns, self.bs_last, self.bias,
+                           self.activation, self.out_bs_last)
+        if tensor.dim() == 2 or self.out_bs_last != bool(self.bs_last):
             return y
         if self.bs_last:
             return y.view(self.out_size, *tensor.shape[1:])

@@ -103,8 +103,11 @@ def _forward(x, y, params, sizes, kinds, keep):
     d = _desc(x, y, z, params, sizes, kinds)
     d.h = None if h is None else h.data_ptr()
     d.stats = None if stats is None else stats.data_ptr()
+    lib = _lib.load()
+    size = lib.ksmm_cu_norm_forward_workspace_bytes(ctypes.byref(d))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     with torch.cuda.device(x.device):
-        _lib.check(_lib.load().ksmm_cu_norm_forward(ctypes.byref(d), _stream_ptr(x.device)))
+        _lib.check(lib.ksmm_cu_norm_forward(ctypes.byref(d), ws.data_ptr() if size else None, size, _stream_ptr(x.device)))
     return z, h, stats
 
 

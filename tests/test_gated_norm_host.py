@@ -71,16 +71,20 @@ def norm_desc(**kw):
 ])
 def test_norm_entry(change, status):
     lib = _lib.load()
-    assert lib.ksmm_cu_norm_forward(ctypes.byref(norm_desc(**change)), None) == status
+    assert lib.ksmm_cu_norm_forward(ctypes.byref(norm_desc(**change)), None, 0, None) == status
     assert lib.ksmm_cu_last_error()
 
 
 def test_norm_entries_of_nothing():
     lib = _lib.load()
     before = lib.ksmm_cu_launch_count()
-    assert lib.ksmm_cu_norm_forward(None, None) == _lib.KSMM_ERR_BAD_ARGUMENT
-    assert lib.ksmm_cu_norm_forward(ctypes.byref(norm_desc(rows=0, x=None, h=None)), None) == _lib.KSMM_OK
+    assert lib.ksmm_cu_norm_forward(None, None, 0, None) == _lib.KSMM_ERR_BAD_ARGUMENT
+    assert lib.ksmm_cu_norm_forward(ctypes.byref(norm_desc(rows=0, x=None, h=None)), None, 0, None) == _lib.KSMM_OK
+    wide = norm_desc(bs_last=1, channels=2000)
+    assert lib.ksmm_cu_norm_forward_workspace_bytes(ctypes.byref(wide)) >= 2 * 2000 * 4 * 4
+    assert lib.ksmm_cu_norm_forward(ctypes.byref(wide), None, 0, None) == _lib.KSMM_ERR_WORKSPACE
     d = norm_desc()
+    assert lib.ksmm_cu_norm_forward_workspace_bytes(ctypes.byref(d)) == 0
     assert lib.ksmm_cu_norm_backward(ctypes.byref(d), None, 0, None) == _lib.KSMM_ERR_BAD_ARGUMENT   # no statistics
     d = norm_desc(grad_h=d.x, stats=(d.x + 15) // 16 * 16, grad_weight=d.x)
     need = lib.ksmm_cu_norm_backward_workspace_bytes(ctypes.byref(d))

@@ -122,3 +122,11 @@ def test_relu(dtype):
 def test_many_tiles(batch):
     for bs_last, out_last in LAYOUTS:
         check(SMALL, torch.float16, bs_last, out_last, batch, act="gelu")
+
+
+@pytest.mark.parametrize("bs_last,out_last", LAYOUTS)
+@pytest.mark.parametrize("batch", [33, 450, 1003])
+def test_ragged_fp32_inference(batch, bs_last, out_last):
+    """Padded intermediates go through the tensor-core kernel with their padding."""
+    for patterns in (BASE, SMALL, CHAIN3):
+        check(patterns, torch.float32, bs_last, out_last, batch, train=False)

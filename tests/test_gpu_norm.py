@@ -196,3 +196,12 @@ def test_many_wide_rows(dtype, channels, rows, samples):
     """Runs of rows through shared memory, a block per row."""
     check(dtype, (rows, channels), norm="layer", post_norm="layer", samples=samples, keys=EVERY)
     check(dtype, (rows, channels), norm="rms", residual=False, keys=("weight",), train=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels,rows,samples", [(1536, 70, 2), (1537, 70, 2), (2304, 413, 7), (4800, 115, 23), (6950, 33, 1)])
+def test_wide_columns(dtype, channels, rows, samples):
+    """Batch-last tensors on either side of what a block keeps of a token."""
+    check(dtype, (channels, rows), norm="layer", post_norm="rms", samples=samples, keys=EVERY, bs_last=True)
+    check(dtype, (channels, rows), norm="rms", residual=False, keys=("weight",), bs_last=True)
+    check(dtype, (channels, rows), norm=None, post_norm="layer", keys=("post_weight",), bs_last=True)
