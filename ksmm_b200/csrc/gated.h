@@ -20,8 +20,9 @@ int launch_gate_backward(const void* gu, int64_t ld, const void* dh, int64_t dh_
 // row strides of what it reads and writes are multiples of 16 bytes, except a batch-last output's.
 bool tc_gated_fits(const int32_t* q, int64_t batch, int dtype, int in_last, int out_last);
 // p: the factor with stacked weights, bias and (group_shared_input == 0) input; p.out = h, p.activation = the
-// gate's.  halves != NULL: both halves are stored there too (batch-last rows halves_ld apart).
-int tc_gated_launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream);
+// gate's.  halves != NULL: both halves are stored there too (batch-last rows halves_ld apart).  turn: the problem's
+// output is batch-last, but h is stored batch-first, element by element (for small batches, in place of a transpose).
+int tc_gated_launch(const Problem& p, void* halves, int64_t halves_ld, bool turn, cudaStream_t stream);
 // p.out = the sum of both halves of a factor with a stacked batch-last input and stacked weights, no bias; for what
 // tc_gated_fits says
 int tc_gated_sum(const Problem& p, cudaStream_t stream);

@@ -52,11 +52,12 @@ struct Params {
   int dtype, act;
   int stacked_input;  // the halves have an input each
   int* status;
-  void* y;            // batch-last output rows that no tensor map can address (y_direct)
+  void* y;            // for outputs stored without a tensor map
   int64_t y_ld;
-  int y_direct;
+  int y_direct;       // kRows: batch-last rows that no map can address; kTurned: batch-first, element by element
 };
 
+enum { kMapped, kRows, kTurned };
 enum { kProduct, kKeep, kSum };  // h; h and both halves; the sum of the halves
 
 template <bool WRES, int NWC, int SX, int STGN, bool PAIR>
@@ -524,7 +525,8 @@ __global__ void __launch_bounds__(kBlock, 1)
           send(&tmH, half);
         }
       }
-      next_tile();
+      const bool turn = OUT_LAST && !SUM && P.y_direct == kTurned;
+      if (!turn) next_tile();
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         uint32_t g[16], w[8];
@@ -549,8 +551,22 @@ __global__ void __launch_bounds__(kBlock, 1)
             default: gate_16<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
           }
         }
-        fill(w, s);
+        if (turn) {
+          // a lane's 16 batch entries of one feature
+          if (q * 32 + lane < row_limit) {
+            const int64_t feats = static_cast<int64_t>(blocks) * P.b;
+            uint16_t* y = static_cast<uint16_t*>(P.y) + (n0 + box * 32 + s * 16) * feats +
+                          (static_cast<int64_t>(i) * P.b + j0 + q * 32 + lane) * d + l;
+            const int exist = col_limit - box * 32 - s * 16;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (e < exist) y[e * feats] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+          }
+        } else {
+          fill(w, s);
+        }
       }
+      if (turn) continue;
       if (OUT_LAST && P.y_direct) {
         // each warp of the pair stores half of the tile's rows
         bar_sync_named(1 + pair, 64);
@@ -583,7 +599,7 @@ __global__ void __launch_bounds__(kBlock, 1)
 }
 
 template <bool IN_LAST, bool OUT_LAST, bool WRES, int NWC, int SX, int STGN, int MODE, bool PAIR = false>
-int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream, bool turn = false) {
   using C = Cfg<WRES, NWC, SX, STGN, PAIR>;
   constexpr bool KEEP = MODE == kKeep;
   auto kern = gated_kernel<IN_LAST, OUT_LAST, WRES, NWC, SX, STGN, MODE, PAIR>;
@@ -616,7 +632,7 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
   Params P = {};
   P.y = p.out;
   P.y_ld = out_stride(p);
-  P.y_direct = OUT_LAST && !rows_addressable(p.out, P.y_ld, 2);
+  P.y_direct = turn ? kTurned : (OUT_LAST && !rows_addressable(p.out, P.y_ld, 2) ? kRows : kMapped);
   auto output_map = [&](CUtensorMap* tm, const void* ptr, int64_t ld, uint64_t groups) {
     if (OUT_LAST) {
       const uint64_t L = ld, dims[4] = {B, d, b, groups * a}, str[4] = {1, L, d * L, b * d * L};
@@ -705,18 +721,18 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
 bool use_pair(const Problem& p) { return p.c <= 3 * kKC && p.b > 128 && p.batch >= 2048; }
 
 template <bool IN_LAST, bool OUT_LAST>
-int launch_layout(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+int launch_layout(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream, bool turn) {
   if constexpr (OUT_LAST) {
     if (use_pair(p))
-      return halves ? launch<IN_LAST, true, true, 3, 4, 2, kKeep, true>(p, halves, halves_ld, stream)
-                    : launch<IN_LAST, true, true, 3, 6, 1, kProduct, true>(p, halves, halves_ld, stream);
+      return halves ? launch<IN_LAST, true, true, 3, 4, 2, kKeep, true>(p, halves, halves_ld, stream, turn)
+                    : launch<IN_LAST, true, true, 3, 6, 1, kProduct, true>(p, halves, halves_ld, stream, turn);
   }
   if (p.c <= 3 * kKC)
-    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 2, 2, kKeep>(p, halves, halves_ld, stream)
-                  : launch<IN_LAST, OUT_LAST, true, 3, 3, 1, kProduct>(p, halves, halves_ld, stream);
+    return halves ? launch<IN_LAST, OUT_LAST, true, 3, 2, 2, kKeep>(p, halves, halves_ld, stream, turn)
+                  : launch<IN_LAST, OUT_LAST, true, 3, 3, 1, kProduct>(p, halves, halves_ld, stream, turn);
   if constexpr (IN_LAST && OUT_LAST) {
-    return halves ? launch<true, true, false, 0, 2, 2, kKeep>(p, halves, halves_ld, stream)
-                  : launch<true, true, false, 0, 2, 1, kProduct>(p, halves, halves_ld, stream);
+    return halves ? launch<true, true, false, 0, 2, 2, kKeep>(p, halves, halves_ld, stream, turn)
+                  : launch<true, true, false, 0, 2, 1, kProduct>(p, halves, halves_ld, stream, turn);
   }
   return set_error(KSMM_ERR_UNSUPPORTED, "gated kernel: blocks longer than %d keep the batch-last layout", 3 * kKC);
 }
@@ -740,12 +756,12 @@ bool tc_gated_fits(const int32_t* q, int64_t batch, int dtype, int in_last, int 
   return batch > 0 && batch <= 0x3fffffffLL && static_cast<int64_t>(q[0]) * q[3] <= 0x3fffffffLL;
 }
 
-int tc_gated_launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream) {
+int tc_gated_launch(const Problem& p, void* halves, int64_t halves_ld, bool turn, cudaStream_t stream) {
   const bool in_last = in_is_last(p), out_last = out_is_last(p);
-  if (in_last) return out_last ? tc::launch_layout<true, true>(p, halves, halves_ld, stream)
-                               : tc::launch_layout<true, false>(p, halves, halves_ld, stream);
-  return out_last ? tc::launch_layout<false, true>(p, halves, halves_ld, stream)
-                  : tc::launch_layout<false, false>(p, halves, halves_ld, stream);
+  if (in_last) return out_last ? tc::launch_layout<true, true>(p, halves, halves_ld, stream, turn)
+                               : tc::launch_layout<true, false>(p, halves, halves_ld, stream, turn);
+  return out_last ? tc::launch_layout<false, true>(p, halves, halves_ld, stream, turn)
+                  : tc::launch_layout<false, false>(p, halves, halves_ld, stream, turn);
 }
 
 int tc_gated_sum(const Problem& p, cudaStream_t stream) {
