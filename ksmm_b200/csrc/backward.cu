@@ -132,6 +132,7 @@ namespace tc {
 
 struct ParamsW {
   int a, b, c, d;
+  int xa;       // blocks of the input: a, or fewer where runs of them share it
   int tiles_k, tiles_j, splits;
   int nchunks;  // ceil(batch / 64)
   uint32_t idesc;
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   const int sp = static_cast<int>(t % P.splits);
   const int blk = static_cast<int>(t / P.splits);
   const int i = blk / P.d, l = blk % P.d;
+  const int xi = i % P.xa, xblk = xi * P.d + l;
   const int k0 = tk * (MB * 128), j0 = tj * NT;
   const int ch_begin = static_cast<int>(static_cast<int64_t>(sp) * P.nchunks / P.splits);
   const int ch_end = static_cast<int>(static_cast<int64_t>(sp + 1) * P.nchunks / P.splits);
@@ -227,11 +229,11 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         const int n0 = ch * 64;
         if constexpr (X_LAST) {
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb) tma_load_4d(dst + mb * 128 * 128, &tmX, bar, n0, l, k0 + mb * 128, i);
+          for (int mb = 0; mb < MB; ++mb) tma_load_4d(dst + mb * 128 * 128, &tmX, bar, n0, l, k0 + mb * 128, xi);
         } else {
           // 64 batch rows x 64 features per box; M groups of 64 follow one another
 #pragma unroll
-          for (int kb = 0; kb < 2 * MB; ++kb) tma_load_3d(dst + kb * 64 * 128, &tmX, bar, k0 + kb * 64, blk, n0);
+          for (int kb = 0; kb < 2 * MB; ++kb) tma_load_3d(dst + kb * 64 * 128, &tmX, bar, k0 + kb * 64, xblk, n0);
         }
         if constexpr (G_LAST) {
           tma_load_4d(dst + C::A_BYTES, &tmG, bar, n0, l, j0, i);
@@ -441,6 +443,7 @@ static int launch_w(const Problem& p, const WgradOperand& x, const WgradOperand&
   // batch-last: (batch, d, features, a), 64 batch entries x 128 (NT) features per box;
   // batch-first (d = 1): (features, a, batch), 64 features x 64 batch entries per box
   auto operand_map = [&](CUtensorMap* tm, bool last, const WgradOperand& o, uint64_t f, uint32_t rows) {
+    const uint64_t a = p.a / o.shared;
     if (last) {
       const uint64_t L = o.ld;
       const uint64_t dims[4] = {B, d, f, a}, str[4] = {1, L, d * L, f * d * L};
@@ -456,6 +459,7 @@ static int launch_w(const Problem& p, const WgradOperand& x, const WgradOperand&
   if ((st = operand_map(&tmG, G_LAST, g, b, NT)) != KSMM_OK) return st;
   ParamsW P;
   P.a = p.a; P.b = p.b; P.c = p.c; P.d = p.d;
+  P.xa = p.a / x.shared;
   P.tiles_k = (p.c + MB * 128 - 1) / (MB * 128);
   P.tiles_j = (p.b + NT - 1) / NT;
   P.splits = splits;
@@ -743,6 +747,12 @@ int launch_bias_sum(const float* part, int slices, void* out, int64_t feats, int
   return KSMM_OK;
 }
 
+bool wgrad_takes_shared(const Problem& p, const WgradOperand& x, const WgradOperand& g) {
+  if (p.in_dtype != KSMM_F16 && p.in_dtype != KSMM_BF16) return false;
+  const WgradPlan w = plan_wgrad(p, x, g, true);
+  return w.tc && !w.copy_x && !w.copy_g;
+}
+
 size_t wgrad_workspace_bytes(const Problem& p, const WgradOperand& x, const WgradOperand& g) {
   return plan_wgrad(p, x, g, false).total();
 }
@@ -756,6 +766,8 @@ int wgrad_launch(const Problem& p, WgradOperand x, WgradOperand g, void* workspa
     return e == cudaSuccess ? KSMM_OK : set_error(KSMM_ERR_CUDA, "memset failed: %s", cudaGetErrorString(e));
   }
   const WgradPlan w = plan_wgrad(p, x, g, true);
+  if (x.shared > 1 && (p.in_dtype == KSMM_F32 || !w.tc || w.copy_x || w.copy_g || workspace_bytes < w.total()))
+    return set_error(KSMM_ERR_UNSUPPORTED, "weight gradient: no kernel for a shared input here");
   if (w.tc && workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= w.total()) {
     char* ws = static_cast<char*>(workspace);
     float* part = reinterpret_cast<float*>(ws + w.x_bytes + w.g_bytes);

@@ -13,11 +13,14 @@ struct WgradOperand {
   int last;    // 1: (features, batch), 0: (batch, features)
   int64_t ld;
   int regrouped = 0;  // batch-first rows in block order (i, l, k) instead of (i, k, l)
+  int shared = 1;     // an input that this many runs of blocks read: it has a / shared blocks of its own
 };
 
 // block transposes of kernel-format weights: (nblk, c, b) -> (nblk, b, c)
 int launch_transpose_blocks(const void* in, void* out, int64_t nblk, int c, int b, int es, cudaStream_t stream);
 
+// Can the operands be used as they stand by the 16-bit tensor-core kernel, the only one that takes a shared input?
+bool wgrad_takes_shared(const Problem& p, const WgradOperand& x, const WgradOperand& g);
 // dW of the factor of `p` (pattern, batch, type; p.out = dW in kernel format).  The workspace holds
 // copies of operands that cannot be addressed as they stand, and the partial sums.
 size_t wgrad_workspace_bytes(const Problem& p, const WgradOperand& x, const WgradOperand& g);

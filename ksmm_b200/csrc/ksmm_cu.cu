@@ -1962,14 +1962,27 @@ static int gated_stacked_backward(bool run, const ksmm_gated_desc_t& D, const vo
     const size_t welems = static_cast<size_t>(q[0]) * q[1] * q[2] * q[3];
     const size_t out_half = static_cast<size_t>(q[0]) * q[1] * q[3] * ld * es;
     if (!run || grad_values[f]) {
-      for (int h = 0; h < (f == 0 ? 2 : 1); ++h) {
-        Problem p = backward_problem(nullptr, nullptr, run ? static_cast<char*>(grad_values[f]) + h * welems * es : dummy, batch,
-                                     f == 0 ? q[0] : 2 * q[0], q[1], q[2], q[3], D.dtype, f == 0 ? D.bs_last : 1);
-        WgradOperand x{run ? D.input : dummy, D.bs_last, batch}, gw{g + h * out_half, 1, ld};
-        if (f > 0) x = WgradOperand{run ? static_cast<const char*>(D.saved) + static_cast<size_t>(f - 1) * one : dummy, 1, ld};
+      // the first factor's halves share their input
+      WgradOperand x{run ? D.input : dummy, D.bs_last, batch}, gw{g, 1, ld};
+      if (f > 0) x = WgradOperand{run ? static_cast<const char*>(D.saved) + static_cast<size_t>(f - 1) * one : dummy, 1, ld};
+      else x.shared = 2;
+      Problem p = backward_problem(nullptr, nullptr, run ? grad_values[f] : dummy, batch, 2 * q[0], q[1], q[2], q[3], D.dtype,
+                                   f == 0 ? D.bs_last : 1);
+      if (f > 0 || wgrad_takes_shared(p, x, gw)) {
         tail_bytes = std::max(tail_bytes, wgrad_workspace_bytes(p, x, gw));
         if (run) st = wgrad_launch(p, x, gw, tail, room, stream);
         if (st != KSMM_OK) return st;
+      }
+      if (f == 0 && (!run || !wgrad_takes_shared(p, x, gw))) {
+        x.shared = 1;
+        p.a = q[0];
+        for (int h = 0; h < 2; ++h) {
+          if (run) p.out = static_cast<char*>(grad_values[f]) + h * welems * es;
+          gw.ptr = g + h * out_half;
+          tail_bytes = std::max(tail_bytes, wgrad_workspace_bytes(p, x, gw));
+          if (run) st = wgrad_launch(p, x, gw, tail, room, stream);
+          if (st != KSMM_OK) return st;
+        }
       }
     }
     if (f == 0 && !need_input) break;
