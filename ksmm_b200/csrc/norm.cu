@@ -274,7 +274,8 @@ __device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t
 // threads beyond.
 // RING: blocks that stay on their SM take equal runs of rows.  Rows come to shared memory by bulk copies, `stages` of
 // them in flight per group of threads, and the parameters of the run's sample are combined there once, for every
-// row of it; a run may pass on to the next sample.  Else every row reads its parameters.  128 x 196 x 768 bf16 with
+// row of it; a run may pass on to the next sample.  Else every row reads its parameters (by groups of eight threads up to
+// 128 channels of 16 bits, where most of a warp would lie idle: 62 x 4446 x 64 fp16 138 -> 85 us).  128 x 196 x 768 bf16 with
 // gate, weight, bias, scale and shift (154 MB, 24 us at the copy's rate): 53 us with parameters read per row, 28 so;
 // 32768 x 4096 bf16 (1.07 GB, 166 us): 217 with a block of 256 threads per row, 175 with four groups of 128 and two
 // rows in flight for each.  (A block of 512 threads per row took 226: a row's waits and sums are paid per thread.)
@@ -283,8 +284,14 @@ constexpr int kRingBlock = 256, kRingWide = 512;
 // the sum over a group of TPR threads
 template <int TPR>
 __device__ __forceinline__ float group_sum(float v, float* red, int& turn, int group) {
+  if constexpr (TPR < 32) {  // a group's lanes only: other groups of the warp may have no row
+    const unsigned mask = ((1u << (TPR & 31)) - 1u) << (threadIdx.x & 31 & ~(TPR - 1));
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    return v;
+  }
   v = warp_sum(v);
-  if constexpr (TPR == 32) {
+  if constexpr (TPR <= 32) {
     return v;
   } else {
     constexpr int W = TPR / 32;
@@ -1114,6 +1121,8 @@ template <typename T, int V>
 int launch_rows(const Args& A, cudaStream_t stream) {
   const int pieces = (A.C + V - 1) / V;
   if constexpr (V > 1) {
+    if (pieces <= 8) return go_rows<T, V, 1, 8>(A, stream);
+    if (pieces <= 16) return go_rows<T, V, 2, 8>(A, stream);
     if (pieces <= 128 && A.per_sample >= 32 && A.rows >= 148 * 16) {
       if (pieces <= 32) return go_rows<T, V, 1, 32, true>(A, stream);
       if (pieces <= 64) return go_rows<T, V, 2, 32, true>(A, stream);
@@ -1124,17 +1133,16 @@ int launch_rows(const Args& A, cudaStream_t stream) {
       if (pieces <= 256) return go_rows<T, V, 2, 128, true>(A, stream);
       return pieces <= 512 ? go_rows<T, V, 4, 128, true>(A, stream) : go_rows<T, V, 4, 256, true>(A, stream);
     }
-    if (pieces <= 64) return go_rows<T, V, 2, 32>(A, stream);
     if (pieces <= 128) return go_rows<T, V, 4, 32>(A, stream);
     if (pieces <= 256) return go_rows<T, V, 1, 256>(A, stream);
-    if (pieces <= 512) return go_rows<T, V, 4, 128>(A, stream);
     if constexpr (V == 4) {
       if (pieces > 1024) return go_rows<T, V, 4, 512>(A, stream);
     }
     return go_rows<T, V, 4, 256>(A, stream);
   } else {
     if (pieces <= 256) return go_rows<T, 1, 8, 32>(A, stream);
-    if (pieces <= 1024) return go_rows<T, 1, 8, 128>(A, stream);
+    // (10000 x 1303 bf16: 417 us with 1024 threads per row, one block on an SM; 101 with 256)
+    if (pieces <= 2048) return go_rows<T, 1, 8, 256>(A, stream);
     return go_rows<T, 1, 8, 1024>(A, stream);
   }
 }
