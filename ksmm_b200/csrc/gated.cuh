@@ -19,7 +19,7 @@ __device__ __forceinline__ float gate_value(float g, int act) {
     case KSMM_ACT_SILU: return g * sigmoid<B16>(g);
     case KSMM_ACT_SIGMOID: return sigmoid<B16>(g);
     case KSMM_ACT_GELU: return B16 ? gelu_16bit(g) : g * normcdff(g);
-    case KSMM_ACT_RELU: return fmaxf(g, 0.f);
+    case KSMM_ACT_RELU: return g < 0.f ? 0.f : g;  // (a NaN stays one)
     default: return g;
   }
 }
@@ -42,8 +42,8 @@ __device__ __forceinline__ void gate_slope(float g, int act, float& value, float
     value = g * cdf;
     slope = fmaf(t * 0.3989422804f, __expf(-0.5f * t * t), cdf);
   } else if (act == KSMM_ACT_RELU) {
-    value = fmaxf(g, 0.f);
-    slope = g > 0.f ? 1.f : 0.f;
+    value = g < 0.f ? 0.f : g;
+    slope = g <= 0.f ? 0.f : 1.f;
   }
 }
 

@@ -143,9 +143,9 @@ __device__ __forceinline__ float rcp_ftz(float x) {
 
 // act(g) * u for two values each, for results that are rounded to 16 bits.  The special-function unit (16 values
 // a cycle) is what the epilogue has least of, so the two sigmoids of SiLU share one reciprocal:
-// 1 / p = q / (p q) with p = 1 + 2^s.  s stops at 62 so that p q stays finite: below g = -43 the factor stays at
-// 2^-62, and what is off is smaller than 1e-17.  (A NaN in one value of a pair must not reach the other: its s
-// becomes 62, and g itself carries it into its product.)
+// 1 / p = q / (p q) with p = 1 + 2^s.  s stops at 62 so that p q stays finite; below, from g = -43 on, the factor
+// is 0 (it is under 2^-62 there, and g may be anything down to -3e38).  A NaN in one value of a pair must not
+// reach the other: its s becomes 62, and g itself carries it into its product.
 template <int ACT>
 __device__ __forceinline__ void gate_2(float g0, float g1, float u0, float u1, float& h0, float& h1) {
   if constexpr (ACT == KSMM_ACT_SILU) {
@@ -154,8 +154,8 @@ __device__ __forceinline__ void gate_2(float g0, float g1, float u0, float u1, f
     unpack_f2(mul_f2(g, pack_f2(-1.4426950409f, -1.4426950409f)), s0, s1);
     const uint64_t p = add_f2(pack_f2(exp2_ftz(fminf(s0, 62.f)), exp2_ftz(fminf(s1, 62.f))), pack_f2(1.f, 1.f));
     unpack_f2(p, p0, p1);
-    const float r = rcp_ftz(p0 * p1);
-    unpack_f2(mul_f2(mul_f2(mul_f2(pack_f2(p1, p0), pack_f2(r, r)), g), pack_f2(u0, u1)), h0, h1);
+    const float r = rcp_ftz(p0 * p1), q0 = s0 < 62.f ? p1 : 0.f, q1 = s1 < 62.f ? p0 : 0.f;
+    unpack_f2(mul_f2(mul_f2(mul_f2(pack_f2(q0, q1), pack_f2(r, r)), g), pack_f2(u0, u1)), h0, h1);
   } else if constexpr (ACT == KSMM_ACT_GELU) {
     uint32_t r0 = __float_as_uint(g0), r1 = __float_as_uint(g1);
     gelu_16bit_2(r0, r1);

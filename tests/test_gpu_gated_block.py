@@ -245,6 +245,36 @@ def test_large_values_of_the_gate(dtype):
     assert (got - want).abs().max().item() <= 4 * torch.finfo(dtype).eps * 40000 and torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("out_last", [False, True])
+def test_the_lowest_gates_close(act, dtype, out_last):
+    """However far below 0 a gate is, nothing passes it (sigmoid(-100) = 4e-44 rounds to 0 or a subnormal number;
+    the up projection multiplies that by 1)."""
+    pats = [(1, 64, 64, 1)]
+    eye = torch.eye(64, device="cuda").reshape(1, 64, 64, 1)
+    layer = kb.KSGatedLinear(pats, gate_weights=[eye], up_weights=[eye.roll(1, 1)], bias=False, dtype=dtype, activation=act,
+                             out_bs_last=out_last)
+    x = torch.zeros(512, 64, device="cuda", dtype=dtype)
+    for k, v in ((0, -100.0), (2, -1e4), (4, torch.finfo(dtype).min / 2)):
+        x[:, k], x[:, k - 1], x[:, (k + 1) % 64] = v, 1.0, 1.0
+    got = layer(x)
+    got = got.t() if out_last else got
+    assert got[:, [0, 2, 4]].abs().max().item() < 1e-37
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_relu_keeps_a_nan_of_the_gate(dtype):
+    layer = kb.KSGatedLinear([(1, 64, 64, 1)], bias=True, dtype=dtype, activation="relu", requires_grad=True)
+    with torch.no_grad():
+        layer.bias[3] = float("nan")
+    out = layer(torch.randn(40, 64, device="cuda").to(dtype))
+    with torch.no_grad():
+        plain = layer(torch.randn(40, 64, device="cuda").to(dtype))
+    for o in (out, plain):
+        assert torch.isnan(o[:, 3]).all() and torch.isfinite(o[:, 4:]).all()
+
+
 def test_neighbours_of_outputs_stay():
     """Outputs are written inside their bounds: rows behind the last token, columns behind the last feature."""
     for batch in (45, 197, 2601):
