@@ -138,6 +138,7 @@ struct Problem {
   // Row strides in elements of a batch-last input / output; 0 = the batch.  Intermediates whose batch
   // is not a whole number of 16-byte pieces have padded rows, so that tensor maps can address them.
   int64_t in_ld = 0, out_ld = 0;
+  int w_ld = 0;    // elements of a weight row, if not b: copies whose rows are whole pieces (tc_f32x3.cu alone takes them)
   int no_pad = 0;  // 1: copies and intermediates keep rows of exactly the batch (what fits without padding)
   float alpha;
   const float* alpha_dev = nullptr;  // fp8: a factor of alpha that a kernel earlier in the stream computes

@@ -11,6 +11,8 @@ constexpr int kGatedWaits = 90;  // codes of tc_gated.cu's bounded waits: 90 to 
 // h = act(g) * u.  g and u: `lines` lines of `len` elements with stride `ld`, u after g; h has stride `h_ld`.
 int launch_gate(const void* gu, int64_t ld, void* h, int64_t h_ld, int64_t lines, int64_t len, int dtype, int act,
                 cudaStream_t stream);
+// the same in the other layout: h is (len, lines) without gaps
+int launch_gate_turn(const void* gu, int64_t ld, void* h, int64_t lines, int64_t len, int dtype, int act, cudaStream_t stream);
 // dg = dh u act'(g), du = dh act(g); `out` holds dg and, out_half elements after it, du (stride ld).
 // bias_grad != NULL: also the sums of every line of dg, then of du, (2, lines) in the tensors' type
 int launch_gate_backward(const void* gu, int64_t ld, const void* dh, int64_t dh_ld, void* out, int64_t out_half, int64_t lines,

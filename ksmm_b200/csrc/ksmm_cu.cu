@@ -1784,8 +1784,33 @@ static size_t gated_saved_bytes(int nfactors, const int32_t* patterns, int64_t l
          align_up(2 * static_cast<size_t>(pl[0]) * pl[1] * pl[3] * ld * es, 256);
 }
 
+// Elements per row of a padded copy of both halves' fp32 weights, which the tensor cores take where b is no
+// multiple of 32; 0 where there is none.  The copy, 2 a d c rows, has to be small beside the product.
+// (4096 rows of (16,176,64,1), both halves: 86 us by the FFMA kernel, 43 so, 3 of them the copy.)
+static int padded_weight_row(const Problem& p) {
+  if (p.in_dtype != KSMM_F32 || p.b % 32 == 0 || p.b % 4 != 0 || p.batch < 512 || in_is_last(p) != out_is_last(p)) return 0;
+  const int ld = (p.b + 31) / 32 * 32;
+  return 4 * ld <= 5 * p.b ? ld : 0;
+}
+static size_t padded_weight_bytes(const Problem& p) {
+  return align_up(2 * static_cast<size_t>(p.a) * p.d * p.c * padded_weight_row(p) * sizeof(float), 256);
+}
+
 // Runs one factor of both chains: the input is shared or two halves, weights, output and bias are two halves.
-static int run_pair(const Problem& p, int shared_input, size_t scratch_room, cudaStream_t stream) {
+// pad_weights: p.scratch may take a copy of the weights.
+static int run_pair(const Problem& given, int shared_input, bool pad_weights, size_t scratch_room, cudaStream_t stream) {
+  Problem p = given;
+  if (pad_weights && padded_weight_row(p) && padded_weight_bytes(p) <= scratch_room && aligned16(p.scratch)) {
+    Problem h = p;
+    h.w_ld = padded_weight_row(p);
+    h.w = p.scratch;
+    if (auto_choice(h).algo == KSMM_ALGO_TC) {
+      const int st = launch_copy_rows(p.w, p.b, p.scratch, h.w_ld, 2 * static_cast<int64_t>(p.a) * p.d * p.c, p.b, sizeof(float), stream);
+      if (st != KSMM_OK) return st;
+      p = h;
+      scratch_room = 0;
+    }
+  }
   Problem g = p;
   g.groups = 2;
   g.group_shared_input = shared_input;
@@ -1799,8 +1824,8 @@ static int run_pair(const Problem& p, int shared_input, size_t scratch_room, cud
     // halves that follow one another are blocks of one problem
     Problem h = p;
     h.a = 2 * p.a;
-    Choice ch = auto_choice(h);
-    h.scratch_bytes = scratch_need(h, ch);
+    Choice ch = p.w_ld ? Choice{KSMM_ALGO_TC, 0} : auto_choice(h);
+    h.scratch_bytes = p.w_ld ? 0 : scratch_need(h, ch);
     if (h.scratch_bytes > scratch_room) {
       ch = Choice{KSMM_ALGO_SIMT, -1};
       h.scratch_bytes = 0;
@@ -1812,11 +1837,11 @@ static int run_pair(const Problem& p, int shared_input, size_t scratch_room, cud
   for (int q = 0; q < 2; ++q) {
     Problem h = p;
     h.in = static_cast<const char*>(p.in) + (shared_input ? 0 : q * in_half);
-    h.w = static_cast<const char*>(p.w) + q * (static_cast<size_t>(p.a) * p.b * p.c * p.d * es);
+    h.w = static_cast<const char*>(p.w) + q * (static_cast<size_t>(p.a) * (p.w_ld ? p.w_ld : p.b) * p.c * p.d * es);
     h.out = static_cast<char*>(p.out) + q * out_half;
     if (p.bias) h.bias = static_cast<const char*>(p.bias) + q * (static_cast<size_t>(p.a) * p.b * p.d * es);
-    Choice ch = h.out_bs_last >= 0 ? Choice{KSMM_ALGO_TC, -1} : auto_choice(h);
-    const size_t need = h.out_bs_last >= 0 ? 0 : scratch_need(h, ch);
+    Choice ch = p.w_ld ? Choice{KSMM_ALGO_TC, 0} : h.out_bs_last >= 0 ? Choice{KSMM_ALGO_TC, -1} : auto_choice(h);
+    const size_t need = h.out_bs_last >= 0 || p.w_ld ? 0 : scratch_need(h, ch);
     if (need > scratch_room) ch = Choice{KSMM_ALGO_SIMT, -1};
     else h.scratch_bytes = need;
     const int st = run_family(h, ch.algo, ch.config, stream);
@@ -1850,7 +1875,7 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   const size_t pre_bytes = plan.pre || pad_in ? align_up(static_cast<size_t>(n_in) * ld * es, 256) : 0;
   const size_t one = gated_buffer_bytes(n, D.patterns, ld, es);
   const size_t halves_bytes = align_up(2 * static_cast<size_t>(n_out) * ld * es, 256);
-  const size_t post_bytes = plan.post ? align_up(static_cast<size_t>(n_out) * ld * es, 256) : 0;
+  const size_t post_bytes = plan.post && fuse ? align_up(static_cast<size_t>(n_out) * ld * es, 256) : 0;
   const int buffers = std::min(n - 1, 2);
   char* ws = run ? static_cast<char*>(D.workspace) : reinterpret_cast<char*>(static_cast<uintptr_t>(1) << 20);
   char* kept = run ? static_cast<char*>(D.saved) : ws;
@@ -1905,7 +1930,7 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
       if (st != KSMM_OK) return st;
     } else if (run) {
       p.scratch = at;
-      st = run_pair(p, f == 0, room, stream);
+      st = run_pair(p, f == 0, !keep, room, stream);
       if (st != KSMM_OK) return st;
     } else {
       st = check_problem(p);
@@ -1914,18 +1939,23 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
       Problem h = p;
       h.a = 2 * p.a;
       if (f > 0 && in_is_last(p) && out_is_last(p)) scratch = std::max(scratch, scratch_need(h, auto_choice(h)));
+      if (!keep) scratch = std::max(scratch, padded_weight_bytes(p));
     }
     cur = p.out;
     if (D.layouts) D.layouts[f] = plan.out_last[f];
   }
   if (run) {
-    void* h = plan.post ? h2 : D.output;
-    if (fuse) st = KSMM_OK;
-    else if (L) st = launch_gate(halves, ld, h, plan.post ? ld : batch, n_out, batch, D.dtype, D.activation, stream);
-    else st = launch_gate(halves, n_out, h, n_out, batch, n_out, D.dtype, D.activation, stream);
-    if (st == KSMM_OK && plan.post)
-      st = L ? launch_transpose(h2, D.output, n_out, batch, es, stream, 0, ld)
-             : launch_transpose(h2, D.output, batch, n_out, es, stream);
+    if (fuse) {
+      if (plan.post)
+        st = L ? launch_transpose(h2, D.output, n_out, batch, es, stream, 0, ld)
+               : launch_transpose(h2, D.output, batch, n_out, es, stream);
+    } else if (plan.post) {
+      st = L ? launch_gate_turn(halves, ld, D.output, n_out, batch, D.dtype, D.activation, stream)
+             : launch_gate_turn(halves, n_out, D.output, batch, n_out, D.dtype, D.activation, stream);
+    } else {
+      st = L ? launch_gate(halves, ld, D.output, batch, n_out, batch, D.dtype, D.activation, stream)
+             : launch_gate(halves, n_out, D.output, n_out, batch, n_out, D.dtype, D.activation, stream);
+    }
   }
   if (need) *need = used + align_up(scratch, 256);
   return st;

@@ -652,8 +652,9 @@ static int launch_f(const Problem& p, cudaStream_t stream) {
   }
   {
     // weights (a*d*c, b) row-major seen as (j % 32, k, j / 32, block): NJ / 32 atoms per box
-    const uint64_t dims[4] = {32, c, b / 32, a * d};
-    const uint64_t str[4] = {1, b, 32, c * b};
+    const uint64_t wb = p.w_ld ? p.w_ld : p.b;
+    const uint64_t dims[4] = {32, c, wb / 32, a * d};
+    const uint64_t str[4] = {1, wb, 32, c * wb};
     const uint32_t box[4] = {32, kKC, static_cast<uint32_t>(C::NJ / 32), 1};
     if ((st = encode_map(&tmW, KSMM_F32, 4, p.w, dims, str, box, true, true)) != KSMM_OK) return st;
   }
@@ -719,7 +720,8 @@ bool tc_f32x3_supported(const Problem& p, bool check_pointers) {
   if (has_padded_rows(p)) return false;
   if (p.batch <= 0 || p.batch > 0x7fffffffLL) return false;
   // the operand tiles are addressed in atoms of 32 columns; global strides are multiples of 16 bytes
-  if (p.b % 32 != 0) return false;
+  // (padded columns of a copy of the weights give results that are clipped)
+  if ((p.w_ld ? p.w_ld : p.b) % 32 != 0 || p.b % 4 != 0) return false;
   const bool out_last = p.out_bs_last < 0 ? p.bs_last != 0 : p.out_bs_last != 0;
   if (out_last != (p.bs_last != 0) && (p.d != 1 || p.groups > 1)) return false;  // layout-changing factors
   if (p.bs_last || out_last) {

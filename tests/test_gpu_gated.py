@@ -130,3 +130,14 @@ def test_ragged_fp32_inference(batch, bs_last, out_last):
     """Padded intermediates go through the tensor-core kernel with their padding."""
     for patterns in (BASE, SMALL, CHAIN3):
         check(patterns, torch.float32, bs_last, out_last, batch, train=False)
+
+
+@pytest.mark.parametrize("bs_last,out_last", LAYOUTS)
+@pytest.mark.parametrize("patterns", [CHAIN3, [(2, 52, 64, 1)], [(2, 52, 64, 2)], [(3, 32, 52, 1), (1, 116, 96, 1)]],
+                         ids=["chain3", "one", "interleaved", "second"])
+@pytest.mark.parametrize("batch", [544, 1003])
+def test_rows_of_weights_that_are_no_whole_pieces(batch, patterns, bs_last, out_last):
+    """fp32 inference copies such weights for the tensor cores, what lies behind a row may be anything."""
+    filler = torch.full((1 << 24,), float("nan"), device="cuda")
+    del filler
+    check(patterns, torch.float32, bs_last, out_last, batch, train=False)
