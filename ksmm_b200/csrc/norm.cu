@@ -950,7 +950,9 @@ __device__ __forceinline__ void put(const Args& A, void* p, int64_t at, float v)
   else static_cast<T*>(p)[at] = ElemTraits<T>::from_float(v);
 }
 
-constexpr int kSlices = 8;
+// Slices of a sum of n: a column of partial sums is a thread's chain of loads (23598 x 143 fp32, 888 partial sums: 23 us
+// in 8 slices, 13 in 32; 64 of 6464 channels: 4 and 8).
+inline unsigned slices_of(int64_t n) { return n >= 256 ? 32 : 8; }
 
 // the parameters of one channel and sample
 struct Params {
@@ -964,13 +966,13 @@ __device__ __forceinline__ Params params_at(const Args& A, int64_t sample, int c
           param_value<T>(A, A.post_bias, pb, 0.f), 1.f + param_value<T>(A, A.scale, sc, 0.f), param_value<T>(A, A.gate, ga, 1.f)};
 }
 
-// 32 channels x 8 slices: first == 1 adds the chunks of sample blockIdx.y and writes the gradients of
+// 32 channels by 8 or 32 slices: first == 1 adds the chunks of sample blockIdx.y and writes the gradients of
 // per-sample parameters and the sample's sums; first == 0 adds the samples.  With one sample the first does all.
 template <typename T>
-__global__ void __launch_bounds__(32 * kSlices) norm_param_grads_kernel(const Args A, const Grads g, const float* part, float* sums,
+__global__ void __launch_bounds__(1024) norm_param_grads_kernel(const Args A, const Grads g, const float* part, float* sums,
                                                                         int first) {
-  __shared__ float red[kSlices][7][32];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  __shared__ float red[32][7][32];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, slices = blockDim.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const bool ok = c < A.C;
   const int at_c = ok ? c : 0;
@@ -980,12 +982,12 @@ __global__ void __launch_bounds__(32 * kSlices) norm_param_grads_kernel(const Ar
   if (first) {
     const float* p = part + sample * A.chunks * 4 * A.C + at_c;
 #pragma unroll 2
-    for (int q = slice; q < A.chunks; q += kSlices)
+    for (int q = slice; q < A.chunks; q += slices)
 #pragma unroll
       for (int s = 0; s < 4; ++s) t[s] += p[(static_cast<int64_t>(q) * 4 + s) * A.C];
   } else {
 #pragma unroll 2
-    for (int64_t s = slice; s < A.samples; s += kSlices) {
+    for (int64_t s = slice; s < A.samples; s += slices) {
       const float* p = part + s * 4 * A.C + at_c;
       const float a = p[0], bb = p[A.C], cc = p[2 * A.C], d = p[3 * A.C];
       const uint32_t sr = raw_param(A, A.scale, s, at_c), gr = raw_param(A, A.gate, s, at_c);
@@ -1006,8 +1008,8 @@ __global__ void __launch_bounds__(32 * kSlices) norm_param_grads_kernel(const Ar
 #pragma unroll
   for (int s = 0; s < 7; ++s) {
     t[s] = 0.f;
-#pragma unroll
-    for (int q = 0; q < kSlices; ++q) t[s] += red[q][s][lane];
+#pragma unroll 8
+    for (int q = 0; q < slices; ++q) t[s] += red[q][s][lane];
   }
   if (first) {
     const bool one = A.samples == 1;
@@ -1276,7 +1278,10 @@ int64_t chunks_of(const ksmm_norm_desc_t& d) {
   const int64_t pieces = (d.channels * dtype_size(d.dtype) + 15) / 16, threads = std::min<int64_t>(512, (pieces + 31) / 32 * 32);
   const int64_t blocks = std::min<int64_t>(8, 65536 / ((threads <= 128 ? 168 : 128) * threads));
   const int64_t want = std::max<int64_t>(1, 148 * blocks / d.samples);
-  return std::max<int64_t>(1, std::min(want, (per + 7) / 8));
+  // (eight rows or more share a block's sums where there are rows enough; 64 rows of 6464 fp32 channels: 56 us with
+  // eight blocks, 17 with 64)
+  const int64_t least = std::max<int64_t>(1, std::min<int64_t>(8, d.rows / 148));
+  return std::max<int64_t>(1, std::min(want, (per + least - 1) / least));
 }
 
 bool wants_sums(const ksmm_norm_desc_t& d) {
@@ -1317,12 +1322,12 @@ int backward_typed(const ksmm_norm_desc_t& d, void* workspace, cudaStream_t stre
     gs.scale = skip(g.scale, g.scale_rows); gs.shift = skip(g.shift, g.shift_rows); gs.gate = skip(g.gate, g.gate_rows);
     auto row = [&](Row r) { return Row{r.p ? static_cast<const char*>(r.p) + s0 * r.ld * ps : nullptr, r.ld}; };
     B.scale = row(A.scale); B.shift = row(A.shift); B.gate = row(A.gate);
-    norm_param_grads_kernel<T><<<dim3(cx, ns), 32 * kSlices, 0, stream>>>(B, gs, A.part + s0 * chunks * 4 * A.C,
+    norm_param_grads_kernel<T><<<dim3(cx, ns), 32 * slices_of(chunks), 0, stream>>>(B, gs, A.part + s0 * chunks * 4 * A.C,
                                                                   totals ? per_sample + s0 * 4 * A.C : nullptr, 1);
     if ((st = launched("norm gradients")) != KSMM_OK) return st;
   }
   if (d.samples > 1 && totals) {
-    norm_param_grads_kernel<T><<<cx, 32 * kSlices, 0, stream>>>(A, g, per_sample, nullptr, 0);
+    norm_param_grads_kernel<T><<<cx, 32 * slices_of(d.samples), 0, stream>>>(A, g, per_sample, nullptr, 0);
     st = launched("norm gradients");
   }
   return st;
