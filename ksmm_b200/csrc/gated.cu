@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(256)
     gate_kernel(const T* __restrict__ gu, int64_t ld, const T* __restrict__ dh, int64_t h_ld, T* __restrict__ out,
                 int64_t half, int64_t out_half, int64_t lines, uint32_t pieces, int act) {
   const int64_t total = lines * pieces;
+#pragma unroll 1
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < total; t += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t line = total <= 0xffffffffLL ? static_cast<uint32_t>(t) / pieces : t / pieces;
     const int64_t x = (t - line * pieces) * V;
@@ -70,9 +71,9 @@ __global__ void __launch_bounds__(256)
     gate_turn_kernel(const T* __restrict__ gu, int64_t ld, T* __restrict__ out, int64_t half, int64_t lines, int64_t len,
                      uint32_t tiles_x, int act) {
   __shared__ float tile[64][65];
-  constexpr int P = 64 / V;
+  constexpr int P = 64 / V, AHEAD = V > 1 ? 4 : 1;
   const int64_t y0 = static_cast<int64_t>(blockIdx.x / tiles_x) * 64, x0 = static_cast<int64_t>(blockIdx.x % tiles_x) * 64;
-#pragma unroll 4
+#pragma unroll AHEAD
   for (int s = threadIdx.x; s < 64 * P; s += 256) {
     const int y = s / P, x = s % P * V;
     if (y0 + y >= lines || x0 + x >= len) continue;
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(256)
     for (int e = 0; e < V; ++e) tile[x + e][y] = gate_value<sizeof(T) == 2>(g[e], act) * u[e];
   }
   __syncthreads();
-#pragma unroll 4
+#pragma unroll AHEAD
   for (int s = threadIdx.x; s < 64 * P; s += 256) {
     const int x = s / P, y = s % P * V;
     if (x0 + x >= len || y0 + y >= lines) continue;

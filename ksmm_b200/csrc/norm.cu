@@ -1136,7 +1136,6 @@ int launch_rows(const Args& A, cudaStream_t stream) {
       return pieces <= 512 ? go_rows<T, V, 4, 128, true>(A, stream) : go_rows<T, V, 4, 256, true>(A, stream);
     }
     if (pieces <= 128) return go_rows<T, V, 4, 32>(A, stream);
-    if (pieces <= 256) return go_rows<T, V, 1, 256>(A, stream);
     if constexpr (V == 4) {
       if (pieces > 1024) return go_rows<T, V, 4, 512>(A, stream);
     }

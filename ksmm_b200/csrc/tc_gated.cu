@@ -547,8 +547,13 @@ __global__ void __launch_bounds__(kBlock, 1)
             case KSMM_ACT_SILU: gate_16<KSMM_ACT_SILU>(g, u, P.dtype, w); break;
             case KSMM_ACT_GELU: gate_16<KSMM_ACT_GELU>(g, u, P.dtype, w); break;
             case KSMM_ACT_SIGMOID: gate_16<KSMM_ACT_SIGMOID>(g, u, P.dtype, w); break;
-            case KSMM_ACT_RELU: gate_16<KSMM_ACT_RELU>(g, u, P.dtype, w); break;
-            default: gate_16<KSMM_ACT_NONE>(g, u, P.dtype, w); break;
+            default: {  // none and relu: a lowest value (a NaN is not below it)
+              const float low = P.act == KSMM_ACT_RELU ? 0.f : -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (__uint_as_float(g[e]) < low) g[e] = __float_as_uint(low);
+              gate_16<KSMM_ACT_NONE>(g, u, P.dtype, w);
+            }
           }
         }
         if (turn) {
