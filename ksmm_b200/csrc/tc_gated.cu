@@ -579,6 +579,9 @@ __global__ void __launch_bounds__(kBlock, 1)
                         (((static_cast<int64_t>(i) * P.b + j0 + q * 32) * d + l) * P.y_ld + n0 + col0) * 2;
         store_rows<2, 8>(stg, yrow, static_cast<int64_t>(d) * P.y_ld * 2, min(32, row_limit - q * 32), col_limit - col0, lane,
                          16 * side, 16 * side + 16);
+        // An empty group for the product's staging tile: next_tile() takes it that every tile handed out has one, and
+        // without it would hand out a tile that a half's store is still reading.
+        if (KEEP && side == 0 && lane == 0) bulk_commit();
       } else {
         send(&tmY, 0);
       }

@@ -1,0 +1,46 @@
+"""Paths of the gated layer's kernels against the definition in 64 bits.
+
+Tolerances are those of test_gpu_gated.py (n factors, u = eps / 2 of the type, relative 2-norms): 2 (3 n + 1) u forward,
+2 (5 n + 5) u backward.
+"""
+import pytest
+import torch
+
+from test_gpu_gated import LAYOUTS, definition, err, layer_and_input, unit
+
+pytestmark = pytest.mark.gpu
+
+
+def params_of(layer):
+    return [*layer.factors, *([] if layer.bias is None else [layer.bias])]
+
+
+def exact_gradients(layer, x, seed, act, out_last):
+    exact = [t.detach().double().requires_grad_(True) for t in (x, *params_of(layer))]
+    n = len(layer.patterns)
+    want = definition(exact[0], exact[1:1 + n], exact[-1] if layer.bias is not None else None, layer.patterns, layer.bs_last,
+                      out_last, act)
+    return want, torch.autograd.grad(want, exact, seed.double())
+
+
+@pytest.mark.parametrize("batch", [1995, 6501])
+@pytest.mark.parametrize("patterns", [[(1, 512, 64, 8)], [(2, 96, 64, 16)]], ids=["pairs", "one_tile"])
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_kept_halves_of_many_ragged_tiles(patterns, batch, bs_last):
+    """Training with batch-last outputs whose rows no tensor map addresses: every CTA walks several tiles (3 to 12
+    here), each of which stores both halves through staging tiles that the product's rows use in between."""
+    layer, x = layer_and_input(patterns, torch.bfloat16, bs_last, True, batch, "silu", train=True)
+    leaf = x.requires_grad_(True)
+    n, u = len(patterns), unit(torch.bfloat16)
+    seed = torch.randn(layer.out_size, batch, device="cuda").bfloat16()
+    want, ref = exact_gradients(layer, leaf, seed, "silu", True)
+    first = None
+    for _ in range(4):
+        h = layer(leaf)
+        got = torch.autograd.grad(h, [leaf, *params_of(layer)], seed)
+        assert err(h, want) <= 2 * (3 * n + 1) * u
+        for a, b in zip(got, ref):
+            assert err(a, b) <= 2 * (5 * n + 5) * u
+        if first is not None:
+            assert all(torch.equal(a, b) for a, b in zip(first, (h, *got)))
+        first = (h, *got)
