@@ -1083,17 +1083,20 @@ Args args_of(const ksmm_norm_desc_t& d) {
   return A;
 }
 
-// Dynamic shared memory beyond 48 KB needs a word with the driver; `granted` remembers it for a kernel and device.
-using Granted = std::atomic<size_t>[64];
-int allow_smem(const void* kern, size_t bytes, Granted& granted) {
+// Dynamic shared memory beyond 48 KB needs a word with the driver, once per kernel and device, for `most`: what any call of
+// the kernel may ask for.  (The driver keeps the last value, so that a limit of a call's own size could be lowered
+// by another thread's call between this one's word and its launch.  A repeated set of one value is harmless.)
+using Granted = std::atomic<bool>[64];
+int allow_smem(const void* kern, size_t bytes, size_t most, Granted& granted) {
   if (bytes <= 48 * 1024) return KSMM_OK;
+  if (bytes > most) return set_error(KSMM_ERR_UNSUPPORTED, "norm: %zu bytes of shared memory", bytes);
   int dev = 0;
   cudaGetDevice(&dev);
   const bool known = dev >= 0 && dev < 64;
-  if (known && granted[dev].load(std::memory_order_relaxed) >= bytes) return KSMM_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  if (e != cudaSuccess) return set_error(KSMM_ERR_CUDA, "cannot reserve %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-  if (known) granted[dev].store(bytes, std::memory_order_relaxed);
+  if (known && granted[dev].load(std::memory_order_relaxed)) return KSMM_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+  if (e != cudaSuccess) return set_error(KSMM_ERR_CUDA, "cannot reserve %zu bytes of shared memory: %s", most, cudaGetErrorString(e));
+  if (known) granted[dev].store(true, std::memory_order_relaxed);
   return KSMM_OK;
 }
 
@@ -1101,19 +1104,19 @@ template <typename T, int V, int K, int TPR, bool RING = false>
 int go_rows(Args A, cudaStream_t stream) {
   constexpr int kBlock = RING ? (TPR == 32 ? kRingBlock : kRingWide) : (TPR < 128 ? 128 : TPR);
   int64_t grid = (A.rows + kBlock / TPR - 1) / (kBlock / TPR);
+  constexpr size_t room = TPR == 32 ? 110 * 1024 : 224 * 1024;  // of a ring
   size_t smem = 0;
   if (RING) {
     A.status = tc::status_word();
     if (!A.status) return set_error(KSMM_ERR_CUDA, "cannot resolve the device status word");
     grid = tc::num_sms() * (TPR == 32 ? 2 : 1);
     const size_t coefs = static_cast<size_t>(A.C) * sizeof(float4), slot = static_cast<size_t>(A.C) * 2 * sizeof(T) * (kBlock / TPR);
-    const size_t room = TPR == 32 ? 110 * 1024 : 224 * 1024;
     A.stages = static_cast<int>(std::min<size_t>(TPR == 32 ? 6 : 12, (room - coefs) / slot));
     smem = coefs + A.stages * slot;
   }
   if (grid > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many rows");
   static Granted granted;
-  const int st = allow_smem(reinterpret_cast<const void*>(norm_rows_kernel<T, V, K, TPR, RING>), smem, granted);
+  const int st = allow_smem(reinterpret_cast<const void*>(norm_rows_kernel<T, V, K, TPR, RING>), smem, room, granted);
   if (st != KSMM_OK) return st;
   norm_rows_kernel<T, V, K, TPR, RING><<<static_cast<unsigned>(grid), kBlock, smem, stream>>>(A);
   return launched("norm");
@@ -1181,9 +1184,10 @@ int forward_typed(const ksmm_norm_desc_t& d, cudaStream_t stream) {
   const int64_t chunks = (A.per_sample + 31) / 32;
   if (chunks * A.samples > 0x7fffffffLL) return set_error(KSMM_ERR_UNSUPPORTED, "norm: too many tokens");
   A.chunks = static_cast<int>(chunks);
-  const size_t smem = static_cast<size_t>(A.C) * (sizeof(float4) + 32 * sizeof(float));
+  constexpr size_t per_channel = sizeof(float4) + 32 * sizeof(float);
+  const size_t smem = A.C * per_channel;
   static Granted granted;
-  const int st = allow_smem(reinterpret_cast<const void*>(norm_columns_kernel<T>), smem, granted);
+  const int st = allow_smem(reinterpret_cast<const void*>(norm_columns_kernel<T>), smem, kColumnChannels * per_channel, granted);
   if (st != KSMM_OK) return st;
   norm_columns_kernel<T><<<static_cast<unsigned>(chunks * A.samples), kColWarps * 32, smem, stream>>>(A);
   return launched("norm");
@@ -1297,9 +1301,8 @@ int backward_typed(const ksmm_norm_desc_t& d, void* workspace, cudaStream_t stre
   A.part = sums ? static_cast<float*>(workspace) : nullptr;
   int st;
   if (d.bs_last) {
+    static_assert(kColumnChannels * sizeof(float2) <= 48 * 1024, "more needs a word with the driver");
     const size_t smem = static_cast<size_t>(A.C) * sizeof(float2);
-    static Granted granted;
-    if ((st = allow_smem(reinterpret_cast<const void*>(norm_columns_backward_kernel<T>), smem, granted)) != KSMM_OK) return st;
     norm_columns_backward_kernel<T><<<static_cast<unsigned>(chunks * d.samples), kColWarps * 32, smem, stream>>>(A);
     st = launched("norm backward");
   } else {
