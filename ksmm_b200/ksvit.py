@@ -96,7 +96,7 @@ class KSGatedFeedForward(nn.Module):
     def forward(self, x, a):
         z, n = self.norm(x, a)
         h = self.gate_up(n)
-        if torch.is_grad_enabled() and (h.requires_grad or self.down.factors[0].requires_grad):
+        if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.down.parameters())):
             return self.down(h).view(z.shape) + z
         return self.down(h, residual=z).view(z.shape)
 

@@ -6,6 +6,7 @@ Tolerances are those of test_gpu_gated.py (n factors, u = eps / 2 of the type, r
 import pytest
 import torch
 
+from ksmm_b200.ksvit import KSGatedFeedForward
 from test_gpu_gated import LAYOUTS, definition, err, layer_and_input, unit
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +45,20 @@ def test_kept_halves_of_many_ragged_tiles(patterns, batch, bs_last):
         if first is not None:
             assert all(torch.equal(a, b) for a, b in zip(first, (h, *got)))
         first = (h, *got)
+
+
+@pytest.mark.parametrize("learns", ["down.factors.0", "down.factors.1", "down.bias", "gate_up.bias", "norm.weight"])
+def test_a_block_with_one_learning_parameter(learns):
+    """The gradient of a parameter is the same whether the others learn or not."""
+    torch.manual_seed(4)
+    ff = KSGatedFeedForward(torch.bfloat16, "cuda", requires_grad=True)
+    x, a, seed = (torch.randn(2, 50, 768, device="cuda").bfloat16() for _ in range(3))
+    p = dict(ff.named_parameters())[learns]
+    (want,) = torch.autograd.grad(ff(x, a), [p], seed)
+    for other in ff.parameters():
+        other.requires_grad_(other is p)
+    out = ff(x, a)
+    assert out.requires_grad
+    (got,) = torch.autograd.grad(out, [p], seed)
+    # (other kernels may run: the bound of a block's gradients in test_gpu_gated_block.py)
+    assert err(got, want.double()) <= 72 * unit(torch.bfloat16)
