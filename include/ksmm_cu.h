@@ -418,7 +418,7 @@ KSMM_API int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* g
  * contiguous.  Statistics, sums and the z that h is made from are fp32.  weight, bias, post_weight and
  * post_bias hold `channels` elements of param_dtype (dtype or fp32) or are NULL (1, 0).  scale, shift and gate
  * hold one row of `channels` elements (stride 0) or one per sample, `stride` elements apart; sample s is the
- * rows / samples tokens from s * rows / samples on.  NULL: 0, 0, 1.
+ * rows / samples tokens from s * rows / samples on.  NULL: 0, 0, 1.  post_weight and post_bias need a post_norm.
  *
  * ksmm_cu_norm_forward reads x, y and the parameters; writes z (with y), h (with a norm) and, where stats is
  * not NULL, 4 floats per token for the backward pass.  The reference composes these steps from separate

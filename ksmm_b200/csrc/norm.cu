@@ -1352,6 +1352,8 @@ int check_norm(const ksmm_norm_desc_t* d) {
     return set_error(KSMM_ERR_UNSUPPORTED, "norms take up to %d channels, not %d", kMaxChannels, d->channels);
   if (d->norm == kNone && !d->y) return set_error(KSMM_ERR_BAD_ARGUMENT, "neither a norm nor a second tensor");
   if (d->post_norm != kNone && !d->y) return set_error(KSMM_ERR_BAD_ARGUMENT, "a norm of y without y");
+  if (d->post_norm == kNone && (d->post_weight || d->post_bias || d->grad_post_weight || d->grad_post_bias))
+    return set_error(KSMM_ERR_BAD_ARGUMENT, "post_weight and post_bias belong to a post_norm");
   if (d->scale_stride < 0 || d->shift_stride < 0 || d->gate_stride < 0)
     return set_error(KSMM_ERR_BAD_ARGUMENT, "negative stride");
   if (!(d->eps >= 0.f)) return set_error(KSMM_ERR_BAD_ARGUMENT, "eps must not be negative");
