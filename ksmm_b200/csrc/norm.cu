@@ -536,7 +536,9 @@ __global__ void __launch_bounds__(RING ? (TPR == 32 ? kRingBlock : kRingWide) : 
 }
 
 // A block walks a run of one sample's rows, R at a time; a thread keeps its channels, so that the sums over
-// rows stay in its registers.  The next R rows are loaded while these are worked on.
+// rows stay in its registers.  The next R rows are loaded while these are worked on.  Normalised values are
+// (z - mean) r as in the forward pass: z r - mean r would round mean r, which costs a row whose mean is thousands of
+// deviations as many of its digits.
 template <typename T, int V, int K, int R, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_kernel(const Args A) {
   using L = Elem<V>;
@@ -605,13 +607,13 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
       float s[2 * R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const E by = L::all(cur.st[r].y), shift = L::all(-cur.st[r].x * cur.st[r].y);
+        const E by = L::all(cur.st[r].y), mean = L::all(-cur.st[r].x);
         E s1 = L::all(0.f), s2 = L::all(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const E g = cur.gh[r][k].get(i), n = e_fma(cur.z[r][k].get(i), by, shift);
+            const E g = cur.gh[r][k].get(i), n = e_mul(e_add(cur.z[r][k].get(i), mean), by);
             const E w = e_mul(g, wp[k][i]);
             s1 = e_add(s1, w);
             s2 = e_fma(w, n, s2);
@@ -625,12 +627,12 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const E m1 = L::all(A.pre == kLayer ? -s[2 * r] * inv : 0.f), m2 = L::all(-s[2 * r + 1] * inv);
-        const E by = L::all(cur.st[r].y), shift = L::all(-cur.st[r].x * cur.st[r].y);
+        const E by = L::all(cur.st[r].y), mean = L::all(-cur.st[r].x);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const E n = e_fma(cur.z[r][k].get(i), by, shift);
+            const E n = e_mul(e_add(cur.z[r][k].get(i), mean), by);
             G[r][k][i] = e_fma(by, e_fma(n, m2, e_fma(cur.gh[r][k].get(i), wp[k][i], m1)), cur.gz[r][k].get(i));
           }
       }
@@ -661,14 +663,14 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
       for (int r = 0; r < R; ++r) {
         s[2 * r] = s[2 * r + 1] = 0.f;
         if (row0 + r >= end) continue;  // (rows of the next run must not join the sums)
-        const E by = L::all(cur.st[r].w), shift = L::all(-cur.st[r].z * cur.st[r].w);
+        const E by = L::all(cur.st[r].w), mean = L::all(-cur.st[r].z);
         E s1 = L::all(0.f), s2 = L::all(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if ((t + k * nt) * V >= A.C) continue;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const E m = e_fma(cur.y[r][k].get(i), by, shift), f = e_mul(G[r][k][i], wq[k][i]);
+            const E m = e_mul(e_add(cur.y[r][k].get(i), mean), by), f = e_mul(G[r][k][i], wq[k][i]);
             s1 = e_add(s1, f);
             s2 = e_fma(f, m, s2);
             sc[k][i] = e_add(sc[k][i], G[r][k][i]);
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const E m1 = L::all(A.post == kLayer ? -s[2 * r] * inv : 0.f), m2 = L::all(A.post != kNone ? -s[2 * r + 1] * inv : 0.f);
-          const E by = L::all(cur.st[r].w), shift = L::all(-cur.st[r].z * cur.st[r].w);
+          const E by = L::all(cur.st[r].w), mean = L::all(-cur.st[r].z);
 #pragma unroll
           for (int k = 0; k < K; ++k) {
             const int c = (t + k * nt) * V;
@@ -691,7 +693,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
             E o[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-              const E m = e_fma(cur.y[r][k].get(i), by, shift);
+              const E m = e_mul(e_add(cur.y[r][k].get(i), mean), by);
               o[i] = e_mul(by, e_fma(m, m2, e_fma(G[r][k][i], wq[k][i], m1)));
             }
             store_piece<T, V>(static_cast<T*>(A.gy) + (row0 + r) * A.C + c, o);

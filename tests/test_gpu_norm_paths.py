@@ -43,3 +43,38 @@ def test_first_calls_of_many_widths_from_many_threads():
     for _ in range(3):
         res = subprocess.run([sys.executable, "-c", THREADS], cwd=root, capture_output=True, text=True, timeout=300)
         assert res.returncode == 0 and res.stdout.strip().endswith("ok"), res.stderr[-3000:]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("channels,rows", [(64, 300), (256, 300), (1024, 90), (2048, 24), (256, 3000)])
+@pytest.mark.parametrize("where", ["pre", "post"])
+def test_gradients_far_from_zero(where, channels, rows, bs_last):
+    """fp32 rows whose mean is some 3000 deviations.  Values are whole numbers near 2^14 and the sum of every 64 channels is a
+    multiple of 64, so that partial sums (integers up to 2^24, multiples of 64 beyond), the mean (the channels
+    are a power of two) and the differences from it are exact in fp32.  What is left are the deviation's rounding and the
+    chains that test_gpu_norm.py counts, 128 u32; doubled, because the seeds have a mean that the gradient takes off."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = 16384 + (2 * torch.randn(rows, channels, device="cuda", generator=g)).round()
+    groups = x.view(rows, -1, 64)
+    groups[..., -1] -= groups.sum(-1) % 64
+    w = torch.randn(channels, device="cuda", generator=g) + 1
+    seed = torch.randn(rows, channels, device="cuda", generator=g) + 1
+    lay = (lambda t: t.t().contiguous()) if bs_last else (lambda t: t)
+    base = torch.zeros_like(x)
+
+    def grads(v, weight, run):
+        v, weight = (t.clone().requires_grad_(True) for t in (v, weight))
+        return torch.autograd.grad(run(v, weight), [v, weight], lay(seed).to(v.dtype))
+
+    def ours(v, weight):
+        if where == "pre":
+            return kb.residual_norm(v, weight=weight, bs_last=bs_last)
+        return kb.residual_norm(lay(base), v, norm=None, post_norm="layer", post_weight=weight, bs_last=bs_last)
+
+    def exact(v, weight):
+        v = lay(v)
+        d = v - v.mean(-1, keepdim=True)
+        return lay(d / torch.sqrt((d * d).mean(-1, keepdim=True) + 1e-5) * weight)
+
+    for a, b in zip(grads(lay(x), w, ours), grads(lay(x.double()), w.double(), exact)):
+        assert ((a.double() - b).norm() / b.norm()).item() <= 256 * 2.0 ** -24
