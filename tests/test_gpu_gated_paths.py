@@ -62,3 +62,26 @@ def test_a_block_with_one_learning_parameter(learns):
     (got,) = torch.autograd.grad(out, [p], seed)
     # (other kernels may run: the bound of a block's gradients in test_gpu_gated_block.py)
     assert err(got, want.double()) <= 72 * unit(torch.bfloat16)
+
+
+@pytest.mark.parametrize("out_last", [False, True])
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("rows,train", [(45, False), (512, False), (2560, False), (2560, True), (2309, True)])
+def test_silu_down_to_the_smallest_numbers(rows, train, bs_last, out_last):
+    """silu(g) between -86 and 10, where a bf16 result is a normal number, element by element, with values of every size
+    next to one another.  The gate is exact (one product by 1); g log2(e), below 125, is rounded to 2^-18, 2^-18.5 of
+    the result; exponential, reciprocal and four products 2^-20; the result 2^-8."""
+    layer, x = layer_and_input([(1, 256, 64, 1)], torch.bfloat16, bs_last, out_last, rows, "silu", train=train)
+    with torch.no_grad():
+        layer.factors[0].zero_()
+        layer.factors[0][:64].copy_(torch.eye(64, device="cuda").repeat(1, 4))   # the gate: feature j takes input j mod 64
+        layer.bias.zero_()
+        layer.bias.view(-1)[256:] = 1                                            # the up projection: 1
+        x.uniform_(-86, 10)
+        x[torch.rand(x.shape, device="cuda") < 0.3] *= 0.02
+    got = layer(x)
+    assert got.requires_grad == train
+    g = (x if bs_last else x.t()).double().repeat(4, 1)
+    want = g / (1 + torch.exp(-g))
+    got = (got if out_last else got.t()).double()
+    assert ((got - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * want.abs()).all()
