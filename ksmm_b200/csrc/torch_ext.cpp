@@ -454,9 +454,13 @@ void differentiable_once() {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "this operator is differentiable once (create_graph=True)");
 }
 
+// a tangent of forward-mode differentiation, which a call through data pointers would lose
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
 // a gated layer without gradients
 bool gated_fits(const at::Tensor& x, const std::vector<at::Tensor>& factors, const Patterns& p, bool last,
                 const c10::optional<at::Tensor>& bias) {
+  if (has_tangent(x) || (bias.has_value() && has_tangent(*bias)) || std::any_of(factors.begin(), factors.end(), has_tangent)) return false;
   return p.n <= 16 && usable(x) && plain_dtype(x) && chain_fits(x, factors, p, last, x.scalar_type(), 2) &&
          bias_fits(bias, x, 2 * p.out(p.n - 1), x.scalar_type());
 }
@@ -612,6 +616,7 @@ struct NormCall {
 
 // Tensors that the kernel takes as they are; everything else goes through Python, which converts or raises.
 bool norm_fits(const at::Tensor& x, const c10::optional<at::Tensor>& y, const NormParams& p, NormCall* c) {
+  if (has_tangent(x) || (y.has_value() && has_tangent(*y))) return false;
   if (!usable(x) || !plain_dtype(x) || x.dim() < 1 || x.dim() > 64 || c->norm < 0 || c->norm > 2 || c->post_norm < 0 || c->post_norm > 2)
     return false;
   c->channels = x.size(c->bs_last ? 0 : x.dim() - 1);
@@ -630,7 +635,7 @@ bool norm_fits(const at::Tensor& x, const c10::optional<at::Tensor>& y, const No
   for (int q = 0; q < kNormParams; ++q) {
     if (!p[q].has_value()) continue;
     const at::Tensor& t = *p[q];
-    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || t.is_conj() || t.device() != x.device()) return false;
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || t.is_conj() || t.device() != x.device() || has_tangent(t)) return false;
     if (any && t.scalar_type() != type) return false;
     type = t.scalar_type();
     any = true;

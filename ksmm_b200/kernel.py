@@ -328,6 +328,13 @@ def differentiable_once():
         raise NotImplementedError("this operator is differentiable once (create_graph=True)")
 
 
+def no_tangents(*tensors):
+    """For operators without forward-mode differentiation, which would lose a tangent."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("this operator has no forward-mode differentiation")
+
+
 def _gated_desc(input, stacked_factors, patterns, bs_last, out_last, bias, activation):
     """Checks the arguments of a gated call; returns its descriptor and (batch, out features, dtype code)."""
     bs_last = int(bool(bs_last))
@@ -376,6 +383,7 @@ def gated_chain_forward(input, stacked_factors, patterns, bs_last, bias=None, ac
         out = _native.gated_forward(input, list(stacked_factors), patterns, bool(bs_last), out_last, bias, _lib.GATES[activation])
         if out is not None:
             return _result(out)
+    no_tangents(input, bias, *stacked_factors)
     lib = _lib.load()
     desc, (batch, feats, code) = _gated_desc(input, stacked_factors, patterns, bs_last, out_last, bias, activation)
     out = torch.empty((feats, batch) if out_last else (batch, feats), dtype=input.dtype, device=input.device)
@@ -438,6 +446,7 @@ def gated_layer(input, stacked_factors, patterns, bs_last, bias=None, activation
         out = _native.gated_layer(input, stacked_factors, patterns, bool(bs_last), out_last, bias, _lib.GATES[activation])
         if out is not None:
             return _result(out)
+    no_tangents(input, bias, *stacked_factors)
     if torch.is_grad_enabled() and (input.requires_grad or any(f.requires_grad for f in stacked_factors)
                                     or (bias is not None and bias.requires_grad)):
         return GatedFunction.apply(input, bias, bool(bs_last), out_last, patterns, activation, *stacked_factors)

@@ -13,7 +13,7 @@ from torch import nn
 
 from . import _lib
 from ._lib import native as _native
-from .kernel import _result, _stream_ptr, differentiable_once, dtype_code
+from .kernel import _result, _stream_ptr, differentiable_once, dtype_code, no_tangents
 
 _ROWS = ("weight", "bias", "post_weight", "post_bias")
 _PER_SAMPLE = ("scale", "shift", "gate")
@@ -172,13 +172,14 @@ def residual_norm(x, y=None, *, norm="layer", post_norm=None, weight=None, bias=
     (rows of any stride: parts of a conditioning network's output are taken as they are).
 
     Returns ``(z, h)``; ``h`` alone without ``y``; ``z`` alone with ``norm=None``.  Differentiable in every
-    tensor.  ``h`` is made from the unrounded ``z``."""
+    tensor, once and in reverse mode.  ``h`` is made from the unrounded ``z``."""
     if _native is not None and isinstance(x, torch.Tensor) and norm in _lib.NORMS and post_norm in _lib.NORMS:
         # one call of the extension module; None where it is not for it (a wrong argument, parameters of two types, ...)
         out = _native.residual_norm(x, y, weight, bias, post_weight, post_bias, scale, shift, gate, _lib.NORMS[norm],
                                     _lib.NORMS[post_norm], alpha, eps, bool(bs_last))
         if out is not None:
             return _result(out)
+    no_tangents(x, y, weight, bias, post_weight, post_bias, scale, shift, gate)
     params = dict(weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, scale=scale, shift=shift, gate=gate)
     x, y, params, sizes = _plan(x, y, params, norm, post_norm, bs_last)
     kinds = (norm, post_norm, float(alpha), float(eps), bool(bs_last))
