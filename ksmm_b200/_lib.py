@@ -258,5 +258,8 @@ def check(status):
 
 
 def int32_array(values):
+    """(ctypes would take a value's low 32 bits without a word)"""
+    if any(not -2 ** 31 <= v < 2 ** 31 for v in values):
+        raise ValueError(f"pattern values are 32-bit integers, got {list(values)}")
     arr = (ctypes.c_int32 * len(values))(*values)
     return arr

@@ -35,6 +35,8 @@ def _plan(x, y, params, norm, post_norm, bs_last):
     channels = x.shape[0] if bs_last else x.shape[-1]
     if channels == 0:
         raise ValueError("x has no channels")
+    if channels >= 2 ** 31:  # (the library takes up to 8192, in a 32-bit field)
+        raise ValueError(f"x has {channels} channels")
     rows = x.numel() // channels
     if y is not None:
         if not isinstance(y, torch.Tensor) or y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:

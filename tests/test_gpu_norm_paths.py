@@ -78,3 +78,12 @@ def test_gradients_far_from_zero(where, channels, rows, bs_last):
 
     for a, b in zip(grads(lay(x), w, ours), grads(lay(x.double()), w.double(), exact)):
         assert ((a.double() - b).norm() / b.norm()).item() <= 256 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("channels", [8193, 2 ** 31, 2 ** 32 + 768])
+def test_more_channels_than_the_library_takes(channels):
+    """(The last one would reach the library as 768 channels.)"""
+    for x, last in ((torch.zeros(1, 1, device="cuda", dtype=torch.float16).expand(1, channels), False),
+                    (torch.zeros(1, 1, device="cuda", dtype=torch.float16).expand(channels, 1), True)):
+        with pytest.raises((ValueError, kb.KsmmError), match="channels"):
+            kb.residual_norm(x, bs_last=last)

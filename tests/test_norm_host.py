@@ -19,3 +19,11 @@ def test_rows_of_a_post_norm_without_one(key):
         assert b"post_norm" in lib.ksmm_cu_last_error()
     assert lib.ksmm_cu_norm_backward_workspace_bytes(ctypes.byref(d)) == 0
     assert lib.ksmm_cu_launch_count() == before
+
+
+def test_pattern_values_keep_their_upper_bits():
+    """A value of 2^32 + 5 must not reach the library as 5."""
+    assert list(_lib.int32_array([1, 2 ** 31 - 1, -1])) == [1, 2 ** 31 - 1, -1]
+    for v in (2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1):
+        with pytest.raises(ValueError, match="32-bit"):
+            _lib.int32_array([1, v, 2, 3])
