@@ -430,8 +430,9 @@ __global__ void __launch_bounds__(RING ? (TPR == 32 ? kRingBlock : kRingWide) : 
   }
   for (; row < end; row += kGroups) {
     if constexpr (RING) {
-      // (a wait that ran out leaves its code; the rows of this block are then not to be used)
-      tc::mbar_wait<0>(bar(slot), phase, &abort_flag, A.status, kNormWaits);
+      // (a wait that ran out leaves its code; the rows of this block are then not to be used, and the slot takes no other
+      // copy: its barrier still expects the last one)
+      const bool arrived = tc::mbar_wait<0>(bar(slot), phase, &abort_flag, A.status, kNormWaits);
       const T* src = reinterpret_cast<const T*>(slots + static_cast<size_t>(slot) * 2 * row_bytes);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -448,7 +449,8 @@ __global__ void __launch_bounds__(RING ? (TPR == 32 ? kRingBlock : kRingWide) : 
       // the row is in registers: its place takes the next one
       if constexpr (TPR == 32) __syncwarp();
       else tc::bar_sync_named(1 + group, TPR);
-      if (t == 0 && row + static_cast<int64_t>(A.stages) * kGroups < run_end) fetch(slot, row + static_cast<int64_t>(A.stages) * kGroups);
+      const int64_t ahead = row + static_cast<int64_t>(A.stages) * kGroups;
+      if (t == 0 && arrived && ahead < run_end) fetch(slot, ahead);
       if (++slot == A.stages) {
         slot = 0;
         phase ^= 1u;
