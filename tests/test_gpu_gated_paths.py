@@ -6,7 +6,8 @@ Tolerances are those of test_gpu_gated.py (n factors, u = eps / 2 of the type, r
 import pytest
 import torch
 
-from ksmm_b200.ksvit import KSGatedFeedForward
+import ksmm_b200 as kb
+from ksmm_b200.ksvit import KSGatedFeedForward, KSViTB
 from test_gpu_gated import LAYOUTS, definition, err, layer_and_input, unit
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +86,105 @@ def test_silu_down_to_the_smallest_numbers(rows, train, bs_last, out_last):
     want = g / (1 + torch.exp(-g))
     got = (got if out_last else got.t()).double()
     assert ((got - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * want.abs()).all()
+
+
+def compare(layer, x, act, out_last):
+    """Forward pass without and with gradients, and every gradient, against the definition."""
+    n, u = len(layer.patterns), unit(layer.dtype)
+    batch = x.numel() // layer.in_size
+    seed = torch.randn(*((layer.out_size, batch) if out_last else (batch, layer.out_size)), device="cuda").to(layer.dtype)
+    want, ref = exact_gradients(layer, x, seed, act, out_last)
+    with torch.no_grad():
+        assert err(layer(x), want) <= 2 * (3 * n + 1) * u
+    leaf = x.detach().clone().requires_grad_(True)
+    h = layer(leaf)
+    assert err(h, want) <= 2 * (3 * n + 1) * u
+    for i, (a, b) in enumerate(zip(torch.autograd.grad(h, [leaf, *params_of(layer)], seed), ref)):
+        assert err(a, b) <= 2 * (5 * n + 5) * u, i
+
+
+def gates_away_from_zero(layer):
+    """Gate biases of 6 and -6, ten deviations of the gates around them: no rounding turns a gate's sign."""
+    with torch.no_grad():
+        half = layer.bias.view(2, -1)[0]
+        half.copy_(torch.where(torch.rand(half.shape, device="cuda") < 0.5, -6.0, 6.0))
+
+
+RAGGED = {"b136": [(4, 96, 96, 1), (1, 136, 96, 4)], "b264": [(2, 64, 64, 1), (1, 264, 64, 2)], "b392": [(2, 392, 192, 1)]}
+
+
+@pytest.mark.parametrize("bs_last,out_last", LAYOUTS)
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "relu", "gelu", None])
+@pytest.mark.parametrize("patterns", list(RAGGED))
+@pytest.mark.parametrize("batch", [2304, 2309])
+def test_two_ctas_and_features_that_fill_no_tile(batch, patterns, act, bs_last, out_last):
+    """From 2048 columns on two CTAs share a tile of 256 features; here a last pair's second CTA has 8 of them, or none."""
+    layer, x = layer_and_input(RAGGED[patterns], torch.bfloat16, bs_last, out_last, batch, act, train=True)
+    if act == "relu":
+        gates_away_from_zero(layer)
+    compare(layer, x, act, out_last)
+
+
+@pytest.mark.parametrize("bs_last,out_last", LAYOUTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("batch", [45, 264])
+def test_gradient_of_relu(batch, dtype, bs_last, out_last):
+    layer, x = layer_and_input([(6, 64, 64, 1), (1, 512, 192, 2)], dtype, bs_last, out_last, batch, "relu", train=True)
+    gates_away_from_zero(layer)
+    compare(layer, x, "relu", out_last)
+
+
+@pytest.mark.parametrize("bs_last,out_last", LAYOUTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("factors", [4, 5, 8, 9, 16])
+def test_long_chains(factors, dtype, bs_last, out_last):
+    """(Weights of a factor are scaled to keep a vector's size.  Layouts are planned up to eight factors.)"""
+    patterns = ([(1, 8, 8, 8), (8, 8, 8, 1)] * 8)[:factors - 1] + [(1, 96, 64, 1)]
+    layer, x = layer_and_input(patterns, dtype, bs_last, out_last, 77, "silu", train=True)
+    with torch.no_grad():
+        for f in layer.factors:
+            f.mul_(3 ** 0.5)
+    compare(layer, x, "silu", out_last)
+
+
+def test_gradients_along_themselves():
+    """fp32, by central differences in the direction of each gradient, where the slope is the gradient's norm.  With a
+    unit direction and a step of 2^-4 an element moves by at most 0.01 or so: the truncation, step^2 / 6 of the third
+    derivative, is 2e-5 times the ratio of third to first derivative (some tens for cubes and products of values near
+    1).  The results' rounding, 1e-6 of 3e5 terms below 1 with random signs, is 1e-3 over twice the step, 1e-2; the
+    gradients' norms are above 30.  Together below 1e-3 of the norm."""
+    torch.manual_seed(3)
+    layer = kb.KSGatedLinear([(6, 64, 64, 1), (1, 512, 192, 2)], dtype=torch.float32, requires_grad=True)
+    rows = lambda *s: torch.randn(*s, device="cuda", requires_grad=True)
+    args = (rows(300, 384), rows(300, 384), rows(384), rows(3, 384), *layer.parameters())
+
+    def f(x, y, w, sc, *params):
+        with torch.no_grad():
+            for p, v in zip(layer.parameters(), params):
+                p.copy_(v)
+        z, n = kb.residual_norm(x, y, norm="rms", post_norm="layer", weight=w, scale=sc, gate=w, alpha=0.75)
+        return layer(n).double().pow(2).sum() + z.double().pow(3).sum() * 0.1
+
+    start = [a.detach().clone() for a in args]
+    grads = torch.autograd.grad(f(*args[:4], *start[4:]), args)
+    step = 2.0 ** -4
+    for i, g in enumerate(grads):
+        size = g.double().norm().item()
+        assert size > 30
+        v = g / size
+        with torch.no_grad():
+            plus = f(*[t + step * v if j == i else t for j, t in enumerate(start)])
+            minus = f(*[t - step * v if j == i else t for j, t in enumerate(start)])
+        slope = ((plus - minus) / (2 * step)).item()
+        assert abs(slope - size) <= 1e-3 * size, (i, slope, size)
+
+
+def test_gradients_through_a_network():
+    """Every learning parameter of a network of gated blocks gets a finite gradient that is not 0."""
+    torch.manual_seed(5)
+    net = KSViTB(dtype=torch.bfloat16, depth=2, gated_mlp=True)
+    for p in net.parameters():
+        p.requires_grad_(True)
+    net(torch.randn(2, 3, 224, 224, device="cuda").bfloat16()).float().pow(2).mean().backward()
+    for name, p in net.named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad.float()).all() and p.grad.float().norm() > 0, name

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import ksmm_b200 as kb
+from test_gpu_norm import EVERY, check
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,13 @@ def test_more_channels_than_the_library_takes(channels):
                     (torch.zeros(1, 1, device="cuda", dtype=torch.float16).expand(channels, 1), True)):
         with pytest.raises((ValueError, kb.KsmmError), match="channels"):
             kb.residual_norm(x, bs_last=last)
+
+
+@pytest.mark.parametrize("alpha", [-1.25, 0.5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,bs_last", [((45, 96), False), ((45, 1303), False), ((2400, 768), False), ((601, 2304), False),
+                                           ((9, 8192), False), ((384, 70), True), ((1000, 33), True), ((2304, 66), True)])
+def test_scaled_streams(shape, bs_last, dtype, alpha):
+    """alpha in every kernel: rows by groups, single elements, resident blocks, wide rows, columns, turned columns."""
+    check(dtype, shape, norm="layer", post_norm="rms", bs_last=bs_last, samples=1, keys=EVERY, alpha=alpha)
+    check(dtype, shape, norm="rms", bs_last=bs_last, keys=("weight", "shift"), alpha=alpha)
