@@ -315,6 +315,9 @@ class KSLinearGroup(nn.Module):
         return tuple(first.post_process(tensor, out[g]) for g in range(len(self.layers)))
 
 
+_FACTOR_NAMES = tuple(str(f) for f in range(_k.MAX_GATED_FACTORS))
+
+
 class KSGatedLinear(nn.Module):
     r"""``activation(gate(x)) * up(x)`` with two Kronecker-sparse layers of the same patterns: the first half of a
     gated feed-forward block (``KSLinear`` is the second).  The reference builds feed-forward blocks from
@@ -384,9 +387,11 @@ class KSGatedLinear(nn.Module):
         x = tensor
         if x.dim() != 2:
             x = x.reshape(x.size(0), -1) if self.bs_last else x.reshape(-1, x.size(-1))
-        # (a ParameterList takes longer to walk than the call to launch)
-        y = _k.gated_layer(x.contiguous(), list(self.factors._parameters.values()), self.patterns, self.bs_last, self.bias,
-                           self.activation, self.out_bs_last)
+        # (a ParameterList takes longer to walk than the call to launch.  Its dictionary serves where it holds the factors in
+        # order: pruning and parametrisations keep their originals there under other names)
+        held = self.factors._parameters
+        factors = list(held.values()) if tuple(held) == _FACTOR_NAMES[:self.num_mat] else list(self.factors)
+        y = _k.gated_layer(x.contiguous(), factors, self.patterns, self.bs_last, self.bias, self.activation, self.out_bs_last)
         if tensor.dim() == 2 or self.out_bs_last != bool(self.bs_last):
             return y
         if self.bs_last:

@@ -5,6 +5,8 @@ Tolerances are those of test_gpu_gated.py (n factors, u = eps / 2 of the type, r
 """
 import pytest
 import torch
+import torch.nn.utils.parametrize
+import torch.nn.utils.prune
 
 import ksmm_b200 as kb
 from ksmm_b200.ksvit import KSGatedFeedForward, KSViTB
@@ -188,3 +190,30 @@ def test_gradients_through_a_network():
     net(torch.randn(2, 3, 224, 224, device="cuda").bfloat16()).float().pow(2).mean().backward()
     for name, p in net.named_parameters():
         assert p.grad is not None and torch.isfinite(p.grad.float()).all() and p.grad.float().norm() > 0, name
+
+
+class Doubled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
+
+
+@pytest.mark.parametrize("how", ["pruned", "parametrised", "replaced"])
+def test_factors_that_are_not_plain_parameters(how):
+    """The layer computes with what its ParameterList gives, factor by factor (all of one shape here)."""
+    torch.manual_seed(6)
+    layer = kb.KSGatedLinear([(1, 64, 64, 1)] * 3, dtype=torch.float32, requires_grad=True)
+    x = torch.randn(33, 64, device="cuda")
+    before = layer(x).detach()
+    if how == "pruned":
+        torch.nn.utils.prune.random_unstructured(layer.factors, "0", 0.5)
+    elif how == "parametrised":
+        torch.nn.utils.parametrize.register_parametrization(layer.factors, "1", Doubled())
+    else:
+        layer.factors[0] = torch.nn.Parameter(3 * layer.factors[0].detach())
+    factors = [f.detach() for f in layer.factors]
+    got = layer(x)
+    assert torch.equal(got, kb.kernel.gated_layer(x, [f.requires_grad_(True) for f in factors], layer.patterns, False, layer.bias))
+    assert not torch.allclose(got, before, rtol=1e-3, atol=1e-3)
+    assert all(p.grad is None for p in layer.parameters())
+    got.sum().backward()
+    assert all(p.grad is not None for p in layer.parameters())
