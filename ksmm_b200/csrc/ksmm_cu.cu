@@ -2278,6 +2278,9 @@ int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* grad_outpu
   for (int f = 0; f < D.nfactors; ++f)
     if (D.layouts[f] != 0 && D.layouts[f] != 1) return set_error(KSMM_ERR_BAD_ARGUMENT, "layouts are those of the forward pass");
   const bool one_layout = train_one_layout(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last);
+  const size_t kept = gated_saved_bytes(D.nfactors, D.patterns, one_layout ? D.batch : padded_ld(D.batch, es), es);
+  if (reinterpret_cast<uintptr_t>(D.saved) % 256 || D.saved_bytes < kept)
+    return set_error(KSMM_ERR_WORKSPACE, "gated backward: need the %zu bytes kept, aligned to 256, got %zu", kept, D.saved_bytes);
   bool aligned = aligned16(grad_input) && aligned_values(D);
   for (int f = 0; f < D.nfactors; ++f) aligned = aligned && aligned16(grad_values[f]);
   const bool allow = aligned && train_may_switch(D.nfactors, D.patterns, D.batch, D.dtype, D.bs_last, true, grad_input != nullptr);
