@@ -744,8 +744,18 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
   return KSMM_OK;
 }
 
-// Two CTAs per tile where there are two feature tiles for them and rows enough to keep the MMAs busy
-bool use_pair(const Problem& p) { return p.c <= 3 * kKC && p.b > 128 && p.batch >= 2048; }
+// Two CTAs per tile where that is faster: three chunks of k (a single CTA then has a shorter ring), features that fill the
+// pairs' tiles, and ten tiles or more for every pair of SMs.  Calls of two-factor layers in bf16, 25088 rows if not
+// said otherwise, single CTAs against pairs:
+//   768 -> 2048, (1,512,192,4) last: 93.1 and 92.5 us, training step 437 and 423; 8192 rows (7 tiles) 34.9 and 35.7
+//   768 -> 4096, (1,1024,192,4): 149 and 147, training 710 and 683; 4096 rows (7 tiles) 33.7 and 34.0
+//   1536 -> 1600, (1,200,192,8): 122.0 and 121.0, training 495 and 487; 4096 rows 29.0 and 29.6
+// and where the rule says single: 512 -> 4096, (1,512,64,8), two chunks less: 110.7 and 112.9; 1024 -> 2816,
+// (1,352,128,8), four of six tiles' features exist: 111 and 129; 768 -> 1536, (1,384,192,4), three of four: 78.6 and 89.0.
+bool use_pair(const Problem& p) {
+  const int64_t tiles = (p.batch + 127) / 128 * p.a * p.d * ((p.b + 255) / 256);
+  return p.c > 2 * kKC && p.c <= 3 * kKC && (p.b - 1) % 256 >= 128 && tiles >= 5 * num_sms();
+}
 
 template <bool IN_LAST, bool OUT_LAST>
 int launch_layout(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t stream, bool turn) {

@@ -28,7 +28,7 @@ def exact_gradients(layer, x, seed, act, out_last):
 
 
 @pytest.mark.parametrize("batch", [1995, 6501])
-@pytest.mark.parametrize("patterns", [[(1, 512, 64, 8)], [(2, 96, 64, 16)]], ids=["pairs", "one_tile"])
+@pytest.mark.parametrize("patterns", [[(1, 512, 160, 8)], [(1, 512, 64, 8)], [(2, 96, 64, 16)]], ids=["pairs", "four_tiles", "one_tile"])
 @pytest.mark.parametrize("bs_last", [False, True])
 def test_kept_halves_of_many_ragged_tiles(patterns, batch, bs_last):
     """Training with batch-last outputs whose rows no tensor map addresses: every CTA walks several tiles (3 to 12
@@ -119,9 +119,23 @@ RAGGED = {"b136": [(4, 96, 96, 1), (1, 136, 96, 4)], "b264": [(2, 64, 64, 1), (1
 @pytest.mark.parametrize("act", ["silu", "sigmoid", "relu", "gelu", None])
 @pytest.mark.parametrize("patterns", list(RAGGED))
 @pytest.mark.parametrize("batch", [2304, 2309])
-def test_two_ctas_and_features_that_fill_no_tile(batch, patterns, act, bs_last, out_last):
-    """From 2048 columns on two CTAs share a tile of 256 features; here a last pair's second CTA has 8 of them, or none."""
+def test_features_that_fill_no_tile(batch, patterns, act, bs_last, out_last):
+    """Tiles of 128 features of which the last has 8."""
     layer, x = layer_and_input(RAGGED[patterns], torch.bfloat16, bs_last, out_last, batch, act, train=True)
+    if act == "relu":
+        gates_away_from_zero(layer)
+    compare(layer, x, act, out_last)
+
+
+@pytest.mark.parametrize("bs_last,out_last", LAYOUTS)
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "relu", "gelu", None])
+@pytest.mark.parametrize("patterns,batch", [([(1, 512, 192, 4)], 12301), ([(1, 392, 160, 8)], 6200), ([(2, 200, 192, 4)], 12304),
+                                            ([(4, 512, 192, 1)], 12304), ([(1, 512, 136, 8)], 6147)])
+def test_two_ctas(patterns, batch, act, bs_last, out_last):
+    """Two CTAs of a cluster share a tile of 256 features (many tiles, blocks of 129 to 192 inputs): the second one of a
+    last pair with all, 72 or 8 of its features; rows that a tensor map addresses or not; a pass over k that ends
+    inside a chunk; with one block per feature group also a batch-first input."""
+    layer, x = layer_and_input(patterns, torch.bfloat16, bs_last, out_last, batch, act, train=True)
     if act == "relu":
         gates_away_from_zero(layer)
     compare(layer, x, act, out_last)
