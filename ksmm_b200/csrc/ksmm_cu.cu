@@ -1868,7 +1868,9 @@ static int gated_walk(bool run, const ksmm_gated_desc_t& D, int out_last, bool k
   // (without `allow` pointers may start anywhere)
   const bool fuse = allow && !one_layout && tc_gated_fits(pl, batch, D.dtype, plan.in_last[n - 1], L);
   // A few tokens: the fused kernel stores its batch-last tiles batch-first, two bytes at a time, which takes less than
-  // the launch of a transpose (16 rows 384 -> 1024: 21 -> 12 us).
+  // a transpose and its launch: 256 rows 768 -> 2048 in (4,192,192,1) (1,512,192,4) bf16 16.4 -> 14.2 us, 384 -> 1024
+  // 16.4 -> 12.8, 1024 -> 2816 in (8,128,128,1) (1,352,128,8) 16.4 -> 15.9.  From 512 rows on blocks interleaved by
+  // eight lose by it (16.4 and 17.3, 1024 rows 18.6 and 23.1); by four they lose from 1536 on (24.6 and 25.1).
   const bool turn = fuse && plan.post && L == 1 && batch <= 256;
   if (turn) plan.post = false;
   const bool pad_in = ld != batch && D.bs_last && !plan.pre && p0[1] >= 32 && p0[2] >= 16;
