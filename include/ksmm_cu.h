@@ -424,7 +424,8 @@ KSMM_API int ksmm_cu_gated_backward(const ksmm_gated_desc_t* desc, const void* g
  * not NULL, 4 floats per token for the backward pass.  The reference composes these steps from separate
  * PyTorch calls (src/ksmm_py/model/vit.py:416-431, 770-800).
  * ksmm_cu_norm_backward reads grad_z and / or grad_h, the forward's x or z, y and stats, and the
- * parameters; writes those of grad_* that are not NULL: grad_x and grad_y laid out as x and y, the others
+ * parameters: with a y it reads z, and not x; 16-bit calls whose z is NULL form it again from x and y, unrounded.  It
+ * writes those of grad_* that are not NULL: grad_x and grad_y laid out as x and y, the others
  * contiguous rows of param_dtype (grad_scale, grad_shift, grad_gate: `samples` rows where their stride is not 0).
  * Its sums over tokens have a fixed order.  Workspaces of the sizes that the two ..._workspace_bytes calls give
  * (often 0), aligned to 16 bytes as stats is.  Up to 8192 channels; outputs overlap no input.

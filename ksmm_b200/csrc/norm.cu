@@ -18,14 +18,16 @@
 //   gate: post_weight D + post_bias C, post_weight: sum gate D, post_bias: sum gate C.
 //
 // All of it is bound by memory: each tensor is read once and written once.  Statistics, sums and the value
-// h is made from stay in fp32; z and h are rounded once.  The backward pass reads the rounded z and the
-// statistics of the unrounded one (16 bytes per token).  Sums over tokens are formed in a fixed order: a
+// h is made from stay in fp32; z and h are rounded once.  The backward pass of 16-bit tensors forms the unrounded
+// z again from x and y, which takes no more bytes than reading the rounded one (that it reads if it is given z): 20
+// deviations from 0 the rounding of z costs 2 % of a gradient in bf16.  It reads the statistics (16 bytes per token).  Sums over tokens are formed in a fixed order: a
 // CTA sums its own run of tokens, two small kernels add the runs up; no atomics.
 //
 // The stock form in the reference's models is a chain of separate PyTorch calls: LayerNorm and the sum around
 // attention and feed-forward block (src/ksmm_py/model/vit.py:416-431, 770-800).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "backward.h"
 #include "common.cuh"
@@ -56,6 +58,7 @@ struct Args {
   int64_t samples;
   int chunks;     // chunks of tokens of one sample
   int C, pre, post, p32;  // p32: parameters are fp32
+  int remake;     // backward, 16 bits: z_in is x, and z is formed from it and y
   float alpha, eps;
   int stages;     // rows in flight per group of threads
   int* status;    // where a wait that ran out leaves its code
@@ -547,8 +550,15 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
   using E = typename L::E;
   constexpr int N = L::N;
   __shared__ float red[2 * 32 * 2 * R];
+  extern __shared__ float4 coef[];  // remake with a post norm, wide rows: gate * post_bias of every thread's pieces
   int turn = 0;
   const int t = threadIdx.x, nt = blockDim.x;
+  // (quarters of a piece apart: a warp's reads are whole lines)
+  auto shift_at = [&](int k, int i) {
+    const int c = (t + k * nt) * V;
+    if constexpr (V == 1) return reinterpret_cast<float*>(coef) + c;
+    else return reinterpret_cast<E*>(coef + (i / 2) * (A.C / V) + c / V) + i % 2;
+  };
   const int64_t sample = blockIdx.x / A.chunks;
   const int chunk = static_cast<int>(blockIdx.x % A.chunks);
   const int64_t begin = sample * A.per_sample + A.per_sample * chunk / A.chunks;
@@ -583,11 +593,12 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
   load(cur, begin);
   E wp[K][N], wq[K][N];  // weight (1 + scale), gate * post_weight
   E sa[K][N], sb[K][N], sc[K][N], sd[K][N];
+  E wb[K][N];                // gate * post_bias, narrow rows
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (t + k * nt) * V;
 #pragma unroll
-    for (int i = 0; i < N; ++i) wp[k][i] = wq[k][i] = sa[k][i] = sb[k][i] = sc[k][i] = sd[k][i] = L::all(0.f);
+    for (int i = 0; i < N; ++i) wp[k][i] = wq[k][i] = wb[k][i] = sa[k][i] = sb[k][i] = sc[k][i] = sd[k][i] = L::all(0.f);
     if (c < A.C) {
       E q[N];
       load_param<T, V>(A, A.weight, 0, c, 1.f, wp[k]);
@@ -596,45 +607,88 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1) norm_rows_backward_
       for (int i = 0; i < N; ++i) wp[k][i] = e_fma(wp[k][i], q[i], wp[k][i]);
       load_param<T, V>(A, A.gate, sample, c, 1.f, wq[k]);
       if (A.post != kNone) {
+        if (sizeof(T) == 2 && A.remake) {  // (a thread reads back what it writes)
+          load_param<T, V>(A, A.post_bias, 0, c, 0.f, q);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if constexpr (MAXT == 128) wb[k][i] = e_mul(wq[k][i], q[i]);
+            else *shift_at(k, i) = e_mul(wq[k][i], q[i]);
+          }
+        }
         load_param<T, V>(A, A.post_weight, 0, c, 1.f, q);
 #pragma unroll
         for (int i = 0; i < N; ++i) wq[k][i] = e_mul(wq[k][i], q[i]);
       }
     }
   }
+  // the normalised value of pre, 16 bits
+  auto n_at = [&](int r, int k, int i) {
+    E z = cur.z[r][k].get(i);
+    if (A.remake) {
+      E p = e_mul(e_add(cur.y[r][k].get(i), L::all(-cur.st[r].z)), L::all(cur.st[r].w));  // (y itself without a post norm)
+      p = A.post != kNone && (t + k * nt) * V < A.C ? e_fma(p, wq[k][i], *shift_at(k, i)) : e_mul(p, wq[k][i]);
+      z = e_fma(L::all(A.alpha), z, p);
+    }
+    return e_mul(e_add(z, L::all(-cur.st[r].x)), L::all(cur.st[r].y));
+  };
   for (int64_t row0 = begin; row0 < end; row0 += R) {
     load(next, row0 + R);
     E G[R][K][N];
     if (ghp) {
       float s[2 * R];
+      // z as it lies in memory (0), or from x and y without (1) and with (2) a post norm; 3 finds out value by value,
+      // which is what wide rows want (32768 x 4096 bf16 without a post norm, forward and backward: 586 us with three
+      // loops, 524 with one, 550 from the rounded z; 50432 x 768 with one: 224, 234, 216)
+      auto pass = [&](auto way) {
+        constexpr int kWay = decltype(way)::value;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const E by = L::all(cur.st[r].y), mean = L::all(-cur.st[r].x);
-        E s1 = L::all(0.f), s2 = L::all(0.f);
+        for (int r = 0; r < R; ++r) {
+          const E by = L::all(cur.st[r].y), mean = L::all(-cur.st[r].x);
+          const E by_y = L::all(cur.st[r].w), mean_y = L::all(-cur.st[r].z), al = L::all(A.alpha);
+          E s1 = L::all(0.f), s2 = L::all(0.f);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+          for (int k = 0; k < K; ++k) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const E g = cur.gh[r][k].get(i), n = e_mul(e_add(cur.z[r][k].get(i), mean), by);
-            const E w = e_mul(g, wp[k][i]);
-            s1 = e_add(s1, w);
-            s2 = e_fma(w, n, s2);
-            sa[k][i] = e_add(sa[k][i], g);
-            sb[k][i] = e_fma(g, n, sb[k][i]);
+            for (int i = 0; i < N; ++i) {
+              const E g = cur.gh[r][k].get(i);
+              E z = cur.z[r][k].get(i);
+              if constexpr (kWay == 1) z = e_fma(al, z, e_mul(cur.y[r][k].get(i), wq[k][i]));
+              if constexpr (kWay == 2)
+                z = e_fma(al, z, e_fma(e_mul(e_add(cur.y[r][k].get(i), mean_y), by_y), wq[k][i], wb[k][i]));
+              E n;
+              if constexpr (kWay == 3) n = n_at(r, k, i);
+              else n = e_mul(e_add(z, mean), by);
+              const E w = e_mul(g, wp[k][i]);
+              G[r][k][i] = n;
+              s1 = e_add(s1, w);
+              s2 = e_fma(w, n, s2);
+              sa[k][i] = e_add(sa[k][i], g);
+              sb[k][i] = e_fma(g, n, sb[k][i]);
+            }
           }
-        s[2 * r] = e_sum(s1);
-        s[2 * r + 1] = e_sum(s2);
+          s[2 * r] = e_sum(s1);
+          s[2 * r + 1] = e_sum(s2);
+        }
+      };
+      if constexpr (sizeof(T) == 4) {
+        pass(std::integral_constant<int, 0>());
+      } else if constexpr (MAXT > 128) {
+        pass(std::integral_constant<int, 3>());
+      } else {
+        if (!A.remake) pass(std::integral_constant<int, 0>());
+        else if (A.post == kNone) pass(std::integral_constant<int, 1>());
+        else pass(std::integral_constant<int, 2>());
       }
       block_sum<2 * R>(s, red, turn);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const E m1 = L::all(A.pre == kLayer ? -s[2 * r] * inv : 0.f), m2 = L::all(-s[2 * r + 1] * inv);
-        const E by = L::all(cur.st[r].y), mean = L::all(-cur.st[r].x);
+        const E by = L::all(cur.st[r].y);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const E n = e_mul(e_add(cur.z[r][k].get(i), mean), by);
+            const E n = G[r][k][i];
             G[r][k][i] = e_fma(by, e_fma(n, m2, e_fma(cur.gh[r][k].get(i), wp[k][i], m1)), cur.gz[r][k].get(i));
           }
       }
@@ -850,17 +904,14 @@ __device__ __forceinline__ float reduce_scatter(float (&v)[32]) {
 template <typename T>
 __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(const Args A) {
   __shared__ float red[kColWarps * 32];
-  extern __shared__ float2 pair[];  // per channel: weight (1 + scale), gate * post_weight
+  extern __shared__ float4 coef[];  // per channel: gate * post_weight, gate * post_bias, weight (1 + scale); then n
+  float* const nc = reinterpret_cast<float*>(coef + A.C);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t sample = blockIdx.x / A.chunks;
   const int64_t in_sample = static_cast<int64_t>(blockIdx.x % A.chunks) * 32 + lane;
   const bool live = in_sample < A.per_sample;
   const int64_t tok = sample * A.per_sample + (live ? in_sample : 0);
-  for (int c = threadIdx.x; c < A.C; c += kColWarps * 32)
-  {
-    const float4 q = combined<T>(A, sample, c);
-    pair[c] = make_float2(q.z, q.x);
-  }
+  for (int c = threadIdx.x; c < A.C; c += kColWarps * 32) coef[c] = combined<T>(A, sample, c);
   __syncthreads();
   const T* zp = static_cast<const T*>(A.z_in) + tok;
   const T* yp = A.y ? static_cast<const T*>(A.y) + tok : nullptr;
@@ -875,9 +926,14 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll 8
     for (int c = warp; c < A.C; c += kColWarps) {
-      const float w = (live ? at(ghp, c) : 0.f) * pair[c].x;
+      const float4 q = coef[c];
+      const float w = (live ? at(ghp, c) : 0.f) * q.z;
+      float z = at(zp, c);
+      if (sizeof(T) == 2 && A.remake) z = fmaf(A.alpha, z, A.post != kNone ? fmaf((at(yp, c) - st.z) * st.w, q.x, q.y) : q.x * at(yp, c));
+      const float n = (z - st.x) * st.y;
+      nc[c * 32 + lane] = n;
       s1 += w;
-      s2 = fmaf(w, (at(zp, c) - st.x) * st.y, s2);
+      s2 = fmaf(w, n, s2);
     }
     if (A.pre == kLayer) m1 = column_sum(s1, red) * inv;
     m2 = column_sum(s2, red) * inv;
@@ -885,7 +941,7 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
   auto G_at = [&](int c, float gh, float n) {
     float g = live && gzp ? at(gzp, c) : 0.f;
     if (ghp) {
-      const float w = gh * pair[c].x;
+      const float w = gh * coef[c].z;
       g = fmaf(st.y, w - m1 - n * m2, g);
     }
     return live ? g : 0.f;
@@ -894,8 +950,8 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll 8
     for (int c = warp; c < A.C; c += kColWarps) {
-      const float gh = live && ghp ? at(ghp, c) : 0.f, n = ghp ? (at(zp, c) - st.x) * st.y : 0.f;
-      const float f = G_at(c, gh, n) * pair[c].y;
+      const float gh = live && ghp ? at(ghp, c) : 0.f, n = ghp ? nc[c * 32 + lane] : 0.f;
+      const float f = G_at(c, gh, n) * coef[c].x;
       s1 += f;
       s2 = fmaf(f, (at(yp, c) - st.z) * st.w, s2);
     }
@@ -914,14 +970,14 @@ __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(c
       if (ok) {
         if (ghp) {
           gh = live ? at(ghp, c) : 0.f;
-          n = (at(zp, c) - st.x) * st.y;
+          n = nc[c * 32 + lane];
         }
         G = G_at(c, gh, n);
         if (live && A.gx) static_cast<T*>(A.gx)[c * A.rows + tok] = ElemTraits<T>::from_float(A.alpha * G);
         if (yp) {
           m = (at(yp, c) - st.z) * st.w;
           if (live && A.gy) {
-            const float f = G * pair[c].y - q1 - m * q2;
+            const float f = G * coef[c].x - q1 - m * q2;
             static_cast<T*>(A.gy)[c * A.rows + tok] = ElemTraits<T>::from_float(st.w * f);
           }
         }
@@ -1068,10 +1124,14 @@ bool vector_rows(const ksmm_norm_desc_t& d) {
   return (static_cast<int64_t>(d.channels) * es) % 16 == 0;
 }
 
+// does the backward pass form z from x and y?
+bool remakes_z(const ksmm_norm_desc_t& d) { return d.y && !d.z && d.grad_h && d.dtype != KSMM_F32; }
+
 Args args_of(const ksmm_norm_desc_t& d) {
   Args A = {};
   A.x = d.x; A.y = d.y; A.z = d.z; A.h = d.h;
-  A.z_in = d.y ? d.z : d.x;
+  A.remake = remakes_z(d);
+  A.z_in = d.y && !A.remake ? d.z : d.x;
   A.gz = d.grad_z; A.gh = d.grad_h; A.gx = d.grad_x; A.gy = d.grad_y;
   A.stats = reinterpret_cast<float4*>(d.stats);
   A.weight = {d.weight, 0}; A.bias = {d.bias, 0};
@@ -1163,7 +1223,7 @@ int launch_rows_backward(const Args& A, cudaStream_t stream) {
   const int k = (pieces + 511) / 512;
   auto go = [&](auto kern, int kk) {
     const int n = ((pieces + kk - 1) / kk + 31) / 32 * 32;
-    kern<<<static_cast<unsigned>(grid), n, 0, stream>>>(A);
+    kern<<<static_cast<unsigned>(grid), n, A.remake && A.post != kNone ? A.C * sizeof(float) : 0, stream>>>(A);
     return launched("norm backward");
   };
   if constexpr (V > 1) {
@@ -1249,9 +1309,9 @@ int turn_in(const ksmm_norm_desc_t& d, bool backward, char* ws, cudaStream_t str
     r->t.h = out(d.norm != kNone ? d.h : nullptr);
     return st;
   }
-  if (d.grad_h) {  // the value that pre normalised
-    void* z = in(d.y ? d.z : d.x, &st);
-    if (d.y) r->t.z = z;
+  if (d.grad_h) {  // the value that pre normalised, or x to form it from
+    void* z = in(d.y && !remakes_z(d) ? d.z : d.x, &st);
+    if (d.y && !remakes_z(d)) r->t.z = z;
     else r->t.x = z;
     r->t.grad_h = in(d.grad_h, &st);
   }
@@ -1305,8 +1365,11 @@ int backward_typed(const ksmm_norm_desc_t& d, void* workspace, cudaStream_t stre
   A.part = sums ? static_cast<float*>(workspace) : nullptr;
   int st;
   if (d.bs_last) {
-    static_assert(kColumnChannels * sizeof(float2) <= 48 * 1024, "more needs a word with the driver");
-    const size_t smem = static_cast<size_t>(A.C) * sizeof(float2);
+    constexpr size_t per_channel = sizeof(float4) + 32 * sizeof(float);
+    const size_t smem = A.C * per_channel;
+    static Granted granted;
+    st = allow_smem(reinterpret_cast<const void*>(norm_columns_backward_kernel<T>), smem, kColumnChannels * per_channel, granted);
+    if (st != KSMM_OK) return st;
     norm_columns_backward_kernel<T><<<static_cast<unsigned>(chunks * d.samples), kColWarps * 32, smem, stream>>>(A);
     st = launched("norm backward");
   } else {
@@ -1430,7 +1493,7 @@ int ksmm_cu_norm_backward(const ksmm_norm_desc_t* d, void* workspace, size_t wor
     }
     return KSMM_OK;
   }
-  if (!d->stats || (d->norm != kNone && d->grad_h && !(d->y ? d->z : d->x)) || (!d->grad_z && !d->grad_h))
+  if (!d->stats || (d->norm != kNone && d->grad_h && !(d->y && !remakes_z(*d) ? d->z : d->x)) || (!d->grad_z && !d->grad_h))
     return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
   if (d->grad_h && d->norm == kNone) return set_error(KSMM_ERR_BAD_ARGUMENT, "a gradient of h without a norm");
   if (d->grad_z && !d->y) return set_error(KSMM_ERR_BAD_ARGUMENT, "a gradient of z without y");

@@ -710,7 +710,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const NormCall c{ints[0], ints[1], ints[2], alpha, eps, ints[3], ints[4], ints[5], static_cast<int>(ints[6])};
     at::Tensor z, h, stats;
     raise_status(norm_run(x, y, p, c, &z, &h, &stats));
-    torch::autograd::variable_list keep{y.has_value() ? z : x, y.has_value() ? *y : at::Tensor(), stats};
+    // (what pre normalised: 16-bit calls form it again from x and y, unrounded)
+    torch::autograd::variable_list keep{y.has_value() && x.scalar_type() == at::kFloat ? z : x, y.has_value() ? *y : at::Tensor(), stats};
     for (const auto& t : p) keep.push_back(t.has_value() ? *t : at::Tensor());
     ctx->save_for_backward(std::move(keep));
     ctx->saved_data["ints"] = std::move(ints);
@@ -727,7 +728,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     differentiable_once();
     const auto kept = ctx->get_saved_variables();
     const std::vector<int64_t> ints = ctx->saved_data["ints"].toIntVector();
-    const at::Tensor& z = kept[0];
+    const at::Tensor& x = kept[0];
     const bool has_y = kept[1].defined();
     c10::optional<at::Tensor> y;
     if (has_y) y = kept[1];
@@ -741,16 +742,16 @@ struct NormNode : torch::autograd::Function<NormNode> {
     if (has_y) gz = grads[0];
     if (c.norm) gh = grads.back();
     if (!gz.defined() && !gh.defined()) return r;
-    const c10::cuda::CUDAGuard guard(z.device());
-    ksmm_norm_desc_t d = norm_desc(z, y, p, c);
-    d.z = z.data_ptr();
+    const c10::cuda::CUDAGuard guard(x.device());
+    ksmm_norm_desc_t d = norm_desc(x, y, p, c);
+    if (x.scalar_type() == at::kFloat) d.z = x.data_ptr();
     d.stats = kept[2].data_ptr<float>();
     if (gz.defined()) {
-      gz = gz.to(z.scalar_type()).contiguous();
+      gz = gz.to(x.scalar_type()).contiguous();
       d.grad_z = gz.data_ptr();
     }
     if (gh.defined()) {
-      gh = gh.to(z.scalar_type()).contiguous();
+      gh = gh.to(x.scalar_type()).contiguous();
       d.grad_h = gh.data_ptr();
     }
     // edges of the graph: x, y if there is one, the parameters that there are
@@ -760,17 +761,17 @@ struct NormNode : torch::autograd::Function<NormNode> {
       r[at] = at::empty(like.sizes(), like.options().requires_grad(false));
       return r[at].data_ptr();
     };
-    d.grad_x = wanted(true, z, 0);
-    d.grad_y = wanted(has_y, z, 1);
+    d.grad_x = wanted(true, x, 0);
+    d.grad_y = wanted(has_y, x, 1);
     void** const outs[kNormParams] = {&d.grad_weight, &d.grad_bias, &d.grad_post_weight, &d.grad_post_bias,
                                       &d.grad_scale, &d.grad_shift, &d.grad_gate};
     for (int q = 0; q < kNormParams; ++q)
-      *outs[q] = wanted(p[q].has_value(), p[q].has_value() ? *p[q] : z, 2 + q);
+      *outs[q] = wanted(p[q].has_value(), p[q].has_value() ? *p[q] : x, 2 + q);
     // (sizes of a cut row are dense in a new tensor: the kernel writes rows one after the other)
     const size_t need = ksmm_cu_norm_backward_workspace_bytes(&d);
     at::Tensor ws;
-    if (need) ws = new_bytes(need, z);
-    raise_status(ksmm_cu_norm_backward(&d, need ? ws.data_ptr() : nullptr, need, stream_of(z)));
+    if (need) ws = new_bytes(need, x);
+    raise_status(ksmm_cu_norm_backward(&d, need ? ws.data_ptr() : nullptr, need, stream_of(x)));
     return r;
   }
 };

@@ -88,7 +88,7 @@ def _desc(x, y, z, params, sizes, kinds):
                       post_norm=_lib.NORMS[post_norm], bs_last=int(bool(bs_last)), dtype=dtype_code(x.dtype),
                       param_dtype=dtype_code(ptype), alpha=float(alpha), eps=float(eps))
     if y is not None:
-        d.y, d.z = y.data_ptr(), z.data_ptr()
+        d.y, d.z = y.data_ptr(), None if z is None else z.data_ptr()
     for k, p in params.items():
         if p is None:
             continue
@@ -120,7 +120,8 @@ class NormFunction(torch.autograd.Function):
     def forward(ctx, x, y, sizes, kinds, *params):
         named = dict(zip(_PARAMS, params))
         z, h, stats = _forward(x, y, named, sizes, kinds, True)
-        ctx.save_for_backward(x if y is None else z, y, stats, *params)
+        # (what pre normalised: 16-bit calls form it again from x and y, unrounded)
+        ctx.save_for_backward(z if y is not None and x.dtype == torch.float32 else x, y, stats, *params)
         ctx.plan = (sizes, kinds)
         ctx.set_materialize_grads(False)
         return (h,) if z is None else (z,) if h is None else (z, h)
@@ -128,7 +129,7 @@ class NormFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         differentiable_once()
-        z, y, stats, *params = ctx.saved_tensors
+        x, y, stats, *params = ctx.saved_tensors
         sizes, kinds = ctx.plan
         grad_z = grads[0] if y is not None else None
         grad_h = grads[-1] if kinds[0] is not None else None
@@ -136,14 +137,14 @@ class NormFunction(torch.autograd.Function):
             return (None,) * (4 + len(params))
         keep = []  # gradients laid out as the kernel reads them
         named = dict(zip(_PARAMS, params))
-        d = _desc(z, y, z, named, sizes, kinds)
+        d = _desc(x, y, x if x.dtype == torch.float32 else None, named, sizes, kinds)
         d.stats = stats.data_ptr()
         for k, g in (("grad_z", grad_z), ("grad_h", grad_h)):
             if g is not None:
-                keep.append(g.to(z.dtype).contiguous())
+                keep.append(g.to(x.dtype).contiguous())
                 setattr(d, k, keep[-1].data_ptr())
         need = ctx.needs_input_grad
-        out = [torch.empty_like(z) if need[0] else None, torch.empty_like(z) if need[1] else None, None, None]
+        out = [torch.empty_like(x) if need[0] else None, torch.empty_like(x) if need[1] else None, None, None]
         out += [torch.empty(p.shape, dtype=p.dtype, device=p.device) if p is not None and n else None
                 for p, n in zip(params, need[4:])]
         for k, g in zip(("x", "y"), out):
@@ -154,9 +155,9 @@ class NormFunction(torch.autograd.Function):
                 setattr(d, "grad_" + k, g.data_ptr())
         lib = _lib.load()
         size = lib.ksmm_cu_norm_backward_workspace_bytes(ctypes.byref(d))
-        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=z.device)
-        with torch.cuda.device(z.device):
-            _lib.check(lib.ksmm_cu_norm_backward(ctypes.byref(d), ws.data_ptr(), size, _stream_ptr(z.device)))
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
+        with torch.cuda.device(x.device):
+            _lib.check(lib.ksmm_cu_norm_backward(ctypes.byref(d), ws.data_ptr(), size, _stream_ptr(x.device)))
         return tuple(out)
 
 

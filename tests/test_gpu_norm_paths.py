@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import ksmm_b200 as kb
-from test_gpu_norm import EVERY, check
+from test_gpu_norm import EVERY, PARAMS, check, definition, make, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,31 @@ def test_scaled_streams(shape, bs_last, dtype, alpha):
     """alpha in every kernel: rows by groups, single elements, resident blocks, wide rows, columns, turned columns."""
     check(dtype, shape, norm="layer", post_norm="rms", bs_last=bs_last, samples=1, keys=EVERY, alpha=alpha)
     check(dtype, shape, norm="rms", bs_last=bs_last, keys=("weight", "shift"), alpha=alpha)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm,post_norm", [("layer", None), ("layer", "layer"), ("rms", "rms")])
+@pytest.mark.parametrize("shape,bs_last,samples", [((300, 768), False, 3), ((301, 720), False, 1), ((40, 1480), False, 2), ((45, 333), False, 1), ((66, 4096), False, 2), ((8, 8192), False, 1),
+                                                   ((30, 5003), False, 1), ((768, 300), True, 3), ((2304, 66), True, 2)])
+def test_gradients_know_the_unrounded_stream(shape, bs_last, samples, norm, post_norm, dtype):
+    """z is 20 deviations from 0 (layer norms), where its rounding is off by 20 u of a deviation.  The statistics and the h of
+    the forward pass are those of the unrounded z, so are the gradients: every result is rounded once, u; before that
+    64 u32 for a chain, times 20 for the differences from the mean, times 4 for the gradient's own (its seeds have
+    a mean of one deviation, and the sums over tokens add up such terms)."""
+    x, y, p = make(dtype, shape, bs_last, samples, EVERY if post_norm else ("weight", "bias", "scale", "shift", "gate"), True, seed=2)
+    if norm == "layer":
+        x = x + 20
+        if post_norm is None:
+            y, p["gate"] = y + 4, 1 + p["gate"] / 4
+    t = {k: v for k, v in {"x": x, "y": y, **p}.items() if v is not None}
+    leaves = {k: v.clone().requires_grad_(True) for k, v in t.items()}
+    exact = {k: v.double().requires_grad_(True) for k, v in t.items()}
+    _, h = kb.residual_norm(leaves["x"], leaves["y"], norm=norm, post_norm=post_norm, alpha=0.75, bs_last=bs_last,
+                            **{k: v for k, v in leaves.items() if k not in "xy"})
+    _, want = definition(exact["x"], exact["y"], {k: exact.get(k) for k in PARAMS}, norm, post_norm, 0.75, 1e-5, bs_last)
+    seed = (torch.randn(shape, device="cuda") + 1).to(dtype)
+    got = torch.autograd.grad(h, list(leaves.values()), seed)
+    ref = torch.autograd.grad(want, list(exact.values()), seed.double())
+    for k, a, b in zip(leaves, got, ref):
+        off = ((a.double() - b).norm() / b.norm()).item()
+        assert off <= unit(dtype) + 64 * 20 * 4 * 2.0 ** -24, (k, off)
