@@ -1152,7 +1152,7 @@ Args args_of(const ksmm_norm_desc_t& d) {
 // by another thread's call between this one's word and its launch.  A repeated set of one value is harmless.)
 using Granted = std::atomic<bool>[64];
 int allow_smem(const void* kern, size_t bytes, size_t most, Granted& granted) {
-  if (bytes <= 48 * 1024) return KSMM_OK;
+  if (bytes <= 40 * 1024) return KSMM_OK;  // (what a kernel declares itself, up to 2 KB here, counts as well)
   if (bytes > most) return set_error(KSMM_ERR_UNSUPPORTED, "norm: %zu bytes of shared memory", bytes);
   int dev = 0;
   cudaGetDevice(&dev);

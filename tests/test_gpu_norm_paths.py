@@ -126,3 +126,24 @@ def test_gradients_know_the_unrounded_stream(shape, bs_last, samples, norm, post
     for k, a, b in zip(leaves, got, ref):
         off = ((a.double() - b).norm() / b.norm()).item()
         assert off <= unit(dtype) + 64 * 20 * 4 * 2.0 ** -24, (k, off)
+
+
+NARROW = """
+import torch
+import ksmm_b200 as kb
+for dtype in (torch.float32, torch.float16, torch.bfloat16):
+    for c in (300, 312, 327, 328, 336, 341, 342, 350):
+        x = torch.randn(c, 40, device="cuda").to(dtype).requires_grad_(True)
+        _, h = kb.residual_norm(x, x, bs_last=True)
+        h.sum().backward()
+torch.cuda.synchronize()
+kb.check_device()
+print("ok")
+"""
+
+
+def test_first_calls_at_the_limit_of_undeclared_shared_memory():
+    """Batch-last calls of 328 to 341 channels take 46 to 48 KB beside the kernel's own 2: the first ones of a process."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", NARROW], cwd=root, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip().endswith("ok"), res.stderr[-3000:]
