@@ -10,8 +10,9 @@
 //
 // PAIR: two CTAs of a cluster work on one tile of 256 features x 128 batch entries with the two-SM form of the MMA.
 // Each holds its own 128 features' weights and accumulators and loads half of the input chunk, so that an SM moves
-// half the input from L2 and reads a quarter less shared memory per product (25088 rows of (1,512,192,4): 54 us on
-// single SMs, 44 by pairs; floor 24 from 54 GFLOP, 22 from the bytes).  The leading CTA issues the MMAs for both; its
+// half the input from L2 and reads a quarter less shared memory per product (25088 rows of (1,512,192,4): 53 us either
+// way, and with both halves kept 93 on single SMs, 75 by pairs; floor 24 from 39.5 GFLOP, 28 from 180 MB; when they are
+// used stands at use_pair).  The leading CTA issues the MMAs for both; its
 // barriers count both CTAs' copies and epilogue warps.  (Arrivals at the other CTA's barrier carry no cluster-scope
 // release: what they order are tensor-memory reads, which have completed; with one, each cost a microsecond.)
 //
@@ -379,9 +380,8 @@ __global__ void __launch_bounds__(kBlock, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ===================== MMA issuer =====================
-    // (elect_one: with the loop in one lane the issuing thread took 640 cycles per 64 of k where the MMAs take 256.)
-    // 25088 rows of (1,512,192,4),
-    // batch-last: 70 -> 59 us, with both halves' chunks in one ring stage 54, by pairs 44.
+    // (The warp walks the loop and one elected lane issues.  25088 rows of (1,512,192,4), batch-last: 70 us with the loop
+    // inside `if (lane == 0)`, 59 so, 54 with both halves' chunks in one ring stage.)
     if (rank == 0) {
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
       constexpr uint32_t kLboMN = static_cast<uint32_t>((kKC * 128) >> 4) << 16, kLboK = 1u << 16;
@@ -525,6 +525,8 @@ __global__ void __launch_bounds__(kBlock, 1)
         }
       };
       if constexpr (KEEP) {
+        // (Rounded to the layer's type, as every intermediate of a chain is: fp32 halves would be 8 bytes an element in place
+        // of 4, written here and read by the backward.  The product is formed from the unrounded halves.)
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           next_tile();

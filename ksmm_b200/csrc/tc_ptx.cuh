@@ -198,9 +198,8 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// One lane of a warp that has converged.  A warp that issues MMAs walks its loop as a whole and lets this lane
-// issue: inside `if (lane == 0)` the compiler cannot keep descriptors in uniform registers, and moving an MMA's
-// operands there one by one costs the issuing thread more time than an MMA with N = 128 takes.
+// One lane of a warp that has converged.  A warp that issues MMAs may walk its loop as a whole and let this lane issue,
+// which was measured to be faster for MMAs with N = 128 than a loop inside `if (lane == 0)` (70 -> 59 us, tc_gated.cu).
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
