@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(Cfg<L>::NT, Cfg<L>::MIN_CTAS)
         }
       }
     }
+    fence_proxy_async();  // (the stage's last loads are done before the copy that refills it)
     __syncwarp();
     if (lane == 0) mbar_arrive(empty_bar(s));
   }

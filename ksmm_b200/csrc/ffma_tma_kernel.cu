@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(WJ * 128, 512 / (WJ * 128))
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[m][t] = fmaf(wf[m], xf[t], acc[m][t]);
     }
+    fence_proxy_async();  // (the stage's last loads are done before the copy that refills it)
     __syncwarp();
     if (lane == 0) mbar_arrive(empty_bar(s));
   }

@@ -450,7 +450,8 @@ __global__ void __launch_bounds__(RING ? (TPR == 32 ? kRingBlock : kRingWide) : 
           yr[k].zero();
         }
       }
-      // the row is in registers: its place takes the next one
+      // the row is in registers: its place takes the next one, once these loads are done
+      tc::fence_proxy_async();
       if constexpr (TPR == 32) __syncwarp();
       else tc::bar_sync_named(1 + group, TPR);
       const int64_t ahead = row + static_cast<int64_t>(A.stages) * kGroups;

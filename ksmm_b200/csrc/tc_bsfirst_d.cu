@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(kThreadsD, 1)
                          : "memory");
         }
         // the raw chunk is in registers: hand its slot back to the producer at once
+        fence_proxy_async();  // (its loads are done before the copy that refills it)
         __syncwarp();
         if (tron) KSMM_TRACE(2, 32);
         if (lane == 0) {
