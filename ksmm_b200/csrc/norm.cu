@@ -903,6 +903,9 @@ __device__ __forceinline__ float reduce_scatter(float (&v)[32]) {
   return v[0];
 }
 
+// The normalised values of pre stay in shared memory between the passes (128 bytes per channel, as z in the forward pass):
+// forward and backward of 768 x 6501 bf16 with both norms 158 us when every pass read z again, 148 so, with z formed
+// from x and y on the way.
 template <typename T>
 __global__ void __launch_bounds__(kColWarps * 32) norm_columns_backward_kernel(const Args A) {
   __shared__ float red[kColWarps * 32];

@@ -726,8 +726,8 @@ int launch(const Problem& p, void* halves, int64_t halves_ld, cudaStream_t strea
   return KSMM_OK;
 }
 
-// Two CTAs per tile where that is faster: three chunks of k (a single CTA then has a shorter ring), features that fill the
-// pairs' tiles, and ten tiles or more for every pair of SMs.  Calls of two-factor layers in bf16, 25088 rows if not
+// Two CTAs per tile where that is faster: three chunks of k, features that fill the pairs' tiles, and ten tiles or more
+// for every pair of SMs.  Calls of two-factor layers in bf16, 25088 rows if not
 // said otherwise, single CTAs against pairs:
 //   768 -> 2048, (1,512,192,4) last: 93.1 and 92.5 us, training step 437 and 423; 8192 rows (7 tiles) 34.9 and 35.7
 //   768 -> 4096, (1,1024,192,4): 149 and 147, training 710 and 683; 4096 rows (7 tiles) 33.7 and 34.0
