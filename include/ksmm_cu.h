@@ -472,6 +472,77 @@ KSMM_API size_t ksmm_cu_norm_backward_workspace_bytes(const ksmm_norm_desc_t* de
 KSMM_API int ksmm_cu_norm_backward(const ksmm_norm_desc_t* desc, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Attention over a paged cache of keys and values: what a generating model needs between the q / k / v projections
+ * (ksmm_cu_grouped_chain_forward) and the output projection.  The reference's attention keeps no cache
+ * (src/ksmm_py/model/vit.py:434-489).
+ *
+ * A pool of `pages` pages holds page_size tokens each: token r of page p, key head h starts at
+ * keys + p * key_strides[0] + h * key_strides[1] + r * key_strides[2] elements (head_dim contiguous elements; values
+ * alike).  table[s * table_stride + i] is the page of tokens i * page_size .. of sequence s; lengths[s] its number of
+ * tokens INCLUDING the new ones of this call, which are its last.  The new tokens are rows of q, k and v (strides in
+ * elements: token, head): sequence s has rows starts[s] .. starts[s + 1] - 1, or, where starts is NULL, tokens /
+ * sequences rows each.  Row t of n new ones has position lengths[s] - n + t.  cache_dtype is dtype (fp32, fp16 or bf16) or
+ * KSMM_F8E4M3 with an fp32 scale for each token and head (key_scales, value_scales): value = element * scale.
+ *
+ * What the device finds wrong stays within bounds: a token with a position below 0, or whose page the table does not
+ * hold (an entry outside the pool, a length beyond table_width pages), is not stored; attention rows that would read such a
+ * page are NaN.  Rows of no sequence (before starts[0], from starts[sequences] on) are left as they are, or set to zero
+ * where clear_rest is not 0.
+ *
+ * ksmm_cu_cache_append stores k and v; k, and q into q_out (q may be NULL), are rotated first: pair i of `pairs` by
+ * position * frequencies[i] radians (formed and reduced in 64 bits), elements (i, i + pairs), or (2 i, 2 i + 1) where
+ * interleaved; elements from 2 * pairs on are taken as they are (frequencies NULL, pairs 0: all).  In 8 bits
+ * scale = max(amax / 448, 2^-126) over the token's head.
+ * ksmm_cu_cache_attention: out = softmax(scale * q K^T) V for each row over the keys at positions
+ * position - window + 1 .. position (window 0: from 0 on), query head h with key head h / (heads / kv_heads); zeros where
+ * there is no key.  Statistics and sums are fp32.  max_new: an upper bound of one sequence's rows that picks the kernels (0:
+ * not known); more rows than that are still computed, slowly.  A value or key that is not finite reaches no row of a
+ * sequence's earlier calls or of other sequences, but may reach this call's rows of its sequence that do not see it.
+ * Workspace: ..._workspace_bytes, aligned to 256 bytes, one for each call that may run at the same time.
+ * head_dim is at most 256.  Outputs overlap no input.
+ */
+typedef struct {
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+  int64_t key_strides[3], value_strides[3], key_scale_strides[3], value_scale_strides[3]; /* page, head, token */
+  int64_t pages;
+  int32_t page_size, kv_heads, head_dim, cache_dtype;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int64_t sequences, tokens;
+} ksmm_cache_t;
+
+typedef struct {
+  ksmm_cache_t cache;
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  int64_t k_strides[2], v_strides[2], q_strides[2], q_out_strides[2]; /* token, head */
+  const double* frequencies;
+  int32_t pairs, interleaved, heads, dtype, clear_rest;
+} ksmm_cache_append_desc_t;
+
+typedef struct {
+  ksmm_cache_t cache;
+  const void* q;
+  void* out;
+  int64_t q_strides[2], out_strides[2]; /* token, head */
+  int64_t window, max_new;
+  float scale;
+  int32_t heads, dtype, clear_rest;
+} ksmm_cache_attention_desc_t;
+
+KSMM_API int ksmm_cu_cache_append(const ksmm_cache_append_desc_t* desc, void* stream);
+KSMM_API size_t ksmm_cu_cache_attention_workspace_bytes(const ksmm_cache_attention_desc_t* desc);
+KSMM_API int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Host-memory variant of ksmm_cu_chain_forward: input, values and output are
  * HOST buffers; the call stages them through device memory that the library
  * owns (grown on demand, reused across calls), runs the chain and returns

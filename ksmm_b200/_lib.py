@@ -48,6 +48,7 @@ EXPORTS = (
     "ksmm_cu_chain_train_bytes", "ksmm_cu_chain_train_forward", "ksmm_cu_chain_backward",
     "ksmm_cu_chain_fp8_workspace_bytes", "ksmm_cu_chain_forward_fp8",
     "ksmm_cu_gated_workspace_bytes", "ksmm_cu_gated_train_bytes", "ksmm_cu_gated_forward", "ksmm_cu_gated_backward",
+    "ksmm_cu_cache_append", "ksmm_cu_cache_attention_workspace_bytes", "ksmm_cu_cache_attention",
     "ksmm_cu_norm_forward_workspace_bytes", "ksmm_cu_norm_forward", "ksmm_cu_norm_backward_workspace_bytes", "ksmm_cu_norm_backward",
 )
 
@@ -116,6 +117,38 @@ class NormDesc(ctypes.Structure):
         + [(n, ctypes.c_void_p) for n in ("grad_z", "grad_h", "grad_x", "grad_y", "grad_weight", "grad_bias",
                                           "grad_post_weight", "grad_post_bias", "grad_scale", "grad_shift", "grad_gate")]
     )
+
+
+class CacheDesc(ctypes.Structure):
+    """Mirror of ksmm_cache_t."""
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("keys", "values", "key_scales", "value_scales")]
+        + [(n, ctypes.c_int64 * 3) for n in ("key_strides", "value_strides", "key_scale_strides", "value_scale_strides")]
+        + [("pages", ctypes.c_int64)]
+        + [(n, ctypes.c_int32) for n in ("page_size", "kv_heads", "head_dim", "cache_dtype")]
+        + [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+           ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("sequences", ctypes.c_int64), ("tokens", ctypes.c_int64)]
+    )
+
+
+class CacheAppendDesc(ctypes.Structure):
+    """Mirror of ksmm_cache_append_desc_t."""
+    _fields_ = (
+        [("cache", CacheDesc)]
+        + [(n, ctypes.c_void_p) for n in ("k", "v", "q", "q_out")]
+        + [(n, ctypes.c_int64 * 2) for n in ("k_strides", "v_strides", "q_strides", "q_out_strides")]
+        + [("frequencies", ctypes.c_void_p)]
+        + [(n, ctypes.c_int32) for n in ("pairs", "interleaved", "heads", "dtype", "clear_rest")]
+    )
+
+
+class CacheAttentionDesc(ctypes.Structure):
+    """Mirror of ksmm_cache_attention_desc_t."""
+    _fields_ = [
+        ("cache", CacheDesc), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 2),
+        ("out_strides", ctypes.c_int64 * 2), ("window", ctypes.c_int64), ("max_new", ctypes.c_int64), ("scale", ctypes.c_float),
+        ("heads", ctypes.c_int32), ("dtype", ctypes.c_int32), ("clear_rest", ctypes.c_int32),
+    ]
 
 
 class KsmmError(RuntimeError):
@@ -214,6 +247,12 @@ def load():
     lib.ksmm_cu_norm_backward_workspace_bytes.argtypes = [ctypes.POINTER(NormDesc)]
     lib.ksmm_cu_norm_backward.restype = i32
     lib.ksmm_cu_norm_backward.argtypes = [ctypes.POINTER(NormDesc), vp, ctypes.c_size_t, vp]
+    lib.ksmm_cu_cache_append.restype = i32
+    lib.ksmm_cu_cache_append.argtypes = [ctypes.POINTER(CacheAppendDesc), vp]
+    lib.ksmm_cu_cache_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.ksmm_cu_cache_attention_workspace_bytes.argtypes = [ctypes.POINTER(CacheAttentionDesc)]
+    lib.ksmm_cu_cache_attention.restype = i32
+    lib.ksmm_cu_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionDesc), vp, ctypes.c_size_t, vp]
     lib.ksmm_cu_host_wait.restype = i32
     lib.ksmm_cu_host_wait.argtypes = [ctypes.c_uint64]
     lib.ksmm_cu_num_configs.restype = i32

@@ -1,0 +1,354 @@
+// Attention over a paged cache on the CUDA cores: fp32, and what the tensor-core kernels do not take (pages that are no
+// multiple of 16 tokens, rows that are no multiple of 16 bytes).
+//
+// Eight lanes hold a token's key: with q in registers each lane multiplies its dims, three shuffles join them.  A warp has four
+// such groups and a block eight warps, and every group keeps a running maximum, sum and output row of its own over its
+// tokens, two at a time; they are joined once, at the end of a segment.
+#include "cache.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
+
+namespace ksmm {
+namespace cache {
+namespace {
+
+constexpr int kRowThreads = 256;
+
+template <int N>
+struct Bytes;
+template <> struct Bytes<16> { using type = uint4; };
+template <> struct Bytes<8> { using type = uint2; };
+template <> struct Bytes<4> { using type = uint32_t; };
+
+// (plain loads: the append before this kernel may still be writing when its blocks start, and nothing is read before the wait)
+template <typename T, int VEC>
+__device__ __forceinline__ void load(const T* p, float* out) {
+  if constexpr (VEC == 1) {
+    out[0] = ElemTraits<T>::to_float(*p);
+  } else {
+    T tmp[VEC];
+    using B = typename Bytes<sizeof(T) * VEC>::type;
+    *reinterpret_cast<B*>(tmp) = *reinterpret_cast<const B*>(p);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[e] = ElemTraits<T>::to_float(tmp[e]);
+  }
+}
+
+// dims (j * 8 + l) * VEC .. of a row, for lane l of eight
+template <typename T, int DPL, int VEC>
+__device__ __forceinline__ void load_row(const T* row, int l, int dim, bool there, float* out) {
+#pragma unroll
+  for (int j = 0; j < DPL / VEC; ++j) {
+    const int d = (j * 8 + l) * VEC;
+    if (there && d < dim) {
+      load<T, VEC>(row + d, out + j * VEC);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out[j * VEC + e] = 0.f;
+    }
+  }
+}
+
+template <typename T, typename C, int DPL, int VEC>
+__global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_constant__ Attend a) {
+  constexpr int R = 64 / DPL;
+  constexpr bool kEight = sizeof(C) == 1;
+  __shared__ int64_t shared[40];
+  __shared__ float stats[2][kRowThreads / 32][R];
+  extern __shared__ float sums[];  // [warp][R][8 DPL]
+  tc::grid_dep_wait();
+  tc::grid_dep_launch();
+  clear_rest<T>(a);
+  Share mine;
+  if (!share<kRowThreads>(a, shared, &mine)) return;
+  const Pool& p = a.pool;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, l = lane % 8, at = warp * 4 + lane / 8;
+  const T* q_rows = reinterpret_cast<const T*>(a.q);
+  const C* data[2] = {reinterpret_cast<const C*>(p.data[0]), reinterpret_cast<const C*>(p.data[1])};
+
+  Segment g;
+  bool slot_used[2] = {false, false};
+  while (mine.next(a, &g)) {
+    const int rows = min(R, g.seq.n * a.group - g.tile * R);
+    float q[R][DPL], o[R][DPL], m[R], sum[R];
+    int position[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = g.tile * R + r, t = row / a.group;
+      position[r] = r < rows ? g.seq.length - g.seq.n + t : -1;
+      const int64_t from = (g.seq.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
+      load_row<T, DPL, VEC>(q_rows + from, l, p.dim, r < rows, q[r]);
+      m[r] = kNone;
+      sum[r] = 0.f;
+#pragma unroll
+      for (int e = 0; e < DPL; ++e) o[r][e] = 0.f;
+    }
+    const int t0 = g.tile * R / a.group, t1 = (g.tile * R + rows - 1) / a.group;
+    const int lo = first_key(a, g.seq, t0), hi = g.seq.length - g.seq.n + t1 + 1;
+    int unit, units;
+    if (a.split) {
+      const int first = first_key(a, g.seq, 0) / kUnit;
+      unit = first + g.from;
+      units = first + g.to;
+    } else {
+      unit = lo / kUnit;
+      units = (max(hi, 0) + kUnit - 1) / kUnit;
+    }
+#pragma unroll 1
+    for (; unit < units; ++unit) {
+      float k[2][DPL], v[2][DPL], ks[2], vs[2];
+      int j[2];
+      bool there[2], bad[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        j[h] = unit * kUnit + h * 32 + at;
+        there[h] = j[h] >= lo && j[h] < hi;
+        bad[h] = false;
+        int64_t page = 0;
+        int nth = 0;
+        if (there[h]) {
+          nth = j[h] / p.page_size;
+          page = p.table[g.s * p.table_stride + nth];
+          nth = j[h] - nth * p.page_size;
+          bad[h] = page < 0 || page >= p.pages;
+        }
+        const bool get = there[h] && !bad[h];
+        load_row<C, DPL, VEC>(data[0] + page * p.page[0] + g.head * p.head[0] + nth * p.token[0], l, p.dim, get, k[h]);
+        load_row<C, DPL, VEC>(data[1] + page * p.page[1] + g.head * p.head[1] + nth * p.token[1], l, p.dim, get, v[h]);
+        ks[h] = vs[h] = 1.f;
+        if (kEight && get) {
+          ks[h] = p.scales[0][page * p.spage[0] + g.head * p.shead[0] + nth * p.stoken[0]];
+          vs[h] = p.scales[1][page * p.spage[1] + g.head * p.shead[1] + nth * p.stoken[1]];
+        }
+      }
+      if (kEight) {
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) {
+          v[0][e] *= vs[0];
+          v[1][e] *= vs[1];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r >= rows) continue;
+        float s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < DPL; ++e) d = fmaf(q[r][e], k[h][e], d);
+          d += __shfl_xor_sync(0xffffffffu, d, 1);
+          d += __shfl_xor_sync(0xffffffffu, d, 2);
+          d += __shfl_xor_sync(0xffffffffu, d, 4);
+          if (kEight) d *= ks[h];
+          s[h] = bad[h] ? __int_as_float(0x7fffffff) : d * a.scale;
+        }
+        bool sees[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sees[h] = there[h] && j[h] <= position[r] && (!a.window || j[h] > position[r] - a.window);
+        float top = m[r];
+        if (sees[0]) top = fmaxf(top, s[0]);
+        if (sees[1]) top = fmaxf(top, s[1]);
+        if (top != m[r]) {
+          const float f = exp2f(m[r] - top);
+          sum[r] *= f;
+#pragma unroll
+          for (int e = 0; e < DPL; ++e) o[r][e] *= f;
+          m[r] = top;
+        }
+        // (a token that the row does not see is left out, whatever it holds)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!sees[h]) continue;
+          const float w = exp2f(s[h] - top);
+          sum[r] += w;
+#pragma unroll
+          for (int e = 0; e < DPL; ++e) o[r][e] = fmaf(w, v[h][e], o[r][e]);
+        }
+      }
+    }
+
+    // the four groups of a warp, then the warps
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int x = 8; x < 32; x *= 2) {
+        const float other = __shfl_xor_sync(0xffffffffu, m[r], x), top = fmaxf(m[r], other);
+        const float f = exp2f(m[r] - top);
+        sum[r] *= f;
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], x);
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) {
+          o[r][e] *= f;
+          o[r][e] += __shfl_xor_sync(0xffffffffu, o[r][e], x);
+        }
+        m[r] = top;
+      }
+      if (lane < 8) {
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) sums[(warp * R + r) * 8 * DPL + (e / VEC * 8 + l) * VEC + e % VEC] = o[r][e];
+        if (lane == 0) {
+          stats[0][warp][r] = m[r];
+          stats[1][warp][r] = sum[r];
+        }
+      }
+    }
+    __syncthreads();
+    const int slot = slot_of(g);
+    if (slot && tid == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
+    if (slot) slot_used[slot - 1] = true;
+    float* part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + slot - 1) * a.tile_rows * (p.dim + 2);
+    for (int i = tid; i < rows * p.dim; i += kRowThreads) {
+      const int r = i / p.dim, d = i - r * p.dim;
+      float top = stats[0][0][r];
+#pragma unroll
+      for (int w = 1; w < kRowThreads / 32; ++w) top = fmaxf(top, stats[0][w][r]);
+      float total = 0.f, out = 0.f;
+#pragma unroll
+      for (int w = 0; w < kRowThreads / 32; ++w) {
+        const float f = exp2f(stats[0][w][r] - top);
+        total = fmaf(f, stats[1][w][r], total);
+        out = fmaf(f, sums[(w * R + r) * 8 * DPL + d], out);
+      }
+      if (g.seq.bad) total = __int_as_float(0x7fffffff);
+      if (slot) {
+        part[i] = out;
+        if (d == 0) {
+          part[a.tile_rows * p.dim + r] = top;
+          part[a.tile_rows * (p.dim + 1) + r] = total;
+        }
+      } else {
+        const int row = g.tile * R + r, t = row / a.group;
+        reinterpret_cast<T*>(a.out)[(g.seq.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head + d] =
+            ElemTraits<T>::from_float(total == 0.f ? 0.f : out / total);
+      }
+    }
+    __syncthreads();
+  }
+  if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
+}
+
+// Joins the parts of items that several blocks shared.  Block (c, r): row r of the item that begins in block c and goes on;
+// its further parts are in slot 0 of the blocks after c, as long as they name the item.  In the order of the blocks, whoever was first.
+constexpr int kJoinThreads = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Attend a, int blocks) {
+  __shared__ float weight[1024 + kJoinThreads];
+  __shared__ float reduce[kJoinThreads / 32];
+  tc::grid_dep_wait();
+  tc::grid_dep_launch();
+  const Pool& p = a.pool;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  const int64_t item = a.slots[2 * c + 1];
+  if (item < 0) return;
+  const int s = static_cast<int>((item >> 32) / p.kv_heads), head = static_cast<int>((item >> 32) % p.kv_heads);
+  const int tile = static_cast<int>(item & 0xffffffff);
+  const Sequence q = sequence(p, s);
+  if (tile * a.tile_rows + r >= q.n * a.group) return;
+  int parts = 1;
+  for (int from = c + 1; from < blocks; from += kJoinThreads) {
+    const int i = from + tid;
+    const int n = __syncthreads_count(i < blocks && a.slots[2 * static_cast<int64_t>(i)] == item);
+    parts += n;
+    if (n < kJoinThreads) break;
+  }
+  const int64_t size = static_cast<int64_t>(a.tile_rows) * (p.dim + 2);
+  auto part = [&](int i) { return a.partial + (i == 0 ? 2 * c + 1 : 2 * static_cast<int64_t>(c + i)) * size; };
+  float top = kNone;
+  for (int i = tid; i < parts; i += kJoinThreads) {
+    weight[i] = part(i)[a.tile_rows * p.dim + r];
+    top = fmaxf(top, weight[i]);
+  }
+#pragma unroll
+  for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  if (tid % 32 == 0) reduce[tid / 32] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, reduce[w]);
+  for (int i = tid; i < parts; i += kJoinThreads) weight[i] = exp2f(weight[i] - top);
+  __syncthreads();
+  float total = 0.f;
+  for (int i = 0; i < parts; ++i) total = fmaf(weight[i], part(i)[a.tile_rows * (p.dim + 1) + r], total);
+  const int row = tile * a.tile_rows + r, t = row / a.group;
+  T* out = reinterpret_cast<T*>(a.out) + (q.start + t) * a.out_token + (head * a.group + row - t * a.group) * a.out_head;
+  for (int d = tid; d < p.dim; d += kJoinThreads) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) sum = fmaf(weight[i], part(i)[r * p.dim + d], sum);
+    out[d] = ElemTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
+  }
+}
+
+template <typename T, typename C, int DPL, int VEC>
+int launch_one(const Attend& a, unsigned grid, cudaStream_t stream) {
+  constexpr size_t smem = kRowThreads / 32 * 64 * 8 * sizeof(float);
+  const cudaError_t err = tc::launch_pdl(rows_kernel<T, C, DPL, VEC>, grid, kRowThreads, smem, stream, a);
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention rows kernel: %s", cudaGetErrorString(err));
+  count_launch();
+  return KSMM_OK;
+}
+
+template <typename T, typename C>
+int launch_typed(const Attend& a, bool vec, unsigned grid, cudaStream_t stream) {
+  const int dim = a.pool.dim;
+  if (vec) {
+    if (dim <= 64) return launch_one<T, C, 8, 4>(a, grid, stream);
+    if (dim <= 128) return launch_one<T, C, 16, 4>(a, grid, stream);
+    return launch_one<T, C, 32, 4>(a, grid, stream);
+  }
+  if (dim <= 64) return launch_one<T, C, 8, 1>(a, grid, stream);
+  if (dim <= 128) return launch_one<T, C, 16, 1>(a, grid, stream);
+  return launch_one<T, C, 32, 1>(a, grid, stream);
+}
+
+template <typename T>
+int launch_cached(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  // rows of four elements at a time where every one starts on their boundary
+  const int es = cache_dtype == KSMM_F8E4M3 ? 1 : static_cast<int>(sizeof(T));
+  auto whole = [](const void* p, int64_t x, int64_t y, int64_t z, int size) {
+    return (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0) && x % 4 == 0 && y % 4 == 0 && z % 4 == 0;
+  };
+  const Pool& p = a.pool;
+  bool vec = p.dim % 4 == 0 && whole(a.q, a.q_token, a.q_head, 0, sizeof(T));
+  for (int i = 0; i < 2; ++i) vec = vec && whole(p.data[i], p.page[i], p.head[i], p.token[i], es);
+  if (cache_dtype == KSMM_F8E4M3) return launch_typed<T, f8e4m3>(a, vec, grid, stream);
+  return launch_typed<T, T>(a, vec, grid, stream);
+}
+
+}  // namespace
+
+int rows_tile(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 4 : 2; }
+
+int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  if (dtype == KSMM_F32) return launch_cached<float>(a, cache_dtype, grid, stream);
+  if (dtype == KSMM_F16) return launch_cached<__half>(a, cache_dtype, grid, stream);
+  return launch_cached<__nv_bfloat16>(a, cache_dtype, grid, stream);
+}
+
+template <typename T>
+static int launch_join_typed(const Attend& a, unsigned blocks, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks, a.tile_rows);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = tc::pdl_enabled() ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, join_kernel<T>, a, static_cast<int>(blocks));
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention join kernel: %s", cudaGetErrorString(err));
+  count_launch();
+  return KSMM_OK;
+}
+
+int launch_join(const Attend& a, int dtype, unsigned blocks, cudaStream_t stream) {
+  if (dtype == KSMM_F32) return launch_join_typed<float>(a, blocks, stream);
+  if (dtype == KSMM_F16) return launch_join_typed<__half>(a, blocks, stream);
+  return launch_join_typed<__nv_bfloat16>(a, blocks, stream);
+}
+
+}  // namespace cache
+}  // namespace ksmm
