@@ -106,7 +106,7 @@ def _heads(name, t, heads, cache, tokens, dtype):
         raise ValueError(f"{t.shape[1]} heads of {name} do not share {cache.heads} key heads evenly")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: a cache is not trained through")
-    if t.shape[0] >= _MAX_INT - 1024:
+    if t.shape[0] >= _MAX_INT - 65536:
         raise ValueError(f"{name} has {t.shape[0]} tokens")
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
@@ -129,7 +129,7 @@ def _cache_desc(cache, table, lengths, starts, tokens):
         raise ValueError(f"{tokens} tokens do not divide into {lengths.shape[0]} sequences")
     if tokens and not lengths.shape[0]:
         raise ValueError("tokens without sequences")
-    if max(table.shape[1] * cache.page_size, cache.pages, cache.heads, lengths.shape[0] * cache.heads) >= _MAX_INT - 1024:
+    if max(table.shape[1] * cache.page_size, cache.pages, cache.heads, lengths.shape[0] * cache.heads) >= _MAX_INT - 65536:
         raise ValueError("the cache or its table is too large")
     d = _lib.CacheDesc(
         keys=cache.keys.data_ptr(), values=cache.values.data_ptr(), key_strides=_strides(cache.keys, 3),

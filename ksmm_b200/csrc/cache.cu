@@ -220,14 +220,14 @@ int check_cache(const ksmm_cache_t& c, int heads, int dtype) {
   if (!plain_type(dtype)) return set_error(KSMM_ERR_UNSUPPORTED, "caches take float32, float16 and bfloat16 models");
   if (c.cache_dtype != dtype && c.cache_dtype != KSMM_F8E4M3)
     return set_error(KSMM_ERR_UNSUPPORTED, "a cache holds the model's type or float8_e4m3fn");
-  if (c.sequences < 0 || c.tokens < 0 || c.sequences >= INT_MAX - 1024 || c.tokens >= INT_MAX - 1024)
-    return set_error(KSMM_ERR_BAD_ARGUMENT, "sequences and tokens are between 0 and 2^31 - 1025");
+  if (c.sequences < 0 || c.tokens < 0 || c.sequences >= INT_MAX - 65536 || c.tokens >= INT_MAX - 65536)
+    return set_error(KSMM_ERR_BAD_ARGUMENT, "sequences and tokens are between 0 and 2^31 - 65537");
   if (c.page_size <= 0 || c.kv_heads <= 0 || c.head_dim <= 0 || heads <= 0 || c.pages < 0 || c.table_width < 0)
     return set_error(KSMM_ERR_BAD_ARGUMENT, "page_size, heads, kv_heads and head_dim are positive");
   if (c.head_dim > kMaxDim) return set_error(KSMM_ERR_UNSUPPORTED, "head_dim is at most %d, not %d", kMaxDim, c.head_dim);
   if (c.pages >= (1ll << 31)) return set_error(KSMM_ERR_BAD_ARGUMENT, "a pool has less than 2^31 pages");
-  if (static_cast<int64_t>(c.table_width) * c.page_size > INT_MAX - 1024)
-    return set_error(KSMM_ERR_BAD_ARGUMENT, "a sequence has at most 2^31 - 1025 tokens: table_width * page_size is more");
+  if (static_cast<int64_t>(c.table_width) * c.page_size > INT_MAX - 65536)
+    return set_error(KSMM_ERR_BAD_ARGUMENT, "a sequence has at most 2^31 - 65537 tokens: table_width * page_size is more");
   if (heads % c.kv_heads || heads > 65535)
     return set_error(KSMM_ERR_BAD_ARGUMENT, "%d heads do not share %d key heads evenly", heads, c.kv_heads);
   if (c.tokens == 0) return KSMM_OK;
@@ -357,7 +357,10 @@ int check_attention(const ksmm_cache_attention_desc_t* d) {
   return KSMM_OK;
 }
 
-Plan plan_of(const ksmm_cache_attention_desc_t& d) { return plan_rows(d, rows_tile(d.cache.head_dim), 1); }
+Plan plan_of(const ksmm_cache_attention_desc_t& d) {
+  if (token_fits(d)) return plan_rows(d, kTokenRows, token_blocks_per_sm(d.cache.cache_dtype, d.cache.head_dim));
+  return plan_rows(d, rows_tile(d.cache.head_dim), 1);
+}
 
 }  // namespace
 }  // namespace cache
@@ -429,13 +432,14 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
   a.clear_rest = d->clear_rest != 0;
   a.least = 1;
   a.most = INT_MAX;
-  a.tile_rows = rows_tile(c.head_dim);
+  const bool token = token_fits(*d);
+  a.tile_rows = token ? kTokenRows : rows_tile(c.head_dim);
   a.split = plan.split;
   a.partial = static_cast<float*>(workspace);
   a.slots = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + plan.partial_bytes);
   a.status = tc::status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = launch_rows(a, d->dtype, c.cache_dtype, plan.grid, s);
+  st = token ? launch_token(a, d->dtype, c.cache_dtype, plan.grid, s) : launch_rows(a, d->dtype, c.cache_dtype, plan.grid, s);
   if (st == KSMM_OK && plan.split) st = launch_join(a, d->dtype, plan.grid, s);
   return st;
 }

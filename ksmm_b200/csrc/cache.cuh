@@ -135,6 +135,7 @@ __device__ int64_t find_place(const Attend& a, int64_t* shared, At at, int* s, i
   __syncthreads();
   *s = static_cast<int>(shared[33]);
   *offset = shared[34];
+  __syncthreads();  // (the caller may use the array again)
   return total;
 }
 
@@ -142,14 +143,16 @@ __device__ int64_t find_place(const Attend& a, int64_t* shared, At at, int* s, i
 struct Segment {
   Sequence seq;
   int s, head, tile;
-  int from, to;      // units of the item
-  int units;
-  int64_t item;      // its number, for the partial results
+  int lo, hi;          // the keys that its rows see lie in [lo, hi)
+  int first_position;  // of its first row
+  int from, to;        // the units to be gone through, counted from the sequence's first token
+  int slot;            // where the result goes: 0 the output, 1 or 2 the block's first or second slot
+  int64_t item;        // its number, for the partial results
 };
 
 struct Share {
   int64_t begin, end, done;
-  int s, block, blocks;
+  int s;
   int64_t offset;
   Work work;
   Sequence seq;
@@ -164,19 +167,34 @@ struct Share {
       work = work_of(a, seq);
     }
     const int64_t item = offset / work.units;
-    g->from = static_cast<int>(offset - item * work.units);
+    const int from = static_cast<int>(offset - item * work.units);
     const int64_t left = end - done;
-    g->to = static_cast<int>(left < work.units - g->from ? g->from + left : work.units);
-    g->units = work.units;
+    const int to = static_cast<int>(left < work.units - from ? from + left : work.units);
+    done += to - from;
+    offset += to - from;
     g->seq = seq;
     g->s = s;
     g->head = static_cast<int>(item / work.tiles);
-    // (without a split the last tile comes first: it sees the most keys)
     g->tile = static_cast<int>(item - static_cast<int64_t>(g->head) * work.tiles);
+    // (without a split the last tile comes first: it sees the most keys)
     if (!a.split) g->tile = work.tiles - 1 - g->tile;
+    const int t0 = static_cast<int>(static_cast<int64_t>(g->tile) * a.tile_rows / a.group);
+    g->first_position = seq.length - seq.n + t0;
+    g->lo = first_key(a, seq, a.split ? 0 : t0);
+    g->hi = seq.length;
+    if (a.split) {
+      // (all tiles of a sequence go through the same units, so that they count the same)
+      g->from = g->lo / kUnit + from;
+      g->to = g->lo / kUnit + to;
+    } else {
+      const int64_t t1 = (static_cast<int64_t>(g->tile + 1) * a.tile_rows - 1) / a.group;
+      g->hi = max(seq.length - seq.n + static_cast<int>(t1 < seq.n ? t1 + 1 : seq.n), 0);
+      g->from = g->lo / kUnit;
+      g->to = (g->hi + kUnit - 1) / kUnit;
+    }
+    // a block's first segment may continue an item, its last may be continued; one that is both is the first
+    g->slot = from == 0 && to == work.units ? 0 : from > 0 ? 1 : 2;
     g->item = (static_cast<int64_t>(s) * a.pool.kv_heads + g->head) << 32 | g->tile;
-    done += g->to - g->from;
-    offset += g->to - g->from;
     return true;
   }
 };
@@ -211,12 +229,6 @@ __device__ bool share(const Attend& a, int64_t* shared, Share* r) {
   return true;
 }
 
-// Where a segment's result goes: 0 the output, else 1 + the block's slot.  A block's first segment may continue an item (slot 0),
-// its last may be continued (slot 1); one that is both is in slot 0.
-__device__ __forceinline__ int slot_of(const Segment& g) {
-  return g.from == 0 && g.to == g.units ? 0 : g.from > 0 ? 1 : 2;
-}
-
 // Rows of no sequence, as asked for.
 template <typename T>
 __device__ void clear_rest(const Attend& a) {
@@ -237,6 +249,10 @@ __device__ void clear_rest(const Attend& a) {
 constexpr int kMaxBlocks = 1024;  // of a split launch (the join kernel's table of weights)
 int rows_tile(int dim);           // rows of an item in the CUDA-core kernel
 int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
+int token_blocks_per_sm(int cache_dtype, int dim);
+constexpr int kTokenRows = 16;    // rows of an item in the 16- and 8-bit kernel
+bool token_fits(const ksmm_cache_attention_desc_t& d);
+int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
 int launch_join(const Attend& a, int dtype, unsigned blocks, cudaStream_t stream);
 
 }  // namespace cache

@@ -83,26 +83,15 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
 #pragma unroll
       for (int e = 0; e < DPL; ++e) o[r][e] = 0.f;
     }
-    const int t0 = g.tile * R / a.group, t1 = (g.tile * R + rows - 1) / a.group;
-    const int lo = first_key(a, g.seq, t0), hi = g.seq.length - g.seq.n + t1 + 1;
-    int unit, units;
-    if (a.split) {
-      const int first = first_key(a, g.seq, 0) / kUnit;
-      unit = first + g.from;
-      units = first + g.to;
-    } else {
-      unit = lo / kUnit;
-      units = (max(hi, 0) + kUnit - 1) / kUnit;
-    }
 #pragma unroll 1
-    for (; unit < units; ++unit) {
+    for (int unit = g.from; unit < g.to; ++unit) {
       float k[2][DPL], v[2][DPL], ks[2], vs[2];
       int j[2];
       bool there[2], bad[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         j[h] = unit * kUnit + h * 32 + at;
-        there[h] = j[h] >= lo && j[h] < hi;
+        there[h] = j[h] >= g.lo && j[h] < g.hi;
         bad[h] = false;
         int64_t page = 0;
         int nth = 0;
@@ -195,7 +184,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       }
     }
     __syncthreads();
-    const int slot = slot_of(g);
+    const int slot = g.slot;
     if (slot && tid == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
     if (slot) slot_used[slot - 1] = true;
     float* part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + slot - 1) * a.tile_rows * (p.dim + 2);

@@ -1,0 +1,605 @@
+// Attention of few new tokens over a paged cache in 16 or 8 bits.
+//
+// Each key and value is read once and met by the few rows of q that share its head: 4 rows x 2 products per element, far
+// below what the tensor cores need to be busy, so the kernel is a stream of memory.  Its blocks share all sequences' units of
+// 64 tokens evenly (cache.cuh) and are as many as fit the SMs; one warp keeps a ring of 3 to 6 units in flight through TMA
+// (~190 KB on an SM; 43 GB/s per SM times 1.5 us of latency need 65), four warps take 16 tokens of a unit each, with a running
+// maximum, sum and output of their own, and meet only at the end of a segment.  Warps that each wait for their unit
+// alone hide the latency that a block-wide step for each unit would show.
+//
+// mma.sync, not tcgen05: an item has at most 16 rows (heads that share a key head, new tokens), an eighth of tcgen05's
+// smallest tile, and the scores have to come back to registers at once; 32 or 48 MMAs per 16 tokens take a quarter of the
+// time that their bytes take.  q sits in registers as the A operand; K (rows of a token) is the B operand as it lies in shared
+// memory, V through transposing loads.  The weights enter the second product as two 16-bit parts (w = hi + lo, each
+// rounded): one part would add an error as large as the result's final rounding.
+//
+// 8-bit caches: the products run in fp16, which holds e4m3 exactly.  q is scaled by a power of two per row so that bf16's
+// range fits; a token's key scale multiplies its scores; its value scale multiplies its weight, relative to a running
+// power of two `vm` that is at least every scale so far.  One 16-byte chunk of a key row is a k step: its elements are
+// taken in the order 4 q, 4 q + 1 | 4 q + 2, 4 q + 3 that the load gives, by q as well.
+#include <atomic>
+#include <climits>
+#include <type_traits>
+
+#include "cache.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
+
+namespace ksmm {
+namespace cache {
+namespace {
+
+using namespace tc;
+
+constexpr int kConsumers = 4;
+constexpr int kTokenThreads = (kConsumers + 1) * 32;
+constexpr int kTileRows = kTokenRows;
+
+template <bool EIGHT, int DP>
+struct Layout {
+  static constexpr int kBoxes = EIGHT ? (DP + 127) / 128 : DP / 64;     // 128-byte columns of a row
+  static constexpr int kOperand = kBoxes * kUnit * 128;                 // a unit's keys
+  static constexpr int kScales = EIGHT ? 2 * kUnit * 4 : 0;
+  static constexpr int kStageBytes = 2 * kOperand;
+  static constexpr int kBlocks = DP == 256 ? 1 : 2;                     // on an SM
+  static constexpr int kStages = 196608 / kBlocks / (kStageBytes + kScales);
+  static constexpr int kMerge = DP / 2 * 32 * 4;                        // a warp's output
+  static constexpr int kMergeAt = kStages * kStageBytes;
+  static constexpr int kScalesAt = kMergeAt + 2 * kMerge;
+  static constexpr int kStatsAt = kScalesAt + kStages * kScales;        // of the merges: 2 x 4 x 8 floats
+  static constexpr int kBarsAt = kStatsAt + 2 * 4 * 8 * 4;
+  static constexpr int kFlagsAt = kBarsAt + 2 * kStages * 8;
+  static constexpr int kBytes = kFlagsAt + kStages * 4 + 4;
+  static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
+};
+
+struct Maps {
+  CUtensorMap keys, values;
+};
+
+template <typename H>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(H) == 2 && ElemTraits<H>::kDtype == KSMM_F16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// two e4m3 (the low 16 bits) as fp16
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t v) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename H>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  return pack2(lo, hi, ElemTraits<H>::kDtype);
+}
+template <typename H>
+__device__ __forceinline__ float2 unpack(uint32_t v) {
+  if constexpr (ElemTraits<H>::kDtype == KSMM_F16) return __half22float2(*reinterpret_cast<__half2*>(&v));
+  else return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// T: q and the output.  Tokens of a page that one TMA box covers: `box`.
+template <typename T, bool EIGHT, int DP>
+__global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
+    token_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Attend a, const int box) {
+  using L = Layout<EIGHT, DP>;
+  using H = typename std::conditional<EIGHT, __half, T>::type;  // of the products
+  extern __shared__ __align__(1024) char smem[];
+  const uint32_t base = smem_u32(smem);
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  int* flags = reinterpret_cast<int*>(smem + L::kFlagsAt);
+  volatile int* abort_flag = flags + L::kStages;
+  const uint32_t full = base + L::kBarsAt, empty = full + 8 * L::kStages;
+  if (base % 1024) {  // (without static shared memory it starts there; swizzled tiles need it)
+    if (tid == 0) atomicCAS(a.status, 0, kWaits + 3);
+    return;
+  }
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, kConsumers);
+    }
+    fence_mbar_init();
+  }
+  if (warp == kConsumers && lane == 0) {
+    prefetch_tensormap(&maps.keys);
+    prefetch_tensormap(&maps.values);
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+  clear_rest<T>(a);
+  Share mine;
+  if (!share<kTokenThreads>(a, reinterpret_cast<int64_t*>(smem + L::kMergeAt), &mine)) return;
+  const Pool& p = a.pool;
+  uint32_t n = 0;  // units so far
+  Segment g;
+
+  if (warp == kConsumers) {
+    // ---------------- producer: a lane for each box of a unit, tables 32 boxes ahead ----------------
+    const int boxes = kUnit / box;
+    const uint32_t bytes = static_cast<uint32_t>(box) * 128 * L::kBoxes * 2 + (EIGHT ? 2 * box * 4 : 0);
+    bool alive = true;
+    while (alive && mine.next(a, &g)) {
+      const int32_t* table = p.table + g.s * p.table_stride;
+      int ahead = 0, page_ahead = -1;
+      for (int u = g.from; u < g.to; ++u, ++n) {
+        const int in_batch = (u - g.from) % (32 / boxes);
+        if (in_batch == 0) {
+          // the pages of the next 32 boxes
+          const int token = u * kUnit + lane * box;
+          ahead = token / p.page_size;
+          const bool there = token < g.hi && token + box > g.lo;
+          page_ahead = there ? table[ahead] : -2;  // -2: nothing to load, -1: a page that is not there
+          if (there && (page_ahead < 0 || page_ahead >= p.pages)) page_ahead = -1;
+          ahead = token - ahead * p.page_size;
+        }
+        const int from = in_batch * boxes + lane;
+        const int page = __shfl_sync(0xffffffffu, page_ahead, from & 31), row = __shfl_sync(0xffffffffu, ahead, from & 31);
+        const bool get = lane < boxes && page >= 0;
+        const uint32_t missing = __ballot_sync(0xffffffffu, lane < boxes && page == -1);
+        const uint32_t load = __popc(__ballot_sync(0xffffffffu, get));
+        const int st = n % L::kStages;
+        alive = __all_sync(0xffffffffu, mbar_wait<0>(empty + 8 * st, (n / L::kStages & 1) ^ 1, abort_flag, a.status, kWaits));
+        if (!alive) break;
+        if (lane == 0) {
+          flags[st] = static_cast<int>(missing);
+          if (load) mbar_expect_tx(full + 8 * st, load * bytes);
+          else mbar_arrive(full + 8 * st);
+        }
+        __syncwarp();
+        if (get) {
+          const uint32_t to = base + st * L::kStageBytes + lane * box * 128;
+#pragma unroll
+          for (int b = 0; b < L::kBoxes; ++b) {
+            const int x = b * (EIGHT ? 128 : 64);
+            tma_load_4d(to + b * kUnit * 128, &maps.keys, full + 8 * st, x, row, g.head, page);
+            tma_load_4d(to + L::kOperand + b * kUnit * 128, &maps.values, full + 8 * st, x, row, g.head, page);
+          }
+          if (EIGHT) {
+            const uint32_t at = base + L::kScalesAt + st * L::kScales + lane * box * 4;
+            bulk_load(at, p.scales[0] + page * p.spage[0] + g.head * p.shead[0] + row, box * 4, full + 8 * st);
+            bulk_load(at + kUnit * 4, p.scales[1] + page * p.spage[1] + g.head * p.shead[1] + row, box * 4, full + 8 * st);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (!alive) {
+      // the copies in flight end before the block does
+      int zero = 0;
+      for (uint32_t i = n > L::kStages ? n - L::kStages : 0; i < n; ++i)
+        mbar_wait<100>(full + 8 * (i % L::kStages), i / L::kStages & 1, &zero, a.status, kWaits + 1);
+    }
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  const int gq = lane / 4, q4 = lane % 4;
+  bool alive = true;
+  bool slot_used[2] = {false, false};
+  float* merge = reinterpret_cast<float*>(smem + L::kMergeAt);
+  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt);
+  // lane's row and chunk in the loads of four matrices: K: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1;
+  // V: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1
+  const int k_row = warp * 16 + (lane / 16) * 8 + lane % 8, k_chunk = lane / 8 % 2;
+  const int v_row = warp * 16 + (lane / 8 % 2) * 8 + lane % 8, v_chunk = lane / 16;
+  while (mine.next(a, &g)) {
+    const int rows = min(kTileRows, g.seq.n * a.group - g.tile * kTileRows);
+    uint32_t qf[DP / 16][4];
+    float m[2], sum[2], row_scale[2], vm = 0.f;
+    int position[2];
+    float o[DP / 8][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = gq + 8 * h, row = g.tile * kTileRows + r, t = row / a.group;
+      position[h] = r < rows ? g.seq.length - g.seq.n + t : INT_MAX;  // (a row that is not there masks nothing)
+      m[h] = kNone;
+      sum[h] = 0.f;
+      row_scale[h] = a.scale;
+      const T* from = reinterpret_cast<const T*>(a.q) + (g.seq.start + t) * a.q_token +
+                      (g.head * a.group + row - t * a.group) * a.q_head;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = c * 16 + (EIGHT ? 4 * q4 + 2 * e : 2 * q4 + 8 * e);
+          qf[c][h + 2 * e] = r < rows && d < p.dim ? *reinterpret_cast<const uint32_t*>(from + d) : 0u;
+        }
+      if constexpr (EIGHT && ElemTraits<T>::kDtype == KSMM_BF16) {
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 v = unpack<T>(qf[c][h + 2 * e]);
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^-e, e the largest element's exponent; subnormal rows are taken as 0, rows with infinities as they are
+        const int e = static_cast<int>(__float_as_uint(top) >> 23);
+        const float down = e == 0 || e >= 253 ? (e == 255 ? 1.f : e ? 0x1p-126f : 0.f) : __uint_as_float((254 - e) << 23);
+        const float up = e == 0 || e >= 253 ? (e == 255 ? 1.f : e ? 0x1p126f : 0.f) : __uint_as_float(e << 23);
+        row_scale[h] = a.scale * up;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+          for (int e2 = 0; e2 < 2; ++e2) {
+            const float2 v = unpack<T>(qf[c][h + 2 * e2]);
+            qf[c][h + 2 * e2] = pack<H>(v.x * down, v.y * down);
+          }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+
+    // tokens from `clear` to below `sure` are seen by every row
+    const int sure = g.first_position + 1;
+    const int64_t clear = a.window ? static_cast<int64_t>(g.hi) - a.window : 0;
+#pragma unroll 1
+    for (int u = g.from; u < g.to; ++u, ++n) {
+      const int st = n % L::kStages;
+      alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(full + 8 * st, n / L::kStages & 1, abort_flag, a.status, kWaits + 2));
+      const int token = u * kUnit + warp * 16;  // the warp's first
+      if (alive && token < g.hi && token + 16 > g.lo) {
+        const uint32_t ks = base + st * L::kStageBytes, vs = ks + L::kOperand;
+        const bool missing = flags[st] >> (warp * 16 / box) & 1;
+        // ---- scores ----
+        float s[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        if constexpr (!EIGHT) {
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t b[4];
+            ldmatrix4(b, ks + c / 4 * (kUnit * 128) + k_row * 128 + (((c % 4 * 2 + k_chunk) ^ (k_row & 7)) << 4));
+            mma<H>(s[0], qf[c], b[0], b[1]);
+            mma<H>(s[1], qf[c], b[2], b[3]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < DP / 16; c += 2) {
+            uint32_t b[4];
+            ldmatrix4(b, ks + c / 8 * (kUnit * 128) + k_row * 128 + (((c % 8 + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              mma<H>(s[0], qf[c + e], e4m3_to_half2(b[e]), e4m3_to_half2(b[e] >> 16));
+              mma<H>(s[1], qf[c + e], e4m3_to_half2(b[2 + e]), e4m3_to_half2(b[2 + e] >> 16));
+            }
+          }
+        }
+        float value_scale[2][2];
+        if constexpr (EIGHT) {
+          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + warp * 16 + 2 * q4;
+          float key_scale[2][2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * i), v2 = *reinterpret_cast<const float2*>(sc + kUnit + 8 * i);
+            key_scale[i][0] = k2.x;
+            key_scale[i][1] = k2.y;
+            value_scale[i][0] = v2.x;
+            value_scale[i][1] = v2.y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2] * key_scale[i][e % 2];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2];
+        }
+        const bool edge = token + 16 > sure || token < clear || token < g.lo || missing;
+        bool kept[2][2];  // whether the lane's tokens are the sequence's and there
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = token + 8 * i + 2 * q4 + e % 2;
+              const bool in = j < g.hi && j >= g.lo;
+              kept[i][e % 2] = in && !missing;
+              const bool sees = in && j <= position[e / 2] && (!a.window || j > position[e / 2] - a.window);
+              s[i][e] = sees ? (missing ? __int_as_float(0x7fffffff) : s[i][e]) : -INFINITY;
+              if (EIGHT && !kept[i][e % 2]) value_scale[i][e % 2] = 0.f;
+            }
+        }
+        // ---- running maximum and sum ----
+        float scale_o[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m[h]);
+          scale_o[h] = exp2_fast(m[h] - top);
+          m[h] = top;
+          sum[h] *= scale_o[h];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s[i][2 * h + e] = exp2_fast(s[i][2 * h + e] - top);
+              sum[h] += s[i][2 * h + e];
+            }
+        }
+        if constexpr (EIGHT) {
+          // the weights times the values' scales, relative to a power of two that is at least each of them
+          float top = fmaxf(fmaxf(value_scale[0][0], value_scale[0][1]), fmaxf(value_scale[1][0], value_scale[1][1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          if (top > vm) {
+            const uint32_t e = min((__float_as_uint(top) >> 23) + 1, 254u);
+            const float next = __uint_as_float(e << 23), f = vm / next;
+            vm = next;
+            scale_o[0] *= f;
+            scale_o[1] *= f;
+          }
+          const float back = vm > 0.f ? 1.f / vm : 0.f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][e] *= value_scale[i][e % 2] * back;
+        }
+        if (__any_sync(0xffffffffu, scale_o[0] != 1.f || scale_o[1] != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] *= scale_o[e / 2];
+        }
+        // ---- values ----
+        uint32_t hi[4], part[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x = s[i][2 * h], y = s[i][2 * h + 1];
+            hi[2 * i + h] = pack<H>(x, y);
+            const float2 r = unpack<H>(hi[2 * i + h]);
+            part[2 * i + h] = pack<H>(x - r.x, y - r.y);
+          }
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // 16-bit pairs of tokens, of the first and the second eight
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) keep[i] = (kept[i][0] ? 0xffffu : 0u) | (kept[i][1] ? 0xffff0000u : 0u);
+        }
+        if constexpr (!EIGHT) {
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, vs + c / 4 * (kUnit * 128) + v_row * 128 + (((c % 4 * 2 + v_chunk) ^ (v_row & 7)) << 4));
+            if (edge) {
+              b[0] &= keep[0];
+              b[1] &= keep[1];
+              b[2] &= keep[0];
+              b[3] &= keep[1];
+            }
+            mma<H>(o[2 * c], hi, b[0], b[1]);
+            mma<H>(o[2 * c + 1], hi, b[2], b[3]);
+            mma<H>(o[2 * c], part, b[0], b[1]);
+            mma<H>(o[2 * c + 1], part, b[2], b[3]);
+          }
+        } else {
+          // a chunk of 16 elements: the even ones are one tile of eight, the odd ones the next
+#pragma unroll
+          for (int c = 0; c < DP / 16; c += 2) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, vs + c / 8 * (kUnit * 128) + v_row * 128 + (((c % 8 + v_chunk) ^ (v_row & 7)) << 4));
+            if (edge) {
+              b[0] &= keep[0];
+              b[1] &= keep[1];
+              b[2] &= keep[0];
+              b[3] &= keep[1];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t even0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0020)), odd0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0031));
+              const uint32_t even1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0020));
+              const uint32_t odd1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0031));
+              mma<H>(o[2 * (c + e)], hi, even0, even1);
+              mma<H>(o[2 * (c + e) + 1], hi, odd0, odd1);
+              mma<H>(o[2 * (c + e)], part, even0, even1);
+              mma<H>(o[2 * (c + e) + 1], part, odd0, odd1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + 8 * st);
+    }
+
+    // ---- the four warps' results: 2 and 3 to 0 and 1, then 1 to 0; a lane meets the same lane ----
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+    }
+    if (EIGHT) {
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= vm;
+    }
+    auto give = [&](int buffer) {
+      float* to = merge + buffer * (DP / 2 * 32) + lane;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[(4 * i + e) * 32] = o[i][e];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (q4) continue;
+        stats[(buffer * 4 + h) * 8 + gq] = m[h];
+        stats[(buffer * 4 + 2 + h) * 8 + gq] = sum[h];
+      }
+    };
+    auto take = [&](int buffer) {
+      const float* from = merge + buffer * (DP / 2 * 32) + lane;
+      float mine_f[2], other_f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float other = stats[(buffer * 4 + h) * 8 + gq], top = fmaxf(m[h], other);
+        mine_f[h] = exp2_fast(m[h] - top);
+        other_f[h] = exp2_fast(other - top);
+        m[h] = top;
+        sum[h] = sum[h] * mine_f[h] + stats[(buffer * 4 + 2 + h) * 8 + gq] * other_f[h];
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * mine_f[e / 2] + from[(4 * i + e) * 32] * other_f[e / 2];
+    };
+    bar_sync_named(1, kConsumers * 32);  // (the last segment's have been read)
+    if (warp >= 2) give(warp - 2);
+    bar_sync_named(1, kConsumers * 32);
+    if (warp < 2) take(warp);
+    bar_sync_named(1, kConsumers * 32);
+    if (warp == 1) give(0);
+    bar_sync_named(1, kConsumers * 32);
+    const int slot = g.slot;
+    if (slot) slot_used[slot - 1] = true;
+    if (warp != 0) continue;
+    take(0);
+    if (g.seq.bad || !alive) sum[0] = sum[1] = __int_as_float(0x7fffffff);
+    if (slot && lane == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
+    float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + slot - 1) * kTileRows * (p.dim + 2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = gq + 8 * h;
+      if (r >= rows) continue;
+      const int row = g.tile * kTileRows + r, t = row / a.group;
+      T* to = reinterpret_cast<T*>(a.out) + (g.seq.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
+      const float f = slot ? 1.f : sum[h] == 0.f ? 0.f : 1.f / sum[h];
+      if (slot && q4 == 0) {
+        to_part[kTileRows * p.dim + r] = m[h];
+        to_part[kTileRows * (p.dim + 1) + r] = sum[h];
+      }
+      // pairs of neighbours: 8-bit chunks have them in the two tiles
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        const int d = EIGHT ? i / 2 * 16 + 4 * q4 + 2 * (i % 2) : i * 8 + 2 * q4;
+        const float x = EIGHT ? o[i / 2 * 2][2 * h + i % 2] : o[i][2 * h], y = EIGHT ? o[i / 2 * 2 + 1][2 * h + i % 2] : o[i][2 * h + 1];
+        if (d >= p.dim) continue;
+        if (slot) *reinterpret_cast<float2*>(to_part + r * p.dim + d) = make_float2(x, y);
+        else *reinterpret_cast<uint32_t*>(to + d) = pack<T>(x * f, y * f);
+      }
+    }
+  }
+  if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
+}
+
+template <typename T, bool EIGHT, int DP>
+int launch_one(const Maps& maps, const Attend& a, int box, unsigned grid, cudaStream_t stream) {
+  using L = Layout<EIGHT, DP>;
+  auto kern = token_kernel<T, EIGHT, DP>;
+  static std::atomic<uint64_t> ready{0};  // a bit per device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (err == cudaSuccess && !(ready.load(std::memory_order_acquire) & bit)) {
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    if (err == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  }
+  if (err == cudaSuccess) err = launch_pdl(kern, grid, kTokenThreads, L::kBytes, stream, maps, a, box);
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention token kernel: %s", cudaGetErrorString(err));
+  count_launch();
+  return KSMM_OK;
+}
+
+int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <typename T, bool EIGHT>
+int launch_dim(const Maps& maps, const Attend& a, int box, unsigned grid, cudaStream_t stream) {
+  switch (padded(a.pool.dim)) {
+    case 64: return launch_one<T, EIGHT, 64>(maps, a, box, grid, stream);
+    case 128: return launch_one<T, EIGHT, 128>(maps, a, box, grid, stream);
+    default: return launch_one<T, EIGHT, 256>(maps, a, box, grid, stream);
+  }
+}
+
+}  // namespace
+
+int token_blocks_per_sm(int cache_dtype, int dim) {
+  const bool eight = cache_dtype == KSMM_F8E4M3;
+  switch (padded(dim)) {
+    case 64: return eight ? Layout<true, 64>::kBlocks : Layout<false, 64>::kBlocks;
+    case 128: return eight ? Layout<true, 128>::kBlocks : Layout<false, 128>::kBlocks;
+    default: return eight ? Layout<true, 256>::kBlocks : Layout<false, 256>::kBlocks;
+  }
+}
+
+int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  const Pool& p = a.pool;
+  const bool eight = cache_dtype == KSMM_F8E4M3;
+  const int box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16;
+  Maps maps;
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[4] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(p.page_size), static_cast<uint64_t>(p.kv_heads),
+                              static_cast<uint64_t>(p.pages)};
+    const uint64_t strides[4] = {1, static_cast<uint64_t>(p.token[i]), static_cast<uint64_t>(p.head[i]), static_cast<uint64_t>(p.page[i])};
+    const uint32_t size[4] = {eight ? 128u : 64u, static_cast<uint32_t>(box), 1, 1};
+    const int st = encode_map(i ? &maps.values : &maps.keys, cache_dtype, 4, p.data[i], dims, strides, size);
+    if (st != KSMM_OK) return st;
+  }
+  if (dtype == KSMM_F16)
+    return eight ? launch_dim<__half, true>(maps, a, box, grid, stream) : launch_dim<__half, false>(maps, a, box, grid, stream);
+  return eight ? launch_dim<__nv_bfloat16, true>(maps, a, box, grid, stream)
+               : launch_dim<__nv_bfloat16, false>(maps, a, box, grid, stream);
+}
+
+// Whether TMA can address the pool and the rows of q and out are pairs on their boundary.
+bool token_fits(const ksmm_cache_attention_desc_t& d) {
+  const ksmm_cache_t& c = d.cache;
+  const bool eight = c.cache_dtype == KSMM_F8E4M3;
+  const int per16 = eight ? 16 : 8;
+  if (d.dtype == KSMM_F32 || c.head_dim % per16 || c.page_size % 16 || c.pages == 0) return false;
+  for (int i = 0; i < 2; ++i) {
+    if (reinterpret_cast<uintptr_t>(i ? c.values : c.keys) % 16) return false;
+    const int64_t* s = i ? c.value_strides : c.key_strides;
+    for (int k = 0; k < 3; ++k)
+      if (s[k] <= 0 || s[k] % per16 || s[k] >= (1ll << 38)) return false;
+    if (eight) {
+      const int64_t* f = i ? c.value_scale_strides : c.key_scale_strides;
+      if (reinterpret_cast<uintptr_t>(i ? c.value_scales : c.key_scales) % 16 || f[0] % 4 || f[1] % 4 || f[2] != 1) return false;
+    }
+  }
+  return reinterpret_cast<uintptr_t>(d.q) % 4 == 0 && reinterpret_cast<uintptr_t>(d.out) % 4 == 0 && d.q_strides[0] % 2 == 0 &&
+         d.q_strides[1] % 2 == 0 && d.out_strides[0] % 2 == 0 && d.out_strides[1] % 2 == 0;
+}
+
+}  // namespace cache
+}  // namespace ksmm
