@@ -64,7 +64,7 @@ def _load_native():
         from . import ksmm_torch_ext
     except ImportError:
         return None
-    return ksmm_torch_ext if hasattr(ksmm_torch_ext, "residual_norm") else None
+    return ksmm_torch_ext if hasattr(ksmm_torch_ext, "cache_attention") else None
 
 
 native = _load_native()

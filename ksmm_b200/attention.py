@@ -10,7 +10,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernel import _stream_ptr, dtype_code, no_tangents
+from ._lib import native as _native
+from .kernel import _result, _stream_ptr, dtype_code, no_tangents
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _MAX_INT = 2 ** 31
@@ -111,6 +112,14 @@ def _heads(name, t, heads, cache, tokens, dtype):
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def _tensors(*ts):
+    return all(isinstance(t, torch.Tensor) for t in ts)
+
+
+def _tensors_or_none(*ts):
+    return all(t is None or isinstance(t, torch.Tensor) for t in ts)
+
+
 def _strides(t, n):
     return (ctypes.c_int64 * n)(*t.stride()[:n])
 
@@ -165,6 +174,12 @@ def cache_append(cache, table, lengths, k, v, q=None, *, starts=None, frequencie
     zero in a q that the call makes, and left alone in ``q_out``.  A token whose page is not in the pool is not stored."""
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
+    if _native is not None and _tensors(table, lengths, k, v) and _tensors_or_none(q, starts, frequencies, q_out):
+        # one call of the extension module; None where it is not for it (a wrong argument, another order of elements)
+        done = _native.cache_append(cache.keys, cache.values, cache.key_scales, cache.value_scales, table, lengths, k, v, q, starts,
+                                    frequencies, bool(interleaved), q_out)
+        if done is not None:
+            return None if done is False else _result(done)
     no_tangents(k, v, q)
     k = _heads("k", k, cache.heads, cache, None, None)
     v = _heads("v", v, cache.heads, cache, k.shape[0], k.dtype)
@@ -203,13 +218,20 @@ def cache_attention(q, cache, table, lengths, *, starts=None, scale=None, window
     and left alone in ``out``.  Rows that need a page which is not in the pool are NaN.  Nothing learns through this call."""
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
+    if window is not None and window <= 0 or max_new is not None and max_new <= 0:
+        raise ValueError("window and max_new are positive")
+    if _native is not None and _tensors(q, table, lengths) and _tensors_or_none(starts, out):
+        done = _native.cache_attention(q, cache.keys, cache.values, cache.key_scales, cache.value_scales, table, lengths, starts,
+                                       cache.keys.shape[3] ** -0.5 if scale is None else float(scale),
+                                       0 if window is None else min(int(window), _MAX_INT),
+                                       0 if max_new is None else min(int(max_new), _MAX_INT), out)
+        if done is not None:
+            return _result(done)
     no_tangents(q)
     q = _heads("q", q, None, cache, None, None)
     desc, keep = _cache_desc(cache, table, lengths, starts, q.shape[0])
     if q.shape[1] > 65535:
         raise ValueError(f"q has {q.shape[1]} heads")
-    if window is not None and window <= 0 or max_new is not None and max_new <= 0:
-        raise ValueError("window and max_new are positive")
     result = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else _output("out", out, q, cache.device)
     d = _lib.CacheAttentionDesc(
         cache=desc, q=q.data_ptr(), out=result.data_ptr(), q_strides=_strides(q, 2), out_strides=_strides(result, 2),

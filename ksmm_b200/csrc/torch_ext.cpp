@@ -806,6 +806,163 @@ py::object residual_norm(const at::Tensor& x, const c10::optional<at::Tensor>& y
   return py::cast(z.defined() ? z : h);
 }
 
+// ---------------------------------------------------------------------------
+// a paged cache: cache_append and cache_attention of ksmm_b200.attention
+// ---------------------------------------------------------------------------
+using OptTensor = c10::optional<at::Tensor>;
+constexpr int64_t kCacheMost = 0x7fffffffLL - 65535;
+
+bool strided(const at::Tensor& t) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !t.is_conj(); }
+
+bool indexes(const at::Tensor& t, const at::Device& device, int64_t dims) {
+  return strided(t) && t.scalar_type() == at::kInt && t.device() == device && t.dim() == dims &&
+         (t.numel() == 0 || t.stride(dims - 1) == 1 || t.size(dims - 1) == 1);
+}
+
+void strides_of(const at::Tensor& t, int n, int64_t* to) {
+  for (int i = 0; i < n; ++i) to[i] = t.stride(i);
+}
+
+// the cache, the tables and `tokens` rows; false for what Python has to look at
+bool cache_fits(const at::Tensor& keys, const at::Tensor& values, const OptTensor& key_scales, const OptTensor& value_scales,
+                const at::Tensor& table, const at::Tensor& lengths, const OptTensor& starts, int64_t tokens, ksmm_cache_t* c) {
+  if (!strided(keys) || !strided(values) || keys.dim() != 4 || values.sizes() != keys.sizes() || values.scalar_type() != keys.scalar_type() ||
+      values.device() != keys.device() || (keys.size(3) != 1 && (keys.stride(3) != 1 || values.stride(3) != 1)))
+    return false;
+  const bool eight = keys.scalar_type() == at::kFloat8_e4m3fn;
+  if (!eight && !plain_dtype(keys)) return false;
+  for (int i = 1; i < 4; ++i)
+    if (keys.size(i) <= 0 || keys.size(i) >= kCacheMost) return false;
+  if (keys.size(0) >= kCacheMost) return false;
+  const OptTensor* scales[2] = {&key_scales, &value_scales};
+  for (const OptTensor* q : scales) {
+    if (q->has_value() != eight) return false;
+    if (!eight) continue;
+    const at::Tensor& t = **q;
+    if (!strided(t) || t.scalar_type() != at::kFloat || t.device() != keys.device() || t.sizes() != keys.sizes().slice(0, 3)) return false;
+  }
+  const at::Device device = keys.device();
+  if (!indexes(lengths, device, 1) || !indexes(table, device, 2) || table.size(0) != lengths.size(0)) return false;
+  const int64_t n = lengths.size(0);
+  if (starts.has_value() ? !indexes(*starts, device, 1) || starts->size(0) != n + 1 : n == 0 || tokens % n) return false;
+  if (n == 0 || n >= kCacheMost / keys.size(1) || table.size(1) >= kCacheMost / keys.size(2)) return false;
+  *c = {};
+  c->keys = keys.data_ptr();
+  c->values = values.data_ptr();
+  strides_of(keys, 3, c->key_strides);
+  strides_of(values, 3, c->value_strides);
+  if (eight) {
+    c->key_scales = key_scales->data_ptr<float>();
+    c->value_scales = value_scales->data_ptr<float>();
+    strides_of(*key_scales, 3, c->key_scale_strides);
+    strides_of(*value_scales, 3, c->value_scale_strides);
+  }
+  c->pages = keys.size(0);
+  c->kv_heads = static_cast<int32_t>(keys.size(1));
+  c->page_size = static_cast<int32_t>(keys.size(2));
+  c->head_dim = static_cast<int32_t>(keys.size(3));
+  c->cache_dtype = eight ? KSMM_F8E4M3 : dtype_code(keys);
+  c->table = table.data_ptr<int32_t>();
+  c->table_stride = table.stride(0);
+  c->table_width = static_cast<int32_t>(table.size(1));
+  c->lengths = lengths.data_ptr<int32_t>();
+  c->starts = starts.has_value() ? starts->data_ptr<int32_t>() : nullptr;
+  c->sequences = n;
+  c->tokens = tokens;
+  return true;
+}
+
+// (tokens, heads, head_dim) as the kernels take it; heads 0: any that share the key heads evenly
+bool heads_fit(const at::Tensor& t, const at::Tensor& keys, int64_t heads, at::ScalarType type) {
+  if (!strided(t) || !plain_dtype(t) || t.scalar_type() != type || t.device() != keys.device() || t.dim() != 3 || has_tangent(t) ||
+      t.size(2) != keys.size(3) || (t.size(2) != 1 && t.stride(2) != 1) || t.size(0) >= kCacheMost ||
+      (keys.scalar_type() != type && keys.scalar_type() != at::kFloat8_e4m3fn))
+    return false;
+  if (t.requires_grad() && at::GradMode::is_enabled()) return false;
+  return heads ? t.size(1) == heads : t.size(1) > 0 && t.size(1) <= 65535 && t.size(1) % keys.size(1) == 0;
+}
+
+bool output_fits(const at::Tensor& out, const at::Tensor& like) {
+  return strided(out) && out.sizes() == like.sizes() && out.scalar_type() == like.scalar_type() && out.device() == like.device() &&
+         (out.size(2) == 1 || out.stride(2) == 1) && !out.requires_grad();
+}
+
+py::object cache_append(const at::Tensor& keys, const at::Tensor& values, const OptTensor& key_scales, const OptTensor& value_scales,
+                        const at::Tensor& table, const at::Tensor& lengths, const at::Tensor& k, const at::Tensor& v, const OptTensor& q,
+                        const OptTensor& starts, const OptTensor& frequencies, bool interleaved, const OptTensor& q_out) {
+  ksmm_cache_append_desc_t d = {};
+  if (!strided(keys) || keys.dim() != 4 || keys.size(1) == 0 || !k.defined() || !heads_fit(k, keys, keys.size(1), k.scalar_type()) ||
+      !heads_fit(v, keys, keys.size(1), k.scalar_type()) || v.size(0) != k.size(0) ||
+      !cache_fits(keys, values, key_scales, value_scales, table, lengths, starts, k.size(0), &d.cache))
+    return py::none();
+  if (q.has_value() ? !heads_fit(*q, keys, 0, k.scalar_type()) || q->size(0) != k.size(0) : q_out.has_value()) return py::none();
+  if (q_out.has_value() && !output_fits(*q_out, *q)) return py::none();
+  if (frequencies.has_value()) {
+    if (!strided(*frequencies) || frequencies->scalar_type() != at::kDouble || frequencies->device() != keys.device() ||
+        !frequencies->is_contiguous() || frequencies->dim() != 1 || 2 * frequencies->size(0) > keys.size(3))
+      return py::none();
+    d.frequencies = frequencies->data_ptr<double>();
+    d.pairs = static_cast<int32_t>(frequencies->size(0));
+  }
+  int st;
+  at::Tensor out;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(keys.device());
+    d.k = k.data_ptr();
+    d.v = v.data_ptr();
+    strides_of(k, 2, d.k_strides);
+    strides_of(v, 2, d.v_strides);
+    d.heads = d.cache.kv_heads;
+    d.dtype = dtype_code(k);
+    d.interleaved = interleaved;
+    if (q.has_value()) {
+      out = q_out.has_value() ? *q_out : at::empty(q->sizes(), q->options().requires_grad(false));
+      d.q = q->data_ptr();
+      d.q_out = out.data_ptr();
+      strides_of(*q, 2, d.q_strides);
+      strides_of(out, 2, d.q_out_strides);
+      d.heads = static_cast<int32_t>(q->size(1));
+      d.clear_rest = !q_out.has_value();
+    }
+    st = ksmm_cu_cache_append(&d, stream_of(keys));
+  }
+  if (st != KSMM_OK) return py::cast(st);
+  return q.has_value() ? py::cast(out) : py::cast(false);
+}
+
+py::object cache_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values, const OptTensor& key_scales,
+                           const OptTensor& value_scales, const at::Tensor& table, const at::Tensor& lengths, const OptTensor& starts,
+                           double scale, int64_t window, int64_t max_new, const OptTensor& result_in) {
+  ksmm_cache_attention_desc_t d = {};
+  if (!strided(keys) || keys.dim() != 4 || keys.size(1) == 0 || !q.defined() || !heads_fit(q, keys, 0, q.scalar_type()) ||
+      !cache_fits(keys, values, key_scales, value_scales, table, lengths, starts, q.size(0), &d.cache) ||
+      (result_in.has_value() && !output_fits(*result_in, q)))
+    return py::none();
+  int st;
+  at::Tensor out;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(keys.device());
+    out = result_in.has_value() ? *result_in : at::empty(q.sizes(), q.options().requires_grad(false));
+    d.q = q.data_ptr();
+    d.out = out.data_ptr();
+    strides_of(q, 2, d.q_strides);
+    strides_of(out, 2, d.out_strides);
+    d.window = window;
+    d.max_new = max_new;
+    d.scale = static_cast<float>(scale);
+    d.heads = static_cast<int32_t>(q.size(1));
+    d.dtype = dtype_code(q);
+    d.clear_rest = !result_in.has_value();
+    const size_t need = ksmm_cu_cache_attention_workspace_bytes(&d);
+    at::Tensor ws;
+    if (need) ws = new_bytes(need, out);
+    st = ksmm_cu_cache_attention(&d, need ? ws.data_ptr() : nullptr, need, stream_of(keys));
+  }
+  return result(st, out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -819,6 +976,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_forward", &fp8_forward, "The factors of an fp8 KSLinear");
   m.def("grouped_forward", &grouped_forward, "Several chains on one input");
   m.def("residual_norm", &residual_norm, "Norms around a block, gate, residual scale and modulation");
+  m.def("cache_append", &cache_append, "New tokens' keys and values into a paged cache");
+  m.def("cache_attention", &cache_attention, "Attention over a paged cache");
   m.def("gated_forward", &gated_forward, "A gated layer without gradients");
   m.def("gated_layer", &gated_layer, "A gated layer, as one autograd node where something learns");
 }
