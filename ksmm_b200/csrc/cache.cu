@@ -314,39 +314,61 @@ int launch_append_typed(Append& a, int cache_dtype, cudaStream_t stream) {
   return vec ? launch_append<T, T, VEC>(a, stream) : launch_append<T, T, 1>(a, stream);
 }
 
+// Sequences of up to kFewRows rows (new tokens x heads of a group) are the token kernel's, in up to four tiles that read the keys
+// one after the other; with more the prompt kernel's tiles of 128 rows are at least half full.
+constexpr int kFewRows = 64;
+
 struct Plan {
+  unsigned prompt;        // blocks of the prompt kernel; 0: none
+  int prompt_tile;
+  bool token;             // the other kernel: the token kernel or the CUDA cores'
+  unsigned grid;          // its blocks; 0: none
+  int tile;
   bool split;
-  unsigned grid;
-  size_t bytes;
-  size_t partial_bytes;
+  int most;               // rows of its sequences
+  size_t bytes, partial_bytes;
 };
 
-// A launch over items of tile_rows rows.  Few of them (decoding) are split over their length in units: as many blocks as run at
-// the same time share all units evenly, however the lengths differ.  Many (prompts) get a block each.
-Plan plan_rows(const ksmm_cache_attention_desc_t& d, int tile_rows, int blocks_per_sm) {
+int64_t items(const ksmm_cache_t& c, int64_t group, int tile) { return (c.sequences + c.tokens * group / tile) * c.kv_heads; }
+
+// Few rows (decoding) are split over their length in units: as many blocks as run at the same time share all units evenly,
+// however the lengths differ.  Many get a block for each item.
+bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   const ksmm_cache_t& c = d.cache;
-  Plan p = {};
+  *p = {};
   const int64_t group = d.heads / c.kv_heads;
-  const int64_t most = d.max_new > 0 ? d.max_new : c.starts ? c.tokens : c.tokens / c.sequences;
-  p.split = most * group <= 4 * tile_rows;
-  if (p.split) {
-    int sms = tc::num_sms();
-    if (sms <= 0) sms = 148;
-    // (no more than there can be units)
-    const int64_t units = (static_cast<int64_t>(c.table_width) * c.page_size + kUnit - 1) / kUnit + 1;
-    const int64_t tiles = (most * group + tile_rows - 1) / tile_rows;
-    int64_t blocks = units * tiles * c.kv_heads;
-    blocks = blocks > (1 << 20) ? blocks : blocks * c.sequences;
-    int64_t limit = static_cast<int64_t>(sms) * blocks_per_sm;
-    limit = limit < kMaxBlocks ? limit : kMaxBlocks;
-    p.grid = static_cast<unsigned>(blocks < limit ? (blocks > 0 ? blocks : 1) : limit);
-    p.partial_bytes = (2 * sizeof(float) * p.grid * tile_rows * (c.head_dim + 2) + 255) / 256 * 256;
-    p.bytes = p.partial_bytes + 2 * sizeof(int64_t) * p.grid;
-  } else {
-    const int64_t items = (c.sequences + c.tokens * group / tile_rows) * c.kv_heads;
-    p.grid = items < INT_MAX ? static_cast<unsigned>(items) : 0;
+  int64_t most = c.starts ? c.tokens : c.tokens / c.sequences;
+  if (d.max_new > 0 && d.max_new < most) most = d.max_new;
+  int64_t rows = most * group;
+  p->most = INT_MAX;
+  if (rows > kFewRows && prompt_fits(d)) {
+    p->prompt_tile = prompt_rows(c.head_dim, static_cast<int>(group));
+    const int64_t n = items(c, group, p->prompt_tile);
+    if (n >= INT_MAX) return false;
+    p->prompt = static_cast<unsigned>(n);
+    if (!c.starts) return true;
+    rows = p->most = kFewRows;
   }
-  return p;
+  p->token = token_fits(d);
+  p->tile = p->token ? kTokenRows : rows_tile(c.head_dim);
+  p->split = rows <= kFewRows;
+  if (!p->split) {
+    const int64_t n = items(c, group, p->tile);
+    if (n >= INT_MAX) return false;
+    p->grid = static_cast<unsigned>(n);
+    return true;
+  }
+  int sms = tc::num_sms();
+  if (sms <= 0) sms = 148;
+  // (no more than there can be units)
+  const double units = static_cast<double>(static_cast<int64_t>(c.table_width) * c.page_size / kUnit + 2) *
+                       static_cast<double>((rows + p->tile - 1) / p->tile) * c.kv_heads * static_cast<double>(c.sequences);
+  int limit = sms * (p->token ? token_blocks_per_sm(c.cache_dtype, c.head_dim) : 1);
+  limit = limit < kMaxBlocks ? limit : kMaxBlocks;
+  p->grid = units < limit ? static_cast<unsigned>(units) : static_cast<unsigned>(limit);
+  p->partial_bytes = (2 * sizeof(float) * p->grid * p->tile * (c.head_dim + 2) + 255) / 256 * 256;
+  p->bytes = p->partial_bytes + 2 * sizeof(int64_t) * p->grid;
+  return true;
 }
 
 int check_attention(const ksmm_cache_attention_desc_t* d) {
@@ -355,11 +377,6 @@ int check_attention(const ksmm_cache_attention_desc_t* d) {
   if (st != KSMM_OK) return st;
   if (d->window < 0 || d->max_new < 0) return set_error(KSMM_ERR_BAD_ARGUMENT, "window and max_new are not negative");
   return KSMM_OK;
-}
-
-Plan plan_of(const ksmm_cache_attention_desc_t& d) {
-  if (token_fits(d)) return plan_rows(d, kTokenRows, token_blocks_per_sm(d.cache.cache_dtype, d.cache.head_dim));
-  return plan_rows(d, rows_tile(d.cache.head_dim), 1);
 }
 
 }  // namespace
@@ -405,7 +422,8 @@ int ksmm_cu_cache_append(const ksmm_cache_append_desc_t* d, void* stream) {
 
 size_t ksmm_cu_cache_attention_workspace_bytes(const ksmm_cache_attention_desc_t* d) {
   if (check_attention(d) != KSMM_OK || d->cache.tokens == 0) return 0;
-  return plan_of(*d).bytes;
+  Plan plan;
+  return plan_of(*d, &plan) ? plan.bytes : 0;
 }
 
 int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -413,8 +431,8 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
   if (st != KSMM_OK || d->cache.tokens == 0) return st;
   if (!d->q || !d->out) return set_error(KSMM_ERR_BAD_ARGUMENT, "null pointer");
   const ksmm_cache_t& c = d->cache;
-  const Plan plan = plan_of(*d);
-  if (plan.grid == 0) return set_error(KSMM_ERR_UNSUPPORTED, "too many rows for one call");
+  Plan plan;
+  if (!plan_of(*d, &plan)) return set_error(KSMM_ERR_UNSUPPORTED, "too many rows for one call");
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || reinterpret_cast<uintptr_t>(workspace) % 256))
     return set_error(KSMM_ERR_WORKSPACE, "cache attention needs a workspace of %zu bytes, aligned to 256", plan.bytes);
   Attend a = {};
@@ -430,16 +448,24 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
   a.group = d->heads / c.kv_heads;
   a.scale = d->scale * 1.4426950408889634f;
   a.clear_rest = d->clear_rest != 0;
-  a.least = 1;
-  a.most = INT_MAX;
-  const bool token = token_fits(*d);
-  a.tile_rows = token ? kTokenRows : rows_tile(c.head_dim);
-  a.split = plan.split;
   a.partial = static_cast<float*>(workspace);
   a.slots = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + plan.partial_bytes);
   a.status = tc::status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = token ? launch_token(a, d->dtype, c.cache_dtype, plan.grid, s) : launch_rows(a, d->dtype, c.cache_dtype, plan.grid, s);
+  if (plan.prompt) {
+    a.tile_rows = plan.prompt_tile;
+    a.least = plan.grid ? plan.most + 1 : 1;
+    a.most = INT_MAX;
+    a.split = 0;
+    st = launch_prompt(a, d->dtype, plan.prompt, s);
+    if (st != KSMM_OK || !plan.grid) return st;
+    a.clear_rest = 0;
+  }
+  a.tile_rows = plan.tile;
+  a.least = 1;
+  a.most = plan.most;
+  a.split = plan.split;
+  st = plan.token ? launch_token(a, d->dtype, c.cache_dtype, plan.grid, s) : launch_rows(a, d->dtype, c.cache_dtype, plan.grid, s);
   if (st == KSMM_OK && plan.split) st = launch_join(a, d->dtype, plan.grid, s);
   return st;
 }

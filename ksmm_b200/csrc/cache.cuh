@@ -174,10 +174,15 @@ struct Share {
     offset += to - from;
     g->seq = seq;
     g->s = s;
-    g->head = static_cast<int>(item / work.tiles);
-    g->tile = static_cast<int>(item - static_cast<int64_t>(g->head) * work.tiles);
-    // (without a split the last tile comes first: it sees the most keys)
-    if (!a.split) g->tile = work.tiles - 1 - g->tile;
+    if (a.split) {
+      g->head = static_cast<int>(item / work.tiles);
+      g->tile = static_cast<int>(item - static_cast<int64_t>(g->head) * work.tiles);
+    } else {
+      // the last tiles of all heads come first: they see the most keys
+      const int64_t tile = item / a.pool.kv_heads;
+      g->head = static_cast<int>(item - tile * a.pool.kv_heads);
+      g->tile = work.tiles - 1 - static_cast<int>(tile);
+    }
     const int t0 = static_cast<int>(static_cast<int64_t>(g->tile) * a.tile_rows / a.group);
     g->first_position = seq.length - seq.n + t0;
     g->lo = first_key(a, seq, a.split ? 0 : t0);
@@ -253,6 +258,9 @@ int token_blocks_per_sm(int cache_dtype, int dim);
 constexpr int kTokenRows = 16;    // rows of an item in the 16- and 8-bit kernel
 bool token_fits(const ksmm_cache_attention_desc_t& d);
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
+int prompt_rows(int dim, int group);  // rows of an item in the prompt kernel
+bool prompt_fits(const ksmm_cache_attention_desc_t& d);
+int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
 int launch_join(const Attend& a, int dtype, unsigned blocks, cudaStream_t stream);
 
 }  // namespace cache

@@ -1,0 +1,483 @@
+// Attention of many new tokens (prompts) over a paged cache in 16 bits, on tcgen05.
+//
+// An item is one key head and 1 or 2 tiles of up to 128 rows: a row is (token, head of the group), all heads that share the
+// key head side by side, so that keys and values are read once for them.  Per tile of keys: S = Q K^T into tensor memory, a
+// thread per row turns its S into weights (running maximum, exponentials, sum in fp32) and writes them back as 16-bit
+// pairs, O += P V takes them from tensor memory as its A operand.  P lies over S.  Two row tiles alternate: while the softmax
+// threads of one work, the tensor cores run the other's products.
+//
+// Warps 0..3 and 4..7: rows of the first and second tile; then a TMA warp and a warp that issues the MMAs.  K is K-major as
+// it lies in the pages, V is the MN-major operand (its tokens are the contraction), so neither is turned.  O stays in tensor
+// memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the last time: weights are then at most
+// 256, which 16 bits hold as well as 1, and the sum is exact to fp32 either way.  Weights are rounded once to 16 bits; the sum is
+// that of the unrounded ones (their errors are independent: together as large as the result's own rounding).
+#include <atomic>
+#include <climits>
+
+#include "cache.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
+
+namespace ksmm {
+namespace cache {
+namespace {
+
+using namespace tc;
+
+template <int DP>
+struct Prompt {
+  static constexpr int kTiles = DP == 256 ? 1 : 2;
+  static constexpr int kKeys = DP == 256 ? 64 : 128;           // tokens of a tile of keys
+  static constexpr int kBoxes = DP / 64;                       // 128-byte columns of a row
+  static constexpr int kQ = 128 * DP * 2;                      // a row tile's q
+  static constexpr int kOperand = kKeys * DP * 2;              // a tile of keys or values
+  static constexpr int kStages = (192 * 1024 - kTiles * kQ) / (2 * kOperand);
+  static constexpr int kRingAt = kTiles * kQ;
+  static constexpr int kBarsAt = kRingAt + 2 * kStages * kOperand;
+  // q | k full, k empty, v full, v empty | s, p, o per row tile | a load of its own
+  static constexpr int kBars = 1 + 4 * kStages + 3 * kTiles + 1;
+  static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
+  static constexpr int kSharedAt = kFlagsAt + 8;
+  static constexpr int kBytes = kSharedAt + 40 * 8;
+  static constexpr int kThreads = 128 * kTiles + 64;
+  static constexpr int kSCols = kKeys;
+  static constexpr int kOAt = kTiles * kSCols;
+  static_assert(kOAt + kTiles * DP <= 512, "tensor memory");
+};
+
+struct PromptMaps {
+  CUtensorMap q, keys, values;
+};
+
+struct PromptArgs {
+  Attend a;
+  int tile_tokens;  // of a row tile: its rows are tile_tokens * group
+  int box;          // tokens of a page that a TMA box covers
+  uint32_t idesc_s, idesc_o;
+};
+
+// A from tensor memory: 128 rows, 16 k in 8 columns of pairs
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+constexpr int kPromptWaits = kWaits + 4;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
+    prompt_kernel(const __grid_constant__ PromptMaps maps, const __grid_constant__ PromptArgs args) {
+  using C = Prompt<DP>;
+  extern __shared__ __align__(1024) char smem[];
+  const Attend& a = args.a;
+  const Pool& p = a.pool;
+  const uint32_t base = smem_u32(smem);
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  constexpr int kProducer = 4 * C::kTiles, kIssuer = kProducer + 1;
+  volatile int* abort_flag = reinterpret_cast<int*>(smem + C::kFlagsAt);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kFlagsAt + 4);
+  const uint32_t q_full = base + C::kBarsAt;
+  auto k_full = [&](int i) { return q_full + 8 * (1 + i); };
+  auto k_empty = [&](int i) { return q_full + 8 * (1 + C::kStages + i); };
+  auto v_full = [&](int i) { return q_full + 8 * (1 + 2 * C::kStages + i); };
+  auto v_empty = [&](int i) { return q_full + 8 * (1 + 3 * C::kStages + i); };
+  auto s_full = [&](int t) { return q_full + 8 * (1 + 4 * C::kStages + t); };
+  auto p_full = [&](int t) { return q_full + 8 * (1 + 4 * C::kStages + C::kTiles + t); };
+  auto o_full = [&](int t) { return q_full + 8 * (1 + 4 * C::kStages + 2 * C::kTiles + t); };
+  const uint32_t alone = q_full + 8 * (C::kBars - 1);
+  if (base % 1024) {  // (without static shared memory it starts there; swizzled tiles need it)
+    if (tid == 0) atomicCAS(a.status, 0, kPromptWaits);
+    return;
+  }
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < C::kBars; ++i) mbar_init(q_full + 8 * i, 1);
+    for (int t = 0; t < C::kTiles; ++t) mbar_init(p_full(t), 4);
+    fence_mbar_init();
+  }
+  if (warp == kProducer && lane == 0) {
+    prefetch_tensormap(&maps.q);
+    prefetch_tensormap(&maps.keys);
+    prefetch_tensormap(&maps.values);
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+  clear_rest<T>(a);
+  Share mine;
+  Segment g;
+  if (!share<C::kThreads>(a, reinterpret_cast<int64_t*>(smem + C::kSharedAt), &mine)) return;
+  mine.next(a, &g);
+  if (warp == kIssuer) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // tiles of keys: [first, first + count[t]) for row tile t
+  const int first = g.lo / C::kKeys, token0 = g.tile * C::kTiles * args.tile_tokens;
+  int count[C::kTiles], most = 0;
+#pragma unroll
+  for (int t = 0; t < C::kTiles; ++t) {
+    const int from = token0 + t * args.tile_tokens, to = min(from + args.tile_tokens, g.seq.n);
+    const int hi = from < g.seq.n ? max(g.seq.length - g.seq.n + to, 0) : 0;
+    count[t] = max((hi + C::kKeys - 1) / C::kKeys - first, 0);
+    most = max(most, count[t]);
+  }
+
+  if (warp == kProducer) {
+    // ---------------- TMA: a lane for each box of a tile, tables 32 boxes ahead ----------------
+    const int boxes = C::kKeys / args.box;
+    const uint32_t bytes = static_cast<uint32_t>(args.box) * DP * 2;
+    const int32_t* table = p.table + g.s * p.table_stride;
+    if (most > 0 && lane == 0) {
+      mbar_expect_tx(q_full, static_cast<uint32_t>(args.tile_tokens * a.group) * DP * 2 * C::kTiles);
+#pragma unroll
+      for (int t = 0; t < C::kTiles; ++t)
+#pragma unroll
+        for (int b = 0; b < C::kBoxes; ++b)
+          tma_load_3d(base + t * C::kQ + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group,
+                      g.seq.start + token0 + t * args.tile_tokens);
+    }
+    int page_ahead = -2, ahead = 0;
+    int loaded_k = 0, loaded_v = 0, lone = 0;
+    bool alive = true;
+    for (int j = 0; j < most && alive; ++j) {
+      const int in_batch = j % (32 / boxes);
+      if (in_batch == 0) {
+        const int token = (first + j) * C::kKeys + lane * args.box;
+        ahead = token / p.page_size;
+        const bool there = token < g.hi && token + args.box > g.lo;
+        page_ahead = there ? table[ahead] : -2;
+        if (page_ahead < 0 || page_ahead >= p.pages) page_ahead = -2;
+        ahead = token - ahead * p.page_size;
+      }
+      const int from = in_batch * boxes + lane;
+      const int page = __shfl_sync(0xffffffffu, page_ahead, from & 31), row = __shfl_sync(0xffffffffu, ahead, from & 31);
+      const bool get = lane < boxes && page >= 0;
+      const uint32_t gets = __ballot_sync(0xffffffffu, get);
+      const uint32_t load = __popc(gets);
+      const int tile_token = (first + j) * C::kKeys;
+      const int st = j % C::kStages;
+      const uint32_t parity = (j / C::kStages & 1) ^ 1;
+      alive = __all_sync(0xffffffffu, mbar_wait<20>(k_empty(st), parity, abort_flag, a.status, kPromptWaits + 1));
+      if (!alive) break;
+      if (lane == 0) {
+        if (load) mbar_expect_tx(k_full(st), load * bytes);
+        else mbar_arrive(k_full(st));
+      }
+      ++loaded_k;
+      __syncwarp();
+      const uint32_t kt = base + C::kRingAt + st * C::kOperand, vt = kt + C::kStages * C::kOperand;
+      if (get) {
+#pragma unroll
+        for (int b = 0; b < C::kBoxes; ++b)
+          tma_load_4d(kt + b * C::kKeys * 128 + lane * args.box * 128, &maps.keys, k_full(st), b * 64, row, g.head, page);
+      }
+      __syncwarp();
+      alive = __all_sync(0xffffffffu, mbar_wait<20>(v_empty(st), parity, abort_flag, a.status, kPromptWaits + 1));
+      if (!alive) break;
+      // values that no row may meet are zeros, whatever lies in the page behind the sequence or in the stage from before
+      const bool ragged = load < boxes || tile_token < g.lo || tile_token + C::kKeys > g.hi;
+      const uint32_t bar = ragged ? alone : v_full(st);
+      if (lane == 0 && load) mbar_expect_tx(bar, load * bytes);
+      __syncwarp();
+      if (get) {
+#pragma unroll
+        for (int b = 0; b < C::kBoxes; ++b)
+          tma_load_4d(vt + b * C::kKeys * 128 + lane * args.box * 128, &maps.values, bar, b * 64, row, g.head, page);
+      }
+      __syncwarp();
+      if (!ragged) {
+        ++loaded_v;
+        continue;
+      }
+      if (load) {
+        alive = __all_sync(0xffffffffu, mbar_wait<20>(alone, lone & 1, abort_flag, a.status, kPromptWaits + 2));
+        if (!alive) break;
+        ++lone;
+      }
+      for (int i = lane; i < C::kKeys * C::kBoxes * 8; i += 32) {
+        const int r = i / 8 % C::kKeys, token = tile_token + r;
+        const bool keep = token >= g.lo && token < g.hi && (gets >> (r / args.box) & 1);
+        if (!keep) *reinterpret_cast<uint4*>(smem + (vt - base) + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_full(st));
+      ++loaded_v;
+    }
+    if (!alive) {
+      // the copies in flight end before the block does (one of its own: `alone`; waits that give up already did)
+      int zero = 0;
+      for (int j = loaded_k > C::kStages ? loaded_k - C::kStages : 0; j < loaded_k; ++j)
+        mbar_wait<100>(k_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
+      for (int j = loaded_v > C::kStages ? loaded_v - C::kStages : 0; j < loaded_v; ++j)
+        mbar_wait<100>(v_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
+      if (most > 0) mbar_wait<100>(q_full, 0, &zero, a.status, kPromptWaits + 2);
+    }
+  } else if (warp == kIssuer) {
+    // ---------------- MMAs: the warp walks the loop, one lane issues ----------------
+    constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    const bool one = elect_one();
+    bool alive = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(bar, parity, abort_flag, a.status, kPromptWaits + 3));
+      return alive;
+    };
+    auto commit = [&](uint32_t bar) {
+      if (one) umma_commit(bar);
+    };
+    auto scores = [&](int t, int st) {
+      if (one) {
+        const uint32_t q = (base + t * C::kQ) >> 4 | 1u << 16, k = (base + C::kRingAt + st * C::kOperand) >> 4 | 1u << 16;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint64_t qd = static_cast<uint64_t>(kDescHi) << 32 | (q + i / 4 * (128 * 128 >> 4) + i % 4 * 2);
+          const uint64_t kd = static_cast<uint64_t>(kDescHi) << 32 | (k + i / 4 * (C::kKeys * 128 >> 4) + i % 4 * 2);
+          umma<2>(tmem + t * C::kSCols, qd, kd, args.idesc_s, i != 0);
+        }
+      }
+      commit(s_full(t));
+    };
+    auto outputs = [&](int t, int st, bool more) {
+      if (one) {
+        const uint32_t v = (base + C::kRingAt + (C::kStages + st) * C::kOperand) >> 4 | static_cast<uint32_t>(C::kKeys * 128 >> 4) << 16;
+#pragma unroll
+        for (int i = 0; i < C::kKeys / 16; ++i) {
+          const uint64_t vd = static_cast<uint64_t>(kDescHi) << 32 | (v + i * (16 * 128 >> 4));
+          umma_ts(tmem + C::kOAt + t * DP, tmem + t * C::kSCols + i * 8, vd, args.idesc_o, more || i != 0);
+        }
+      }
+    };
+    if (most > 0 && wait(q_full, 0) && wait(k_full(0), 0)) {
+      tc_fence_after();
+#pragma unroll
+      for (int t = 0; t < C::kTiles; ++t)
+        if (count[t] > 0) scores(t, 0);
+      commit(k_empty(0));
+      for (int j = 0; j < most; ++j) {
+        const int st = j % C::kStages, next = (j + 1) % C::kStages;
+        if (!wait(v_full(st), j / C::kStages & 1)) break;
+        if (j + 1 < most && !wait(k_full(next), (j + 1) / C::kStages & 1)) break;
+#pragma unroll
+        for (int t = 0; t < C::kTiles; ++t) {
+          if (j >= count[t] || !wait(p_full(t), j & 1)) continue;
+          tc_fence_after();
+          outputs(t, st, j > 0);
+          if (j + 1 == count[t]) commit(o_full(t));
+          else scores(t, next);  // (over P, which the MMAs before have read: they run in order)
+        }
+        if (!alive) break;
+        commit(v_empty(st));
+        if (j + 1 < most) commit(k_empty(next));
+      }
+    }
+    if (!alive) {
+      // MMAs in flight end before tensor memory is given back
+      int zero = 0;
+      commit(alone);
+      mbar_wait<100>(alone, 0, &zero, a.status, kPromptWaits + 3);
+    }
+  } else {
+    // ---------------- a thread per row ----------------
+    const int t = warp / 4, r = tid % 128;
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const uint32_t s_at = tmem + lanes + t * C::kSCols, o_at = tmem + lanes + C::kOAt + t * DP;
+    const int token = token0 + t * args.tile_tokens + r / a.group;
+    const bool live = r < args.tile_tokens * a.group && token < g.seq.n;
+    const int position = g.seq.length - g.seq.n + token;
+    const int mine_count = t == 0 ? count[0] : count[C::kTiles - 1];
+    const int sure = g.seq.length - g.seq.n + token0 + t * args.tile_tokens + 1;  // keys below are seen by all rows of the tile
+    const int64_t clear = a.window ? static_cast<int64_t>(sure) - 1 + args.tile_tokens - a.window : 0;  // so are keys from here on
+    const int64_t oldest = a.window ? position - a.window + 1 : 0;
+    const int boxes = C::kKeys / args.box;
+    float top = kNone, sum = 0.f;
+    bool alive = true;
+    // whether lane i's box of the next tile is a page that is not there
+    auto missing_box = [&](int j) {
+      const int at = (first + j) * C::kKeys + lane * args.box;
+      if (lane >= boxes || at >= g.hi || at + args.box <= g.lo) return false;
+      const int page = p.table[g.s * p.table_stride + at / p.page_size];
+      return page < 0 || page >= p.pages;
+    };
+    bool missing_next = mine_count > 0 && missing_box(0);
+    for (int j = 0; j < mine_count; ++j) {
+      const uint32_t missing = __ballot_sync(0xffffffffu, missing_next);
+      if (j + 1 < mine_count) missing_next = missing_box(j + 1);
+      alive = __all_sync(0xffffffffu, mbar_wait<0>(s_full(t), j & 1, abort_flag, a.status, kPromptWaits + 4));
+      if (!alive) break;
+      tc_fence_after();
+      float s[C::kKeys];
+#pragma unroll
+      for (int c = 0; c < C::kKeys; c += 32) tmem_ld32(s_at + c, reinterpret_cast<uint32_t*>(s) + c);
+      tmem_ld_wait();
+      const int key = (first + j) * C::kKeys;
+      if (key + C::kKeys > sure || key < clear || key < g.lo || missing) {
+#pragma unroll
+        for (int c = 0; c < C::kKeys; ++c) {
+          const int at = key + c;
+          if (missing && (missing >> (c / args.box) & 1)) s[c] = __int_as_float(0x7fffffff);
+          if (at > position || at < oldest || at >= g.hi) s[c] = -INFINITY;
+        }
+      }
+      float high[4] = {top, s[0], s[1], s[2]};
+#pragma unroll
+      for (int c = 3; c < C::kKeys; ++c) high[c % 4] = fmaxf(high[c % 4], s[c]);
+      const float now = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+      const bool grown = (now - top) * a.scale > 8.f;
+      if (j == 0) {
+        top = now;
+      } else if (__any_sync(0xffffffffu, grown)) {
+        const float f = grown ? exp2_fast((top - now) * a.scale) : 1.f;
+        if (grown) top = now;
+        sum *= f;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_at + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st32(o_at + c, o);
+        }
+      }
+      const float shift = top == kNone ? 0.f : -top * a.scale;
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < C::kKeys; c += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float x = exp2_fast(fmaf(s[c + 2 * e], a.scale, shift)), y = exp2_fast(fmaf(s[c + 2 * e + 1], a.scale, shift));
+          sums[e % 4] += x + y;
+          w[e] = pack2(x, y, ElemTraits<T>::kDtype);
+        }
+        tmem_st32(s_at + c / 2, w);
+      }
+      sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(t));
+    }
+    if (mine_count > 0 && alive)
+      alive = __all_sync(0xffffffffu, mbar_wait<20>(o_full(t), 0, abort_flag, a.status, kPromptWaits + 4));
+    tc_fence_after();
+    T* to = reinterpret_cast<T*>(a.out) + static_cast<int64_t>(g.seq.start + token) * a.out_token +
+            static_cast<int64_t>(g.head * a.group + r % a.group) * a.out_head;
+    if (g.seq.bad || !alive) sum = __int_as_float(0x7fffffff);
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+    for (int c = 0; c < DP; c += 32) {
+      uint32_t o[32];
+      if (mine_count > 0 && alive) {
+        tmem_ld32(o_at + c, o);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0u;
+      }
+      if (!live) continue;
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        if (c + e >= p.dim) break;
+        uint4 v;
+        v.x = pack2(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, ElemTraits<T>::kDtype);
+        v.y = pack2(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f, ElemTraits<T>::kDtype);
+        v.z = pack2(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f, ElemTraits<T>::kDtype);
+        v.w = pack2(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f, ElemTraits<T>::kDtype);
+        *reinterpret_cast<uint4*>(to + c + e) = v;
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kIssuer) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int DP>
+int launch_one(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cudaStream_t stream) {
+  using C = Prompt<DP>;
+  auto kern = prompt_kernel<T, DP>;
+  static std::atomic<uint64_t> ready{0};  // a bit per device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (err == cudaSuccess && !(ready.load(std::memory_order_acquire) & bit)) {
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (err == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  }
+  if (err == cudaSuccess) err = launch_pdl(kern, grid, C::kThreads, C::kBytes, stream, maps, args);
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention prompt kernel: %s", cudaGetErrorString(err));
+  count_launch();
+  return KSMM_OK;
+}
+
+template <typename T>
+int launch_dim(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cudaStream_t stream) {
+  if (args.a.pool.dim <= 64) return launch_one<T, 64>(maps, args, grid, stream);
+  if (args.a.pool.dim <= 128) return launch_one<T, 128>(maps, args, grid, stream);
+  return launch_one<T, 256>(maps, args, grid, stream);
+}
+
+}  // namespace
+
+int prompt_rows(int dim, int group) { return (dim <= 128 ? 2 : 1) * (128 / group) * group; }
+
+bool prompt_fits(const ksmm_cache_attention_desc_t& d) {
+  const int group = d.heads / d.cache.kv_heads;
+  if (d.cache.cache_dtype == KSMM_F8E4M3 || !token_fits(d) || group > 128) return false;
+  // (a negative scale would turn the maximum round)
+  if (!(d.scale > 0.f) || d.scale > 1e30f) return false;
+  return reinterpret_cast<uintptr_t>(d.q) % 16 == 0 && reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.q_strides[0] > 0 &&
+         d.q_strides[1] > 0 && d.q_strides[0] % 8 == 0 && d.q_strides[1] % 8 == 0 && d.q_strides[0] < (1ll << 38) &&
+         d.q_strides[1] < (1ll << 38) && d.out_strides[0] % 8 == 0 && d.out_strides[1] % 8 == 0;
+}
+
+int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream) {
+  const Pool& p = a.pool;
+  PromptArgs args = {};
+  args.a = a;
+  args.tile_tokens = 128 / a.group;
+  const int keys = p.dim <= 128 ? Prompt<128>::kKeys : Prompt<256>::kKeys;
+  static_assert(Prompt<64>::kKeys == Prompt<128>::kKeys, "one tile of keys up to 128 dims");
+  args.box = keys;
+  while (p.page_size % args.box) args.box /= 2;
+  const uint32_t fmt = dtype == KSMM_F16 ? 0u : 1u;
+  const uint32_t common = 1u << 4 | fmt << 7 | fmt << 10 | 128u >> 4 << 24;
+  const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
+  args.idesc_s = common | static_cast<uint32_t>(keys >> 3) << 17;
+  args.idesc_o = common | 1u << 16 | dp >> 3 << 17;
+  PromptMaps maps;
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[4] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(p.page_size), static_cast<uint64_t>(p.kv_heads),
+                              static_cast<uint64_t>(p.pages)};
+    const uint64_t strides[4] = {1, static_cast<uint64_t>(p.token[i]), static_cast<uint64_t>(p.head[i]), static_cast<uint64_t>(p.page[i])};
+    const uint32_t size[4] = {64, static_cast<uint32_t>(args.box), 1, 1};
+    const int st = encode_map(i ? &maps.values : &maps.keys, dtype, 4, p.data[i], dims, strides, size);
+    if (st != KSMM_OK) return st;
+  }
+  const uint64_t dims[3] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(a.heads), static_cast<uint64_t>(p.tokens)};
+  const uint64_t strides[3] = {1, static_cast<uint64_t>(a.q_head), static_cast<uint64_t>(a.q_token)};
+  const uint32_t size[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(args.tile_tokens)};
+  const int st = encode_map(&maps.q, dtype, 3, a.q, dims, strides, size);
+  if (st != KSMM_OK) return st;
+  return dtype == KSMM_F16 ? launch_dim<__half>(maps, args, grid, stream) : launch_dim<__nv_bfloat16>(maps, args, grid, stream);
+}
+
+}  // namespace cache
+}  // namespace ksmm
