@@ -1,9 +1,12 @@
 // Attention over a paged cache: the append kernel and the C entry points.
 //
-// Append: a block per token (and per 4 rounds of its rows) finds the token's sequence, position and page, forms the cosines and
-// sines of its rotation once for all heads, and moves its rows of q, k and v.  The rows are loaded before all of that: their
-// way from memory overlaps the chain starts -> length -> page.  An angle is position * frequency, formed and reduced to a
-// part of a turn in 64 bits (a position of 10^6 leaves 32 bits four digits of the angle).
+// Append: a warp takes a token (or, where there are few, some of its rows).  It finds the token's sequence, position and page,
+// forms the cosines and sines of its rotation once for all heads and keeps them in registers, and moves its rows of q, k and v, four
+// rounds in flight; the next token's chain starts -> length -> page is on its way meanwhile, and no warp waits for another (blocks
+// of 8 warps that met at barriers for each token: 366 us for 32768 tokens of 32 + 16 rows of 128 in bf16).  An angle is
+// position * frequency, formed and reduced to a part of a turn in 64 bits (a position of 10^6 leaves 32 bits four digits of the
+// angle).
+#include <algorithm>
 #include <climits>
 
 #include "cache.cuh"
@@ -15,7 +18,7 @@ namespace cache {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kRounds = 4;
+constexpr int kFlight = 4;  // rounds of a warp in flight
 
 struct Append {
   Pool pool;
@@ -25,12 +28,78 @@ struct Append {
   const double* frequencies;
   int pairs, interleaved, heads, clear_rest;
   int lanes;             // threads of a row, a power of two up to 32
+  int chunks;            // of a token: chunk_rows rows each
+  int chunk_rows;
+};
+
+// VEC elements of type T as they lie in memory.  (Words and shifts: packing through arrays of 16-bit elements put them into local
+// memory, 84 of every 100 instructions.)
+template <typename T, int VEC>
+struct Packed {
+  static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 4;
+  uint32_t w[kWords];
+  __device__ void load(const T* p) {
+    if constexpr (kWords == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x;
+      w[1] = v.y;
+      w[2] = v.z;
+      w[3] = v.w;
+    } else {
+      static_assert(kWords == 4, "16 bytes");
+    }
+  }
+  __device__ void unpack(float (&f)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else if constexpr (ElemTraits<T>::kDtype == KSMM_BF16) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const uint32_t bits = w[i];
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&bits));
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+      }
+    }
+  }
+};
+template <typename T>
+struct Packed<T, 1> {
+  T v;
+  __device__ void load(const T* p) { v = *p; }
+  __device__ void unpack(float (&f)[1]) const { f[0] = ElemTraits<T>::to_float(v); }
 };
 
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
-  T v[VEC];
-};
+__device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = ElemTraits<T>::from_float(f[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  } else {
+    constexpr int kDt = ElemTraits<T>::kDtype;
+    *reinterpret_cast<uint4*>(p) = make_uint4(tc::pack2(f[0], f[1], kDt), tc::pack2(f[2], f[3], kDt), tc::pack2(f[4], f[5], kDt), tc::pack2(f[6], f[7], kDt));
+  }
+}
+// as e4m3; the quotient by the scale, not the product with its reciprocal: that is what the scale stands for
+__device__ __forceinline__ uint32_t e4m3_pair(float x, float y, float scale) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(x / scale, y / scale), __NV_SATFINITE, __NV_E4M3);
+}
+template <int VEC>
+__device__ __forceinline__ void store_eight(char* p, const float (&f)[VEC], float scale) {
+  if constexpr (VEC == 1) {
+    *reinterpret_cast<uint8_t*>(p) = __nv_cvt_float_to_fp8(f[0] / scale, __NV_SATFINITE, __NV_E4M3);
+  } else {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) w[i] = e4m3_pair(f[4 * i], f[4 * i + 1], scale) | e4m3_pair(f[4 * i + 2], f[4 * i + 3], scale) << 16;
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+}
 
 // Element of a row where piece `u` of VEC pairs starts, first and second half.  Pieces are rotated pairs first, then the rest.
 template <int VEC>
@@ -48,165 +117,215 @@ __device__ __forceinline__ void piece(int u, int pairs, int interleaved, int* fi
   }
 }
 
-// T: the model's type, C: the cache's; VEC elements at a time, with PIECES pieces of a row per thread (VEC 1: pairs is any number
+// What a block knows of a token before it moves its rows.
+struct Place {
+  int64_t position;
+  int64_t page;  // -1: not stored
+  int slot;
+  int there;     // whether it is a sequence's
+};
+
+__device__ __forceinline__ Place place_of(const Pool& p, int t) {
+  Place r = {0, -1, 0, 0};
+  int s;
+  if (p.starts) {
+    // the last sequence that starts at or before it
+    int low = 0, high = p.sequences + 1;  // the first `low` do, those from `high` on do not
+    while (low < high) {
+      const int mid = low + (high - low) / 2;
+      if (p.starts[mid] <= t) low = mid + 1;
+      else high = mid;
+    }
+    s = low - 1;
+  } else {
+    s = t / p.each;
+  }
+  if (s < 0 || s >= p.sequences) return r;
+  r.there = 1;
+  const int64_t start = p.starts ? p.starts[s] : static_cast<int64_t>(s) * p.each;
+  const int64_t n = p.starts ? p.starts[s + 1] - start : p.each;
+  r.position = static_cast<int64_t>(p.lengths[s]) - n + (t - start);
+  if (r.position >= 0 && r.position < static_cast<int64_t>(p.table_width) * p.page_size) {
+    const int at = static_cast<int>(r.position) / p.page_size;
+    r.slot = static_cast<int>(r.position) - at * p.page_size;
+    r.page = p.table[s * p.table_stride + at];
+    if (r.page >= p.pages || r.page < 0) r.page = -1;
+  }
+  return r;
+}
+
+// Rows of one kind (heads of q, k or v) of a token, [from, to), per_round at a time.
+template <typename T, int VEC, int PIECES, bool EIGHT, bool INTER>
+__device__ __forceinline__ void move_rows(const T* src, int64_t src_head, char* dst, int64_t dst_head, float* scales, int64_t scale_head,
+                                          int from, int to, int dim, int lanes, int lane, int nth, bool turns, bool eight,
+                                          const int (&first)[PIECES], const int (&second)[PIECES], const bool (&turned)[PIECES],
+                                          const float2 (&turn)[PIECES][VEC]) {
+  const int per_round = 32 / lanes;
+  src += (from + nth) * src_head;
+  const int64_t dst_step = dst_head * (EIGHT && eight ? 1 : static_cast<int64_t>(sizeof(T)));
+  dst += (from + nth) * dst_step;
+#pragma unroll 1
+  for (int row0 = from; row0 < to; row0 += kFlight * per_round) {
+    Packed<T, VEC> x[kFlight][PIECES], y[kFlight][PIECES];
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      if (row0 + i * per_round + nth < to) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+          if (first[k] < dim) x[i][k].load(src + first[k]);
+          if (second[k] < dim) y[i][k].load(src + second[k]);
+        }
+      }
+      src += per_round * src_head;
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      // (the rows of a round stay together: their lanes meet in shuffles)
+      const int row = row0 + i * per_round + nth;
+      if (row - nth >= to) break;
+      float u[PIECES][VEC], v[PIECES][VEC], top = 0.f;
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        x[i][k].unpack(u[k]);
+        y[i][k].unpack(v[k]);
+        if (turns && turned[k]) {
+          if constexpr (INTER && VEC > 1) {
+            // the pairs are neighbours: VEC / 2 in each vector
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+              const float2 c = turn[k][j], d = turn[k][VEC / 2 + j];
+              const float u0 = u[k][2 * j], u1 = u[k][2 * j + 1], v0 = v[k][2 * j], v1 = v[k][2 * j + 1];
+              u[k][2 * j] = u0 * c.x - u1 * c.y;
+              u[k][2 * j + 1] = u0 * c.y + u1 * c.x;
+              v[k][2 * j] = v0 * d.x - v1 * d.y;
+              v[k][2 * j + 1] = v0 * d.y + v1 * d.x;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              const float u0 = u[k][j], v0 = v[k][j];
+              u[k][j] = u0 * turn[k][j].x - v0 * turn[k][j].y;
+              v[k][j] = u0 * turn[k][j].y + v0 * turn[k][j].x;
+            }
+          }
+        }
+        if (EIGHT && eight) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            if (first[k] < dim) top = fmaxf(top, fabsf(u[k][j]));
+            if (second[k] < dim) top = fmaxf(top, fabsf(v[k][j]));
+          }
+        }
+      }
+      if (EIGHT && eight) {
+        for (int w = lanes / 2; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        const float scale = fmaxf(top / 448.f, 1.1754943508e-38f);
+        if (row < to) {
+          if (lane == 0) scales[row * scale_head] = scale;
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k) {
+            if (first[k] < dim) store_eight<VEC>(dst + first[k], u[k], scale);
+            if (second[k] < dim) store_eight<VEC>(dst + second[k], v[k], scale);
+          }
+        }
+      } else if (row < to) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+          if (first[k] < dim) store<T, VEC>(reinterpret_cast<T*>(dst) + first[k], u[k]);
+          if (second[k] < dim) store<T, VEC>(reinterpret_cast<T*>(dst) + second[k], v[k]);
+        }
+      }
+      dst += per_round * dst_step;
+    }
+  }
+}
+
+// T: the model's type, C: the cache's; VEC elements at a time, with PIECES pieces of a row per lane (VEC 1: pairs is any number
 // and a row up to 4 * 32 * 2 elements).
-template <typename T, typename C, int VEC>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ Append a) {
+template <typename T, typename C, int VEC, bool INTER>
+__global__ void __launch_bounds__(kAppendThreads, 2) append_kernel(const __grid_constant__ Append a) {
   constexpr bool kEight = sizeof(C) == 1;
   constexpr int PIECES = VEC == 1 ? 4 : 1;
-  __shared__ float2 turn[kMaxDim / 2];
+  constexpr int kWarps = kAppendThreads / 32;
+  __shared__ __align__(16) float2 turns[VEC == 1 ? 1 : kWarps][kMaxDim / 2];
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   const Pool& p = a.pool;
-  const int t = blockIdx.x, tid = threadIdx.x;
-  const int lane = tid % a.lanes, per_round = kAppendThreads / a.lanes;
+  const int warp = threadIdx.x / 32, wl = threadIdx.x % 32;
+  const int lane = wl % a.lanes, nth = wl / a.lanes;
   const int q_rows = a.in[0] ? a.heads : 0, rows = q_rows + 2 * p.kv_heads;
-  const int first_row = blockIdx.y * kRounds * per_round + tid / a.lanes;
-
-  Vec<T, VEC> x[kRounds][PIECES], y[kRounds][PIECES];
+  const int64_t items = static_cast<int64_t>(p.tokens) * a.chunks, warps = static_cast<int64_t>(gridDim.x) * kWarps;
+  int first[PIECES], second[PIECES];
+  bool turned[PIECES];
 #pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const int row = first_row + i * per_round;
-    if (row >= rows) break;
-    const int what = row < q_rows ? 0 : row < q_rows + p.kv_heads ? 1 : 2;
-    const int head = what == 0 ? row : row - q_rows - (what - 1) * p.kv_heads;
-    const T* from = reinterpret_cast<const T*>(a.in[what]) + t * a.token[what] + head * a.head[what];
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      int d, e;
-      piece<VEC>(lane + k * 32, a.pairs, a.interleaved, &d, &e);
-      if (d < p.dim) x[i][k] = *reinterpret_cast<const Vec<T, VEC>*>(from + d);
-      if (e < p.dim) y[i][k] = *reinterpret_cast<const Vec<T, VEC>*>(from + e);
-    }
+  for (int k = 0; k < PIECES; ++k) {
+    piece<VEC>(lane + k * 32, a.pairs, INTER, &first[k], &second[k]);
+    turned[k] = (lane + k * 32) * VEC < a.pairs;
   }
 
-  // the token's sequence: as many as start at or before it
-  int s;
-  int64_t start, n;
-  if (p.starts) {
-    int count = 0;
-    for (int i = 0; i <= p.sequences; i += kAppendThreads)
-      count += __syncthreads_count(i + tid <= p.sequences && p.starts[i + tid] <= t);
-    s = count - 1;
-    const bool there = s >= 0 && s < p.sequences;
-    start = there ? p.starts[s] : 0;
-    n = there ? static_cast<int64_t>(p.starts[s + 1]) - start : 0;
-    if (!there) {
-      // a row of no sequence
-      if (!a.clear_rest || !a.q_out) return;
-#pragma unroll
-      for (int i = 0; i < kRounds; ++i) {
-        const int row = first_row + i * per_round;
-        if (row >= q_rows) return;
-        T* to = reinterpret_cast<T*>(a.q_out) + t * a.out_token + row * a.out_head;
-        for (int d = lane; d < p.dim; d += a.lanes) to[d] = ElemTraits<T>::from_float(0.f);
-      }
-      return;
+  int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  if (item >= items) return;
+  int t = static_cast<int>(item / a.chunks);
+  Place next = place_of(p, t);
+#pragma unroll 1
+  for (; item < items; item += warps) {
+    const Place place = next;
+    const int this_t = t, row0 = static_cast<int>(item - static_cast<int64_t>(t) * a.chunks) * a.chunk_rows;
+    const int end = min(rows, row0 + a.chunk_rows);
+    if (item + warps < items) {
+      t = static_cast<int>((item + warps) / a.chunks);
+      next = place_of(p, t);
     }
-  } else {
-    s = t / p.each;
-    start = static_cast<int64_t>(s) * p.each;
-    n = p.each;
-  }
-  const int64_t position = static_cast<int64_t>(p.lengths[s]) - n + (t - start);
-  int64_t page = -1;
-  int slot = 0;
-  if (position >= 0 && position < static_cast<int64_t>(p.table_width) * p.page_size) {
-    const int at = static_cast<int>(position / p.page_size);
-    slot = static_cast<int>(position - static_cast<int64_t>(at) * p.page_size);
-    page = p.table[s * p.table_stride + at];
-    if (page >= p.pages) page = -1;
-  }
-  for (int i = tid; i < a.pairs; i += kAppendThreads) {
-    const double turns = static_cast<double>(position) * a.frequencies[i] * 0.15915494309189533577;
-    float sn, cs;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-    turn[i] = make_float2(cs, sn);
-  }
-  __syncthreads();
 
+    // cosines and sines of the lane's pairs
+    float2 turn[PIECES][VEC];
+    auto angle = [&](int pair) {
+      const double part = static_cast<double>(place.position) * a.frequencies[pair] * 0.15915494309189533577;
+      float sn, cs;
+      sincospif(2.f * static_cast<float>(part - rint(part)), &sn, &cs);
+      return make_float2(cs, sn);
+    };
+    if constexpr (VEC == 1) {
 #pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    // (whole rows leave together, and a warp's shuffles below name its lanes: no break before them)
-    const int row = first_row + i * per_round;
-    const bool live = row < rows;
-    const int what = row < q_rows ? 0 : row < q_rows + p.kv_heads ? 1 : 2;
-    const int head = what == 0 ? row : row - q_rows - (what - 1) * p.kv_heads;
-    float u[PIECES][VEC], v[PIECES][VEC], top = 0.f;
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int unit = lane + k * 32;
-      int d, e;
-      piece<VEC>(unit, a.pairs, a.interleaved, &d, &e);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        u[k][j] = live && d < p.dim ? ElemTraits<T>::to_float(x[i][k].v[j]) : 0.f;
-        v[k][j] = live && e < p.dim ? ElemTraits<T>::to_float(y[i][k].v[j]) : 0.f;
-      }
-      if (what < 2 && unit * VEC < a.pairs) {
-        if (a.interleaved && VEC > 1) {
-          // the pairs are neighbours: VEC / 2 in each vector
-#pragma unroll
-          for (int j = 0; j < VEC / 2; ++j) {
-            const float2 c = turn[unit * VEC + j], f = turn[unit * VEC + VEC / 2 + j];
-            const float u0 = u[k][2 * j], u1 = u[k][2 * j + 1], v0 = v[k][2 * j], v1 = v[k][2 * j + 1];
-            u[k][2 * j] = u0 * c.x - u1 * c.y;
-            u[k][2 * j + 1] = u0 * c.y + u1 * c.x;
-            v[k][2 * j] = v0 * f.x - v1 * f.y;
-            v[k][2 * j + 1] = v0 * f.y + v1 * f.x;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float2 c = turn[unit * VEC + j];
-            const float u0 = u[k][j], v0 = v[k][j];
-            u[k][j] = u0 * c.x - v0 * c.y;
-            v[k][j] = u0 * c.y + v0 * c.x;
-          }
-        }
-      }
-      if (kEight) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) top = fmaxf(top, fmaxf(fabsf(u[k][j]), fabsf(v[k][j])));
-      }
-    }
-    float scale = 1.f;
-    if (kEight) {
-      for (int w = a.lanes / 2; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-      scale = fmaxf(top / 448.f, 1.1754943508e-38f);
-    }
-    if (!live || (what > 0 && page < 0)) continue;
-    char* to;
-    if (what == 0) {
-      to = a.q_out + sizeof(T) * (t * a.out_token + head * a.out_head);
+      for (int k = 0; k < PIECES; ++k) turn[k][0] = turned[k] ? angle(lane + k * 32) : make_float2(1.f, 0.f);
     } else {
-      to = p.data[what - 1] + sizeof(C) * (page * p.page[what - 1] + head * p.head[what - 1] + slot * p.token[what - 1]);
-      if (kEight && lane == 0)
-        p.scales[what - 1][page * p.spage[what - 1] + head * p.shead[what - 1] + slot * p.stoken[what - 1]] = scale;
-    }
+      // (each lane forms some; a lane's VEC pairs then are VEC / 2 vectors, and lanes side by side read vectors side by side)
+      __syncwarp();
+      for (int i = wl; i < a.pairs; i += 32) turns[warp][((i % VEC / 2) * a.lanes + i / VEC) * 2 + i % 2] = angle(i);
+      __syncwarp();
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      int d, e;
-      piece<VEC>(lane + k * 32, a.pairs, a.interleaved, &d, &e);
-      if (kEight && what > 0) {
-        Vec<uint8_t, VEC> first, second;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          first.v[j] = __nv_cvt_float_to_fp8(u[k][j] / scale, __NV_SATFINITE, __NV_E4M3);
-          second.v[j] = __nv_cvt_float_to_fp8(v[k][j] / scale, __NV_SATFINITE, __NV_E4M3);
-        }
-        if (d < p.dim) *reinterpret_cast<Vec<uint8_t, VEC>*>(to + d) = first;
-        if (e < p.dim) *reinterpret_cast<Vec<uint8_t, VEC>*>(to + e) = second;
-      } else {
-        Vec<T, VEC> first, second;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          first.v[j] = ElemTraits<T>::from_float(u[k][j]);
-          second.v[j] = ElemTraits<T>::from_float(v[k][j]);
-        }
-        if (d < p.dim) *reinterpret_cast<Vec<T, VEC>*>(to + d * sizeof(T)) = first;
-        if (e < p.dim) *reinterpret_cast<Vec<T, VEC>*>(to + e * sizeof(T)) = second;
+      for (int j = 0; j < VEC; j += 2) {
+        const float4 c = turned[0] ? reinterpret_cast<const float4*>(turns[warp])[j / 2 * a.lanes + lane] : make_float4(1.f, 0.f, 1.f, 0.f);
+        turn[0][j] = make_float2(c.x, c.y);
+        turn[0][j + 1] = make_float2(c.z, c.w);
       }
+    }
+
+    if (row0 < q_rows && !place.there && a.clear_rest) {
+      // rows of no sequence
+      T* to = reinterpret_cast<T*>(a.q_out) + this_t * a.out_token;
+      for (int i = row0 * p.dim + wl; i < min(end, q_rows) * p.dim; i += 32) to[i / p.dim * a.out_head + i % p.dim] = ElemTraits<T>::from_float(0.f);
+    }
+    // (one copy of the code for the three kinds: with three the registers go to addresses)
+#pragma unroll 1
+    for (int kind = 0; kind < 3; ++kind) {
+      const int kv = kind == 2, begin = kind == 0 ? 0 : q_rows + kv * p.kv_heads;
+      const int from = max(row0 - begin, 0), to = min(end - begin, kind == 0 ? q_rows : p.kv_heads);
+      if (from >= to || (kind == 0 ? !place.there : place.page < 0)) continue;
+      char* dst;
+      int64_t dst_head;
+      float* scales = nullptr;
+      if (kind == 0) {
+        dst = a.q_out + this_t * a.out_token * static_cast<int64_t>(sizeof(T));
+        dst_head = a.out_head;
+      } else {
+        dst = p.data[kv] + (place.page * p.page[kv] + place.slot * p.token[kv]) * static_cast<int64_t>(sizeof(C));
+        dst_head = p.head[kv];
+        if (kEight) scales = p.scales[kv] + place.page * p.spage[kv] + place.slot * p.stoken[kv];
+      }
+      move_rows<T, VEC, PIECES, kEight, INTER>(reinterpret_cast<const T*>(a.in[kind]) + this_t * a.token[kind], a.head[kind], dst, dst_head,
+                                               scales, p.shead[kv], from, to, p.dim, a.lanes, lane, nth, kind < 2, kind > 0, first, second,
+                                               turned, turn);
     }
   }
 }
@@ -279,22 +398,28 @@ bool whole(const void* p, int64_t x, int64_t y, int64_t z, int vec, int size) {
   return reinterpret_cast<uintptr_t>(p) % (vec * size) == 0 && x % vec == 0 && y % vec == 0 && z % vec == 0;
 }
 
-template <typename T, typename C, int VEC>
-int launch_append(const Append& a, cudaStream_t stream) {
-  const int rows = (a.in[0] ? a.heads : 0) + 2 * a.pool.kv_heads, per_block = kAppendThreads / a.lanes * kRounds;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.pool.tokens, (rows + per_block - 1) / per_block);
-  cfg.blockDim = dim3(kAppendThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = tc::pdl_enabled() ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, append_kernel<T, C, VEC>, a);
+template <typename T, typename C, int VEC, bool INTER>
+int launch_append(Append& a, cudaStream_t stream) {
+  int sms = tc::num_sms();
+  constexpr int kWarps = kAppendThreads / 32;
+  const int64_t blocks = (sms > 0 ? sms : 148) * 2;
+  const int rows = (a.in[0] ? a.heads : 0) + 2 * a.pool.kv_heads, rounds = (rows + 32 / a.lanes - 1) / (32 / a.lanes);
+  // (where the tokens are fewer than the warps that run at a time, a token is several warps': each forms its rotation again)
+  a.chunk_rows = (a.pool.tokens < blocks * kWarps ? kFlight : rounds) * (32 / a.lanes);
+  a.chunks = (rows + a.chunk_rows - 1) / a.chunk_rows;
+  const int64_t needed = (static_cast<int64_t>(a.pool.tokens) * a.chunks + kWarps - 1) / kWarps;
+  const cudaError_t err =
+      tc::launch_pdl(append_kernel<T, C, VEC, INTER>, static_cast<unsigned>(std::min(needed, blocks)), kAppendThreads, 0, stream, a);
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "cache append kernel: %s", cudaGetErrorString(err));
   count_launch();
   return KSMM_OK;
+}
+
+template <typename T, typename C>
+int launch_append_order(Append& a, bool vec, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (a.interleaved) return vec ? launch_append<T, C, VEC, true>(a, stream) : launch_append<T, C, 1, true>(a, stream);
+  return vec ? launch_append<T, C, VEC, false>(a, stream) : launch_append<T, C, 1, false>(a, stream);
 }
 
 template <typename T>
@@ -310,8 +435,8 @@ int launch_append_typed(Append& a, int cache_dtype, cudaStream_t stream) {
   const int per = vec ? VEC : 1, pieces = (p.dim + 2 * per - 1) / (2 * per);
   a.lanes = 1;
   while (a.lanes < pieces && a.lanes < 32) a.lanes *= 2;
-  if (eight) return vec ? launch_append<T, f8e4m3, VEC>(a, stream) : launch_append<T, f8e4m3, 1>(a, stream);
-  return vec ? launch_append<T, T, VEC>(a, stream) : launch_append<T, T, 1>(a, stream);
+  if (eight) return launch_append_order<T, f8e4m3>(a, vec, stream);
+  return launch_append_order<T, T>(a, vec, stream);
 }
 
 // Sequences of up to kFewRows rows (new tokens x heads of a group) are the token kernel's, in up to four tiles that read the keys

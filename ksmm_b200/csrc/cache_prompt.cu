@@ -300,7 +300,6 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     const int mine_count = t == 0 ? count[0] : count[C::kTiles - 1];
     const int sure = g.seq.length - g.seq.n + token0 + t * args.tile_tokens + 1;  // keys below are seen by all rows of the tile
     const int64_t clear = a.window ? static_cast<int64_t>(sure) - 1 + args.tile_tokens - a.window : 0;  // so are keys from here on
-    const int64_t oldest = a.window ? position - a.window + 1 : 0;
     const int boxes = C::kKeys / args.box;
     float top = kNone, sum = 0.f;
     bool alive = true;
@@ -324,12 +323,19 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
       tmem_ld_wait();
       const int key = (first + j) * C::kKeys;
       if (key + C::kKeys > sure || key < clear || key < g.lo || missing) {
+        if (missing) {
 #pragma unroll
-        for (int c = 0; c < C::kKeys; ++c) {
-          const int at = key + c;
-          if (missing && (missing >> (c / args.box) & 1)) s[c] = __int_as_float(0x7fffffff);
-          if (at > position || at < oldest || at >= g.hi) s[c] = -INFINITY;
+          for (int c = 0; c < C::kKeys; c += 16)
+            if (missing >> (c / args.box) & 1) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[c + e] = __int_as_float(0x7fffffff);
+            }
         }
+        const int64_t oldest = a.window ? position - a.window + 1 - key : 0;
+        const int to = min(position + 1, g.hi) - key, from = static_cast<int>(oldest < 0 ? 0 : oldest < C::kKeys ? oldest : C::kKeys);
+#pragma unroll
+        for (int c = 0; c < C::kKeys; ++c)
+          if (c >= to || c < from) s[c] = -INFINITY;
       }
       float high[4] = {top, s[0], s[1], s[2]};
 #pragma unroll
