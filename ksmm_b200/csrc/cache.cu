@@ -451,6 +451,7 @@ struct Plan {
   int tile;
   bool split;
   int most;               // rows of its sequences
+  int rows;               // of its items, at most
   size_t bytes, partial_bytes;
 };
 
@@ -462,9 +463,8 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   const ksmm_cache_t& c = d.cache;
   *p = {};
   const int64_t group = d.heads / c.kv_heads;
-  int64_t most = c.starts ? c.tokens : c.tokens / c.sequences;
-  if (d.max_new > 0 && d.max_new < most) most = d.max_new;
-  int64_t rows = most * group;
+  const int64_t sure = c.starts ? c.tokens : c.tokens / c.sequences;
+  int64_t rows = (d.max_new > 0 && d.max_new < sure ? d.max_new : sure) * group;
   p->most = INT_MAX;
   if (rows > kFewRows && prompt_fits(d)) {
     p->prompt_tile = prompt_rows(c.head_dim, static_cast<int>(group));
@@ -477,6 +477,7 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   p->token = token_fits(d);
   p->tile = p->token ? kTokenRows : rows_tile(c.head_dim);
   p->split = rows <= kFewRows;
+  p->rows = static_cast<int>(std::min<int64_t>(sure * group, p->tile));  // (max_new is the caller's word)
   if (!p->split) {
     const int64_t n = items(c, group, p->tile);
     if (n >= INT_MAX) return false;
@@ -591,7 +592,7 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
   a.most = plan.most;
   a.split = plan.split;
   st = plan.token ? launch_token(a, d->dtype, c.cache_dtype, plan.grid, s) : launch_rows(a, d->dtype, c.cache_dtype, plan.grid, s);
-  if (st == KSMM_OK && plan.split) st = launch_join(a, d->dtype, plan.grid, s);
+  if (st == KSMM_OK && plan.split) st = launch_join(a, d->dtype, plan.grid, plan.rows, s);
   return st;
 }
 

@@ -64,11 +64,10 @@ struct Attend {
   int* status;
 };
 
-// An item: up to tile_rows rows of one sequence and one key head.  They are numbered sequence by sequence, then head by head; in a
-// split launch each counts as its units of kUnit tokens.
+// An item: up to tile_rows rows of one sequence and one key head.  They are numbered sequence by sequence, then head by head.
 struct Work {
-  int units, tiles;  // of an item; items of a head
-  int64_t weight;    // of the sequence
+  int units, tiles;  // pieces of kUnit tokens of an item (of a split launch), items of a head
+  int64_t items;     // of the sequence
 };
 
 __device__ __forceinline__ int first_key(const Attend& a, const Sequence& q, int row_token) {
@@ -82,64 +81,17 @@ __device__ __forceinline__ Work work_of(const Attend& a, const Sequence& q) {
   const int64_t rows = static_cast<int64_t>(q.n) * a.group;
   if (rows < a.least || rows > a.most) {
     w.units = w.tiles = 0;
-    w.weight = 0;
+    w.items = 0;
     return w;
   }
   w.tiles = static_cast<int>((rows + a.tile_rows - 1) / a.tile_rows);
   // (a sequence without keys is a unit of work as well: its rows are zeros)
-  w.units = a.split ? max(1, (q.length + kUnit - 1) / kUnit - first_key(a, q, 0) / kUnit) : 1;
-  w.weight = static_cast<int64_t>(w.units) * w.tiles * a.pool.kv_heads;
+  w.units = max(1, (q.length + kUnit - 1) / kUnit - first_key(a, q, 0) / kUnit);
+  w.items = static_cast<int64_t>(w.tiles) * a.pool.kv_heads;
   return w;
 }
 
-// Finds the sequence that holds place `at(total)` of all sequences' weights.  Every thread of the block calls it; `shared` holds
-// 32 + 3 values.  Returns the total; *s and *offset are set to the sequence and the place in it (s = sequences if at >= total).
-// A thread sums a run of sequences, the block forms the runs' prefix sums, the run that holds the place is walked by its
-// thread: lengths and starts are read once, side by side.
-template <int THREADS, typename At>
-__device__ int64_t find_place(const Attend& a, int64_t* shared, At at, int* s, int64_t* offset) {
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int run = (a.pool.sequences + THREADS - 1) / THREADS;
-  const int from = min(tid * run, a.pool.sequences), to = min(from + run, a.pool.sequences);
-  int64_t sum = 0;
-  for (int i = from; i < to; ++i) sum += work_of(a, sequence(a.pool, i)).weight;
-  int64_t before = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before += v;
-  }
-  if (lane == 31) shared[warp] = before;
-  if (tid == 0) shared[33] = a.pool.sequences;
-  __syncthreads();
-  constexpr int kWarps = THREADS / 32;
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += shared[w];
-    total += shared[w];
-  }
-  const int64_t place = at(total);
-  before -= sum;
-  if (sum > 0 && place >= before && place < before + sum) {
-    for (int i = from; i < to; ++i) {
-      const int64_t w = work_of(a, sequence(a.pool, i)).weight;
-      if (place < before + w) {
-        shared[33] = i;
-        shared[34] = place - before;
-        break;
-      }
-      before += w;
-    }
-  }
-  __syncthreads();
-  *s = static_cast<int>(shared[33]);
-  *offset = shared[34];
-  __syncthreads();  // (the caller may use the array again)
-  return total;
-}
-
-// A block's share of a split launch, places [begin, end), as segments of items; without a split one item.
+// A piece of an item, from a block's share.
 struct Segment {
   Sequence seq;
   int s, head, tile;
@@ -150,27 +102,34 @@ struct Segment {
   int64_t item;        // its number, for the partial results
 };
 
+// A block's share: `left` units from unit `offset` of sequence s on, counted through its items; in a launch without a split, or of few
+// short sequences, one whole item.
 struct Share {
-  int64_t begin, end, done;
+  int64_t left, offset;
   int s;
-  int64_t offset;
+  bool whole;
   Work work;
   Sequence seq;
 
+  __device__ void set(const Attend& a, int which) {
+    s = which;
+    seq = sequence(a.pool, s);
+    work = work_of(a, seq);
+    if (whole) work.units = 1;  // (items count as one)
+  }
+
   // the next segment, by one thread or by all alike; false where there is none
   __device__ bool next(const Attend& a, Segment* g) {
-    if (done >= end) return false;
-    while (offset >= work.weight) {
-      offset -= work.weight;
-      if (++s >= a.pool.sequences) return false;  // (not reached: the places end with the last sequence's)
-      seq = sequence(a.pool, s);
-      work = work_of(a, seq);
+    if (left <= 0) return false;
+    while (offset >= work.items * work.units) {
+      offset -= work.items * work.units;
+      if (s + 1 >= a.pool.sequences) return false;  // (not reached: the units end with the last sequence's)
+      set(a, s + 1);
     }
     const int64_t item = offset / work.units;
     const int from = static_cast<int>(offset - item * work.units);
-    const int64_t left = end - done;
     const int to = static_cast<int>(left < work.units - from ? from + left : work.units);
-    done += to - from;
+    left -= to - from;
     offset += to - from;
     g->seq = seq;
     g->s = s;
@@ -190,7 +149,7 @@ struct Share {
     if (a.split) {
       // (all tiles of a sequence go through the same units, so that they count the same)
       g->from = g->lo / kUnit + from;
-      g->to = g->lo / kUnit + to;
+      g->to = whole ? max(g->from + 1, (seq.length + kUnit - 1) / kUnit) : g->lo / kUnit + to;
     } else {
       const int64_t t1 = (static_cast<int64_t>(g->tile + 1) * a.tile_rows - 1) / a.group;
       g->hi = max(seq.length - seq.n + static_cast<int>(t1 < seq.n ? t1 + 1 : seq.n), 0);
@@ -204,33 +163,89 @@ struct Share {
   }
 };
 
-// Every thread of the block: its share.  false: nothing to do (a split block then has marked its slots).
+// Every thread of the block: its share.  false: nothing to do (a split block then has marked its slots).  A thread sums a run of
+// sequences, the block forms the runs' prefix sums, and the run that holds the block's first unit is walked by its thread: lengths
+// and starts are read once, side by side.  `shared`: kShareWords values.
+constexpr int kShareWords = 3 * 32 + 2;
+constexpr int kWholeUnits = 8;  // items of up to so many units stay whole where there is a block for each: joining parts costs more
+
 template <int THREADS>
 __device__ bool share(const Attend& a, int64_t* shared, Share* r) {
-  int64_t place = 0, last = 0;
+  constexpr int kWarps = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int run = (a.pool.sequences + THREADS - 1) / THREADS;
+  const int from = min(tid * run, a.pool.sequences), to = min(from + run, a.pool.sequences);
+  int64_t units = 0, items = 0;
+  int most = 0;
+  for (int i = from; i < to; ++i) {
+    const Work w = work_of(a, sequence(a.pool, i));
+    units += w.items * w.units;
+    items += w.items;
+    most = max(most, w.units);
+  }
+  int64_t units_before = units, items_before = items;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, units_before, d), n = __shfl_up_sync(0xffffffffu, items_before, d);
+    if (lane >= d) {
+      units_before += u;
+      items_before += n;
+    }
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+  }
+  if (lane == 31) {
+    shared[warp] = units_before;
+    shared[32 + warp] = items_before;
+    shared[64 + warp] = most;
+  }
+  if (tid == 0) shared[96] = -1;
+  __syncthreads();
+  int64_t all_units = 0, all_items = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      units_before += shared[w];
+      items_before += shared[32 + w];
+    }
+    all_units += shared[w];
+    all_items += shared[32 + w];
+    most = max(most, static_cast<int>(shared[64 + w]));
+  }
   const int64_t block = blockIdx.x, blocks = gridDim.x;
-  int s;
-  int64_t offset;
-  find_place<THREADS>(
-      a, shared,
-      [&](int64_t total) {
-        // (with fewer units than blocks the first `total` blocks have one each)
-        const int64_t n = a.split ? (total < blocks ? total : blocks) : total;
-        place = !a.split ? block : block < n ? block * total / n : total;
-        last = !a.split ? (block < total ? block + 1 : block) : block < n ? (block + 1) * total / n : total;
-        return place;
-      },
-      &s, &offset);
-  if (place >= last || s >= a.pool.sequences) {
-    if (a.split && threadIdx.x < 2) a.slots[2 * block + threadIdx.x] = -1;
+  const bool whole = !a.split || (most <= kWholeUnits && all_items <= blocks);
+  int64_t place = block, last = block + 1, total = all_items, mine = items, before = items_before - items;
+  if (!whole) {
+    // (with fewer units than blocks the first all_units blocks have one each)
+    total = all_units;
+    mine = units;
+    before = units_before - units;
+    const int64_t n = min(total, blocks);
+    place = block < n ? block * total / n : total;
+    last = block < n ? (block + 1) * total / n : total;
+  }
+  if (place < last && place >= before && place < before + mine) {
+    for (int i = from; i < to; ++i) {
+      const Work w = work_of(a, sequence(a.pool, i));
+      const int64_t n = whole ? w.items : w.items * w.units;
+      if (place < before + n) {
+        shared[97] = place - before;
+        shared[96] = i;
+        break;
+      }
+      before += n;
+    }
+  }
+  __syncthreads();
+  const int s = static_cast<int>(shared[96]);
+  r->offset = shared[97];
+  __syncthreads();  // (the caller may use the array again)
+  if (s < 0) {
+    if (a.split && tid < 2) a.slots[2 * block + tid] = -1;
     return false;
   }
-  r->begin = r->done = place;
-  r->end = last;
-  r->s = s;
-  r->offset = offset;
-  r->seq = sequence(a.pool, s);
-  r->work = work_of(a, r->seq);
+  r->left = last - place;
+  r->whole = whole;
+  r->set(a, s);
   return true;
 }
 
@@ -251,7 +266,7 @@ __device__ void clear_rest(const Attend& a) {
 }
 
 // host side: each returns a status
-constexpr int kMaxBlocks = 1024;  // of a split launch (the join kernel's table of weights)
+constexpr int kMaxBlocks = 512;  // of a split launch (the join kernel's table of weights)
 int rows_tile(int dim);           // rows of an item in the CUDA-core kernel
 int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
 int token_blocks_per_sm(int cache_dtype, int dim);
@@ -261,7 +276,7 @@ int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cud
 int prompt_rows(int dim, int group);  // rows of an item in the prompt kernel
 bool prompt_fits(const ksmm_cache_attention_desc_t& d);
 int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
-int launch_join(const Attend& a, int dtype, unsigned blocks, cudaStream_t stream);
+int launch_join(const Attend& a, int dtype, unsigned blocks, int rows, cudaStream_t stream);  // rows: of an item, at most
 
 }  // namespace cache
 }  // namespace ksmm

@@ -38,7 +38,7 @@ struct Prompt {
   static constexpr int kBars = 1 + 4 * kStages + 3 * kTiles + 1;
   static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
   static constexpr int kSharedAt = kFlagsAt + 8;
-  static constexpr int kBytes = kSharedAt + 40 * 8;
+  static constexpr int kBytes = kSharedAt + kShareWords * 8;
   static constexpr int kThreads = 128 * kTiles + 64;
   static constexpr int kSCols = kKeys;
   static constexpr int kOAt = kTiles * kSCols;

@@ -53,7 +53,7 @@ template <typename T, typename C, int DPL, int VEC>
 __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_constant__ Attend a) {
   constexpr int R = 64 / DPL;
   constexpr bool kEight = sizeof(C) == 1;
-  __shared__ int64_t shared[40];
+  __shared__ int64_t shared[kShareWords];
   __shared__ float stats[2][kRowThreads / 32][R];
   extern __shared__ float sums[];  // [warp][R][8 DPL]
   tc::grid_dep_wait();
@@ -218,56 +218,91 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
   if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
 }
 
-// Joins the parts of items that several blocks shared.  Block (c, r): row r of the item that begins in block c and goes on;
-// its further parts are in slot 0 of the blocks after c, as long as they name the item.  In the order of the blocks, whoever was first.
-constexpr int kJoinThreads = 128;
+// Joins the parts of items that several blocks shared.  Block (c, r): row r of the item that begins in block c and goes on; its
+// further parts are in slot 0 of the blocks after c, as long as they name the item.  They are summed in the order of the blocks,
+// eight runs side by side, whoever was first.  A chain of reads is all the time that it takes: what may turn out not to be a
+// part (maxima and sums of the blocks after c) is read before that is known.
+constexpr int kJoinThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Attend a, int blocks) {
-  __shared__ float weight[1024 + kJoinThreads];
-  __shared__ float reduce[kJoinThreads / 32];
+  constexpr int kWarps = kJoinThreads / 32, kReads = kMaxBlocks / kJoinThreads;
+  __shared__ float weight[kMaxBlocks];
+  __shared__ float reduce[2][kWarps];
+  __shared__ float sums[kWarps][kMaxDim];
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   const Pool& p = a.pool;
-  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int64_t size = static_cast<int64_t>(a.tile_rows) * (p.dim + 2);
+  auto part = [&](int i) { return a.partial + (i == 0 ? 2 * c + 1 : 2 * static_cast<int64_t>(c + i)) * size; };
   const int64_t item = a.slots[2 * c + 1];
   if (item < 0) return;
+  int64_t named[kReads];
+  float m[kReads], l[kReads];
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) {
+    const int i = tid + k * kJoinThreads;
+    const bool there = c + i < blocks;
+    named[k] = !there ? -1 : i == 0 ? item : a.slots[2 * static_cast<int64_t>(c + i)];
+    m[k] = there ? part(i)[a.tile_rows * p.dim + r] : 0.f;
+    l[k] = there ? part(i)[a.tile_rows * (p.dim + 1) + r] : 0.f;
+  }
   const int s = static_cast<int>((item >> 32) / p.kv_heads), head = static_cast<int>((item >> 32) % p.kv_heads);
   const int tile = static_cast<int>(item & 0xffffffff);
   const Sequence q = sequence(p, s);
   if (tile * a.tile_rows + r >= q.n * a.group) return;
-  int parts = 1;
-  for (int from = c + 1; from < blocks; from += kJoinThreads) {
-    const int i = from + tid;
-    const int n = __syncthreads_count(i < blocks && a.slots[2 * static_cast<int64_t>(i)] == item);
-    parts += n;
-    if (n < kJoinThreads) break;
-  }
-  const int64_t size = static_cast<int64_t>(a.tile_rows) * (p.dim + 2);
-  auto part = [&](int i) { return a.partial + (i == 0 ? 2 * c + 1 : 2 * static_cast<int64_t>(c + i)) * size; };
+  int parts = 0;
   float top = kNone;
-  for (int i = tid; i < parts; i += kJoinThreads) {
-    weight[i] = part(i)[a.tile_rows * p.dim + r];
-    top = fmaxf(top, weight[i]);
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) {
+    // (an item's blocks follow one another)
+    parts += __syncthreads_count(named[k] == item);
+    if (named[k] == item) top = fmaxf(top, m[k]);
   }
 #pragma unroll
   for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  if (tid % 32 == 0) reduce[tid / 32] = top;
+  if (lane == 0) reduce[0][warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, reduce[w]);
-  for (int i = tid; i < parts; i += kJoinThreads) weight[i] = exp2f(weight[i] - top);
-  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, reduce[0][w]);
   float total = 0.f;
-  for (int i = 0; i < parts; ++i) total = fmaf(weight[i], part(i)[a.tile_rows * (p.dim + 1) + r], total);
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) {
+    if (named[k] != item) continue;
+    const float f = exp2f(m[k] - top);
+    weight[tid + k * kJoinThreads] = f;
+    total = fmaf(f, l[k], total);
+  }
+#pragma unroll
+  for (int x = 16; x; x /= 2) total += __shfl_xor_sync(0xffffffffu, total, x);
+  if (lane == 0) reduce[1][warp] = total;
+  __syncthreads();
+  total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) total += reduce[1][w];
+  constexpr int kPer = kMaxDim / 32;
+  float sum[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) sum[k] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < parts; i += kWarps) {
+    const float* from = part(i) + r * p.dim + lane;
+    const float f = weight[i];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (lane + 32 * k < p.dim) sum[k] = fmaf(f, from[32 * k], sum[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) sums[warp][lane + 32 * k] = sum[k];
+  __syncthreads();
   const int row = tile * a.tile_rows + r, t = row / a.group;
   T* out = reinterpret_cast<T*>(a.out) + (q.start + t) * a.out_token + (head * a.group + row - t * a.group) * a.out_head;
-  for (int d = tid; d < p.dim; d += kJoinThreads) {
-    float sum = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) sum = fmaf(weight[i], part(i)[r * p.dim + d], sum);
-    out[d] = ElemTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
-  }
+  if (tid >= p.dim) return;
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) all += sums[w][tid];
+  out[tid] = ElemTraits<T>::from_float(total == 0.f ? 0.f : all / total);
 }
 
 template <typename T, typename C, int DPL, int VEC>
@@ -317,9 +352,9 @@ int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cuda
 }
 
 template <typename T>
-static int launch_join_typed(const Attend& a, unsigned blocks, cudaStream_t stream) {
+static int launch_join_typed(const Attend& a, unsigned blocks, int rows, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks, a.tile_rows);
+  cfg.gridDim = dim3(blocks, rows);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
@@ -333,10 +368,10 @@ static int launch_join_typed(const Attend& a, unsigned blocks, cudaStream_t stre
   return KSMM_OK;
 }
 
-int launch_join(const Attend& a, int dtype, unsigned blocks, cudaStream_t stream) {
-  if (dtype == KSMM_F32) return launch_join_typed<float>(a, blocks, stream);
-  if (dtype == KSMM_F16) return launch_join_typed<__half>(a, blocks, stream);
-  return launch_join_typed<__nv_bfloat16>(a, blocks, stream);
+int launch_join(const Attend& a, int dtype, unsigned blocks, int rows, cudaStream_t stream) {
+  if (dtype == KSMM_F32) return launch_join_typed<float>(a, blocks, rows, stream);
+  if (dtype == KSMM_F16) return launch_join_typed<__half>(a, blocks, rows, stream);
+  return launch_join_typed<__nv_bfloat16>(a, blocks, rows, stream);
 }
 
 }  // namespace cache

@@ -367,6 +367,21 @@ def test_two_streams_graphs_and_repeats(dtype):
     kb.check_device()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sequences,length", [(1, 1), (1, 512), (1, 513), (2, 4000), (700, 130), (1500, 3)])
+def test_few_and_many_sequences(sequences, length, dtype):
+    """Whole items, items cut into parts, more sequences than a block has threads; bounds of max_new that do not hold."""
+    gen = torch.Generator().manual_seed(sequences + length)
+    lengths = [length - s % 2 * (length // 3) for s in range(sequences)]
+    cache, table, L, _, q, _, _ = make(gen, lengths, [1] * sequences, 4, 2, 64, 16, dtype)
+    check(kb.cache_attention(q, cache, table, L), attended(q, cache, table, lengths, [1] * sequences), cache)
+    if sequences <= 2 and length > 600:
+        new = [9, 70][:sequences]
+        cache, table, L, starts, q, _, _ = make(gen, lengths, new, 4, 2, 64, 16, dtype)
+        for bound in (1, 3, None):
+            check(kb.cache_attention(q, cache, table, L, starts=starts, max_new=bound), attended(q, cache, table, lengths, new), cache)
+
+
 def test_empty_calls():
     cache = kb.KVCache(2, 16, 2, 64)
     empty = torch.zeros(0, 2, 64, dtype=torch.float16, device=DEV)
