@@ -449,7 +449,8 @@ struct Plan {
   bool token;             // the other kernel: the token kernel or the CUDA cores'
   unsigned grid;          // its blocks; 0: none
   int tile;
-  bool split;
+  int unit;
+  bool split, narrow;
   int most;               // rows of its sequences
   int rows;               // of its items, at most
   size_t bytes, partial_bytes;
@@ -475,6 +476,8 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
     rows = p->most = kFewRows;
   }
   p->token = token_fits(d);
+  const TokenShape shape = p->token ? token_shape(c.cache_dtype, c.head_dim) : TokenShape{1, kRowsUnit};
+  p->unit = shape.unit;
   p->tile = p->token ? kTokenRows : rows_tile(c.head_dim);
   p->split = rows <= kFewRows;
   p->rows = static_cast<int>(std::min<int64_t>(sure * group, p->tile));  // (max_new is the caller's word)
@@ -487,9 +490,11 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   int sms = tc::num_sms();
   if (sms <= 0) sms = 148;
   // (no more than there can be units)
-  const double units = static_cast<double>(static_cast<int64_t>(c.table_width) * c.page_size / kUnit + 2) *
+  const double units = static_cast<double>(static_cast<int64_t>(c.table_width) * c.page_size / p->unit + 2) *
                        static_cast<double>((rows + p->tile - 1) / p->tile) * c.kv_heads * static_cast<double>(c.sequences);
-  int limit = sms * (p->token ? token_blocks_per_sm(c.cache_dtype, c.head_dim) : 1);
+  // (rows are max_new's word; all tiles that there can be)
+  p->narrow = units / static_cast<double>((rows + p->tile - 1) / p->tile) * static_cast<double>(sure * group / p->tile + 1) < 2e9;
+  int limit = sms * shape.blocks;
   limit = limit < kMaxBlocks ? limit : kMaxBlocks;
   p->grid = units < limit ? static_cast<unsigned>(units) : static_cast<unsigned>(limit);
   p->partial_bytes = (2 * sizeof(float) * p->grid * p->tile * (c.head_dim + 2) + 255) / 256 * 256;
@@ -580,6 +585,8 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.prompt) {
     a.tile_rows = plan.prompt_tile;
+    a.unit_log2 = 0;  // (its items are whole; their number is the grid's)
+    a.narrow = 1;
     a.least = plan.grid ? plan.most + 1 : 1;
     a.most = INT_MAX;
     a.split = 0;
@@ -588,6 +595,8 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
     a.clear_rest = 0;
   }
   a.tile_rows = plan.tile;
+  a.unit_log2 = 31 - __builtin_clz(plan.unit);
+  a.narrow = plan.narrow || !plan.split;
   a.least = 1;
   a.most = plan.most;
   a.split = plan.split;

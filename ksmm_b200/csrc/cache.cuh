@@ -7,7 +7,6 @@ namespace ksmm {
 namespace cache {
 
 constexpr int kWaits = 110;      // codes of this family's bounded waits: 110 to 119
-constexpr int kUnit = 64;        // tokens of a unit, the piece in which a cache's length is split
 constexpr int kMaxDim = 256;
 constexpr float kNone = -3.402823466e38f;  // a running maximum before the first key: differences of two are 0, not NaN
 
@@ -57,6 +56,8 @@ struct Attend {
   float scale;          // of the scores, times log2(e)
   int clear_rest;
   int tile_rows;        // rows (token, head of the group) of an item
+  int unit_log2;        // of the tokens of a unit, the piece in which a cache's length is split
+  int narrow;           // all sequences' units fit 31 bits
   int least, most;      // sequences with fewer or more rows in a group are another kernel's
   int split;            // an item's units may be several CTAs'
   float* partial;       // split: 2 slots per CTA of tile_rows * (dim + 2) floats
@@ -66,7 +67,7 @@ struct Attend {
 
 // An item: up to tile_rows rows of one sequence and one key head.  They are numbered sequence by sequence, then head by head.
 struct Work {
-  int units, tiles;  // pieces of kUnit tokens of an item (of a split launch), items of a head
+  int units, tiles;  // units of an item (of a split launch), items of a head
   int64_t items;     // of the sequence
 };
 
@@ -74,6 +75,15 @@ __device__ __forceinline__ int first_key(const Attend& a, const Sequence& q, int
   if (!a.window) return 0;
   const int64_t lo = static_cast<int64_t>(q.length) - q.n + row_token - a.window + 1;
   return static_cast<int>(lo < 0 ? 0 : lo);
+}
+
+// units up to a token; a length is at most 2^31 - 65537
+__device__ __forceinline__ int units_to(const Attend& a, int length) { return (length + (1 << a.unit_log2) - 1) >> a.unit_log2; }
+
+// (a division in 64 bits takes several hundred cycles, and a block's start is a chain of them)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 
 __device__ __forceinline__ Work work_of(const Attend& a, const Sequence& q) {
@@ -86,7 +96,7 @@ __device__ __forceinline__ Work work_of(const Attend& a, const Sequence& q) {
   }
   w.tiles = static_cast<int>((rows + a.tile_rows - 1) / a.tile_rows);
   // (a sequence without keys is a unit of work as well: its rows are zeros)
-  w.units = max(1, (q.length + kUnit - 1) / kUnit - first_key(a, q, 0) / kUnit);
+  w.units = max(1, units_to(a, q.length) - (first_key(a, q, 0) >> a.unit_log2));
   w.items = static_cast<int64_t>(w.tiles) * a.pool.kv_heads;
   return w;
 }
@@ -126,7 +136,7 @@ struct Share {
       if (s + 1 >= a.pool.sequences) return false;  // (not reached: the units end with the last sequence's)
       set(a, s + 1);
     }
-    const int64_t item = offset / work.units;
+    const int64_t item = divide(offset, work.units);
     const int from = static_cast<int>(offset - item * work.units);
     const int to = static_cast<int>(left < work.units - from ? from + left : work.units);
     left -= to - from;
@@ -134,27 +144,27 @@ struct Share {
     g->seq = seq;
     g->s = s;
     if (a.split) {
-      g->head = static_cast<int>(item / work.tiles);
+      g->head = static_cast<int>(divide(item, work.tiles));
       g->tile = static_cast<int>(item - static_cast<int64_t>(g->head) * work.tiles);
     } else {
       // the last tiles of all heads come first: they see the most keys
-      const int64_t tile = item / a.pool.kv_heads;
+      const int64_t tile = divide(item, a.pool.kv_heads);
       g->head = static_cast<int>(item - tile * a.pool.kv_heads);
       g->tile = work.tiles - 1 - static_cast<int>(tile);
     }
-    const int t0 = static_cast<int>(static_cast<int64_t>(g->tile) * a.tile_rows / a.group);
+    const int t0 = static_cast<int>(divide(static_cast<int64_t>(g->tile) * a.tile_rows, a.group));
     g->first_position = seq.length - seq.n + t0;
     g->lo = first_key(a, seq, a.split ? 0 : t0);
     g->hi = seq.length;
     if (a.split) {
       // (all tiles of a sequence go through the same units, so that they count the same)
-      g->from = g->lo / kUnit + from;
-      g->to = whole ? max(g->from + 1, (seq.length + kUnit - 1) / kUnit) : g->lo / kUnit + to;
+      g->from = (g->lo >> a.unit_log2) + from;
+      g->to = whole ? max(g->from + 1, units_to(a, seq.length)) : (g->lo >> a.unit_log2) + to;
     } else {
-      const int64_t t1 = (static_cast<int64_t>(g->tile + 1) * a.tile_rows - 1) / a.group;
+      const int64_t t1 = divide(static_cast<int64_t>(g->tile + 1) * a.tile_rows - 1, a.group);
       g->hi = max(seq.length - seq.n + static_cast<int>(t1 < seq.n ? t1 + 1 : seq.n), 0);
-      g->from = g->lo / kUnit;
-      g->to = (g->hi + kUnit - 1) / kUnit;
+      g->from = (g->lo >> a.unit_log2);
+      g->to = units_to(a, g->hi);
     }
     // a block's first segment may continue an item, its last may be continued; one that is both is the first
     g->slot = from == 0 && to == work.units ? 0 : from > 0 ? 1 : 2;
@@ -169,24 +179,24 @@ struct Share {
 constexpr int kShareWords = 3 * 32 + 2;
 constexpr int kWholeUnits = 8;  // items of up to so many units stay whole where there is a block for each: joining parts costs more
 
-template <int THREADS>
-__device__ bool share(const Attend& a, int64_t* shared, Share* r) {
+template <int THREADS, typename Count>
+__device__ bool share_counted(const Attend& a, int64_t* shared, Share* r) {
   constexpr int kWarps = THREADS / 32;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int run = (a.pool.sequences + THREADS - 1) / THREADS;
   const int from = min(tid * run, a.pool.sequences), to = min(from + run, a.pool.sequences);
-  int64_t units = 0, items = 0;
+  Count units = 0, items = 0;
   int most = 0;
   for (int i = from; i < to; ++i) {
     const Work w = work_of(a, sequence(a.pool, i));
-    units += w.items * w.units;
-    items += w.items;
+    units += static_cast<Count>(w.items) * w.units;
+    items += static_cast<Count>(w.items);
     most = max(most, w.units);
   }
-  int64_t units_before = units, items_before = items;
+  Count units_before = units, items_before = items;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, units_before, d), n = __shfl_up_sync(0xffffffffu, items_before, d);
+    const Count u = __shfl_up_sync(0xffffffffu, units_before, d), n = __shfl_up_sync(0xffffffffu, items_before, d);
     if (lane >= d) {
       units_before += u;
       items_before += n;
@@ -204,8 +214,8 @@ __device__ bool share(const Attend& a, int64_t* shared, Share* r) {
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) {
-      units_before += shared[w];
-      items_before += shared[32 + w];
+      units_before += static_cast<Count>(shared[w]);
+      items_before += static_cast<Count>(shared[32 + w]);
     }
     all_units += shared[w];
     all_items += shared[32 + w];
@@ -220,8 +230,8 @@ __device__ bool share(const Attend& a, int64_t* shared, Share* r) {
     mine = units;
     before = units_before - units;
     const int64_t n = min(total, blocks);
-    place = block < n ? block * total / n : total;
-    last = block < n ? (block + 1) * total / n : total;
+    place = block < n ? divide(block * total, n) : total;
+    last = block < n ? divide((block + 1) * total, n) : total;
   }
   if (place < last && place >= before && place < before + mine) {
     for (int i = from; i < to; ++i) {
@@ -249,6 +259,11 @@ __device__ bool share(const Attend& a, int64_t* shared, Share* r) {
   return true;
 }
 
+template <int THREADS>
+__device__ __forceinline__ bool share(const Attend& a, int64_t* shared, Share* r) {
+  return a.narrow ? share_counted<THREADS, int>(a, shared, r) : share_counted<THREADS, int64_t>(a, shared, r);
+}
+
 // Rows of no sequence, as asked for.
 template <typename T>
 __device__ void clear_rest(const Attend& a) {
@@ -267,9 +282,13 @@ __device__ void clear_rest(const Attend& a) {
 
 // host side: each returns a status
 constexpr int kMaxBlocks = 512;  // of a split launch (the join kernel's table of weights)
-int rows_tile(int dim);           // rows of an item in the CUDA-core kernel
+constexpr int kRowsUnit = 64;     // tokens of a unit in the CUDA-core kernel
+int rows_tile(int dim);           // rows of an item there
 int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
-int token_blocks_per_sm(int cache_dtype, int dim);
+struct TokenShape {
+  int blocks, unit;  // blocks on an SM, tokens of a unit
+};
+TokenShape token_shape(int cache_dtype, int dim);
 constexpr int kTokenRows = 16;    // rows of an item in the 16- and 8-bit kernel
 bool token_fits(const ksmm_cache_attention_desc_t& d);
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       bool there[2], bad[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        j[h] = unit * kUnit + h * 32 + at;
+        j[h] = unit * kRowsUnit + h * 32 + at;
         there[h] = j[h] >= g.lo && j[h] < g.hi;
         bad[h] = false;
         int64_t page = 0;

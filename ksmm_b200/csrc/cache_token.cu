@@ -37,9 +37,13 @@ constexpr int kTileRows = kTokenRows;
 
 template <bool EIGHT, int DP>
 struct Layout {
+  // Tokens of a warp's step.  A step is a chain (load, products, maximum, exponentials, products) of 1000 to 1500 cycles
+  // however many tokens it has, and an SM's eight warps have to pass 23 bytes a cycle: small rows take 32 tokens at a time.
+  static constexpr int kStep = DP == 256 || (!EIGHT && DP == 128) ? 16 : 32;
+  static constexpr int kTokens = kConsumers * kStep;                    // a unit, a stage of the ring
   static constexpr int kBoxes = EIGHT ? (DP + 127) / 128 : DP / 64;     // 128-byte columns of a row
-  static constexpr int kOperand = kBoxes * kUnit * 128;                 // a unit's keys
-  static constexpr int kScales = EIGHT ? 2 * kUnit * 4 : 0;
+  static constexpr int kOperand = kBoxes * kTokens * 128;               // a unit's keys
+  static constexpr int kScales = EIGHT ? 2 * kTokens * 4 : 0;
   static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kBlocks = DP == 256 ? 1 : 2;                     // on an SM
   static constexpr int kStages = 196608 / kBlocks / (kStageBytes + kScales);
@@ -51,6 +55,7 @@ struct Layout {
   static constexpr int kFlagsAt = kBarsAt + 2 * kStages * 8;
   static constexpr int kBytes = kFlagsAt + kStages * 4 + 4;
   static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
+  static_assert(kStages >= 2, "a ring");
 };
 
 struct Maps {
@@ -109,12 +114,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
-// T: q and the output.  Tokens of a page that one TMA box covers: `box`.
+// A place in the ring.
+template <int STAGES>
+struct Turn {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// T: q and the output.  Tokens of a page that one TMA box covers: 2^box_log2; a box lies in its stage as [128-byte column][token].
+// `joined`: a map with the columns as a dimension of their own brings all of a box's at once.
 template <typename T, bool EIGHT, int DP>
 __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
-    token_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Attend a, const int box) {
+    token_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Attend a, const int box_log2, const int joined) {
   using L = Layout<EIGHT, DP>;
   using H = typename std::conditional<EIGHT, __half, T>::type;  // of the products
+  // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
+  constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
+  constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
   extern __shared__ __align__(1024) char smem[];
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -143,63 +165,73 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
   Share mine;
   if (!share<kTokenThreads>(a, reinterpret_cast<int64_t*>(smem + L::kMergeAt), &mine)) return;
   const Pool& p = a.pool;
-  uint32_t n = 0;  // units so far
+  const int box = 1 << box_log2, box_bytes = box * 128;
+  Turn<L::kStages> turn;
   Segment g;
 
   if (warp == kConsumers) {
-    // ---------------- producer: a lane for each box of a unit, tables 32 boxes ahead ----------------
-    const int boxes = kUnit / box;
-    const uint32_t bytes = static_cast<uint32_t>(box) * 128 * L::kBoxes * 2 + (EIGHT ? 2 * box * 4 : 0);
+    // ---------------- producer: the warp walks the loop, tables 32 boxes ahead, one lane issues ----------------
+    const int boxes = L::kTokens >> box_log2;
+    const uint32_t bytes = static_cast<uint32_t>(box_bytes) * L::kBoxes * 2 + (EIGHT ? 2 * box * 4 : 0);
+    const bool one = elect_one();
+    uint32_t issued = 0;
     bool alive = true;
     while (alive && mine.next(a, &g)) {
       const int32_t* table = p.table + g.s * p.table_stride;
-      int ahead = 0, page_ahead = -1;
-      for (int u = g.from; u < g.to; ++u, ++n) {
-        const int in_batch = (u - g.from) % (32 / boxes);
-        if (in_batch == 0) {
+      int row_ahead = 0, page_ahead = -1, batch = 0;
+      for (int u = g.from; u < g.to; ++u) {
+        if (batch == 0) {
           // the pages of the next 32 boxes
-          const int token = u * kUnit + lane * box;
-          ahead = token / p.page_size;
+          const int token = u * L::kTokens + (lane << box_log2), nth = token / p.page_size;
           const bool there = token < g.hi && token + box > g.lo;
-          page_ahead = there ? table[ahead] : -2;  // -2: nothing to load, -1: a page that is not there
+          page_ahead = there ? table[nth] : -2;  // -2: nothing to load, -1: a page that is not there
           if (there && (page_ahead < 0 || page_ahead >= p.pages)) page_ahead = -1;
-          ahead = token - ahead * p.page_size;
+          row_ahead = token - nth * p.page_size;
         }
-        const int from = in_batch * boxes + lane;
-        const int page = __shfl_sync(0xffffffffu, page_ahead, from & 31), row = __shfl_sync(0xffffffffu, ahead, from & 31);
-        const bool get = lane < boxes && page >= 0;
-        const uint32_t missing = __ballot_sync(0xffffffffu, lane < boxes && page == -1);
-        const uint32_t load = __popc(__ballot_sync(0xffffffffu, get));
-        const int st = n % L::kStages;
-        alive = __all_sync(0xffffffffu, mbar_wait<0>(empty + 8 * st, (n / L::kStages & 1) ^ 1, abort_flag, a.status, kWaits));
+        const bool of_unit = lane >= batch && lane < batch + boxes;
+        const uint32_t missing = __ballot_sync(0xffffffffu, of_unit && page_ahead == -1) >> batch;
+        const uint32_t load = __ballot_sync(0xffffffffu, of_unit && page_ahead >= 0) >> batch;
+        const int st = turn.stage;
+        alive = __all_sync(0xffffffffu, mbar_wait<0>(empty + 8 * st, turn.parity ^ 1, abort_flag, a.status, kWaits));
         if (!alive) break;
-        if (lane == 0) {
+        const uint32_t bar = full + 8 * st;
+        if (one) {
           flags[st] = static_cast<int>(missing);
-          if (load) mbar_expect_tx(full + 8 * st, load * bytes);
-          else mbar_arrive(full + 8 * st);
+          if (load) mbar_expect_tx(bar, __popc(load) * bytes);
+          else mbar_arrive(bar);
         }
-        __syncwarp();
-        if (get) {
-          const uint32_t to = base + st * L::kStageBytes + lane * box * 128;
+        // (same values in all lanes: addresses in uniform registers.  A lane for each box took 170 cycles per copy)
+        for (int b = 0; b < boxes; ++b) {
+          const int page = __shfl_sync(0xffffffffu, page_ahead, batch + b), row = __shfl_sync(0xffffffffu, row_ahead, batch + b);
+          if (page < 0 || !one) continue;
+          const uint32_t to = base + st * L::kStageBytes + b * box_bytes * L::kBoxes;
+          if (joined) {
+            tma_load_5d(to, &maps.keys, bar, 0, row, 0, g.head, page);
+            tma_load_5d(to + L::kOperand, &maps.values, bar, 0, row, 0, g.head, page);
+          } else {
 #pragma unroll
-          for (int b = 0; b < L::kBoxes; ++b) {
-            const int x = b * (EIGHT ? 128 : 64);
-            tma_load_4d(to + b * kUnit * 128, &maps.keys, full + 8 * st, x, row, g.head, page);
-            tma_load_4d(to + L::kOperand + b * kUnit * 128, &maps.values, full + 8 * st, x, row, g.head, page);
+            for (int k = 0; k < L::kBoxes; ++k) {
+              tma_load_4d(to + k * box_bytes, &maps.keys, bar, k * (EIGHT ? 128 : 64), row, g.head, page);
+              tma_load_4d(to + L::kOperand + k * box_bytes, &maps.values, bar, k * (EIGHT ? 128 : 64), row, g.head, page);
+            }
           }
           if (EIGHT) {
-            const uint32_t at = base + L::kScalesAt + st * L::kScales + lane * box * 4;
-            bulk_load(at, p.scales[0] + page * p.spage[0] + g.head * p.shead[0] + row, box * 4, full + 8 * st);
-            bulk_load(at + kUnit * 4, p.scales[1] + page * p.spage[1] + g.head * p.shead[1] + row, box * 4, full + 8 * st);
+            const uint32_t at = base + L::kScalesAt + st * L::kScales + b * box * 4;
+            bulk_load(at, p.scales[0] + page * p.spage[0] + g.head * p.shead[0] + row, box * 4, bar);
+            bulk_load(at + L::kTokens * 4, p.scales[1] + page * p.spage[1] + g.head * p.shead[1] + row, box * 4, bar);
           }
         }
         __syncwarp();
+        ++issued;
+        turn.next();
+        batch += boxes;
+        if (batch == 32) batch = 0;
       }
     }
     if (!alive) {
       // the copies in flight end before the block does
       int zero = 0;
-      for (uint32_t i = n > L::kStages ? n - L::kStages : 0; i < n; ++i)
+      for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; ++i)
         mbar_wait<100>(full + 8 * (i % L::kStages), i / L::kStages & 1, &zero, a.status, kWaits + 1);
     }
     return;
@@ -213,8 +245,15 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
   float* stats = reinterpret_cast<float*>(smem + L::kStatsAt);
   // lane's row and chunk in the loads of four matrices: K: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1;
   // V: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1
-  const int k_row = warp * 16 + (lane / 16) * 8 + lane % 8, k_chunk = lane / 8 % 2;
-  const int v_row = warp * 16 + (lane / 8 % 2) * 8 + lane % 8, v_chunk = lane / 16;
+  const int k_row = (lane / 16) * 8 + lane % 8, k_chunk = lane / 8 % 2;
+  const int v_row = (lane / 8 % 2) * 8 + lane % 8, v_chunk = lane / 16;
+  // where the groups of 16 tokens lie in a stage
+  uint32_t group_at[G];
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    const int t = warp * L::kStep + i * 16, b = t >> box_log2;
+    group_at[i] = b * box_bytes * L::kBoxes + (t - (b << box_log2)) * 128;
+  }
   while (mine.next(a, &g)) {
     const int rows = min(kTileRows, g.seq.n * a.group - g.tile * kTileRows);
     uint32_t qf[DP / 16][4];
@@ -271,86 +310,92 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
     const int sure = g.first_position + 1;
     const int64_t clear = a.window ? static_cast<int64_t>(g.hi) - a.window : 0;
 #pragma unroll 1
-    for (int u = g.from; u < g.to; ++u, ++n) {
-      const int st = n % L::kStages;
-      alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(full + 8 * st, n / L::kStages & 1, abort_flag, a.status, kWaits + 2));
-      const int token = u * kUnit + warp * 16;  // the warp's first
-      if (alive && token < g.hi && token + 16 > g.lo) {
+    for (int u = g.from; u < g.to; ++u) {
+      const int st = turn.stage;
+      alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(full + 8 * st, turn.parity, abort_flag, a.status, kWaits + 2));
+      const int token = u * L::kTokens + warp * L::kStep;  // the warp's first
+      if (alive && token < g.hi && token + L::kStep > g.lo) {
         const uint32_t ks = base + st * L::kStageBytes, vs = ks + L::kOperand;
-        const bool missing = flags[st] >> (warp * 16 / box) & 1;
+        const int missing = flags[st];
         // ---- scores ----
-        float s[2][4];
+        float s[2 * G][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
         if constexpr (!EIGHT) {
 #pragma unroll
-          for (int c = 0; c < DP / 16; ++c) {
-            uint32_t b[4];
-            ldmatrix4(b, ks + c / 4 * (kUnit * 128) + k_row * 128 + (((c % 4 * 2 + k_chunk) ^ (k_row & 7)) << 4));
-            mma<H>(s[0], qf[c], b[0], b[1]);
-            mma<H>(s[1], qf[c], b[2], b[3]);
-          }
+          for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+              uint32_t b[4];
+              ldmatrix4(b, ks + group_at[i] + c / 4 * box_bytes + k_row * 128 + (((c % 4 * 2 + k_chunk) ^ (k_row & 7)) << 4));
+              mma<H>(s[2 * i], qf[c], b[0], b[1]);
+              mma<H>(s[2 * i + 1], qf[c], b[2], b[3]);
+            }
         } else {
 #pragma unroll
-          for (int c = 0; c < DP / 16; c += 2) {
-            uint32_t b[4];
-            ldmatrix4(b, ks + c / 8 * (kUnit * 128) + k_row * 128 + (((c % 8 + k_chunk) ^ (k_row & 7)) << 4));
+          for (int c = 0; c < DP / 16; c += 2)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              mma<H>(s[0], qf[c + e], e4m3_to_half2(b[e]), e4m3_to_half2(b[e] >> 16));
-              mma<H>(s[1], qf[c + e], e4m3_to_half2(b[2 + e]), e4m3_to_half2(b[2 + e] >> 16));
+            for (int i = 0; i < G; ++i) {
+              uint32_t b[4];
+              ldmatrix4(b, ks + group_at[i] + c / 8 * box_bytes + k_row * 128 + (((c % 8 + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                mma<H>(s[2 * i], qf[c + e], e4m3_to_half2(b[e]), e4m3_to_half2(b[e] >> 16));
+                mma<H>(s[2 * i + 1], qf[c + e], e4m3_to_half2(b[2 + e]), e4m3_to_half2(b[2 + e] >> 16));
+              }
             }
-          }
         }
-        float value_scale[2][2];
+        float value_scale[2 * G][2];
         if constexpr (EIGHT) {
-          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + warp * 16 + 2 * q4;
-          float key_scale[2][2];
+          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + warp * L::kStep + 2 * q4;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * i), v2 = *reinterpret_cast<const float2*>(sc + kUnit + 8 * i);
-            key_scale[i][0] = k2.x;
-            key_scale[i][1] = k2.y;
+          for (int i = 0; i < 2 * G; ++i) {
+            const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * i), v2 = *reinterpret_cast<const float2*>(sc + L::kTokens + 8 * i);
             value_scale[i][0] = v2.x;
             value_scale[i][1] = v2.y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2] * key_scale[i][e % 2];
+            for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2] * (e % 2 ? k2.y : k2.x);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2];
         }
-        const bool edge = token + 16 > sure || token < clear || token < g.lo || missing;
-        bool kept[2][2];  // whether the lane's tokens are the sequence's and there
+        const bool edge = token + L::kStep > sure || token < clear || token < g.lo || missing;
+        uint32_t keep[2 * G];  // 16-bit pairs of the lane's tokens: whether they are the sequence's and there
         if (edge) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2 * G; ++i) {
+            keep[i] = 0;
+            const bool gone = missing >> ((warp * L::kStep + i * 8) >> box_log2) & 1;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = token + 8 * i + 2 * q4 + e % 2;
               const bool in = j < g.hi && j >= g.lo;
-              kept[i][e % 2] = in && !missing;
+              if (in && !gone) keep[i] |= e % 2 ? 0xffff0000u : 0xffffu;
               const bool sees = in && j <= position[e / 2] && (!a.window || j > position[e / 2] - a.window);
-              s[i][e] = sees ? (missing ? __int_as_float(0x7fffffff) : s[i][e]) : -INFINITY;
-              if (EIGHT && !kept[i][e % 2]) value_scale[i][e % 2] = 0.f;
+              s[i][e] = sees ? (gone ? __int_as_float(0x7fffffff) : s[i][e]) : -INFINITY;
+              if (EIGHT && !(in && !gone)) value_scale[i][e % 2] = 0.f;
             }
+          }
         }
         // ---- running maximum and sum ----
         float scale_o[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+          float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+#pragma unroll
+          for (int i = 1; i < 2 * G; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m[h]);
           scale_o[h] = exp2_fast(m[h] - top);
           m[h] = top;
           sum[h] *= scale_o[h];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               s[i][2 * h + e] = exp2_fast(s[i][2 * h + e] - top);
@@ -359,7 +404,9 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
         }
         if constexpr (EIGHT) {
           // the weights times the values' scales, relative to a power of two that is at least each of them
-          float top = fmaxf(fmaxf(value_scale[0][0], value_scale[0][1]), fmaxf(value_scale[1][0], value_scale[1][1]));
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2 * G; ++i) top = fmaxf(top, fmaxf(value_scale[i][0], value_scale[i][1]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           if (top > vm) {
@@ -371,7 +418,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
           }
           const float back = vm > 0.f ? 1.f / vm : 0.f;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[i][e] *= value_scale[i][e % 2] * back;
         }
@@ -382,64 +429,68 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
             for (int e = 0; e < 4; ++e) o[i][e] *= scale_o[e / 2];
         }
         // ---- values ----
-        uint32_t hi[4], part[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < G; ++i) {
+          uint32_t hi[4], part[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float x = s[i][2 * h], y = s[i][2 * h + 1];
-            hi[2 * i + h] = pack<H>(x, y);
-            const float2 r = unpack<H>(hi[2 * i + h]);
-            part[2 * i + h] = pack<H>(x - r.x, y - r.y);
-          }
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // 16-bit pairs of tokens, of the first and the second eight
-        if (edge) {
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) keep[i] = (kept[i][0] ? 0xffffu : 0u) | (kept[i][1] ? 0xffff0000u : 0u);
-        }
-        if constexpr (!EIGHT) {
-#pragma unroll
-          for (int c = 0; c < DP / 16; ++c) {
-            uint32_t b[4];
-            ldmatrix4_trans(b, vs + c / 4 * (kUnit * 128) + v_row * 128 + (((c % 4 * 2 + v_chunk) ^ (v_row & 7)) << 4));
-            if (edge) {
-              b[0] &= keep[0];
-              b[1] &= keep[1];
-              b[2] &= keep[0];
-              b[3] &= keep[1];
+            for (int h = 0; h < 2; ++h) {
+              const float x = s[2 * i + k][2 * h], y = s[2 * i + k][2 * h + 1];
+              hi[2 * k + h] = pack<H>(x, y);
+              if (kParts) {
+                const float2 r = unpack<H>(hi[2 * k + h]);
+                part[2 * k + h] = pack<H>(x - r.x, y - r.y);
+              }
             }
-            mma<H>(o[2 * c], hi, b[0], b[1]);
-            mma<H>(o[2 * c + 1], hi, b[2], b[3]);
-            mma<H>(o[2 * c], part, b[0], b[1]);
-            mma<H>(o[2 * c + 1], part, b[2], b[3]);
-          }
-        } else {
-          // a chunk of 16 elements: the even ones are one tile of eight, the odd ones the next
+          const uint32_t at = vs + group_at[i] + v_row * 128;
+          if constexpr (!EIGHT) {
 #pragma unroll
-          for (int c = 0; c < DP / 16; c += 2) {
-            uint32_t b[4];
-            ldmatrix4_trans(b, vs + c / 8 * (kUnit * 128) + v_row * 128 + (((c % 8 + v_chunk) ^ (v_row & 7)) << 4));
-            if (edge) {
-              b[0] &= keep[0];
-              b[1] &= keep[1];
-              b[2] &= keep[0];
-              b[3] &= keep[1];
+            for (int c = 0; c < DP / 16; ++c) {
+              uint32_t b[4];
+              ldmatrix4_trans(b, at + c / 4 * box_bytes + (((c % 4 * 2 + v_chunk) ^ (v_row & 7)) << 4));
+              if (edge) {
+                b[0] &= keep[2 * i];
+                b[1] &= keep[2 * i + 1];
+                b[2] &= keep[2 * i];
+                b[3] &= keep[2 * i + 1];
+              }
+              mma<H>(o[2 * c], hi, b[0], b[1]);
+              mma<H>(o[2 * c + 1], hi, b[2], b[3]);
+              mma<H>(o[2 * c], part, b[0], b[1]);
+              mma<H>(o[2 * c + 1], part, b[2], b[3]);
             }
+          } else {
+            // a chunk of 16 elements: the even ones are one tile of eight, the odd ones the next
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t even0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0020)), odd0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0031));
-              const uint32_t even1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0020));
-              const uint32_t odd1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0031));
-              mma<H>(o[2 * (c + e)], hi, even0, even1);
-              mma<H>(o[2 * (c + e) + 1], hi, odd0, odd1);
-              mma<H>(o[2 * (c + e)], part, even0, even1);
-              mma<H>(o[2 * (c + e) + 1], part, odd0, odd1);
+            for (int c = 0; c < DP / 16; c += 2) {
+              uint32_t b[4];
+              ldmatrix4_trans(b, at + c / 8 * box_bytes + (((c % 8 + v_chunk) ^ (v_row & 7)) << 4));
+              if (edge) {
+                b[0] &= keep[2 * i];
+                b[1] &= keep[2 * i + 1];
+                b[2] &= keep[2 * i];
+                b[3] &= keep[2 * i + 1];
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t even0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0020)), odd0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0031));
+                const uint32_t even1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0020));
+                const uint32_t odd1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0031));
+                mma<H>(o[2 * (c + e)], hi, even0, even1);
+                mma<H>(o[2 * (c + e) + 1], hi, odd0, odd1);
+                if (kParts) {
+                  mma<H>(o[2 * (c + e)], part, even0, even1);
+                  mma<H>(o[2 * (c + e) + 1], part, odd0, odd1);
+                }
+              }
             }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + 8 * st);
+      turn.next();
     }
 
     // ---- the four warps' results: 2 and 3 to 0 and 1, then 1 to 0; a lane meets the same lane ----
@@ -523,7 +574,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
 }
 
 template <typename T, bool EIGHT, int DP>
-int launch_one(const Maps& maps, const Attend& a, int box, unsigned grid, cudaStream_t stream) {
+int launch_one(const Maps& maps, const Attend& a, int box, int joined, unsigned grid, cudaStream_t stream) {
   using L = Layout<EIGHT, DP>;
   auto kern = token_kernel<T, EIGHT, DP>;
   static std::atomic<uint64_t> ready{0};  // a bit per device
@@ -534,7 +585,7 @@ int launch_one(const Maps& maps, const Attend& a, int box, unsigned grid, cudaSt
     err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (err == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
   }
-  if (err == cudaSuccess) err = launch_pdl(kern, grid, kTokenThreads, L::kBytes, stream, maps, a, box);
+  if (err == cudaSuccess) err = launch_pdl(kern, grid, kTokenThreads, L::kBytes, stream, maps, a, 31 - __builtin_clz(box), joined);
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention token kernel: %s", cudaGetErrorString(err));
   count_launch();
   return KSMM_OK;
@@ -542,43 +593,52 @@ int launch_one(const Maps& maps, const Attend& a, int box, unsigned grid, cudaSt
 
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
+template <typename T, bool EIGHT, int DP>
+int launch_maps(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  using L = Layout<EIGHT, DP>;
+  const Pool& p = a.pool;
+  int box = L::kTokens;
+  while (p.page_size % box) box /= 2;
+  constexpr uint64_t kColumn = EIGHT ? 128 : 64;  // elements of 128 bytes
+  const bool joined = L::kBoxes > 1 && p.dim % kColumn == 0;
+  Maps maps;
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dim = p.dim, rows = p.page_size, heads = p.kv_heads, pages = p.pages, token = p.token[i], head = p.head[i], page = p.page[i];
+    const uint64_t dims4[4] = {dim, rows, heads, pages}, strides4[4] = {1, token, head, page};
+    const uint64_t dims5[5] = {kColumn, rows, dim / kColumn, heads, pages}, strides5[5] = {1, token, kColumn, head, page};
+    const uint32_t size[5] = {static_cast<uint32_t>(kColumn), static_cast<uint32_t>(box), joined ? L::kBoxes : 1u, 1, 1};
+    const int st = encode_map(i ? &maps.values : &maps.keys, cache_dtype, joined ? 5 : 4, p.data[i], joined ? dims5 : dims4,
+                              joined ? strides5 : strides4, size);
+    if (st != KSMM_OK) return st;
+  }
+  return launch_one<T, EIGHT, DP>(maps, a, box, joined, grid, stream);
+}
+
 template <typename T, bool EIGHT>
-int launch_dim(const Maps& maps, const Attend& a, int box, unsigned grid, cudaStream_t stream) {
+int launch_dim(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
   switch (padded(a.pool.dim)) {
-    case 64: return launch_one<T, EIGHT, 64>(maps, a, box, grid, stream);
-    case 128: return launch_one<T, EIGHT, 128>(maps, a, box, grid, stream);
-    default: return launch_one<T, EIGHT, 256>(maps, a, box, grid, stream);
+    case 64: return launch_maps<T, EIGHT, 64>(a, cache_dtype, grid, stream);
+    case 128: return launch_maps<T, EIGHT, 128>(a, cache_dtype, grid, stream);
+    default: return launch_maps<T, EIGHT, 256>(a, cache_dtype, grid, stream);
   }
 }
 
 }  // namespace
 
-int token_blocks_per_sm(int cache_dtype, int dim) {
+TokenShape token_shape(int cache_dtype, int dim) {
   const bool eight = cache_dtype == KSMM_F8E4M3;
   switch (padded(dim)) {
-    case 64: return eight ? Layout<true, 64>::kBlocks : Layout<false, 64>::kBlocks;
-    case 128: return eight ? Layout<true, 128>::kBlocks : Layout<false, 128>::kBlocks;
-    default: return eight ? Layout<true, 256>::kBlocks : Layout<false, 256>::kBlocks;
+    case 64: return eight ? TokenShape{Layout<true, 64>::kBlocks, Layout<true, 64>::kTokens} : TokenShape{Layout<false, 64>::kBlocks, Layout<false, 64>::kTokens};
+    case 128: return eight ? TokenShape{Layout<true, 128>::kBlocks, Layout<true, 128>::kTokens} : TokenShape{Layout<false, 128>::kBlocks, Layout<false, 128>::kTokens};
+    default: return eight ? TokenShape{Layout<true, 256>::kBlocks, Layout<true, 256>::kTokens} : TokenShape{Layout<false, 256>::kBlocks, Layout<false, 256>::kTokens};
   }
 }
 
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
-  const Pool& p = a.pool;
   const bool eight = cache_dtype == KSMM_F8E4M3;
-  const int box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16;
-  Maps maps;
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t dims[4] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(p.page_size), static_cast<uint64_t>(p.kv_heads),
-                              static_cast<uint64_t>(p.pages)};
-    const uint64_t strides[4] = {1, static_cast<uint64_t>(p.token[i]), static_cast<uint64_t>(p.head[i]), static_cast<uint64_t>(p.page[i])};
-    const uint32_t size[4] = {eight ? 128u : 64u, static_cast<uint32_t>(box), 1, 1};
-    const int st = encode_map(i ? &maps.values : &maps.keys, cache_dtype, 4, p.data[i], dims, strides, size);
-    if (st != KSMM_OK) return st;
-  }
   if (dtype == KSMM_F16)
-    return eight ? launch_dim<__half, true>(maps, a, box, grid, stream) : launch_dim<__half, false>(maps, a, box, grid, stream);
-  return eight ? launch_dim<__nv_bfloat16, true>(maps, a, box, grid, stream)
-               : launch_dim<__nv_bfloat16, false>(maps, a, box, grid, stream);
+    return eight ? launch_dim<__half, true>(a, cache_dtype, grid, stream) : launch_dim<__half, false>(a, cache_dtype, grid, stream);
+  return eight ? launch_dim<__nv_bfloat16, true>(a, cache_dtype, grid, stream) : launch_dim<__nv_bfloat16, false>(a, cache_dtype, grid, stream);
 }
 
 // Whether TMA can address the pool and the rows of q and out are pairs on their boundary.
