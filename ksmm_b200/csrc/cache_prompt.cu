@@ -15,6 +15,7 @@
 #include <climits>
 
 #include "cache.cuh"
+#include "tc_epilogue.cuh"
 #include "tc_host.h"
 #include "tc_ptx.cuh"
 
@@ -39,10 +40,18 @@ struct Prompt {
   static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
   static constexpr int kSharedAt = kFlagsAt + 8;
   static constexpr int kBytes = kSharedAt + kShareWords * 8;
-  static constexpr int kThreads = 128 * kTiles + 64;
+  static constexpr int kThreads = 128 * kTiles + (kTiles == 2 ? 128 : 64);  // the last: TMA, MMAs, two warps without work
   static constexpr int kSCols = kKeys;
   static constexpr int kOAt = kTiles * kSCols;
   static_assert(kOAt + kTiles * DP <= 512, "tensor memory");
+  // The launch gives every thread 168 registers (three warps on a scheduler); a row's thread holds 128 scores and more.
+  // 256 x 208 + 128 x 88 = 384 x 168.  (The code after the instruction has its limit: one branch for each.)
+  __device__ static void take_registers() {
+    if constexpr (kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  }
+  __device__ static void give_registers() {
+    if constexpr (kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
 };
 
 struct PromptMaps {
@@ -67,6 +76,12 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -135,162 +150,9 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     most = max(most, count[t]);
   }
 
-  if (warp == kProducer) {
-    // ---------------- TMA: a lane for each box of a tile, tables 32 boxes ahead ----------------
-    const int boxes = C::kKeys / args.box;
-    const uint32_t bytes = static_cast<uint32_t>(args.box) * DP * 2;
-    const int32_t* table = p.table + g.s * p.table_stride;
-    if (most > 0 && lane == 0) {
-      mbar_expect_tx(q_full, static_cast<uint32_t>(args.tile_tokens * a.group) * DP * 2 * C::kTiles);
-#pragma unroll
-      for (int t = 0; t < C::kTiles; ++t)
-#pragma unroll
-        for (int b = 0; b < C::kBoxes; ++b)
-          tma_load_3d(base + t * C::kQ + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group,
-                      g.seq.start + token0 + t * args.tile_tokens);
-    }
-    int page_ahead = -2, ahead = 0;
-    int loaded_k = 0, loaded_v = 0, lone = 0;
-    bool alive = true;
-    for (int j = 0; j < most && alive; ++j) {
-      const int in_batch = j % (32 / boxes);
-      if (in_batch == 0) {
-        const int token = (first + j) * C::kKeys + lane * args.box;
-        ahead = token / p.page_size;
-        const bool there = token < g.hi && token + args.box > g.lo;
-        page_ahead = there ? table[ahead] : -2;
-        if (page_ahead < 0 || page_ahead >= p.pages) page_ahead = -2;
-        ahead = token - ahead * p.page_size;
-      }
-      const int from = in_batch * boxes + lane;
-      const int page = __shfl_sync(0xffffffffu, page_ahead, from & 31), row = __shfl_sync(0xffffffffu, ahead, from & 31);
-      const bool get = lane < boxes && page >= 0;
-      const uint32_t gets = __ballot_sync(0xffffffffu, get);
-      const uint32_t load = __popc(gets);
-      const int tile_token = (first + j) * C::kKeys;
-      const int st = j % C::kStages;
-      const uint32_t parity = (j / C::kStages & 1) ^ 1;
-      alive = __all_sync(0xffffffffu, mbar_wait<20>(k_empty(st), parity, abort_flag, a.status, kPromptWaits + 1));
-      if (!alive) break;
-      if (lane == 0) {
-        if (load) mbar_expect_tx(k_full(st), load * bytes);
-        else mbar_arrive(k_full(st));
-      }
-      ++loaded_k;
-      __syncwarp();
-      const uint32_t kt = base + C::kRingAt + st * C::kOperand, vt = kt + C::kStages * C::kOperand;
-      if (get) {
-#pragma unroll
-        for (int b = 0; b < C::kBoxes; ++b)
-          tma_load_4d(kt + b * C::kKeys * 128 + lane * args.box * 128, &maps.keys, k_full(st), b * 64, row, g.head, page);
-      }
-      __syncwarp();
-      alive = __all_sync(0xffffffffu, mbar_wait<20>(v_empty(st), parity, abort_flag, a.status, kPromptWaits + 1));
-      if (!alive) break;
-      // values that no row may meet are zeros, whatever lies in the page behind the sequence or in the stage from before
-      const bool ragged = load < boxes || tile_token < g.lo || tile_token + C::kKeys > g.hi;
-      const uint32_t bar = ragged ? alone : v_full(st);
-      if (lane == 0 && load) mbar_expect_tx(bar, load * bytes);
-      __syncwarp();
-      if (get) {
-#pragma unroll
-        for (int b = 0; b < C::kBoxes; ++b)
-          tma_load_4d(vt + b * C::kKeys * 128 + lane * args.box * 128, &maps.values, bar, b * 64, row, g.head, page);
-      }
-      __syncwarp();
-      if (!ragged) {
-        ++loaded_v;
-        continue;
-      }
-      if (load) {
-        alive = __all_sync(0xffffffffu, mbar_wait<20>(alone, lone & 1, abort_flag, a.status, kPromptWaits + 2));
-        if (!alive) break;
-        ++lone;
-      }
-      for (int i = lane; i < C::kKeys * C::kBoxes * 8; i += 32) {
-        const int r = i / 8 % C::kKeys, token = tile_token + r;
-        const bool keep = token >= g.lo && token < g.hi && (gets >> (r / args.box) & 1);
-        if (!keep) *reinterpret_cast<uint4*>(smem + (vt - base) + i * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(v_full(st));
-      ++loaded_v;
-    }
-    if (!alive) {
-      // the copies in flight end before the block does (one of its own: `alone`; waits that give up already did)
-      int zero = 0;
-      for (int j = loaded_k > C::kStages ? loaded_k - C::kStages : 0; j < loaded_k; ++j)
-        mbar_wait<100>(k_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
-      for (int j = loaded_v > C::kStages ? loaded_v - C::kStages : 0; j < loaded_v; ++j)
-        mbar_wait<100>(v_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
-      if (most > 0) mbar_wait<100>(q_full, 0, &zero, a.status, kPromptWaits + 2);
-    }
-  } else if (warp == kIssuer) {
-    // ---------------- MMAs: the warp walks the loop, one lane issues ----------------
-    constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    const bool one = elect_one();
-    bool alive = true;
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(bar, parity, abort_flag, a.status, kPromptWaits + 3));
-      return alive;
-    };
-    auto commit = [&](uint32_t bar) {
-      if (one) umma_commit(bar);
-    };
-    auto scores = [&](int t, int st) {
-      if (one) {
-        const uint32_t q = (base + t * C::kQ) >> 4 | 1u << 16, k = (base + C::kRingAt + st * C::kOperand) >> 4 | 1u << 16;
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const uint64_t qd = static_cast<uint64_t>(kDescHi) << 32 | (q + i / 4 * (128 * 128 >> 4) + i % 4 * 2);
-          const uint64_t kd = static_cast<uint64_t>(kDescHi) << 32 | (k + i / 4 * (C::kKeys * 128 >> 4) + i % 4 * 2);
-          umma<2>(tmem + t * C::kSCols, qd, kd, args.idesc_s, i != 0);
-        }
-      }
-      commit(s_full(t));
-    };
-    auto outputs = [&](int t, int st, bool more) {
-      if (one) {
-        const uint32_t v = (base + C::kRingAt + (C::kStages + st) * C::kOperand) >> 4 | static_cast<uint32_t>(C::kKeys * 128 >> 4) << 16;
-#pragma unroll
-        for (int i = 0; i < C::kKeys / 16; ++i) {
-          const uint64_t vd = static_cast<uint64_t>(kDescHi) << 32 | (v + i * (16 * 128 >> 4));
-          umma_ts(tmem + C::kOAt + t * DP, tmem + t * C::kSCols + i * 8, vd, args.idesc_o, more || i != 0);
-        }
-      }
-    };
-    if (most > 0 && wait(q_full, 0) && wait(k_full(0), 0)) {
-      tc_fence_after();
-#pragma unroll
-      for (int t = 0; t < C::kTiles; ++t)
-        if (count[t] > 0) scores(t, 0);
-      commit(k_empty(0));
-      for (int j = 0; j < most; ++j) {
-        const int st = j % C::kStages, next = (j + 1) % C::kStages;
-        if (!wait(v_full(st), j / C::kStages & 1)) break;
-        if (j + 1 < most && !wait(k_full(next), (j + 1) / C::kStages & 1)) break;
-#pragma unroll
-        for (int t = 0; t < C::kTiles; ++t) {
-          if (j >= count[t] || !wait(p_full(t), j & 1)) continue;
-          tc_fence_after();
-          outputs(t, st, j > 0);
-          if (j + 1 == count[t]) commit(o_full(t));
-          else scores(t, next);  // (over P, which the MMAs before have read: they run in order)
-        }
-        if (!alive) break;
-        commit(v_empty(st));
-        if (j + 1 < most) commit(k_empty(next));
-      }
-    }
-    if (!alive) {
-      // MMAs in flight end before tensor memory is given back
-      int zero = 0;
-      commit(alone);
-      mbar_wait<100>(alone, 0, &zero, a.status, kPromptWaits + 3);
-    }
-  } else {
+  if (warp < kProducer) {
     // ---------------- a thread per row ----------------
+    C::take_registers();
     const int t = warp / 4, r = tid % 128;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * C::kSCols, o_at = tmem + lanes + C::kOAt + t * DP;
@@ -337,9 +199,9 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
         for (int c = 0; c < C::kKeys; ++c)
           if (c >= to || c < from) s[c] = -INFINITY;
       }
-      float high[4] = {top, s[0], s[1], s[2]};
+      float high[4] = {top, kNone, kNone, kNone};
 #pragma unroll
-      for (int c = 3; c < C::kKeys; ++c) high[c % 4] = fmaxf(high[c % 4], s[c]);
+      for (int c = 0; c < C::kKeys; c += 2) high[c / 2 % 4] = fmaxf(fmaxf(high[c / 2 % 4], s[c]), s[c + 1]);  // (of three: one instruction)
       const float now = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
       const bool grown = (now - top) * a.scale > 8.f;
       if (j == 0) {
@@ -359,19 +221,27 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
         }
       }
       const float shift = top == kNone ? 0.f : -top * a.scale;
-      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = pack_f2(a.scale, a.scale), shift2 = pack_f2(shift, shift);
+      uint64_t sums[2] = {0, 0};  // pairs
 #pragma unroll
       for (int c = 0; c < C::kKeys; c += 64) {
         uint32_t w[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = exp2_fast(fmaf(s[c + 2 * e], a.scale, shift)), y = exp2_fast(fmaf(s[c + 2 * e + 1], a.scale, shift));
-          sums[e % 4] += x + y;
+          float x, y;
+          unpack_f2(fma_f2(pack_f2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2), x, y);
+          x = exp2_fast(x);
+          y = exp2_fast(y);
+          sums[e % 2] = add_f2(sums[e % 2], pack_f2(x, y));
           w[e] = pack2(x, y, ElemTraits<T>::kDtype);
         }
         tmem_st32(s_at + c / 2, w);
       }
-      sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      {
+        float x, y;
+        unpack_f2(add_f2(sums[0], sums[1]), x, y);
+        sum += x + y;
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -407,6 +277,163 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
       }
     }
     tc_fence_before();
+  } else {
+    C::give_registers();
+    if (warp == kProducer) {
+      // ---------------- TMA: a lane for each box of a tile, tables 32 boxes ahead ----------------
+      const int boxes = C::kKeys / args.box;
+      const uint32_t bytes = static_cast<uint32_t>(args.box) * DP * 2;
+      const int32_t* table = p.table + g.s * p.table_stride;
+      if (most > 0 && lane == 0) {
+        mbar_expect_tx(q_full, static_cast<uint32_t>(args.tile_tokens * a.group) * DP * 2 * C::kTiles);
+#pragma unroll
+        for (int t = 0; t < C::kTiles; ++t)
+#pragma unroll
+          for (int b = 0; b < C::kBoxes; ++b)
+            tma_load_3d(base + t * C::kQ + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group,
+                        g.seq.start + token0 + t * args.tile_tokens);
+      }
+      int page_ahead = -2, ahead = 0;
+      int loaded_k = 0, loaded_v = 0, lone = 0;
+      bool alive = true;
+      for (int j = 0; j < most && alive; ++j) {
+        const int in_batch = j % (32 / boxes);
+        if (in_batch == 0) {
+          const int token = (first + j) * C::kKeys + lane * args.box;
+          ahead = token / p.page_size;
+          const bool there = token < g.hi && token + args.box > g.lo;
+          page_ahead = there ? table[ahead] : -2;
+          if (page_ahead < 0 || page_ahead >= p.pages) page_ahead = -2;
+          ahead = token - ahead * p.page_size;
+        }
+        const int from = in_batch * boxes + lane;
+        const int page = __shfl_sync(0xffffffffu, page_ahead, from & 31), row = __shfl_sync(0xffffffffu, ahead, from & 31);
+        const bool get = lane < boxes && page >= 0;
+        const uint32_t gets = __ballot_sync(0xffffffffu, get);
+        const uint32_t load = __popc(gets);
+        const int tile_token = (first + j) * C::kKeys;
+        const int st = j % C::kStages;
+        const uint32_t parity = (j / C::kStages & 1) ^ 1;
+        alive = __all_sync(0xffffffffu, mbar_wait<20>(k_empty(st), parity, abort_flag, a.status, kPromptWaits + 1));
+        if (!alive) break;
+        if (lane == 0) {
+          if (load) mbar_expect_tx(k_full(st), load * bytes);
+          else mbar_arrive(k_full(st));
+        }
+        ++loaded_k;
+        __syncwarp();
+        const uint32_t kt = base + C::kRingAt + st * C::kOperand, vt = kt + C::kStages * C::kOperand;
+        if (get) {
+#pragma unroll
+          for (int b = 0; b < C::kBoxes; ++b)
+            tma_load_4d(kt + b * C::kKeys * 128 + lane * args.box * 128, &maps.keys, k_full(st), b * 64, row, g.head, page);
+        }
+        __syncwarp();
+        alive = __all_sync(0xffffffffu, mbar_wait<20>(v_empty(st), parity, abort_flag, a.status, kPromptWaits + 1));
+        if (!alive) break;
+        // values that no row may meet are zeros, whatever lies in the page behind the sequence or in the stage from before
+        const bool ragged = load < boxes || tile_token < g.lo || tile_token + C::kKeys > g.hi;
+        const uint32_t bar = ragged ? alone : v_full(st);
+        if (lane == 0 && load) mbar_expect_tx(bar, load * bytes);
+        __syncwarp();
+        if (get) {
+#pragma unroll
+          for (int b = 0; b < C::kBoxes; ++b)
+            tma_load_4d(vt + b * C::kKeys * 128 + lane * args.box * 128, &maps.values, bar, b * 64, row, g.head, page);
+        }
+        __syncwarp();
+        if (!ragged) {
+          ++loaded_v;
+          continue;
+        }
+        if (load) {
+          alive = __all_sync(0xffffffffu, mbar_wait<20>(alone, lone & 1, abort_flag, a.status, kPromptWaits + 2));
+          if (!alive) break;
+          ++lone;
+        }
+        for (int i = lane; i < C::kKeys * C::kBoxes * 8; i += 32) {
+          const int r = i / 8 % C::kKeys, token = tile_token + r;
+          const bool keep = token >= g.lo && token < g.hi && (gets >> (r / args.box) & 1);
+          if (!keep) *reinterpret_cast<uint4*>(smem + (vt - base) + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full(st));
+        ++loaded_v;
+      }
+      if (!alive) {
+        // the copies in flight end before the block does (one of its own: `alone`; waits that give up already did)
+        int zero = 0;
+        for (int j = loaded_k > C::kStages ? loaded_k - C::kStages : 0; j < loaded_k; ++j)
+          mbar_wait<100>(k_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
+        for (int j = loaded_v > C::kStages ? loaded_v - C::kStages : 0; j < loaded_v; ++j)
+          mbar_wait<100>(v_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
+        if (most > 0) mbar_wait<100>(q_full, 0, &zero, a.status, kPromptWaits + 2);
+      }
+    } else if (warp == kIssuer) {
+      // ---------------- MMAs: the warp walks the loop, one lane issues ----------------
+      constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      const bool one = elect_one();
+      bool alive = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(bar, parity, abort_flag, a.status, kPromptWaits + 3));
+        return alive;
+      };
+      auto commit = [&](uint32_t bar) {
+        if (one) umma_commit(bar);
+      };
+      auto scores = [&](int t, int st) {
+        if (one) {
+          const uint32_t q = (base + t * C::kQ) >> 4 | 1u << 16, k = (base + C::kRingAt + st * C::kOperand) >> 4 | 1u << 16;
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) {
+            const uint64_t qd = static_cast<uint64_t>(kDescHi) << 32 | (q + i / 4 * (128 * 128 >> 4) + i % 4 * 2);
+            const uint64_t kd = static_cast<uint64_t>(kDescHi) << 32 | (k + i / 4 * (C::kKeys * 128 >> 4) + i % 4 * 2);
+            umma<2>(tmem + t * C::kSCols, qd, kd, args.idesc_s, i != 0);
+          }
+        }
+        commit(s_full(t));
+      };
+      auto outputs = [&](int t, int st, bool more) {
+        if (one) {
+          const uint32_t v = (base + C::kRingAt + (C::kStages + st) * C::kOperand) >> 4 | static_cast<uint32_t>(C::kKeys * 128 >> 4) << 16;
+#pragma unroll
+          for (int i = 0; i < C::kKeys / 16; ++i) {
+            const uint64_t vd = static_cast<uint64_t>(kDescHi) << 32 | (v + i * (16 * 128 >> 4));
+            umma_ts(tmem + C::kOAt + t * DP, tmem + t * C::kSCols + i * 8, vd, args.idesc_o, more || i != 0);
+          }
+        }
+      };
+      if (most > 0 && wait(q_full, 0) && wait(k_full(0), 0)) {
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < C::kTiles; ++t)
+          if (count[t] > 0) scores(t, 0);
+        commit(k_empty(0));
+        for (int j = 0; j < most; ++j) {
+          const int st = j % C::kStages, next = (j + 1) % C::kStages;
+          if (!wait(v_full(st), j / C::kStages & 1)) break;
+          if (j + 1 < most && !wait(k_full(next), (j + 1) / C::kStages & 1)) break;
+#pragma unroll
+          for (int t = 0; t < C::kTiles; ++t) {
+            if (j >= count[t] || !wait(p_full(t), j & 1)) continue;
+            tc_fence_after();
+            outputs(t, st, j > 0);
+            if (j + 1 == count[t]) commit(o_full(t));
+            else scores(t, next);  // (over P, which the MMAs before have read: they run in order)
+          }
+          if (!alive) break;
+          commit(v_empty(st));
+          if (j + 1 < most) commit(k_empty(next));
+        }
+      }
+      if (!alive) {
+        // MMAs in flight end before tensor memory is given back
+        int zero = 0;
+        commit(alone);
+        mbar_wait<100>(alone, 0, &zero, a.status, kPromptWaits + 3);
+      }
+    }
   }
   __syncthreads();
   if (warp == kIssuer) {

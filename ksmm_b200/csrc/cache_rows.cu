@@ -221,8 +221,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
 // Joins the parts of items that several blocks shared.  Block (c, r): row r of the item that begins in block c and goes on; its
 // further parts are in slot 0 of the blocks after c, as long as they name the item.  They are summed in the order of the blocks,
 // eight runs side by side, whoever was first.  A chain of reads is all the time that it takes: what may turn out not to be a
-// part (maxima and sums of the blocks after c) is read before that is known.
+// part (maxima and sums of the first blocks after c) is read before that is known.
 constexpr int kJoinThreads = 256;
+constexpr int kAhead = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Attend a, int blocks) {
@@ -245,8 +246,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const int i = tid + k * kJoinThreads;
     const bool there = c + i < blocks;
     named[k] = !there ? -1 : i == 0 ? item : a.slots[2 * static_cast<int64_t>(c + i)];
-    m[k] = there ? part(i)[a.tile_rows * p.dim + r] : 0.f;
-    l[k] = there ? part(i)[a.tile_rows * (p.dim + 1) + r] : 0.f;
+    m[k] = l[k] = 0.f;
+    // (few items have more parts than this; reading all blocks' values took 4 us more than the second wait)
+    if (there && i < kAhead) {
+      m[k] = part(i)[a.tile_rows * p.dim + r];
+      l[k] = part(i)[a.tile_rows * (p.dim + 1) + r];
+    }
   }
   const int s = static_cast<int>((item >> 32) / p.kv_heads), head = static_cast<int>((item >> 32) % p.kv_heads);
   const int tile = static_cast<int>(item & 0xffffffff);
@@ -258,7 +263,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   for (int k = 0; k < kReads; ++k) {
     // (an item's blocks follow one another)
     parts += __syncthreads_count(named[k] == item);
-    if (named[k] == item) top = fmaxf(top, m[k]);
+    if (named[k] != item) continue;
+    const int i = tid + k * kJoinThreads;
+    if (i >= kAhead) {
+      m[k] = part(i)[a.tile_rows * p.dim + r];
+      l[k] = part(i)[a.tile_rows * (p.dim + 1) + r];
+    }
+    top = fmaxf(top, m[k]);
   }
 #pragma unroll
   for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));

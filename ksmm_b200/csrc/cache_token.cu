@@ -31,28 +31,32 @@ namespace {
 
 using namespace tc;
 
-constexpr int kConsumers = 4;
-constexpr int kTokenThreads = (kConsumers + 1) * 32;
 constexpr int kTileRows = kTokenRows;
 
 template <bool EIGHT, int DP>
 struct Layout {
+  // Warps that meet different tokens; rows of 256 have two for the same tokens, each with half of the output's columns (one alone has
+  // 96 products and 32 loads in a step, and nothing else on its scheduler)
+  static constexpr int kRuns = 4, kHalves = DP == 256 ? 2 : 1, kConsumers = kRuns * kHalves;
+  static constexpr int kThreads = (kConsumers + 1) * 32;
+  static constexpr int kCols = DP / kHalves;                            // of a warp's output
   // Tokens of a warp's step.  A step is a chain (load, products, maximum, exponentials, products) of 1000 to 1500 cycles
   // however many tokens it has, and an SM's eight warps have to pass 23 bytes a cycle: small rows take 32 tokens at a time.
   static constexpr int kStep = DP == 256 || (!EIGHT && DP == 128) ? 16 : 32;
-  static constexpr int kTokens = kConsumers * kStep;                    // a unit, a stage of the ring
+  static constexpr int kTokens = kRuns * kStep;                         // a unit, a stage of the ring
   static constexpr int kBoxes = EIGHT ? (DP + 127) / 128 : DP / 64;     // 128-byte columns of a row
   static constexpr int kOperand = kBoxes * kTokens * 128;               // a unit's keys
   static constexpr int kScales = EIGHT ? 2 * kTokens * 4 : 0;
   static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kBlocks = DP == 256 ? 1 : 2;                     // on an SM
   static constexpr int kStages = 196608 / kBlocks / (kStageBytes + kScales);
-  static constexpr int kMerge = DP / 2 * 32 * 4;                        // a warp's output
+  static constexpr int kMerge = kCols / 2 * 32 * 4;                     // a warp's output
   static constexpr int kMergeAt = kStages * kStageBytes;
-  static constexpr int kScalesAt = kMergeAt + 2 * kMerge;
-  static constexpr int kStatsAt = kScalesAt + kStages * kScales;        // of the merges: 2 x 4 x 8 floats
-  static constexpr int kBarsAt = kStatsAt + 2 * 4 * 8 * 4;
+  static constexpr int kScalesAt = kMergeAt + 2 * kHalves * kMerge;
+  static constexpr int kStatsAt = kScalesAt + kStages * kScales;        // of the merges: 2 x 4 x 8 floats a half
+  static constexpr int kBarsAt = kStatsAt + kHalves * 2 * 4 * 8 * 4;
   static constexpr int kFlagsAt = kBarsAt + 2 * kStages * 8;
+  static constexpr int kQRow = DP * 2 + 16;                             // bytes of a row of q in shared memory
   static constexpr int kBytes = kFlagsAt + kStages * 4 + 4;
   static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
   static_assert(kStages >= 2, "a ring");
@@ -130,12 +134,14 @@ struct Turn {
 // T: q and the output.  Tokens of a page that one TMA box covers: 2^box_log2; a box lies in its stage as [128-byte column][token].
 // `joined`: a map with the columns as a dimension of their own brings all of a box's at once.
 template <typename T, bool EIGHT, int DP>
-__global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
+__global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>::kBlocks)
     token_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Attend a, const int box_log2, const int joined) {
   using L = Layout<EIGHT, DP>;
   using H = typename std::conditional<EIGHT, __half, T>::type;  // of the products
   // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
   constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
+  // q in shared memory where registers do not hold it and the output
+  constexpr bool kQShared = DP == 256;
   constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
   extern __shared__ __align__(1024) char smem[];
   const uint32_t base = smem_u32(smem);
@@ -151,11 +157,11 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
     *abort_flag = 0;
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, kConsumers);
+      mbar_init(empty + 8 * i, L::kConsumers);
     }
     fence_mbar_init();
   }
-  if (warp == kConsumers && lane == 0) {
+  if (warp == L::kConsumers && lane == 0) {
     prefetch_tensormap(&maps.keys);
     prefetch_tensormap(&maps.values);
   }
@@ -163,13 +169,13 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
   grid_dep_launch();
   clear_rest<T>(a);
   Share mine;
-  if (!share<kTokenThreads>(a, reinterpret_cast<int64_t*>(smem + L::kMergeAt), &mine)) return;
+  if (!share<L::kThreads>(a, reinterpret_cast<int64_t*>(smem + L::kMergeAt), &mine)) return;
   const Pool& p = a.pool;
   const int box = 1 << box_log2, box_bytes = box * 128;
   Turn<L::kStages> turn;
   Segment g;
 
-  if (warp == kConsumers) {
+  if (warp == L::kConsumers) {
     // ---------------- producer: the warp walks the loop, tables 32 boxes ahead, one lane issues ----------------
     const int boxes = L::kTokens >> box_log2;
     const uint32_t bytes = static_cast<uint32_t>(box_bytes) * L::kBoxes * 2 + (EIGHT ? 2 * box * 4 : 0);
@@ -241,8 +247,9 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
   const int gq = lane / 4, q4 = lane % 4;
   bool alive = true;
   bool slot_used[2] = {false, false};
-  float* merge = reinterpret_cast<float*>(smem + L::kMergeAt);
-  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt);
+  const int run = warp % L::kRuns, half = warp / L::kRuns;
+  float* merge = reinterpret_cast<float*>(smem + L::kMergeAt + half * 2 * L::kMerge);
+  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt) + half * 2 * 4 * 8;
   // lane's row and chunk in the loads of four matrices: K: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1;
   // V: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1
   const int k_row = (lane / 16) * 8 + lane % 8, k_chunk = lane / 8 % 2;
@@ -251,7 +258,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
   uint32_t group_at[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    const int t = warp * L::kStep + i * 16, b = t >> box_log2;
+    const int t = run * L::kStep + i * 16, b = t >> box_log2;
     group_at[i] = b * box_bytes * L::kBoxes + (t - (b << box_log2)) * 128;
   }
   while (mine.next(a, &g)) {
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
     uint32_t qf[DP / 16][4];
     float m[2], sum[2], row_scale[2], vm = 0.f;
     int position[2];
-    float o[DP / 8][4];
+    float o[L::kCols / 8][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = gq + 8 * h, row = g.tile * kTileRows + r, t = row / a.group;
@@ -302,10 +309,23 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
       }
     }
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i)
+    for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
+    if constexpr (kQShared) {
+      // (one warp for all; the region is the merges', whose last reads are over)
+      bar_sync_named(1, L::kConsumers * 32);
+      if (warp == 0) {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint32_t*>(smem + L::kMergeAt + (gq + 8 * (e % 2)) * L::kQRow + (c * 16 + 2 * q4 + 8 * (e / 2)) * 2) = qf[c][e];
+      }
+      bar_sync_named(1, L::kConsumers * 32);
+    }
+    const uint32_t q_at = base + L::kMergeAt + v_row * L::kQRow + v_chunk * 16;
     // tokens from `clear` to below `sure` are seen by every row
     const int sure = g.first_position + 1;
     const int64_t clear = a.window ? static_cast<int64_t>(g.hi) - a.window : 0;
@@ -313,7 +333,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
     for (int u = g.from; u < g.to; ++u) {
       const int st = turn.stage;
       alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(full + 8 * st, turn.parity, abort_flag, a.status, kWaits + 2));
-      const int token = u * L::kTokens + warp * L::kStep;  // the warp's first
+      const int token = u * L::kTokens + run * L::kStep;  // the warp's first
       if (alive && token < g.hi && token + L::kStep > g.lo) {
         const uint32_t ks = base + st * L::kStageBytes, vs = ks + L::kOperand;
         const int missing = flags[st];
@@ -329,6 +349,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
 #pragma unroll
             for (int i = 0; i < G; ++i) {
               uint32_t b[4];
+              if (kQShared && i == 0) ldmatrix4(qf[c], q_at + c * 32);
               ldmatrix4(b, ks + group_at[i] + c / 4 * box_bytes + k_row * 128 + (((c % 4 * 2 + k_chunk) ^ (k_row & 7)) << 4));
               mma<H>(s[2 * i], qf[c], b[0], b[1]);
               mma<H>(s[2 * i + 1], qf[c], b[2], b[3]);
@@ -339,6 +360,10 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
 #pragma unroll
             for (int i = 0; i < G; ++i) {
               uint32_t b[4];
+              if (kQShared && i == 0) {
+                ldmatrix4(qf[c], q_at + c * 32);
+                ldmatrix4(qf[c + 1], q_at + c * 32 + 32);
+              }
               ldmatrix4(b, ks + group_at[i] + c / 8 * box_bytes + k_row * 128 + (((c % 8 + k_chunk) ^ (k_row & 7)) << 4));
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
@@ -349,7 +374,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
         }
         float value_scale[2 * G][2];
         if constexpr (EIGHT) {
-          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + warp * L::kStep + 2 * q4;
+          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + run * L::kStep + 2 * q4;
 #pragma unroll
           for (int i = 0; i < 2 * G; ++i) {
             const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * i), v2 = *reinterpret_cast<const float2*>(sc + L::kTokens + 8 * i);
@@ -370,7 +395,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
 #pragma unroll
           for (int i = 0; i < 2 * G; ++i) {
             keep[i] = 0;
-            const bool gone = missing >> ((warp * L::kStep + i * 8) >> box_log2) & 1;
+            const bool gone = missing >> ((run * L::kStep + i * 8) >> box_log2) & 1;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = token + 8 * i + 2 * q4 + e % 2;
@@ -424,7 +449,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
         }
         if (__any_sync(0xffffffffu, scale_o[0] != 1.f || scale_o[1] != 1.f)) {
 #pragma unroll
-          for (int i = 0; i < DP / 8; ++i)
+          for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] *= scale_o[e / 2];
         }
@@ -443,10 +468,10 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
                 part[2 * k + h] = pack<H>(x - r.x, y - r.y);
               }
             }
-          const uint32_t at = vs + group_at[i] + v_row * 128;
+          const uint32_t at = vs + group_at[i] + half * (L::kBoxes / L::kHalves) * box_bytes + v_row * 128;
           if constexpr (!EIGHT) {
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
+            for (int c = 0; c < L::kCols / 16; ++c) {
               uint32_t b[4];
               ldmatrix4_trans(b, at + c / 4 * box_bytes + (((c % 4 * 2 + v_chunk) ^ (v_row & 7)) << 4));
               if (edge) {
@@ -463,7 +488,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
           } else {
             // a chunk of 16 elements: the even ones are one tile of eight, the odd ones the next
 #pragma unroll
-            for (int c = 0; c < DP / 16; c += 2) {
+            for (int c = 0; c < L::kCols / 16; c += 2) {
               uint32_t b[4];
               ldmatrix4_trans(b, at + c / 8 * box_bytes + (((c % 8 + v_chunk) ^ (v_row & 7)) << 4));
               if (edge) {
@@ -493,7 +518,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
       turn.next();
     }
 
-    // ---- the four warps' results: 2 and 3 to 0 and 1, then 1 to 0; a lane meets the same lane ----
+    // ---- the four runs' results: 2 and 3 to 0 and 1, then 1 to 0; a lane meets the same lane ----
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
@@ -501,14 +526,14 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
     }
     if (EIGHT) {
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i)
+      for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] *= vm;
     }
     auto give = [&](int buffer) {
-      float* to = merge + buffer * (DP / 2 * 32) + lane;
+      float* to = merge + buffer * (L::kCols / 2 * 32) + lane;
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i)
+      for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) to[(4 * i + e) * 32] = o[i][e];
 #pragma unroll
@@ -519,7 +544,7 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
       }
     };
     auto take = [&](int buffer) {
-      const float* from = merge + buffer * (DP / 2 * 32) + lane;
+      const float* from = merge + buffer * (L::kCols / 2 * 32) + lane;
       float mine_f[2], other_f[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -530,23 +555,23 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
         sum[h] = sum[h] * mine_f[h] + stats[(buffer * 4 + 2 + h) * 8 + gq] * other_f[h];
       }
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i)
+      for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * mine_f[e / 2] + from[(4 * i + e) * 32] * other_f[e / 2];
     };
-    bar_sync_named(1, kConsumers * 32);  // (the last segment's have been read)
-    if (warp >= 2) give(warp - 2);
-    bar_sync_named(1, kConsumers * 32);
-    if (warp < 2) take(warp);
-    bar_sync_named(1, kConsumers * 32);
-    if (warp == 1) give(0);
-    bar_sync_named(1, kConsumers * 32);
+    bar_sync_named(1, L::kConsumers * 32);  // (the last segment's have been read)
+    if (run >= 2) give(run - 2);
+    bar_sync_named(1, L::kConsumers * 32);
+    if (run < 2) take(run);
+    bar_sync_named(1, L::kConsumers * 32);
+    if (run == 1) give(0);
+    bar_sync_named(1, L::kConsumers * 32);
     const int slot = g.slot;
     if (slot) slot_used[slot - 1] = true;
-    if (warp != 0) continue;
+    if (run != 0) continue;
     take(0);
     if (g.seq.bad || !alive) sum[0] = sum[1] = __int_as_float(0x7fffffff);
-    if (slot && lane == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
+    if (slot && warp == 0 && lane == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
     float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + slot - 1) * kTileRows * (p.dim + 2);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -555,14 +580,14 @@ __global__ void __launch_bounds__(kTokenThreads, Layout<EIGHT, DP>::kBlocks)
       const int row = g.tile * kTileRows + r, t = row / a.group;
       T* to = reinterpret_cast<T*>(a.out) + (g.seq.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
       const float f = slot ? 1.f : sum[h] == 0.f ? 0.f : 1.f / sum[h];
-      if (slot && q4 == 0) {
+      if (slot && q4 == 0 && half == 0) {
         to_part[kTileRows * p.dim + r] = m[h];
         to_part[kTileRows * (p.dim + 1) + r] = sum[h];
       }
       // pairs of neighbours: 8-bit chunks have them in the two tiles
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i) {
-        const int d = EIGHT ? i / 2 * 16 + 4 * q4 + 2 * (i % 2) : i * 8 + 2 * q4;
+      for (int i = 0; i < L::kCols / 8; ++i) {
+        const int d = half * L::kCols + (EIGHT ? i / 2 * 16 + 4 * q4 + 2 * (i % 2) : i * 8 + 2 * q4);
         const float x = EIGHT ? o[i / 2 * 2][2 * h + i % 2] : o[i][2 * h], y = EIGHT ? o[i / 2 * 2 + 1][2 * h + i % 2] : o[i][2 * h + 1];
         if (d >= p.dim) continue;
         if (slot) *reinterpret_cast<float2*>(to_part + r * p.dim + d) = make_float2(x, y);
@@ -585,7 +610,7 @@ int launch_one(const Maps& maps, const Attend& a, int box, int joined, unsigned 
     err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (err == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
   }
-  if (err == cudaSuccess) err = launch_pdl(kern, grid, kTokenThreads, L::kBytes, stream, maps, a, 31 - __builtin_clz(box), joined);
+  if (err == cudaSuccess) err = launch_pdl(kern, grid, L::kThreads, L::kBytes, stream, maps, a, 31 - __builtin_clz(box), joined);
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention token kernel: %s", cudaGetErrorString(err));
   count_launch();
   return KSMM_OK;
