@@ -476,9 +476,9 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
     rows = p->most = kFewRows;
   }
   p->token = token_fits(d);
-  const TokenShape shape = p->token ? token_shape(c.cache_dtype, c.head_dim) : TokenShape{1, kRowsUnit};
+  p->tile = p->token ? kTokenRows : rows_tile(c.head_dim, rows);
+  const TokenShape shape = p->token ? token_shape(c.cache_dtype, c.head_dim) : TokenShape{row_blocks(c.head_dim, p->tile), kRowsUnit};
   p->unit = shape.unit;
-  p->tile = p->token ? kTokenRows : rows_tile(c.head_dim);
   p->split = rows <= kFewRows;
   p->rows = static_cast<int>(std::min<int64_t>(sure * group, p->tile));  // (max_new is the caller's word)
   if (!p->split) {

@@ -283,7 +283,9 @@ __device__ void clear_rest(const Attend& a) {
 // host side: each returns a status
 constexpr int kMaxBlocks = 512;  // of a split launch (the join kernel's table of weights)
 constexpr int kRowsUnit = 64;     // tokens of a unit in the CUDA-core kernel
-int rows_tile(int dim);           // rows of an item there
+constexpr int kFewRowsTile = 2;
+int rows_tile(int dim, int64_t rows);  // rows of an item there, where there are so many
+constexpr int row_blocks(int dim, int tile) { return tile == kFewRowsTile && dim <= 64 ? 2 : 1; }  // on an SM
 int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
 struct TokenShape {
   int blocks, unit;  // blocks on an SM, tokens of a unit

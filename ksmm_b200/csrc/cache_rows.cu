@@ -4,6 +4,8 @@
 // Eight lanes hold a token's key: with q in registers each lane multiplies its dims, three shuffles join them.  A warp has four
 // such groups and a block eight warps, and every group keeps a running maximum, sum and output row of its own over its
 // tokens, two at a time; they are joined once, at the end of a segment.
+#include <atomic>
+
 #include "cache.cuh"
 #include "tc_host.h"
 #include "tc_ptx.cuh"
@@ -13,6 +15,10 @@ namespace cache {
 namespace {
 
 constexpr int kRowThreads = 256;
+// Keys and values on their way: each thread copies its own pieces asynchronously into shared memory, kSlots units deep, and reads
+// them back itself, without a barrier.  Wider rows would fill it with one unit; elements one by one cannot be copied so.
+constexpr int kSlots = 3;
+constexpr bool row_ring(int vec, int dpl) { return vec == 4 && dpl <= 16; }
 
 template <int N>
 struct Bytes;
@@ -49,13 +55,17 @@ __device__ __forceinline__ void load_row(const T* row, int l, int dim, bool ther
   }
 }
 
-template <typename T, typename C, int DPL, int VEC>
-__global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_constant__ Attend a) {
-  constexpr int R = 64 / DPL;
+// R: rows of an item.  Where a key head has one or two, registers for no more let several blocks share an SM, which is what keeps
+// enough loads in flight (32 sequences of 12 heads of 64, fp32: 123 us with one block of eight rows, 67 with two of two rows, 74 with three).
+template <typename T, typename C, int DPL, int VEC, int R>
+__global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kernel(const __grid_constant__ Attend a) {
   constexpr bool kEight = sizeof(C) == 1;
+  constexpr bool kRing = row_ring(VEC, DPL);
   __shared__ int64_t shared[kShareWords];
   __shared__ float stats[2][kRowThreads / 32][R];
-  extern __shared__ float sums[];  // [warp][R][8 DPL]
+  extern __shared__ __align__(16) char smem[];
+  float* sums = reinterpret_cast<float*>(smem);  // [warp][R][8 DPL]
+  const uint32_t smem_base = tc::smem_u32(smem), ring = smem_base + kRowThreads / 32 * R * 8 * DPL * sizeof(float);
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   clear_rest<T>(a);
@@ -83,33 +93,96 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
 #pragma unroll
       for (int e = 0; e < DPL; ++e) o[r][e] = 0.f;
     }
+    const int32_t* table = p.table + g.s * p.table_stride;
+    int page_next[2], row_next[2];  // of the next unit to be fetched: looked up a unit ahead
+    auto look = [&](int unit) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int token = unit * kRowsUnit + h * 32 + at, nth = token / p.page_size;
+        row_next[h] = token - nth * p.page_size;
+        page_next[h] = unit < g.to && token >= g.lo && token < g.hi ? table[nth] : -2;
+      }
+    };
+    // a thread's own bytes of the ring: nobody else reads them
+    auto mine_at = [&](int slot, int h, int kv, int j) {
+      constexpr int kPiece = VEC * static_cast<int>(sizeof(C));
+      return ring + static_cast<uint32_t>(((((slot * 2 + h) * 2 + kv) * (DPL / VEC) + j) * kRowThreads + tid) * kPiece);
+    };
+    uint32_t gone = 0;  // a bit per token fetched, the last ones lowest: its page is not there
+    int fetched = g.from, slot_in = 0, slot_out = 0;
+    auto fetch = [&]() {
+      gone <<= 2;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool get = page_next[h] >= 0 && page_next[h] < p.pages;
+        if (!get && page_next[h] != -2) gone |= 1u << h;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const C* row = data[kv] + static_cast<int64_t>(get ? page_next[h] : 0) * p.page[kv] + g.head * p.head[kv] + row_next[h] * p.token[kv];
+#pragma unroll
+          for (int j = 0; j < DPL / VEC; ++j) {
+            const int d = (j * 8 + l) * VEC;
+            const bool take = get && d < p.dim;
+            // (zeros where there is nothing)
+            if constexpr (VEC * sizeof(C) == 16)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at(slot_in, h, kv, j)), "l"(take ? row + d : data[kv]), "r"(take ? 16 : 0) : "memory");
+            else if constexpr (kRing)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(mine_at(slot_in, h, kv, j)), "l"(take ? row + d : data[kv]), "r"(take ? static_cast<int>(VEC * sizeof(C)) : 0), "n"(VEC * sizeof(C)) : "memory");
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      slot_in = slot_in + 1 == kSlots ? 0 : slot_in + 1;
+      look(++fetched);
+    };
+    look(g.from);
+    if constexpr (kRing) {
+#pragma unroll 1
+      for (int i = 0; i < kSlots - 1; ++i) fetch();
+    }
 #pragma unroll 1
     for (int unit = g.from; unit < g.to; ++unit) {
       float k[2][DPL], v[2][DPL], ks[2], vs[2];
       int j[2];
       bool there[2], bad[2];
+      if constexpr (kRing) {
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         j[h] = unit * kRowsUnit + h * 32 + at;
         there[h] = j[h] >= g.lo && j[h] < g.hi;
-        bad[h] = false;
-        int64_t page = 0;
-        int nth = 0;
-        if (there[h]) {
-          nth = j[h] / p.page_size;
-          page = p.table[g.s * p.table_stride + nth];
-          nth = j[h] - nth * p.page_size;
-          bad[h] = page < 0 || page >= p.pages;
-        }
-        const bool get = there[h] && !bad[h];
-        load_row<C, DPL, VEC>(data[0] + page * p.page[0] + g.head * p.head[0] + nth * p.token[0], l, p.dim, get, k[h]);
-        load_row<C, DPL, VEC>(data[1] + page * p.page[1] + g.head * p.head[1] + nth * p.token[1], l, p.dim, get, v[h]);
         ks[h] = vs[h] = 1.f;
-        if (kEight && get) {
+        int64_t page;
+        int nth;
+        if constexpr (kRing) {
+          bad[h] = gone >> (2 * (kSlots - 1) + h) & 1;
+#pragma unroll
+          for (int c = 0; c < DPL / VEC; ++c) {
+            load<C, VEC>(reinterpret_cast<const C*>(smem + (mine_at(slot_out, h, 0, c) - smem_base)), k[h] + c * VEC);
+            load<C, VEC>(reinterpret_cast<const C*>(smem + (mine_at(slot_out, h, 1, c) - smem_base)), v[h] + c * VEC);
+          }
+          if (kEight) {
+            nth = j[h] / p.page_size;
+            page = there[h] && !bad[h] ? table[nth] : 0;
+            nth = j[h] - nth * p.page_size;
+          }
+        } else {
+          page = page_next[h];
+          nth = row_next[h];
+          bad[h] = there[h] && (page < 0 || page >= p.pages);
+          const bool get = there[h] && !bad[h];
+          load_row<C, DPL, VEC>(data[0] + page * p.page[0] + g.head * p.head[0] + nth * p.token[0], l, p.dim, get, k[h]);
+          load_row<C, DPL, VEC>(data[1] + page * p.page[1] + g.head * p.head[1] + nth * p.token[1], l, p.dim, get, v[h]);
+        }
+        if (kEight && there[h] && !bad[h]) {
           ks[h] = p.scales[0][page * p.spage[0] + g.head * p.shead[0] + nth * p.stoken[0]];
           vs[h] = p.scales[1][page * p.spage[1] + g.head * p.shead[1] + nth * p.stoken[1]];
         }
       }
+      if constexpr (kRing) slot_out = slot_out + 1 == kSlots ? 0 : slot_out + 1;
+      else look(unit + 1);
       if (kEight) {
 #pragma unroll
         for (int e = 0; e < DPL; ++e) {
@@ -158,6 +231,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(const __grid_const
       }
     }
 
+    if constexpr (kRing) asm volatile("cp.async.wait_group 0;" ::: "memory");  // (what was fetched beyond the end: zeros)
     // the four groups of a warp, then the warps
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -316,26 +390,36 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   out[tid] = ElemTraits<T>::from_float(total == 0.f ? 0.f : all / total);
 }
 
-template <typename T, typename C, int DPL, int VEC>
+template <typename T, typename C, int DPL, int VEC, int R>
 int launch_one(const Attend& a, unsigned grid, cudaStream_t stream) {
-  constexpr size_t smem = kRowThreads / 32 * 64 * 8 * sizeof(float);
-  const cudaError_t err = tc::launch_pdl(rows_kernel<T, C, DPL, VEC>, grid, kRowThreads, smem, stream, a);
+  constexpr size_t smem = kRowThreads / 32 * R * DPL * 8 * sizeof(float) +
+                          (row_ring(VEC, DPL) ? kSlots * 4 * DPL * sizeof(C) * kRowThreads : 0);
+  static std::atomic<uint64_t> ready{0};  // a bit per device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (err == cudaSuccess && !(ready.load(std::memory_order_acquire) & bit)) {
+    err = cudaFuncSetAttribute(rows_kernel<T, C, DPL, VEC, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  }
+  if (err == cudaSuccess) err = tc::launch_pdl(rows_kernel<T, C, DPL, VEC, R>, grid, kRowThreads, smem, stream, a);
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention rows kernel: %s", cudaGetErrorString(err));
   count_launch();
   return KSMM_OK;
 }
 
+template <typename T, typename C, int VEC>
+int launch_vec(const Attend& a, unsigned grid, cudaStream_t stream) {
+  const int dim = a.pool.dim;
+  const bool few = a.tile_rows == kFewRowsTile;
+  if (dim <= 64) return few ? launch_one<T, C, 8, VEC, kFewRowsTile>(a, grid, stream) : launch_one<T, C, 8, VEC, 8>(a, grid, stream);
+  if (dim <= 128) return few ? launch_one<T, C, 16, VEC, kFewRowsTile>(a, grid, stream) : launch_one<T, C, 16, VEC, 4>(a, grid, stream);
+  return launch_one<T, C, 32, VEC, kFewRowsTile>(a, grid, stream);
+}
+
 template <typename T, typename C>
 int launch_typed(const Attend& a, bool vec, unsigned grid, cudaStream_t stream) {
-  const int dim = a.pool.dim;
-  if (vec) {
-    if (dim <= 64) return launch_one<T, C, 8, 4>(a, grid, stream);
-    if (dim <= 128) return launch_one<T, C, 16, 4>(a, grid, stream);
-    return launch_one<T, C, 32, 4>(a, grid, stream);
-  }
-  if (dim <= 64) return launch_one<T, C, 8, 1>(a, grid, stream);
-  if (dim <= 128) return launch_one<T, C, 16, 1>(a, grid, stream);
-  return launch_one<T, C, 32, 1>(a, grid, stream);
+  return vec ? launch_vec<T, C, 4>(a, grid, stream) : launch_vec<T, C, 1>(a, grid, stream);
 }
 
 template <typename T>
@@ -354,7 +438,7 @@ int launch_cached(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t 
 
 }  // namespace
 
-int rows_tile(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 4 : 2; }
+int rows_tile(int dim, int64_t rows) { return rows <= kFewRowsTile || dim > 128 ? kFewRowsTile : dim <= 64 ? 8 : 4; }
 
 int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
   if (dtype == KSMM_F32) return launch_cached<float>(a, cache_dtype, grid, stream);
