@@ -94,7 +94,7 @@ __device__ __forceinline__ Work work_of(const Attend& a, const Sequence& q) {
     w.items = 0;
     return w;
   }
-  w.tiles = static_cast<int>((rows + a.tile_rows - 1) / a.tile_rows);
+  w.tiles = static_cast<int>(divide(rows + a.tile_rows - 1, a.tile_rows));
   // (a sequence without keys is a unit of work as well: its rows are zeros)
   w.units = max(1, units_to(a, q.length) - (first_key(a, q, 0) >> a.unit_log2));
   w.items = static_cast<int64_t>(w.tiles) * a.pool.kv_heads;
@@ -103,166 +103,156 @@ __device__ __forceinline__ Work work_of(const Attend& a, const Sequence& q) {
 
 // A piece of an item, from a block's share.
 struct Segment {
-  Sequence seq;
-  int s, head, tile;
-  int lo, hi;          // the keys that its rows see lie in [lo, hi)
+  int64_t item;        // its number, for the partial results
+  int s, head, tile;   // s < 0: no more segments
+  int start, n;        // the sequence's rows
+  int length;          // its tokens
+  int bad;             // it is longer than its table
+  int lo, hi;          // the keys that the item's rows see lie in [lo, hi)
   int first_position;  // of its first row
   int from, to;        // the units to be gone through, counted from the sequence's first token
   int slot;            // where the result goes: 0 the output, 1 or 2 the block's first or second slot
-  int64_t item;        // its number, for the partial results
 };
 
-// A block's share: `left` units from unit `offset` of sequence s on, counted through its items; in a launch without a split, or of few
-// short sequences, one whole item.
-struct Share {
-  int64_t left, offset;
-  int s;
-  bool whole;
-  Work work;
+constexpr int kWholeUnits = 8;  // items of up to so many units stay whole where there is a block for each: joining parts costs more
+
+// A block's share, walked segment by segment by ONE warp, all lanes alike: as many units of the launch's, counted sequence by sequence
+// and head by head, as every other block's; in a launch without a split, or of few short sequences, one whole item.  The warp hands the
+// segments on: what a segment is takes a chain of reads and divisions (several microseconds where every thread followed it).
+struct Walker {
   Sequence seq;
+  Work work;
+  int s, head, tile, from;
+  int64_t left;  // units, or whole items
+  bool whole;
 
   __device__ void set(const Attend& a, int which) {
     s = which;
     seq = sequence(a.pool, s);
     work = work_of(a, seq);
-    if (whole) work.units = 1;  // (items count as one)
   }
 
-  // the next segment, by one thread or by all alike; false where there is none
-  __device__ bool next(const Attend& a, Segment* g) {
-    if (left <= 0) return false;
-    while (offset >= work.items * work.units) {
-      offset -= work.items * work.units;
-      if (s + 1 >= a.pool.sequences) return false;  // (not reached: the units end with the last sequence's)
-      set(a, s + 1);
+  // A lane sums a run of sequences, the warp forms the runs' prefix sums, and the run that holds the block's first unit is walked by
+  // its lane.  false: nothing to do (a split block then has marked its slots).
+  template <typename Count>
+  __device__ bool start_counted(const Attend& a) {
+    constexpr uint32_t kAll = 0xffffffffu;
+    const int lane = threadIdx.x % 32;
+    const int run = (a.pool.sequences + 31) / 32;
+    const int first = min(lane * run, a.pool.sequences), end = min(first + run, a.pool.sequences);
+    Count units = 0, items = 0;
+    int most = 0;
+#pragma unroll 4
+    for (int i = first; i < end; ++i) {
+      const Work w = work_of(a, sequence(a.pool, i));
+      units += static_cast<Count>(w.items) * w.units;
+      items += static_cast<Count>(w.items);
+      most = max(most, w.units);
     }
-    const int64_t item = divide(offset, work.units);
-    const int from = static_cast<int>(offset - item * work.units);
-    const int to = static_cast<int>(left < work.units - from ? from + left : work.units);
-    left -= to - from;
-    offset += to - from;
-    g->seq = seq;
-    g->s = s;
+    Count units_before = units, items_before = items;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const Count u = __shfl_up_sync(kAll, units_before, d), n = __shfl_up_sync(kAll, items_before, d);
+      if (lane >= d) {
+        units_before += u;
+        items_before += n;
+      }
+    }
+    most = __reduce_max_sync(kAll, most);
+    const int64_t all_units = __shfl_sync(kAll, units_before, 31), all_items = __shfl_sync(kAll, items_before, 31);
+    const int64_t block = blockIdx.x, blocks = gridDim.x;
+    whole = !a.split || (most <= kWholeUnits && all_items <= blocks);
+    int64_t place = block, last = block + 1, mine = items, before = items_before - items;
+    if (!whole) {
+      // (with fewer units than blocks the first all_units blocks have one each)
+      mine = units;
+      before = units_before - units;
+      const int64_t n = min(all_units, blocks);
+      place = block < n ? divide(block * all_units, n) : all_units;
+      last = block < n ? divide((block + 1) * all_units, n) : all_units;
+    }
+    const uint32_t holds = __ballot_sync(kAll, place < last && place >= before && place < before + mine);
+    left = last - place;
+    if (!holds) {
+      if (a.split && lane < 2) a.slots[2 * block + lane] = -1;
+      return false;
+    }
+    int which = 0;
+    int64_t offset = 0;
+    if (holds >> lane & 1) {
+      for (int i = first; i < end; ++i) {
+        const Work w = work_of(a, sequence(a.pool, i));
+        const int64_t n = whole ? w.items : w.items * w.units;
+        if (place < before + n) {
+          which = i;
+          offset = place - before;
+          break;
+        }
+        before += n;
+      }
+    }
+    const int holder = __ffs(holds) - 1;
+    which = __shfl_sync(kAll, which, holder);
+    offset = __shfl_sync(kAll, offset, holder);
+    set(a, which);
+    const int64_t item = whole ? offset : divide(offset, work.units);
+    from = whole ? 0 : static_cast<int>(offset - item * work.units);
     if (a.split) {
-      g->head = static_cast<int>(divide(item, work.tiles));
-      g->tile = static_cast<int>(item - static_cast<int64_t>(g->head) * work.tiles);
+      head = static_cast<int>(divide(item, work.tiles));
+      tile = static_cast<int>(item - static_cast<int64_t>(head) * work.tiles);
     } else {
       // the last tiles of all heads come first: they see the most keys
-      const int64_t tile = divide(item, a.pool.kv_heads);
-      g->head = static_cast<int>(item - tile * a.pool.kv_heads);
-      g->tile = work.tiles - 1 - static_cast<int>(tile);
+      const int64_t t = divide(item, a.pool.kv_heads);
+      head = static_cast<int>(item - t * a.pool.kv_heads);
+      tile = work.tiles - 1 - static_cast<int>(t);
     }
-    const int t0 = static_cast<int>(divide(static_cast<int64_t>(g->tile) * a.tile_rows, a.group));
+    return true;
+  }
+
+  __device__ bool start(const Attend& a) { return a.narrow ? start_counted<int>(a) : start_counted<int64_t>(a); }
+
+  // the next segment; one with s < 0 where there is none
+  __device__ void next(const Attend& a, Segment* g) {
+    g->s = -1;
+    if (left <= 0) return;
+    while (work.items == 0 || head >= a.pool.kv_heads) {
+      if (s + 1 >= a.pool.sequences) return;  // (not reached: the units end with the last sequence's)
+      set(a, s + 1);
+      head = tile = from = 0;
+    }
+    const int to = whole ? work.units : static_cast<int>(left < work.units - from ? from + left : work.units);
+    left -= whole ? 1 : to - from;
+    g->item = (static_cast<int64_t>(s) * a.pool.kv_heads + head) << 32 | tile;
+    g->s = s;
+    g->head = head;
+    g->tile = tile;
+    g->start = seq.start;
+    g->n = seq.n;
+    g->length = seq.length;
+    g->bad = seq.bad;
+    const int t0 = static_cast<int>(divide(static_cast<int64_t>(tile) * a.tile_rows, a.group));
     g->first_position = seq.length - seq.n + t0;
     g->lo = first_key(a, seq, a.split ? 0 : t0);
     g->hi = seq.length;
+    g->from = g->lo >> a.unit_log2;
     if (a.split) {
       // (all tiles of a sequence go through the same units, so that they count the same)
-      g->from = (g->lo >> a.unit_log2) + from;
-      g->to = whole ? max(g->from + 1, units_to(a, seq.length)) : (g->lo >> a.unit_log2) + to;
+      g->to = g->from + to;
+      g->from += from;
     } else {
-      const int64_t t1 = divide(static_cast<int64_t>(g->tile + 1) * a.tile_rows - 1, a.group);
+      const int64_t t1 = divide(static_cast<int64_t>(tile + 1) * a.tile_rows - 1, a.group);
       g->hi = max(seq.length - seq.n + static_cast<int>(t1 < seq.n ? t1 + 1 : seq.n), 0);
-      g->from = (g->lo >> a.unit_log2);
       g->to = units_to(a, g->hi);
     }
     // a block's first segment may continue an item, its last may be continued; one that is both is the first
     g->slot = from == 0 && to == work.units ? 0 : from > 0 ? 1 : 2;
-    g->item = (static_cast<int64_t>(s) * a.pool.kv_heads + g->head) << 32 | g->tile;
-    return true;
+    from = to == work.units ? 0 : to;
+    if (from == 0 && ++tile == work.tiles) {
+      tile = 0;
+      ++head;
+    }
   }
 };
-
-// Every thread of the block: its share.  false: nothing to do (a split block then has marked its slots).  A thread sums a run of
-// sequences, the block forms the runs' prefix sums, and the run that holds the block's first unit is walked by its thread: lengths
-// and starts are read once, side by side.  `shared`: kShareWords values.
-constexpr int kShareWords = 3 * 32 + 2;
-constexpr int kWholeUnits = 8;  // items of up to so many units stay whole where there is a block for each: joining parts costs more
-
-template <int THREADS, typename Count>
-__device__ bool share_counted(const Attend& a, int64_t* shared, Share* r) {
-  constexpr int kWarps = THREADS / 32;
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int run = (a.pool.sequences + THREADS - 1) / THREADS;
-  const int from = min(tid * run, a.pool.sequences), to = min(from + run, a.pool.sequences);
-  Count units = 0, items = 0;
-  int most = 0;
-  for (int i = from; i < to; ++i) {
-    const Work w = work_of(a, sequence(a.pool, i));
-    units += static_cast<Count>(w.items) * w.units;
-    items += static_cast<Count>(w.items);
-    most = max(most, w.units);
-  }
-  Count units_before = units, items_before = items;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const Count u = __shfl_up_sync(0xffffffffu, units_before, d), n = __shfl_up_sync(0xffffffffu, items_before, d);
-    if (lane >= d) {
-      units_before += u;
-      items_before += n;
-    }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
-  }
-  if (lane == 31) {
-    shared[warp] = units_before;
-    shared[32 + warp] = items_before;
-    shared[64 + warp] = most;
-  }
-  if (tid == 0) shared[96] = -1;
-  __syncthreads();
-  int64_t all_units = 0, all_items = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      units_before += static_cast<Count>(shared[w]);
-      items_before += static_cast<Count>(shared[32 + w]);
-    }
-    all_units += shared[w];
-    all_items += shared[32 + w];
-    most = max(most, static_cast<int>(shared[64 + w]));
-  }
-  const int64_t block = blockIdx.x, blocks = gridDim.x;
-  const bool whole = !a.split || (most <= kWholeUnits && all_items <= blocks);
-  int64_t place = block, last = block + 1, total = all_items, mine = items, before = items_before - items;
-  if (!whole) {
-    // (with fewer units than blocks the first all_units blocks have one each)
-    total = all_units;
-    mine = units;
-    before = units_before - units;
-    const int64_t n = min(total, blocks);
-    place = block < n ? divide(block * total, n) : total;
-    last = block < n ? divide((block + 1) * total, n) : total;
-  }
-  if (place < last && place >= before && place < before + mine) {
-    for (int i = from; i < to; ++i) {
-      const Work w = work_of(a, sequence(a.pool, i));
-      const int64_t n = whole ? w.items : w.items * w.units;
-      if (place < before + n) {
-        shared[97] = place - before;
-        shared[96] = i;
-        break;
-      }
-      before += n;
-    }
-  }
-  __syncthreads();
-  const int s = static_cast<int>(shared[96]);
-  r->offset = shared[97];
-  __syncthreads();  // (the caller may use the array again)
-  if (s < 0) {
-    if (a.split && tid < 2) a.slots[2 * block + tid] = -1;
-    return false;
-  }
-  r->left = last - place;
-  r->whole = whole;
-  r->set(a, s);
-  return true;
-}
-
-template <int THREADS>
-__device__ __forceinline__ bool share(const Attend& a, int64_t* shared, Share* r) {
-  return a.narrow ? share_counted<THREADS, int>(a, shared, r) : share_counted<THREADS, int64_t>(a, shared, r);
-}
 
 // Rows of no sequence, as asked for.
 template <typename T>

@@ -38,8 +38,8 @@ struct Prompt {
   // q | k full, k empty, v full, v empty | s, p, o per row tile | a load of its own
   static constexpr int kBars = 1 + 4 * kStages + 3 * kTiles + 1;
   static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
-  static constexpr int kSharedAt = kFlagsAt + 8;
-  static constexpr int kBytes = kSharedAt + kShareWords * 8;
+  static constexpr int kSegmentAt = (kFlagsAt + 8 + 7) / 8 * 8;
+  static constexpr int kBytes = kSegmentAt + static_cast<int>(sizeof(Segment));
   static constexpr int kThreads = 128 * kTiles + (kTiles == 2 ? 128 : 64);  // the last: TMA, MMAs, two warps without work
   static constexpr int kSCols = kKeys;
   static constexpr int kOAt = kTiles * kSCols;
@@ -126,10 +126,14 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   grid_dep_wait();
   grid_dep_launch();
   clear_rest<T>(a);
-  Share mine;
-  Segment g;
-  if (!share<C::kThreads>(a, reinterpret_cast<int64_t*>(smem + C::kSharedAt), &mine)) return;
-  mine.next(a, &g);
+  Segment* segment = reinterpret_cast<Segment*>(smem + C::kSegmentAt);
+  if (warp == 0) {
+    Walker walker;
+    Segment next;
+    next.s = -1;
+    if (walker.start(a)) walker.next(a, &next);
+    if (lane == 0) *segment = next;
+  }
   if (warp == kIssuer) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
@@ -138,14 +142,19 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const Segment g = *segment;
+  if (g.s < 0) {
+    if (warp == kIssuer) tmem_dealloc(tmem, 512);
+    return;
+  }
 
   // tiles of keys: [first, first + count[t]) for row tile t
   const int first = g.lo / C::kKeys, token0 = g.tile * C::kTiles * args.tile_tokens;
   int count[C::kTiles], most = 0;
 #pragma unroll
   for (int t = 0; t < C::kTiles; ++t) {
-    const int from = token0 + t * args.tile_tokens, to = min(from + args.tile_tokens, g.seq.n);
-    const int hi = from < g.seq.n ? max(g.seq.length - g.seq.n + to, 0) : 0;
+    const int from = token0 + t * args.tile_tokens, to = min(from + args.tile_tokens, g.n);
+    const int hi = from < g.n ? max(g.length - g.n + to, 0) : 0;
     count[t] = max((hi + C::kKeys - 1) / C::kKeys - first, 0);
     most = max(most, count[t]);
   }
@@ -157,10 +166,10 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * C::kSCols, o_at = tmem + lanes + C::kOAt + t * DP;
     const int token = token0 + t * args.tile_tokens + r / a.group;
-    const bool live = r < args.tile_tokens * a.group && token < g.seq.n;
-    const int position = g.seq.length - g.seq.n + token;
+    const bool live = r < args.tile_tokens * a.group && token < g.n;
+    const int position = g.length - g.n + token;
     const int mine_count = t == 0 ? count[0] : count[C::kTiles - 1];
-    const int sure = g.seq.length - g.seq.n + token0 + t * args.tile_tokens + 1;  // keys below are seen by all rows of the tile
+    const int sure = g.length - g.n + token0 + t * args.tile_tokens + 1;  // keys below are seen by all rows of the tile
     const int64_t clear = a.window ? static_cast<int64_t>(sure) - 1 + args.tile_tokens - a.window : 0;  // so are keys from here on
     const int boxes = C::kKeys / args.box;
     float top = kNone, sum = 0.f;
@@ -250,9 +259,9 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     if (mine_count > 0 && alive)
       alive = __all_sync(0xffffffffu, mbar_wait<20>(o_full(t), 0, abort_flag, a.status, kPromptWaits + 4));
     tc_fence_after();
-    T* to = reinterpret_cast<T*>(a.out) + static_cast<int64_t>(g.seq.start + token) * a.out_token +
+    T* to = reinterpret_cast<T*>(a.out) + static_cast<int64_t>(g.start + token) * a.out_token +
             static_cast<int64_t>(g.head * a.group + r % a.group) * a.out_head;
-    if (g.seq.bad || !alive) sum = __int_as_float(0x7fffffff);
+    if (g.bad || !alive) sum = __int_as_float(0x7fffffff);
     const float f = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
     for (int c = 0; c < DP; c += 32) {
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
 #pragma unroll
           for (int b = 0; b < C::kBoxes; ++b)
             tma_load_3d(base + t * C::kQ + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group,
-                        g.seq.start + token0 + t * args.tile_tokens);
+                        g.start + token0 + t * args.tile_tokens);
       }
       int page_ahead = -2, ahead = 0;
       int loaded_k = 0, loaded_v = 0, lone = 0;

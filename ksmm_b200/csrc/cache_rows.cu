@@ -61,7 +61,7 @@ template <typename T, typename C, int DPL, int VEC, int R>
 __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kernel(const __grid_constant__ Attend a) {
   constexpr bool kEight = sizeof(C) == 1;
   constexpr bool kRing = row_ring(VEC, DPL);
-  __shared__ int64_t shared[kShareWords];
+  __shared__ Segment segment;
   __shared__ float stats[2][kRowThreads / 32][R];
   extern __shared__ __align__(16) char smem[];
   float* sums = reinterpret_cast<float*>(smem);  // [warp][R][8 DPL]
@@ -69,24 +69,33 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   clear_rest<T>(a);
-  Share mine;
-  if (!share<kRowThreads>(a, shared, &mine)) return;
+  Walker walker;  // the first warp's
+  bool some = true;
+  if (threadIdx.x < 32) some = walker.start(a);
+  if (!__syncthreads_or(threadIdx.x < 32 && some)) return;
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, l = lane % 8, at = warp * 4 + lane / 8;
   const T* q_rows = reinterpret_cast<const T*>(a.q);
   const C* data[2] = {reinterpret_cast<const C*>(p.data[0]), reinterpret_cast<const C*>(p.data[1])};
 
-  Segment g;
   bool slot_used[2] = {false, false};
-  while (mine.next(a, &g)) {
-    const int rows = min(R, g.seq.n * a.group - g.tile * R);
+  while (true) {
+    if (warp == 0) {
+      Segment next;
+      walker.next(a, &next);
+      if (lane == 0) segment = next;
+    }
+    __syncthreads();
+    const Segment g = segment;
+    if (g.s < 0) break;
+    const int rows = min(R, g.n * a.group - g.tile * R);
     float q[R][DPL], o[R][DPL], m[R], sum[R];
     int position[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = g.tile * R + r, t = row / a.group;
-      position[r] = r < rows ? g.seq.length - g.seq.n + t : -1;
-      const int64_t from = (g.seq.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
+      position[r] = r < rows ? g.length - g.n + t : -1;
+      const int64_t from = (g.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
       load_row<T, DPL, VEC>(q_rows + from, l, p.dim, r < rows, q[r]);
       m[r] = kNone;
       sum[r] = 0.f;
@@ -274,7 +283,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
         total = fmaf(f, stats[1][w][r], total);
         out = fmaf(f, sums[(w * R + r) * 8 * DPL + d], out);
       }
-      if (g.seq.bad) total = __int_as_float(0x7fffffff);
+      if (g.bad) total = __int_as_float(0x7fffffff);
       if (slot) {
         part[i] = out;
         if (d == 0) {
@@ -283,7 +292,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
         }
       } else {
         const int row = g.tile * R + r, t = row / a.group;
-        reinterpret_cast<T*>(a.out)[(g.seq.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head + d] =
+        reinterpret_cast<T*>(a.out)[(g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head + d] =
             ElemTraits<T>::from_float(total == 0.f ? 0.f : out / total);
       }
     }

@@ -50,13 +50,15 @@ struct Layout {
   static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kBlocks = DP == 256 ? 1 : 2;                     // on an SM
   static constexpr int kStages = 196608 / kBlocks / (kStageBytes + kScales);
-  static constexpr int kMerge = kCols / 2 * 32 * 4;                     // a warp's output
+  static constexpr int kMerge = kCols / 2 * 32 * 4;                     // a warp's output; half of it where there are up to 8 rows
   static constexpr int kMergeAt = kStages * kStageBytes;
-  static constexpr int kScalesAt = kMergeAt + 2 * kHalves * kMerge;
-  static constexpr int kStatsAt = kScalesAt + kStages * kScales;        // of the merges: 2 x 4 x 8 floats a half
-  static constexpr int kBarsAt = kStatsAt + kHalves * 2 * 4 * 8 * 4;
-  static constexpr int kFlagsAt = kBarsAt + 2 * kStages * 8;
-  static constexpr int kQRow = DP * 2 + 16;                             // bytes of a row of q in shared memory
+  static constexpr int kScalesAt = kMergeAt + kHalves * kMerge;
+  static constexpr int kQRow = DP * 2 + 16;                             // bytes of a row of q (and no two rows on the same banks)
+  static constexpr int kQAt = kScalesAt + kStages * kScales;
+  static constexpr int kStatsAt = kQAt + kTileRows * kQRow;             // of the merges: 2 x 4 x 8 floats a half
+  static constexpr int kBarsAt = kStatsAt + kHalves * 2 * 4 * 8 * 4;    // full, empty | a segment full, empty
+  static constexpr int kSegmentAt = kBarsAt + (2 * kStages + 2) * 8;
+  static constexpr int kFlagsAt = kSegmentAt + static_cast<int>(sizeof(Segment));
   static constexpr int kBytes = kFlagsAt + kStages * 4 + 4;
   static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
   static_assert(kStages >= 2, "a ring");
@@ -118,6 +120,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// a barrier of the consumers that tells all whether one says so
+template <int THREADS>
+__device__ __forceinline__ bool any_of(bool v) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(v ? 1u : 0u), "n"(THREADS)
+               : "memory");
+  return r != 0;
+}
+
 // A place in the ring.
 template <int STAGES>
 struct Turn {
@@ -140,7 +153,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
   using H = typename std::conditional<EIGHT, __half, T>::type;  // of the products
   // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
   constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
-  // q in shared memory where registers do not hold it and the output
+  // q stays in shared memory where registers do not hold it beside the output
   constexpr bool kQShared = DP == 256;
   constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
   extern __shared__ __align__(1024) char smem[];
@@ -148,7 +161,8 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   int* flags = reinterpret_cast<int*>(smem + L::kFlagsAt);
   volatile int* abort_flag = flags + L::kStages;
-  const uint32_t full = base + L::kBarsAt, empty = full + 8 * L::kStages;
+  const uint32_t full = base + L::kBarsAt, empty = full + 8 * L::kStages, segment_full = empty + 8 * L::kStages, segment_empty = segment_full + 8;
+  Segment* const segment = reinterpret_cast<Segment*>(smem + L::kSegmentAt);
   if (base % 1024) {  // (without static shared memory it starts there; swizzled tiles need it)
     if (tid == 0) atomicCAS(a.status, 0, kWaits + 3);
     return;
@@ -159,8 +173,11 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, L::kConsumers);
     }
+    mbar_init(segment_full, 1);
+    mbar_init(segment_empty, L::kConsumers);
     fence_mbar_init();
   }
+  for (int i = tid; i < kTileRows * L::kQRow / 4; i += L::kThreads) reinterpret_cast<uint32_t*>(smem + L::kQAt)[i] = 0;
   if (warp == L::kConsumers && lane == 0) {
     prefetch_tensormap(&maps.keys);
     prefetch_tensormap(&maps.values);
@@ -168,12 +185,11 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
   grid_dep_wait();
   grid_dep_launch();
   clear_rest<T>(a);
-  Share mine;
-  if (!share<L::kThreads>(a, reinterpret_cast<int64_t*>(smem + L::kMergeAt), &mine)) return;
+  __syncthreads();
   const Pool& p = a.pool;
   const int box = 1 << box_log2, box_bytes = box * 128;
   Turn<L::kStages> turn;
-  Segment g;
+  uint32_t segments = 0;  // so far
 
   if (warp == L::kConsumers) {
     // ---------------- producer: the warp walks the loop, tables 32 boxes ahead, one lane issues ----------------
@@ -182,9 +198,38 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
     const bool one = elect_one();
     uint32_t issued = 0;
     bool alive = true;
-    while (alive && mine.next(a, &g)) {
+    Walker walker;
+    bool more = walker.start(a);
+    while (alive) {
+      Segment g;
+      g.s = -1;
+      if (more) walker.next(a, &g);
+      more = more && g.s >= 0;
+      // hand it on, with its rows of q
+      alive = __all_sync(0xffffffffu, mbar_wait<20>(segment_empty, (segments & 1) ^ 1, abort_flag, a.status, kWaits));
+      if (!alive) break;
+      if (more) {
+        const int rows = min(kTileRows, g.n * a.group - g.tile * kTileRows);
+        const int row = g.tile * kTileRows + min(lane, rows - 1), t = row / a.group;
+        const int64_t row_at = (g.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+          const T* from = reinterpret_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, row_at, r);
+#pragma unroll
+          for (int d = 0; d < DP; d += 64) {
+            const int at = d + 2 * lane;
+            if (at < p.dim) *reinterpret_cast<uint32_t*>(smem + L::kQAt + r * L::kQRow + at * 2) = *reinterpret_cast<const uint32_t*>(from + at);
+          }
+        }
+      }
+      if (lane == 0) *segment = g;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(segment_full);
+      ++segments;
+      if (!more) break;
+      int batch = 0;
       const int32_t* table = p.table + g.s * p.table_stride;
-      int row_ahead = 0, page_ahead = -1, batch = 0;
+      int row_ahead = 0, page_ahead = -1;
       for (int u = g.from; u < g.to; ++u) {
         if (batch == 0) {
           // the pages of the next 32 boxes
@@ -248,7 +293,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
   bool alive = true;
   bool slot_used[2] = {false, false};
   const int run = warp % L::kRuns, half = warp / L::kRuns;
-  float* merge = reinterpret_cast<float*>(smem + L::kMergeAt + half * 2 * L::kMerge);
+  float* merge = reinterpret_cast<float*>(smem + L::kMergeAt + half * L::kMerge);
   float* stats = reinterpret_cast<float*>(smem + L::kStatsAt) + half * 2 * 4 * 8;
   // lane's row and chunk in the loads of four matrices: K: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1;
   // V: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1
@@ -261,28 +306,43 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
     const int t = run * L::kStep + i * 16, b = t >> box_log2;
     group_at[i] = b * box_bytes * L::kBoxes + (t - (b << box_log2)) * 128;
   }
-  while (mine.next(a, &g)) {
-    const int rows = min(kTileRows, g.seq.n * a.group - g.tile * kTileRows);
+  while (true) {
+    alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(segment_full, segments & 1, abort_flag, a.status, kWaits + 2));
+    // (one that gave up takes all with it: nobody is left at a barrier.  And the last segment's merges have been read)
+    if (any_of<L::kConsumers * 32>(!alive)) {
+      alive = false;
+      break;
+    }
+    ++segments;
+    const Segment g = *segment;
+    if (g.s < 0) break;
+    const int rows = min(kTileRows, g.n * a.group - g.tile * kTileRows);
+    const bool upper = rows > 8;  // whether a lane's second row is one
     uint32_t qf[DP / 16][4];
     float m[2], sum[2], row_scale[2], vm = 0.f;
     int position[2];
     float o[L::kCols / 8][4];
+    // (8-bit chunks: elements 4 q4 + 2 e and the next instead of 2 q4 + 8 e)
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      if constexpr (EIGHT) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 v = *reinterpret_cast<const uint2*>(smem + L::kQAt + (gq + 8 * h) * L::kQRow + (c * 16 + 4 * q4) * 2);
+          qf[c][h] = v.x;
+          qf[c][h + 2] = v.y;
+        }
+      } else if constexpr (!kQShared) {
+        ldmatrix4(qf[c], base + L::kQAt + v_row * L::kQRow + v_chunk * 16 + c * 32);
+      }
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = gq + 8 * h, row = g.tile * kTileRows + r, t = row / a.group;
-      position[h] = r < rows ? g.seq.length - g.seq.n + t : INT_MAX;  // (a row that is not there masks nothing)
+      const int r = gq + 8 * h;
+      position[h] = r < rows ? g.length - g.n + (g.tile * kTileRows + r) / a.group : INT_MAX;  // (a row that is not there masks nothing)
       m[h] = kNone;
       sum[h] = 0.f;
       row_scale[h] = a.scale;
-      const T* from = reinterpret_cast<const T*>(a.q) + (g.seq.start + t) * a.q_token +
-                      (g.head * a.group + row - t * a.group) * a.q_head;
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = c * 16 + (EIGHT ? 4 * q4 + 2 * e : 2 * q4 + 8 * e);
-          qf[c][h + 2 * e] = r < rows && d < p.dim ? *reinterpret_cast<const uint32_t*>(from + d) : 0u;
-        }
       if constexpr (EIGHT && ElemTraits<T>::kDtype == KSMM_BF16) {
         float top = 0.f;
 #pragma unroll
@@ -313,19 +373,23 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
-    if constexpr (kQShared) {
-      // (one warp for all; the region is the merges', whose last reads are over)
+    if constexpr (kQShared && EIGHT) {
+      // in the order of the chunks, and in fp16; one warp for all
       bar_sync_named(1, L::kConsumers * 32);
       if (warp == 0) {
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint32_t*>(smem + L::kMergeAt + (gq + 8 * (e % 2)) * L::kQRow + (c * 16 + 2 * q4 + 8 * (e / 2)) * 2) = qf[c][e];
+            *reinterpret_cast<uint32_t*>(smem + L::kQAt + (gq + 8 * (e % 2)) * L::kQRow + (c * 16 + 2 * q4 + 8 * (e / 2)) * 2) = qf[c][e];
       }
       bar_sync_named(1, L::kConsumers * 32);
     }
-    const uint32_t q_at = base + L::kMergeAt + v_row * L::kQRow + v_chunk * 16;
+    if constexpr (!kQShared) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(segment_empty);
+    }
+    const uint32_t q_at = base + L::kQAt + v_row * L::kQRow + v_chunk * 16;
     // tokens from `clear` to below `sure` are seen by every row
     const int sure = g.first_position + 1;
     const int64_t clear = a.window ? static_cast<int64_t>(g.hi) - a.window : 0;
@@ -411,6 +475,8 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
         float scale_o[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          scale_o[h] = 1.f;
+          if (h == 1 && !upper) continue;
           float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
           for (int i = 1; i < 2 * G; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
@@ -518,6 +584,11 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       turn.next();
     }
 
+    if constexpr (kQShared) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(segment_empty);
+    }
+
     // ---- the four runs' results: 2 and 3 to 0 and 1, then 1 to 0; a lane meets the same lane ----
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -530,47 +601,67 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] *= vm;
     }
-    auto give = [&](int buffer) {
-      float* to = merge + buffer * (L::kCols / 2 * 32) + lane;
+    // (with up to 8 rows a lane has half as much to give, and two warps' fit the buffer)
+    auto give = [&](int place) {
+      float* to = merge + (upper ? 0 : place) * (L::kCols / 4 * 32) + lane;
 #pragma unroll
       for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[(4 * i + e) * 32] = o[i][e];
+        for (int e = 0; e < 2; ++e) {
+          to[(2 * i + e) * 32] = o[i][e];
+          if (upper) to[(L::kCols / 4 + 2 * i + e) * 32] = o[i][2 + e];
+        }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (q4) continue;
-        stats[(buffer * 4 + h) * 8 + gq] = m[h];
-        stats[(buffer * 4 + 2 + h) * 8 + gq] = sum[h];
+        stats[(place * 4 + h) * 8 + gq] = m[h];
+        stats[(place * 4 + 2 + h) * 8 + gq] = sum[h];
       }
     };
-    auto take = [&](int buffer) {
-      const float* from = merge + buffer * (L::kCols / 2 * 32) + lane;
+    auto take = [&](int place) {
+      const float* from = merge + (upper ? 0 : place) * (L::kCols / 4 * 32) + lane;
       float mine_f[2], other_f[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float other = stats[(buffer * 4 + h) * 8 + gq], top = fmaxf(m[h], other);
+        const float other = stats[(place * 4 + h) * 8 + gq], top = fmaxf(m[h], other);
         mine_f[h] = exp2_fast(m[h] - top);
         other_f[h] = exp2_fast(other - top);
         m[h] = top;
-        sum[h] = sum[h] * mine_f[h] + stats[(buffer * 4 + 2 + h) * 8 + gq] * other_f[h];
+        sum[h] = sum[h] * mine_f[h] + stats[(place * 4 + 2 + h) * 8 + gq] * other_f[h];
       }
 #pragma unroll
       for (int i = 0; i < L::kCols / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * mine_f[e / 2] + from[(4 * i + e) * 32] * other_f[e / 2];
+        for (int e = 0; e < 2; ++e) {
+          o[i][e] = o[i][e] * mine_f[0] + from[(2 * i + e) * 32] * other_f[0];
+          if (upper) o[i][2 + e] = o[i][2 + e] * mine_f[1] + from[(L::kCols / 4 + 2 * i + e) * 32] * other_f[1];
+        }
     };
-    bar_sync_named(1, L::kConsumers * 32);  // (the last segment's have been read)
-    if (run >= 2) give(run - 2);
-    bar_sync_named(1, L::kConsumers * 32);
-    if (run < 2) take(run);
-    bar_sync_named(1, L::kConsumers * 32);
-    if (run == 1) give(0);
-    bar_sync_named(1, L::kConsumers * 32);
+    auto meet = [&]() { bar_sync_named(1, L::kConsumers * 32); };
+    if (upper) {
+      if (run == 3) give(1);
+      meet();
+      if (run == 2) take(1);
+      meet();
+      if (run == 1) give(1);
+      meet();
+      if (run == 0) take(1);
+      meet();
+      if (run == 2) give(0);
+      meet();
+    } else {
+      if (run >= 2) give(run - 2);
+      meet();
+      if (run < 2) take(run);
+      meet();
+      if (run == 1) give(0);
+      meet();
+    }
     const int slot = g.slot;
     if (slot) slot_used[slot - 1] = true;
     if (run != 0) continue;
     take(0);
-    if (g.seq.bad || !alive) sum[0] = sum[1] = __int_as_float(0x7fffffff);
+    if (g.bad || !alive) sum[0] = sum[1] = __int_as_float(0x7fffffff);
     if (slot && warp == 0 && lane == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
     float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + slot - 1) * kTileRows * (p.dim + 2);
 #pragma unroll
@@ -578,7 +669,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       const int r = gq + 8 * h;
       if (r >= rows) continue;
       const int row = g.tile * kTileRows + r, t = row / a.group;
-      T* to = reinterpret_cast<T*>(a.out) + (g.seq.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
+      T* to = reinterpret_cast<T*>(a.out) + (g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
       const float f = slot ? 1.f : sum[h] == 0.f ? 0.f : 1.f / sum[h];
       if (slot && q4 == 0 && half == 0) {
         to_part[kTileRows * p.dim + r] = m[h];
@@ -595,6 +686,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       }
     }
   }
+  if (!alive && a.split && tid < 2) slot_used[tid] = false;
   if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
 }
 
