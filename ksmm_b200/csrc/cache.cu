@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2) append_kernel(const __grid_
   constexpr int PIECES = VEC == 1 ? 4 : 1;
   constexpr int kWarps = kAppendThreads / 32;
   __shared__ __align__(16) float2 turns[VEC == 1 ? 1 : kWarps][kMaxDim / 2];
+  touch_parameters(a);
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   const Pool& p = a.pool;

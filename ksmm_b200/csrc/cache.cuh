@@ -254,6 +254,15 @@ struct Walker {
   }
 };
 
+// Reads a word of every 64 bytes of a kernel's parameters, before the wait for the kernel before it: the first use of each such piece
+// otherwise waits for it alone, one after the other, in the chain that starts a block.
+template <typename P>
+__device__ __forceinline__ void touch_parameters(const P& parameters) {
+  const int* words = reinterpret_cast<const int*>(&parameters);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(P) / 4); i += 16) asm volatile("" ::"r"(words[i]));
+}
+
 // Rows of no sequence, as asked for.
 template <typename T>
 __device__ void clear_rest(const Attend& a) {

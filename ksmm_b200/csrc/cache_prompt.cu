@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     prefetch_tensormap(&maps.keys);
     prefetch_tensormap(&maps.values);
   }
+  touch_parameters(args);
   grid_dep_wait();
   grid_dep_launch();
   clear_rest<T>(a);

@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
   extern __shared__ __align__(16) char smem[];
   float* sums = reinterpret_cast<float*>(smem);  // [warp][R][8 DPL]
   const uint32_t smem_base = tc::smem_u32(smem), ring = smem_base + kRowThreads / 32 * R * 8 * DPL * sizeof(float);
+  touch_parameters(a);
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   clear_rest<T>(a);
@@ -314,6 +315,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   __shared__ float weight[kMaxBlocks];
   __shared__ float reduce[2][kWarps];
   __shared__ float sums[kWarps][kMaxDim];
+  touch_parameters(a);
   tc::grid_dep_wait();
   tc::grid_dep_launch();
   const Pool& p = a.pool;

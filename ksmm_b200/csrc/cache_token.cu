@@ -50,13 +50,13 @@ struct Layout {
   static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kBlocks = DP == 256 ? 1 : 2;                     // on an SM
   static constexpr int kStages = 196608 / kBlocks / (kStageBytes + kScales);
-  static constexpr int kMerge = kCols / 2 * 32 * 4;                     // a warp's output; half of it where there are up to 8 rows
+  static constexpr int kMerge = kRuns * 4 * kCols * 4;                  // the runs' output for 4 rows, or part of it for more
   static constexpr int kMergeAt = kStages * kStageBytes;
   static constexpr int kScalesAt = kMergeAt + kHalves * kMerge;
   static constexpr int kQRow = DP * 2 + 16;                             // bytes of a row of q (and no two rows on the same banks)
   static constexpr int kQAt = kScalesAt + kStages * kScales;
-  static constexpr int kStatsAt = kQAt + kTileRows * kQRow;             // of the merges: 2 x 4 x 8 floats a half
-  static constexpr int kBarsAt = kStatsAt + kHalves * 2 * 4 * 8 * 4;    // full, empty | a segment full, empty
+  static constexpr int kStatsAt = kQAt + kTileRows * kQRow;             // of the runs: maxima and sums of 16 rows, a half
+  static constexpr int kBarsAt = kStatsAt + kHalves * kRuns * 2 * kTileRows * 4;    // full, empty | a segment full, empty
   static constexpr int kSegmentAt = kBarsAt + (2 * kStages + 2) * 8;
   static constexpr int kFlagsAt = kSegmentAt + static_cast<int>(sizeof(Segment));
   static constexpr int kBytes = kFlagsAt + kStages * 4 + 4;
@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
     prefetch_tensormap(&maps.keys);
     prefetch_tensormap(&maps.values);
   }
+  touch_parameters(a);
   grid_dep_wait();
   grid_dep_launch();
   clear_rest<T>(a);
@@ -205,6 +206,16 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       g.s = -1;
       if (more) walker.next(a, &g);
       more = more && g.s >= 0;
+      const int32_t* table = p.table + g.s * p.table_stride;
+      int row_ahead = 0, page_ahead = -1, batch = 0;
+      auto look = [&](int u) {
+        // the pages of the next 32 boxes
+        const int token = u * L::kTokens + (lane << box_log2), nth = token / p.page_size;
+        const bool there = token < g.hi && token + box > g.lo;
+        page_ahead = there ? table[nth] : -2;  // -2: nothing to load, -1 or beyond the pool: a page that is not there
+        row_ahead = token - nth * p.page_size;
+      };
+      if (more) look(g.from);
       // hand it on, with its rows of q
       alive = __all_sync(0xffffffffu, mbar_wait<20>(segment_empty, (segments & 1) ^ 1, abort_flag, a.status, kWaits));
       if (!alive) break;
@@ -227,17 +238,10 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       if (lane == 0) mbar_arrive(segment_full);
       ++segments;
       if (!more) break;
-      int batch = 0;
-      const int32_t* table = p.table + g.s * p.table_stride;
-      int row_ahead = 0, page_ahead = -1;
       for (int u = g.from; u < g.to; ++u) {
         if (batch == 0) {
-          // the pages of the next 32 boxes
-          const int token = u * L::kTokens + (lane << box_log2), nth = token / p.page_size;
-          const bool there = token < g.hi && token + box > g.lo;
-          page_ahead = there ? table[nth] : -2;  // -2: nothing to load, -1: a page that is not there
-          if (there && (page_ahead < 0 || page_ahead >= p.pages)) page_ahead = -1;
-          row_ahead = token - nth * p.page_size;
+          if (u > g.from) look(u);
+          if (page_ahead >= p.pages || page_ahead < -2) page_ahead = -1;
         }
         const bool of_unit = lane >= batch && lane < batch + boxes;
         const uint32_t missing = __ballot_sync(0xffffffffu, of_unit && page_ahead == -1) >> batch;
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
   bool slot_used[2] = {false, false};
   const int run = warp % L::kRuns, half = warp / L::kRuns;
   float* merge = reinterpret_cast<float*>(smem + L::kMergeAt + half * L::kMerge);
-  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt) + half * 2 * 4 * 8;
+  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt) + half * L::kRuns * 2 * kTileRows;
   // lane's row and chunk in the loads of four matrices: K: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1;
   // V: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1
   const int k_row = (lane / 16) * 8 + lane % 8, k_chunk = lane / 8 % 2;
@@ -589,11 +593,16 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       if (lane == 0) mbar_arrive(segment_empty);
     }
 
-    // ---- the four runs' results: 2 and 3 to 0 and 1, then 1 to 0; a lane meets the same lane ----
+    // ---- the four runs' results, in pieces of the columns that the buffer holds for all rows: every warp gives, then every
+    // thread joins some pairs of neighbours and writes them ----
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+      if (q4 == 0) {
+        stats[(run * 2) * kTileRows + gq + 8 * h] = m[h];
+        stats[(run * 2 + 1) * kTileRows + gq + 8 * h] = !alive || g.bad ? __int_as_float(0x7fffffff) : sum[h];
+      }
     }
     if (EIGHT) {
 #pragma unroll
@@ -601,90 +610,67 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] *= vm;
     }
-    // (with up to 8 rows a lane has half as much to give, and two warps' fit the buffer)
-    auto give = [&](int place) {
-      float* to = merge + (upper ? 0 : place) * (L::kCols / 4 * 32) + lane;
+    if (g.slot) {
+      slot_used[g.slot - 1] = true;
+      if (tid == 0) a.slots[2 * blockIdx.x + g.slot - 1] = g.item;
+    }
+    float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + g.slot - 1) * kTileRows * (p.dim + 2);
+    // CAP: rows that fit, a power of two
+    auto join = [&](auto cap) {
+      constexpr int CAP = decltype(cap)::value, W = L::kMerge / 4 / 4 / CAP, kPieces = L::kCols / W;  // columns of a piece
+      // (rows side by side in a store are moved by eight columns against each other: other banks)
+      auto place = [&](int of_run, int r, int col) { return merge + (of_run * CAP + r) * W + (col ^ (r & 3) * 8 % W); };
 #pragma unroll
-      for (int i = 0; i < L::kCols / 8; ++i)
+      for (int piece = 0; piece < kPieces; ++piece) {
+        if (piece) bar_sync_named(1, L::kConsumers * 32);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          to[(2 * i + e) * 32] = o[i][e];
-          if (upper) to[(L::kCols / 4 + 2 * i + e) * 32] = o[i][2 + e];
+        for (int h = 0; h < 2; ++h) {
+          const int r = gq + 8 * h;
+          if (8 * h >= CAP || r >= CAP) continue;
+          // (8-bit chunks have their even and odd columns in two tiles)
+#pragma unroll
+          for (int i = piece * (W / 8); i < (piece + 1) * (W / 8); i += EIGHT ? 2 : 1) {
+            const int col = i * 8 - piece * W;
+            if constexpr (EIGHT)
+              *reinterpret_cast<float4*>(place(run, r, col + 4 * q4)) = make_float4(o[i][2 * h], o[i + 1][2 * h], o[i][2 * h + 1], o[i + 1][2 * h + 1]);
+            else
+              *reinterpret_cast<float2*>(place(run, r, col + 2 * q4)) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+          }
         }
+        bar_sync_named(1, L::kConsumers * 32);
+        for (int e = run * 32 + lane; e < rows * (W / 2); e += L::kRuns * 32) {
+          const int r = e / (W / 2), col = e % (W / 2) * 2, d = half * L::kCols + piece * W + col;
+          float f[L::kRuns], top = stats[r];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (q4) continue;
-        stats[(place * 4 + h) * 8 + gq] = m[h];
-        stats[(place * 4 + 2 + h) * 8 + gq] = sum[h];
+          for (int k = 1; k < L::kRuns; ++k) top = fmaxf(top, stats[2 * k * kTileRows + r]);
+          float total = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+          for (int k = 0; k < L::kRuns; ++k) {
+            f[k] = exp2_fast(stats[2 * k * kTileRows + r] - top);
+            total = fmaf(stats[(2 * k + 1) * kTileRows + r], f[k], total);
+            const float2 v = *reinterpret_cast<const float2*>(place(k, r, col));
+            x = fmaf(v.x, f[k], x);
+            y = fmaf(v.y, f[k], y);
+          }
+          if (d >= p.dim) continue;
+          if (g.slot) {
+            *reinterpret_cast<float2*>(to_part + r * p.dim + d) = make_float2(x, y);
+            if (d == 0) {
+              to_part[kTileRows * p.dim + r] = top;
+              to_part[kTileRows * (p.dim + 1) + r] = total;
+            }
+          } else {
+            const int row = g.tile * kTileRows + r, t = row / a.group;
+            const float back = total == 0.f ? 0.f : 1.f / total;
+            T* to = reinterpret_cast<T*>(a.out) + (g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
+            *reinterpret_cast<uint32_t*>(to + d) = pack<T>(x * back, y * back);
+          }
+        }
       }
     };
-    auto take = [&](int place) {
-      const float* from = merge + (upper ? 0 : place) * (L::kCols / 4 * 32) + lane;
-      float mine_f[2], other_f[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float other = stats[(place * 4 + h) * 8 + gq], top = fmaxf(m[h], other);
-        mine_f[h] = exp2_fast(m[h] - top);
-        other_f[h] = exp2_fast(other - top);
-        m[h] = top;
-        sum[h] = sum[h] * mine_f[h] + stats[(place * 4 + 2 + h) * 8 + gq] * other_f[h];
-      }
-#pragma unroll
-      for (int i = 0; i < L::kCols / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          o[i][e] = o[i][e] * mine_f[0] + from[(2 * i + e) * 32] * other_f[0];
-          if (upper) o[i][2 + e] = o[i][2 + e] * mine_f[1] + from[(L::kCols / 4 + 2 * i + e) * 32] * other_f[1];
-        }
-    };
-    auto meet = [&]() { bar_sync_named(1, L::kConsumers * 32); };
-    if (upper) {
-      if (run == 3) give(1);
-      meet();
-      if (run == 2) take(1);
-      meet();
-      if (run == 1) give(1);
-      meet();
-      if (run == 0) take(1);
-      meet();
-      if (run == 2) give(0);
-      meet();
-    } else {
-      if (run >= 2) give(run - 2);
-      meet();
-      if (run < 2) take(run);
-      meet();
-      if (run == 1) give(0);
-      meet();
-    }
-    const int slot = g.slot;
-    if (slot) slot_used[slot - 1] = true;
-    if (run != 0) continue;
-    take(0);
-    if (g.bad || !alive) sum[0] = sum[1] = __int_as_float(0x7fffffff);
-    if (slot && warp == 0 && lane == 0) a.slots[2 * blockIdx.x + slot - 1] = g.item;
-    float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + slot - 1) * kTileRows * (p.dim + 2);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = gq + 8 * h;
-      if (r >= rows) continue;
-      const int row = g.tile * kTileRows + r, t = row / a.group;
-      T* to = reinterpret_cast<T*>(a.out) + (g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
-      const float f = slot ? 1.f : sum[h] == 0.f ? 0.f : 1.f / sum[h];
-      if (slot && q4 == 0 && half == 0) {
-        to_part[kTileRows * p.dim + r] = m[h];
-        to_part[kTileRows * (p.dim + 1) + r] = sum[h];
-      }
-      // pairs of neighbours: 8-bit chunks have them in the two tiles
-#pragma unroll
-      for (int i = 0; i < L::kCols / 8; ++i) {
-        const int d = half * L::kCols + (EIGHT ? i / 2 * 16 + 4 * q4 + 2 * (i % 2) : i * 8 + 2 * q4);
-        const float x = EIGHT ? o[i / 2 * 2][2 * h + i % 2] : o[i][2 * h], y = EIGHT ? o[i / 2 * 2 + 1][2 * h + i % 2] : o[i][2 * h + 1];
-        if (d >= p.dim) continue;
-        if (slot) *reinterpret_cast<float2*>(to_part + r * p.dim + d) = make_float2(x, y);
-        else *reinterpret_cast<uint32_t*>(to + d) = pack<T>(x * f, y * f);
-      }
-    }
+    if (rows <= 4) join(std::integral_constant<int, 4>());
+    else if (rows <= 8) join(std::integral_constant<int, 8>());
+    else join(std::integral_constant<int, 16>());
   }
   if (!alive && a.split && tid < 2) slot_used[tid] = false;
   if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
