@@ -496,6 +496,12 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   // (rows are max_new's word; all tiles that there can be)
   p->narrow = units / static_cast<double>((rows + p->tile - 1) / p->tile) * static_cast<double>(sure * group / p->tile + 1) < 2e9;
   int limit = sms * shape.blocks;
+  // (where no table is longer than an item that stays whole, and each has its block, nothing will have to be joined)
+  if (static_cast<int64_t>(c.table_width) * c.page_size <= static_cast<int64_t>(kWholeUnits) * p->unit && items(c, group, p->tile) <= limit) {
+    p->split = false;
+    p->grid = static_cast<unsigned>(items(c, group, p->tile));
+    return true;
+  }
   limit = limit < kMaxBlocks ? limit : kMaxBlocks;
   p->grid = units < limit ? static_cast<unsigned>(units) : static_cast<unsigned>(limit);
   p->partial_bytes = (2 * sizeof(float) * p->grid * p->tile * (c.head_dim + 2) + 255) / 256 * 256;
