@@ -477,7 +477,7 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
     rows = p->most = kFewRows;
   }
   p->token = token_fits(d);
-  p->tile = p->token ? kTokenRows : rows_tile(c.head_dim, rows);
+  p->tile = p->token ? token_rows(rows) : rows_tile(c.head_dim, rows);
   const TokenShape shape = p->token ? token_shape(c.cache_dtype, c.head_dim) : TokenShape{row_blocks(c.head_dim, p->tile), kRowsUnit};
   p->unit = shape.unit;
   p->split = rows <= kFewRows;

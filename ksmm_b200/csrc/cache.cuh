@@ -290,7 +290,7 @@ struct TokenShape {
   int blocks, unit;  // blocks on an SM, tokens of a unit
 };
 TokenShape token_shape(int cache_dtype, int dim);
-constexpr int kTokenRows = 16;    // rows of an item in the 16- and 8-bit kernel
+inline int token_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }  // of an item in the 16- and 8-bit kernel
 bool token_fits(const ksmm_cache_attention_desc_t& d);
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
 int prompt_rows(int dim, int group);  // rows of an item in the prompt kernel

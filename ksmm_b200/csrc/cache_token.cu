@@ -7,11 +7,13 @@
 // maximum, sum and output of their own, and meet only at the end of a segment.  Warps that each wait for their unit
 // alone hide the latency that a block-wide step for each unit would show.
 //
-// mma.sync, not tcgen05: an item has at most 16 rows (heads that share a key head, new tokens), an eighth of tcgen05's
-// smallest tile, and the scores have to come back to registers at once; 32 or 48 MMAs per 16 tokens take a quarter of the
-// time that their bytes take.  q sits in registers as the A operand; K (rows of a token) is the B operand as it lies in shared
-// memory, V through transposing loads.  The weights enter the second product as two 16-bit parts (w = hi + lo, each
-// rounded): one part would add an error as large as the result's final rounding.
+// mma.sync, not tcgen05: an item has 8 or 16 rows (heads that share a key head, new tokens), a sixteenth of tcgen05's
+// smallest tile, and the scores have to come back to registers at once.  Its rate is what a step costs (two warps on a
+// scheduler took 1800 cycles for 48 products each of 16 tokens x 128), so the tokens are the 16 rows of a product and the rows of q its
+// 8 columns: S^T = K q^T with K as the A operand as it lies in shared memory, o^T = V^T w^T with V through transposing loads and w^T
+// transposed in registers; with the rows of q as A half of a tile's 16 rows stood idle.  Of 16-bit caches the weights enter the
+// second product as two 16-bit parts (w = hi + lo, each rounded): one part would add an error as large as the result's final
+// rounding.
 //
 // 8-bit caches: the products run in fp16, which holds e4m3 exactly.  q is scaled by a power of two per row so that bf16's
 // range fits; a token's key scale multiplies its scores; its value scale multiplies its weight, relative to a running
@@ -31,10 +33,10 @@ namespace {
 
 using namespace tc;
 
-constexpr int kTileRows = kTokenRows;
 
-template <bool EIGHT, int DP>
+template <bool EIGHT, int DP, int NT>
 struct Layout {
+  static constexpr int kRows = 8 * NT;                                  // of an item
   // Warps that meet different tokens; rows of 256 have two for the same tokens, each with half of the output's columns (one alone has
   // 96 products and 32 loads in a step, and nothing else on its scheduler)
   static constexpr int kRuns = 4, kHalves = DP == 256 ? 2 : 1, kConsumers = kRuns * kHalves;
@@ -55,8 +57,8 @@ struct Layout {
   static constexpr int kScalesAt = kMergeAt + kHalves * kMerge;
   static constexpr int kQRow = DP * 2 + 16;                             // bytes of a row of q (and no two rows on the same banks)
   static constexpr int kQAt = kScalesAt + kStages * kScales;
-  static constexpr int kStatsAt = kQAt + kTileRows * kQRow;             // of the runs: maxima and sums of 16 rows, a half
-  static constexpr int kBarsAt = kStatsAt + kHalves * kRuns * 2 * kTileRows * 4;    // full, empty | a segment full, empty
+  static constexpr int kStatsAt = kQAt + kRows * kQRow;             // of the runs: maxima and sums of 16 rows, a half
+  static constexpr int kBarsAt = kStatsAt + kHalves * kRuns * 2 * kRows * 4;    // full, empty | a segment full, empty
   static constexpr int kSegmentAt = kBarsAt + (2 * kStages + 2) * 8;
   static constexpr int kFlagsAt = kSegmentAt + static_cast<int>(sizeof(Segment));
   static constexpr int kBytes = kFlagsAt + kStages * 4 + 4;
@@ -93,6 +95,12 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+// 8 x 8 values of 16 bits, a row of four pairs in the lanes 4 r .. 4 r + 3: transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 // two e4m3 (the low 16 bits) as fp16
 __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t v) {
@@ -146,15 +154,15 @@ struct Turn {
 
 // T: q and the output.  Tokens of a page that one TMA box covers: 2^box_log2; a box lies in its stage as [128-byte column][token].
 // `joined`: a map with the columns as a dimension of their own brings all of a box's at once.
-template <typename T, bool EIGHT, int DP>
-__global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>::kBlocks)
+template <typename T, bool EIGHT, int DP, int NT>
+__global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT, DP, NT>::kBlocks)
     token_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Attend a, const int box_log2, const int joined) {
-  using L = Layout<EIGHT, DP>;
+  using L = Layout<EIGHT, DP, NT>;
   using H = typename std::conditional<EIGHT, __half, T>::type;  // of the products
   // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
   constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
   // q stays in shared memory where registers do not hold it beside the output
-  constexpr bool kQShared = DP == 256;
+  constexpr bool kQShared = DP == 256 && NT == 2;
   constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
   extern __shared__ __align__(1024) char smem[];
   const uint32_t base = smem_u32(smem);
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
     mbar_init(segment_empty, L::kConsumers);
     fence_mbar_init();
   }
-  for (int i = tid; i < kTileRows * L::kQRow / 4; i += L::kThreads) reinterpret_cast<uint32_t*>(smem + L::kQAt)[i] = 0;
+  for (int i = tid; i < L::kRows * L::kQRow / 4; i += L::kThreads) reinterpret_cast<uint32_t*>(smem + L::kQAt)[i] = 0;
   if (warp == L::kConsumers && lane == 0) {
     prefetch_tensormap(&maps.keys);
     prefetch_tensormap(&maps.values);
@@ -220,8 +228,8 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       alive = __all_sync(0xffffffffu, mbar_wait<20>(segment_empty, (segments & 1) ^ 1, abort_flag, a.status, kWaits));
       if (!alive) break;
       if (more) {
-        const int rows = min(kTileRows, g.n * a.group - g.tile * kTileRows);
-        const int row = g.tile * kTileRows + min(lane, rows - 1), t = row / a.group;
+        const int rows = min(L::kRows, g.n * a.group - g.tile * L::kRows);
+        const int row = g.tile * L::kRows + min(lane, rows - 1), t = row / a.group;
         const int64_t row_at = (g.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
 #pragma unroll 4
         for (int r = 0; r < rows; ++r) {
@@ -298,11 +306,11 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
   bool slot_used[2] = {false, false};
   const int run = warp % L::kRuns, half = warp / L::kRuns;
   float* merge = reinterpret_cast<float*>(smem + L::kMergeAt + half * L::kMerge);
-  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt) + half * L::kRuns * 2 * kTileRows;
-  // lane's row and chunk in the loads of four matrices: K: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1;
-  // V: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1
-  const int k_row = (lane / 16) * 8 + lane % 8, k_chunk = lane / 8 % 2;
-  const int v_row = (lane / 8 % 2) * 8 + lane % 8, v_chunk = lane / 16;
+  float* stats = reinterpret_cast<float*>(smem + L::kStatsAt) + half * L::kRuns * 2 * L::kRows;
+  // lane's token and chunk in the loads of four matrices: keys: tokens 0-7 | 8-15 | 0-7 | 8-15, chunks c, c, c + 1, c + 1;
+  // values, transposed: tokens 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1
+  const int k_row = (lane / 8 % 2) * 8 + lane % 8, k_chunk = lane / 16;
+  const int v_row = (lane / 16) * 8 + lane % 8, v_chunk = lane / 8 % 2;
   // where the groups of 16 tokens lie in a stage
   uint32_t group_at[G];
 #pragma unroll
@@ -320,40 +328,35 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
     ++segments;
     const Segment g = *segment;
     if (g.s < 0) break;
-    const int rows = min(kTileRows, g.n * a.group - g.tile * kTileRows);
-    const bool upper = rows > 8;  // whether a lane's second row is one
-    uint32_t qf[DP / 16][4];
-    float m[2], sum[2], row_scale[2], vm = 0.f;
-    int position[2];
-    float o[L::kCols / 8][4];
-    // (8-bit chunks: elements 4 q4 + 2 e and the next instead of 2 q4 + 8 e)
+    const int rows = min(L::kRows, g.n * a.group - g.tile * L::kRows);
+    // A lane's columns of a product are the rows 2 q4 and 2 q4 + 1 of each eight, its rows the tokens gq and gq + 8.
+    uint32_t qf[DP / 16][NT][2];
+    float m[NT][2], sum[NT][2], row_scale[NT][2], vm = 0.f;
+    int position[NT][2];
+    float o[L::kCols / 16][NT][4];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      if constexpr (EIGHT) {
+    for (int t = 0; t < NT; ++t) {
+      // (8-bit chunks: elements 4 q4 + 2 e and the next instead of 2 q4 + 8 e)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint2 v = *reinterpret_cast<const uint2*>(smem + L::kQAt + (gq + 8 * h) * L::kQRow + (c * 16 + 4 * q4) * 2);
-          qf[c][h] = v.x;
-          qf[c][h + 2] = v.y;
+      for (int c = 0; c < DP / 16; ++c) {
+        const char* at = smem + L::kQAt + (gq + 8 * t) * L::kQRow + c * 32;
+        if constexpr (EIGHT) {
+          const uint2 v = *reinterpret_cast<const uint2*>(at + 8 * q4);
+          qf[c][t][0] = v.x;
+          qf[c][t][1] = v.y;
+        } else if constexpr (!kQShared) {
+          qf[c][t][0] = *reinterpret_cast<const uint32_t*>(at + 4 * q4);
+          qf[c][t][1] = *reinterpret_cast<const uint32_t*>(at + 4 * q4 + 16);
         }
-      } else if constexpr (!kQShared) {
-        ldmatrix4(qf[c], base + L::kQAt + v_row * L::kQRow + v_chunk * 16 + c * 32);
       }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = gq + 8 * h;
-      position[h] = r < rows ? g.length - g.n + (g.tile * kTileRows + r) / a.group : INT_MAX;  // (a row that is not there masks nothing)
-      m[h] = kNone;
-      sum[h] = 0.f;
-      row_scale[h] = a.scale;
+      float up = 1.f;  // of row gq
       if constexpr (EIGHT && ElemTraits<T>::kDtype == KSMM_BF16) {
         float top = 0.f;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float2 v = unpack<T>(qf[c][h + 2 * e]);
+            const float2 v = unpack<T>(qf[c][t][e]);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -361,21 +364,31 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
         // 2^-e, e the largest element's exponent; subnormal rows are taken as 0, rows with infinities as they are
         const int e = static_cast<int>(__float_as_uint(top) >> 23);
         const float down = e == 0 || e >= 253 ? (e == 255 ? 1.f : e ? 0x1p-126f : 0.f) : __uint_as_float((254 - e) << 23);
-        const float up = e == 0 || e >= 253 ? (e == 255 ? 1.f : e ? 0x1p126f : 0.f) : __uint_as_float(e << 23);
-        row_scale[h] = a.scale * up;
+        up = e == 0 || e >= 253 ? (e == 255 ? 1.f : e ? 0x1p126f : 0.f) : __uint_as_float(e << 23);
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
           for (int e2 = 0; e2 < 2; ++e2) {
-            const float2 v = unpack<T>(qf[c][h + 2 * e2]);
-            qf[c][h + 2 * e2] = pack<H>(v.x * down, v.y * down);
+            const float2 v = unpack<T>(qf[c][t][e2]);
+            qf[c][t][e2] = pack<H>(v.x * down, v.y * down);
           }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * t + 2 * q4 + e;
+        position[t][e] = r < rows ? g.length - g.n + (g.tile * L::kRows + r) / a.group : INT_MAX;  // (a row that is not there masks nothing)
+        m[t][e] = kNone;
+        sum[t][e] = 0.f;
+        row_scale[t][e] = a.scale;
+        if constexpr (EIGHT && ElemTraits<T>::kDtype == KSMM_BF16) row_scale[t][e] *= __shfl_sync(0xffffffffu, up, (2 * q4 + e) * 4);
       }
     }
 #pragma unroll
-    for (int i = 0; i < L::kCols / 8; ++i)
+    for (int c = 0; c < L::kCols / 16; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][t][e] = 0.f;
 
     if constexpr (kQShared && EIGHT) {
       // in the order of the chunks, and in fp16; one warp for all
@@ -384,8 +397,11 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint32_t*>(smem + L::kQAt + (gq + 8 * (e % 2)) * L::kQRow + (c * 16 + 2 * q4 + 8 * (e / 2)) * 2) = qf[c][e];
+          for (int t = 0; t < NT; ++t) {
+            char* at = smem + L::kQAt + (gq + 8 * t) * L::kQRow + c * 32 + 4 * q4;
+            *reinterpret_cast<uint32_t*>(at) = qf[c][t][0];
+            *reinterpret_cast<uint32_t*>(at + 16) = qf[c][t][1];
+          }
       }
       bar_sync_named(1, L::kConsumers * 32);
     }
@@ -393,7 +409,19 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       __syncwarp();
       if (lane == 0) mbar_arrive(segment_empty);
     }
-    const uint32_t q_at = base + L::kQAt + v_row * L::kQRow + v_chunk * 16;
+    // (q from shared memory in every step: rows 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1)
+    const uint32_t q_at = base + L::kQAt + (v_row % L::kRows) * L::kQRow + v_chunk * 16;
+    auto q_load = [&](int c) {
+      if constexpr (kQShared) {
+        uint32_t r[4];
+        ldmatrix4(r, q_at + c * 32);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          qf[c][t][0] = r[2 * t];
+          qf[c][t][1] = r[2 * t + 1];
+        }
+      }
+    };
     // tokens from `clear` to below `sure` are seen by every row
     const int sure = g.first_position + 1;
     const int64_t clear = a.window ? static_cast<int64_t>(g.hi) - a.window : 0;
@@ -406,136 +434,164 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
         const uint32_t ks = base + st * L::kStageBytes, vs = ks + L::kOperand;
         const int missing = flags[st];
         // ---- scores ----
-        float s[2 * G][4];
+        float s[G][NT][4];
 #pragma unroll
-        for (int i = 0; i < 2 * G; ++i)
+        for (int i = 0; i < G; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][t][e] = 0.f;
         if constexpr (!EIGHT) {
 #pragma unroll
-          for (int c = 0; c < DP / 16; ++c)
+          for (int c = 0; c < DP / 16; ++c) {
+            q_load(c);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-              uint32_t b[4];
-              if (kQShared && i == 0) ldmatrix4(qf[c], q_at + c * 32);
-              ldmatrix4(b, ks + group_at[i] + c / 4 * box_bytes + k_row * 128 + (((c % 4 * 2 + k_chunk) ^ (k_row & 7)) << 4));
-              mma<H>(s[2 * i], qf[c], b[0], b[1]);
-              mma<H>(s[2 * i + 1], qf[c], b[2], b[3]);
+              uint32_t k[4];
+              ldmatrix4(k, ks + group_at[i] + c / 4 * box_bytes + k_row * 128 + (((c % 4 * 2 + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma<H>(s[i][t], k, qf[c][t][0], qf[c][t][1]);
             }
+          }
         } else {
 #pragma unroll
-          for (int c = 0; c < DP / 16; c += 2)
+          for (int c = 0; c < DP / 16; c += 2) {
+            q_load(c);
+            q_load(c + 1);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-              uint32_t b[4];
-              if (kQShared && i == 0) {
-                ldmatrix4(qf[c], q_at + c * 32);
-                ldmatrix4(qf[c + 1], q_at + c * 32 + 32);
-              }
+              uint32_t b[4];  // tokens 0-7 and 8-15 of chunk c, then of c + 1
               ldmatrix4(b, ks + group_at[i] + c / 8 * box_bytes + k_row * 128 + (((c % 8 + k_chunk) ^ (k_row & 7)) << 4));
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                mma<H>(s[2 * i], qf[c + e], e4m3_to_half2(b[e]), e4m3_to_half2(b[e] >> 16));
-                mma<H>(s[2 * i + 1], qf[c + e], e4m3_to_half2(b[2 + e]), e4m3_to_half2(b[2 + e] >> 16));
+                const uint32_t k[4] = {e4m3_to_half2(b[2 * e]), e4m3_to_half2(b[2 * e + 1]), e4m3_to_half2(b[2 * e] >> 16),
+                                       e4m3_to_half2(b[2 * e + 1] >> 16)};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma<H>(s[i][t], k, qf[c + e][t][0], qf[c + e][t][1]);
               }
             }
-        }
-        float value_scale[2 * G][2];
-        if constexpr (EIGHT) {
-          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + run * L::kStep + 2 * q4;
-#pragma unroll
-          for (int i = 0; i < 2 * G; ++i) {
-            const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * i), v2 = *reinterpret_cast<const float2*>(sc + L::kTokens + 8 * i);
-            value_scale[i][0] = v2.x;
-            value_scale[i][1] = v2.y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2] * (e % 2 ? k2.y : k2.x);
           }
+        }
+        float value_scale[G][2];  // of the lane's tokens
+        if constexpr (EIGHT) {
+          const float* sc = reinterpret_cast<const float*>(smem + L::kScalesAt + st * L::kScales) + run * L::kStep + gq;
+#pragma unroll
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float key_scale = sc[16 * i + 8 * h];
+              value_scale[i][h] = sc[L::kTokens + 16 * i + 8 * h];
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) s[i][t][2 * h + e] *= row_scale[t][e] * key_scale;
+            }
         } else {
 #pragma unroll
-          for (int i = 0; i < 2 * G; ++i)
+          for (int i = 0; i < G; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] *= row_scale[e / 2];
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[i][t][e] *= row_scale[t][e % 2];
         }
         const bool edge = token + L::kStep > sure || token < clear || token < g.lo || missing;
-        uint32_t keep[2 * G];  // 16-bit pairs of the lane's tokens: whether they are the sequence's and there
+        uint32_t keep[2 * G];  // 16-bit pairs of tokens 2 q4, 2 q4 + 1 of each eight: whether they are the sequence's and there
         if (edge) {
 #pragma unroll
           for (int i = 0; i < 2 * G; ++i) {
-            keep[i] = 0;
             const bool gone = missing >> ((run * L::kStep + i * 8) >> box_log2) & 1;
+            keep[i] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = token + 8 * i + 2 * q4 + e % 2;
-              const bool in = j < g.hi && j >= g.lo;
-              if (in && !gone) keep[i] |= e % 2 ? 0xffff0000u : 0xffffu;
-              const bool sees = in && j <= position[e / 2] && (!a.window || j > position[e / 2] - a.window);
-              s[i][e] = sees ? (gone ? __int_as_float(0x7fffffff) : s[i][e]) : -INFINITY;
-              if (EIGHT && !(in && !gone)) value_scale[i][e % 2] = 0.f;
+            for (int e = 0; e < 2; ++e) {
+              const int j = token + 8 * i + 2 * q4 + e;
+              if (j < g.hi && j >= g.lo && !gone) keep[i] |= e ? 0xffff0000u : 0xffffu;
             }
+            const int j = token + 8 * i + gq;  // the lane's own of these eight
+            const bool in = j < g.hi && j >= g.lo;
+            if (EIGHT && (!in || gone)) value_scale[i / 2][i % 2] = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float& x = s[i / 2][t][i % 2 * 2 + e];
+                const bool sees = in && j <= position[t][e] && (!a.window || j > position[t][e] - a.window);
+                x = sees ? (gone ? __int_as_float(0x7fffffff) : x) : -INFINITY;
+              }
           }
         }
         // ---- running maximum and sum ----
-        float scale_o[2];
+        float scale_o[NT][2];
+        bool grown = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          scale_o[h] = 1.f;
-          if (h == 1 && !upper) continue;
-          float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 1; i < 2 * G; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m[h]);
-          scale_o[h] = exp2_fast(m[h] - top);
-          m[h] = top;
-          sum[h] *= scale_o[h];
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[0][t][e], s[0][t][2 + e]);
 #pragma unroll
-          for (int i = 0; i < 2 * G; ++i)
+            for (int i = 1; i < G; ++i) top = fmaxf(top, fmaxf(s[i][t][e], s[i][t][2 + e]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), m[t][e]);
+            scale_o[t][e] = exp2_fast(m[t][e] - top);
+            m[t][e] = top;
+            sum[t][e] *= scale_o[t][e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              s[i][2 * h + e] = exp2_fast(s[i][2 * h + e] - top);
-              sum[h] += s[i][2 * h + e];
-            }
-        }
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                s[i][t][2 * h + e] = exp2_fast(s[i][t][2 * h + e] - top);
+                sum[t][e] += s[i][t][2 * h + e];
+              }
+          }
         if constexpr (EIGHT) {
           // the weights times the values' scales, relative to a power of two that is at least each of them
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2 * G; ++i) top = fmaxf(top, fmaxf(value_scale[i][0], value_scale[i][1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          for (int i = 0; i < G; ++i) top = fmaxf(top, fmaxf(value_scale[i][0], value_scale[i][1]));
+#pragma unroll
+          for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
           if (top > vm) {
             const uint32_t e = min((__float_as_uint(top) >> 23) + 1, 254u);
             const float next = __uint_as_float(e << 23), f = vm / next;
             vm = next;
-            scale_o[0] *= f;
-            scale_o[1] *= f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              scale_o[t][0] *= f;
+              scale_o[t][1] *= f;
+            }
           }
           const float back = vm > 0.f ? 1.f / vm : 0.f;
 #pragma unroll
-          for (int i = 0; i < 2 * G; ++i)
+          for (int i = 0; i < G; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] *= value_scale[i][e % 2] * back;
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[i][t][e] *= value_scale[i][e / 2] * back;
         }
-        if (__any_sync(0xffffffffu, scale_o[0] != 1.f || scale_o[1] != 1.f)) {
 #pragma unroll
-          for (int i = 0; i < L::kCols / 8; ++i)
+        for (int t = 0; t < NT; ++t) grown = grown || scale_o[t][0] != 1.f || scale_o[t][1] != 1.f;
+        if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] *= scale_o[e / 2];
+          for (int c = 0; c < L::kCols / 16; ++c)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[c][t][e] *= scale_o[t][e % 2];
         }
         // ---- values ----
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-          uint32_t hi[4], part[4];
+          uint32_t hi[NT][2], part[NT][2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float x = s[2 * i + k][2 * h], y = s[2 * i + k][2 * h + 1];
-              hi[2 * k + h] = pack<H>(x, y);
+              const float x = s[i][t][2 * h], y = s[i][t][2 * h + 1];
+              const uint32_t w = pack<H>(x, y);
+              hi[t][h] = transpose8(w);
               if (kParts) {
-                const float2 r = unpack<H>(hi[2 * k + h]);
-                part[2 * k + h] = pack<H>(x - r.x, y - r.y);
+                const float2 r = unpack<H>(w);
+                part[t][h] = transpose8(pack<H>(x - r.x, y - r.y));
               }
             }
           const uint32_t at = vs + group_at[i] + half * (L::kBoxes / L::kHalves) * box_bytes + v_row * 128;
@@ -546,37 +602,36 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
               ldmatrix4_trans(b, at + c / 4 * box_bytes + (((c % 4 * 2 + v_chunk) ^ (v_row & 7)) << 4));
               if (edge) {
                 b[0] &= keep[2 * i];
-                b[1] &= keep[2 * i + 1];
-                b[2] &= keep[2 * i];
+                b[1] &= keep[2 * i];
+                b[2] &= keep[2 * i + 1];
                 b[3] &= keep[2 * i + 1];
               }
-              mma<H>(o[2 * c], hi, b[0], b[1]);
-              mma<H>(o[2 * c + 1], hi, b[2], b[3]);
-              mma<H>(o[2 * c], part, b[0], b[1]);
-              mma<H>(o[2 * c + 1], part, b[2], b[3]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                mma<H>(o[c][t], b, hi[t][0], hi[t][1]);
+                mma<H>(o[c][t], b, part[t][0], part[t][1]);
+              }
             }
           } else {
-            // a chunk of 16 elements: the even ones are one tile of eight, the odd ones the next
+            // a chunk of 16 elements: the even ones are the first eight rows of the product, the odd ones the others
 #pragma unroll
             for (int c = 0; c < L::kCols / 16; c += 2) {
-              uint32_t b[4];
+              uint32_t b[4];  // tokens 0-7 of chunks c and c + 1, then tokens 8-15
               ldmatrix4_trans(b, at + c / 8 * box_bytes + (((c % 8 + v_chunk) ^ (v_row & 7)) << 4));
               if (edge) {
                 b[0] &= keep[2 * i];
-                b[1] &= keep[2 * i + 1];
-                b[2] &= keep[2 * i];
+                b[1] &= keep[2 * i];
+                b[2] &= keep[2 * i + 1];
                 b[3] &= keep[2 * i + 1];
               }
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const uint32_t even0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0020)), odd0 = e4m3_to_half2(__byte_perm(b[2 * e], 0, 0x0031));
-                const uint32_t even1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0020));
-                const uint32_t odd1 = e4m3_to_half2(__byte_perm(b[2 * e + 1], 0, 0x0031));
-                mma<H>(o[2 * (c + e)], hi, even0, even1);
-                mma<H>(o[2 * (c + e) + 1], hi, odd0, odd1);
-                if (kParts) {
-                  mma<H>(o[2 * (c + e)], part, even0, even1);
-                  mma<H>(o[2 * (c + e) + 1], part, odd0, odd1);
+                const uint32_t v[4] = {e4m3_to_half2(__byte_perm(b[e], 0, 0x0020)), e4m3_to_half2(__byte_perm(b[e], 0, 0x0031)),
+                                       e4m3_to_half2(__byte_perm(b[2 + e], 0, 0x0020)), e4m3_to_half2(__byte_perm(b[2 + e], 0, 0x0031))};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  mma<H>(o[c + e][t], v, hi[t][0], hi[t][1]);
+                  if (kParts) mma<H>(o[c + e][t], v, part[t][0], part[t][1]);
                 }
               }
             }
@@ -587,7 +642,6 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       if (lane == 0) mbar_arrive(empty + 8 * st);
       turn.next();
     }
-
     if constexpr (kQShared) {
       __syncwarp();
       if (lane == 0) mbar_arrive(segment_empty);
@@ -596,71 +650,79 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
     // ---- the four runs' results, in pieces of the columns that the buffer holds for all rows: every warp gives, then every
     // thread joins some pairs of neighbours and writes them ----
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-      if (q4 == 0) {
-        stats[(run * 2) * kTileRows + gq + 8 * h] = m[h];
-        stats[(run * 2 + 1) * kTileRows + gq + 8 * h] = !alive || g.bad ? __int_as_float(0x7fffffff) : sum[h];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) sum[t][e] += __shfl_xor_sync(0xffffffffu, sum[t][e], x);
+        if (gq == 0) {
+          const int r = 8 * t + 2 * q4 + e;
+          stats[run * 2 * L::kRows + r] = m[t][e];
+          stats[(run * 2 + 1) * L::kRows + r] = !alive || g.bad ? __int_as_float(0x7fffffff) : sum[t][e];
+        }
       }
-    }
     if (EIGHT) {
 #pragma unroll
-      for (int i = 0; i < L::kCols / 8; ++i)
+      for (int c = 0; c < L::kCols / 16; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] *= vm;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][t][e] *= vm;
     }
     if (g.slot) {
       slot_used[g.slot - 1] = true;
       if (tid == 0) a.slots[2 * blockIdx.x + g.slot - 1] = g.item;
     }
-    float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + g.slot - 1) * kTileRows * (p.dim + 2);
+    float* to_part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + g.slot - 1) * L::kRows * (p.dim + 2);
     // CAP: rows that fit, a power of two
     auto join = [&](auto cap) {
       constexpr int CAP = decltype(cap)::value, W = L::kMerge / 4 / 4 / CAP, kPieces = L::kCols / W;  // columns of a piece
-      // (rows side by side in a store are moved by eight columns against each other: other banks)
-      auto place = [&](int of_run, int r, int col) { return merge + (of_run * CAP + r) * W + (col ^ (r & 3) * 8 % W); };
+      // (a store's rows, two apart, are moved by eight columns against each other: other banks)
+      auto place = [&](int of_run, int r, int col) { return merge + (of_run * CAP + r) * W + (col ^ (r / 2 % 4) * 8 % W); };
 #pragma unroll
       for (int piece = 0; piece < kPieces; ++piece) {
         if (piece) bar_sync_named(1, L::kConsumers * 32);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = gq + 8 * h;
-          if (8 * h >= CAP || r >= CAP) continue;
-          // (8-bit chunks have their even and odd columns in two tiles)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = piece * (W / 8); i < (piece + 1) * (W / 8); i += EIGHT ? 2 : 1) {
-            const int col = i * 8 - piece * W;
-            if constexpr (EIGHT)
-              *reinterpret_cast<float4*>(place(run, r, col + 4 * q4)) = make_float4(o[i][2 * h], o[i + 1][2 * h], o[i][2 * h + 1], o[i + 1][2 * h + 1]);
-            else
-              *reinterpret_cast<float2*>(place(run, r, col + 2 * q4)) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * t + 2 * q4 + e;
+            if (8 * t >= CAP || r >= CAP) continue;
+#pragma unroll
+            for (int c = piece * (W / 16); c < (piece + 1) * (W / 16); ++c) {
+              const int col = c * 16 - piece * W;
+              if constexpr (EIGHT) {
+                *reinterpret_cast<float2*>(place(run, r, col + 2 * gq)) = make_float2(o[c][t][e], o[c][t][2 + e]);
+              } else {
+                *place(run, r, col + gq) = o[c][t][e];
+                *place(run, r, col + 8 + gq) = o[c][t][2 + e];
+              }
+            }
           }
-        }
         bar_sync_named(1, L::kConsumers * 32);
         for (int e = run * 32 + lane; e < rows * (W / 2); e += L::kRuns * 32) {
           const int r = e / (W / 2), col = e % (W / 2) * 2, d = half * L::kCols + piece * W + col;
-          float f[L::kRuns], top = stats[r];
+          float top = stats[r];
 #pragma unroll
-          for (int k = 1; k < L::kRuns; ++k) top = fmaxf(top, stats[2 * k * kTileRows + r]);
+          for (int k = 1; k < L::kRuns; ++k) top = fmaxf(top, stats[2 * k * L::kRows + r]);
           float total = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
           for (int k = 0; k < L::kRuns; ++k) {
-            f[k] = exp2_fast(stats[2 * k * kTileRows + r] - top);
-            total = fmaf(stats[(2 * k + 1) * kTileRows + r], f[k], total);
+            const float f = exp2_fast(stats[2 * k * L::kRows + r] - top);
+            total = fmaf(stats[(2 * k + 1) * L::kRows + r], f, total);
             const float2 v = *reinterpret_cast<const float2*>(place(k, r, col));
-            x = fmaf(v.x, f[k], x);
-            y = fmaf(v.y, f[k], y);
+            x = fmaf(v.x, f, x);
+            y = fmaf(v.y, f, y);
           }
           if (d >= p.dim) continue;
           if (g.slot) {
             *reinterpret_cast<float2*>(to_part + r * p.dim + d) = make_float2(x, y);
             if (d == 0) {
-              to_part[kTileRows * p.dim + r] = top;
-              to_part[kTileRows * (p.dim + 1) + r] = total;
+              to_part[L::kRows * p.dim + r] = top;
+              to_part[L::kRows * (p.dim + 1) + r] = total;
             }
           } else {
-            const int row = g.tile * kTileRows + r, t = row / a.group;
+            const int row = g.tile * L::kRows + r, t = row / a.group;
             const float back = total == 0.f ? 0.f : 1.f / total;
             T* to = reinterpret_cast<T*>(a.out) + (g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
             *reinterpret_cast<uint32_t*>(to + d) = pack<T>(x * back, y * back);
@@ -669,17 +731,17 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP>::kThreads, Layout<EIGHT, DP>
       }
     };
     if (rows <= 4) join(std::integral_constant<int, 4>());
-    else if (rows <= 8) join(std::integral_constant<int, 8>());
-    else join(std::integral_constant<int, 16>());
+    else if (NT == 1 || rows <= 8) join(std::integral_constant<int, 8>());
+    else if constexpr (NT == 2) join(std::integral_constant<int, 16>());
   }
   if (!alive && a.split && tid < 2) slot_used[tid] = false;
   if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
 }
 
-template <typename T, bool EIGHT, int DP>
+template <typename T, bool EIGHT, int DP, int NT>
 int launch_one(const Maps& maps, const Attend& a, int box, int joined, unsigned grid, cudaStream_t stream) {
-  using L = Layout<EIGHT, DP>;
-  auto kern = token_kernel<T, EIGHT, DP>;
+  using L = Layout<EIGHT, DP, NT>;
+  auto kern = token_kernel<T, EIGHT, DP, NT>;
   static std::atomic<uint64_t> ready{0};  // a bit per device
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -696,9 +758,9 @@ int launch_one(const Maps& maps, const Attend& a, int box, int joined, unsigned 
 
 int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-template <typename T, bool EIGHT, int DP>
+template <typename T, bool EIGHT, int DP, int NT>
 int launch_maps(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
-  using L = Layout<EIGHT, DP>;
+  using L = Layout<EIGHT, DP, NT>;
   const Pool& p = a.pool;
   int box = L::kTokens;
   while (p.page_size % box) box /= 2;
@@ -714,34 +776,47 @@ int launch_maps(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t st
                               joined ? strides5 : strides4, size);
     if (st != KSMM_OK) return st;
   }
-  return launch_one<T, EIGHT, DP>(maps, a, box, joined, grid, stream);
+  return launch_one<T, EIGHT, DP, NT>(maps, a, box, joined, grid, stream);
 }
 
-template <typename T, bool EIGHT>
+template <typename T, bool EIGHT, int NT>
 int launch_dim(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
   switch (padded(a.pool.dim)) {
-    case 64: return launch_maps<T, EIGHT, 64>(a, cache_dtype, grid, stream);
-    case 128: return launch_maps<T, EIGHT, 128>(a, cache_dtype, grid, stream);
-    default: return launch_maps<T, EIGHT, 256>(a, cache_dtype, grid, stream);
+    case 64: return launch_maps<T, EIGHT, 64, NT>(a, cache_dtype, grid, stream);
+    case 128: return launch_maps<T, EIGHT, 128, NT>(a, cache_dtype, grid, stream);
+    default: return launch_maps<T, EIGHT, 256, NT>(a, cache_dtype, grid, stream);
   }
 }
 
 }  // namespace
 
+template <bool EIGHT, int DP>
+static TokenShape shape_of() {
+  using L = Layout<EIGHT, DP, 1>;
+  static_assert(L::kBlocks == Layout<EIGHT, DP, 2>::kBlocks && L::kTokens == Layout<EIGHT, DP, 2>::kTokens, "whatever the rows");
+  return {L::kBlocks, L::kTokens};
+}
+
 TokenShape token_shape(int cache_dtype, int dim) {
   const bool eight = cache_dtype == KSMM_F8E4M3;
   switch (padded(dim)) {
-    case 64: return eight ? TokenShape{Layout<true, 64>::kBlocks, Layout<true, 64>::kTokens} : TokenShape{Layout<false, 64>::kBlocks, Layout<false, 64>::kTokens};
-    case 128: return eight ? TokenShape{Layout<true, 128>::kBlocks, Layout<true, 128>::kTokens} : TokenShape{Layout<false, 128>::kBlocks, Layout<false, 128>::kTokens};
-    default: return eight ? TokenShape{Layout<true, 256>::kBlocks, Layout<true, 256>::kTokens} : TokenShape{Layout<false, 256>::kBlocks, Layout<false, 256>::kTokens};
+    case 64: return eight ? shape_of<true, 64>() : shape_of<false, 64>();
+    case 128: return eight ? shape_of<true, 128>() : shape_of<false, 128>();
+    default: return eight ? shape_of<true, 256>() : shape_of<false, 256>();
   }
+}
+
+template <typename T, bool EIGHT>
+static int launch_rows_of(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  if (a.tile_rows == 8) return launch_dim<T, EIGHT, 1>(a, cache_dtype, grid, stream);
+  return launch_dim<T, EIGHT, 2>(a, cache_dtype, grid, stream);
 }
 
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
   const bool eight = cache_dtype == KSMM_F8E4M3;
   if (dtype == KSMM_F16)
-    return eight ? launch_dim<__half, true>(a, cache_dtype, grid, stream) : launch_dim<__half, false>(a, cache_dtype, grid, stream);
-  return eight ? launch_dim<__nv_bfloat16, true>(a, cache_dtype, grid, stream) : launch_dim<__nv_bfloat16, false>(a, cache_dtype, grid, stream);
+    return eight ? launch_rows_of<__half, true>(a, cache_dtype, grid, stream) : launch_rows_of<__half, false>(a, cache_dtype, grid, stream);
+  return eight ? launch_rows_of<__nv_bfloat16, true>(a, cache_dtype, grid, stream) : launch_rows_of<__nv_bfloat16, false>(a, cache_dtype, grid, stream);
 }
 
 // Whether TMA can address the pool and the rows of q and out are pairs on their boundary.
