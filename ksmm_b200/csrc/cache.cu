@@ -469,7 +469,7 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   int64_t rows = (d.max_new > 0 && d.max_new < sure ? d.max_new : sure) * group;
   p->most = INT_MAX;
   if (rows > kFewRows && prompt_fits(d)) {
-    p->prompt_tile = prompt_rows(c.head_dim, static_cast<int>(group));
+    p->prompt_tile = prompt_rows(static_cast<int>(group));
     const int64_t n = items(c, group, p->prompt_tile);
     if (n >= INT_MAX) return false;
     p->prompt = static_cast<unsigned>(n);

@@ -209,7 +209,24 @@ struct Walker {
     return true;
   }
 
-  __device__ bool start(const Attend& a) { return a.narrow ? start_counted<int>(a) : start_counted<int64_t>(a); }
+  __device__ bool start(const Attend& a) {
+    if (!a.split && !a.pool.starts) {
+      // (all sequences have the same number of items)
+      const int64_t rows = static_cast<int64_t>(a.pool.each) * a.group;
+      const int64_t per = rows < a.least || rows > a.most ? 0 : divide(rows + a.tile_rows - 1, a.tile_rows) * a.pool.kv_heads;
+      if (blockIdx.x >= per * a.pool.sequences) return false;
+      const int which = static_cast<int>(divide(blockIdx.x, per));
+      left = 1;
+      whole = true;
+      from = 0;
+      set(a, which);
+      const int64_t item = blockIdx.x - which * per, t = divide(item, a.pool.kv_heads);
+      head = static_cast<int>(item - t * a.pool.kv_heads);
+      tile = work.tiles - 1 - static_cast<int>(t);
+      return true;
+    }
+    return a.narrow ? start_counted<int>(a) : start_counted<int64_t>(a);
+  }
 
   // the next segment; one with s < 0 where there is none
   __device__ void next(const Attend& a, Segment* g) {
@@ -293,7 +310,7 @@ TokenShape token_shape(int cache_dtype, int dim);
 inline int token_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }  // of an item in the 16- and 8-bit kernel
 bool token_fits(const ksmm_cache_attention_desc_t& d);
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
-int prompt_rows(int dim, int group);  // rows of an item in the prompt kernel
+int prompt_rows(int group);       // rows of an item in the prompt kernel
 bool prompt_fits(const ksmm_cache_attention_desc_t& d);
 int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
 int launch_join(const Attend& a, int dtype, unsigned blocks, int rows, cudaStream_t stream);  // rows: of an item, at most

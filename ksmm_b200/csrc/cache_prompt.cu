@@ -1,14 +1,17 @@
 // Attention of many new tokens (prompts) over a paged cache in 16 bits, on tcgen05.
 //
-// An item is one key head and 1 or 2 tiles of up to 128 rows: a row is (token, head of the group), all heads that share the
-// key head side by side, so that keys and values are read once for them.  Per tile of keys: S = Q K^T into tensor memory, a
-// thread per row turns its S into weights (running maximum, exponentials, sum in fp32) and writes them back as 16-bit
-// pairs, O += P V takes them from tensor memory as its A operand.  P lies over S.  Two row tiles alternate: while the softmax
-// threads of one work, the tensor cores run the other's products.
+// An item is one key head and a tile of up to 128 rows: a row is (token, head of the group), all heads that share the key head
+// side by side, so that keys and values are read once for them.  Per tile of keys: S = Q K^T into tensor memory, a thread per row
+// turns its S into weights (running maximum, exponentials, sum in fp32) and writes them back as 16-bit pairs, O += P V takes them
+// from tensor memory as its A operand.  P lies over S.
 //
-// Warps 0..3 and 4..7: rows of the first and second tile; then a TMA warp and a warp that issues the MMAs.  K is K-major as
-// it lies in the pages, V is the MN-major operand (its tokens are the contraction), so neither is turned.  O stays in tensor
-// memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the last time: weights are then at most
+// Four warps of rows, one that issues TMA loads, one that issues MMAs; two blocks on an SM (up to 128 columns), each with half of
+// its tensor memory: while the rows of one work, the tensor cores run the other's products, and one's start and end (6 us, as
+// much as five tiles) pass under the other's work.  One block with two row tiles kept the same balance inside but not at its ends:
+// 32 prompts of 1000 tokens of 12 heads of 64 took 186 us.
+//
+// K is K-major as it lies in the pages, V is the MN-major operand (its tokens are the contraction), so neither is turned.  O stays in
+// tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the last time: weights are then at most
 // 256, which 16 bits hold as well as 1, and the sum is exact to fp32 either way.  Weights are rounded once to 16 bits; the sum is
 // that of the unrounded ones (their errors are independent: together as large as the result's own rounding).
 #include <atomic>
@@ -27,31 +30,25 @@ using namespace tc;
 
 template <int DP>
 struct Prompt {
-  static constexpr int kTiles = DP == 256 ? 1 : 2;
+  static constexpr int kBlocks = DP == 256 ? 1 : 2;            // on an SM
   static constexpr int kKeys = DP == 256 ? 64 : 128;           // tokens of a tile of keys
   static constexpr int kBoxes = DP / 64;                       // 128-byte columns of a row
-  static constexpr int kQ = 128 * DP * 2;                      // a row tile's q
+  static constexpr int kQ = 128 * DP * 2;
   static constexpr int kOperand = kKeys * DP * 2;              // a tile of keys or values
-  static constexpr int kStages = (192 * 1024 - kTiles * kQ) / (2 * kOperand);
-  static constexpr int kRingAt = kTiles * kQ;
+  // (one of each for 128 columns: the next keys are loaded while the rows work, the next values while they work again)
+  static constexpr int kStages = DP == 64 ? 3 : DP == 128 ? 1 : 2;
+  static constexpr int kRingAt = kQ;
   static constexpr int kBarsAt = kRingAt + 2 * kStages * kOperand;
-  // q | k full, k empty, v full, v empty | s, p, o per row tile | a load of its own
-  static constexpr int kBars = 1 + 4 * kStages + 3 * kTiles + 1;
+  // q | k full, k empty, v full, v empty | s, p, o | a load of its own
+  static constexpr int kBars = 1 + 4 * kStages + 3 + 1;
   static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
   static constexpr int kSegmentAt = (kFlagsAt + 8 + 7) / 8 * 8;
   static constexpr int kBytes = kSegmentAt + static_cast<int>(sizeof(Segment));
-  static constexpr int kThreads = 128 * kTiles + (kTiles == 2 ? 128 : 64);  // the last: TMA, MMAs, two warps without work
-  static constexpr int kSCols = kKeys;
-  static constexpr int kOAt = kTiles * kSCols;
-  static_assert(kOAt + kTiles * DP <= 512, "tensor memory");
-  // The launch gives every thread 168 registers (three warps on a scheduler); a row's thread holds 128 scores and more.
-  // 256 x 208 + 128 x 88 = 384 x 168.  (The code after the instruction has its limit: one branch for each.)
-  __device__ static void take_registers() {
-    if constexpr (kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-  }
-  __device__ static void give_registers() {
-    if constexpr (kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  }
+  static constexpr int kThreads = 128 + 64;
+  static constexpr int kOAt = kKeys;                           // columns of tensor memory: S, then O
+  static constexpr int kColumns = DP == 256 ? 512 : 256;
+  static_assert(kOAt + DP <= kColumns, "tensor memory");
+  static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
 };
 
 struct PromptMaps {
@@ -85,10 +82,24 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   return r;
 }
 
+template <int N>
+__device__ __forceinline__ void store_weights(uint32_t at, const uint32_t (&w)[N]) {
+  if constexpr (N == 32) {
+    tmem_st32(at, w);
+  } else {
+    static_assert(N == 16, "half of a tile of 64 keys");
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+        "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11]),
+        "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+        : "memory");
+  }
+}
+
 constexpr int kPromptWaits = kWaits + 4;
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
+__global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
     prompt_kernel(const __grid_constant__ PromptMaps maps, const __grid_constant__ PromptArgs args) {
   using C = Prompt<DP>;
   extern __shared__ __align__(1024) char smem[];
@@ -96,7 +107,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   const Pool& p = a.pool;
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  constexpr int kProducer = 4 * C::kTiles, kIssuer = kProducer + 1;
+  constexpr int kProducer = 4, kIssuer = 5;
   volatile int* abort_flag = reinterpret_cast<int*>(smem + C::kFlagsAt);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kFlagsAt + 4);
   const uint32_t q_full = base + C::kBarsAt;
@@ -104,9 +115,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   auto k_empty = [&](int i) { return q_full + 8 * (1 + C::kStages + i); };
   auto v_full = [&](int i) { return q_full + 8 * (1 + 2 * C::kStages + i); };
   auto v_empty = [&](int i) { return q_full + 8 * (1 + 3 * C::kStages + i); };
-  auto s_full = [&](int t) { return q_full + 8 * (1 + 4 * C::kStages + t); };
-  auto p_full = [&](int t) { return q_full + 8 * (1 + 4 * C::kStages + C::kTiles + t); };
-  auto o_full = [&](int t) { return q_full + 8 * (1 + 4 * C::kStages + 2 * C::kTiles + t); };
+  const uint32_t s_full = q_full + 8 * (1 + 4 * C::kStages), p_full = s_full + 8, o_full = p_full + 8;
   const uint32_t alone = q_full + 8 * (C::kBars - 1);
   if (base % 1024) {  // (without static shared memory it starts there; swizzled tiles need it)
     if (tid == 0) atomicCAS(a.status, 0, kPromptWaits);
@@ -115,7 +124,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   if (tid == 0) {
     *abort_flag = 0;
     for (int i = 0; i < C::kBars; ++i) mbar_init(q_full + 8 * i, 1);
-    for (int t = 0; t < C::kTiles; ++t) mbar_init(p_full(t), 4);
+    mbar_init(p_full, 4);
     fence_mbar_init();
   }
   if (warp == kProducer && lane == 0) {
@@ -136,7 +145,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     if (lane == 0) *segment = next;
   }
   if (warp == kIssuer) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_alloc(smem_u32(tmem_slot), C::kColumns);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -145,32 +154,23 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const Segment g = *segment;
   if (g.s < 0) {
-    if (warp == kIssuer) tmem_dealloc(tmem, 512);
+    if (warp == kIssuer) tmem_dealloc(tmem, C::kColumns);
     return;
   }
 
-  // tiles of keys: [first, first + count[t]) for row tile t
-  const int first = g.lo / C::kKeys, token0 = g.tile * C::kTiles * args.tile_tokens;
-  int count[C::kTiles], most = 0;
-#pragma unroll
-  for (int t = 0; t < C::kTiles; ++t) {
-    const int from = token0 + t * args.tile_tokens, to = min(from + args.tile_tokens, g.n);
-    const int hi = from < g.n ? max(g.length - g.n + to, 0) : 0;
-    count[t] = max((hi + C::kKeys - 1) / C::kKeys - first, 0);
-    most = max(most, count[t]);
-  }
+  // tiles of keys: [first, first + count)
+  const int first = g.lo / C::kKeys, token0 = g.tile * args.tile_tokens;
+  const int count = max((g.hi + C::kKeys - 1) / C::kKeys - first, 0);
 
   if (warp < kProducer) {
     // ---------------- a thread per row ----------------
-    C::take_registers();
-    const int t = warp / 4, r = tid % 128;
+    const int r = tid;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-    const uint32_t s_at = tmem + lanes + t * C::kSCols, o_at = tmem + lanes + C::kOAt + t * DP;
-    const int token = token0 + t * args.tile_tokens + r / a.group;
+    const uint32_t s_at = tmem + lanes, o_at = s_at + C::kOAt;
+    const int token = token0 + r / a.group;
     const bool live = r < args.tile_tokens * a.group && token < g.n;
     const int position = g.length - g.n + token;
-    const int mine_count = t == 0 ? count[0] : count[C::kTiles - 1];
-    const int sure = g.length - g.n + token0 + t * args.tile_tokens + 1;  // keys below are seen by all rows of the tile
+    const int sure = g.first_position + 1;  // keys below are seen by all rows
     const int64_t clear = a.window ? static_cast<int64_t>(sure) - 1 + args.tile_tokens - a.window : 0;  // so are keys from here on
     const int boxes = C::kKeys / args.box;
     float top = kNone, sum = 0.f;
@@ -182,36 +182,48 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
       const int page = p.table[g.s * p.table_stride + at / p.page_size];
       return page < 0 || page >= p.pages;
     };
-    bool missing_next = mine_count > 0 && missing_box(0);
-    for (int j = 0; j < mine_count; ++j) {
+    bool missing_next = count > 0 && missing_box(0);
+    for (int j = 0; j < count; ++j) {
       const uint32_t missing = __ballot_sync(0xffffffffu, missing_next);
-      if (j + 1 < mine_count) missing_next = missing_box(j + 1);
-      alive = __all_sync(0xffffffffu, mbar_wait<0>(s_full(t), j & 1, abort_flag, a.status, kPromptWaits + 4));
+      if (j + 1 < count) missing_next = missing_box(j + 1);
+      alive = __all_sync(0xffffffffu, mbar_wait<0>(s_full, j & 1, abort_flag, a.status, kPromptWaits + 4));
       if (!alive) break;
       tc_fence_after();
-      float s[C::kKeys];
-#pragma unroll
-      for (int c = 0; c < C::kKeys; c += 32) tmem_ld32(s_at + c, reinterpret_cast<uint32_t*>(s) + c);
-      tmem_ld_wait();
+      // In halves of the columns: the second is kept while the maximum is found and turned into weights first, the first is read
+      // again (registers for a whole row at once do not go round with two blocks).
+      constexpr int kHalf = C::kKeys / 2;
       const int key = (first + j) * C::kKeys;
-      if (key + C::kKeys > sure || key < clear || key < g.lo || missing) {
+      const bool edge = key + C::kKeys > sure || key < clear || key < g.lo || missing;
+      float s[kHalf];
+      auto load = [&](int half) {
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 32) tmem_ld32(s_at + half * kHalf + c, reinterpret_cast<uint32_t*>(s) + c);
+        tmem_ld_wait();
+        if (!edge) return;
         if (missing) {
 #pragma unroll
-          for (int c = 0; c < C::kKeys; c += 16)
-            if (missing >> (c / args.box) & 1) {
+          for (int c = 0; c < kHalf; c += 16)
+            if (missing >> ((half * kHalf + c) / args.box) & 1) {
 #pragma unroll
               for (int e = 0; e < 16; ++e) s[c + e] = __int_as_float(0x7fffffff);
             }
         }
         const int64_t oldest = a.window ? position - a.window + 1 - key : 0;
-        const int to = min(position + 1, g.hi) - key, from = static_cast<int>(oldest < 0 ? 0 : oldest < C::kKeys ? oldest : C::kKeys);
+        const int to = min(position + 1, g.hi) - key - half * kHalf;
+        const int from = static_cast<int>(oldest < 0 ? 0 : oldest < C::kKeys ? oldest : C::kKeys) - half * kHalf;
 #pragma unroll
-        for (int c = 0; c < C::kKeys; ++c)
+        for (int c = 0; c < kHalf; ++c)
           if (c >= to || c < from) s[c] = -INFINITY;
-      }
+      };
       float high[4] = {top, kNone, kNone, kNone};
+      auto highest = [&]() {
 #pragma unroll
-      for (int c = 0; c < C::kKeys; c += 2) high[c / 2 % 4] = fmaxf(fmaxf(high[c / 2 % 4], s[c]), s[c + 1]);  // (of three: one instruction)
+        for (int c = 0; c < kHalf; c += 2) high[c / 2 % 4] = fmaxf(fmaxf(high[c / 2 % 4], s[c]), s[c + 1]);  // (of three: one instruction)
+      };
+      load(0);
+      highest();
+      load(1);
+      highest();
       const float now = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
       const bool grown = (now - top) * a.scale > 8.f;
       if (j == 0) {
@@ -233,20 +245,27 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
       const float shift = top == kNone ? 0.f : -top * a.scale;
       const uint64_t scale2 = pack_f2(a.scale, a.scale), shift2 = pack_f2(shift, shift);
       uint64_t sums[2] = {0, 0};  // pairs
+      uint32_t w[kHalf / 2];
+      auto weights = [&]() {
 #pragma unroll
-      for (int c = 0; c < C::kKeys; c += 64) {
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < kHalf / 2; ++e) {
           float x, y;
-          unpack_f2(fma_f2(pack_f2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2), x, y);
+          unpack_f2(fma_f2(pack_f2(s[2 * e], s[2 * e + 1]), scale2, shift2), x, y);
           x = exp2_fast(x);
           y = exp2_fast(y);
           sums[e % 2] = add_f2(sums[e % 2], pack_f2(x, y));
           w[e] = pack2(x, y, ElemTraits<T>::kDtype);
         }
-        tmem_st32(s_at + c / 2, w);
-      }
+      };
+      // (P's second half lies over S's first, which is read again before it is written)
+      uint32_t second[kHalf / 2];
+      weights();
+#pragma unroll
+      for (int e = 0; e < kHalf / 2; ++e) second[e] = w[e];
+      load(0);
+      weights();
+      store_weights<kHalf / 2>(s_at, w);
+      store_weights<kHalf / 2>(s_at + kHalf / 2, second);
       {
         float x, y;
         unpack_f2(add_f2(sums[0], sums[1]), x, y);
@@ -255,10 +274,10 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(t));
+      if (lane == 0) mbar_arrive(p_full);
     }
-    if (mine_count > 0 && alive)
-      alive = __all_sync(0xffffffffu, mbar_wait<20>(o_full(t), 0, abort_flag, a.status, kPromptWaits + 4));
+    if (count > 0 && alive)
+      alive = __all_sync(0xffffffffu, mbar_wait<20>(o_full, 0, abort_flag, a.status, kPromptWaits + 4));
     tc_fence_after();
     T* to = reinterpret_cast<T*>(a.out) + static_cast<int64_t>(g.start + token) * a.out_token +
             static_cast<int64_t>(g.head * a.group + r % a.group) * a.out_head;
@@ -267,7 +286,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
 #pragma unroll 1
     for (int c = 0; c < DP; c += 32) {
       uint32_t o[32];
-      if (mine_count > 0 && alive) {
+      if (count > 0 && alive) {
         tmem_ld32(o_at + c, o);
         tmem_ld_wait();
       } else {
@@ -288,25 +307,20 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
     }
     tc_fence_before();
   } else {
-    C::give_registers();
     if (warp == kProducer) {
       // ---------------- TMA: a lane for each box of a tile, tables 32 boxes ahead ----------------
       const int boxes = C::kKeys / args.box;
       const uint32_t bytes = static_cast<uint32_t>(args.box) * DP * 2;
       const int32_t* table = p.table + g.s * p.table_stride;
-      if (most > 0 && lane == 0) {
-        mbar_expect_tx(q_full, static_cast<uint32_t>(args.tile_tokens * a.group) * DP * 2 * C::kTiles);
+      if (count > 0 && lane == 0) {
+        mbar_expect_tx(q_full, static_cast<uint32_t>(args.tile_tokens * a.group) * DP * 2);
 #pragma unroll
-        for (int t = 0; t < C::kTiles; ++t)
-#pragma unroll
-          for (int b = 0; b < C::kBoxes; ++b)
-            tma_load_3d(base + t * C::kQ + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group,
-                        g.start + token0 + t * args.tile_tokens);
+        for (int b = 0; b < C::kBoxes; ++b) tma_load_3d(base + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group, g.start + token0);
       }
       int page_ahead = -2, ahead = 0;
       int loaded_k = 0, loaded_v = 0, lone = 0;
       bool alive = true;
-      for (int j = 0; j < most && alive; ++j) {
+      for (int j = 0; j < count && alive; ++j) {
         const int in_batch = j % (32 / boxes);
         if (in_batch == 0) {
           const int token = (first + j) * C::kKeys + lane * args.box;
@@ -378,7 +392,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
           mbar_wait<100>(k_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
         for (int j = loaded_v > C::kStages ? loaded_v - C::kStages : 0; j < loaded_v; ++j)
           mbar_wait<100>(v_full(j % C::kStages), j / C::kStages & 1, &zero, a.status, kPromptWaits + 2);
-        if (most > 0) mbar_wait<100>(q_full, 0, &zero, a.status, kPromptWaits + 2);
+        if (count > 0) mbar_wait<100>(q_full, 0, &zero, a.status, kPromptWaits + 2);
       }
     } else if (warp == kIssuer) {
       // ---------------- MMAs: the warp walks the loop, one lane issues ----------------
@@ -392,49 +406,46 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
       auto commit = [&](uint32_t bar) {
         if (one) umma_commit(bar);
       };
-      auto scores = [&](int t, int st) {
+      auto scores = [&](int st) {
         if (one) {
-          const uint32_t q = (base + t * C::kQ) >> 4 | 1u << 16, k = (base + C::kRingAt + st * C::kOperand) >> 4 | 1u << 16;
+          const uint32_t q = base >> 4 | 1u << 16, k = (base + C::kRingAt + st * C::kOperand) >> 4 | 1u << 16;
 #pragma unroll
           for (int i = 0; i < DP / 16; ++i) {
             const uint64_t qd = static_cast<uint64_t>(kDescHi) << 32 | (q + i / 4 * (128 * 128 >> 4) + i % 4 * 2);
             const uint64_t kd = static_cast<uint64_t>(kDescHi) << 32 | (k + i / 4 * (C::kKeys * 128 >> 4) + i % 4 * 2);
-            umma<2>(tmem + t * C::kSCols, qd, kd, args.idesc_s, i != 0);
+            umma<2>(tmem, qd, kd, args.idesc_s, i != 0);
           }
         }
-        commit(s_full(t));
+        commit(s_full);
       };
-      auto outputs = [&](int t, int st, bool more) {
+      auto outputs = [&](int st, bool more) {
         if (one) {
           const uint32_t v = (base + C::kRingAt + (C::kStages + st) * C::kOperand) >> 4 | static_cast<uint32_t>(C::kKeys * 128 >> 4) << 16;
 #pragma unroll
           for (int i = 0; i < C::kKeys / 16; ++i) {
             const uint64_t vd = static_cast<uint64_t>(kDescHi) << 32 | (v + i * (16 * 128 >> 4));
-            umma_ts(tmem + C::kOAt + t * DP, tmem + t * C::kSCols + i * 8, vd, args.idesc_o, more || i != 0);
+            umma_ts(tmem + C::kOAt, tmem + i * 8, vd, args.idesc_o, more || i != 0);
           }
         }
       };
-      if (most > 0 && wait(q_full, 0) && wait(k_full(0), 0)) {
+      if (count > 0 && wait(q_full, 0) && wait(k_full(0), 0)) {
         tc_fence_after();
-#pragma unroll
-        for (int t = 0; t < C::kTiles; ++t)
-          if (count[t] > 0) scores(t, 0);
+        scores(0);
         commit(k_empty(0));
-        for (int j = 0; j < most; ++j) {
+        for (int j = 0; j < count; ++j) {
           const int st = j % C::kStages, next = (j + 1) % C::kStages;
-          if (!wait(v_full(st), j / C::kStages & 1)) break;
-          if (j + 1 < most && !wait(k_full(next), (j + 1) / C::kStages & 1)) break;
-#pragma unroll
-          for (int t = 0; t < C::kTiles; ++t) {
-            if (j >= count[t] || !wait(p_full(t), j & 1)) continue;
-            tc_fence_after();
-            outputs(t, st, j > 0);
-            if (j + 1 == count[t]) commit(o_full(t));
-            else scores(t, next);  // (over P, which the MMAs before have read: they run in order)
-          }
-          if (!alive) break;
+          if (!wait(v_full(st), j / C::kStages & 1) || !wait(p_full, j & 1)) break;
+          tc_fence_after();
+          outputs(st, j > 0);
           commit(v_empty(st));
-          if (j + 1 < most) commit(k_empty(next));
+          if (j + 1 == count) {
+            commit(o_full);
+          } else {
+            if (!wait(k_full(next), (j + 1) / C::kStages & 1)) break;
+            tc_fence_after();
+            scores(next);  // (over P, which the products before have read: they run in order)
+            commit(k_empty(next));
+          }
         }
       }
       if (!alive) {
@@ -448,7 +459,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, 1)
   __syncthreads();
   if (warp == kIssuer) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, C::kColumns);
   }
 }
 
@@ -479,7 +490,7 @@ int launch_dim(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cu
 
 }  // namespace
 
-int prompt_rows(int dim, int group) { return (dim <= 128 ? 2 : 1) * (128 / group) * group; }
+int prompt_rows(int group) { return 128 / group * group; }
 
 bool prompt_fits(const ksmm_cache_attention_desc_t& d) {
   const int group = d.heads / d.cache.kv_heads;
