@@ -5,10 +5,12 @@
 // turns its S into weights (running maximum, exponentials, sum in fp32) and writes them back as 16-bit pairs, O += P V takes them
 // from tensor memory as its A operand.  P lies over S.
 //
-// Four warps of rows, one that issues TMA loads, one that issues MMAs; two blocks on an SM (up to 128 columns), each with half of
-// its tensor memory: while the rows of one work, the tensor cores run the other's products, and one's start and end (6 us, as
-// much as five tiles) pass under the other's work.  One block with two row tiles kept the same balance inside but not at its ends:
-// 32 prompts of 1000 tokens of 12 heads of 64 took 186 us.
+// Four warps of rows, one that issues TMA loads, one that issues MMAs; two blocks on an SM (four for up to 64 columns), each with its
+// part of the tensor memory: while the rows of one work, the tensor cores run another's products, and one's start and end (6 us,
+// as much as five tiles) pass under the others' work.  32 prompts of 1000 tokens, 12 heads of 64: 186 us with one block of two row
+// tiles, 181 with two blocks, 154 with four.  A prompt of 8192 tokens, 32/8 heads of 128: 505 us, 1090 TFLOP/s.
+// What bounds it: the issue of the rows' warps, not the exponentials' unit (a quarter of them as polynomials: 650 us), and the chain
+// of a tile: 3700 cycles for two blocks, of which the products are 2050.
 //
 // K is K-major as it lies in the pages, V is the MN-major operand (its tokens are the contraction), so neither is turned.  O stays in
 // tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the last time: weights are then at most
@@ -30,13 +32,15 @@ using namespace tc;
 
 template <int DP>
 struct Prompt {
-  static constexpr int kBlocks = DP == 256 ? 1 : 2;            // on an SM
-  static constexpr int kKeys = DP == 256 ? 64 : 128;           // tokens of a tile of keys
+  // Blocks on an SM, as tensor memory has room for their S and O; the more the better: a tile is a chain (products, loads, maximum,
+  // exponentials, stores) whose parts leave each unit idle most of the time.
+  static constexpr int kBlocks = DP == 64 ? 4 : DP == 128 ? 2 : 1;
+  static constexpr int kKeys = DP == 128 ? 128 : 64;           // tokens of a tile of keys
   static constexpr int kBoxes = DP / 64;                       // 128-byte columns of a row
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kOperand = kKeys * DP * 2;              // a tile of keys or values
   // (one of each for 128 columns: the next keys are loaded while the rows work, the next values while they work again)
-  static constexpr int kStages = DP == 64 ? 3 : DP == 128 ? 1 : 2;
+  static constexpr int kStages = DP == 128 ? 1 : 2;
   static constexpr int kRingAt = kQ;
   static constexpr int kBarsAt = kRingAt + 2 * kStages * kOperand;
   // q | k full, k empty, v full, v empty | s, p, o | a load of its own
@@ -46,7 +50,7 @@ struct Prompt {
   static constexpr int kBytes = kSegmentAt + static_cast<int>(sizeof(Segment));
   static constexpr int kThreads = 128 + 64;
   static constexpr int kOAt = kKeys;                           // columns of tensor memory: S, then O
-  static constexpr int kColumns = DP == 256 ? 512 : 256;
+  static constexpr int kColumns = 512 / kBlocks;
   static_assert(kOAt + DP <= kColumns, "tensor memory");
   static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
 };
@@ -507,8 +511,7 @@ int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream
   PromptArgs args = {};
   args.a = a;
   args.tile_tokens = 128 / a.group;
-  const int keys = p.dim <= 128 ? Prompt<128>::kKeys : Prompt<256>::kKeys;
-  static_assert(Prompt<64>::kKeys == Prompt<128>::kKeys, "one tile of keys up to 128 dims");
+  const int keys = p.dim <= 64 ? Prompt<64>::kKeys : p.dim <= 128 ? Prompt<128>::kKeys : Prompt<256>::kKeys;
   args.box = keys;
   while (p.page_size % args.box) args.box /= 2;
   const uint32_t fmt = dtype == KSMM_F16 ? 0u : 1u;
