@@ -5,7 +5,7 @@ A drop-in for the ``algo='kernel'`` path of the reference project: the same
 (``libksmm_cu.so``, declared in ``include/ksmm_cu.h``).
 """
 from ._lib import KsmmError, LIB_PATH  # noqa: F401
-from .attention import KVCache, cache_append, cache_attention, rotary_frequencies  # noqa: F401
+from .attention import KSAttention, KVCache, cache_append, cache_attention, rotary_frequencies  # noqa: F401
 from .interface import (KSGatedLinear, KSLinear, KSLinearGroup, from_kernel_format_to_abcd,  # noqa: F401
                         from_kernel_format_to_dense, generate_factor)
 from .kernel import (FactorFunction, Kernel, alloc_count, backward_input, backward_weights, chain_forward, check_device, default_choice, forward,  # noqa: F401
@@ -23,6 +23,6 @@ __all__ = [
     "backward_input", "backward_weights", "forward", "forward_ex", "forward_fp8", "chain_forward",
     "quantize_e4m3", "check_device", "launch_count", "default_choice", "generate_factor",
     "from_kernel_format_to_dense", "from_kernel_format_to_abcd", "KSGatedLinear", "gated_chain_forward", "residual_norm", "ResidualNorm",
-    "KVCache", "cache_append", "cache_attention", "rotary_frequencies",
+    "KSAttention", "KVCache", "cache_append", "cache_attention", "rotary_frequencies",
     "KsmmError", "LIB_PATH",
 ]

@@ -8,9 +8,11 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch import nn
 
 from . import _lib
 from ._lib import native as _native
+from .interface import KSLinear, KSLinearGroup
 from .kernel import _result, _stream_ptr, dtype_code, no_tangents
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -244,3 +246,88 @@ def cache_attention(q, cache, table, lengths, *, starts=None, scale=None, window
         ws = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
         _lib.check(lib.ksmm_cu_cache_attention(ctypes.byref(d), ws.data_ptr() if size else None, size, _stream_ptr(cache.device)))
     return result
+
+
+class KSAttention(nn.Module):
+    """Causal attention of a generating model with Kronecker-sparse projections: q, k and v from one input
+    (``KSLinearGroup``), rotated and appended to a ``KVCache`` (``cache_append``), attention over it (``cache_attention``) and the
+    output layer (``KSLinear``), whose last kernel adds the residual.  It serves prompts, single tokens and batches of
+    both; nothing learns through it.  The reference swaps the same four projections for Kronecker-sparse layers
+    (src/ksmm_py/model/get_vit.py:164-215) around an attention without a cache.
+
+    ``patterns``: of q, and of k and v where ``kv_patterns`` is None; ``kv_patterns`` with fewer features out give
+    fewer key heads (each ``heads * head_dim / features`` query heads share one).  ``rotary_base`` None: no rotation;
+    ``rotary_dim``: the features of a head that are rotated (default all)."""
+
+    def __init__(self, patterns, out_patterns, heads, kv_patterns=None, bias=True, algo="kernel", dtype: torch.dtype = torch.float16,
+                 device: str = "cuda", rotary_base=10000.0, rotary_dim=None, interleaved: bool = False, window=None, scale=None):
+        super().__init__()
+        if dtype not in _TYPES:
+            raise TypeError(f"attention runs in float32, float16 or bfloat16, not {dtype}")
+        if heads <= 0 or (window is not None and window <= 0):
+            raise ValueError("heads and window are positive")
+
+        def features(p):
+            return p[-1][0] * p[-1][1] * p[-1][3]
+
+        wide = features(patterns)
+        if wide % heads:
+            raise ValueError(f"{wide} features do not divide into {heads} heads")
+        self.heads, self.head_dim = int(heads), wide // heads
+        narrow = wide if kv_patterns is None else features(kv_patterns)
+        if narrow % self.head_dim or self.heads % max(narrow // self.head_dim, 1):
+            raise ValueError(f"{narrow} features of keys are no part of {heads} heads of {self.head_dim}")
+        self.kv_heads = narrow // self.head_dim
+        rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
+        if rotary_dim % 2 or not 0 <= rotary_dim <= self.head_dim:
+            raise ValueError(f"rotary_dim={rotary_dim}: an even number up to {self.head_dim}")
+        kw = dict(bias=bias, algo=algo, dtype=dtype, device=device)
+        out_in = out_patterns[0][0] * out_patterns[0][2] * out_patterns[0][3]
+        if out_in != wide:
+            raise ValueError(f"the output layer takes {out_in} features, the heads have {wide}")
+        if kv_patterns is None:
+            self.qkv = KSLinearGroup([KSLinear(patterns, **kw) for _ in range(3)])
+        else:
+            self.q = KSLinear(patterns, **kw)
+            self.kv = KSLinearGroup([KSLinear(kv_patterns, **kw) for _ in range(2)])
+        self.out = KSLinear(out_patterns, **kw)
+        self.rotary_base = rotary_base
+        self.dtype, self.window, self.scale, self.interleaved = dtype, window, scale, bool(interleaved)
+        frequencies = None if rotary_base is None else rotary_frequencies(rotary_dim // 2, rotary_base, device)
+        self.register_buffer("frequencies", frequencies, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        # (a change of the layers' type leaves the frequencies in 64 bits)
+        super()._apply(fn, recurse)
+        if self.frequencies is not None and self.frequencies.dtype != torch.float64:
+            self.frequencies = rotary_frequencies(self.frequencies.shape[0], self.rotary_base, self.frequencies.device)
+        return self
+
+    def new_cache(self, pages, page_size=64, eight=False):
+        """A ``KVCache`` for this layer, in its type or (``eight``) in 8 bits."""
+        device = next(self.out.parameters()).device
+        return KVCache(pages, page_size, self.kv_heads, self.head_dim, torch.float8_e4m3fn if eight else self.dtype, device)
+
+    def forward(self, x, cache, table, lengths, starts=None, max_new=None, residual=None):
+        """x: (..., features), flattened to tokens in the order that ``starts`` counts; with (sequences, n, features) and no
+        ``starts`` every sequence has n new tokens.  ``table``, ``lengths`` (with the new tokens), ``starts`` and ``max_new`` as in
+        ``cache_attention``; ``residual``: a tensor of the result's shape that is added to it."""
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise ValueError("x requires a gradient: a cache is not trained through")
+        flat = x.reshape(-1, x.shape[-1])
+        tokens = flat.shape[0]
+        if hasattr(self, "qkv"):
+            q, k, v = self.qkv(flat)
+        else:
+            q = self.q(flat)
+            k, v = self.kv(flat)
+        q = q.view(tokens, self.heads, self.head_dim)
+        k, v = (t.view(tokens, self.kv_heads, self.head_dim) for t in (k, v))
+        q = cache_append(cache, table, lengths, k, v, q=q, starts=starts, frequencies=self.frequencies, interleaved=self.interleaved)
+        a = cache_attention(q, cache, table, lengths, starts=starts, scale=self.scale, window=self.window, max_new=max_new)
+        y = self.out(a.view(tokens, -1), residual=None if residual is None else residual.reshape(tokens, -1))
+        return y.view(*x.shape[:-1], -1)
+
+    def extra_repr(self):
+        return "heads={}, kv_heads={}, head_dim={}, window={}, interleaved={}".format(
+            self.heads, self.kv_heads, self.head_dim, self.window, self.interleaved)

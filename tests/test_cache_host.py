@@ -114,6 +114,8 @@ def test_each_call_refuses():
     assert lib.ksmm_cu_cache_append(None, None) == _lib.KSMM_ERR_BAD_ARGUMENT
     assert lib.ksmm_cu_cache_attention(None, None, 0, None) == _lib.KSMM_ERR_BAD_ARGUMENT
     _, t = descs()
+    assert lib.ksmm_cu_cache_attention_workspace_bytes(ctypes.byref(t)) == 0  # (a table too short for anything to be split)
+    _, t = descs(table_width=4096)
     need = lib.ksmm_cu_cache_attention_workspace_bytes(ctypes.byref(t))
     assert need > 0
     for ws, size in ((None, need), (t.q, need - 1), (t.q + 16, need)):
@@ -121,3 +123,19 @@ def test_each_call_refuses():
     a, t = descs(tokens=0, sequences=0)
     assert lib.ksmm_cu_cache_append(ctypes.byref(a), None) == _lib.KSMM_OK
     assert lib.ksmm_cu_cache_attention(ctypes.byref(t), None, 0, None) == _lib.KSMM_OK
+
+
+def test_attention_layer_arguments():
+    q, o = [(6, 64, 64, 1), (1, 192, 192, 2)], [(6, 64, 64, 1), (1, 192, 192, 2)]
+    kw = dict(device="meta")
+    for args, more, text in (((q, o, 5), {}, "heads"), ((q, o, 0), {}, "positive"), ((q, o, 6), dict(window=0), "positive"),
+                             ((q, o, 6), dict(kv_patterns=[(6, 64, 64, 1), (1, 80, 192, 2)]), "no part"),
+                             ((q, o, 6), dict(kv_patterns=[(6, 64, 64, 1), (1, 128, 192, 2)]), "no part"),
+                             ((q, o, 6), dict(rotary_dim=33), "rotary_dim"), ((q, o, 6), dict(rotary_dim=66), "rotary_dim"),
+                             ((q, [(1, 64, 64, 4)], 6), {}, "output layer")):
+        with pytest.raises(ValueError, match=text):
+            kb.KSAttention(*args, **more, **kw)
+    with pytest.raises(TypeError):
+        kb.KSAttention(q, o, 6, dtype=torch.float8_e4m3fn)
+    with pytest.raises(NotImplementedError):
+        kb.KSAttention(q, o, 6, algo="dense")
