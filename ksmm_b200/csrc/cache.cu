@@ -468,8 +468,9 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   const int64_t sure = c.starts ? c.tokens : c.tokens / c.sequences;
   int64_t rows = (d.max_new > 0 && d.max_new < sure ? d.max_new : sure) * group;
   p->most = INT_MAX;
-  if (rows > kFewRows && prompt_fits(d)) {
-    p->prompt_tile = prompt_rows(static_cast<int>(group));
+  const bool floats = float_fits(d);
+  if (rows > kFewRows && (floats || prompt_fits(d))) {
+    p->prompt_tile = floats ? kFloatRows : prompt_rows(static_cast<int>(group));
     const int64_t n = items(c, group, p->prompt_tile);
     if (n >= INT_MAX) return false;
     p->prompt = static_cast<unsigned>(n);
@@ -592,12 +593,12 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.prompt) {
     a.tile_rows = plan.prompt_tile;
-    a.unit_log2 = 0;  // (its items are whole; their number is the grid's)
+    a.unit_log2 = 6;  // (its items are whole, and their number is the grid's; the fp32 kernel goes by units of 64 keys)
     a.narrow = 1;
     a.least = plan.grid ? plan.most + 1 : 1;
     a.most = INT_MAX;
     a.split = 0;
-    st = launch_prompt(a, d->dtype, plan.prompt, s);
+    st = d->dtype == KSMM_F32 ? launch_float(a, plan.prompt, s) : launch_prompt(a, d->dtype, plan.prompt, s);
     if (st != KSMM_OK || !plan.grid) return st;
     a.clear_rest = 0;
   }

@@ -313,6 +313,9 @@ int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cud
 int prompt_rows(int group);       // rows of an item in the prompt kernel
 bool prompt_fits(const ksmm_cache_attention_desc_t& d);
 int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
+constexpr int kFloatRows = 64;    // rows and keys of a tile in the fp32 prompt kernel
+bool float_fits(const ksmm_cache_attention_desc_t& d);
+int launch_float(const Attend& a, unsigned grid, cudaStream_t stream);
 int launch_join(const Attend& a, int dtype, unsigned blocks, int rows, cudaStream_t stream);  // rows: of an item, at most
 
 }  // namespace cache
