@@ -6,6 +6,7 @@ The reference's attention sees one image at a time and keeps nothing (src/ksmm_p
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 from torch import nn
@@ -220,13 +221,14 @@ def cache_attention(q, cache, table, lengths, *, starts=None, scale=None, window
     and left alone in ``out``.  Rows that need a page which is not in the pool are NaN.  Nothing learns through this call."""
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
+    window, max_new = (None if n is None else operator.index(n) for n in (window, max_new))
     if window is not None and window <= 0 or max_new is not None and max_new <= 0:
         raise ValueError("window and max_new are positive")
     if _native is not None and _tensors(q, table, lengths) and _tensors_or_none(starts, out):
         done = _native.cache_attention(q, cache.keys, cache.values, cache.key_scales, cache.value_scales, table, lengths, starts,
                                        cache.keys.shape[3] ** -0.5 if scale is None else float(scale),
-                                       0 if window is None else min(int(window), _MAX_INT),
-                                       0 if max_new is None else min(int(max_new), _MAX_INT), out)
+                                       0 if window is None else min(window, _MAX_INT),
+                                       0 if max_new is None else min(max_new, _MAX_INT), out)
         if done is not None:
             return _result(done)
     no_tangents(q)
@@ -237,7 +239,7 @@ def cache_attention(q, cache, table, lengths, *, starts=None, scale=None, window
     result = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else _output("out", out, q, cache.device)
     d = _lib.CacheAttentionDesc(
         cache=desc, q=q.data_ptr(), out=result.data_ptr(), q_strides=_strides(q, 2), out_strides=_strides(result, 2),
-        window=0 if window is None else min(int(window), _MAX_INT), max_new=0 if max_new is None else min(int(max_new), _MAX_INT),
+        window=0 if window is None else min(window, _MAX_INT), max_new=0 if max_new is None else min(max_new, _MAX_INT),
         scale=cache.head_dim ** -0.5 if scale is None else float(scale), heads=q.shape[1], dtype=dtype_code(q.dtype),
         clear_rest=int(out is None))
     lib = _lib.load()
@@ -325,8 +327,9 @@ class KSAttention(nn.Module):
         k, v = (t.view(tokens, self.kv_heads, self.head_dim) for t in (k, v))
         q = cache_append(cache, table, lengths, k, v, q=q, starts=starts, frequencies=self.frequencies, interleaved=self.interleaved)
         a = cache_attention(q, cache, table, lengths, starts=starts, scale=self.scale, window=self.window, max_new=max_new)
-        y = self.out(a.view(tokens, -1), residual=None if residual is None else residual.reshape(tokens, -1))
-        return y.view(*x.shape[:-1], -1)
+        wide, out = self.heads * self.head_dim, self.out.out_size
+        y = self.out(a.view(tokens, wide), residual=None if residual is None else residual.reshape(tokens, out))
+        return y.view(*x.shape[:-1], out)
 
     def extra_repr(self):
         return "heads={}, kv_heads={}, head_dim={}, window={}, interleaved={}".format(

@@ -1,4 +1,4 @@
-"""Builds libksmm_cu.so in-tree with nvcc for sm_100a (`python -m ksmm_b200.build`)."""
+"""Builds libksmm_cu.so and libksmm_cache.so in-tree with nvcc for sm_100a (`python -m ksmm_b200.build`)."""
 from __future__ import annotations
 
 import os
@@ -16,9 +16,10 @@ def build_library(jobs=None, verbose=False):
     if res.returncode != 0:
         sys.stderr.write((res.stdout or "") + (res.stderr or ""))
         raise RuntimeError("building libksmm_cu.so failed")
-    lib = os.path.join(HERE, "libksmm_cu.so")
-    if not os.path.exists(lib):
-        raise RuntimeError(f"{lib} was not produced")
+    lib, cache = (os.path.join(HERE, name) for name in ("libksmm_cu.so", "libksmm_cache.so"))
+    for path in (lib, cache):
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} was not produced")
     return lib
 
 

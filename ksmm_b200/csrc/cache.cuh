@@ -57,12 +57,23 @@ struct Attend {
   int clear_rest;
   int tile_rows;        // rows (token, head of the group) of an item
   int unit_log2;        // of the tokens of a unit, the piece in which a cache's length is split
-  int narrow;           // all sequences' units fit 31 bits
   int least, most;      // sequences with fewer or more rows in a group are another kernel's
   int split;            // an item's units may be several CTAs'
   float* partial;       // split: 2 slots per CTA of tile_rows * (dim + 2) floats
   int64_t* slots;       // split: the item of each slot, or -1
   int* status;
+};
+
+struct Append {
+  Pool pool;
+  const char* in[3];     // q, k, v
+  char* q_out;
+  int64_t token[3], head[3], out_token, out_head;
+  const double* frequencies;
+  int pairs, interleaved, heads, clear_rest;
+  int lanes;             // threads of a row, a power of two up to 32
+  int chunks;            // of a token: chunk_rows rows each
+  int chunk_rows;
 };
 
 // An item: up to tile_rows rows of one sequence and one key head.  They are numbered sequence by sequence, then head by head.
@@ -80,23 +91,21 @@ __device__ __forceinline__ int first_key(const Attend& a, const Sequence& q, int
 // units up to a token; a length is at most 2^31 - 65537
 __device__ __forceinline__ int units_to(const Attend& a, int length) { return (length + (1 << a.unit_log2) - 1) >> a.unit_log2; }
 
-// (a division in 64 bits takes several hundred cycles, and a block's start is a chain of them)
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+// (Out of line, once: inlined in a dozen places it was three quarters of a kernel's code, and a block's start waited for that to be
+// fetched.  In 32 bits where they suffice: 64 take several hundred cycles.)
+static __device__ __noinline__ int64_t divide(int64_t a, int64_t b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
 
+// (the host has seen to it that rows and their tiles fit 32 bits)
 __device__ __forceinline__ Work work_of(const Attend& a, const Sequence& q) {
   Work w;
-  const int64_t rows = static_cast<int64_t>(q.n) * a.group;
-  if (rows < a.least || rows > a.most) {
-    w.units = w.tiles = 0;
-    w.items = 0;
-    return w;
-  }
-  w.tiles = static_cast<int>(divide(rows + a.tile_rows - 1, a.tile_rows));
+  const int rows = q.n * a.group;
+  const bool mine = rows >= a.least && rows <= a.most;
+  w.tiles = mine ? static_cast<unsigned>(rows + a.tile_rows - 1) / static_cast<unsigned>(a.tile_rows) : 0;
   // (a sequence without keys is a unit of work as well: its rows are zeros)
-  w.units = max(1, units_to(a, q.length) - (first_key(a, q, 0) >> a.unit_log2));
+  w.units = mine ? max(1, units_to(a, q.length) - (first_key(a, q, 0) >> a.unit_log2)) : 0;
   w.items = static_cast<int64_t>(w.tiles) * a.pool.kv_heads;
   return w;
 }
@@ -134,25 +143,39 @@ struct Walker {
 
   // A lane sums a run of sequences, the warp forms the runs' prefix sums, and the run that holds the block's first unit is walked by
   // its lane.  false: nothing to do (a split block then has marked its slots).
-  template <typename Count>
-  __device__ bool start_counted(const Attend& a) {
+  __device__ bool start(const Attend& a) {
+    if (!a.split && !a.pool.starts) {
+      // (all sequences have the same number of items)
+      const int rows = a.pool.each * a.group;
+      const int per = rows < a.least || rows > a.most ? 0 : (rows + a.tile_rows - 1) / a.tile_rows * a.pool.kv_heads;
+      const int which = per ? blockIdx.x / static_cast<unsigned>(per) : a.pool.sequences;
+      if (which >= a.pool.sequences) return false;
+      left = 1;
+      whole = true;
+      from = 0;
+      set(a, which);
+      const int item = blockIdx.x - which * per, t = item / a.pool.kv_heads;
+      head = item - t * a.pool.kv_heads;
+      tile = work.tiles - 1 - t;
+      return true;
+    }
     constexpr uint32_t kAll = 0xffffffffu;
     const int lane = threadIdx.x % 32;
     const int run = (a.pool.sequences + 31) / 32;
     const int first = min(lane * run, a.pool.sequences), end = min(first + run, a.pool.sequences);
-    Count units = 0, items = 0;
+    int64_t units = 0, items = 0;
     int most = 0;
-#pragma unroll 4
+#pragma unroll 1
     for (int i = first; i < end; ++i) {
       const Work w = work_of(a, sequence(a.pool, i));
-      units += static_cast<Count>(w.items) * w.units;
-      items += static_cast<Count>(w.items);
+      units += w.items * w.units;
+      items += w.items;
       most = max(most, w.units);
     }
-    Count units_before = units, items_before = items;
-#pragma unroll
+    int64_t units_before = units, items_before = items;
+#pragma unroll 1
     for (int d = 1; d < 32; d *= 2) {
-      const Count u = __shfl_up_sync(kAll, units_before, d), n = __shfl_up_sync(kAll, items_before, d);
+      const int64_t u = __shfl_up_sync(kAll, units_before, d), n = __shfl_up_sync(kAll, items_before, d);
       if (lane >= d) {
         units_before += u;
         items_before += n;
@@ -209,25 +232,6 @@ struct Walker {
     return true;
   }
 
-  __device__ bool start(const Attend& a) {
-    if (!a.split && !a.pool.starts) {
-      // (all sequences have the same number of items)
-      const int64_t rows = static_cast<int64_t>(a.pool.each) * a.group;
-      const int64_t per = rows < a.least || rows > a.most ? 0 : divide(rows + a.tile_rows - 1, a.tile_rows) * a.pool.kv_heads;
-      if (blockIdx.x >= per * a.pool.sequences) return false;
-      const int which = static_cast<int>(divide(blockIdx.x, per));
-      left = 1;
-      whole = true;
-      from = 0;
-      set(a, which);
-      const int64_t item = blockIdx.x - which * per, t = divide(item, a.pool.kv_heads);
-      head = static_cast<int>(item - t * a.pool.kv_heads);
-      tile = work.tiles - 1 - static_cast<int>(t);
-      return true;
-    }
-    return a.narrow ? start_counted<int>(a) : start_counted<int64_t>(a);
-  }
-
   // the next segment; one with s < 0 where there is none
   __device__ void next(const Attend& a, Segment* g) {
     g->s = -1;
@@ -247,7 +251,7 @@ struct Walker {
     g->n = seq.n;
     g->length = seq.length;
     g->bad = seq.bad;
-    const int t0 = static_cast<int>(divide(static_cast<int64_t>(tile) * a.tile_rows, a.group));
+    const int t0 = tile * a.tile_rows / a.group;
     g->first_position = seq.length - seq.n + t0;
     g->lo = first_key(a, seq, a.split ? 0 : t0);
     g->hi = seq.length;
@@ -257,8 +261,8 @@ struct Walker {
       g->to = g->from + to;
       g->from += from;
     } else {
-      const int64_t t1 = divide(static_cast<int64_t>(tile + 1) * a.tile_rows - 1, a.group);
-      g->hi = max(seq.length - seq.n + static_cast<int>(t1 < seq.n ? t1 + 1 : seq.n), 0);
+      const int t1 = ((tile + 1) * a.tile_rows - 1) / a.group;
+      g->hi = max(seq.length - seq.n + (t1 < seq.n ? t1 + 1 : seq.n), 0);
       g->to = units_to(a, g->hi);
     }
     // a block's first segment may continue an item, its last may be continued; one that is both is the first
@@ -296,26 +300,39 @@ __device__ void clear_rest(const Attend& a) {
   }
 }
 
-// host side: each returns a status
-constexpr int kMaxBlocks = 512;  // of a split launch (the join kernel's table of weights)
-constexpr int kRowsUnit = 64;     // tokens of a unit in the CUDA-core kernel
-constexpr int kFewRowsTile = 2;
-int rows_tile(int dim, int64_t rows);  // rows of an item there, where there are so many
-constexpr int row_blocks(int dim, int tile) { return tile == kFewRowsTile && dim <= 64 ? 2 : 1; }  // on an SM
-int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
+// ---------------------------------------------------------------------------
+// host side: what the entry points plan with, and the launches (each returns a status)
+// ---------------------------------------------------------------------------
+constexpr int kMaxBlocks = 512;   // of a split launch (the join kernel's table of weights)
+
 struct TokenShape {
   int blocks, unit;  // blocks on an SM, tokens of a unit
 };
-TokenShape token_shape(int cache_dtype, int dim);
-inline int token_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }  // of an item in the 16- and 8-bit kernel
-bool token_fits(const ksmm_cache_attention_desc_t& d);
-int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
-int prompt_rows(int group);       // rows of an item in the prompt kernel
-bool prompt_fits(const ksmm_cache_attention_desc_t& d);
-int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
+
+// The 16- and 8-bit kernel for few rows.  A step of a warp is a chain (load, products, maximum, exponentials, products) of 1000 to
+// 1500 cycles however many tokens it has, and an SM has to pass 23 bytes a cycle: small rows take 32 tokens of a step, wide ones 16.
+constexpr int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+constexpr TokenShape token_shape(bool eight, int dp) { return {dp == 256 ? 1 : 2, 4 * (dp == 256 || (!eight && dp == 128) ? 16 : 32)}; }
+// Rows of an item.  Sixteen are built for 16-bit caches of up to 128 columns; others go through their keys, the second time in the cache
+// of the GPU, once for every eight (each variant is 90 KB of code).
+inline int token_rows(int64_t rows, bool eight, int dim) { return rows <= 8 || eight || dim > 128 ? 8 : 16; }
+
+// The fp32 kernel for few rows: rows and tokens of an item's pieces, blocks on an SM.
+constexpr int kRowsUnit = 64;
+constexpr int kFewRowsTile = 2;
+inline int rows_tile(int dim, int64_t rows) { return rows <= kFewRowsTile || dim > 128 ? kFewRowsTile : dim <= 64 ? 8 : 4; }
+constexpr int row_blocks(int dim, int tile) { return tile == kFewRowsTile && dim <= 64 ? 2 : 1; }
+
+constexpr int kPlainRows = 8;     // rows of an item in the kernel for what no other takes
 constexpr int kFloatRows = 64;    // rows and keys of a tile in the fp32 prompt kernel
-bool float_fits(const ksmm_cache_attention_desc_t& d);
+inline int prompt_rows(int group) { return 128 / group * group; }
+
+int launch_append(Append& a, int dtype, int cache_dtype, cudaStream_t stream);
+int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
+int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
 int launch_float(const Attend& a, unsigned grid, cudaStream_t stream);
+int launch_rows(const Attend& a, unsigned grid, cudaStream_t stream);
+int launch_plain(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
 int launch_join(const Attend& a, int dtype, unsigned blocks, int rows, cudaStream_t stream);  // rows: of an item, at most
 
 }  // namespace cache

@@ -494,18 +494,6 @@ int launch_dim(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cu
 
 }  // namespace
 
-int prompt_rows(int group) { return 128 / group * group; }
-
-bool prompt_fits(const ksmm_cache_attention_desc_t& d) {
-  const int group = d.heads / d.cache.kv_heads;
-  if (d.cache.cache_dtype == KSMM_F8E4M3 || !token_fits(d) || group > 128) return false;
-  // (a negative scale would turn the maximum round)
-  if (!(d.scale > 0.f) || d.scale > 1e30f) return false;
-  return reinterpret_cast<uintptr_t>(d.q) % 16 == 0 && reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.q_strides[0] > 0 &&
-         d.q_strides[1] > 0 && d.q_strides[0] % 8 == 0 && d.q_strides[1] % 8 == 0 && d.q_strides[0] < (1ll << 38) &&
-         d.q_strides[1] < (1ll << 38) && d.out_strides[0] % 8 == 0 && d.out_strides[1] % 8 == 0;
-}
-
 int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream) {
   const Pool& p = a.pool;
   PromptArgs args = {};

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kFloatThreads, Float<DP>::kBlocks) float_kerne
       const int r = e / (DP / 4), d = e % (DP / 4) * 4;
       const int64_t at = from[r];
       const bool there = at >= 0 && d < p.dim;  // (zeros else: what the rows do not see stays out of the sums)
-      copy16(to + 4 * (r * C::kRow + d), there ? data[kv] + at + d : data[kv], there);
+      copy16(to + 4 * (r * C::kRow + d), there ? data[kv] + at + d : reinterpret_cast<const float*>(a.q), there);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -231,18 +231,6 @@ int launch_one(const Attend& a, unsigned grid, cudaStream_t stream) {
 }
 
 }  // namespace
-
-// Vectors of four everywhere.
-bool float_fits(const ksmm_cache_attention_desc_t& d) {
-  const ksmm_cache_t& c = d.cache;
-  if (d.dtype != KSMM_F32 || c.cache_dtype != KSMM_F32 || c.head_dim % 4 || c.pages == 0) return false;
-  auto whole = [](const void* p, const int64_t* s, int n) {
-    bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
-    for (int i = 0; i < n; ++i) ok = ok && s[i] % 4 == 0;
-    return ok;
-  };
-  return whole(c.keys, c.key_strides, 3) && whole(c.values, c.value_strides, 3) && whole(d.q, d.q_strides, 2) && whole(d.out, d.out_strides, 2);
-}
 
 int launch_float(const Attend& a, unsigned grid, cudaStream_t stream) {
   if (a.pool.dim <= 64) return launch_one<64>(a, grid, stream);

@@ -16,9 +16,9 @@ namespace {
 
 constexpr int kRowThreads = 256;
 // Keys and values on their way: each thread copies its own pieces asynchronously into shared memory, kSlots units deep, and reads
-// them back itself, without a barrier.  Wider rows would fill it with one unit; elements one by one cannot be copied so.
+// them back itself, without a barrier.  Wider rows would fill it with one unit.
 constexpr int kSlots = 3;
-constexpr bool row_ring(int vec, int dpl) { return vec == 4 && dpl <= 16; }
+constexpr bool row_ring(int dpl) { return dpl <= 16; }
 
 template <int N>
 struct Bytes;
@@ -57,10 +57,12 @@ __device__ __forceinline__ void load_row(const T* row, int l, int dim, bool ther
 
 // R: rows of an item.  Where a key head has one or two, registers for no more let several blocks share an SM, which is what keeps
 // enough loads in flight (32 sequences of 12 heads of 64, fp32: 123 us with one block of eight rows, 67 with two of two rows, 74 with three).
-template <typename T, typename C, int DPL, int VEC, int R>
+template <int DPL, int R>
 __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kernel(const __grid_constant__ Attend a) {
-  constexpr bool kEight = sizeof(C) == 1;
-  constexpr bool kRing = row_ring(VEC, DPL);
+  using T = float;
+  using C = float;
+  constexpr int VEC = 4;
+  constexpr bool kRing = row_ring(DPL);
   __shared__ Segment segment;
   __shared__ float stats[2][kRowThreads / 32][R];
   extern __shared__ __align__(16) char smem[];
@@ -118,6 +120,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
       constexpr int kPiece = VEC * static_cast<int>(sizeof(C));
       return ring + static_cast<uint32_t>(((((slot * 2 + h) * 2 + kv) * (DPL / VEC) + j) * kRowThreads + tid) * kPiece);
     };
+    const C* nowhere = reinterpret_cast<const C*>(a.q);  // (a copy of no bytes still names an address)
     uint32_t gone = 0;  // a bit per token fetched, the last ones lowest: its page is not there
     int fetched = g.from, slot_in = 0, slot_out = 0;
     auto fetch = [&]() {
@@ -134,10 +137,8 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
             const int d = (j * 8 + l) * VEC;
             const bool take = get && d < p.dim;
             // (zeros where there is nothing)
-            if constexpr (VEC * sizeof(C) == 16)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at(slot_in, h, kv, j)), "l"(take ? row + d : data[kv]), "r"(take ? 16 : 0) : "memory");
-            else if constexpr (kRing)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(mine_at(slot_in, h, kv, j)), "l"(take ? row + d : data[kv]), "r"(take ? static_cast<int>(VEC * sizeof(C)) : 0), "n"(VEC * sizeof(C)) : "memory");
+            if constexpr (kRing)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_at(slot_in, h, kv, j)), "l"(take ? row + d : nowhere), "r"(take ? 16 : 0) : "memory");
           }
         }
       }
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
     }
 #pragma unroll 1
     for (int unit = g.from; unit < g.to; ++unit) {
-      float k[2][DPL], v[2][DPL], ks[2], vs[2];
+      float k[2][DPL], v[2][DPL];
       int j[2];
       bool there[2], bad[2];
       if constexpr (kRing) {
@@ -163,9 +164,6 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
       for (int h = 0; h < 2; ++h) {
         j[h] = unit * kRowsUnit + h * 32 + at;
         there[h] = j[h] >= g.lo && j[h] < g.hi;
-        ks[h] = vs[h] = 1.f;
-        int64_t page;
-        int nth;
         if constexpr (kRing) {
           bad[h] = gone >> (2 * (kSlots - 1) + h) & 1;
 #pragma unroll
@@ -173,33 +171,17 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
             load<C, VEC>(reinterpret_cast<const C*>(smem + (mine_at(slot_out, h, 0, c) - smem_base)), k[h] + c * VEC);
             load<C, VEC>(reinterpret_cast<const C*>(smem + (mine_at(slot_out, h, 1, c) - smem_base)), v[h] + c * VEC);
           }
-          if (kEight) {
-            nth = j[h] / p.page_size;
-            page = there[h] && !bad[h] ? table[nth] : 0;
-            nth = j[h] - nth * p.page_size;
-          }
         } else {
-          page = page_next[h];
-          nth = row_next[h];
+          const int64_t page = page_next[h];
+          const int nth = row_next[h];
           bad[h] = there[h] && (page < 0 || page >= p.pages);
           const bool get = there[h] && !bad[h];
           load_row<C, DPL, VEC>(data[0] + page * p.page[0] + g.head * p.head[0] + nth * p.token[0], l, p.dim, get, k[h]);
           load_row<C, DPL, VEC>(data[1] + page * p.page[1] + g.head * p.head[1] + nth * p.token[1], l, p.dim, get, v[h]);
         }
-        if (kEight && there[h] && !bad[h]) {
-          ks[h] = p.scales[0][page * p.spage[0] + g.head * p.shead[0] + nth * p.stoken[0]];
-          vs[h] = p.scales[1][page * p.spage[1] + g.head * p.shead[1] + nth * p.stoken[1]];
-        }
       }
       if constexpr (kRing) slot_out = slot_out + 1 == kSlots ? 0 : slot_out + 1;
       else look(unit + 1);
-      if (kEight) {
-#pragma unroll
-        for (int e = 0; e < DPL; ++e) {
-          v[0][e] *= vs[0];
-          v[1][e] *= vs[1];
-        }
-      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r >= rows) continue;
@@ -212,7 +194,6 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
           d += __shfl_xor_sync(0xffffffffu, d, 1);
           d += __shfl_xor_sync(0xffffffffu, d, 2);
           d += __shfl_xor_sync(0xffffffffu, d, 4);
-          if (kEight) d *= ks[h];
           s[h] = bad[h] ? __int_as_float(0x7fffffff) : d * a.scale;
         }
         bool sees[2];
@@ -295,6 +276,117 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
         const int row = g.tile * R + r, t = row / a.group;
         reinterpret_cast<T*>(a.out)[(g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head + d] =
             ElemTraits<T>::from_float(total == 0.f ? 0.f : out / total);
+      }
+    }
+    __syncthreads();
+  }
+  if (a.split && tid < 2 && !slot_used[tid]) a.slots[2 * blockIdx.x + tid] = -1;
+}
+
+// Any type, alignment and page size, one element at a time: a warp for each row, a lane for each of 32 keys while the scores are
+// formed and for every 32nd column while the values are added.  (Rows of eight lanes in all these variants were 4 MB of code.)
+constexpr int kPlainThreads = 32 * kPlainRows;
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(kPlainThreads) plain_kernel(const __grid_constant__ Attend a) {
+  constexpr bool kEight = sizeof(C) == 1;
+  __shared__ Segment segment;
+  __shared__ float q[kPlainRows][kMaxDim];
+  touch_parameters(a);
+  tc::grid_dep_wait();
+  tc::grid_dep_launch();
+  clear_rest<T>(a);
+  const Pool& p = a.pool;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  Walker walker;  // the first warp's
+  bool some = true;
+  if (warp == 0) some = walker.start(a);
+  if (!__syncthreads_or(warp == 0 && some)) return;
+  bool slot_used[2] = {false, false};
+  while (true) {
+    if (warp == 0) {
+      Segment next;
+      walker.next(a, &next);
+      if (lane == 0) segment = next;
+    }
+    __syncthreads();
+    const Segment g = segment;
+    if (g.s < 0) break;
+    if (g.slot) slot_used[g.slot - 1] = true;
+    const int rows = min(kPlainRows, g.n * a.group - g.tile * kPlainRows);
+    const int row = g.tile * kPlainRows + warp, t = row / a.group, position = g.length - g.n + t;
+    if (warp < rows) {
+      const T* from = reinterpret_cast<const T*>(a.q) + (g.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
+      for (int d = lane; d < p.dim; d += 32) q[warp][d] = ElemTraits<T>::to_float(from[d]);
+      __syncwarp();
+      float m = kNone, sum = 0.f, o[kMaxDim / 32];
+#pragma unroll
+      for (int c = 0; c < kMaxDim / 32; ++c) o[c] = 0.f;
+      const int last = min(g.to << a.unit_log2, g.hi);
+#pragma unroll 1
+      for (int key0 = max(g.from << a.unit_log2, g.lo); key0 < last; key0 += 32) {
+        const int key = key0 + lane;
+        const bool sees = key < last && key <= position && (!a.window || key > position - a.window);
+        int64_t page = -1, nth = 0;
+        float s = -INFINITY;
+        if (sees) {
+          const int at = key / p.page_size;
+          nth = key - at * p.page_size;
+          page = p.table[g.s * p.table_stride + at];
+          if (page < 0 || page >= p.pages) {
+            page = -1;
+            s = __int_as_float(0x7fffffff);
+          } else {
+            const C* k = reinterpret_cast<const C*>(p.data[0]) + page * p.page[0] + g.head * p.head[0] + nth * p.token[0];
+            float dot = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < p.dim; ++d) dot = fmaf(q[warp][d], ElemTraits<C>::to_float(k[d]), dot);
+            if (kEight) dot *= p.scales[0][page * p.spage[0] + g.head * p.shead[0] + nth * p.stoken[0]];
+            s = dot * a.scale;
+          }
+        }
+        float top = s;
+#pragma unroll
+        for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, m);
+        const float f = exp2f(m - top), w = exp2f(s - top);
+        m = top;
+        sum = sum * f + w;  // (of this lane's keys)
+#pragma unroll
+        for (int c = 0; c < kMaxDim / 32; ++c) o[c] *= f;
+        const int64_t at = page * p.page[1] + g.head * p.head[1] + nth * p.token[1];
+        const float scale = kEight && page >= 0 ? p.scales[1][page * p.spage[1] + g.head * p.shead[1] + nth * p.stoken[1]] : 1.f;
+        const int n = min(32, last - key0);
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+          // (keys that the row does not see, or that are not there, add nothing)
+          if (__shfl_sync(0xffffffffu, page, j) < 0) continue;
+          const C* v = reinterpret_cast<const C*>(p.data[1]) + __shfl_sync(0xffffffffu, at, j);
+          const float x = __shfl_sync(0xffffffffu, w * scale, j);
+#pragma unroll
+          for (int c = 0; c < kMaxDim / 32; ++c)
+            if (lane + 32 * c < p.dim) o[c] = fmaf(x, ElemTraits<C>::to_float(v[lane + 32 * c]), o[c]);
+        }
+      }
+#pragma unroll
+      for (int x = 16; x; x /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (g.bad) sum = __int_as_float(0x7fffffff);
+      if (g.slot) {
+        float* part = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + g.slot - 1) * kPlainRows * (p.dim + 2);
+        if (tid == 0) a.slots[2 * blockIdx.x + g.slot - 1] = g.item;
+#pragma unroll
+        for (int c = 0; c < kMaxDim / 32; ++c)
+          if (lane + 32 * c < p.dim) part[warp * p.dim + lane + 32 * c] = o[c];
+        if (lane == 0) {
+          part[kPlainRows * p.dim + warp] = m;
+          part[kPlainRows * (p.dim + 1) + warp] = sum;
+        }
+      } else {
+        T* to = reinterpret_cast<T*>(a.out) + (g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head;
+        const float back = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int c = 0; c < kMaxDim / 32; ++c)
+          if (lane + 32 * c < p.dim) to[lane + 32 * c] = ElemTraits<T>::from_float(o[c] * back);
       }
     }
     __syncthreads();
@@ -401,60 +493,49 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   out[tid] = ElemTraits<T>::from_float(total == 0.f ? 0.f : all / total);
 }
 
-template <typename T, typename C, int DPL, int VEC, int R>
+template <int DPL, int R>
 int launch_one(const Attend& a, unsigned grid, cudaStream_t stream) {
-  constexpr size_t smem = kRowThreads / 32 * R * DPL * 8 * sizeof(float) +
-                          (row_ring(VEC, DPL) ? kSlots * 4 * DPL * sizeof(C) * kRowThreads : 0);
+  constexpr size_t smem = kRowThreads / 32 * R * DPL * 8 * sizeof(float) + (row_ring(DPL) ? kSlots * 4 * DPL * sizeof(float) * kRowThreads : 0);
   static std::atomic<uint64_t> ready{0};  // a bit per device
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (err == cudaSuccess && !(ready.load(std::memory_order_acquire) & bit)) {
-    err = cudaFuncSetAttribute(rows_kernel<T, C, DPL, VEC, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    err = cudaFuncSetAttribute(rows_kernel<DPL, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
   }
-  if (err == cudaSuccess) err = tc::launch_pdl(rows_kernel<T, C, DPL, VEC, R>, grid, kRowThreads, smem, stream, a);
+  if (err == cudaSuccess) err = tc::launch_pdl(rows_kernel<DPL, R>, grid, kRowThreads, smem, stream, a);
   if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention rows kernel: %s", cudaGetErrorString(err));
   count_launch();
   return KSMM_OK;
 }
 
-template <typename T, typename C, int VEC>
-int launch_vec(const Attend& a, unsigned grid, cudaStream_t stream) {
-  const int dim = a.pool.dim;
-  const bool few = a.tile_rows == kFewRowsTile;
-  if (dim <= 64) return few ? launch_one<T, C, 8, VEC, kFewRowsTile>(a, grid, stream) : launch_one<T, C, 8, VEC, 8>(a, grid, stream);
-  if (dim <= 128) return few ? launch_one<T, C, 16, VEC, kFewRowsTile>(a, grid, stream) : launch_one<T, C, 16, VEC, 4>(a, grid, stream);
-  return launch_one<T, C, 32, VEC, kFewRowsTile>(a, grid, stream);
-}
-
 template <typename T, typename C>
-int launch_typed(const Attend& a, bool vec, unsigned grid, cudaStream_t stream) {
-  return vec ? launch_vec<T, C, 4>(a, grid, stream) : launch_vec<T, C, 1>(a, grid, stream);
+int launch_plain_one(const Attend& a, unsigned grid, cudaStream_t stream) {
+  const cudaError_t err = tc::launch_pdl(plain_kernel<T, C>, grid, kPlainThreads, 0, stream, a);
+  if (err != cudaSuccess) return set_error(KSMM_ERR_CUDA, "attention plain kernel: %s", cudaGetErrorString(err));
+  count_launch();
+  return KSMM_OK;
 }
 
 template <typename T>
-int launch_cached(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
-  // rows of four elements at a time where every one starts on their boundary
-  const int es = cache_dtype == KSMM_F8E4M3 ? 1 : static_cast<int>(sizeof(T));
-  auto whole = [](const void* p, int64_t x, int64_t y, int64_t z, int size) {
-    return (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0) && x % 4 == 0 && y % 4 == 0 && z % 4 == 0;
-  };
-  const Pool& p = a.pool;
-  bool vec = p.dim % 4 == 0 && whole(a.q, a.q_token, a.q_head, 0, sizeof(T));
-  for (int i = 0; i < 2; ++i) vec = vec && whole(p.data[i], p.page[i], p.head[i], p.token[i], es);
-  if (cache_dtype == KSMM_F8E4M3) return launch_typed<T, f8e4m3>(a, vec, grid, stream);
-  return launch_typed<T, T>(a, vec, grid, stream);
+int launch_plain_cached(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  return cache_dtype == KSMM_F8E4M3 ? launch_plain_one<T, f8e4m3>(a, grid, stream) : launch_plain_one<T, T>(a, grid, stream);
 }
 
 }  // namespace
 
-int rows_tile(int dim, int64_t rows) { return rows <= kFewRowsTile || dim > 128 ? kFewRowsTile : dim <= 64 ? 8 : 4; }
+int launch_rows(const Attend& a, unsigned grid, cudaStream_t stream) {
+  const bool few = a.tile_rows == kFewRowsTile;
+  if (a.pool.dim <= 64) return few ? launch_one<8, kFewRowsTile>(a, grid, stream) : launch_one<8, 8>(a, grid, stream);
+  if (a.pool.dim <= 128) return few ? launch_one<16, kFewRowsTile>(a, grid, stream) : launch_one<16, 4>(a, grid, stream);
+  return launch_one<32, kFewRowsTile>(a, grid, stream);
+}
 
-int launch_rows(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
-  if (dtype == KSMM_F32) return launch_cached<float>(a, cache_dtype, grid, stream);
-  if (dtype == KSMM_F16) return launch_cached<__half>(a, cache_dtype, grid, stream);
-  return launch_cached<__nv_bfloat16>(a, cache_dtype, grid, stream);
+int launch_plain(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
+  if (dtype == KSMM_F32) return launch_plain_cached<float>(a, cache_dtype, grid, stream);
+  if (dtype == KSMM_F16) return launch_plain_cached<__half>(a, cache_dtype, grid, stream);
+  return launch_plain_cached<__nv_bfloat16>(a, cache_dtype, grid, stream);
 }
 
 template <typename T>

@@ -42,15 +42,13 @@ struct Layout {
   static constexpr int kRuns = 4, kHalves = DP == 256 ? 2 : 1, kConsumers = kRuns * kHalves;
   static constexpr int kThreads = (kConsumers + 1) * 32;
   static constexpr int kCols = DP / kHalves;                            // of a warp's output
-  // Tokens of a warp's step.  A step is a chain (load, products, maximum, exponentials, products) of 1000 to 1500 cycles
-  // however many tokens it has, and an SM's eight warps have to pass 23 bytes a cycle: small rows take 32 tokens at a time.
-  static constexpr int kStep = DP == 256 || (!EIGHT && DP == 128) ? 16 : 32;
+  static constexpr int kStep = token_shape(EIGHT, DP).unit / kRuns;
   static constexpr int kTokens = kRuns * kStep;                         // a unit, a stage of the ring
   static constexpr int kBoxes = EIGHT ? (DP + 127) / 128 : DP / 64;     // 128-byte columns of a row
   static constexpr int kOperand = kBoxes * kTokens * 128;               // a unit's keys
   static constexpr int kScales = EIGHT ? 2 * kTokens * 4 : 0;
   static constexpr int kStageBytes = 2 * kOperand;
-  static constexpr int kBlocks = DP == 256 ? 1 : 2;                     // on an SM
+  static constexpr int kBlocks = token_shape(EIGHT, DP).blocks;         // on an SM
   static constexpr int kStages = 196608 / kBlocks / (kStageBytes + kScales);
   static constexpr int kMerge = kRuns * 4 * kCols * 4;                  // the runs' output for 4 rows, or part of it for more
   static constexpr int kMergeAt = kStages * kStageBytes;
@@ -161,8 +159,6 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
   using H = typename std::conditional<EIGHT, __half, T>::type;  // of the products
   // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
   constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
-  // q stays in shared memory where registers do not hold it beside the output
-  constexpr bool kQShared = DP == 256 && NT == 2;
   constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
   extern __shared__ __align__(1024) char smem[];
   const uint32_t base = smem_u32(smem);
@@ -344,7 +340,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
           const uint2 v = *reinterpret_cast<const uint2*>(at + 8 * q4);
           qf[c][t][0] = v.x;
           qf[c][t][1] = v.y;
-        } else if constexpr (!kQShared) {
+        } else {
           qf[c][t][0] = *reinterpret_cast<const uint32_t*>(at + 4 * q4);
           qf[c][t][1] = *reinterpret_cast<const uint32_t*>(at + 4 * q4 + 16);
         }
@@ -390,38 +386,8 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[c][t][e] = 0.f;
 
-    if constexpr (kQShared && EIGHT) {
-      // in the order of the chunks, and in fp16; one warp for all
-      bar_sync_named(1, L::kConsumers * 32);
-      if (warp == 0) {
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            char* at = smem + L::kQAt + (gq + 8 * t) * L::kQRow + c * 32 + 4 * q4;
-            *reinterpret_cast<uint32_t*>(at) = qf[c][t][0];
-            *reinterpret_cast<uint32_t*>(at + 16) = qf[c][t][1];
-          }
-      }
-      bar_sync_named(1, L::kConsumers * 32);
-    }
-    if constexpr (!kQShared) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(segment_empty);
-    }
-    // (q from shared memory in every step: rows 0-7 | 0-7 | 8-15 | 8-15, chunks c, c + 1, c, c + 1)
-    const uint32_t q_at = base + L::kQAt + (v_row % L::kRows) * L::kQRow + v_chunk * 16;
-    auto q_load = [&](int c) {
-      if constexpr (kQShared) {
-        uint32_t r[4];
-        ldmatrix4(r, q_at + c * 32);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          qf[c][t][0] = r[2 * t];
-          qf[c][t][1] = r[2 * t + 1];
-        }
-      }
-    };
+    __syncwarp();
+    if (lane == 0) mbar_arrive(segment_empty);
     // tokens from `clear` to below `sure` are seen by every row
     const int sure = g.first_position + 1;
     const int64_t clear = a.window ? static_cast<int64_t>(g.hi) - a.window : 0;
@@ -444,7 +410,6 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
         if constexpr (!EIGHT) {
 #pragma unroll
           for (int c = 0; c < DP / 16; ++c) {
-            q_load(c);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
               uint32_t k[4];
@@ -456,8 +421,6 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
         } else {
 #pragma unroll
           for (int c = 0; c < DP / 16; c += 2) {
-            q_load(c);
-            q_load(c + 1);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
               uint32_t b[4];  // tokens 0-7 and 8-15 of chunk c, then of c + 1
@@ -642,10 +605,6 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
       if (lane == 0) mbar_arrive(empty + 8 * st);
       turn.next();
     }
-    if constexpr (kQShared) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(segment_empty);
-    }
 
     // ---- the four runs' results, in pieces of the columns that the buffer holds for all rows: every warp gives, then every
     // thread joins some pairs of neighbours and writes them ----
@@ -756,8 +715,6 @@ int launch_one(const Maps& maps, const Attend& a, int box, int joined, unsigned 
   return KSMM_OK;
 }
 
-int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
 template <typename T, bool EIGHT, int DP, int NT>
 int launch_maps(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
   using L = Layout<EIGHT, DP, NT>;
@@ -779,64 +736,27 @@ int launch_maps(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t st
   return launch_one<T, EIGHT, DP, NT>(maps, a, box, joined, grid, stream);
 }
 
-template <typename T, bool EIGHT, int NT>
+template <typename T, bool EIGHT>
 int launch_dim(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
-  switch (padded(a.pool.dim)) {
-    case 64: return launch_maps<T, EIGHT, 64, NT>(a, cache_dtype, grid, stream);
-    case 128: return launch_maps<T, EIGHT, 128, NT>(a, cache_dtype, grid, stream);
-    default: return launch_maps<T, EIGHT, 256, NT>(a, cache_dtype, grid, stream);
+  const int dp = padded_dim(a.pool.dim);
+  if constexpr (!EIGHT) {
+    if (a.tile_rows == 16) {
+      if (dp == 64) return launch_maps<T, false, 64, 2>(a, cache_dtype, grid, stream);
+      return launch_maps<T, false, 128, 2>(a, cache_dtype, grid, stream);
+    }
   }
+  if (dp == 64) return launch_maps<T, EIGHT, 64, 1>(a, cache_dtype, grid, stream);
+  if (dp == 128) return launch_maps<T, EIGHT, 128, 1>(a, cache_dtype, grid, stream);
+  return launch_maps<T, EIGHT, 256, 1>(a, cache_dtype, grid, stream);
 }
 
 }  // namespace
 
-template <bool EIGHT, int DP>
-static TokenShape shape_of() {
-  using L = Layout<EIGHT, DP, 1>;
-  static_assert(L::kBlocks == Layout<EIGHT, DP, 2>::kBlocks && L::kTokens == Layout<EIGHT, DP, 2>::kTokens, "whatever the rows");
-  return {L::kBlocks, L::kTokens};
-}
-
-TokenShape token_shape(int cache_dtype, int dim) {
-  const bool eight = cache_dtype == KSMM_F8E4M3;
-  switch (padded(dim)) {
-    case 64: return eight ? shape_of<true, 64>() : shape_of<false, 64>();
-    case 128: return eight ? shape_of<true, 128>() : shape_of<false, 128>();
-    default: return eight ? shape_of<true, 256>() : shape_of<false, 256>();
-  }
-}
-
-template <typename T, bool EIGHT>
-static int launch_rows_of(const Attend& a, int cache_dtype, unsigned grid, cudaStream_t stream) {
-  if (a.tile_rows == 8) return launch_dim<T, EIGHT, 1>(a, cache_dtype, grid, stream);
-  return launch_dim<T, EIGHT, 2>(a, cache_dtype, grid, stream);
-}
-
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream) {
   const bool eight = cache_dtype == KSMM_F8E4M3;
   if (dtype == KSMM_F16)
-    return eight ? launch_rows_of<__half, true>(a, cache_dtype, grid, stream) : launch_rows_of<__half, false>(a, cache_dtype, grid, stream);
-  return eight ? launch_rows_of<__nv_bfloat16, true>(a, cache_dtype, grid, stream) : launch_rows_of<__nv_bfloat16, false>(a, cache_dtype, grid, stream);
-}
-
-// Whether TMA can address the pool and the rows of q and out are pairs on their boundary.
-bool token_fits(const ksmm_cache_attention_desc_t& d) {
-  const ksmm_cache_t& c = d.cache;
-  const bool eight = c.cache_dtype == KSMM_F8E4M3;
-  const int per16 = eight ? 16 : 8;
-  if (d.dtype == KSMM_F32 || c.head_dim % per16 || c.page_size % 16 || c.pages == 0) return false;
-  for (int i = 0; i < 2; ++i) {
-    if (reinterpret_cast<uintptr_t>(i ? c.values : c.keys) % 16) return false;
-    const int64_t* s = i ? c.value_strides : c.key_strides;
-    for (int k = 0; k < 3; ++k)
-      if (s[k] <= 0 || s[k] % per16 || s[k] >= (1ll << 38)) return false;
-    if (eight) {
-      const int64_t* f = i ? c.value_scale_strides : c.key_scale_strides;
-      if (reinterpret_cast<uintptr_t>(i ? c.value_scales : c.key_scales) % 16 || f[0] % 4 || f[1] % 4 || f[2] != 1) return false;
-    }
-  }
-  return reinterpret_cast<uintptr_t>(d.q) % 4 == 0 && reinterpret_cast<uintptr_t>(d.out) % 4 == 0 && d.q_strides[0] % 2 == 0 &&
-         d.q_strides[1] % 2 == 0 && d.out_strides[0] % 2 == 0 && d.out_strides[1] % 2 == 0;
+    return eight ? launch_dim<__half, true>(a, cache_dtype, grid, stream) : launch_dim<__half, false>(a, cache_dtype, grid, stream);
+  return eight ? launch_dim<__nv_bfloat16, true>(a, cache_dtype, grid, stream) : launch_dim<__nv_bfloat16, false>(a, cache_dtype, grid, stream);
 }
 
 }  // namespace cache

@@ -110,6 +110,7 @@ def test_residual_and_shapes():
     assert (z.double() - y.double() - x.double()).abs().max() <= 4 * unit(torch.bfloat16) * z.abs().max()
     with pytest.raises(ValueError, match="gradient"):
         attn(x.requires_grad_(), cache, table, lengths)
+    assert attn(x.detach()[:, :0], cache, table, lengths * 0).shape == (2, 0, 384)
     attn.half()
     assert attn.frequencies.dtype == torch.float64
 

@@ -382,6 +382,37 @@ def test_few_and_many_sequences(sequences, length, dtype):
             check(kb.cache_attention(q, cache, table, L, starts=starts, max_new=bound), attended(q, cache, table, lengths, new), cache)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", [96, 130, 200])
+def test_many_heads_of_one_key_head(heads, dtype):
+    gen = torch.Generator().manual_seed(heads)
+    for lengths, new in (([1500, 40], [1, 1]), ([300, 90], [2, 60])):
+        cache, table, L, starts, q, _, _ = make(gen, lengths, new, heads, 1, 64, 16, dtype)
+        check(kb.cache_attention(q, cache, table, L, starts=starts), attended(q, cache, table, lengths, new), cache)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_shared_tables_and_an_empty_pool(dtype):
+    gen = torch.Generator().manual_seed(4)
+    cache, table, L, _, q, _, _ = make(gen, [200], [1], 4, 2, 64, 16, dtype)
+    q = torch.randn(3, 4, 64, generator=gen).to(dtype).to(DEV)
+    L = torch.tensor([200, 150, 7], dtype=torch.int32, device=DEV)
+    out = kb.cache_attention(q, cache, table.expand(3, -1), L)  # one prefix, three sequences
+    check(out, attended(q, cache, table.expand(3, -1), [200, 150, 7], [1] * 3), cache)
+    every = torch.tensor([200, 0, 150, 0, 7, 0], dtype=torch.int32, device=DEV)[::2]  # lengths side by side with something else
+    assert torch.equal(out, kb.cache_attention(q, cache, table.expand(3, -1), every))
+    none = kb.KVCache.of(cache.keys[:0], cache.values[:0])
+    L[2] = 0
+    for x, n in ((q, 1), (torch.cat([q] * 90), 90)):
+        out = kb.cache_attention(x, none, table.expand(3, -1), L)
+        k = torch.zeros(x.shape[0], 2, 64, dtype=dtype, device=DEV)
+        kb.cache_append(none, table.expand(3, -1), L, k, k)
+        assert torch.isnan(out[:2 * n]).all() and (out[2 * n:] == 0).all()
+    with pytest.raises(TypeError):
+        kb.cache_attention(q, cache, table.expand(3, -1), L, window=0.5)
+    kb.check_device()
+
+
 def test_empty_calls():
     cache = kb.KVCache(2, 16, 2, 64)
     empty = torch.zeros(0, 2, 64, dtype=torch.float16, device=DEV)
