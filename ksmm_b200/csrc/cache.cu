@@ -6,9 +6,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cstdarg>
 #include <cstdio>
-#include <string>
 
 #include "cache_lib.h"
 #include "tc_host.h"
