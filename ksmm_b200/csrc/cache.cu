@@ -133,7 +133,7 @@ bool token_fits(const ksmm_cache_attention_desc_t& d) {
 
 bool prompt_fits(const ksmm_cache_attention_desc_t& d) {
   const int group = d.heads / d.cache.kv_heads;
-  if (d.cache.cache_dtype == KSMM_F8E4M3 || !token_fits(d) || group > 128) return false;
+  if (!token_fits(d) || group > 128) return false;
   // (a negative scale would turn the maximum round)
   if (!(d.scale > 0.f) || d.scale > 1e30f) return false;
   return reinterpret_cast<uintptr_t>(d.q) % 16 == 0 && reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.q_strides[0] > 0 &&
@@ -315,7 +315,7 @@ int ksmm_cu_cache_attention(const ksmm_cache_attention_desc_t* d, void* workspac
     a.least = plan.grid ? plan.most + 1 : 1;
     a.most = INT_MAX;
     a.split = 0;
-    st = d->dtype == KSMM_F32 ? k->floats(a, plan.prompt, s) : k->prompt(a, d->dtype, plan.prompt, s);
+    st = d->dtype == KSMM_F32 ? k->floats(a, plan.prompt, s) : k->prompt(a, d->dtype, c.cache_dtype == KSMM_F8E4M3, plan.prompt, s);
     if (st != KSMM_OK || !plan.grid) return st;
     a.clear_rest = 0;
   }

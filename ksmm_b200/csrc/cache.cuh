@@ -23,6 +23,13 @@ struct Pool {
   int sequences, tokens, each;  // each: new tokens of a sequence where there are no starts
 };
 
+// two e4m3 (the low 16 bits) as fp16
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t v) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // A sequence as the kernels see it.
 struct Sequence {
   int start, n;  // its rows
@@ -329,7 +336,7 @@ inline int prompt_rows(int group) { return 128 / group * group; }
 
 int launch_append(Append& a, int dtype, int cache_dtype, cudaStream_t stream);
 int launch_token(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);
-int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream);
+int launch_prompt(const Attend& a, int dtype, bool eight, unsigned grid, cudaStream_t stream);
 int launch_float(const Attend& a, unsigned grid, cudaStream_t stream);
 int launch_rows(const Attend& a, unsigned grid, cudaStream_t stream);
 int launch_plain(const Attend& a, int dtype, int cache_dtype, unsigned grid, cudaStream_t stream);

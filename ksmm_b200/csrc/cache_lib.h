@@ -24,7 +24,7 @@ struct Host {
 struct Kernels {
   int (*append)(Append&, int dtype, int cache_dtype, cudaStream_t);
   int (*token)(const Attend&, int dtype, int cache_dtype, unsigned grid, cudaStream_t);
-  int (*prompt)(const Attend&, int dtype, unsigned grid, cudaStream_t);
+  int (*prompt)(const Attend&, int dtype, bool eight, unsigned grid, cudaStream_t);
   int (*floats)(const Attend&, unsigned grid, cudaStream_t);
   int (*rows)(const Attend&, unsigned grid, cudaStream_t);
   int (*plain)(const Attend&, int dtype, int cache_dtype, unsigned grid, cudaStream_t);

@@ -1,4 +1,4 @@
-// Attention of many new tokens (prompts) over a paged cache in 16 bits, on tcgen05.
+// Attention of many new tokens (prompts) over a paged cache in 16 or 8 bits, on tcgen05.
 //
 // An item is one key head and a tile of up to 128 rows: a row is (token, head of the group), all heads that share the key head
 // side by side, so that keys and values are read once for them.  Per tile of keys: S = Q K^T into tensor memory, a thread per row
@@ -30,28 +30,31 @@ namespace {
 
 using namespace tc;
 
-template <int DP>
+template <int DP, bool EIGHT>
 struct Prompt {
   // Blocks on an SM, as tensor memory has room for their S and O; the more the better: a tile is a chain (products, loads, maximum,
   // exponentials, stores) whose parts leave each unit idle most of the time.
-  static constexpr int kBlocks = DP == 64 ? 4 : DP == 128 ? 2 : 1;
-  static constexpr int kKeys = DP == 128 ? 128 : 64;           // tokens of a tile of keys
+  static constexpr int kBlocks = DP == 64 ? (EIGHT ? 3 : 4) : DP == 128 ? 2 : 1;
+  static constexpr int kKeys = DP == 128 && !EIGHT ? 128 : 64;  // tokens of a tile of keys (8 bits: the converting warps need registers)
   static constexpr int kBoxes = DP / 64;                       // 128-byte columns of a row
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kOperand = kKeys * DP * 2;              // a tile of keys or values
   // (one of each for 128 columns: the next keys are loaded while the rows work, the next values while they work again)
-  static constexpr int kStages = DP == 128 ? 1 : 2;
+  static constexpr int kStages = kKeys == 128 ? 1 : 2;
   static constexpr int kRingAt = kQ;
   static constexpr int kBarsAt = kRingAt + 2 * kStages * kOperand;
-  // q | k full, k empty, v full, v empty | s, p, o | a load of its own
-  static constexpr int kBars = 1 + 4 * kStages + 3 + 1;
+  // q | k full, k empty, v full, v empty | s, p, o | a load of its own | scales
+  static constexpr int kScaleSlots = EIGHT ? 4 : 0;
+  static constexpr int kBars = 1 + 4 * kStages + 3 + 1 + kScaleSlots;
   static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
   static constexpr int kSegmentAt = (kFlagsAt + 8 + 7) / 8 * 8;
-  static constexpr int kBytes = kSegmentAt + static_cast<int>(sizeof(Segment));
-  static constexpr int kThreads = 128 + 64;
+  static constexpr int kScalesAt = (kSegmentAt + static_cast<int>(sizeof(Segment)) + 15) / 16 * 16;  // [slot][keys, values][token]
+  static constexpr int kBytes = kScalesAt + kScaleSlots * 2 * kKeys * 4;
+  static constexpr int kConverters = !EIGHT ? 0 : DP == 64 ? 2 : 4;  // warps, the producer's among them
+  static constexpr int kThreads = 128 + 64 + (EIGHT ? 32 * (kConverters - 1) : 0);
   static constexpr int kOAt = kKeys;                           // columns of tensor memory: S, then O
-  static constexpr int kColumns = 512 / kBlocks;
-  static_assert(kOAt + DP <= kColumns, "tensor memory");
+  static constexpr int kColumns = DP == 64 ? 128 : DP == 128 ? 256 : 512;  // (an allocation is a power of two)
+  static_assert(kOAt + DP <= kColumns && kBlocks * kColumns <= 512, "tensor memory");
   static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
 };
 
@@ -102,10 +105,126 @@ __device__ __forceinline__ void store_weights(uint32_t at, const uint32_t (&w)[N
 
 constexpr int kPromptWaits = kWaits + 4;
 
+// e4m3 pairs as the model's type, exactly: fp16 holds them, times a power of two where `by` is not one
+template <typename T, bool SCALED>
+__device__ __forceinline__ uint32_t widen(uint32_t codes, uint32_t by) {
+  const uint32_t h = e4m3_to_half2(codes);
+  if constexpr (ElemTraits<T>::kDtype == KSMM_F16) {
+    if constexpr (!SCALED) return h;
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&by));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return pack2(f.x, f.y, ElemTraits<T>::kDtype);
+  }
+}
+
+// The converting warps of an 8-bit cache: keys and values of a tile on their way in registers while the tile before is worked on, then
+// widened into the operands' tiles.  A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
+// and V hold the codes as they are.  With fp16, whose weights have no room for any scale, V takes the power of two that lies in
+// [2^-24, 2^7] (below, a value vanishes in fp16 results; above, its code would be infinite) and the weights the rest.
+// A tile's scales are in one of four slots: V's stage, waited for below, is free only when the rows have left the tile two before.
 template <typename T, int DP>
-__global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
+__device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* smem, int first, int count, int thread, uint32_t k_full,
+                                        uint32_t alone, volatile int* abort_flag, int* status) {
+  using C = Prompt<DP, true>;
+  constexpr int kPer = DP / 16;  // 16 codes a piece
+  constexpr int kStep = 32 * C::kConverters / kPer, kPieces = C::kKeys / kStep;
+  constexpr bool kHalf = ElemTraits<T>::kDtype == KSMM_F16;
+  const int piece = thread % kPer, row = thread / kPer, lane = thread % 32;
+  const bool inside = piece * 16 < p.dim;
+  int page[kPieces], slot[kPieces];
+  uint4 codes[2][kPieces];
+  float scale[2][kPieces];
+  auto find = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int token = (first + j) * C::kKeys + row + i * kStep;
+      page[i] = -1;
+      if (j >= count || token < g.lo || token >= g.hi) continue;
+      const int column = token / p.page_size;
+      slot[i] = token - column * p.page_size;
+      const int at = p.table[g.s * p.table_stride + column];
+      if (at >= 0 && at < p.pages) page[i] = at;
+    }
+  };
+  auto get = [&](int of) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      codes[of][i] = make_uint4(0, 0, 0, 0);
+      scale[of][i] = 0.f;
+      if (page[i] < 0) continue;
+      if (inside)
+        codes[of][i] = *reinterpret_cast<const uint4*>(p.data[of] + page[i] * p.page[of] + g.head * p.head[of] + slot[i] * p.token[of] + piece * 16);
+      scale[of][i] = p.scales[of][page[i] * p.spage[of] + g.head * p.shead[of] + slot[i] * p.stoken[of]];
+    }
+  };
+  auto power = [](float f) { return min(max((__float_as_int(f) >> 23 & 255) - 127, -24), 7); };
+  auto put = [&](uint32_t at, int of) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      uint32_t by = 0;
+      if (kHalf && of) {
+        const int e = power(scale[1][i]);
+        by = (e >= -14 ? e + 15 << 10 : 1 << (e + 24)) * 0x10001u;
+      }
+      const uint32_t in[4] = {codes[of][i].x, codes[of][i].y, codes[of][i].z, codes[of][i].w};
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (of) {
+          w[2 * e] = widen<T, true>(in[e], by);
+          w[2 * e + 1] = widen<T, true>(in[e] >> 16, by);
+        } else {
+          w[2 * e] = widen<T, false>(in[e], by);
+          w[2 * e + 1] = widen<T, false>(in[e] >> 16, by);
+        }
+      }
+      const int r = row + i * kStep;
+      char* to = smem + at + piece / 4 * (C::kKeys * 128) + r * 128;
+      const int unit = piece % 4 * 2, turn = piece / 4 & 1;  // (the second box's odd half first: other banks than the first box's)
+      const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
+      *reinterpret_cast<uint4*>(to + ((unit + turn ^ r & 7) << 4)) = turn ? hi : lo;
+      *reinterpret_cast<uint4*>(to + ((unit + 1 - turn ^ r & 7) << 4)) = turn ? lo : hi;
+    }
+    fence_proxy_async();
+    __syncwarp();
+  };
+  find(0);
+  get(0);
+  get(1);
+  for (int j = 0; j < count; ++j) {
+    const int st = j % C::kStages;
+    const uint32_t parity = (j / C::kStages & 1) ^ 1;
+    const uint32_t full = k_full + 8 * st, empty = full + 8 * C::kStages;
+    const int kt = C::kRingAt + st * C::kOperand, vt = kt + C::kStages * C::kOperand;
+    find(j + 1);
+    if (piece == 0) {
+      float* to = reinterpret_cast<float*>(smem + C::kScalesAt) + j % 4 * (2 * C::kKeys);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        to[row + i * kStep] = scale[0][i];
+        to[C::kKeys + row + i * kStep] = kHalf ? scale[1][i] * __int_as_float(127 - power(scale[1][i]) << 23) : scale[1][i];
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(alone + 8 * (1 + j % 4));
+    if (!__all_sync(0xffffffffu, mbar_wait<20>(empty, parity, abort_flag, status, kPromptWaits + 1))) return false;
+    put(kt, 0);
+    if (lane == 0) mbar_arrive(full);
+    get(0);
+    if (!__all_sync(0xffffffffu, mbar_wait<20>(empty + 16 * C::kStages, parity, abort_flag, status, kPromptWaits + 1))) return false;
+    put(vt, 1);
+    if (lane == 0) mbar_arrive(full + 16 * C::kStages);
+    get(1);
+  }
+  return true;
+}
+
+template <typename T, int DP, bool EIGHT>
+__global__ void __launch_bounds__(Prompt<DP, EIGHT>::kThreads, Prompt<DP, EIGHT>::kBlocks)
     prompt_kernel(const __grid_constant__ PromptMaps maps, const __grid_constant__ PromptArgs args) {
-  using C = Prompt<DP>;
+  using C = Prompt<DP, EIGHT>;
   extern __shared__ __align__(1024) char smem[];
   const Attend& a = args.a;
   const Pool& p = a.pool;
@@ -120,21 +239,27 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
   auto v_full = [&](int i) { return q_full + 8 * (1 + 2 * C::kStages + i); };
   auto v_empty = [&](int i) { return q_full + 8 * (1 + 3 * C::kStages + i); };
   const uint32_t s_full = q_full + 8 * (1 + 4 * C::kStages), p_full = s_full + 8, o_full = p_full + 8;
-  const uint32_t alone = q_full + 8 * (C::kBars - 1);
+  const uint32_t alone = o_full + 8;
+  auto scales_full = [&](int i) { return alone + 8 * (1 + i); };
   if (base % 1024) {  // (without static shared memory it starts there; swizzled tiles need it)
     if (tid == 0) atomicCAS(a.status, 0, kPromptWaits);
     return;
   }
   if (tid == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < C::kBars; ++i) mbar_init(q_full + 8 * i, 1);
-    mbar_init(p_full, 4);
+    for (int i = 0; i < C::kBars; ++i) {
+      const uint32_t bar = q_full + 8 * i;
+      const bool converted = EIGHT && ((bar >= k_full(0) && bar < k_empty(0)) || (bar >= v_full(0) && bar < v_empty(0)) || bar > alone);
+      mbar_init(bar, converted ? C::kConverters : bar == p_full ? 4 : 1);
+    }
     fence_mbar_init();
   }
   if (warp == kProducer && lane == 0) {
     prefetch_tensormap(&maps.q);
-    prefetch_tensormap(&maps.keys);
-    prefetch_tensormap(&maps.values);
+    if constexpr (!EIGHT) {
+      prefetch_tensormap(&maps.keys);
+      prefetch_tensormap(&maps.values);
+    }
   }
   touch_parameters(args);
   grid_dep_wait();
@@ -190,9 +315,12 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
     for (int j = 0; j < count; ++j) {
       const uint32_t missing = __ballot_sync(0xffffffffu, missing_next);
       if (j + 1 < count) missing_next = missing_box(j + 1);
-      alive = __all_sync(0xffffffffu, mbar_wait<0>(s_full, j & 1, abort_flag, a.status, kPromptWaits + 4));
+      if constexpr (EIGHT)
+        alive = __all_sync(0xffffffffu, mbar_wait<0>(scales_full(j % 4), j / 4 & 1, abort_flag, a.status, kPromptWaits + 4));
+      alive = alive && __all_sync(0xffffffffu, mbar_wait<0>(s_full, j & 1, abort_flag, a.status, kPromptWaits + 4));
       if (!alive) break;
       tc_fence_after();
+      const float* scales = reinterpret_cast<const float*>(smem + C::kScalesAt) + j % 4 * (2 * C::kKeys);
       // In halves of the columns: the second is kept while the maximum is found and turned into weights first, the first is read
       // again (registers for a whole row at once do not go round with two blocks).
       constexpr int kHalf = C::kKeys / 2;
@@ -203,6 +331,14 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
 #pragma unroll
         for (int c = 0; c < kHalf; c += 32) tmem_ld32(s_at + half * kHalf + c, reinterpret_cast<uint32_t*>(s) + c);
         tmem_ld_wait();
+        if constexpr (EIGHT) {
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(scales + half * kHalf + c);
+            unpack_f2(mul_f2(pack_f2(s[c], s[c + 1]), pack_f2(k.x, k.y)), s[c], s[c + 1]);
+            unpack_f2(mul_f2(pack_f2(s[c + 2], s[c + 3]), pack_f2(k.z, k.w)), s[c + 2], s[c + 3]);
+          }
+        }
         if (!edge) return;
         if (missing) {
 #pragma unroll
@@ -250,7 +386,7 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
       const uint64_t scale2 = pack_f2(a.scale, a.scale), shift2 = pack_f2(shift, shift);
       uint64_t sums[2] = {0, 0};  // pairs
       uint32_t w[kHalf / 2];
-      auto weights = [&]() {
+      auto weights = [&](int half) {
 #pragma unroll
         for (int e = 0; e < kHalf / 2; ++e) {
           float x, y;
@@ -258,16 +394,20 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
           x = exp2_fast(x);
           y = exp2_fast(y);
           sums[e % 2] = add_f2(sums[e % 2], pack_f2(x, y));
+          if constexpr (EIGHT) {
+            const float2 v = *reinterpret_cast<const float2*>(scales + C::kKeys + half * kHalf + 2 * e);
+            unpack_f2(mul_f2(pack_f2(x, y), pack_f2(v.x, v.y)), x, y);
+          }
           w[e] = pack2(x, y, ElemTraits<T>::kDtype);
         }
       };
       // (P's second half lies over S's first, which is read again before it is written)
       uint32_t second[kHalf / 2];
-      weights();
+      weights(1);
 #pragma unroll
       for (int e = 0; e < kHalf / 2; ++e) second[e] = w[e];
       load(0);
-      weights();
+      weights(0);
       store_weights<kHalf / 2>(s_at, w);
       store_weights<kHalf / 2>(s_at + kHalf / 2, second);
       {
@@ -311,7 +451,22 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
     }
     tc_fence_before();
   } else {
-    if (warp == kProducer) {
+    if (EIGHT && warp != kIssuer) {
+      // ---------------- 8-bit keys and values into the tiles' 16 bits ----------------
+      if (count > 0 && warp == kProducer && lane == 0) {
+        mbar_expect_tx(q_full, static_cast<uint32_t>(args.tile_tokens * a.group) * DP * 2);
+#pragma unroll
+        for (int b = 0; b < C::kBoxes; ++b) tma_load_3d(base + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group, g.start + token0);
+      }
+      if constexpr (EIGHT) {
+        const bool alive = convert<T, DP>(p, g, smem, first, count, (warp == kProducer ? 0 : warp - kIssuer) * 32 + lane, k_full(0), alone,
+                                          abort_flag, a.status);
+        if (!alive && count > 0 && warp == kProducer) {
+          int zero = 0;
+          mbar_wait<100>(q_full, 0, &zero, a.status, kPromptWaits + 2);  // (its copy ends before the block does)
+        }
+      }
+    } else if (warp == kProducer) {
       // ---------------- TMA: a lane for each box of a tile, tables 32 boxes ahead ----------------
       const int boxes = C::kKeys / args.box;
       const uint32_t bytes = static_cast<uint32_t>(args.box) * DP * 2;
@@ -467,10 +622,10 @@ __global__ void __launch_bounds__(Prompt<DP>::kThreads, Prompt<DP>::kBlocks)
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool EIGHT>
 int launch_one(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cudaStream_t stream) {
-  using C = Prompt<DP>;
-  auto kern = prompt_kernel<T, DP>;
+  using C = Prompt<DP, EIGHT>;
+  auto kern = prompt_kernel<T, DP, EIGHT>;
   static std::atomic<uint64_t> ready{0};  // a bit per device
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -485,21 +640,21 @@ int launch_one(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cu
   return KSMM_OK;
 }
 
-template <typename T>
+template <typename T, bool EIGHT>
 int launch_dim(const PromptMaps& maps, const PromptArgs& args, unsigned grid, cudaStream_t stream) {
-  if (args.a.pool.dim <= 64) return launch_one<T, 64>(maps, args, grid, stream);
-  if (args.a.pool.dim <= 128) return launch_one<T, 128>(maps, args, grid, stream);
-  return launch_one<T, 256>(maps, args, grid, stream);
+  if (args.a.pool.dim <= 64) return launch_one<T, 64, EIGHT>(maps, args, grid, stream);
+  if (args.a.pool.dim <= 128) return launch_one<T, 128, EIGHT>(maps, args, grid, stream);
+  return launch_one<T, 256, EIGHT>(maps, args, grid, stream);
 }
 
 }  // namespace
 
-int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream) {
+int launch_prompt(const Attend& a, int dtype, bool eight, unsigned grid, cudaStream_t stream) {
   const Pool& p = a.pool;
   PromptArgs args = {};
   args.a = a;
   args.tile_tokens = 128 / a.group;
-  const int keys = p.dim <= 64 ? Prompt<64>::kKeys : p.dim <= 128 ? Prompt<128>::kKeys : Prompt<256>::kKeys;
+  const int keys = p.dim > 64 && p.dim <= 128 && !eight ? Prompt<128, false>::kKeys : 64;
   args.box = keys;
   while (p.page_size % args.box) args.box /= 2;
   const uint32_t fmt = dtype == KSMM_F16 ? 0u : 1u;
@@ -507,8 +662,8 @@ int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream
   const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
   args.idesc_s = common | static_cast<uint32_t>(keys >> 3) << 17;
   args.idesc_o = common | 1u << 16 | dp >> 3 << 17;
-  PromptMaps maps;
-  for (int i = 0; i < 2; ++i) {
+  PromptMaps maps = {};
+  for (int i = 0; i < 2 && !eight; ++i) {
     const uint64_t dims[4] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(p.page_size), static_cast<uint64_t>(p.kv_heads),
                               static_cast<uint64_t>(p.pages)};
     const uint64_t strides[4] = {1, static_cast<uint64_t>(p.token[i]), static_cast<uint64_t>(p.head[i]), static_cast<uint64_t>(p.page[i])};
@@ -521,7 +676,8 @@ int launch_prompt(const Attend& a, int dtype, unsigned grid, cudaStream_t stream
   const uint32_t size[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(args.tile_tokens)};
   const int st = encode_map(&maps.q, dtype, 3, a.q, dims, strides, size);
   if (st != KSMM_OK) return st;
-  return dtype == KSMM_F16 ? launch_dim<__half>(maps, args, grid, stream) : launch_dim<__nv_bfloat16>(maps, args, grid, stream);
+  if (eight) return dtype == KSMM_F16 ? launch_dim<__half, true>(maps, args, grid, stream) : launch_dim<__nv_bfloat16, true>(maps, args, grid, stream);
+  return dtype == KSMM_F16 ? launch_dim<__half, false>(maps, args, grid, stream) : launch_dim<__nv_bfloat16, false>(maps, args, grid, stream);
 }
 
 }  // namespace cache

@@ -106,12 +106,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// two e4m3 (the low 16 bits) as fp16
-__device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t v) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
-  return r;
-}
 template <typename H>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return pack2(lo, hi, ElemTraits<H>::kDtype);
