@@ -40,7 +40,7 @@ struct Prompt {
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kOperand = kKeys * DP * 2;              // a tile of keys or values
   // (one of each for 128 columns: the next keys are loaded while the rows work, the next values while they work again)
-  static constexpr int kStages = kKeys == 128 ? 1 : 2;
+  static constexpr int kStages = DP == 128 || EIGHT ? 1 : 2;
   static constexpr int kRingAt = kQ;
   static constexpr int kBarsAt = kRingAt + 2 * kStages * kOperand;
   // q | k full, k empty, v full, v empty | s, p, o | a load of its own | scales
@@ -49,7 +49,9 @@ struct Prompt {
   static constexpr int kFlagsAt = kBarsAt + 8 * kBars;         // abort, tensor memory's address
   static constexpr int kSegmentAt = (kFlagsAt + 8 + 7) / 8 * 8;
   static constexpr int kScalesAt = (kSegmentAt + static_cast<int>(sizeof(Segment)) + 15) / 16 * 16;  // [slot][keys, values][token]
-  static constexpr int kBytes = kScalesAt + kScaleSlots * 2 * kKeys * 4;
+  static constexpr int kCodesAt = kScalesAt + kScaleSlots * 2 * kKeys * 4;  // two tiles' [keys, values]
+  static constexpr int kCodes = EIGHT ? kKeys * DP : 0;
+  static constexpr int kBytes = kCodesAt + 4 * kCodes;
   static constexpr int kConverters = !EIGHT ? 0 : DP == 64 ? 2 : 4;  // warps, the producer's among them
   static constexpr int kThreads = 128 + 64 + (EIGHT ? 32 * (kConverters - 1) : 0);
   static constexpr int kOAt = kKeys;                           // columns of tensor memory: S, then O
@@ -119,106 +121,134 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes, uint32_t by) {
   }
 }
 
-// The converting warps of an 8-bit cache: keys and values of a tile on their way in registers while the tile before is worked on, then
-// widened into the operands' tiles.  A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
+// The converting warps of an 8-bit cache.  Each thread copies its pieces of two tiles ahead into shared memory and widens them itself
+// into the operands' tiles (in registers instead, every arrival at a barrier waited for the loads: 1566 us against @@ for 8192 tokens
+// of 32/8 heads of 128).  A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
 // and V hold the codes as they are.  With fp16, whose weights have no room for any scale, V takes the power of two that lies in
 // [2^-24, 2^7] (below, a value vanishes in fp16 results; above, its code would be infinite) and the weights the rest.
-// A tile's scales are in one of four slots: V's stage, waited for below, is free only when the rows have left the tile two before.
+// A tile's scales are in one of four slots: V's tile, waited for below, is free only when the rows have left the tile before.
 template <typename T, int DP>
-__device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* smem, int first, int count, int thread, uint32_t k_full,
-                                        uint32_t alone, volatile int* abort_flag, int* status) {
+__device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* smem, int first, int count, int box, int thread,
+                                        uint32_t k_full, uint32_t alone, volatile int* abort_flag, int* status) {
   using C = Prompt<DP, true>;
-  constexpr int kPer = DP / 16;  // 16 codes a piece
+  constexpr int kPer = DP / 16;  // 16 codes a piece; a row's are in one warp
   constexpr int kStep = 32 * C::kConverters / kPer, kPieces = C::kKeys / kStep;
   constexpr bool kHalf = ElemTraits<T>::kDtype == KSMM_F16;
   const int piece = thread % kPer, row = thread / kPer, lane = thread % 32;
   const bool inside = piece * 16 < p.dim;
-  int page[kPieces], slot[kPieces];
-  uint4 codes[2][kPieces];
-  float scale[2][kPieces];
-  auto find = [&](int j) {
+  const int box_log2 = __ffs(box) - 1, boxes = C::kKeys >> box_log2, batch = 32 / boxes;
+  const int32_t* table = p.table + g.s * p.table_stride;
+  const uint32_t base = smem_u32(smem);
+  float* const scales = reinterpret_cast<float*>(smem + C::kScalesAt);
+  // Where a lane's box starts, for the tiles of a batch; before the pool: not there.  (A converting warp's instructions, one after the
+  // other, are the longest part of a tile: nothing is worked out per piece that can be once.)
+  int64_t ahead[2] = {-1, -1}, scales_ahead[2] = {0, 0};
+  const int64_t in_box = row & (box - 1);
+  const uint32_t codes_at = base + C::kCodesAt + row * DP + piece * 16;
+  const uint32_t scale_at = base + C::kScalesAt + (piece * C::kKeys + row) * 4;
+  auto get = [&](int j) {
+    if (j < count) {
+      if (j % batch == 0) {
+        const int token = (first + j) * C::kKeys + (lane << box_log2);
+        const int column = token / p.page_size;
+        const int slot = token - column * p.page_size;
+        const int page = token < g.hi && token + box > g.lo ? table[column] : -1;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int token = (first + j) * C::kKeys + row + i * kStep;
-      page[i] = -1;
-      if (j >= count || token < g.lo || token >= g.hi) continue;
-      const int column = token / p.page_size;
-      slot[i] = token - column * p.page_size;
-      const int at = p.table[g.s * p.table_stride + column];
-      if (at >= 0 && at < p.pages) page[i] = at;
-    }
-  };
-  auto get = [&](int of) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      codes[of][i] = make_uint4(0, 0, 0, 0);
-      scale[of][i] = 0.f;
-      if (page[i] < 0) continue;
-      if (inside)
-        codes[of][i] = *reinterpret_cast<const uint4*>(p.data[of] + page[i] * p.page[of] + g.head * p.head[of] + slot[i] * p.token[of] + piece * 16);
-      scale[of][i] = p.scales[of][page[i] * p.spage[of] + g.head * p.shead[of] + slot[i] * p.stoken[of]];
-    }
-  };
-  auto power = [](float f) { return min(max((__float_as_int(f) >> 23 & 255) - 127, -24), 7); };
-  auto put = [&](uint32_t at, int of) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      uint32_t by = 0;
-      if (kHalf && of) {
-        const int e = power(scale[1][i]);
-        by = (e >= -14 ? e + 15 << 10 : 1 << (e + 24)) * 0x10001u;
-      }
-      const uint32_t in[4] = {codes[of][i].x, codes[of][i].y, codes[of][i].z, codes[of][i].w};
-      uint32_t w[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (of) {
-          w[2 * e] = widen<T, true>(in[e], by);
-          w[2 * e + 1] = widen<T, true>(in[e] >> 16, by);
-        } else {
-          w[2 * e] = widen<T, false>(in[e], by);
-          w[2 * e + 1] = widen<T, false>(in[e] >> 16, by);
+        for (int of = 0; of < 2; ++of) {
+          ahead[of] = page < 0 || page >= p.pages ? -1 : page * p.page[of] + g.head * p.head[of] + slot * p.token[of];
+          scales_ahead[of] = page * p.spage[of] + g.head * p.shead[of] + slot * p.stoken[of];
         }
       }
-      const int r = row + i * kStep;
-      char* to = smem + at + piece / 4 * (C::kKeys * 128) + r * 128;
-      const int unit = piece % 4 * 2, turn = piece / 4 & 1;  // (the second box's odd half first: other banks than the first box's)
+      int64_t at[2], scale = 0;
+      const int token = (first + j) * C::kKeys + row;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        if (i == 0 || boxes > 1) {
+          const int from = j % batch * boxes + ((row + i * kStep) >> box_log2);
+          const int64_t key = __shfl_sync(0xffffffffu, scales_ahead[0], from), value = __shfl_sync(0xffffffffu, scales_ahead[1], from);
+          at[0] = __shfl_sync(0xffffffffu, ahead[0], from);
+          at[1] = __shfl_sync(0xffffffffu, ahead[1], from);
+          scale = piece ? value : key;
+        }
+        const int64_t slot = boxes > 1 ? (row + i * kStep) & (box - 1) : in_box + i * kStep;
+        const bool there = at[0] >= 0 && token + i * kStep >= g.lo && token + i * kStep < g.hi;
+#pragma unroll
+        for (int of = 0; of < 2; ++of)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(codes_at + (j % 2 * 2 + of) * C::kCodes + i * kStep * DP),
+                       "l"(p.data[of] + (there && inside ? at[of] + slot * p.token[of] + piece * 16 : 0)), "r"(there && inside ? 16 : 0)
+                       : "memory");
+        if (piece < 2)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scale_at + (j % 4 * 2 * C::kKeys + i * kStep) * 4),
+                       "l"(p.scales[piece] + (there ? scale + slot * p.stoken[piece] : 0)), "r"(there ? 4 : 0)
+                       : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int unit = piece % 4 * 2, turn = piece / 4 & 1;  // (the second box's odd half first: other banks than the first box's)
+  char* const to = smem + piece / 4 * (C::kKeys * 128) + row * 128;
+  char* const one = to + ((unit + turn ^ row & 7) << 4);  // (kStep is a multiple of 8)
+  char* const other = to + ((unit + 1 - turn ^ row & 7) << 4);
+  static_assert(kStep % 8 == 0, "a thread's pieces are swizzled alike");
+  auto put = [&](int at, int of, int j, const uint32_t (&by)[kPieces]) {
+    uint4 in[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      in[i] = *reinterpret_cast<const uint4*>(smem + (codes_at - base) + (j % 2 * 2 + of) * C::kCodes + i * kStep * DP);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t codes[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t pair = codes[e / 2] >> (e % 2 * 16);
+        w[e] = of ? widen<T, true>(pair, by[i]) : widen<T, false>(pair, 0);
+      }
       const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
-      *reinterpret_cast<uint4*>(to + ((unit + turn ^ r & 7) << 4)) = turn ? hi : lo;
-      *reinterpret_cast<uint4*>(to + ((unit + 1 - turn ^ r & 7) << 4)) = turn ? lo : hi;
+      *reinterpret_cast<uint4*>(one + at + i * kStep * 128) = turn ? hi : lo;
+      *reinterpret_cast<uint4*>(other + at + i * kStep * 128) = turn ? lo : hi;
     }
     fence_proxy_async();
     __syncwarp();
   };
-  find(0);
   get(0);
   get(1);
+  bool alive = true;
   for (int j = 0; j < count; ++j) {
-    const int st = j % C::kStages;
-    const uint32_t parity = (j / C::kStages & 1) ^ 1;
-    const uint32_t full = k_full + 8 * st, empty = full + 8 * C::kStages;
-    const int kt = C::kRingAt + st * C::kOperand, vt = kt + C::kStages * C::kOperand;
-    find(j + 1);
-    if (piece == 0) {
-      float* to = reinterpret_cast<float*>(smem + C::kScalesAt) + j % 4 * (2 * C::kKeys);
+    const int kt = C::kRingAt, vt = kt + C::kOperand;
+    const uint32_t parity = (j & 1) ^ 1;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    uint32_t by[kPieces] = {};
+    if constexpr (kHalf) {
+      float rest[kPieces];
+      float* const v = scales + (j % 4 * 2 + 1) * C::kKeys + row;
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        to[row + i * kStep] = scale[0][i];
-        to[C::kKeys + row + i * kStep] = kHalf ? scale[1][i] * __int_as_float(127 - power(scale[1][i]) << 23) : scale[1][i];
+        const float f = v[i * kStep];
+        const int e = min(max((__float_as_int(f) >> 23 & 255) - 127, -24), 7);
+        by[i] = (e >= -14 ? e + 15 << 10 : 1 << (e + 24)) * 0x10001u;
+        rest[i] = f * __int_as_float(127 - e << 23);
       }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if (piece == 0) v[i * kStep] = rest[i];
+      __syncwarp();
     }
-    __syncwarp();
     if (lane == 0) mbar_arrive(alone + 8 * (1 + j % 4));
-    if (!__all_sync(0xffffffffu, mbar_wait<20>(empty, parity, abort_flag, status, kPromptWaits + 1))) return false;
-    put(kt, 0);
-    if (lane == 0) mbar_arrive(full);
-    get(0);
-    if (!__all_sync(0xffffffffu, mbar_wait<20>(empty + 16 * C::kStages, parity, abort_flag, status, kPromptWaits + 1))) return false;
-    put(vt, 1);
-    if (lane == 0) mbar_arrive(full + 16 * C::kStages);
-    get(1);
+    alive = __all_sync(0xffffffffu, mbar_wait<20>(k_full + 8, parity, abort_flag, status, kPromptWaits + 1));
+    if (!alive) break;
+    put(kt, 0, j, by);
+    if (lane == 0) mbar_arrive(k_full);
+    alive = __all_sync(0xffffffffu, mbar_wait<20>(k_full + 24, parity, abort_flag, status, kPromptWaits + 1));
+    if (!alive) break;
+    put(vt, 1, j, by);
+    if (lane == 0) mbar_arrive(k_full + 16);
+    get(j + 2);
   }
-  return true;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  return alive;
 }
 
 template <typename T, int DP, bool EIGHT>
@@ -459,7 +489,7 @@ __global__ void __launch_bounds__(Prompt<DP, EIGHT>::kThreads, Prompt<DP, EIGHT>
         for (int b = 0; b < C::kBoxes; ++b) tma_load_3d(base + b * 128 * 128, &maps.q, q_full, b * 64, g.head * a.group, g.start + token0);
       }
       if constexpr (EIGHT) {
-        const bool alive = convert<T, DP>(p, g, smem, first, count, (warp == kProducer ? 0 : warp - kIssuer) * 32 + lane, k_full(0), alone,
+        const bool alive = convert<T, DP>(p, g, smem, first, count, args.box, (warp == kProducer ? 0 : warp - kIssuer) * 32 + lane, k_full(0), alone,
                                           abort_flag, a.status);
         if (!alive && count > 0 && warp == kProducer) {
           int zero = 0;
