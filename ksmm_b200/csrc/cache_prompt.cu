@@ -34,8 +34,8 @@ template <int DP, bool EIGHT>
 struct Prompt {
   // Blocks on an SM, as tensor memory has room for their S and O; the more the better: a tile is a chain (products, loads, maximum,
   // exponentials, stores) whose parts leave each unit idle most of the time.
-  static constexpr int kBlocks = DP == 64 ? (EIGHT ? 3 : 4) : DP == 128 ? 2 : 1;
-  static constexpr int kKeys = DP == 128 && !EIGHT ? 128 : 64;  // tokens of a tile of keys (8 bits: the converting warps need registers)
+  static constexpr int kBlocks = DP == 64 ? (EIGHT ? 2 : 4) : DP == 128 ? 2 : 1;
+  static constexpr int kKeys = DP == 128 && !EIGHT ? 128 : 64;  // tokens of a tile of keys (8 bits: the widening warps need registers)
   static constexpr int kBoxes = DP / 64;                       // 128-byte columns of a row
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kOperand = kKeys * DP * 2;              // a tile of keys or values
@@ -52,7 +52,7 @@ struct Prompt {
   static constexpr int kCodesAt = kScalesAt + kScaleSlots * 2 * kKeys * 4;  // two tiles' [keys, values]
   static constexpr int kCodes = EIGHT ? kKeys * DP : 0;
   static constexpr int kBytes = kCodesAt + 4 * kCodes;
-  static constexpr int kConverters = !EIGHT ? 0 : DP == 64 ? 2 : 4;  // warps, the producer's among them
+  static constexpr int kConverters = !EIGHT ? 0 : DP == 256 ? 8 : 4;  // warps that widen, the producer's among them
   static constexpr int kThreads = 128 + 64 + (EIGHT ? 32 * (kConverters - 1) : 0);
   static constexpr int kOAt = kKeys;                           // columns of tensor memory: S, then O
   static constexpr int kColumns = DP == 64 ? 128 : DP == 128 ? 256 : 512;  // (an allocation is a power of two)
@@ -122,8 +122,12 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes, uint32_t by) {
 }
 
 // The converting warps of an 8-bit cache.  Each thread copies its pieces of two tiles ahead into shared memory and widens them itself
-// into the operands' tiles (in registers instead, every arrival at a barrier waited for the loads: 1566 us against @@ for 8192 tokens
-// of 32/8 heads of 128).  A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
+// into the operands' tiles.  What one warp does one after the other is the longest part of a tile (without it 8192 tokens of 32/8 heads
+// of 128 would take 800 us): loads into registers, which every arrival at a barrier waits for, 1566 us; copies 1483; addresses worked
+// out once per box of a page 1196; half of the warps for keys, half for values 1842 (twice the pieces in a row).  More warps leave the
+// rows too few registers with two blocks on an SM; heads of 256, one block, have eight (689 -> 499 us with 8/1 heads), and heads of 64
+// four with two blocks (282 us for 32 prompts of 1000; two warps with three blocks 297).
+// A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
 // and V hold the codes as they are.  With fp16, whose weights have no room for any scale, V takes the power of two that lies in
 // [2^-24, 2^7] (below, a value vanishes in fp16 results; above, its code would be infinite) and the weights the rest.
 // A tile's scales are in one of four slots: V's tile, waited for below, is free only when the rows have left the tile before.
@@ -140,10 +144,8 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
   const int32_t* table = p.table + g.s * p.table_stride;
   const uint32_t base = smem_u32(smem);
   float* const scales = reinterpret_cast<float*>(smem + C::kScalesAt);
-  // Where a lane's box starts, for the tiles of a batch; before the pool: not there.  (A converting warp's instructions, one after the
-  // other, are the longest part of a tile: nothing is worked out per piece that can be once.)
+  // Where a lane's box starts, for the tiles of a batch; before the pool: not there.
   int64_t ahead[2] = {-1, -1}, scales_ahead[2] = {0, 0};
-  const int64_t in_box = row & (box - 1);
   const uint32_t codes_at = base + C::kCodesAt + row * DP + piece * 16;
   const uint32_t scale_at = base + C::kScalesAt + (piece * C::kKeys + row) * 4;
   auto get = [&](int j) {
@@ -170,7 +172,7 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
           at[1] = __shfl_sync(0xffffffffu, ahead[1], from);
           scale = piece ? value : key;
         }
-        const int64_t slot = boxes > 1 ? (row + i * kStep) & (box - 1) : in_box + i * kStep;
+        const int64_t slot = (row + i * kStep) & (box - 1);
         const bool there = at[0] >= 0 && token + i * kStep >= g.lo && token + i * kStep < g.hi;
 #pragma unroll
         for (int of = 0; of < 2; ++of)
