@@ -124,9 +124,9 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes, uint32_t by) {
 // The converting warps of an 8-bit cache.  Each thread copies its pieces of two tiles ahead into shared memory and widens them itself
 // into the operands' tiles.  What one warp does one after the other is the longest part of a tile (without it 8192 tokens of 32/8 heads
 // of 128 would take 800 us): loads into registers, which every arrival at a barrier waits for, 1566 us; copies 1483; addresses worked
-// out once per box of a page 1196; half of the warps for keys, half for values 1842 (twice the pieces in a row).  More warps leave the
+// out once per box of a page 1196, a row's place in it once per thread 1116; half of the warps for keys, half for values 1842 (twice the pieces in a row).  More warps leave the
 // rows too few registers with two blocks on an SM; heads of 256, one block, have eight (689 -> 499 us with 8/1 heads), and heads of 64
-// four with two blocks (282 us for 32 prompts of 1000; two warps with three blocks 297).
+// four with two blocks (282 against 297 us with two warps and three blocks, 32 prompts of 1000).
 // A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
 // and V hold the codes as they are.  With fp16, whose weights have no room for any scale, V takes the power of two that lies in
 // [2^-24, 2^7] (below, a value vanishes in fp16 results; above, its code would be infinite) and the weights the rest.
@@ -146,6 +146,9 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
   float* const scales = reinterpret_cast<float*>(smem + C::kScalesAt);
   // Where a lane's box starts, for the tiles of a batch; before the pool: not there.
   int64_t ahead[2] = {-1, -1}, scales_ahead[2] = {0, 0};
+  // (a row's place in its box is that of its thread's first row plus a part that all threads share)
+  const int64_t in_box = row & (box - 1);
+  const int64_t codes_in_box[2] = {in_box * p.token[0] + piece * 16, in_box * p.token[1] + piece * 16};
   const uint32_t codes_at = base + C::kCodesAt + row * DP + piece * 16;
   const uint32_t scale_at = base + C::kScalesAt + (piece * C::kKeys + row) * 4;
   auto get = [&](int j) {
@@ -158,7 +161,7 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
 #pragma unroll
         for (int of = 0; of < 2; ++of) {
           ahead[of] = page < 0 || page >= p.pages ? -1 : page * p.page[of] + g.head * p.head[of] + slot * p.token[of];
-          scales_ahead[of] = page * p.spage[of] + g.head * p.shead[of] + slot * p.stoken[of];
+          scales_ahead[of] = page * p.spage[of] + g.head * p.shead[of] + slot;  // (a box's scales lie side by side: the host's check)
         }
       }
       int64_t at[2], scale = 0;
@@ -172,16 +175,16 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
           at[1] = __shfl_sync(0xffffffffu, ahead[1], from);
           scale = piece ? value : key;
         }
-        const int64_t slot = (row + i * kStep) & (box - 1);
+        const int64_t slot = (i * kStep) & (box - 1);
         const bool there = at[0] >= 0 && token + i * kStep >= g.lo && token + i * kStep < g.hi;
 #pragma unroll
         for (int of = 0; of < 2; ++of)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(codes_at + (j % 2 * 2 + of) * C::kCodes + i * kStep * DP),
-                       "l"(p.data[of] + (there && inside ? at[of] + slot * p.token[of] + piece * 16 : 0)), "r"(there && inside ? 16 : 0)
+                       "l"(p.data[of] + (there && inside ? at[of] + codes_in_box[of] + slot * p.token[of] : 0)), "r"(there && inside ? 16 : 0)
                        : "memory");
         if (piece < 2)
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scale_at + (j % 4 * 2 * C::kKeys + i * kStep) * 4),
-                       "l"(p.scales[piece] + (there ? scale + slot * p.stoken[piece] : 0)), "r"(there ? 4 : 0)
+                       "l"(p.scales[piece] + (there ? scale + in_box + slot : 0)), "r"(there ? 4 : 0)
                        : "memory");
       }
     }
@@ -191,7 +194,7 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
   char* const to = smem + piece / 4 * (C::kKeys * 128) + row * 128;
   char* const one = to + ((unit + turn ^ row & 7) << 4);  // (kStep is a multiple of 8)
   char* const other = to + ((unit + 1 - turn ^ row & 7) << 4);
-  static_assert(kStep % 8 == 0, "a thread's pieces are swizzled alike");
+  static_assert(kStep % 8 == 0 && (kStep & (kStep - 1)) == 0, "a thread's pieces are swizzled alike, boxes hold steps or steps boxes");
   auto put = [&](int at, int of, int j, const uint32_t (&by)[kPieces]) {
     uint4 in[kPieces];
 #pragma unroll
