@@ -173,7 +173,7 @@ def cache_append(cache, table, lengths, k, v, q=None, *, starts=None, frequencie
 
     ``frequencies`` (float64, up to head_dim / 2; ``rotary_frequencies``) rotates pair i of every head of k and q by
     ``position * frequencies[i]``: elements (i, i + pairs), or (2 i, 2 i + 1) with ``interleaved``; the rest of the head is
-    taken as it is.  Returns the rotated q (in ``q_out`` if given), or None without q.  Rows of no sequence are
+    taken as it is.  Returns the rotated q (in ``q_out`` if given, which may be q), or None without q.  Rows of no sequence are
     zero in a q that the call makes, and left alone in ``q_out``.  A token whose page is not in the pool is not stored."""
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
@@ -218,7 +218,8 @@ def cache_attention(q, cache, table, lengths, *, starts=None, scale=None, window
     serves head h.  ``table``, ``lengths`` and ``starts`` as in ``cache_append``, whose call comes first.  ``scale`` defaults to
     ``head_dim ** -0.5``.  ``max_new``: an upper bound of one sequence's new tokens, where the caller knows one (it picks the
     kernels; more tokens are still computed, slowly).  Rows of no sequence are zero in a result that the call makes,
-    and left alone in ``out``.  Rows that need a page which is not in the pool are NaN.  Nothing learns through this call."""
+    and left alone in ``out``, which may be q.  Rows that need a page which is not in the pool are NaN.  Nothing learns
+    through this call."""
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
     window, max_new = (None if n is None else operator.index(n) for n in (window, max_new))

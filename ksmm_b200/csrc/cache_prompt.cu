@@ -121,12 +121,12 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes, uint32_t by) {
   }
 }
 
-// The converting warps of an 8-bit cache.  Each thread copies its pieces of two tiles ahead into shared memory and widens them itself
-// into the operands' tiles.  What one warp does one after the other is the longest part of a tile (without it 8192 tokens of 32/8 heads
-// of 128 would take 800 us): loads into registers, which every arrival at a barrier waits for, 1566 us; copies 1483; addresses worked
-// out once per box of a page 1196, a row's place in it once per thread 1116; half of the warps for keys, half for values 1842 (twice the pieces in a row).  More warps leave the
-// rows too few registers with two blocks on an SM; heads of 256, one block, have eight (689 -> 499 us with 8/1 heads), and heads of 64
-// four with two blocks (282 against 297 us with two warps and three blocks, 32 prompts of 1000).
+// The widening warps of an 8-bit cache.  Each thread copies its pieces of two tiles ahead into shared memory and widens them itself
+// into the operands' tiles.  What one warp does one after the other is the longest part of a tile (without it 8192 tokens of 32/8
+// heads of 128 would take 800 us): loads into registers, which every arrival at a barrier waits for, 1566 us; copies 1483; addresses
+// worked out once per box of a page 1196, a row's place in it once per thread 1116; half of the warps for keys, half for values 1842
+// (twice the pieces in a row).  More warps leave the rows too few registers with two blocks on an SM; heads of 256, one block, have
+// eight (689 -> 499 us with 8/1 heads), and heads of 64 four (282 against 297 us with two warps and three blocks, 32 prompts of 1000).
 // A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
 // and V hold the codes as they are.  With fp16, whose weights have no room for any scale, V takes the power of two that lies in
 // [2^-24, 2^7] (below, a value vanishes in fp16 results; above, its code would be infinite) and the weights the rest.
