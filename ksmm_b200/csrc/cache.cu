@@ -157,6 +157,11 @@ bool float_fits(const ksmm_cache_attention_desc_t& d) {
 // through the keys; with more the prompt kernel's tiles of 128 rows are at least half full.  (A sequence that it decoded would
 // not be split: 96 heads that share one key head are 96 rows for a single token.)
 constexpr int kFewRows = 64;
+// In fp32 both kernels are bound by their products, and a tile of the prompt kernel takes as long for one row as for 64: it gains where its
+// items, which are not split, keep the SMs busy.  Rows from which it does: 20 with an item for every SM (64 sequences of 1000
+// tokens, 32/8 heads of 128: 16 rows 502 us here and 584 there, 32 rows 990 and 585), more with fewer (8 sequences, 64 items: 32 rows
+// 138 and 147, 64 rows 258 and 147; one sequence, 64 rows: 44 and 145).
+inline int64_t few_float_rows(int64_t pairs) { return std::max<int64_t>(20, 2400 / pairs); }
 
 struct Plan {
   unsigned prompt;        // blocks of the prompt kernel; 0: none
@@ -182,8 +187,8 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   const int64_t sure = c.starts ? c.tokens : c.tokens / c.sequences;
   int64_t rows = (d.max_new > 0 && d.max_new < sure ? d.max_new : sure) * group;
   p->most = INT_MAX;
-  const int64_t few = std::max<int64_t>(kFewRows, 2 * group);
   const bool floats = float_fits(d);
+  const int64_t few = std::max<int64_t>(floats ? few_float_rows(c.sequences * c.kv_heads) : kFewRows, 2 * group);
   if (rows > few && (floats || prompt_fits(d))) {
     p->prompt_tile = floats ? kFloatRows : prompt_rows(static_cast<int>(group));
     const int64_t n = items(c, group, p->prompt_tile);
