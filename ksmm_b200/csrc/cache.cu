@@ -153,15 +153,19 @@ bool float_fits(const ksmm_cache_attention_desc_t& d) {
   return whole(c.keys, c.key_strides, 3) && whole(c.values, c.value_strides, 3) && whole(d.q, d.q_strides, 2) && whole(d.out, d.out_strides, 2);
 }
 
-// Sequences of up to kFewRows rows (new tokens x heads of a group), or two new tokens, are the token kernel's, in tiles that each go
-// through the keys; with more the prompt kernel's tiles of 128 rows are at least half full.  (A sequence that it decoded would
-// not be split: 96 heads that share one key head are 96 rows for a single token.)
-constexpr int kFewRows = 64;
-// In fp32 both kernels are bound by their products, and a tile of the prompt kernel takes as long for one row as for 64: it gains where its
-// items, which are not split, keep the SMs busy.  Rows from which it does: 20 with an item for every SM (64 sequences of 1000
-// tokens, 32/8 heads of 128: 16 rows 502 us here and 584 there, 32 rows 990 and 585), more with fewer (8 sequences, 64 items: 32 rows
-// 138 and 147, 64 rows 258 and 147; one sequence, 64 rows: 44 and 145).
-inline int64_t few_float_rows(int64_t pairs) { return std::max<int64_t>(20, 2400 / pairs); }
+// Sequences of up to this many rows (new tokens x heads of a group), or of two new tokens, are the kernels' for few rows, which share a
+// batch's keys evenly over the GPU but go through them once for every 4 to 16 rows.  The prompt kernels take 64 or 128 rows as fast as
+// one, but an item of theirs (a tile of rows of one sequence and key head) is not split.  They gain with rows x sequences x key
+// heads above about 2500: with enough items for every SM from 20 rows on, with fewer items later (64 sequences, 32/8 heads of 128, few
+// rows / prompt: bf16, 4000 tokens, 16 rows 194 / 190 us, 32 rows 348 / 191, 64 rows 643 / 191; fp32, 1000 tokens, 16 rows 502 / 584, 32 rows
+// 990 / 585; 8 sequences of 4000, 32 rows, bf16 63 / 70, 8 bits 74 / 118, 64 rows 99 / 70 and 134 / 119; one sequence, 64 rows, bf16 30 / 64).
+// Lengths are on the device: where tables are long, one sequence of many may be too, and its items alone would be waited for (1 us per
+// 64 tokens, in fp32 9); such batches stay shared evenly up to 64 rows.
+int64_t few_rows(bool floats, int64_t pairs, int64_t longest) {
+  const int64_t even = std::max<int64_t>(20, 2500 / pairs);
+  const int64_t rows = longest <= (floats ? 1024 : 4096) ? even : std::max<int64_t>(even, 64);
+  return floats ? rows : std::min<int64_t>(rows, 64);  // (more for 16 bits: not measured to gain)
+}
 
 struct Plan {
   unsigned prompt;        // blocks of the prompt kernel; 0: none
@@ -188,7 +192,8 @@ bool plan_of(const ksmm_cache_attention_desc_t& d, Plan* p) {
   int64_t rows = (d.max_new > 0 && d.max_new < sure ? d.max_new : sure) * group;
   p->most = INT_MAX;
   const bool floats = float_fits(d);
-  const int64_t few = std::max<int64_t>(floats ? few_float_rows(c.sequences * c.kv_heads) : kFewRows, 2 * group);
+  const int64_t few = std::max<int64_t>(
+      few_rows(floats, c.sequences * c.kv_heads, static_cast<int64_t>(c.table_width) * c.page_size), 2 * group);
   if (rows > few && (floats || prompt_fits(d))) {
     p->prompt_tile = floats ? kFloatRows : prompt_rows(static_cast<int>(group));
     const int64_t n = items(c, group, p->prompt_tile);
