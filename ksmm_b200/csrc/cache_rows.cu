@@ -107,12 +107,14 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
     }
     const int32_t* table = p.table + g.s * p.table_stride;
     int page_next[2], row_next[2];  // of the next unit to be fetched: looked up a unit ahead
+    bool want_next[2];              // whether the token is the sequence's (an entry outside the pool says nothing of it)
     auto look = [&](int unit) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int token = unit * kRowsUnit + h * 32 + at, nth = token / p.page_size;
         row_next[h] = token - nth * p.page_size;
-        page_next[h] = unit < g.to && token >= g.lo && token < g.hi ? table[nth] : -2;
+        want_next[h] = unit < g.to && token >= g.lo && token < g.hi;
+        page_next[h] = want_next[h] ? table[nth] : -1;
       }
     };
     // a thread's own bytes of the ring: nobody else reads them
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const bool get = page_next[h] >= 0 && page_next[h] < p.pages;
-        if (!get && page_next[h] != -2) gone |= 1u << h;
+        if (!get && want_next[h]) gone |= 1u << h;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const C* row = data[kv] + static_cast<int64_t>(get ? page_next[h] : 0) * p.page[kv] + g.head * p.head[kv] + row_next[h] * p.token[kv];

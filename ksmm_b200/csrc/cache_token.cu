@@ -212,11 +212,12 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
       more = more && g.s >= 0;
       const int32_t* table = p.table + g.s * p.table_stride;
       int row_ahead = 0, page_ahead = -1, batch = 0;
+      bool wanted = false;  // (whether a box is the sequence's; an entry outside the pool says nothing of it, whatever its value)
       auto look = [&](int u) {
         // the pages of the next 32 boxes
         const int token = u * L::kTokens + (lane << box_log2), nth = token / p.page_size;
-        const bool there = token < g.hi && token + box > g.lo;
-        page_ahead = there ? table[nth] : -2;  // -2: nothing to load, -1 or beyond the pool: a page that is not there
+        wanted = token < g.hi && token + box > g.lo;
+        page_ahead = wanted ? table[nth] : -1;
         row_ahead = token - nth * p.page_size;
       };
       if (more) look(g.from);
@@ -245,10 +246,10 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
       for (int u = g.from; u < g.to; ++u) {
         if (batch == 0) {
           if (u > g.from) look(u);
-          if (page_ahead >= p.pages || page_ahead < -2) page_ahead = -1;
+          if (page_ahead >= p.pages) page_ahead = -1;
         }
         const bool of_unit = lane >= batch && lane < batch + boxes;
-        const uint32_t missing = __ballot_sync(0xffffffffu, of_unit && page_ahead == -1) >> batch;
+        const uint32_t missing = __ballot_sync(0xffffffffu, of_unit && wanted && page_ahead < 0) >> batch;
         const uint32_t load = __ballot_sync(0xffffffffu, of_unit && page_ahead >= 0) >> batch;
         const int st = turn.stage;
         alive = __all_sync(0xffffffffu, mbar_wait<0>(empty + 8 * st, turn.parity ^ 1, abort_flag, a.status, kWaits));
