@@ -23,7 +23,7 @@
 //
 // 8-bit caches: the products run in fp16, which holds e4m3 exactly.  q is scaled by a power of two per row so that bf16's
 // range fits; a token's key scale multiplies its scores; its value scale multiplies its weight, relative to a running
-// power of two `vm` that is at least every scale so far.  One 16-byte chunk of a key row is a k step: its elements are
+// power of two `vm` that is at least the size of every scale so far.  One 16-byte chunk of a key row is a k step: its elements are
 // taken in the order 4 q, 4 q + 1 | 4 q + 2, 4 q + 3 that the load gives, by q as well.
 #include <atomic>
 #include <climits>
@@ -508,10 +508,10 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
               }
           }
         if constexpr (EIGHT) {
-          // the weights times the values' scales, relative to a power of two that is at least each of them
+          // the weights times the values' scales, relative to a power of two that is at least each of their sizes
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < G; ++i) top = fmaxf(top, fmaxf(value_scale[i][0], value_scale[i][1]));
+          for (int i = 0; i < G; ++i) top = fmaxf(top, fmaxf(fabsf(value_scale[i][0]), fabsf(value_scale[i][1])));
 #pragma unroll
           for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
           if (top > vm) {

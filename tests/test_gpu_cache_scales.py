@@ -1,0 +1,64 @@
+"""8-bit caches whose scales have any sign and size, single and few tokens and prompts, against the formula in 64 bits.
+
+Tolerance, relative to the sum of |weight * value| of a row (A), which is what the signs cannot cancel: scores and sums as in
+test_gpu_cache (2e-5); one rounding of the weights to fp16 (bf16 models, few tokens: 2^-11, half a step) or to
+the model's type (prompts: u), or two parts (fp16 models, few tokens: 2^-22).  Then the result's own rounding, and in fp16 its
+smallest step.
+"""
+import pytest
+import torch
+
+import ksmm_b200 as kb
+from test_gpu_cache import DEV, attended, make, unit
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float8_e4m3fn
+
+
+def sizes(cache):
+    """The cache with the absolute values of its values."""
+    return kb.KVCache.of(cache.keys, (cache.values.view(torch.uint8) & 127).view(F8), cache.key_scales, cache.value_scales.abs())
+
+
+def close(out, ref, total, rounding):
+    t = out.dtype
+    most = unit(t) * ref.abs() + (2e-5 + rounding) * total + (2.0 ** -24 if t == torch.float16 else 0)
+    off = (out.double() - ref).abs()
+    assert (off <= most).all(), (off / most).max().item()
+
+
+def rounding(dtype, few):
+    return (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22) if few else unit(dtype)
+
+
+SIGNS = [(-1, -1, -1), (-1, 1, 1), (-1, 0, 1), (0, 0, 0), (0, 0, -1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(6, 6, 64), (8, 2, 128), (4, 1, 256), (32, 2, 112)])
+@pytest.mark.parametrize("new", [1, 2])
+def test_signs(new, heads, kv, dim, dtype):
+    gen = torch.Generator().manual_seed(dim + new)
+    for lengths in ([40, 333, 1, 129], [3000, 64, 700, 5]):  # whole items, and items in parts
+        lengths = [max(n, new) for n in lengths]
+        cache, table, L, _, q, _, _ = make(gen, lengths, [new] * 4, heads, kv, dim, 16, dtype, eight=True)
+        scales = cache.value_scales.clone()
+        for signs in SIGNS:
+            pick = torch.randint(0, 3, scales.shape, generator=gen)
+            cache.value_scales.copy_(scales * torch.tensor(signs, dtype=torch.float32)[pick].to(DEV))
+            ref, total = (attended(q, c, table, lengths, [new] * 4) for c in (cache, sizes(cache)))
+            close(kb.cache_attention(q, cache, table, L), ref, total, rounding(dtype, True))
+    kb.check_device()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_few_tokens_and_prompts_agree_with_the_formula(dtype):
+    """The same cache with negative scales, as the last 1, 2, 20 and 300 tokens see it."""
+    gen = torch.Generator().manual_seed(3)
+    n, heads, kv, dim = 333, 8, 2, 64
+    cache, table, L, _, q, _, _ = make(gen, [n], [n], heads, kv, dim, 16, dtype, eight=True)
+    cache.value_scales.neg_()
+    cache.key_scales.mul_(torch.randint(0, 2, cache.key_scales.shape, generator=gen).float().to(DEV) * 2 - 1)
+    for last in (1, 2, 20, 300):
+        ref, total = (attended(q[-last:], c, table, [n], [last]) for c in (cache, sizes(cache)))
+        close(kb.cache_attention(q[-last:], cache, table, L), ref, total, max(rounding(dtype, few) for few in (False, True)))
