@@ -500,7 +500,7 @@ KSMM_API int ksmm_cu_norm_backward(const ksmm_norm_desc_t* desc, void* workspace
  * sequence's earlier calls or of other sequences, but may reach this call's rows of its sequence that do not see it.
  * Workspace: ..._workspace_bytes, aligned to 256 bytes, one for each call that may run at the same time.
  * head_dim is at most 256.  q_out and out may be q itself, with its strides; else outputs overlap no input.  Elements times their
- * scales lie in the range of dtype.
+ * scales, and scales themselves, lie in the range of dtype.
  */
 typedef struct {
   void* keys;

@@ -13,9 +13,13 @@
 // of a tile: 3700 cycles for two blocks, of which the products are 2050.
 //
 // K is K-major as it lies in the pages, V is the MN-major operand (its tokens are the contraction), so neither is turned.  O stays in
-// tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the last time: weights are then at most
-// 256, which 16 bits hold as well as 1, and the sum is exact to fp32 either way.  Weights are rounded once to 16 bits; the sum is
-// that of the unrounded ones (their errors are independent: together as large as the result's own rounding).
+// tensor memory; it is rescaled only when a row's maximum has grown by more than 2^kLag since the last time, and the sum is exact to
+// fp32 either way.  Weights are rounded once to 16 bits; the sum is that of the unrounded ones (their errors are independent:
+// together as large as the result's own rounding).  fp16 numbers are subnormal below 2^-14 and end at 2^-24, where the sum would still
+// count what the product lost: a key that takes nearly all of a row's weight, and has small values, leaves the result to thousands of
+// weights down there.  So fp16 weights are raised by 2^kRaise, to 2^15 with the lag, and lose digits from 25 octaves below a row's
+// largest on, not from 14 (the sum has the same factor).  A lag of 2 octaves and two more of range took 156 us for 32 prompts of
+// 1000 tokens, 12 heads of 64, where 4 take 151 and 8 150.
 #include <atomic>
 #include <climits>
 
@@ -57,6 +61,11 @@ struct Prompt {
   static constexpr int kOAt = kKeys;                           // columns of tensor memory: S, then O
   static constexpr int kColumns = DP == 64 ? 128 : DP == 128 ? 256 : 512;  // (an allocation is a power of two)
   static_assert(kOAt + DP <= kColumns && kBlocks * kColumns <= 512, "tensor memory");
+  // log2 of how much a maximum may grow before O is rescaled, and of what fp16 weights are raised by (8 bits: up to twice as
+  // much, with a part of a value's scale)
+  template <typename T> static constexpr bool kHalfs = ElemTraits<T>::kDtype == KSMM_F16;
+  template <typename T> static constexpr float kLag = kHalfs<T> ? 4.f : 8.f;
+  template <typename T> static constexpr float kRaise = !kHalfs<T> ? 0.f : EIGHT ? 10.f : 11.f;
   static_assert(kBlocks * (kBytes + 1024) <= 228 * 1024, "the blocks of an SM fit its shared memory");
 };
 
@@ -129,7 +138,8 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes, uint32_t by) {
 // eight (689 -> 499 us with 8/1 heads), and heads of 64 four (282 against 297 us with two warps and three blocks, 32 prompts of 1000).
 // A key's scale multiplies its scores and a value's scale its weights, in fp32 and for the rows to do: K
 // and V hold the codes as they are.  With fp16, whose weights have no room for any scale, V takes the power of two that lies in
-// [2^-24, 2^7] (below, a value vanishes in fp16 results; above, its code would be infinite) and the weights the rest.
+// [2^-24, 2^15] (below, a value vanishes in fp16 results) and the weights the rest, below 2 for scales that fp16 holds: a code times
+// its scale's power of two is no more than the element itself, which does not pass 65504.
 // A tile's scales are in one of four slots: V's tile, waited for below, is free only when the rows have left the tile before.
 template <typename T, int DP>
 __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* smem, int first, int count, int box, int thread,
@@ -231,7 +241,7 @@ __device__ __forceinline__ bool convert(const Pool& p, const Segment& g, char* s
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const float f = v[i * kStep];
-        const int e = min(max((__float_as_int(f) >> 23 & 255) - 127, -24), 7);
+        const int e = min(max((__float_as_int(f) >> 23 & 255) - 127, -24), 15);
         by[i] = (e >= -14 ? e + 15 << 10 : 1 << (e + 24)) * 0x10001u;
         rest[i] = f * __int_as_float(127 - e << 23);
       }
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(Prompt<DP, EIGHT>::kThreads, Prompt<DP, EIGHT>
       load(1);
       highest();
       const float now = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
-      const bool grown = (now - top) * a.scale > 8.f;
+      const bool grown = (now - top) * a.scale > C::template kLag<T>;
       if (j == 0) {
         top = now;
       } else if (__any_sync(0xffffffffu, grown)) {
@@ -417,7 +427,7 @@ __global__ void __launch_bounds__(Prompt<DP, EIGHT>::kThreads, Prompt<DP, EIGHT>
           tmem_st32(o_at + c, o);
         }
       }
-      const float shift = top == kNone ? 0.f : -top * a.scale;
+      const float shift = (top == kNone ? 0.f : -top * a.scale) + C::template kRaise<T>;
       const uint64_t scale2 = pack_f2(a.scale, a.scale), shift2 = pack_f2(shift, shift);
       uint64_t sums[2] = {0, 0};  // pairs
       uint32_t w[kHalf / 2];

@@ -62,3 +62,16 @@ def test_few_tokens_and_prompts_agree_with_the_formula(dtype):
     for last in (1, 2, 20, 300):
         ref, total = (attended(q[-last:], c, table, [n], [last]) for c in (cache, sizes(cache)))
         close(kb.cache_attention(q[-last:], cache, table, L), ref, total, max(rounding(dtype, few) for few in (False, True)))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scales_up_to_what_fp16_holds(sign):
+    """Small codes with large scales: prompts, single tokens and the formula agree as far as elements lie in the type's range."""
+    gen = torch.Generator().manual_seed(7)
+    n, heads, kv, dim = 333, 8, 2, 64
+    cache, table, L, _, q, _, _ = make(gen, [n], [n], heads, kv, dim, 16, torch.float16, eight=True)
+    cache.values.copy_((0.25 * torch.randn(cache.values.shape, generator=gen)).clamp(-0.9, 0.9).to(F8).to(DEV))
+    cache.value_scales.copy_(sign * torch.exp2(torch.rand(cache.value_scales.shape, generator=gen) * 15.99))
+    for last in (1, 2, 300):
+        ref, total = (attended(q[-last:], c, table, [n], [last]) for c in (cache, sizes(cache)))
+        close(kb.cache_attention(q[-last:], cache, table, L), ref, total, rounding(torch.float16, last < 20))
