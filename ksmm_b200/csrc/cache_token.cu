@@ -19,7 +19,8 @@
 // 8 columns: S^T = K q^T with K as the A operand as it lies in shared memory, o^T = V^T w^T with V through transposing loads and w^T
 // transposed in registers; with the rows of q as A half of a tile's 16 rows stood idle.  Of 16-bit caches the weights enter the
 // second product as two 16-bit parts (w = hi + lo, each rounded): one part would add an error as large as the result's final
-// rounding.
+// rounding.  fp16 parts are subnormal below 2^-14 and end at 2^-24, so weights of fp16 products are raised by 2^15 (a row's reference is
+// its maximum less 15; the sum has the same factor): they lose digits from 2^-29 of the row's largest on.
 //
 // 8-bit caches: the products run in fp16, which holds e4m3 exactly.  q is scaled by a power of two per row so that bf16's
 // range fits; a token's key scale multiplies its scores; its value scale multiplies its weight, relative to a running
@@ -160,6 +161,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
   // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
   constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
   constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
+  constexpr float kRaise = !EIGHT && ElemTraits<H>::kDtype == KSMM_F16 ? 15.f : 0.f;
   extern __shared__ __align__(1024) char smem[];
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
             for (int i = 1; i < G; ++i) top = fmaxf(top, fmaxf(s[i][t][e], s[i][t][2 + e]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), m[t][e]);
+            top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kRaise, m[t][e]);
             scale_o[t][e] = exp2_fast(m[t][e] - top);
             m[t][e] = top;
             sum[t][e] *= scale_o[t][e];
