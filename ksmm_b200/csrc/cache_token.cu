@@ -19,13 +19,16 @@
 // 8 columns: S^T = K q^T with K as the A operand as it lies in shared memory, o^T = V^T w^T with V through transposing loads and w^T
 // transposed in registers; with the rows of q as A half of a tile's 16 rows stood idle.  Of 16-bit caches the weights enter the
 // second product as two 16-bit parts (w = hi + lo, each rounded): one part would add an error as large as the result's final
-// rounding.  fp16 parts are subnormal below 2^-14 and end at 2^-24, so weights of fp16 products are raised by 2^15 (a row's reference is
-// its maximum less 15; the sum has the same factor): they lose digits from 2^-29 of the row's largest on.
+// rounding.  fp16 parts are subnormal below 2^-14 and end at 2^-24, so weights of fp16 products are raised by 2^15 (a row's reference m
+// is its maximum less 15; the sum has the same factor): they lose digits from 2^-29 of the row's largest on.
 //
 // 8-bit caches: the products run in fp16, which holds e4m3 exactly.  q is scaled by a power of two per row so that bf16's
-// range fits; a token's key scale multiplies its scores; its value scale multiplies its weight, relative to a running
-// power of two `vm` that is at least the size of every scale so far.  One 16-byte chunk of a key row is a k step: its elements are
-// taken in the order 4 q, 4 q + 1 | 4 q + 2, 4 q + 3 that the load gives, by q as well.
+// range fits; a token's key scale multiplies its scores; its value scale f, of any sign, multiplies its weight.  What has to fit
+// fp16 is that product, so a row's reference is the maximum of score + log2 |f|, less 15: a token of a large scale and hardly any weight
+// does not take the others' digits, nor one of a large weight and values near zero.  Weights alone then reach 2^95, which fp32
+// holds 2^31 of (log2 |f| counts as -80 at least).  A bf16 model's products go in as one fp16 number, off by 2^-11 at most, an eighth
+// of the result's own rounding.  One 16-byte chunk of a key row is a k step: its elements are taken in the order 4 q, 4 q + 1 | 4 q +
+// 2, 4 q + 3 that the load gives, by q as well.
 #include <atomic>
 #include <climits>
 #include <type_traits>
@@ -126,6 +129,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float log2_fast(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // a barrier of the consumers that tells all whether one says so
 template <int THREADS>
@@ -161,7 +169,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
   // whether the weights go in as two parts: e4m3 values times fp16 weights are far within a bf16 result's rounding
   constexpr bool kParts = !(EIGHT && ElemTraits<T>::kDtype == KSMM_BF16);
   constexpr int G = L::kStep / 16;  // groups of 16 tokens of a step
-  constexpr float kRaise = !EIGHT && ElemTraits<H>::kDtype == KSMM_F16 ? 15.f : 0.f;
+  constexpr float kRaise = ElemTraits<H>::kDtype == KSMM_F16 ? 15.f : 0.f;
   extern __shared__ __align__(1024) char smem[];
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -330,7 +338,7 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
     const int rows = min(L::kRows, g.n * a.group - g.tile * L::kRows);
     // A lane's columns of a product are the rows 2 q4 and 2 q4 + 1 of each eight, its rows the tokens gq and gq + 8.
     uint32_t qf[DP / 16][NT][2];
-    float m[NT][2], sum[NT][2], row_scale[NT][2], vm = 0.f;
+    float m[NT][2], sum[NT][2], row_scale[NT][2];
     int position[NT][2];
     float o[L::kCols / 16][NT][4];
 #pragma unroll
@@ -486,15 +494,26 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
           }
         }
         // ---- running maximum and sum ----
+        float value_size[G][2];  // log2 of the values' scales
+        if constexpr (EIGHT) {
+#pragma unroll
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) value_size[i][h] = fmaxf(log2_fast(fabsf(value_scale[i][h])), -80.f);
+        }
+        auto sized = [&](int i, int t, int e) {
+          if constexpr (EIGHT) return s[i][t][e] + value_size[i][e / 2];
+          else return s[i][t][e];
+        };
         float scale_o[NT][2];
         bool grown = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(s[0][t][e], s[0][t][2 + e]);
+            float top = fmaxf(sized(0, t, e), sized(0, t, 2 + e));
 #pragma unroll
-            for (int i = 1; i < G; ++i) top = fmaxf(top, fmaxf(s[i][t][e], s[i][t][2 + e]));
+            for (int i = 1; i < G; ++i) top = fmaxf(top, fmaxf(sized(i, t, e), sized(i, t, 2 + e)));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kRaise, m[t][e]);
@@ -510,29 +529,12 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
               }
           }
         if constexpr (EIGHT) {
-          // the weights times the values' scales, relative to a power of two that is at least each of their sizes
-          float top = 0.f;
-#pragma unroll
-          for (int i = 0; i < G; ++i) top = fmaxf(top, fmaxf(fabsf(value_scale[i][0]), fabsf(value_scale[i][1])));
-#pragma unroll
-          for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          if (top > vm) {
-            const uint32_t e = min((__float_as_uint(top) >> 23) + 1, 254u);
-            const float next = __uint_as_float(e << 23), f = vm / next;
-            vm = next;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              scale_o[t][0] *= f;
-              scale_o[t][1] *= f;
-            }
-          }
-          const float back = vm > 0.f ? 1.f / vm : 0.f;
 #pragma unroll
           for (int i = 0; i < G; ++i)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[i][t][e] *= value_scale[i][e / 2] * back;
+              for (int e = 0; e < 4; ++e) s[i][t][e] *= value_scale[i][e / 2];
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) grown = grown || scale_o[t][0] != 1.f || scale_o[t][1] != 1.f;
@@ -623,14 +625,6 @@ __global__ void __launch_bounds__(Layout<EIGHT, DP, NT>::kThreads, Layout<EIGHT,
           stats[(run * 2 + 1) * L::kRows + r] = !alive || g.bad ? __int_as_float(0x7fffffff) : sum[t][e];
         }
       }
-    if (EIGHT) {
-#pragma unroll
-      for (int c = 0; c < L::kCols / 16; ++c)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][t][e] *= vm;
-    }
     if (g.slot) {
       slot_used[g.slot - 1] = true;
       if (tid == 0) a.slots[2 * blockIdx.x + g.slot - 1] = g.item;

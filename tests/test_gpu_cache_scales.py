@@ -3,7 +3,8 @@
 Tolerance, relative to the sum of |weight * value| of a row (A), which is what the signs cannot cancel: scores and sums as in
 test_gpu_cache (2e-5); one rounding of the weights to fp16 (bf16 models, few tokens: 2^-11, half a step) or to
 the model's type (prompts: u), or two parts (fp16 models, few tokens: 2^-22).  Then the result's own rounding, and in fp16 its
-smallest step.
+smallest step.  A weight times its scale that lies below 2^-29 of the row's largest is a subnormal fp16 number, off by 2^-40 of that largest and
+no more: 2000 of them are 2^-29 of A, which the 2e-5 has room for.
 """
 import pytest
 import torch
@@ -49,6 +50,44 @@ def test_signs(new, heads, kv, dim, dtype):
             ref, total = (attended(q, c, table, lengths, [new] * 4) for c in (cache, sizes(cache)))
             close(kb.cache_attention(q, cache, table, L), ref, total, rounding(dtype, True))
     kb.check_device()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(6, 6, 64), (8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_sizes(new, heads, kv, dim, dtype):
+    """Scales over 24 powers of two in one sequence."""
+    gen = torch.Generator().manual_seed(dim + new)
+    lengths = [50, 333, 2600]
+    cache, table, L, _, q, _, _ = make(gen, lengths, [new] * 3, heads, kv, dim, 16, dtype, eight=True)
+    size = torch.exp2(torch.randint(-24, 1, cache.value_scales.shape, generator=gen).float())
+    sign = torch.randint(0, 2, size.shape, generator=gen).float() * 2 - 1
+    cache.value_scales.mul_((size * sign).to(DEV))
+    ref, total = (attended(q, c, table, lengths, [new] * 3) for c in (cache, sizes(cache)))
+    close(kb.cache_attention(q, cache, table, L), ref, total, rounding(dtype, True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ratio", [2.0 ** 16, 2.0 ** 20])
+@pytest.mark.parametrize("first", [False, True])
+def test_a_large_scale_of_little_weight(first, ratio, dtype):
+    """One token whose values are up to 2^20 times the others' and whose weight is about as small: what the others give is not
+    lost.  bf16: 2^20, 40 nats down (its part is 2^-38); fp16: the others' values small, their sum well above the type's smallest."""
+    gen = torch.Generator().manual_seed(int(ratio) % 97 + first)
+    n, heads, kv, dim = 600, 8, 2, 64
+    cache, table, L, _, q, _, _ = make(gen, [n], [1], heads, kv, dim, 16, dtype, eight=True)
+    far = 3 if first else n - 2
+    page, slot = table[0, far // 16].long(), far % 16
+    q[..., 0] = 8.0
+    cache.keys.view(torch.uint8)[page, :, slot] = 0
+    cache.keys.view(torch.uint8)[page, :, slot, 0] = 0x78  # 256
+    cache.key_scales[page, :, slot] = -40.0 / 256  # score: 8 * -40 / sqrt(64) = -40
+    cache.value_scales[page, :, slot] *= ratio if dtype == torch.bfloat16 else 1
+    if dtype == torch.float16:
+        cache.value_scales.div_(ratio / 2.0 ** 7)
+        cache.value_scales[page, :, slot] *= ratio
+    ref, total = (attended(q, c, table, [n], [1]) for c in (cache, sizes(cache)))
+    close(kb.cache_attention(q, cache, table, L), ref, total, rounding(dtype, True))
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])

@@ -43,8 +43,6 @@ def dominated(gen, length, new, heads, kv, dim, dtype, eight):
 @pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (8, 2, 128), (4, 1, 256)])
 @pytest.mark.parametrize("length,new", [(500, 1), (1000, 2), (8192, 1), (8192, 3), (131072, 1), (700, 200), (8192, 150), (131072, 130)])
 def test_a_key_that_takes_the_weight(length, new, heads, kv, dim, dtype, eight):
-    if eight and new < 100:
-        pytest.skip("16 bits")
     if dim > 64 and new > 100 and length > 8192:
         pytest.skip("the same kernel as 8192 tokens, which 64 columns show at this length")
     gen = torch.Generator().manual_seed(length + new + dim)
