@@ -10,6 +10,7 @@ import operator
 
 import torch
 from torch import nn
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import native as _native
@@ -123,6 +124,11 @@ def _tensors_or_none(*ts):
     return all(t is None or isinstance(t, torch.Tensor) for t in ts)
 
 
+def _changed(*ts):
+    """What a caller gave to be written counts as changed in place: a graph that kept it for its backward pass then raises."""
+    increment_version([t for t in ts if t is not None and not t.is_inference()])
+
+
 def _strides(t, n):
     return (ctypes.c_int64 * n)(*t.stride()[:n])
 
@@ -207,6 +213,7 @@ def cache_append(cache, table, lengths, k, v, q=None, *, starts=None, frequencie
         raise ValueError("q_out without q")
     with torch.cuda.device(cache.device):
         _lib.check(_lib.load().ksmm_cu_cache_append(ctypes.byref(d), _stream_ptr(cache.device)))
+    _changed(cache.keys, cache.values, cache.key_scales, cache.value_scales, q_out)
     return out
 
 
@@ -248,6 +255,7 @@ def cache_attention(q, cache, table, lengths, *, starts=None, scale=None, window
         size = lib.ksmm_cu_cache_attention_workspace_bytes(ctypes.byref(d))
         ws = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
         _lib.check(lib.ksmm_cu_cache_attention(ctypes.byref(d), ws.data_ptr() if size else None, size, _stream_ptr(cache.device)))
+    _changed(out)
     return result
 
 

@@ -887,6 +887,14 @@ bool output_fits(const at::Tensor& out, const at::Tensor& like) {
          (out.size(2) == 1 || out.stride(2) == 1) && !out.requires_grad();
 }
 
+// What a caller gave to be written counts as changed in place: a graph that kept it for its backward pass then raises.
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void changed(const OptTensor& t) {
+  if (t.has_value()) changed(*t);
+}
+
 py::object cache_append(const at::Tensor& keys, const at::Tensor& values, const OptTensor& key_scales, const OptTensor& value_scales,
                         const at::Tensor& table, const at::Tensor& lengths, const at::Tensor& k, const at::Tensor& v, const OptTensor& q,
                         const OptTensor& starts, const OptTensor& frequencies, bool interleaved, const OptTensor& q_out) {
@@ -928,6 +936,11 @@ py::object cache_append(const at::Tensor& keys, const at::Tensor& values, const 
     st = ksmm_cu_cache_append(&d, stream_of(keys));
   }
   if (st != KSMM_OK) return py::cast(st);
+  changed(keys);
+  changed(values);
+  changed(key_scales);
+  changed(value_scales);
+  changed(q_out);
   return q.has_value() ? py::cast(out) : py::cast(false);
 }
 
@@ -960,6 +973,7 @@ py::object cache_attention(const at::Tensor& q, const at::Tensor& keys, const at
     if (need) ws = new_bytes(need, out);
     st = ksmm_cu_cache_attention(&d, need ? ws.data_ptr() : nullptr, need, stream_of(keys));
   }
+  if (st == KSMM_OK) changed(result_in);
   return result(st, out);
 }
 
