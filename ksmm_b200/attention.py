@@ -308,10 +308,16 @@ class KSAttention(nn.Module):
         self.register_buffer("frequencies", frequencies, persistent=False)
 
     def _apply(self, fn, recurse=True):
-        # (a change of the layers' type leaves the frequencies in 64 bits)
+        # (a change of the layers' type leaves the frequencies in 64 bits; memory that is not filled, which to_empty gives, is
+        # filled: no state dict holds them)
+        before = self.frequencies
         super()._apply(fn, recurse)
-        if self.frequencies is not None and self.frequencies.dtype != torch.float64:
-            self.frequencies = rotary_frequencies(self.frequencies.shape[0], self.rotary_base, self.frequencies.device)
+        if before is not None:
+            device = self.frequencies.device
+            if before.is_meta:
+                self.frequencies = rotary_frequencies(before.shape[0], self.rotary_base, device)
+            elif device.type != "meta":
+                self.frequencies = before.to(device)
         return self
 
     def new_cache(self, pages, page_size=64, eight=False):
