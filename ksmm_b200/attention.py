@@ -329,8 +329,9 @@ class KSAttention(nn.Module):
         """x: (..., features), flattened to tokens in the order that ``starts`` counts; with (sequences, n, features) and no
         ``starts`` every sequence has n new tokens.  ``table``, ``lengths`` (with the new tokens), ``starts`` and ``max_new`` as in
         ``cache_attention``; ``residual``: a tensor of the result's shape that is added to it."""
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise ValueError("x requires a gradient: a cache is not trained through")
+        for name, t in (("x", x), ("residual", residual)):
+            if t is not None and t.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"{name} requires a gradient: a cache is not trained through")
         flat = x.reshape(-1, x.shape[-1])
         tokens = flat.shape[0]
         if hasattr(self, "qkv"):
