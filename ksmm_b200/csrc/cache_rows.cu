@@ -1,8 +1,9 @@
-// Attention over a paged cache on the CUDA cores: fp32, and what the tensor-core kernels do not take (pages that are no
-// multiple of 16 tokens, rows that are no multiple of 16 bytes).
+// Attention of few new tokens over a paged cache on the CUDA cores: rows_kernel for fp32 rows of whole 16-byte vectors, plain_kernel for
+// what no other kernel takes (pages that are no multiple of 16 tokens, other alignments and orders, fp32 models on 8-bit caches), and
+// the kernel that joins the parts of items which blocks shared.
 //
-// Eight lanes hold a token's key: with q in registers each lane multiplies its dims, three shuffles join them.  A warp has four
-// such groups and a block eight warps, and every group keeps a running maximum, sum and output row of its own over its
+// rows_kernel: eight lanes hold a token's key: with q in registers each lane multiplies its dims, three shuffles join them.  A warp
+// has four such groups and a block eight warps, and every group keeps a running maximum, sum and output row of its own over its
 // tokens, two at a time; they are joined once, at the end of a segment.
 #include <atomic>
 
@@ -20,37 +21,21 @@ constexpr int kRowThreads = 256;
 constexpr int kSlots = 3;
 constexpr bool row_ring(int dpl) { return dpl <= 16; }
 
-template <int N>
-struct Bytes;
-template <> struct Bytes<16> { using type = uint4; };
-template <> struct Bytes<8> { using type = uint2; };
-template <> struct Bytes<4> { using type = uint32_t; };
-
-// (plain loads: the append before this kernel may still be writing when its blocks start, and nothing is read before the wait)
-template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* p, float* out) {
-  if constexpr (VEC == 1) {
-    out[0] = ElemTraits<T>::to_float(*p);
-  } else {
-    T tmp[VEC];
-    using B = typename Bytes<sizeof(T) * VEC>::type;
-    *reinterpret_cast<B*>(tmp) = *reinterpret_cast<const B*>(p);
+// Dims (j * 8 + l) * 4 .. of a row, for lane l of eight.  (Plain loads: the append before this kernel may still be writing when its
+// blocks start, and nothing is read before the wait.)
+template <int DPL>
+__device__ __forceinline__ void load_row(const float* row, int l, int dim, bool there, float* out) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) out[e] = ElemTraits<T>::to_float(tmp[e]);
-  }
-}
-
-// dims (j * 8 + l) * VEC .. of a row, for lane l of eight
-template <typename T, int DPL, int VEC>
-__device__ __forceinline__ void load_row(const T* row, int l, int dim, bool there, float* out) {
-#pragma unroll
-  for (int j = 0; j < DPL / VEC; ++j) {
-    const int d = (j * 8 + l) * VEC;
+  for (int j = 0; j < DPL / 4; ++j) {
+    const int d = (j * 8 + l) * 4;
     if (there && d < dim) {
-      load<T, VEC>(row + d, out + j * VEC);
+      const float4 v = *reinterpret_cast<const float4*>(row + d);
+      out[4 * j] = v.x;
+      out[4 * j + 1] = v.y;
+      out[4 * j + 2] = v.z;
+      out[4 * j + 3] = v.w;
     } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) out[j * VEC + e] = 0.f;
+      out[4 * j] = out[4 * j + 1] = out[4 * j + 2] = out[4 * j + 3] = 0.f;
     }
   }
 }
@@ -59,9 +44,6 @@ __device__ __forceinline__ void load_row(const T* row, int l, int dim, bool ther
 // enough loads in flight (32 sequences of 12 heads of 64, fp32: 123 us with one block of eight rows, 67 with two of two rows, 74 with three).
 template <int DPL, int R>
 __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kernel(const __grid_constant__ Attend a) {
-  using T = float;
-  using C = float;
-  constexpr int VEC = 4;
   constexpr bool kRing = row_ring(DPL);
   __shared__ Segment segment;
   __shared__ float stats[2][kRowThreads / 32][R];
@@ -71,15 +53,15 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
   touch_parameters(a);
   tc::grid_dep_wait();
   tc::grid_dep_launch();
-  clear_rest<T>(a);
+  clear_rest<float>(a);
   Walker walker;  // the first warp's
   bool some = true;
   if (threadIdx.x < 32) some = walker.start(a);
   if (!__syncthreads_or(threadIdx.x < 32 && some)) return;
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, l = lane % 8, at = warp * 4 + lane / 8;
-  const T* q_rows = reinterpret_cast<const T*>(a.q);
-  const C* data[2] = {reinterpret_cast<const C*>(p.data[0]), reinterpret_cast<const C*>(p.data[1])};
+  const float* q_rows = reinterpret_cast<const float*>(a.q);
+  const float* data[2] = {reinterpret_cast<const float*>(p.data[0]), reinterpret_cast<const float*>(p.data[1])};
 
   bool slot_used[2] = {false, false};
   while (true) {
@@ -99,7 +81,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
       const int row = g.tile * R + r, t = row / a.group;
       position[r] = r < rows ? g.length - g.n + t : -1;
       const int64_t from = (g.start + t) * a.q_token + (g.head * a.group + row - t * a.group) * a.q_head;
-      load_row<T, DPL, VEC>(q_rows + from, l, p.dim, r < rows, q[r]);
+      load_row<DPL>(q_rows + from, l, p.dim, r < rows, q[r]);
       m[r] = kNone;
       sum[r] = 0.f;
 #pragma unroll
@@ -119,10 +101,9 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
     };
     // a thread's own bytes of the ring: nobody else reads them
     auto mine_at = [&](int slot, int h, int kv, int j) {
-      constexpr int kPiece = VEC * static_cast<int>(sizeof(C));
-      return ring + static_cast<uint32_t>(((((slot * 2 + h) * 2 + kv) * (DPL / VEC) + j) * kRowThreads + tid) * kPiece);
+      return ring + static_cast<uint32_t>(((((slot * 2 + h) * 2 + kv) * (DPL / 4) + j) * kRowThreads + tid) * 16);
     };
-    const C* nowhere = reinterpret_cast<const C*>(a.q);  // (a copy of no bytes still names an address)
+    const float* nowhere = reinterpret_cast<const float*>(a.q);  // (a copy of no bytes still names an address)
     uint32_t gone = 0;  // a bit per token fetched, the last ones lowest: its page is not there
     int fetched = g.from, slot_in = 0, slot_out = 0;
     auto fetch = [&]() {
@@ -133,10 +114,10 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
         if (!get && want_next[h]) gone |= 1u << h;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          const C* row = data[kv] + static_cast<int64_t>(get ? page_next[h] : 0) * p.page[kv] + g.head * p.head[kv] + row_next[h] * p.token[kv];
+          const float* row = data[kv] + static_cast<int64_t>(get ? page_next[h] : 0) * p.page[kv] + g.head * p.head[kv] + row_next[h] * p.token[kv];
 #pragma unroll
-          for (int j = 0; j < DPL / VEC; ++j) {
-            const int d = (j * 8 + l) * VEC;
+          for (int j = 0; j < DPL / 4; ++j) {
+            const int d = (j * 8 + l) * 4;
             const bool take = get && d < p.dim;
             // (zeros where there is nothing)
             if constexpr (kRing)
@@ -169,17 +150,25 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
         if constexpr (kRing) {
           bad[h] = gone >> (2 * (kSlots - 1) + h) & 1;
 #pragma unroll
-          for (int c = 0; c < DPL / VEC; ++c) {
-            load<C, VEC>(reinterpret_cast<const C*>(smem + (mine_at(slot_out, h, 0, c) - smem_base)), k[h] + c * VEC);
-            load<C, VEC>(reinterpret_cast<const C*>(smem + (mine_at(slot_out, h, 1, c) - smem_base)), v[h] + c * VEC);
+          for (int c = 0; c < DPL / 4; ++c) {
+            const float4 x = *reinterpret_cast<const float4*>(smem + (mine_at(slot_out, h, 0, c) - smem_base));
+            const float4 y = *reinterpret_cast<const float4*>(smem + (mine_at(slot_out, h, 1, c) - smem_base));
+            k[h][4 * c] = x.x;
+            k[h][4 * c + 1] = x.y;
+            k[h][4 * c + 2] = x.z;
+            k[h][4 * c + 3] = x.w;
+            v[h][4 * c] = y.x;
+            v[h][4 * c + 1] = y.y;
+            v[h][4 * c + 2] = y.z;
+            v[h][4 * c + 3] = y.w;
           }
         } else {
           const int64_t page = page_next[h];
           const int nth = row_next[h];
           bad[h] = there[h] && (page < 0 || page >= p.pages);
           const bool get = there[h] && !bad[h];
-          load_row<C, DPL, VEC>(data[0] + page * p.page[0] + g.head * p.head[0] + nth * p.token[0], l, p.dim, get, k[h]);
-          load_row<C, DPL, VEC>(data[1] + page * p.page[1] + g.head * p.head[1] + nth * p.token[1], l, p.dim, get, v[h]);
+          load_row<DPL>(data[0] + page * p.page[0] + g.head * p.head[0] + nth * p.token[0], l, p.dim, get, k[h]);
+          load_row<DPL>(data[1] + page * p.page[1] + g.head * p.head[1] + nth * p.token[1], l, p.dim, get, v[h]);
         }
       }
       if constexpr (kRing) slot_out = slot_out + 1 == kSlots ? 0 : slot_out + 1;
@@ -243,7 +232,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
       }
       if (lane < 8) {
 #pragma unroll
-        for (int e = 0; e < DPL; ++e) sums[(warp * R + r) * 8 * DPL + (e / VEC * 8 + l) * VEC + e % VEC] = o[r][e];
+        for (int e = 0; e < DPL; ++e) sums[(warp * R + r) * 8 * DPL + (e / 4 * 8 + l) * 4 + e % 4] = o[r][e];
         if (lane == 0) {
           stats[0][warp][r] = m[r];
           stats[1][warp][r] = sum[r];
@@ -276,8 +265,8 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks(8 * DPL, R)) rows_kern
         }
       } else {
         const int row = g.tile * R + r, t = row / a.group;
-        reinterpret_cast<T*>(a.out)[(g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head + d] =
-            ElemTraits<T>::from_float(total == 0.f ? 0.f : out / total);
+        reinterpret_cast<float*>(a.out)[(g.start + t) * a.out_token + (g.head * a.group + row - t * a.group) * a.out_head + d] =
+            total == 0.f ? 0.f : out / total;
       }
     }
     __syncthreads();
