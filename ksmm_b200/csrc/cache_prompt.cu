@@ -8,14 +8,17 @@
 // Four warps of rows, one that issues TMA loads, one that issues MMAs; two blocks on an SM (four for up to 64 columns), each with its
 // part of the tensor memory: while the rows of one work, the tensor cores run another's products, and one's start and end (6 us,
 // as much as five tiles) pass under the others' work.  32 prompts of 1000 tokens, 12 heads of 64: 186 us with one block of two row
-// tiles, 181 with two blocks, 154 with four.  A prompt of 8192 tokens, 32/8 heads of 128: 505 us, 1090 TFLOP/s.
-// What bounds it: the issue of the rows' warps, not the exponentials' unit (a quarter of them as polynomials: 650 us), and the chain
-// of a tile: 3700 cycles for two blocks, of which the products are 2050.
+// tiles, 181 with two blocks, 154 with four (now 151).  A prompt of 8192 tokens, 32/8 heads of 128: 507 to 515 us, 1070 TFLOP/s or more, as
+// a replayed graph; call after call 585 to 595, where the power limit holds the clock down.
+// What bounds it: the chain of a tile (products, scores to registers, maximum, exponentials, weights back, products), 3700 cycles for two
+// blocks, of which the products are 2050.  No unit is full: heads of 64 issue in 42 % of the cycles and keep the tensor pipe busy for
+// 17 %; a quarter of the exponentials as polynomials made it slower (650 us).
 //
 // K is K-major as it lies in the pages, V is the MN-major operand (its tokens are the contraction), so neither is turned.  O stays in
 // tensor memory; it is rescaled only when a row's maximum has grown by more than 2^kLag since the last time, and the sum is exact to
-// fp32 either way.  Weights are rounded once to 16 bits; the sum is that of the unrounded ones (their errors are independent:
-// together as large as the result's own rounding).  fp16 numbers are subnormal below 2^-14 and end at 2^-24, where the sum would still
+// fp32 either way.  Weights are rounded once to 16 bits, a choice: the sum is that of the unrounded ones, the errors are
+// independent and together as large as the result's own rounding (1.3 to 1.4 times the error of fp32 weights, against 64 bits), and a
+// second part would double the second product.  fp16 numbers are subnormal below 2^-14 and end at 2^-24, where the sum would still
 // count what the product lost: a key that takes nearly all of a row's weight, and has small values, leaves the result to thousands of
 // weights down there.  So fp16 weights are raised by 2^kRaise, to 2^15 with the lag, and lose digits from 25 octaves below a row's
 // largest on, not from 14 (the sum has the same factor).  A lag of 2 octaves and two more of range took 156 us for 32 prompts of

@@ -6,8 +6,9 @@
 // the FMA pipes wait for neither loads nor shared memory (the kernel for few rows, a token per eight lanes, met each key with four
 // rows only: 6.6 ms against 4.1 ms for the same formula as library products).  V's rows are on their way while the scores are formed, the
 // next K's while the output is; blocks side by side on an SM fill the rest.  28 to 35 TFLOP/s of the pairs that are seen, of 72 that
-// the FMA pipes have (2000 tokens of 32/8 heads of 128: 1.0 ms).  Three bf16 or tf32 products per term on the tensor cores would
-// lose digits that a caller of fp32 asked for.
+// the FMA pipes have (2000 tokens of 32/8 heads of 128: 1.0 ms).  What bounds it: the FMA pipes are busy for 50 % of the cycles (tiles on
+// the diagonal form twice the pairs that are seen) and 63 % issue, with two warps on a scheduler that wait for shared memory.  The tensor
+// cores are not used: three tf32 products per term keep 21 bits, six of bf16 parts would keep 24 and are not built.
 #include <atomic>
 
 #include "cache.cuh"

@@ -9,7 +9,7 @@
 // join_kernel (cache_rows.cu).
 //
 // Measured (one B200, kernel and join): 64 sequences of 1 to 8192 tokens, 32/8 heads of 128, bf16: 184 us, 5.9 TB/s of the 6.4 that a
-// copy reaches; 131077 tokens of one sequence 93 us (86 the kernel, 7 the join); 128 sequences in 8 bits 218 us, 5.5 TB/s; a window
+// copy reaches; 131077 tokens of one sequence 93 us (86 the kernel, 7 the join); 128 sequences in 8 bits 213 us, 5.6 TB/s; a window
 // of 4096 tokens on heads of 256: 76 us, 4.6 TB/s.  Short sequences are bound by a block's start and a segment's chain: 64 of up to 512
 // tokens take 33 us for 71 MB.
 //
